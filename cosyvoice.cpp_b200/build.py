@@ -35,7 +35,8 @@ def _units():
     units = []
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers.append(os.path.join(INCLUDE, "cvattn.h"))
-    for src in ("kv_append.cu", "decode.cu", "flash_tc.cu", "capi.cpp", "decode_noalloc.cu"):
+    for src in ("kv_append.cu", "decode.cu", "flash_tc.cu", "capi.cpp", "decode_noalloc.cu",
+                "tree_decode.cu", "kv_scores.cu", "kv_evict.cu"):
         obj = os.path.join(BUILD, src.replace(".", "_") + ".o")
         units.append((os.path.join(CSRC, src), obj, []))
     for name, tid in K_TYPES.items():

@@ -2,8 +2,8 @@
 //
 // Argument validation, the per-worker context (device status word), type
 // negotiation, host<->device KV copies, the cvattn_kv_cache host object and
-// the DiT step planner.  Kernels live in kv_append.cu, decode*.cu and
-// flash_tc.cu; nothing here computes attention on the CPU.
+// the DiT step planner.  Kernels live in kv_append.cu, decode*.cu, flash_tc.cu,
+// tree_decode.cu, kv_scores.cu and kv_evict.cu; nothing here computes attention on the CPU.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -133,6 +133,10 @@ size_t cvattn_abi_sizeof(int32_t which) {
     case 3: return sizeof(cvattn_kv_cache_params);
     case 4: return sizeof(cvattn_dit_step);
     case 5: return sizeof(cvattn_rope_params);
+    case 6: return sizeof(cvattn_tree_params);
+    case 7: return sizeof(cvattn_tree_commit_params);
+    case 8: return sizeof(cvattn_kv_scores_params);
+    case 9: return sizeof(cvattn_kv_evict_params);
     default: return 0;
     }
 }
@@ -470,6 +474,168 @@ cvattn_status cvattn_flash(cvattn_context* ctx, void* stream, const cvattn_flash
     DeviceGuard dg(ctx->device);
     if (dg.error() != cudaSuccess) return from_cuda(dg.error());
     return from_cuda(launch_flash(as_stream(stream), *p, ctx->status));
+}
+
+// ------------------------------------------- speculative decoding, bounded cache
+
+// A cache that is addressed through per-sequence row-0 pointers needs no data
+// pointer of its own; everything else about it must still be a tensor.
+static bool cache_ok(const cvattn_tensor& t, const uint64_t* seq_ptrs, int32_t n_seq) {
+    cvattn_tensor c = t;
+    if (t.type == CVATTN_TYPE_F32 && (((seq_ptrs ? 0 : reinterpret_cast<uintptr_t>(t.data)) | (uintptr_t)t.nb1 | (uintptr_t)t.nb2) & 3))
+        return false;
+    if (seq_ptrs) {
+        c.data = const_cast<uint64_t*>(seq_ptrs);
+        c.ne2 = 1;
+        return tensor_ok(&c);
+    }
+    return tensor_ok(&c) && c.ne2 >= n_seq;
+}
+
+static bool same_rows(const cvattn_tensor& a, const cvattn_tensor& b) {
+    return a.type == b.type && a.n_heads == b.n_heads && a.head_dim == b.head_dim;
+}
+
+// Whether [a, a + an) and [b, b + bn) share bytes.
+static bool overlap(const void* a, int64_t an, const void* b, int64_t bn) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)bn && y < x + (uintptr_t)an;
+}
+
+static int64_t tensor_span(const cvattn_tensor& t, int64_t n_seq) {
+    return (n_seq - 1) * t.nb2 + (t.ne1 - 1) * t.nb1 + type_row_bytes(t.type, (int64_t)t.n_heads * t.head_dim);
+}
+
+// A kernel's grid takes sequences and heads in its second and third dimension.
+constexpr int32_t kMaxGridSeq = 65535;
+
+size_t cvattn_tree_decode_workspace_size(int32_t k_type, int32_t v_type, int32_t n_seq, int32_t max_kv_len, int32_t max_nodes,
+                                         int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
+    if (n_seq <= 0 || max_kv_len < 0 || max_nodes <= 0 || max_nodes > CVATTN_TREE_MAX_NODES) return 0;
+    if (!tree_supported(k_type, v_type, head_dim, n_q_heads, n_kv_heads)) return 0;
+    return tree_workspace_bytes(n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
+}
+
+cvattn_status cvattn_tree_decode(cvattn_context* ctx, void* stream, const cvattn_tree_params* p) {
+    if (!ctx || !p || !p->q || !p->out || !p->kv_len || p->flags) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq < 0 || p->max_nodes < 0 || p->max_kv_len < 0 || p->n_q_heads <= 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0 || p->max_nodes == 0) return CVATTN_OK;
+    if (!cache_ok(p->k, p->k_seq_ptrs, p->n_seq) || !cache_ok(p->v, p->v_seq_ptrs, p->n_seq)) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->k.n_heads != p->v.n_heads || p->k.head_dim != p->v.head_dim) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (!tree_supported(p->k.type, p->v.type, p->k.head_dim, p->n_q_heads, p->k.n_heads)) return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_nodes > CVATTN_TREE_MAX_NODES || p->n_seq > kMaxGridSeq) return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_kv_len > p->k.ne1 || p->max_kv_len > p->v.ne1) return CVATTN_ERR_LENGTH;
+    const bool drafts = p->k_draft.data || p->v_draft.data;
+    if (drafts) {
+        if (!cache_ok(p->k_draft, nullptr, p->n_seq) || !cache_ok(p->v_draft, nullptr, p->n_seq) ||
+            !same_rows(p->k, p->k_draft) || !same_rows(p->v, p->v_draft))
+            return CVATTN_ERR_INVALID_ARGUMENT;
+        if (p->k_draft.ne1 < p->max_nodes || p->v_draft.ne1 < p->max_nodes) return CVATTN_ERR_LENGTH;
+    } else if (p->mask) {
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    }
+    const int64_t row = (int64_t)p->n_q_heads * p->k.head_dim;
+    if (p->q_nb_node < row || p->out_nb_node < row || (p->q_nb_node & 3) || (p->out_nb_node & 3) || (p->q_nb_seq & 3) ||
+        (p->out_nb_seq & 3) || (reinterpret_cast<uintptr_t>(p->q) & 15) || (reinterpret_cast<uintptr_t>(p->out) & 15))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    // sequences may share queries (stride 0) but not outputs
+    const int64_t all = (p->max_nodes - 1) * p->out_nb_node + row;
+    if (p->q_nb_seq < 0 || (p->n_seq > 1 && p->out_nb_seq < all && p->out_nb_node < (p->n_seq - 1) * p->out_nb_seq + row))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq > 1 && p->out_nb_seq < row) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->mask && (p->mask_nb_seq < 0 || (p->mask_nb_seq && p->mask_nb_seq < (int64_t)p->max_nodes * ((p->max_nodes + 31) / 32))))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const size_t need = tree_workspace_bytes(p->n_seq, p->max_kv_len, p->max_nodes, p->n_q_heads, p->k.n_heads);
+    if (need && (!p->workspace || p->workspace_size < need || (reinterpret_cast<uintptr_t>(p->workspace) & 15)))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_tree_decode(as_stream(stream), *p, ctx->status));
+}
+
+cvattn_status cvattn_tree_commit(cvattn_context* ctx, void* stream, const cvattn_tree_commit_params* p) {
+    if (!ctx || !p || p->n_tensors < 0 || p->n_seq < 0 || p->max_accepted < 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0) return CVATTN_OK;
+    if (p->n_tensors == 0 || !p->caches || !p->drafts || !p->accepted || !p->n_accepted || !p->kv_len || !p->kv_len_out)
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq > 1 && p->accepted_stride < p->max_accepted) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->n_accepted, 4 * (int64_t)p->n_seq)) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->kv_len_out != p->kv_len && overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->kv_len, 4 * (int64_t)p->n_seq))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    int64_t capacity = INT32_MAX, draft_rows = INT32_MAX;
+    for (int32_t i = 0; i < p->n_tensors; ++i) {
+        const cvattn_tensor &c = p->caches[i], &d = p->drafts[i];
+        if (!tensor_ok(&c) || !tensor_ok(&d) || !same_rows(c, d) || c.ne2 < p->n_seq || d.ne2 < p->n_seq)
+            return CVATTN_ERR_INVALID_ARGUMENT;
+        if (overlap(c.data, tensor_span(c, p->n_seq), d.data, tensor_span(d, p->n_seq))) return CVATTN_ERR_INVALID_ARGUMENT;
+        if (c.ne1 < capacity) capacity = c.ne1;
+        if (d.ne1 < draft_rows) draft_rows = d.ne1;
+    }
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_tree_commit(as_stream(stream), *p, capacity, draft_rows, ctx->status));
+}
+
+cvattn_status cvattn_kv_scores(cvattn_context* ctx, void* stream, const cvattn_kv_scores_params* p) {
+    if (!ctx || !p || !p->q || !p->lse || !p->kv_len || !p->scores || !p->scores_out || p->reserved) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq < 0 || p->max_kv_len < 0 || p->n_q_heads <= 0 || p->max_rows < 0 || p->n_q_rows < 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0 || p->max_kv_len == 0) return CVATTN_OK;
+    if (!cache_ok(p->k, p->k_seq_ptrs, p->n_seq)) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (!tree_supported(p->k.type, p->k.type, p->k.head_dim, p->n_q_heads, p->k.n_heads) || p->n_seq > kMaxGridSeq)
+        return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_kv_len > p->k.ne1) return CVATTN_ERR_LENGTH;
+    if (!p->rows && p->max_rows > p->n_q_rows) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->q_nb_node < (int64_t)p->n_q_heads * p->k.head_dim || (p->q_nb_node & 3) || (p->q_nb_seq & 3) || p->q_nb_seq < 0 ||
+        (reinterpret_cast<uintptr_t>(p->q) & 15))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if ((p->k.n_heads > 1 && p->scores_nb_head < p->max_kv_len) ||
+        (p->n_seq > 1 && p->scores_nb_seq < (p->k.n_heads - 1) * p->scores_nb_head + p->max_kv_len))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_kv_scores(as_stream(stream), *p, ctx->status));
+}
+
+size_t cvattn_kv_evict_workspace_size(int32_t n_layers, int32_t n_seq, int32_t n_kv_heads, int32_t max_kv_len, int32_t budget) {
+    if (n_layers <= 0 || n_seq <= 0 || n_kv_heads <= 0 || max_kv_len < 0 || budget <= 0) return 0;
+    return kv_evict_workspace_bytes(n_layers, n_seq, n_kv_heads, max_kv_len, budget);
+}
+
+cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv_evict_params* p) {
+    if (!ctx || !p || p->n_layers < 0 || p->n_seq < 0 || p->max_kv_len < 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_layers == 0 || p->n_seq == 0) return CVATTN_OK;
+    if (!p->k || !p->v || !p->scores || !p->scores_out || !p->pos_out || !p->kv_len || !p->kv_len_out || (p->kept_len && !p->pos))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->budget <= 0 || p->n_sink < 0 || p->n_recent < 0 || (int64_t)p->n_sink + p->n_recent > p->budget)
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const cvattn_tensor &k = p->k[0], &v = p->v[0];
+    for (int32_t i = 0; i < p->n_layers; ++i) {
+        if (!tensor_ok(&p->k[i]) || !tensor_ok(&p->v[i]) || !same_rows(p->k[i], k) || !same_rows(p->v[i], v) ||
+            p->k[i].nb1 != k.nb1 || p->k[i].nb2 != k.nb2 || p->v[i].nb1 != v.nb1 || p->v[i].nb2 != v.nb2)
+            return CVATTN_ERR_INVALID_ARGUMENT;
+        if (p->k[i].ne2 < p->n_seq || p->v[i].ne2 < p->n_seq) return CVATTN_ERR_INVALID_ARGUMENT;
+        if (p->max_kv_len > p->k[i].ne1 || p->max_kv_len > p->v[i].ne1) return CVATTN_ERR_LENGTH;
+    }
+    // a head's slice of a row must be whole blocks
+    if (k.n_heads != v.n_heads || k.head_dim % 32 || v.head_dim % 32) return CVATTN_ERR_UNSUPPORTED;
+    if (p->n_seq > kMaxGridSeq / k.n_heads) return CVATTN_ERR_UNSUPPORTED;
+    if ((k.n_heads > 1 && p->nb_head < p->max_kv_len) ||
+        (p->n_seq > 1 && p->nb_seq < (k.n_heads - 1) * p->nb_head + p->max_kv_len) ||
+        (p->n_layers > 1 && p->nb_layer < (p->n_seq - 1) * p->nb_seq + (k.n_heads - 1) * p->nb_head + p->max_kv_len))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->kv_len_out != p->kv_len && overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->kv_len, 4 * (int64_t)p->n_seq))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->kept_len && p->kv_len_out != p->kept_len &&
+        overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->kept_len, 4 * (int64_t)p->n_seq))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_tokens && overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->n_tokens, 4 * (int64_t)p->n_seq))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const size_t need = kv_evict_workspace_bytes(p->n_layers, p->n_seq, k.n_heads, p->max_kv_len, p->budget);
+    if (!p->workspace || p->workspace_size < need || (reinterpret_cast<uintptr_t>(p->workspace) & 15)) return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_kv_evict(as_stream(stream), *p, type_row_bytes(k.type, k.head_dim), type_row_bytes(v.type, v.head_dim),
+                                     ctx->status));
 }
 
 // ------------------------------------------------------------ copies

@@ -51,4 +51,19 @@ cudaError_t launch_combine(cudaStream_t stream, const float* partial_o, const fl
 bool flash_supported(int k_type, int v_type, int head_dim, int n_q_heads, int n_kv_heads);
 cudaError_t launch_flash(cudaStream_t stream, const cvattn_flash_params& p, int* status);
 
+// tree_decode.cu
+bool tree_supported(int k_type, int v_type, int head_dim, int n_q_heads, int n_kv_heads);
+size_t tree_workspace_bytes(int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads);
+cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p, int* status);
+
+// kv_scores.cu
+cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params& p, int* status);
+
+// kv_evict.cu (slices: bytes of one head in a K and a V row; capacity, draft_rows: the least over the tensors)
+size_t kv_evict_workspace_bytes(int n_layers, int n_seq, int n_kv_heads, int max_kv_len, int budget);
+cudaError_t launch_kv_evict(cudaStream_t stream, const cvattn_kv_evict_params& p, int64_t k_slice, int64_t v_slice,
+                            int* status);
+cudaError_t launch_tree_commit(cudaStream_t stream, const cvattn_tree_commit_params& p, int64_t capacity,
+                               int64_t draft_rows, int* status);
+
 }  // namespace cvattn

@@ -1,0 +1,153 @@
+// kv_scores.cu -- cvattn_kv_scores: the attention weight of each cached position.
+#include "internal.h"
+#include "common.cuh"
+
+namespace cvattn {
+namespace kvscore {
+
+constexpr int kD = 64;
+constexpr int kTile = 64;   // keys per CTA
+constexpr int kRows = 32;   // (token, head) rows at a time
+constexpr int kPad = kD + 4;
+
+struct Args {
+    const float* q;
+    int64_t q_nb_node, q_nb_seq;
+    const float* lse;
+    const uint8_t* k;
+    int64_t k_nb1, k_nb2;
+    const uint64_t* k_seq_ptrs;
+    const int32_t *rows, *n_rows, *kv_len;
+    const float* scores;
+    float* out;
+    int64_t nb_head, nb_seq;
+    int k_type, n_seq, n_q_rows, max_rows, Hq, Hkv, G, max_kv_len;
+    float scale_log2, decay;
+    int* status;
+};
+
+// s_j = decay s_j + sum over rows of exp2(c q.k_j - lse log2 e): the row sums are
+// known, so a key's column needs no second pass and no exchange between CTAs.
+__global__ void __launch_bounds__(128) scores_f32_kernel(const __grid_constant__ Args a) {
+    __shared__ float4 qs4[kRows][kPad / 4], ks4[kTile][kPad / 4];
+    __shared__ float ls[kRows], red[8][kTile];
+    __shared__ int far[kRows];  // keys that the row sees
+    const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
+    const int s = blockIdx.z, kvh = blockIdx.y, p0 = blockIdx.x * kTile;
+    const int L = a.kv_len[s], n = a.n_rows ? a.n_rows[s] : a.max_rows;
+    const bool odd = a.k_seq_ptrs && (a.k_seq_ptrs[s] & (a.k_type == kF32 ? 3 : 1));
+    if (L < 0 || L > a.max_kv_len || n < 0 || n > a.max_rows || n > L || odd) {
+        if (tid == 0) record_status(a.status, kStatusBadLength);
+        return;
+    }
+    if (p0 >= L) return;
+    const int count = min(kTile, L - p0);
+    const uint8_t* kb = a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[s]) : a.k + (int64_t)s * a.k_nb2;
+    float* ks = reinterpret_cast<float*>(ks4);
+    float* qs = reinterpret_cast<float*>(qs4);
+    const int gb = group_bytes(a.k_type);
+    {
+        const int key = tid >> 1, half = tid & 1;
+        float* d = ks + key * kPad + half * 32;
+        const uint8_t* g = kb + (int64_t)(p0 + key) * a.k_nb1 + (int64_t)(kvh * 2 + half) * gb;
+        for (int e = 0; e < 32; ++e) d[e] = key < count ? dequant_elem_rt(a.k_type, g, e) : 0.0f;
+    }
+    float sum[4] = {};
+    const int total = n * a.G;
+    for (int r0 = 0; r0 < total; r0 += kRows) {
+        __syncthreads();
+        for (int i = tid; i < kRows; i += 128) {
+            const int r = r0 + i, t = r / a.G, h = kvh * a.G + r % a.G;
+            ls[i] = 0.0f;
+            far[i] = 0;
+            if (r < total) {
+                const int at = a.rows ? a.rows[(int64_t)s * a.max_rows + t] : t;
+                if (at < 0 || at >= a.n_q_rows) {
+                    record_status(a.status, kStatusBadPosition);
+                } else {
+                    const float v = a.lse[((int64_t)s * a.n_q_rows + at) * a.Hq + h];
+                    ls[i] = v * 1.4426950408889634f;
+                    far[i] = v == -INFINITY ? 0 : L - n + t + 1;
+                }
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < kRows * kD; i += 128) {
+            const int r = r0 + i / kD, d = i % kD;
+            float v = 0.0f;
+            if (far[i / kD] > 0) {
+                const int t = r / a.G, at = a.rows ? a.rows[(int64_t)s * a.max_rows + t] : t;
+                v = a.q[(int64_t)s * a.q_nb_seq + (int64_t)at * a.q_nb_node + (kvh * a.G + r % a.G) * kD + d];
+            }
+            qs[(i / kD) * kPad + d] = v * a.scale_log2;
+        }
+        __syncthreads();
+        float sc[4][4] = {};
+#pragma unroll 4
+        for (int d = 0; d < kD / 4; ++d) {
+            float4 kk[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kk[j] = ks4[tc + 16 * j][d];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 qq = qs4[tr * 4 + i][d];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    sc[i][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, sc[i][j]))));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p0 + tc + 16 * j < far[tr * 4 + i]) sum[j] += exp2f(sc[i][j] - ls[tr * 4 + i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[tr][tc + 16 * j] = sum[j];
+    __syncthreads();
+    if (tid < count) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += red[i][tid];
+        const int64_t at = (int64_t)s * a.nb_seq + (int64_t)kvh * a.nb_head + p0 + tid;
+        a.out[at] = fmaf(a.decay, a.scores[at], v);
+    }
+}
+
+}  // namespace kvscore
+
+cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params& p, int* status) {
+    using namespace kvscore;
+    Args a{};
+    a.q = p.q;
+    a.q_nb_node = p.q_nb_node;
+    a.q_nb_seq = p.q_nb_seq;
+    a.lse = p.lse;
+    a.k = static_cast<const uint8_t*>(p.k.data);
+    a.k_nb1 = p.k.nb1;
+    a.k_nb2 = p.k.nb2;
+    a.k_seq_ptrs = p.k_seq_ptrs;
+    a.rows = p.rows;
+    a.n_rows = p.n_rows;
+    a.kv_len = p.kv_len;
+    a.scores = p.scores;
+    a.out = p.scores_out;
+    a.nb_head = p.scores_nb_head;
+    a.nb_seq = p.scores_nb_seq;
+    a.k_type = p.k.type;
+    a.n_seq = p.n_seq;
+    a.n_q_rows = p.n_q_rows;
+    a.max_rows = p.max_rows;
+    a.Hq = p.n_q_heads;
+    a.Hkv = p.k.n_heads;
+    a.G = a.Hq / a.Hkv;
+    a.max_kv_len = p.max_kv_len;
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.decay = p.decay;
+    a.status = status;
+    const dim3 grid((unsigned)((a.max_kv_len + kTile - 1) / kTile), (unsigned)a.Hkv, (unsigned)a.n_seq);
+    scores_f32_kernel<<<grid, 128, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace cvattn

@@ -14,7 +14,8 @@ import math
 from typing import Sequence
 
 from . import _lib
-from ._lib import DecodeParams, DitStep, FlashParams, KVCacheParams, RopeParams, Tensor, load
+from ._lib import (TREE_MAX_NODES, DecodeParams, DitStep, FlashParams, KVCacheParams, KVEvictParams, KVScoresParams,
+                   RopeParams, Tensor, TreeCommitParams, TreeParams, load)
 
 # ggml type ids
 F32, F16, Q4_0, Q4_1, Q5_0, Q5_1, Q8_0 = 0, 1, 2, 3, 6, 7, 8
@@ -311,6 +312,245 @@ def flash(ctx: Context, q, k: Tensor, v: Tensor, n_kv: int, out=None, stream=Non
     p = flash_params(q, k, v, n_kv, out, **kw)
     check(lib.cvattn_flash(ctx.handle, _stream(stream), ctypes.byref(p)), "flash")
     return out
+
+
+# ------------------------------------------- speculative decoding, bounded cache
+
+def pack_tree_mask(parents):
+    """Mask bits for tree_decode from parents int [n_seq, max_nodes] (-1: the last committed token; a parent
+    comes before its nodes): node i sees itself and its ancestors.  Returns int32 [n_seq, max_nodes, words] on the CPU."""
+    torch = _torch()
+    par = torch.as_tensor(parents).cpu().long()
+    S, n = par.shape
+    if bool((par >= torch.arange(n)).any()) or bool((par < -1).any()):
+        raise ValueError("pack_tree_mask: a node's parent is -1 or a node before it")
+    sees = torch.zeros((S, n, (n + 31) // 32 * 32), dtype=torch.bool)
+    every = torch.arange(S)
+    for i in range(n):
+        has = par[:, i] >= 0
+        sees[has, i] = sees[every[has], par[has, i]]
+        sees[:, i, i] = True
+    bits = sees.view(S, n, -1, 32).long() << torch.arange(32)
+    words = bits.sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).int()
+
+
+def tree_decode_workspace_size(k_type, v_type, n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads, head_dim=64) -> int:
+    return int(lib.cvattn_tree_decode_workspace_size(k_type, v_type, n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads,
+                                                     head_dim))
+
+
+def _dense(t, dtypes, what, shape=None):
+    """A CUDA tensor of the wanted type whose elements lie one after another."""
+    if t.dtype not in dtypes or not t.is_cuda or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{what}: want a contiguous CUDA tensor of {dtypes}" + ("" if shape is None else f" and shape {tuple(shape)}"))
+    return t
+
+
+def _rows4(t, what):
+    """A CUDA f32 tensor [n_seq, rows, heads, head_dim] whose rows are dense."""
+    torch = _torch()
+    if t.dtype != torch.float32 or not t.is_cuda or t.dim() != 4 or t.stride(3) != 1 or t.stride(2) != t.shape[3]:
+        raise ValueError(f"{what}: want a CUDA f32 tensor [n_seq, rows, heads, head_dim] with dense rows")
+    return t
+
+
+class TreeDecoder:
+    """Reusable launcher of tree attention (pre-built params, one workspace): q f32 [n_seq, max_nodes, Hq, D] over the
+    cache k, v and the drafted rows k_draft, v_draft (None, None: the cache only).  mask: int32 bits
+    [n_seq or 1, max_nodes, words] (pack_tree_mask); None: a chain.  kv_len, n_nodes: int32 [n_seq] on the device."""
+
+    def __init__(self, ctx: Context, k: Tensor, v: Tensor, k_draft: Tensor | None, v_draft: Tensor | None, q, out, kv_len,
+                 max_kv_len: int, lse=None, mask=None, n_nodes=None, k_seq_ptrs=None, v_seq_ptrs=None,
+                 scale: float | None = None, workspace=None):
+        torch = _torch()
+        self.ctx = ctx
+        n_seq, n, Hq, D = _rows4(q, "TreeDecoder q").shape
+        if _rows4(out, "TreeDecoder out").shape != q.shape:
+            raise ValueError("TreeDecoder out: another shape than q")
+        _dense(kv_len, (torch.int32,), "TreeDecoder kv_len", (n_seq,))
+        p = TreeParams()
+        p.q, p.q_nb_seq, p.q_nb_node = q.data_ptr(), q.stride(0), q.stride(1)
+        p.out, p.out_nb_seq, p.out_nb_node = out.data_ptr(), out.stride(0), out.stride(1)
+        if n == 1:  # a stride over one element says nothing
+            p.q_nb_node = p.out_nb_node = Hq * D
+        if lse is not None:
+            p.lse = _dense(lse, (torch.float32,), "TreeDecoder lse", (n_seq, n, Hq)).data_ptr()
+        p.k, p.v = k, v
+        p.k_seq_ptrs, p.v_seq_ptrs = _ptr(k_seq_ptrs), _ptr(v_seq_ptrs)
+        if k_draft is not None:
+            p.k_draft = k_draft
+        if v_draft is not None:
+            p.v_draft = v_draft
+        p.kv_len = kv_len.data_ptr()
+        if n_nodes is not None:
+            p.n_nodes = _dense(n_nodes, (torch.int32,), "TreeDecoder n_nodes", (n_seq,)).data_ptr()
+        if mask is not None:
+            words = (n + 31) // 32
+            _dense(mask, (torch.int32,), "TreeDecoder mask")
+            if tuple(mask.shape) not in ((n_seq, n, words), (1, n, words)):
+                raise ValueError("TreeDecoder mask: want [n_seq or 1, max_nodes, (max_nodes + 31) // 32]")
+            p.mask, p.mask_nb_seq = mask.data_ptr(), 0 if mask.shape[0] == 1 else n * words
+        p.n_seq, p.max_nodes, p.n_q_heads, p.max_kv_len = n_seq, n, Hq, max_kv_len
+        p.scale = 1.0 / math.sqrt(D) if scale is None else scale
+        need = tree_decode_workspace_size(k.type, v.type, n_seq, max_kv_len, n, Hq, k.n_heads, k.head_dim)
+        if workspace is None and need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        self.workspace = workspace
+        if workspace is not None:
+            p.workspace, p.workspace_size = workspace.data_ptr(), workspace.numel()
+        self.params = p
+        self._ref = ctypes.byref(p)
+        self._keep = (q, out, kv_len, lse, mask, n_nodes, k_seq_ptrs, v_seq_ptrs)
+
+    def __call__(self, stream=None) -> None:
+        check(lib.cvattn_tree_decode(self.ctx.handle, _stream(stream), self._ref), "tree_decode")
+
+
+def tree_decode(ctx: Context, q, k: Tensor, v: Tensor, k_draft: Tensor | None, v_draft: Tensor | None, kv_len, max_kv_len: int,
+                out=None, lse=None, stream=None, **kw):
+    """One verification of a tree of drafts; returns out f32 [n_seq, max_nodes, Hq, D]."""
+    torch = _torch()
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    TreeDecoder(ctx, k, v, k_draft, v_draft, q, out, kv_len, max_kv_len, lse=lse, **kw)(stream)
+    return out
+
+
+class TreeCommitter:
+    """Reusable launcher that copies accepted drafts' rows to the end of the cache, one call for all caches (every layer's
+    K and V) and their drafts.  accepted int32 [n_seq, max_accepted], n_accepted, kv_len, kv_len_out int32 [n_seq];
+    kv_len_out may be kv_len."""
+
+    def __init__(self, ctx: Context, caches: Sequence[Tensor], drafts: Sequence[Tensor], accepted, n_accepted, kv_len,
+                 kv_len_out):
+        torch = _torch()
+        if len(caches) != len(drafts) or not caches:
+            raise ValueError("TreeCommitter: as many drafts as caches, one at least")
+        n_seq, most = _dense(accepted, (torch.int32,), "TreeCommitter accepted").shape
+        for t, what in ((n_accepted, "n_accepted"), (kv_len, "kv_len"), (kv_len_out, "kv_len_out")):
+            _dense(t, (torch.int32,), f"TreeCommitter {what}", (n_seq,))
+        self.ctx = ctx
+        p = TreeCommitParams()
+        self._caches, self._drafts = (Tensor * len(caches))(*caches), (Tensor * len(drafts))(*drafts)
+        p.caches, p.drafts, p.n_tensors, p.n_seq = self._caches, self._drafts, len(caches), n_seq
+        p.accepted, p.accepted_stride, p.max_accepted = accepted.data_ptr(), most, most
+        p.n_accepted, p.kv_len, p.kv_len_out = n_accepted.data_ptr(), kv_len.data_ptr(), kv_len_out.data_ptr()
+        self.params = p
+        self._ref = ctypes.byref(p)
+        self._keep = (list(caches), list(drafts), accepted, n_accepted, kv_len, kv_len_out)
+
+    def __call__(self, stream=None) -> None:
+        check(lib.cvattn_tree_commit(self.ctx.handle, _stream(stream), self._ref), "tree_commit")
+
+
+def tree_commit(ctx: Context, caches, drafts, accepted, n_accepted, kv_len, kv_len_out=None, stream=None):
+    """Commit accepted drafts; returns kv_len_out (by default kv_len, in place)."""
+    kv_len_out = kv_len if kv_len_out is None else kv_len_out
+    TreeCommitter(ctx, caches, drafts, accepted, n_accepted, kv_len, kv_len_out)(stream)
+    return kv_len_out
+
+
+class KVScorer:
+    """Reusable launcher that adds the attention weight of the rows q f32 [n_seq, n_q_rows, Hq, D] with log-sums
+    lse f32 [n_seq, n_q_rows, Hq] to scores f32 [n_seq, Hkv, slots] (scores_out may be scores).  rows int32
+    [n_seq, max_rows] picks the rows; None: the first max_rows (n_q_rows)."""
+
+    def __init__(self, ctx: Context, k: Tensor, q, lse, kv_len, scores, scores_out=None, max_kv_len: int | None = None,
+                 decay: float = 1.0, rows=None, n_rows=None, k_seq_ptrs=None, scale: float | None = None):
+        torch = _torch()
+        self.ctx = ctx
+        scores_out = scores if scores_out is None else scores_out
+        n_seq, n, Hq, D = _rows4(q, "KVScorer q").shape
+        _dense(lse, (torch.float32,), "KVScorer lse", (n_seq, n, Hq))
+        _dense(kv_len, (torch.int32,), "KVScorer kv_len", (n_seq,))
+        if scores.dim() != 3 or scores.shape[:2] != (n_seq, k.n_heads) or scores.stride(2) != 1 or scores.dtype != torch.float32:
+            raise ValueError("KVScorer scores: want f32 [n_seq, Hkv, slots]")
+        if scores_out.shape != scores.shape or scores_out.stride() != scores.stride() or scores_out.dtype != torch.float32:
+            raise ValueError("KVScorer scores_out: want the layout of scores")
+        p = KVScoresParams()
+        p.q, p.q_nb_seq, p.q_nb_node = q.data_ptr(), q.stride(0), Hq * D if n == 1 else q.stride(1)
+        p.lse, p.k, p.k_seq_ptrs = lse.data_ptr(), k, _ptr(k_seq_ptrs)
+        p.n_q_rows = p.max_rows = n
+        if rows is not None:
+            _dense(rows, (torch.int32,), "KVScorer rows")
+            if rows.dim() != 2 or rows.shape[0] != n_seq:
+                raise ValueError("KVScorer rows: want [n_seq, max_rows]")
+            p.rows, p.max_rows = rows.data_ptr(), rows.shape[1]
+        if n_rows is not None:
+            p.n_rows = _dense(n_rows, (torch.int32,), "KVScorer n_rows", (n_seq,)).data_ptr()
+        p.kv_len = kv_len.data_ptr()
+        p.scores, p.scores_out = scores.data_ptr(), scores_out.data_ptr()
+        p.scores_nb_seq, p.scores_nb_head = scores.stride(0), scores.stride(1)
+        p.n_seq, p.n_q_heads = n_seq, Hq
+        p.max_kv_len = scores.shape[2] if max_kv_len is None else max_kv_len
+        if p.max_kv_len > scores.shape[2]:
+            raise ValueError("KVScorer max_kv_len: above the slots of scores")
+        p.scale, p.decay = 1.0 / math.sqrt(D) if scale is None else scale, decay
+        self.params = p
+        self._ref = ctypes.byref(p)
+        self._keep = (q, lse, kv_len, scores, scores_out, rows, n_rows, k_seq_ptrs)
+
+    def __call__(self, stream=None) -> None:
+        check(lib.cvattn_kv_scores(self.ctx.handle, _stream(stream), self._ref), "kv_scores")
+
+
+def kv_scores(ctx: Context, k: Tensor, q, lse, kv_len, scores, scores_out=None, stream=None, **kw):
+    """Add the weights of the given rows to the scores; returns scores_out (by default scores, in place)."""
+    KVScorer(ctx, k, q, lse, kv_len, scores, scores_out, **kw)(stream)
+    return scores if scores_out is None else scores_out
+
+
+class KVEvictor:
+    """Reusable launcher that shrinks every (layer, sequence, KV head) to `budget` positions.  k, v: the layers' caches;
+    scores f32 and pos int32 [layers, n_seq, Hkv, slots]; kv_len, kept_len (None: none), n_tokens (None: kv_len),
+    kv_len_out int32 [n_seq].  scores_out, pos_out may be scores, pos (the defaults), kv_len_out may be kv_len or kept_len."""
+
+    def __init__(self, ctx: Context, k: Sequence[Tensor], v: Sequence[Tensor], scores, pos, kv_len, kept_len, n_tokens,
+                 budget: int, scores_out=None, pos_out=None, kv_len_out=None, max_kv_len: int | None = None, n_sink: int = 0,
+                 n_recent: int = 0, workspace=None):
+        torch = _torch()
+        self.ctx = ctx
+        scores_out, pos_out = scores if scores_out is None else scores_out, pos if pos_out is None else pos_out
+        kv_len_out = kv_len if kv_len_out is None else kv_len_out
+        if len(k) != len(v) or not k:
+            raise ValueError("KVEvictor: as many V as K tensors, one at least")
+        if scores.dim() != 4 or scores.shape[0] != len(k) or scores.shape[2] != k[0].n_heads or scores.stride(3) != 1:
+            raise ValueError("KVEvictor scores: want [layers, n_seq, Hkv, slots]")
+        for t, dtype, what in ((scores, torch.float32, "scores"), (scores_out, torch.float32, "scores_out"),
+                               (pos, torch.int32, "pos"), (pos_out, torch.int32, "pos_out")):
+            if t.shape != scores.shape or t.stride() != scores.stride() or t.dtype != dtype or not t.is_cuda:
+                raise ValueError(f"KVEvictor {what}: want {dtype} in the layout of scores")
+        n_seq = scores.shape[1]
+        for t, what in ((kv_len, "kv_len"), (kept_len, "kept_len"), (n_tokens, "n_tokens"), (kv_len_out, "kv_len_out")):
+            if t is not None:
+                _dense(t, (torch.int32,), f"KVEvictor {what}", (n_seq,))
+        p = KVEvictParams()
+        self._k, self._v = (Tensor * len(k))(*k), (Tensor * len(v))(*v)
+        p.k, p.v, p.n_layers, p.n_seq = self._k, self._v, len(k), n_seq
+        p.scores, p.scores_out, p.pos, p.pos_out = scores.data_ptr(), scores_out.data_ptr(), pos.data_ptr(), pos_out.data_ptr()
+        p.nb_layer, p.nb_seq, p.nb_head = scores.stride(0), scores.stride(1), scores.stride(2)
+        p.kv_len, p.kept_len, p.n_tokens, p.kv_len_out = kv_len.data_ptr(), _ptr(kept_len), _ptr(n_tokens), kv_len_out.data_ptr()
+        p.max_kv_len = scores.shape[3] if max_kv_len is None else max_kv_len
+        if p.max_kv_len > scores.shape[3]:
+            raise ValueError("KVEvictor max_kv_len: above the slots of scores")
+        p.budget, p.n_sink, p.n_recent = budget, n_sink, n_recent
+        if workspace is None:
+            need = int(lib.cvattn_kv_evict_workspace_size(len(k), n_seq, k[0].n_heads, p.max_kv_len, budget))
+            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=scores.device)
+        self.workspace = workspace
+        p.workspace, p.workspace_size = workspace.data_ptr(), workspace.numel()
+        self.params = p
+        self._ref = ctypes.byref(p)
+        self._keep = (list(k), list(v), scores, scores_out, pos, pos_out, kv_len, kept_len, n_tokens, kv_len_out)
+
+    def __call__(self, stream=None) -> None:
+        check(lib.cvattn_kv_evict(self.ctx.handle, _stream(stream), self._ref), "kv_evict")
+
+
+def kv_evict(ctx: Context, k, v, scores, pos, kv_len, kept_len, n_tokens, budget: int, stream=None, **kw) -> None:
+    """Shrink the caches to the budget (in place unless *_out are given)."""
+    KVEvictor(ctx, k, v, scores, pos, kv_len, kept_len, n_tokens, budget, **kw)(stream)
 
 
 class KVCache:

@@ -13,6 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcvattn.so")
 ABI_VERSION = 2
 MAX_CHUNK_BOUNDS = 64
+TREE_MAX_NODES = 256
 
 c_void_p, c_int32, c_int64, c_uint32, c_float, c_size_t, c_uint8 = (
     ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_float, ctypes.c_size_t, ctypes.c_uint8)
@@ -71,7 +72,49 @@ class RopeParams(ctypes.Structure):
     ]
 
 
-STRUCTS = {0: Tensor, 1: DecodeParams, 2: FlashParams, 3: KVCacheParams, 4: DitStep, 5: RopeParams}
+class TreeParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_nb_node", c_int64), ("q_nb_seq", c_int64),
+        ("out", c_void_p), ("out_nb_node", c_int64), ("out_nb_seq", c_int64), ("lse", c_void_p),
+        ("k", Tensor), ("v", Tensor), ("k_seq_ptrs", c_void_p), ("v_seq_ptrs", c_void_p),
+        ("k_draft", Tensor), ("v_draft", Tensor), ("kv_len", c_void_p), ("n_nodes", c_void_p),
+        ("mask", c_void_p), ("mask_nb_seq", c_int64), ("n_seq", c_int32), ("max_nodes", c_int32),
+        ("n_q_heads", c_int32), ("max_kv_len", c_int32), ("scale", c_float), ("flags", c_int32),
+        ("workspace", c_void_p), ("workspace_size", c_size_t),
+    ]
+
+
+class TreeCommitParams(ctypes.Structure):
+    _fields_ = [
+        ("caches", ctypes.POINTER(Tensor)), ("drafts", ctypes.POINTER(Tensor)), ("n_tensors", c_int32),
+        ("n_seq", c_int32), ("accepted", c_void_p), ("accepted_stride", c_int64), ("max_accepted", c_int32),
+        ("reserved", c_int32), ("n_accepted", c_void_p), ("kv_len", c_void_p), ("kv_len_out", c_void_p),
+    ]
+
+
+class KVScoresParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_nb_node", c_int64), ("q_nb_seq", c_int64), ("lse", c_void_p), ("k", Tensor),
+        ("k_seq_ptrs", c_void_p), ("rows", c_void_p), ("n_rows", c_void_p), ("kv_len", c_void_p),
+        ("scores", c_void_p), ("scores_out", c_void_p), ("scores_nb_head", c_int64), ("scores_nb_seq", c_int64),
+        ("n_seq", c_int32), ("n_q_rows", c_int32), ("max_rows", c_int32), ("n_q_heads", c_int32),
+        ("max_kv_len", c_int32), ("scale", c_float), ("decay", c_float), ("reserved", c_int32),
+    ]
+
+
+class KVEvictParams(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.POINTER(Tensor)), ("v", ctypes.POINTER(Tensor)), ("n_layers", c_int32), ("n_seq", c_int32),
+        ("scores", c_void_p), ("scores_out", c_void_p), ("pos", c_void_p), ("pos_out", c_void_p),
+        ("nb_head", c_int64), ("nb_seq", c_int64), ("nb_layer", c_int64), ("kv_len", c_void_p),
+        ("kept_len", c_void_p), ("n_tokens", c_void_p), ("kv_len_out", c_void_p), ("max_kv_len", c_int32),
+        ("budget", c_int32), ("n_sink", c_int32), ("n_recent", c_int32), ("workspace", c_void_p),
+        ("workspace_size", c_size_t),
+    ]
+
+
+STRUCTS = {0: Tensor, 1: DecodeParams, 2: FlashParams, 3: KVCacheParams, 4: DitStep, 5: RopeParams, 6: TreeParams,
+           7: TreeCommitParams, 8: KVScoresParams, 9: KVEvictParams}
 
 # (name, restype, argtypes) for every symbol include/cvattn.h declares.
 P = ctypes.POINTER
@@ -103,6 +146,12 @@ SIGNATURES = [
     ("cvattn_decode_rope", c_int32, [c_void_p, c_void_p, P(DecodeParams), P(RopeParams)]),
     ("cvattn_combine", c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p]),
     ("cvattn_flash", c_int32, [c_void_p, c_void_p, P(FlashParams)]),
+    ("cvattn_tree_decode_workspace_size", c_size_t, [c_int32] * 8),
+    ("cvattn_tree_decode", c_int32, [c_void_p, c_void_p, P(TreeParams)]),
+    ("cvattn_tree_commit", c_int32, [c_void_p, c_void_p, P(TreeCommitParams)]),
+    ("cvattn_kv_scores", c_int32, [c_void_p, c_void_p, P(KVScoresParams)]),
+    ("cvattn_kv_evict_workspace_size", c_size_t, [c_int32] * 5),
+    ("cvattn_kv_evict", c_int32, [c_void_p, c_void_p, P(KVEvictParams)]),
     ("cvattn_kv_copy_to_host", c_int32, [c_void_p, P(Tensor), c_int32, c_void_p]),
     ("cvattn_kv_copy_from_host", c_int32, [c_void_p, P(Tensor), c_int32, c_void_p]),
     ("cvattn_kv_cache_create", c_int32, [c_void_p, P(KVCacheParams), P(c_void_p)]),

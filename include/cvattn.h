@@ -54,7 +54,9 @@ int32_t cvattn_status_to_ggml(cvattn_status s);
 
 /* ABI version and struct sizes, so bindings can verify their mirrors.
  * which: 0 cvattn_tensor, 1 cvattn_decode_params, 2 cvattn_flash_params,
- *        3 cvattn_kv_cache_params, 4 cvattn_dit_step, 5 cvattn_rope_params. */
+ *        3 cvattn_kv_cache_params, 4 cvattn_dit_step, 5 cvattn_rope_params,
+ *        6 cvattn_tree_params, 7 cvattn_tree_commit_params,
+ *        8 cvattn_kv_scores_params, 9 cvattn_kv_evict_params. */
 int32_t cvattn_abi_version(void);
 size_t cvattn_abi_sizeof(int32_t which);
 
@@ -350,6 +352,171 @@ enum {
 };
 
 cvattn_status cvattn_flash(cvattn_context* ctx, void* stream, const cvattn_flash_params* p);
+
+/* -------------------------------------------------- speculative decoding */
+
+/* Attention for a tree of drafted tokens (no counterpart in the reference,
+ * which decodes one token a step, src/cosyvoice-llm.cpp:204-318).  A draft of
+ * up to CVATTN_TREE_MAX_NODES tokens per sequence is verified in one pass:
+ * node i of sequence s sees the kv_len[s] committed positions of the cache and
+ * the drafted rows whose bit its mask row has set (its ancestors and itself).
+ *   out[s][i][h] = sum_j p_j v_j,  p = softmax_j(scale q.k_j),
+ *   lse[s][i][h] = log(sum_j exp(scale q.k_j))                (natural log).
+ * The drafted K/V rows lie beside the cache in tensors of the cache's types
+ * (append them with cvattn_kv_append at positions 0 .. n - 1, their keys rotated
+ * by their own positions with cvattn_rope), so a rejected draft leaves no trace
+ * in the cache and an accepted one attends exactly as it will once committed.
+ * Products are exact in f32 for every cache type, as in cvattn_decode.
+ *   - A row that sees nothing gives zeros and lse = -inf.
+ *   - Rows from n_nodes[s] up to max_nodes are written as such rows too.
+ *   - A kv_len[s] outside [0, max_kv_len] or n_nodes[s] outside [0, max_nodes]
+ *     is recorded in the status word and the sequence gives such rows only.
+ * cache and draft rows may have any even stride of at least a row. */
+#define CVATTN_TREE_MAX_NODES 256
+
+typedef struct cvattn_tree_params {
+    const float*    q;            /* device f32; element (d, h, i, s) at           */
+    int64_t         q_nb_node;    /* q + s*q_nb_seq + i*q_nb_node + h*head_dim + d */
+    int64_t         q_nb_seq;     /* (strides in floats, multiples of 4)           */
+    float*          out;          /* device f32, laid out the same way             */
+    int64_t         out_nb_node;
+    int64_t         out_nb_seq;
+    float*          lse;          /* optional device f32 [n_seq][max_nodes][n_q_heads] */
+    cvattn_tensor   k;            /* the cache, as in cvattn_decode_params */
+    cvattn_tensor   v;
+    const uint64_t* k_seq_ptrs;   /* optional device [n_seq]: row-0 address per sequence */
+    const uint64_t* v_seq_ptrs;
+    cvattn_tensor   k_draft;      /* drafted rows: node i of sequence s at data + s*nb2 + i*nb1; */
+    cvattn_tensor   v_draft;      /* both data NULL: the queries see the cache only              */
+    const int32_t*  kv_len;       /* device [n_seq]: committed positions */
+    const int32_t*  n_nodes;      /* optional device [n_seq]; NULL: max_nodes each */
+    const uint32_t* mask;         /* optional device bits: node i sees node j iff bit j % 32 of     */
+    int64_t         mask_nb_seq;  /* mask[s*mask_nb_seq + i*((max_nodes+31)/32) + j/32]; NULL: a    */
+                                  /* chain (j <= i); mask_nb_seq 0: one tree for all sequences      */
+    int32_t         n_seq;
+    int32_t         max_nodes;
+    int32_t         n_q_heads;
+    int32_t         max_kv_len;   /* host bound on kv_len[] */
+    float           scale;
+    int32_t         flags;        /* 0 */
+    void*           workspace;    /* device scratch of cvattn_tree_decode_workspace_size bytes; */
+    size_t          workspace_size; /* needs no initialization                                  */
+} cvattn_tree_params;
+
+/* Workspace bytes for cvattn_tree_decode; 0 if the shape is unsupported or
+ * needs none (cvattn_supports tells the two apart). */
+size_t cvattn_tree_decode_workspace_size(int32_t k_type, int32_t v_type, int32_t n_seq, int32_t max_kv_len,
+                                         int32_t max_nodes, int32_t n_q_heads, int32_t n_kv_heads,
+                                         int32_t head_dim);
+
+cvattn_status cvattn_tree_decode(cvattn_context* ctx, void* stream, const cvattn_tree_params* p);
+
+/* Copy the accepted drafts' rows to the end of the cache, every layer's K and V
+ * in one call: row accepted[s][i] of draft tensor t goes to position
+ * kv_len[s] + i of cache tensor t, and kv_len_out[s] = kv_len[s] + n_accepted[s].
+ * drafts[t] must have the type and heads of caches[t] and other memory.
+ * A sequence whose rows do not fit its cache, or with a count or node out of
+ * range, is left as it is and recorded in the status word. */
+typedef struct cvattn_tree_commit_params {
+    const cvattn_tensor* caches;    /* host array [n_tensors] */
+    const cvattn_tensor* drafts;    /* host array [n_tensors] */
+    int32_t         n_tensors;
+    int32_t         n_seq;
+    const int32_t*  accepted;       /* device: node i of sequence s at accepted[s*accepted_stride + i] */
+    int64_t         accepted_stride;
+    int32_t         max_accepted;
+    int32_t         reserved;       /* 0 */
+    const int32_t*  n_accepted;     /* device [n_seq]: 0 .. max_accepted */
+    const int32_t*  kv_len;         /* device [n_seq] */
+    int32_t*        kv_len_out;     /* device [n_seq]; may be kv_len (one launch more) */
+} cvattn_tree_commit_params;
+
+cvattn_status cvattn_tree_commit(cvattn_context* ctx, void* stream, const cvattn_tree_commit_params* p);
+
+/* ------------------------------------------------------ a bounded KV cache */
+
+/* Attention weight per cached position (no counterpart in the reference, whose
+ * cache ends the generation when it is full, src/cosyvoice-llm.cpp:207):
+ *   scores_out[s][g][j] = decay * scores[s][g][j]
+ *       + sum over rows i < n_rows[s] that see j, query heads h of KV head g, of
+ *         exp(scale q_ih.k_j - lse_ih),          j < kv_len[s].
+ * The rows are the sequence's last n_rows[s] tokens in slot order: row i sees
+ * the slots j < kv_len[s] - n_rows[s] + i + 1.  q and lse are those of the
+ * attention that verified them (cvattn_tree_decode); rows, if given, picks the
+ * i-th row's place in q and lse (an accepted path).  A row with lse = -inf adds
+ * nothing.  Entries from kv_len[s] on are not written.  A kv_len, n_rows (above
+ * max_rows or kv_len) or row index (outside [0, n_q_rows)) out of range is
+ * recorded in the status word and the sequence skipped, the row left out. */
+typedef struct cvattn_kv_scores_params {
+    const float*    q;              /* device f32; strides as in cvattn_tree_params */
+    int64_t         q_nb_node;
+    int64_t         q_nb_seq;
+    const float*    lse;            /* device f32; (h, i, s) at lse + (s*n_q_rows + i)*n_q_heads + h */
+    cvattn_tensor   k;
+    const uint64_t* k_seq_ptrs;     /* optional device [n_seq] */
+    const int32_t*  rows;           /* optional device [n_seq][max_rows] */
+    const int32_t*  n_rows;         /* optional device [n_seq]; NULL: max_rows each */
+    const int32_t*  kv_len;         /* device [n_seq] */
+    const float*    scores;         /* device f32; slot j of KV head g at            */
+    float*          scores_out;     /* s*scores_nb_seq + g*scores_nb_head + j; may be scores */
+    int64_t         scores_nb_head;
+    int64_t         scores_nb_seq;
+    int32_t         n_seq;
+    int32_t         n_q_rows;       /* rows of q and lse per sequence */
+    int32_t         max_rows;
+    int32_t         n_q_heads;
+    int32_t         max_kv_len;
+    float           scale;
+    float           decay;
+    int32_t         reserved;       /* 0 */
+} cvattn_kv_scores_params;
+
+cvattn_status cvattn_kv_scores(cvattn_context* ctx, void* stream, const cvattn_kv_scores_params* p);
+
+/* Shrink every sequence to at most `budget` positions by its accumulated
+ * attention weight, for each layer and KV head on its own.  Slot j holds token
+ * pos[j] where j < kept_len (what the last eviction left), else the next tokens
+ * in order, the last slot holding token n_tokens - 1.  Kept are the first n_sink
+ * tokens, the last n_recent ones and, up to the budget, the highest scores (ties:
+ * the lower slot; a NaN ranks below every number).  Kept rows at slots >= budget
+ * move into the freed slots below it, both in ascending order; other rows stay.
+ * Attention does not depend on the order of the rows, and cached keys carry
+ * their rotation, so the heads may keep different tokens.
+ *   scores_out, pos_out  the scores and tokens of slots [0, new length);
+ *                        scores_out is 0 from there to kv_len;
+ *   kv_len_out[s]        min(kv_len[s], budget).
+ * A sequence within the budget keeps its rows, scores and (filled in) tokens.
+ * scores_out, pos_out may be scores, pos, and kv_len_out may be kv_len or
+ * kept_len (one launch more).  A kv_len outside [0, max_kv_len] or kept_len
+ * outside [0, kv_len] is recorded in the status word and the sequence skipped. */
+typedef struct cvattn_kv_evict_params {
+    const cvattn_tensor* k;         /* host arrays [n_layers]; all layers share types, shapes */
+    const cvattn_tensor* v;         /* and strides                                            */
+    int32_t         n_layers;
+    int32_t         n_seq;
+    const float*    scores;         /* device; (layer, s, g, j) at layer*nb_layer + s*nb_seq + */
+    float*          scores_out;     /* g*nb_head + j (elements) in all four arrays             */
+    const int32_t*  pos;
+    int32_t*        pos_out;
+    int64_t         nb_head;
+    int64_t         nb_seq;
+    int64_t         nb_layer;
+    const int32_t*  kv_len;         /* device [n_seq] */
+    const int32_t*  kept_len;       /* device [n_seq]: slots whose pos is set; NULL: none (pos may be NULL) */
+    const int32_t*  n_tokens;       /* device [n_seq]: tokens seen so far; NULL: kv_len */
+    int32_t*        kv_len_out;     /* device [n_seq] */
+    int32_t         max_kv_len;
+    int32_t         budget;         /* >= 1 */
+    int32_t         n_sink;         /* >= 0, n_sink + n_recent <= budget */
+    int32_t         n_recent;
+    void*           workspace;      /* device scratch of cvattn_kv_evict_workspace_size bytes; */
+    size_t          workspace_size; /* needs no initialization                                 */
+} cvattn_kv_evict_params;
+
+size_t cvattn_kv_evict_workspace_size(int32_t n_layers, int32_t n_seq, int32_t n_kv_heads, int32_t max_kv_len,
+                                      int32_t budget);
+
+cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv_evict_params* p);
 
 /* ------------------------------------------------------- offload and load */
 
