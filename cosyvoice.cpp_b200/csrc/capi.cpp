@@ -513,7 +513,7 @@ size_t cvattn_tree_decode_workspace_size(int32_t k_type, int32_t v_type, int32_t
                                          int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
     if (n_seq <= 0 || max_kv_len < 0 || max_nodes <= 0 || max_nodes > CVATTN_TREE_MAX_NODES) return 0;
     if (!tree_supported(k_type, v_type, head_dim, n_q_heads, n_kv_heads)) return 0;
-    return tree_workspace_bytes(n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
+    return tree_workspace_bytes(k_type, v_type, n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
 }
 
 cvattn_status cvattn_tree_decode(cvattn_context* ctx, void* stream, const cvattn_tree_params* p) {
@@ -545,7 +545,8 @@ cvattn_status cvattn_tree_decode(cvattn_context* ctx, void* stream, const cvattn
     if (p->n_seq > 1 && p->out_nb_seq < row) return CVATTN_ERR_INVALID_ARGUMENT;
     if (p->mask && (p->mask_nb_seq < 0 || (p->mask_nb_seq && p->mask_nb_seq < (int64_t)p->max_nodes * ((p->max_nodes + 31) / 32))))
         return CVATTN_ERR_INVALID_ARGUMENT;
-    const size_t need = tree_workspace_bytes(p->n_seq, p->max_kv_len, p->max_nodes, p->n_q_heads, p->k.n_heads);
+    const size_t need = tree_workspace_bytes(p->k.type, p->v.type, p->n_seq, p->max_kv_len, p->max_nodes, p->n_q_heads,
+                                             p->k.n_heads);
     if (need && (!p->workspace || p->workspace_size < need || (reinterpret_cast<uintptr_t>(p->workspace) & 15)))
         return CVATTN_ERR_INVALID_ARGUMENT;
     DeviceGuard dg(ctx->device);

@@ -53,7 +53,8 @@ cudaError_t launch_flash(cudaStream_t stream, const cvattn_flash_params& p, int*
 
 // tree_decode.cu
 bool tree_supported(int k_type, int v_type, int head_dim, int n_q_heads, int n_kv_heads);
-size_t tree_workspace_bytes(int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads);
+size_t tree_workspace_bytes(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads,
+                            int n_kv_heads);
 cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p, int* status);
 
 // kv_scores.cu

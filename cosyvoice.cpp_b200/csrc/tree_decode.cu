@@ -1,5 +1,5 @@
 // tree_decode.cu -- kernels and host side of cvattn_tree_decode.
-#include "tree_decode.cuh"
+#include "tree_mma.cuh"
 
 namespace cvattn {
 namespace tree {
@@ -10,6 +10,7 @@ namespace tree {
 // are dequantized to f32 in shared memory; a thread owns 4 rows x 4 keys of S and
 // then 4 rows x 4 dims of the output.  Rows are padded to 68 floats, so the eight
 // float4s of a phase (keys apart by one row) touch different banks.
+constexpr int kTile = 64;  // keys per tile
 constexpr int kRows = 32;
 constexpr int kPad = kD + 4;
 
@@ -124,6 +125,7 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const __grid_constant__ A
         }
         __syncwarp();
     }
+    griddep_launch_dependents();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = r0 + tr * 4 + i;
@@ -138,68 +140,155 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const __grid_constant__ A
         } else if (r < rows) {
             const int64_t slot = (((int64_t)s * a.Hkv + kvh) * a.n_splits + split) * all_rows + r;
             *reinterpret_cast<float4*>(a.ws_o + slot * kD + tc * 4) = o[i];
-            if (tc == 0) *reinterpret_cast<float2*>(a.ws_ml + slot * 2) = make_float2(m[i], l[i]);
+            // (a row whose scores are all NaN has no maximum, but was seen)
+            if (tc == 0) *reinterpret_cast<float2*>(a.ws_ml + slot * 2) = make_float2(m[i] == -INFINITY && l[i] != 0.0f ? 0.0f : m[i], l[i]);
         }
     }
 }
 
 // --------------------------------------------------------------- combine --
 //
-// A half-warp per row joins the splits that its sequence has: out = sum_k
-// 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k, in the order of the splits.
+// out = sum_k 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k over the splits that the
+// sequence has.  16 threads (4 dims each) follow every kLanes-th split of a row;
+// the kLanes partial sums of a row are joined through shared memory in order.
+template <int kLanes>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Args a) {
-    const int half = threadIdx.x >> 4, c = threadIdx.x & 15;
+    constexpr int kPer = 16 / kLanes;  // rows per CTA
+    __shared__ float4 so[16][16];
+    __shared__ float2 sml[16];
+    griddep_wait();
+    const int unit = threadIdx.x >> 4, c = threadIdx.x & 15, lane = unit % kLanes;
     const int all_rows = a.max_nodes * a.G;
-    const int r = blockIdx.x * 16 + half, kvh = blockIdx.y, s = blockIdx.z;
-    if (r >= all_rows) return;
+    const int r = blockIdx.x * kPer + unit / kLanes, kvh = blockIdx.y, s = blockIdx.z;
     const Lens x = lens_of(a, s, false);
     const int node = r / a.G, h = kvh * a.G + r % a.G;
-    const int n = node < x.n ? (x.tiles + a.split_tiles - 1) / a.split_tiles : 0;
+    const int n = node < x.n ? (x.tiles + a.split_tiles - 1) / a.split_tiles : 0;  // (rows past the last: none)
     const int64_t slot = ((int64_t)s * a.Hkv + kvh) * a.n_splits * all_rows + r;
     float M = -INFINITY, l = 0.0f;
-    for (int k = 0; k < n; ++k) M = fmaxf(M, a.ws_ml[(slot + (int64_t)k * all_rows) * 2]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (M != -INFINITY) {
-        for (int k = 0; k < n; ++k) {
-            const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (slot + (int64_t)k * all_rows) * 2);
-            const float4 v = *reinterpret_cast<const float4*>(a.ws_o + (slot + (int64_t)k * all_rows) * kD + c * 4);
-            const float f = exp2f(ml.x - M);
-            l = fmaf(f, ml.y, l);
-            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+    for (int k0 = lane; k0 < n; k0 += 4 * kLanes) {
+        float2 ml[4];
+        float4 v[4];
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int k = k0 + u * kLanes;
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (k < n) {
+                ml[u] = *reinterpret_cast<const float2*>(a.ws_ml + (slot + (int64_t)k * all_rows) * 2);
+                v[u] = *reinterpret_cast<const float4*>(a.ws_o + (slot + (int64_t)k * all_rows) * kD + c * 4);
+            }
+            top = fmaxf(top, ml[u].x);
+        }
+        if (top == -INFINITY) continue;
+        const float f0 = exp2f(M - top);
+        M = top;
+        l *= f0;
+        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (ml[u].x == -INFINITY) continue;
+            const float f = exp2f(ml[u].x - M);
+            l = fmaf(f, ml[u].y, l);
+            o.x = fmaf(f, v[u].x, o.x); o.y = fmaf(f, v[u].y, o.y); o.z = fmaf(f, v[u].z, o.z); o.w = fmaf(f, v[u].w, o.w);
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if constexpr (kLanes > 1) {
+        so[unit][c] = o;
+        if (c == 0) sml[unit] = make_float2(M, l);
+        __syncthreads();
+        if (lane) return;
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) top = fmaxf(top, sml[unit + k].x);
+        l = 0.0f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        M = top;
+        if (top != -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < kLanes; ++k) {
+                if (sml[unit + k].x == -INFINITY) continue;
+                const float f = exp2f(sml[unit + k].x - top);
+                const float4 v = so[unit + k][c];
+                l = fmaf(f, sml[unit + k].y, l);
+                o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+            }
+        }
+    }
+    if (r >= all_rows) return;
+    const bool seen = M != -INFINITY;
+    const float inv = seen ? 1.0f / l : 0.0f;
     *reinterpret_cast<float4*>(a.out + (int64_t)s * a.out_nb_seq + (int64_t)node * a.out_nb_node + h * kD + c * 4) =
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (a.lse && c == 0) a.lse[((int64_t)s * a.max_nodes + node) * a.Hq + h] = (M + log2f(l)) * 0.69314718055994531f;
+    if (a.lse && c == 0) a.lse[((int64_t)s * a.max_nodes + node) * a.Hq + h] = seen ? (M + log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
 // ------------------------------------------------------------------ host --
 
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// How the keys are split: about kWantCtas CTAs over (sequence, KV head, row tile, split), each with at least two tiles.
-constexpr int kWantCtas = 296;
+static bool mma_type(int t) { return t != kF32; }
 
+// Which kernel, its shape, and how the keys are split.
 struct Plan {
-    int split_tiles, n_splits;
+    bool mma;
+    int mt;
+    Shape sh;
+    int tile, split_tiles, n_splits;
 };
 
-static Plan plan_of(int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
-    const int tiles = (max_kv_len + kTile - 1) / kTile + (max_nodes + kTile - 1) / kTile;
-    const int64_t row_tiles = ((int64_t)max_nodes * (n_q_heads / n_kv_heads) + kRows - 1) / kRows;
-    const int64_t units = (int64_t)n_seq * n_kv_heads * row_tiles;
+static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
+    Plan p{};
+    const int64_t rows = (int64_t)max_nodes * (n_q_heads / n_kv_heads);
+    p.mma = mma_type(k_type) && mma_type(v_type);
+    int64_t units;
+    if (p.mma) {
+        p.tile = kKeys;
+        p.mt = rows <= 16 ? 1 : 2;
+        p.sh.hc = n_kv_heads % 2 == 0 && rows <= 64 ? 2 : 1;
+        const int64_t groups = (rows + 16 * p.mt - 1) / (16 * p.mt);  // warps along the rows, up to 8
+        p.sh.wr = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
+        p.sh.wk = kWarps / (p.sh.hc * p.sh.wr);
+        p.sh.row_groups = (int)((rows + 16 * p.mt * p.sh.wr - 1) / (16 * p.mt * p.sh.wr));
+        p.sh.stages = kMaxStages;
+        if (Smem(k_type, v_type, p.mt, p.sh.hc, p.sh.wr, kMaxStages).total > kSmemLimit) p.sh.stages = 2;
+        units = (int64_t)n_seq * (n_kv_heads / p.sh.hc) * p.sh.row_groups;
+    } else {
+        p.tile = kTile;
+        units = (int64_t)n_seq * n_kv_heads * ((rows + kRows - 1) / kRows);
+    }
+    // about kWantCtas CTAs, each with at least two tiles
+    constexpr int kWantCtas = 296;
+    const int tiles = (max_kv_len + p.tile - 1) / p.tile + (max_nodes + p.tile - 1) / p.tile;
     int64_t want = (kWantCtas + units - 1) / units;
     if (want > tiles / 2) want = tiles / 2;
     if (want < 1) want = 1;
-    Plan p;
     p.split_tiles = (int)((tiles + want - 1) / want);
     p.n_splits = (tiles + p.split_tiles - 1) / p.split_tiles;
     return p;
 }
 
-size_t workspace_bytes(int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
-    const Plan p = plan_of(n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
+template <int kLanes>
+static cudaError_t run_combine(cudaStream_t stream, const Args& a) {
+    const int rows = a.max_nodes * a.G;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)a.Hkv, (unsigned)a.n_seq);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tree_combine_kernel<kLanes>, a);
+}
+
+static cudaError_t launch_combine(cudaStream_t stream, const Args& a) {
+    return a.n_splits > 32 ? run_combine<16>(stream, a) : a.n_splits > 8 ? run_combine<4>(stream, a) : run_combine<1>(stream, a);
+}
+
+size_t workspace_bytes(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
+    const Plan p = plan_of(k_type, v_type, n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
     if (p.n_splits == 1) return 0;
     const size_t rows = (size_t)n_seq * p.n_splits * max_nodes * n_q_heads;
     return align256(rows * 2 * 4) + rows * kD * 4;
@@ -212,8 +301,8 @@ bool tree_supported(int k_type, int v_type, int head_dim, int n_q_heads, int n_k
            n_q_heads % n_kv_heads == 0 && n_q_heads / n_kv_heads <= 8;
 }
 
-size_t tree_workspace_bytes(int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
-    return tree::workspace_bytes(n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
+size_t tree_workspace_bytes(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
+    return tree::workspace_bytes(k_type, v_type, n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
 }
 
 cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p, int* status) {
@@ -249,7 +338,8 @@ cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p,
     a.max_kv_len = p.max_kv_len;
     a.scale_log2 = p.scale * 1.4426950408889634f;
     a.status = status;
-    const Plan plan = plan_of(a.n_seq, a.max_kv_len, a.max_nodes, a.Hq, a.Hkv);
+    const Plan plan = plan_of(a.k_type, a.v_type, a.n_seq, a.max_kv_len, a.max_nodes, a.Hq, a.Hkv);
+    a.tile = plan.tile;
     a.split_tiles = plan.split_tiles;
     a.n_splits = plan.n_splits;
     if (plan.n_splits > 1) {
@@ -257,16 +347,28 @@ cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p,
         a.ws_ml = static_cast<float*>(p.workspace);
         a.ws_o = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + align256(rows * 2 * 4));
     }
-    const int rows = a.max_nodes * a.G;
-    const int smem = (2 * kRows + 2 * kTile) * kPad * 4;
-    cudaError_t e = cudaFuncSetAttribute(tree_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)plan.n_splits, (unsigned)(a.Hkv * ((rows + kRows - 1) / kRows)), (unsigned)a.n_seq);
-    tree_f32_kernel<<<grid, 128, smem, stream>>>(a);
-    e = cudaGetLastError();
+    cudaError_t e = cudaErrorInvalidValue;
+    if (plan.mma) {
+        switch (a.k_type) {
+        case kF16: e = launch_mma_for_k<kF16>(stream, a, plan.sh, plan.mt); break;
+        case kQ4_0: e = launch_mma_for_k<kQ4_0>(stream, a, plan.sh, plan.mt); break;
+        case kQ4_1: e = launch_mma_for_k<kQ4_1>(stream, a, plan.sh, plan.mt); break;
+        case kQ5_0: e = launch_mma_for_k<kQ5_0>(stream, a, plan.sh, plan.mt); break;
+        case kQ5_1: e = launch_mma_for_k<kQ5_1>(stream, a, plan.sh, plan.mt); break;
+        case kQ8_0: e = launch_mma_for_k<kQ8_0>(stream, a, plan.sh, plan.mt); break;
+        default: break;
+        }
+    } else {
+        const int rows = a.max_nodes * a.G;
+        const int smem = (2 * kRows + 2 * kTile) * kPad * 4;
+        e = cudaFuncSetAttribute(tree_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        const dim3 grid((unsigned)plan.n_splits, (unsigned)(a.Hkv * ((rows + kRows - 1) / kRows)), (unsigned)a.n_seq);
+        tree_f32_kernel<<<grid, 128, smem, stream>>>(a);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess || plan.n_splits == 1) return e;
-    tree_combine_kernel<<<dim3((unsigned)((rows + 15) / 16), (unsigned)a.Hkv, (unsigned)a.n_seq), 256, 0, stream>>>(a);
-    return cudaGetLastError();
+    return launch_combine(stream, a);
 }
 
 }  // namespace cvattn

@@ -5,9 +5,9 @@
 // cache and the drafted keys its mask row lists:
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp2(c q.k_j - m),  c = scale log2 e,
 // in one pass with a running maximum m and sum per row.  The keys of a sequence
-// form ceil(L / 64) cache tiles and ceil(n / 64) draft tiles; a split is a run of
-// consecutive tiles, and splits leave (m, sum) and an unnormalized output per row
-// for tree_combine_kernel.
+// form ceil(L / T) cache tiles and ceil(n / T) draft tiles of T keys; a split is a
+// run of consecutive tiles, and splits leave (m, sum) and an unnormalized output
+// per row for tree_combine_kernel.
 #pragma once
 
 #include "common.cuh"
@@ -17,7 +17,6 @@ namespace cvattn {
 namespace tree {
 
 constexpr int kD = 64;      // head size
-constexpr int kTile = 64;   // keys per tile
 
 struct Args {
     const float* q;
@@ -34,6 +33,7 @@ struct Args {
     int mask_words;
     int k_type, v_type;
     int n_seq, max_nodes, Hq, Hkv, G, max_kv_len;
+    int tile;                    // keys per tile
     int split_tiles, n_splits;   // tiles per split, most splits of a sequence
     float scale_log2;
     float* ws_ml;                // [seq][KV head][split][max_nodes * G][2]
@@ -56,8 +56,8 @@ __device__ __forceinline__ Lens lens_of(const Args& a, int s, bool record) {
         if (record) record_status(a.status, kStatusBadLength);
         x.L = x.n = 0;
     }
-    x.cache_tiles = (x.L + kTile - 1) / kTile;
-    x.tiles = x.n == 0 ? 0 : x.cache_tiles + (a.kd ? (x.n + kTile - 1) / kTile : 0);
+    x.cache_tiles = (x.L + a.tile - 1) / a.tile;
+    x.tiles = x.n == 0 ? 0 : x.cache_tiles + (a.kd ? (x.n + a.tile - 1) / a.tile : 0);
     return x;
 }
 

@@ -329,7 +329,8 @@ def test_refusals(ctx, cv, cuda):
     q = torch.zeros((2, 8, 14, D), device="cuda")
     out = torch.zeros_like(q)
     kl = torch.zeros(2, dtype=torch.int32, device="cuda")
-    plan = lambda: cv.TreeDecoder(ctx, k, k, d, d, q, out, kl, 640)  # noqa: E731
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")  # enough for every type
+    plan = lambda: cv.TreeDecoder(ctx, k, k, d, d, q, out, kl, 640, workspace=ws)  # noqa: E731
 
     def status(**kw):
         p = plan().params
