@@ -232,10 +232,11 @@ static bool mma_type(int t) { return t != kF32; }
 // Which kernel, its shape, and how the keys are split.
 struct Plan {
     bool mma;
-    int mt;
     Shape sh;
     int tile, split_tiles, n_splits;
 };
+
+constexpr int kSlots = 296;  // two CTAs on each of 148 SMs
 
 static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
     Plan p{};
@@ -244,24 +245,21 @@ static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_n
     int64_t units;
     if (p.mma) {
         p.tile = kKeys;
-        p.mt = rows <= 16 ? 1 : 2;
-        p.sh.hc = n_kv_heads % 2 == 0 && rows <= 64 ? 2 : 1;
-        const int64_t groups = (rows + 16 * p.mt - 1) / (16 * p.mt);  // warps along the rows, up to 8
-        p.sh.wr = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
-        p.sh.wk = kWarps / (p.sh.hc * p.sh.wr);
-        p.sh.row_groups = (int)((rows + 16 * p.mt * p.sh.wr - 1) / (16 * p.mt * p.sh.wr));
+        p.sh.row_groups = (int)((rows + 16 * kWarps - 1) / (16 * kWarps));
         p.sh.stages = kMaxStages;
-        if (Smem(k_type, v_type, p.mt, p.sh.hc, p.sh.wr, kMaxStages).total > kSmemLimit) p.sh.stages = 2;
-        units = (int64_t)n_seq * (n_kv_heads / p.sh.hc) * p.sh.row_groups;
+        while (p.sh.stages > 2 && Smem(k_type, v_type, p.sh.stages).total > kHalfSm) --p.sh.stages;
+        units = (int64_t)n_seq * n_kv_heads * p.sh.row_groups;
+        if (units * ((max_kv_len + kKeys - 1) / kKeys) < kSlots / 2) p.tile = kKeys / 2;  // few tiles: smaller ones, on more SMs
     } else {
         p.tile = kTile;
         units = (int64_t)n_seq * n_kv_heads * ((rows + kRows - 1) / kRows);
     }
-    // about kWantCtas CTAs, each with at least two tiles
-    constexpr int kWantCtas = 296;
+    // One wave of CTAs; two where the lengths of several sequences may differ, so that short ones leave room for parts of
+    // long ones.  At least two tiles per split once every slot has work.
     const int tiles = (max_kv_len + p.tile - 1) / p.tile + (max_nodes + p.tile - 1) / p.tile;
-    int64_t want = (kWantCtas + units - 1) / units;
-    if (want > tiles / 2) want = tiles / 2;
+    const int64_t most = units * tiles <= kSlots ? tiles : tiles / 2;
+    int64_t want = ((n_seq > 2 ? 2 : 1) * kSlots + units - 1) / units;
+    if (want > most) want = most;
     if (want < 1) want = 1;
     p.split_tiles = (int)((tiles + want - 1) / want);
     p.n_splits = (tiles + p.split_tiles - 1) / p.split_tiles;
@@ -350,12 +348,12 @@ cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p,
     cudaError_t e = cudaErrorInvalidValue;
     if (plan.mma) {
         switch (a.k_type) {
-        case kF16: e = launch_mma_for_k<kF16>(stream, a, plan.sh, plan.mt); break;
-        case kQ4_0: e = launch_mma_for_k<kQ4_0>(stream, a, plan.sh, plan.mt); break;
-        case kQ4_1: e = launch_mma_for_k<kQ4_1>(stream, a, plan.sh, plan.mt); break;
-        case kQ5_0: e = launch_mma_for_k<kQ5_0>(stream, a, plan.sh, plan.mt); break;
-        case kQ5_1: e = launch_mma_for_k<kQ5_1>(stream, a, plan.sh, plan.mt); break;
-        case kQ8_0: e = launch_mma_for_k<kQ8_0>(stream, a, plan.sh, plan.mt); break;
+        case kF16: e = launch_mma_for_k<kF16>(stream, a, plan.sh); break;
+        case kQ4_0: e = launch_mma_for_k<kQ4_0>(stream, a, plan.sh); break;
+        case kQ4_1: e = launch_mma_for_k<kQ4_1>(stream, a, plan.sh); break;
+        case kQ5_0: e = launch_mma_for_k<kQ5_0>(stream, a, plan.sh); break;
+        case kQ5_1: e = launch_mma_for_k<kQ5_1>(stream, a, plan.sh); break;
+        case kQ8_0: e = launch_mma_for_k<kQ8_0>(stream, a, plan.sh); break;
         default: break;
         }
     } else {

@@ -6,10 +6,10 @@
 namespace cvattn {
 namespace tree {
 
-template <int KT, int VT, int MT>
+template <int KT, int VT>
 static cudaError_t run(cudaStream_t stream, const Args& a, const Shape& sh) {
-    const auto fn = tree_mma_kernel<KT, VT, MT>;
-    const int smem = Smem(KT, VT, MT, sh.hc, sh.wr, sh.stages).total;
+    const auto fn = tree_mma_kernel<KT, VT>;
+    const int smem = Smem(KT, VT, sh.stages).total;
     static std::atomic<int> allowed[64];  // dynamic shared memory granted so far, per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -19,25 +19,20 @@ static cudaError_t run(cudaStream_t stream, const Args& a, const Shape& sh) {
         if (e != cudaSuccess) return e;
         if (dev < 64) allowed[dev].store(smem, std::memory_order_relaxed);
     }
-    const dim3 grid((unsigned)a.n_splits, (unsigned)(a.Hkv / sh.hc * sh.row_groups), (unsigned)a.n_seq);
+    const dim3 grid((unsigned)a.n_splits, (unsigned)(a.Hkv * sh.row_groups), (unsigned)a.n_seq);
     fn<<<grid, kWarps * 32, smem, stream>>>(a, sh);
     return cudaGetLastError();
 }
 
-template <int KT, int VT>
-static cudaError_t run_mt(cudaStream_t stream, const Args& a, const Shape& sh, int mt) {
-    return mt == 1 ? run<KT, VT, 1>(stream, a, sh) : run<KT, VT, 2>(stream, a, sh);
-}
-
 template <>
-cudaError_t launch_mma_for_k<CVATTN_KT>(cudaStream_t stream, const Args& a, const Shape& sh, int mt) {
+cudaError_t launch_mma_for_k<CVATTN_KT>(cudaStream_t stream, const Args& a, const Shape& sh) {
     switch (a.v_type) {
-    case kF16: return run_mt<CVATTN_KT, kF16>(stream, a, sh, mt);
-    case kQ4_0: return run_mt<CVATTN_KT, kQ4_0>(stream, a, sh, mt);
-    case kQ4_1: return run_mt<CVATTN_KT, kQ4_1>(stream, a, sh, mt);
-    case kQ5_0: return run_mt<CVATTN_KT, kQ5_0>(stream, a, sh, mt);
-    case kQ5_1: return run_mt<CVATTN_KT, kQ5_1>(stream, a, sh, mt);
-    case kQ8_0: return run_mt<CVATTN_KT, kQ8_0>(stream, a, sh, mt);
+    case kF16: return run<CVATTN_KT, kF16>(stream, a, sh);
+    case kQ4_0: return run<CVATTN_KT, kQ4_0>(stream, a, sh);
+    case kQ4_1: return run<CVATTN_KT, kQ4_1>(stream, a, sh);
+    case kQ5_0: return run<CVATTN_KT, kQ5_0>(stream, a, sh);
+    case kQ5_1: return run<CVATTN_KT, kQ5_1>(stream, a, sh);
+    case kQ8_0: return run<CVATTN_KT, kQ8_0>(stream, a, sh);
     default: return cudaErrorInvalidValue;
     }
 }
