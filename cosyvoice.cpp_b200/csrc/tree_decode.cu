@@ -1,5 +1,6 @@
 // tree_decode.cu -- kernels and host side of cvattn_tree_decode.
 #include "tree_mma.cuh"
+#include "tree_tc.cuh"
 
 namespace cvattn {
 namespace tree {
@@ -232,17 +233,28 @@ static bool mma_type(int t) { return t != kF32; }
 // Which kernel, its shape, and how the keys are split.
 struct Plan {
     bool mma;
+    int tc_grid;   // > 0: the tcgen05 kernel on that many CTAs
     Shape sh;
     int tile, split_tiles, n_splits;
 };
 
-constexpr int kSlots = 296;  // two CTAs on each of 148 SMs
+constexpr int kSms = 148;
+constexpr int kSlots = 2 * kSms;  // two CTAs of tree_mma_kernel per SM
+constexpr int kTcMinRows = 32;    // up to here tree_mma_kernel, whose row tiles are 16 rows
 
 static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
     Plan p{};
     const int64_t rows = (int64_t)max_nodes * (n_q_heads / n_kv_heads);
     p.mma = mma_type(k_type) && mma_type(v_type);
     int64_t units;
+    const int64_t entries = (int64_t)n_seq * n_kv_heads * ((rows + kTcRows - 1) / kTcRows) *
+                            ((max_kv_len + kTcTile - 1) / kTcTile + (max_nodes + kTcTile - 1) / kTcTile);
+    if (p.mma && rows > kTcMinRows && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
+        p.tile = kTcTile;
+        p.tc_grid = (int)(entries < kSms ? entries : kSms);
+        p.n_splits = p.tc_grid / (int64_t)(n_seq * n_kv_heads) > 0 ? p.tc_grid / (n_seq * n_kv_heads) : 1;  // (for the combine)
+        return p;
+    }
     if (p.mma) {
         p.tile = kKeys;
         p.sh.row_groups = (int)((rows + 16 * kWarps - 1) / (16 * kWarps));
@@ -281,12 +293,52 @@ static cudaError_t run_combine(cudaStream_t stream, const Args& a) {
     return cudaLaunchKernelEx(&cfg, tree_combine_kernel<kLanes>, a);
 }
 
+template <int kLanes>
+static cudaError_t run_tc_combine(cudaStream_t stream, const TcArgs& ta) {
+    const int rows = ta.a.max_nodes * ta.a.G;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)ta.a.Hkv, (unsigned)ta.a.n_seq);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tree_tc_combine_kernel<kLanes>, ta);
+}
+
+static cudaError_t launch_tc(cudaStream_t stream, const Args& a, const Plan& plan, void* workspace) {
+    TcArgs ta{};
+    ta.a = a;
+    ta.grid = plan.tc_grid;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    ta.ws_pref = reinterpret_cast<int32_t*>(ws);
+    ws += align256((size_t)(a.n_seq + 1) * 4);
+    ta.ws_o = reinterpret_cast<float*>(ws);
+    ta.ws_ml = ta.ws_o + (size_t)2 * ta.grid * kTcRows * kD;
+    cudaError_t e = cudaErrorInvalidValue;
+    switch (a.k_type) {
+    case kF16: e = launch_tc_for_k<kF16>(stream, ta); break;
+    case kQ4_0: e = launch_tc_for_k<kQ4_0>(stream, ta); break;
+    case kQ4_1: e = launch_tc_for_k<kQ4_1>(stream, ta); break;
+    case kQ5_0: e = launch_tc_for_k<kQ5_0>(stream, ta); break;
+    case kQ5_1: e = launch_tc_for_k<kQ5_1>(stream, ta); break;
+    case kQ8_0: e = launch_tc_for_k<kQ8_0>(stream, ta); break;
+    default: break;
+    }
+    if (e != cudaSuccess) return e;
+    return plan.n_splits > 16 ? run_tc_combine<16>(stream, ta) : plan.n_splits > 4 ? run_tc_combine<4>(stream, ta)
+                                                                                   : run_tc_combine<1>(stream, ta);
+}
+
 static cudaError_t launch_combine(cudaStream_t stream, const Args& a) {
     return a.n_splits > 32 ? run_combine<16>(stream, a) : a.n_splits > 8 ? run_combine<4>(stream, a) : run_combine<1>(stream, a);
 }
 
 size_t workspace_bytes(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
     const Plan p = plan_of(k_type, v_type, n_seq, max_kv_len, max_nodes, n_q_heads, n_kv_heads);
+    if (p.tc_grid) return align256((size_t)(n_seq + 1) * 4) + (size_t)2 * p.tc_grid * kTcRows * (kD + 2) * 4;
     if (p.n_splits == 1) return 0;
     const size_t rows = (size_t)n_seq * p.n_splits * max_nodes * n_q_heads;
     return align256(rows * 2 * 4) + rows * kD * 4;
@@ -340,6 +392,7 @@ cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p,
     a.tile = plan.tile;
     a.split_tiles = plan.split_tiles;
     a.n_splits = plan.n_splits;
+    if (plan.tc_grid) return launch_tc(stream, a, plan, p.workspace);
     if (plan.n_splits > 1) {
         const size_t rows = (size_t)a.n_seq * plan.n_splits * a.max_nodes * a.Hq;
         a.ws_ml = static_cast<float*>(p.workspace);

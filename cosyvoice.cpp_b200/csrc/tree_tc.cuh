@@ -1,0 +1,763 @@
+// tree_tc.cuh -- tree attention on the 5th-generation tensor cores (tcgen05), for
+// f16 and block-quantized caches and more than 32 rows per KV head.
+//
+// Work is cut evenly: the key tiles (128 keys) of all units (sequence, KV head,
+// tile of 128 rows) form one list, and CTA c of G takes the entries [c N / G,
+// (c + 1) N / G).  A run is the part of one unit that a CTA has; a whole unit is
+// written out directly, parts go to the workspace and tree_tc_combine_kernel joins
+// them.  (Ragged sequences and few long ones fill the SMs alike.)
+//   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the
+//                   CTA's tiles 2 k + g, so one computes while the other's MMAs run
+//   warps 8-11      producer: raw rows by cp.async, then f16 tiles (128B swizzle);
+//                   f16 caches are copied straight into the tiles
+//   warps 12, 13    MMA issuers of the two groups
+// Precision: products of split numbers.  x = hi + lo in f16, S = Qh Kh + Ql Kh
+// (+ Qh Kl), O = Ph Vh + Pl Vh (+ Ph Vl); the dropped low x low term is 2^-22 of the
+// largest.  Q is scaled per row, K and V per tile, by powers of two so that hi and
+// lo keep their bits; P is kept 2^7 large.  A scale d times integer quants splits in
+// two half-precision instructions: hi = RN(d q), lo = d q - hi, exact.  An f16 cache
+// is its own hi and has no lo.
+// The output of a tile is a fresh accumulator, added in f32 to the row's registers:
+// adds inside the tensor cores truncate, and over a long cache that would show.
+// TMEM per group: S of the tile (128 columns), overwritten 32 keys at a time by
+// that chunk's P (16 columns hi, 16 lo), and the tile's O (64 columns).
+#pragma once
+
+#include "flash_pipe.cuh"
+#include "tree_mma.cuh"
+
+namespace cvattn {
+namespace tree {
+
+constexpr int kTcTile = 128;
+constexpr int kTcRows = 128;
+constexpr int kTcThreads = 14 * 32;
+constexpr int kTcMaxSeq = 1024;       // prefix table in shared memory
+constexpr int kTcExps = 8;            // tiles whose scales may be in flight
+constexpr int kTcTileBytes = kTcTile * kD * 2;
+constexpr float kTcOffs = 7.0f;
+
+struct TcArgs {
+    Args a;
+    int grid;                         // CTAs that share the list
+    float* ws_o;                      // [2 * grid][128][64]
+    float* ws_ml;                     // [2 * grid][128][2]
+    int32_t* ws_pref;                 // [n_seq + 1], written by CTA 0 for the combine
+};
+
+struct TcBars {
+    uint64_t kv_full[4], k_empty[4], v_empty[4];
+    uint64_t q_full;
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint32_t tmem_base;
+    int err;
+    uint32_t maxk[2], maxv[2];        // largest |scale| of a tile, by tile parity
+    float2 exps[kTcExps];             // 2^-e of K and V of tile i at i % kTcExps
+    uint32_t bad[kTcExps][4];         // draft keys whose V is not finite
+};
+
+template <int KT, int VT>
+struct TcShape {
+    static constexpr int NK = KT == kF16 ? 1 : 2, NV = VT == kF16 ? 1 : 2;  // pieces of an operand
+    static constexpr int kStages = NK + NV == 2 ? 4 : NK + NV == 3 ? 3 : 2;
+    static constexpr int kStage = (NK + NV) * kTcTileBytes;
+    static constexpr int rawK = NK == 1 ? 0 : kTcTile * raw_stride(KT), rawV = NV == 1 ? 0 : kTcTile * raw_stride(VT);
+    static constexpr int kQ = 0;                       // Q hi, Q lo; then the groups' halves at a run's end
+    static constexpr int kTiles = 2 * kTcTileBytes;
+    static constexpr int kRaw = kTiles + kStages * kStage;
+    static constexpr int kMl = kRaw + 2 * (rawK + rawV);
+    static constexpr int kBars = kMl + 2 * kTcRows * 8;
+    static constexpr int kPref = kBars + (int)((sizeof(TcBars) + 15) / 16 * 16);
+    static constexpr int kBytes = kPref + (kTcMaxSeq + 1) * 4;
+    static_assert(kBytes <= 227 * 1024, "one CTA per SM");
+};
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long ra = *reinterpret_cast<unsigned long long*>(&a), rb = *reinterpret_cast<unsigned long long*>(&b), rd;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+    return *reinterpret_cast<float2*>(&rd);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long ra = *reinterpret_cast<unsigned long long*>(&a), rb = *reinterpret_cast<unsigned long long*>(&b), rd;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+    return *reinterpret_cast<float2*>(&rd);
+}
+
+// Units of sequence s: row tiles times KV heads, row tile major.
+__device__ __forceinline__ int units_of(const Args& a, const Lens& x) { return (x.n * a.G + kTcRows - 1) / kTcRows * a.Hkv; }
+
+struct Run {
+    int s, kvh, rt, t0, t1, T;   // tiles [t0, t1) of T
+    Lens x;
+};
+// The run that starts at list entry i and ends before hi.
+__device__ __forceinline__ Run run_at(const Args& a, const int32_t* pref, int i, int hi) {
+    int lo = 0, up = a.n_seq;  // last s with pref[s] <= i: its list is not empty
+    while (up - lo > 1) {
+        const int mid = (lo + up) >> 1;
+        if (pref[mid] <= i) lo = mid;
+        else up = mid;
+    }
+    Run r;
+    r.s = lo;
+    r.x = lens_of(a, lo, false);
+    r.T = r.x.tiles;
+    const int u = (i - pref[lo]) / r.T;
+    r.t0 = (i - pref[lo]) - u * r.T;
+    r.t1 = min(r.T, r.t0 + (hi - i));
+    r.kvh = u % a.Hkv;
+    r.rt = u / a.Hkv;
+    return r;
+}
+
+__device__ __forceinline__ int tc_cut(int c, int n, int g) { return (int)((long long)c * n / g); }
+__device__ __forceinline__ int tc_owner(int i, int n, int g) { return (int)(((long long)(i + 1) * g - 1) / n); }
+
+// hi and lo of 32 values of one key into rows of two tiles; w holds exact integers (convert_group), d and m the block's
+// scale and min times the tile's power of two.
+template <int T>
+__device__ __forceinline__ void split_block(uint8_t* hi_tile, uint8_t* lo_tile, int key, int blk, const uint32_t (&w)[16], float d, float m) {
+    uint32_t h[16], l[16];
+    if constexpr (!BlockTraits<T>::HAS_MIN) {
+        const __half2 d2 = __float2half2_rn(d);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const __half2 q = *reinterpret_cast<const __half2*>(&w[i]);
+            const __half2 p = __hmul2_rn(d2, q);
+            const __half2 e = __hfma2(d2, q, __hneg2(p));
+            h[i] = *reinterpret_cast<const uint32_t*>(&p);
+            l[i] = *reinterpret_cast<const uint32_t*>(&e);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            split2(fmaf(q.x, d, m), fmaf(q.y, d, m), h[i], l[i]);
+        }
+    }
+    store_block(hi_tile, key, blk, h);
+    store_block(lo_tile, key, blk, l);
+}
+
+// Power of two that brings the largest scale (or min) of a tile to [2^6, 2^7): quants times it stay below 2^15.
+__device__ __forceinline__ int tile_exp(float mx) {
+    if (!(mx > 0.0f)) return 0;
+    const int e = 6 - dstream::ilog2f(mx);
+    return e > 100 ? 100 : (e < -100 ? -100 : e);
+}
+
+template <int KT, int VT>
+__global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ TcArgs ta) {
+    using Sh = TcShape<KT, VT>;
+    constexpr int NK = Sh::NK, NV = Sh::NV, kSt = Sh::kStages;
+    constexpr int sliceK = 2 * group_bytes(KT), sliceV = 2 * group_bytes(VT);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const Args& a = ta.a;
+    TcBars* B = reinterpret_cast<TcBars*>(smem + Sh::kBars);
+    int32_t* pref = reinterpret_cast<int32_t*>(smem + Sh::kPref);
+    if (smem_addr(smem) & 1023u) {
+        if (threadIdx.x == 0) record_status(a.status, kStatusTimeout);
+        return;
+    }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < kSt; ++i) {
+            mbar_init(&B->kv_full[i], 128);
+            mbar_init(&B->k_empty[i], 1);
+            mbar_init(&B->v_empty[i], 1);
+        }
+        mbar_init(&B->q_full, 256);
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&B->s_full[g], 1);
+            mbar_init(&B->p_full[g], 128);
+            mbar_init(&B->o_full[g], 1);
+            B->maxk[g] = B->maxv[g] = 0u;
+        }
+        B->err = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tc::tmem_alloc(&B->tmem_base, 512);
+        tc::tmem_relinquish();
+    }
+    if (warp == 1) {  // list entries before each sequence
+        int carry = 0;
+        for (int base = 0; base < a.n_seq; base += 32) {
+            const int s = base + lane;
+            int n = 0;
+            if (s < a.n_seq) {
+                const Lens x = lens_of(a, s, blockIdx.x == 0);
+                n = x.tiles * units_of(a, x);
+            }
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (s < a.n_seq) {
+                pref[s] = carry + incl - n;
+                if (blockIdx.x == 0) ta.ws_pref[s] = carry + incl - n;
+            }
+            carry += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) {
+            pref[a.n_seq] = carry;
+            if (blockIdx.x == 0) ta.ws_pref[a.n_seq] = carry;
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    griddep_launch_dependents();
+    const uint32_t tmem = B->tmem_base;
+    const int total = pref[a.n_seq];
+    const int lo = tc_cut(blockIdx.x, total, ta.grid), hi = tc_cut(blockIdx.x + 1, total, ta.grid);
+
+    if (warp < 8) {
+        // ------------------------------------------------------ softmax group g
+        const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        const uint32_t sp = tmem + lane_base + g * 128, ot = tmem + lane_base + 256 + g * 64;
+        uint8_t* qhi = smem + Sh::kQ;
+        uint8_t* qlo = qhi + kTcTileBytes;
+        float* xch = reinterpret_cast<float*>(smem + Sh::kQ);  // [group][row][32 floats of the other group's half]
+        float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl);
+        uint32_t k = 0;  // tiles of this group so far
+        bool ok = true;
+        for (int i = lo; i < hi;) {
+            const Run r = run_at(a, pref, i, hi);
+            const int rr = r.rt * kTcRows + row, rows = r.x.n * a.G;
+            const bool real = rr < rows;
+            const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
+            const int node = rr / a.G, h = r.kvh * a.G + rr % a.G;
+            // Q: each group reads the row and writes its half of the dims
+            float rs;
+            {
+                const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)node * a.q_nb_node + h * kD);
+                float4 v[8];
+                float am = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float4 o = real ? q[8 * (g ^ 1) + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[c] = real ? q[8 * g + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    am = fmaxf(am, fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w))));
+                    am = fmaxf(am, fmaxf(fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w))));
+                }
+                const int ex = dtc::norm_exp(am);
+                const float sc = pow2f(ex);
+                rs = pow2f(-ex) * a.scale_log2;
+                // nothing reads the last run's Q, or its exchanged halves, any more
+                if (i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t wh[4], wl[4];
+                    split2(v[2 * c].x * sc, v[2 * c].y * sc, wh[0], wl[0]);
+                    split2(v[2 * c].z * sc, v[2 * c].w * sc, wh[1], wl[1]);
+                    split2(v[2 * c + 1].x * sc, v[2 * c + 1].y * sc, wh[2], wl[2]);
+                    split2(v[2 * c + 1].z * sc, v[2 * c + 1].w * sc, wh[3], wl[3]);
+                    const uint32_t at = tc::sw128_offset(row, 4 * g + c);
+                    *reinterpret_cast<uint4*>(qhi + at) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+                    *reinterpret_cast<uint4*>(qlo + at) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&B->q_full);
+            }
+            float2 O[32];
+#pragma unroll
+            for (int d = 0; d < 32; ++d) O[d] = make_float2(0.f, 0.f);
+            float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 0.0f;
+            bool pending = false;  // a tile's output still to be added, times vs_last
+            auto add_output = [&]() {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t ov[32];
+                    tc::tmem_ld32(ot + 32 * c, ov);
+                    tc::tmem_ld_wait();
+                    const float2 f = make_float2(vs_last, vs_last);
+#pragma unroll
+                    for (int d = 0; d < 16; ++d)
+                        O[16 * c + d] = ffma2(make_float2(__uint_as_float(ov[2 * d]), __uint_as_float(ov[2 * d + 1])), f, O[16 * c + d]);
+                }
+            };
+            const int first = i, last = i + (r.t1 - r.t0);
+            for (int j = first + ((first ^ g ^ lo) & 1); ok && j < last; j += 2) {  // the CTA's tile j - lo of parity g
+                const int tile = r.t0 + (j - first);
+                const bool draft = tile >= r.x.cache_tiles;
+                const int p0 = (draft ? tile - r.x.cache_tiles : tile) * kTcTile;
+                const int count = min(kTcTile, (draft ? r.x.n : r.x.L) - p0);
+                ok = fp::wait_or_err(&B->s_full[g], k & 1, &B->err, a.status, 31);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ++k;
+                tc::fence_after();
+                if (warp_real) {
+                    if (pending) add_output();
+                    const float2 ex = B->exps[(j - lo) % kTcExps];
+                    const float rst = rs * ex.x;
+                    const bool masked = draft || count < kTcTile;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t sv[32];
+                        tc::tmem_ld32(sp + 32 * c, sv);
+                        tc::tmem_ld_wait();
+                        float2 x[16];
+                        {
+                            const float2 f = make_float2(rst, rst), b = make_float2(-base, -base);
+#pragma unroll
+                            for (int d = 0; d < 16; ++d)
+                                x[d] = ffma2(make_float2(__uint_as_float(sv[2 * d]), __uint_as_float(sv[2 * d + 1])), f, b);
+                        }
+                        if (masked) {
+                            const int left = count - 32 * c;
+                            uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                            if (draft && bits && real) {
+                                const int j0 = p0 + 32 * c;
+                                if (a.mask) bits &= a.mask[(int64_t)r.s * a.mask_nb_seq + (int64_t)node * a.mask_words + (j0 >> 5)];
+                                else if (node < j0 + 31) bits &= node < j0 ? 0u : (2u << (node - j0)) - 1u;
+                            }
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) {
+                                if (!((bits >> (2 * d)) & 1u)) x[d].x = -INFINITY;
+                                if (!((bits >> (2 * d + 1)) & 1u)) x[d].y = -INFINITY;
+                            }
+                        }
+                        float mx = fmaxf(x[0].x, x[0].y);
+#pragma unroll
+                        for (int d = 1; d < 16; ++d) mx = fmaxf(mx, fmaxf(x[d].x, x[d].y));
+                        if (__any_sync(0xffffffffu, mx > thr)) {
+                            float f = 1.0f, up = 0.0f;
+                            if (mx > thr) {
+                                up = mx - kTcOffs;
+                                f = thr == -INFINITY ? 0.0f : fast_exp2(-up);
+                                base += up;
+                                thr = kLazy + kTcOffs;
+                                l *= f;
+                            }
+                            const float2 f2 = make_float2(f, f), u2 = make_float2(-up, -up);
+#pragma unroll
+                            for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) x[d] = add2(x[d], u2);
+                            if (c) tc::tmem_st_wait();
+#pragma unroll 1
+                            for (int e = 0; e < c; ++e) {  // this tile's P so far
+                                uint32_t pv[32];
+                                tc::tmem_ld32(sp + 32 * e, pv);
+                                tc::tmem_ld_wait();
+#pragma unroll
+                                for (int d = 0; d < 16; ++d) {
+                                    const float2 ph = __half22float2(*reinterpret_cast<const __half2*>(&pv[d]));
+                                    const float2 pl = __half22float2(*reinterpret_cast<const __half2*>(&pv[16 + d]));
+                                    split2((ph.x + pl.x) * f, (ph.y + pl.y) * f, pv[d], pv[16 + d]);
+                                }
+                                tc::tmem_st32(sp + 32 * e, pv);
+                            }
+                        }
+                        float2 ls = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int d = 0; d < 16; ++d) {
+                            x[d].x = fast_exp2(x[d].x);
+                            x[d].y = fast_exp2(x[d].y);
+                            ls = add2(ls, x[d]);
+                        }
+                        l += ls.x + ls.y;
+                        if (draft) {
+                            // keys whose V is not finite have zeros in the tile; rows that see one add it here
+                            uint32_t bad = B->bad[(j - lo) % kTcExps][c];
+                            while (bad) {
+                                const int b = __ffs(bad) - 1;
+                                bad &= bad - 1;
+                                float pb = 0.0f;
+#pragma unroll
+                                for (int d = 0; d < 16; ++d) {
+                                    if (2 * d == b) pb = x[d].x;
+                                    if (2 * d + 1 == b) pb = x[d].y;
+                                }
+                                if (pb == 0.0f) continue;
+                                const uint8_t* vr = a.vd + (int64_t)r.s * a.vd_nb2 + (int64_t)(p0 + 32 * c + b) * a.vd_nb1 + r.kvh * sliceV;
+#pragma unroll
+                                for (int d = 0; d < 32; ++d) {
+                                    const uint8_t* vg = vr + (d >> 4) * group_bytes(VT);
+                                    O[d].x = fmaf(pb, dequant_elem<VT>(vg, (2 * d) & 31), O[d].x);
+                                    O[d].y = fmaf(pb, dequant_elem<VT>(vg, (2 * d + 1) & 31), O[d].y);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int d = 0; d < 16; ++d) {
+                            const float2 t = make_float2(__uint_as_float(__float_as_uint(x[d].x) & 0xFFFFE000u),
+                                                         __uint_as_float(__float_as_uint(x[d].y) & 0xFFFFE000u));
+                            const float2 e = add2(x[d], make_float2(-t.x, -t.y));
+                            sv[d] = tc::pack_f16x2(t.x, t.y);
+                            sv[16 + d] = tc::pack_f16x2(e.x, e.y);
+                        }
+                        tc::tmem_st32(sp + 32 * c, sv);
+                    }
+                    vs_last = ex.y;
+                    pending = true;
+                    tc::tmem_st_wait();
+                }
+                tc::fence_before();
+                mbar_arrive(&B->p_full[g]);
+            }
+            // the last tile's output (o_full counts every tile of this group)
+            if (ok && pending) {
+                ok = fp::wait_or_err(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
+                ok = __all_sync(0xffffffffu, ok);
+                tc::fence_after();
+                if (ok) add_output();
+            }
+            tc::fence_before();
+            if (!fp::prod_bar_and(2, 256, ok)) break;  // every MMA of the run is done; all threads leave together
+            // each group finishes 32 of the 64 dims: the other half goes to the other group
+            {
+                float4* mine = reinterpret_cast<float4*>(xch + (g * kTcRows + row) * 32);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float2 u = g ? O[2 * c] : O[16 + 2 * c], v = g ? O[2 * c + 1] : O[16 + 2 * c + 1];
+                    mine[c ^ (row & 7)] = make_float4(u.x, u.y, v.x, v.y);
+                }
+                mls[g * kTcRows + row] = make_float2(thr == -INFINITY && l == 0.0f ? -INFINITY : base, l);
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            {
+                const float2 m0 = mls[g * kTcRows + row], m1 = mls[(g ^ 1) * kTcRows + row];
+                const float M = fmaxf(m0.x, m1.x);
+                const float f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - M), f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - M);
+                const float sum = (f0 == 0.0f ? 0.0f : f0 * m0.y) + (f1 == 0.0f ? 0.0f : f1 * m1.y);
+                const bool whole = r.t1 - r.t0 == r.T, seen = M != -INFINITY;
+                const float inv = !whole ? 1.0f : seen ? 1.0f / sum : 0.0f;
+                const int slot = 2 * blockIdx.x + (first == lo ? 0 : 1);
+                float4* dst = whole ? reinterpret_cast<float4*>(a.out + (int64_t)r.s * a.out_nb_seq + (int64_t)node * a.out_nb_node + h * kD + 32 * g)
+                                    : reinterpret_cast<float4*>(ta.ws_o + ((int64_t)slot * kTcRows + row) * kD + 32 * g);
+                const float4* other = reinterpret_cast<const float4*>(xch + ((g ^ 1) * kTcRows + row) * 32);
+                if (real) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float2 u = g ? O[16 + 2 * c] : O[2 * c], v = g ? O[16 + 2 * c + 1] : O[2 * c + 1];
+                        const float4 w = other[c ^ (row & 7)];
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (f0 != 0.0f) o = make_float4(f0 * u.x, f0 * u.y, f0 * v.x, f0 * v.y);
+                        if (f1 != 0.0f) o = make_float4(fmaf(f1, w.x, o.x), fmaf(f1, w.y, o.y), fmaf(f1, w.z, o.z), fmaf(f1, w.w, o.w));
+                        dst[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                    }
+                    if (g == 0) {
+                        if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + ((int64_t)slot * kTcRows + row) * 2) = make_float2(M, sum);
+                        else if (a.lse)
+                            a.lse[((int64_t)r.s * a.max_nodes + node) * a.Hq + h] = seen ? (M + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+                    }
+                }
+            }
+            i = last;
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------------ producer: thread = key
+        const int key = tid - 256;
+        auto tile_of = [&](const Run& r, int tile, bool& draft, int& p0, int& count) {
+            draft = tile >= r.x.cache_tiles;
+            p0 = (draft ? tile - r.x.cache_tiles : tile) * kTcTile;
+            count = min(kTcTile, (draft ? r.x.n : r.x.L) - p0);
+        };
+        // keys [0, count) of a tile into shared memory, zeros up to 128
+        auto copy = [&](auto type_tag, bool raw, uint8_t* dst, const uint8_t* src, int64_t nb1, int count) {
+            constexpr int T = decltype(type_tag)::value;
+            const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)nb1;
+            const int unit = T == kF16 && (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 2;
+            const int w = 2 * group_bytes(T) / unit, per = 128 / w;
+            const int k0 = key / w, col = (key - k0 * w) * unit;
+            if (k0 >= per) return;
+            for (int kk = k0; kk < kTcTile; kk += per) {
+                const bool there = kk < count;
+                const uint8_t* from = src + (int64_t)(there ? kk : 0) * nb1 + col;
+                uint8_t* to = raw ? dst + kk * raw_stride(T) + col : dst + kk * 128 + (col ^ ((kk & 7) << 4));
+                if (unit == 16) cp_async16(to, from, there);
+                else if (unit == 4) cp_async4(to, from, there);
+                else *reinterpret_cast<uint16_t*>(to) = there ? *reinterpret_cast<const uint16_t*>(from) : (uint16_t)0;
+            }
+        };
+        // cursors: the tile whose copies start (n_issue) and the tile that is finished (n)
+        Run ri{}, rc{};
+        int ii = lo, ic = lo;            // list entries
+        int fi = lo, fc = lo;            // first entries of the cursors' runs
+        if (lo < hi) ri = rc = run_at(a, pref, lo, hi);
+        bool ok = true;
+        auto issue = [&](int n) {        // copies of the CTA's tile n (list entry ii)
+            if (ii < hi) {
+                if (ii - fi >= ri.t1 - ri.t0) {
+                    fi = ii;
+                    ri = run_at(a, pref, ii, hi);
+                }
+                bool draft;
+                int p0, count;
+                tile_of(ri, ri.t0 + (ii - fi), draft, p0, count);
+                const uint8_t* ks = (draft ? a.kd + (int64_t)ri.s * a.kd_nb2 : seq_base(a.k_seq_ptrs, a.k, a.k_nb2, ri.s)) + ri.kvh * sliceK;
+                const uint8_t* vs = (draft ? a.vd + (int64_t)ri.s * a.vd_nb2 : seq_base(a.v_seq_ptrs, a.v, a.v_nb2, ri.s)) + ri.kvh * sliceV;
+                const int64_t nk = draft ? a.kd_nb1 : a.k_nb1, nv = draft ? a.vd_nb1 : a.v_nb1;
+                const int st = n % kSt;
+                uint8_t* tiles = smem + Sh::kTiles + st * Sh::kStage;
+                uint8_t* raw = smem + Sh::kRaw + (n & 1) * (Sh::rawK + Sh::rawV);
+                const uint32_t use = n / kSt;
+                if constexpr (NK == 1)
+                    if (use > 0) ok = ok && fp::wait_or_err(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 33);
+                if constexpr (NV == 1)
+                    if (use > 0) ok = ok && fp::wait_or_err(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 34);
+                if (ok) {
+                    copy(std::integral_constant<int, KT>{}, NK == 2, NK == 2 ? raw : tiles, ks + (int64_t)p0 * nk, nk, count);
+                    copy(std::integral_constant<int, VT>{}, NV == 2, NV == 2 ? raw + Sh::rawK : tiles + NK * kTcTileBytes, vs + (int64_t)p0 * nv, nv, count);
+                }
+                ++ii;
+            }
+            cp_async_commit();
+        };
+        constexpr int kAhead = NK + NV == 2 ? kSt - 2 : 1;  // tiles whose copies run ahead of the finished one
+        for (int n = 0; n < kAhead; ++n) issue(n);
+        for (int n = 0; ic < hi; ++n, ++ic) {
+            cp_async_wait<kAhead - 1>();
+            // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
+            if (!fp::prod_bar_and(4, 128, ok)) break;
+            issue(n + kAhead);
+            if (ic - fc >= rc.t1 - rc.t0) {
+                fc = ic;
+                rc = run_at(a, pref, ic, hi);
+            }
+            bool draft;
+            int p0, count;
+            tile_of(rc, rc.t0 + (ic - fc), draft, p0, count);
+            const int st = n % kSt;
+            const uint32_t use = n / kSt;
+            uint8_t* tiles = smem + Sh::kTiles + st * Sh::kStage;
+            const uint8_t* rawk = smem + Sh::kRaw + (n & 1) * (Sh::rawK + Sh::rawV);
+            const uint8_t* rawv = rawk + Sh::rawK;
+            bool bad = false;
+            float fk = 1.0f, fv = 1.0f;
+            if constexpr (NK + NV > 2) {
+                // the tile's largest scales
+                uint32_t mk = 0, mv = 0;
+                auto scale_max = [&](auto type_tag, const uint8_t* rowp, bool& special) {
+                    constexpr int T = decltype(type_tag)::value;
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const uint8_t* gb = rowp + b * group_bytes(T);
+                        float d = fabsf(h2f(*reinterpret_cast<const uint16_t*>(gb)));
+                        if constexpr (BlockTraits<T>::HAS_MIN) {
+                            // |d q + m| <= 16 d + |m + 16 d|: in units of 127 quants of a scale
+                            const float mm = h2f(*reinterpret_cast<const uint16_t*>(gb + BlockTraits<T>::OFF_M));
+                            special |= !isfinite(mm);
+                            d = (32.0f * d + fabsf(mm)) * (1.0f / 64.0f);
+                        }
+                        special |= !isfinite(d);
+                        if (isfinite(d)) m = max(m, __float_as_uint(d));
+                    }
+                    return __reduce_max_sync(0xffffffffu, m);
+                };
+                bool kbad = false;
+                if constexpr (NK == 2) mk = scale_max(std::integral_constant<int, KT>{}, rawk + key * raw_stride(KT), kbad);
+                if constexpr (NV == 2) mv = scale_max(std::integral_constant<int, VT>{}, rawv + key * raw_stride(VT), bad);
+                if (lane == 0) {
+                    if (mk) atomicMax(&B->maxk[n & 1], mk);
+                    if (mv) atomicMax(&B->maxv[n & 1], mv);
+                }
+                asm volatile("bar.sync 5, 128;" ::: "memory");
+                const int ek = tile_exp(__uint_as_float(B->maxk[n & 1])), ev = tile_exp(__uint_as_float(B->maxv[n & 1]));
+                fk = pow2f(ek);
+                fv = pow2f(ev);
+                if (key == 0) {
+                    B->exps[n % kTcExps] = make_float2(NK == 2 ? pow2f(-ek) : 1.0f, NV == 2 ? pow2f(-ev) : 1.0f);
+                    B->maxk[(n + 1) & 1] = B->maxv[(n + 1) & 1] = 0u;
+                }
+            } else if (key == 0) {
+                B->exps[n % kTcExps] = make_float2(1.0f, 1.0f);
+            }
+            if constexpr (NK == 2) {
+                if (use > 0) ok = ok && fp::wait_or_err(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 35);
+                if (ok) {
+#pragma unroll 1
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t w[16];
+                        float d, m;
+                        dtc::convert_group<KT>(rawk + key * raw_stride(KT) + b * group_bytes(KT), w, d, m);
+                        split_block<KT>(tiles, tiles + kTcTileBytes, key, b, w, d * fk, m * fk);
+                    }
+                }
+            }
+            if constexpr (NV == 1) {
+                if (draft) {  // this thread's key
+                    uint4* p = reinterpret_cast<uint4*>(tiles + NK * kTcTileBytes + key * 128);
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 w = p[c];
+                        bad |= f16x2_special(w.x) || f16x2_special(w.y) || f16x2_special(w.z) || f16x2_special(w.w);
+                    }
+                    if (bad)
+                        for (int c = 0; c < 8; ++c) p[c] = make_uint4(0u, 0u, 0u, 0u);
+                }
+            } else {
+                if (use > 0) ok = ok && fp::wait_or_err(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 36);
+                if (ok) {
+                    const bool drop = draft && bad;
+#pragma unroll 1
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t w[16];
+                        float d, m;
+                        dtc::convert_group<VT>(rawv + key * raw_stride(VT) + b * group_bytes(VT), w, d, m);
+                        split_block<VT>(tiles + NK * kTcTileBytes, tiles + (NK + 1) * kTcTileBytes, key, b, w, drop ? 0.0f : d * fv,
+                                        drop ? 0.0f : m * fv);
+                    }
+                }
+            }
+            if (draft) {
+                const uint32_t vote = __ballot_sync(0xffffffffu, bad);
+                if (lane == 0) B->bad[n % kTcExps][key >> 5] = vote;
+            }
+            if (ok) {
+                fence_proxy_async_smem();
+                mbar_arrive(&B->kv_full[st]);
+            }
+        }
+        cp_async_wait<0>();
+    } else if (lane == 0) {
+        // ------------------------------------------------------ MMA issuer of group g
+        const int g = warp - 12;
+        const uint32_t idesc_s = tc::idesc_f16_f32(128, kTcTile, false), idesc_o = tc::idesc_f16_f32(128, 64, true);
+        const uint32_t sp = tmem + g * 128, ot = tmem + 256 + g * 64;
+        const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
+        const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
+        uint32_t k = 0, n_run = 0;
+        bool ok = true;
+        for (int i = lo; ok && i < hi; ++n_run) {
+            const Run r = run_at(a, pref, i, hi);
+            const int first = i, last = i + (r.t1 - r.t0);
+            ok = fp::wait_or_err(&B->q_full, n_run & 1, &B->err, a.status, 37);
+            for (int j = first + ((first ^ g ^ lo) & 1); ok && j < last; j += 2, ++k) {
+                const int n = j - lo, st = n % kSt;
+                const uint32_t tiles = smem_addr(smem + Sh::kTiles + st * Sh::kStage);
+                ok = fp::wait_or_err(&B->kv_full[st], (n / kSt) & 1, &B->err, a.status, 38);
+                if (!ok) break;
+                tc::fence_after();
+                const uint64_t dk = tc::sdesc_sw128(tiles, 16, 1024);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc_s, kk > 0 ? 1u : 0u);
+                    tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc_s, 1u);
+                    if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc_s, 1u);
+                }
+                tc::mma_commit(&B->s_full[g]);
+                tc::mma_commit(&B->k_empty[st]);
+                ok = fp::wait_or_err(&B->p_full[g], k & 1, &B->err, a.status, 39);
+                if (!ok) break;
+                tc::fence_after();
+                const uint64_t dv = tc::sdesc_sw128(tiles + NK * kTcTileBytes, 16, 1024);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk) {
+                    const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
+                    tc::mma_ts(ot, ph, dv + kk * 128, idesc_o, kk > 0 ? 1u : 0u);
+                    tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc_o, 1u);
+                    if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc_o, 1u);
+                }
+                tc::mma_commit(&B->o_full[g]);
+                tc::mma_commit(&B->v_empty[st]);
+            }
+            i = last;
+        }
+    }
+
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc::fence_after();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
+// Join of the parts of units that several CTAs shared, and the rows that no unit
+// holds (a sequence without keys, rows past the last node).  16 threads per row
+// (4 dims each) follow every kLanes-th part.
+template <int kLanes>
+__global__ void __launch_bounds__(256) tree_tc_combine_kernel(const __grid_constant__ TcArgs ta) {
+    constexpr int kPer = 16 / kLanes;
+    __shared__ float4 so[16][16];
+    __shared__ float2 sml[16];
+    const Args& a = ta.a;
+    griddep_wait();
+    const int unit = threadIdx.x >> 4, c = threadIdx.x & 15, lane = unit % kLanes;
+    const int all_rows = a.max_nodes * a.G;
+    const int r = blockIdx.x * kPer + unit / kLanes, kvh = blockIdx.y, s = blockIdx.z;
+    const Lens x = lens_of(a, s, false);
+    const int node = r / a.G, h = kvh * a.G + r % a.G, rt = r / kTcRows;
+    const int n = ta.ws_pref[a.n_seq];
+    int b0 = 0, c0 = 0, c1 = -1;
+    if (r < x.n * a.G && x.tiles > 0) {
+        b0 = ta.ws_pref[s] + (rt * a.Hkv + kvh) * x.tiles;
+        c0 = tc_owner(b0, n, ta.grid);
+        c1 = tc_owner(b0 + x.tiles - 1, n, ta.grid);
+        if (kLanes == 1 && c0 == c1) return;  // written whole
+    }
+    const bool done = c0 == c1;
+    float M = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = c0 + lane; k0 <= c1 && !done; k0 += 4 * kLanes) {
+        float2 ml[4];
+        float4 v[4];
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int cta = k0 + u * kLanes;
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (cta <= c1) {
+                const int64_t slot = 2 * cta + (tc_cut(cta, n, ta.grid) >= b0 ? 0 : 1);
+                const int64_t at = slot * kTcRows + r % kTcRows;
+                if (tc_cut(cta + 1, n, ta.grid) > tc_cut(cta, n, ta.grid)) {
+                    ml[u] = *reinterpret_cast<const float2*>(ta.ws_ml + at * 2);
+                    v[u] = *reinterpret_cast<const float4*>(ta.ws_o + at * kD + c * 4);
+                }
+            }
+            top = fmaxf(top, ml[u].x);
+        }
+        if (top == -INFINITY) continue;
+        const float f0 = exp2f(M - top);
+        M = top;
+        l *= f0;
+        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (ml[u].x == -INFINITY) continue;
+            const float f = exp2f(ml[u].x - M);
+            l = fmaf(f, ml[u].y, l);
+            o.x = fmaf(f, v[u].x, o.x); o.y = fmaf(f, v[u].y, o.y); o.z = fmaf(f, v[u].z, o.z); o.w = fmaf(f, v[u].w, o.w);
+        }
+    }
+    if constexpr (kLanes > 1) {
+        so[unit][c] = o;
+        if (c == 0) sml[unit] = make_float2(M, l);
+        __syncthreads();
+        if (lane || done) return;
+        M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) M = fmaxf(M, sml[unit + k].x);
+        l = 0.0f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (M != -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < kLanes; ++k) {
+                if (sml[unit + k].x == -INFINITY) continue;
+                const float f = exp2f(sml[unit + k].x - M);
+                const float4 v = so[unit + k][c];
+                l = fmaf(f, sml[unit + k].y, l);
+                o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+            }
+        }
+    }
+    if (r >= all_rows) return;
+    const bool seen = M != -INFINITY;
+    const float inv = seen ? 1.0f / l : 0.0f;
+    *reinterpret_cast<float4*>(a.out + (int64_t)s * a.out_nb_seq + (int64_t)node * a.out_nb_node + h * kD + c * 4) =
+        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (a.lse && c == 0) a.lse[((int64_t)s * a.max_nodes + node) * a.Hq + h] = seen ? (M + log2f(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+// Launch for K type KT (tree_tc_inst.cu, one unit per K type).
+template <int KT> cudaError_t launch_tc_for_k(cudaStream_t stream, const TcArgs& a);
+
+}  // namespace tree
+}  // namespace cvattn
