@@ -10,7 +10,7 @@
 //                   CTA's tiles 2 k + g, so one computes while the other's MMAs run
 //   warps 8-11      producer: raw rows by cp.async, then f16 tiles (128B swizzle);
 //                   f16 caches are copied straight into the tiles
-//   warps 12, 13    MMA issuers of the two groups
+//   warps 12, 13    MMA issuers of the two groups (14, 15 fill up their warpgroup)
 // Precision: products of split numbers.  x = hi + lo in f16, S = Qh Kh + Ql Kh
 // (+ Qh Kl), O = Ph Vh + Pl Vh (+ Ph Vl); the dropped low x low term is 2^-22 of the
 // largest.  Q is scaled per row, K and V per tile, by powers of two so that hi and
@@ -31,7 +31,10 @@ namespace tree {
 
 constexpr int kTcTile = 128;
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 14 * 32;
+constexpr int kTcThreads = 16 * 32;
+// Registers of a thread by role: launched with 128; 256 * 168 + 128 * 88 + 128 * 80 <= 512 * 128.
+constexpr int kTcRegsSoftmax = 168, kTcRegsProducer = 88, kTcRegsIssuer = 80;
+static_assert(256 * kTcRegsSoftmax + 128 * kTcRegsProducer + 128 * kTcRegsIssuer <= 65536, "the block's registers");
 constexpr int kTcMaxSeq = 1024;       // prefix table in shared memory
 constexpr int kTcExps = 8;            // tiles whose scales may be in flight
 constexpr int kTcTileBytes = kTcTile * kD * 2;
@@ -71,6 +74,9 @@ struct TcShape {
     static constexpr int kBytes = kPref + (kTcMaxSeq + 1) * 4;
     static_assert(kBytes <= 227 * 1024, "one CTA per SM");
 };
+
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long ra = *reinterpret_cast<unsigned long long*>(&a), rb = *reinterpret_cast<unsigned long long*>(&b), rd;
@@ -217,6 +223,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 
     if (warp < 8) {
         // ------------------------------------------------------ softmax group g
+        regs_up<kTcRegsSoftmax>();
         const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         const uint32_t sp = tmem + lane_base + g * 128, ot = tmem + lane_base + 256 + g * 64;
@@ -453,6 +460,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         }
     } else if (warp < 12) {
         // ------------------------------------------------------ producer: thread = key
+        regs_down<kTcRegsProducer>();
         const int key = tid - 256;
         auto tile_of = [&](const Run& r, int tile, bool& draft, int& p0, int& count) {
             draft = tile >= r.x.cache_tiles;
@@ -616,7 +624,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
         }
         cp_async_wait<0>();
-    } else if (lane == 0) {
+    } else {
+        regs_down<kTcRegsIssuer>();
+        if (warp < 14 && lane == 0) {
         // ------------------------------------------------------ MMA issuer of group g
         const int g = warp - 12;
         const uint32_t idesc_s = tc::idesc_f16_f32(128, kTcTile, false), idesc_o = tc::idesc_f16_f32(128, 64, true);
@@ -659,6 +669,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 tc::mma_commit(&B->v_empty[st]);
             }
             i = last;
+        }
         }
     }
 
