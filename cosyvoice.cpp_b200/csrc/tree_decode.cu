@@ -312,6 +312,7 @@ static cudaError_t launch_tc(cudaStream_t stream, const Args& a, const Plan& pla
     TcArgs ta{};
     ta.a = a;
     ta.grid = plan.tc_grid;
+    ta.inv_g = (uint32_t)((65536 + a.G - 1) / a.G);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     ta.ws_pref = reinterpret_cast<int32_t*>(ws);
     ws += align256((size_t)(a.n_seq + 1) * 4);

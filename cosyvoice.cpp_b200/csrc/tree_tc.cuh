@@ -42,6 +42,7 @@ constexpr float kTcOffs = 7.0f;
 
 struct TcArgs {
     Args a;
+    uint32_t inv_g;                   // ceil(2^16 / G): r * inv_g >> 16 = r / G for r < 2^13 / G
     int grid;                         // CTAs that share the list
     float* ws_o;                      // [2 * grid][128][64]
     float* ws_ml;                     // [2 * grid][128][2]
@@ -71,12 +72,31 @@ struct TcShape {
     static constexpr int kMl = kRaw + 2 * (rawK + rawV);
     static constexpr int kBars = kMl + 2 * kTcRows * 8;
     static constexpr int kPref = kBars + (int)((sizeof(TcBars) + 15) / 16 * 16);
-    static constexpr int kBytes = kPref + (kTcMaxSeq + 1) * 4;
+    static constexpr int kLen = kPref + (kTcMaxSeq + 4) * 4, kNodes = kLen + kTcMaxSeq * 4;
+    static constexpr int kBytes = kNodes + kTcMaxSeq * 2;
     static_assert(kBytes <= 227 * 1024, "one CTA per SM");
 };
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Bounded wait; a short poll first, since most phases end within a few hundred cycles.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* err, int* status, int site) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+        if (mbar_test(bar, parity)) return true;
+    return fp::wait_or_err(bar, parity, err, status, site);
+}
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long ra = *reinterpret_cast<unsigned long long*>(&a), rb = *reinterpret_cast<unsigned long long*>(&b), rd;
@@ -92,29 +112,68 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // Units of sequence s: row tiles times KV heads, row tile major.
 __device__ __forceinline__ int units_of(const Args& a, const Lens& x) { return (x.n * a.G + kTcRows - 1) / kTcRows * a.Hkv; }
 
-struct Run {
-    int s, kvh, rt, t0, t1, T;   // tiles [t0, t1) of T
-    Lens x;
+// A CTA's walk through its part of the list, run by run.  Lengths come from shared memory (SeqTab), so that a new run
+// costs no trip to global memory and no division.
+struct SeqTab {
+    const int32_t *pref, *len;
+    const uint16_t* nodes;
 };
-// The run that starts at list entry i and ends before hi.
-__device__ __forceinline__ Run run_at(const Args& a, const int32_t* pref, int i, int hi) {
-    int lo = 0, up = a.n_seq;  // last s with pref[s] <= i: its list is not empty
-    while (up - lo > 1) {
-        const int mid = (lo + up) >> 1;
-        if (pref[mid] <= i) lo = mid;
-        else up = mid;
+struct Run {
+    int s, kvh, rt;       // unit: sequence, KV head, tile of 128 rows
+    int i, end;           // list entries [i, end) of this run
+    int t0, T;            // its first tile, and the unit's tiles
+    int L, n, cache_tiles, units_left;
+
+    __device__ __forceinline__ void sequence(const Args& a, const SeqTab& tab, int seq) {
+        s = seq;
+        L = tab.len[seq];
+        n = tab.nodes[seq];
+        cache_tiles = (L + kTcTile - 1) / kTcTile;
+        T = n == 0 ? 0 : cache_tiles + (a.kd ? (n + kTcTile - 1) / kTcTile : 0);
     }
-    Run r;
-    r.s = lo;
-    r.x = lens_of(a, lo, false);
-    r.T = r.x.tiles;
-    const int u = (i - pref[lo]) / r.T;
-    r.t0 = (i - pref[lo]) - u * r.T;
-    r.t1 = min(r.T, r.t0 + (hi - i));
-    r.kvh = u % a.Hkv;
-    r.rt = u / a.Hkv;
-    return r;
-}
+    __device__ __forceinline__ void start(const Args& a, const SeqTab& tab, int entry, int hi) {
+        i = end = entry;
+        if (entry >= hi) return;
+        int lo = 0, up = a.n_seq;  // last s with pref[s] <= entry: its list is not empty
+        while (up - lo > 1) {
+            const int mid = (lo + up) >> 1;
+            if (tab.pref[mid] <= entry) lo = mid;
+            else up = mid;
+        }
+        sequence(a, tab, lo);
+        const int u = (entry - tab.pref[lo]) / T;
+        t0 = entry - tab.pref[lo] - u * T;
+        rt = u / a.Hkv;
+        kvh = u - rt * a.Hkv;
+        units_left = (tab.pref[lo + 1] - tab.pref[lo]) / T - u - 1;
+        end = min(hi, i + T - t0);
+    }
+    __device__ __forceinline__ void next(const Args& a, const SeqTab& tab, int hi) {
+        i = end;
+        if (i >= hi) return;
+        t0 = 0;
+        if (units_left > 0) {
+            --units_left;
+            if (++kvh == a.Hkv) {
+                kvh = 0;
+                ++rt;
+            }
+        } else {
+            int q = s + 1;
+            while (tab.pref[q + 1] == i) ++q;  // sequences without entries
+            sequence(a, tab, q);
+            rt = kvh = 0;
+            units_left = (n * a.G + kTcRows - 1) / kTcRows * a.Hkv - 1;
+        }
+        end = min(hi, i + T);
+    }
+    __device__ __forceinline__ void tile(int entry, bool& draft, int& p0, int& count) const {
+        const int t = t0 + (entry - i);
+        draft = t >= cache_tiles;
+        p0 = (draft ? t - cache_tiles : t) * kTcTile;
+        count = min(kTcTile, (draft ? n : L) - p0);
+    }
+};
 
 __device__ __forceinline__ int tc_cut(int c, int n, int g) { return (int)((long long)c * n / g); }
 __device__ __forceinline__ int tc_owner(int i, int n, int g) { return (int)(((long long)(i + 1) * g - 1) / n); }
@@ -161,6 +220,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     const Args& a = ta.a;
     TcBars* B = reinterpret_cast<TcBars*>(smem + Sh::kBars);
     int32_t* pref = reinterpret_cast<int32_t*>(smem + Sh::kPref);
+    const SeqTab tab{pref, reinterpret_cast<int32_t*>(smem + Sh::kLen), reinterpret_cast<uint16_t*>(smem + Sh::kNodes)};
     if (smem_addr(smem) & 1023u) {
         if (threadIdx.x == 0) record_status(a.status, kStatusTimeout);
         return;
@@ -195,6 +255,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             if (s < a.n_seq) {
                 const Lens x = lens_of(a, s, blockIdx.x == 0);
                 n = x.tiles * units_of(a, x);
+                reinterpret_cast<int32_t*>(smem + Sh::kLen)[s] = x.L;
+                reinterpret_cast<uint16_t*>(smem + Sh::kNodes)[s] = (uint16_t)x.n;
             }
             int incl = n;
 #pragma unroll
@@ -229,34 +291,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         const uint32_t sp = tmem + lane_base + g * 128, ot = tmem + lane_base + 256 + g * 64;
         uint8_t* qhi = smem + Sh::kQ;
         uint8_t* qlo = qhi + kTcTileBytes;
-        float* xch = reinterpret_cast<float*>(smem + Sh::kQ);  // [group][row][32 floats of the other group's half]
-        float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl);
+        float4* xch = reinterpret_cast<float4*>(smem + Sh::kQ) + row * 16;  // group 1's output row at a run's end
+        float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl) + row;
         uint32_t k = 0;  // tiles of this group so far
         bool ok = true;
-        for (int i = lo; i < hi;) {
-            const Run r = run_at(a, pref, i, hi);
-            const int rr = r.rt * kTcRows + row, rows = r.x.n * a.G;
+        Run r;
+        for (r.start(a, tab, lo, hi); r.i < hi; r.next(a, tab, hi)) {
+            const int rr = r.rt * kTcRows + row, rows = r.n * a.G;
             const bool real = rr < rows;
             const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
-            const int node = rr / a.G, h = r.kvh * a.G + rr % a.G;
-            // Q: each group reads the row and writes its half of the dims
+            const int node = (int)(((uint32_t)rr * ta.inv_g) >> 16), h = r.kvh * a.G + rr - node * a.G;
+            const int64_t orow = (int64_t)r.s * a.out_nb_seq + (int64_t)node * a.out_nb_node + h * kD;
+            // Q: both groups look at the whole row, each writes its half of the dims
             float rs;
             {
                 const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)node * a.q_nb_node + h * kD);
-                float4 v[8];
                 float am = 0.0f;
+                float4 v[8];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const float4 o = real ? q[8 * (g ^ 1) + c] : make_float4(0.f, 0.f, 0.f, 0.f);
                     v[c] = real ? q[8 * g + c] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    am = fmaxf(am, fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w))));
-                    am = fmaxf(am, fmaxf(fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w))));
+                    am = max3(am, fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
+                    am = max3(am, fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w)));
                 }
                 const int ex = dtc::norm_exp(am);
                 const float sc = pow2f(ex);
                 rs = pow2f(-ex) * a.scale_log2;
-                // nothing reads the last run's Q, or its exchanged halves, any more
-                if (i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
+                // nothing reads the last run's Q, or its exchanged rows, any more
+                if (r.i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t wh[4], wl[4];
@@ -277,37 +340,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 0.0f;
             bool pending = false;  // a tile's output still to be added, times vs_last
             auto add_output = [&]() {
+                uint32_t o0[32], o1[32];
+                tc::tmem_ld32(ot, o0);
+                tc::tmem_ld32(ot + 32, o1);
+                tc::tmem_ld_wait();
+                const float2 f = make_float2(vs_last, vs_last);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t ov[32];
-                    tc::tmem_ld32(ot + 32 * c, ov);
-                    tc::tmem_ld_wait();
-                    const float2 f = make_float2(vs_last, vs_last);
-#pragma unroll
-                    for (int d = 0; d < 16; ++d)
-                        O[16 * c + d] = ffma2(make_float2(__uint_as_float(ov[2 * d]), __uint_as_float(ov[2 * d + 1])), f, O[16 * c + d]);
+                for (int d = 0; d < 16; ++d) {
+                    O[d] = ffma2(make_float2(__uint_as_float(o0[2 * d]), __uint_as_float(o0[2 * d + 1])), f, O[d]);
+                    O[16 + d] = ffma2(make_float2(__uint_as_float(o1[2 * d]), __uint_as_float(o1[2 * d + 1])), f, O[16 + d]);
                 }
             };
-            const int first = i, last = i + (r.t1 - r.t0);
-            for (int j = first + ((first ^ g ^ lo) & 1); ok && j < last; j += 2) {  // the CTA's tile j - lo of parity g
-                const int tile = r.t0 + (j - first);
-                const bool draft = tile >= r.x.cache_tiles;
-                const int p0 = (draft ? tile - r.x.cache_tiles : tile) * kTcTile;
-                const int count = min(kTcTile, (draft ? r.x.n : r.x.L) - p0);
-                ok = fp::wait_or_err(&B->s_full[g], k & 1, &B->err, a.status, 31);
+            for (int j = r.i + ((r.i ^ g ^ lo) & 1); j < r.end; j += 2) {  // the CTA's tiles j - lo of parity g
+                bool draft;
+                int p0, count;
+                r.tile(j, draft, p0, count);
+                ok = tc_wait(&B->s_full[g], k & 1, &B->err, a.status, 31);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 ++k;
                 tc::fence_after();
                 if (warp_real) {
+                    uint32_t sv[32];
+                    tc::tmem_ld32(sp, sv);
                     if (pending) add_output();
                     const float2 ex = B->exps[(j - lo) % kTcExps];
                     const float rst = rs * ex.x;
                     const bool masked = draft || count < kTcTile;
+                    tc::tmem_ld_wait();
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t sv[32];
-                        tc::tmem_ld32(sp + 32 * c, sv);
-                        tc::tmem_ld_wait();
                         float2 x[16];
                         {
                             const float2 f = make_float2(rst, rst), b = make_float2(-base, -base);
@@ -315,6 +376,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                             for (int d = 0; d < 16; ++d)
                                 x[d] = ffma2(make_float2(__uint_as_float(sv[2 * d]), __uint_as_float(sv[2 * d + 1])), f, b);
                         }
+                        tc::tmem_ld32(sp + 32 * min(c + 1, 3), sv);  // under way during this chunk's arithmetic
                         if (masked) {
                             const int left = count - 32 * c;
                             uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
@@ -329,9 +391,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                 if (!((bits >> (2 * d + 1)) & 1u)) x[d].y = -INFINITY;
                             }
                         }
-                        float mx = fmaxf(x[0].x, x[0].y);
+                        float mx;
+                        {
+                            float m4[4];
 #pragma unroll
-                        for (int d = 1; d < 16; ++d) mx = fmaxf(mx, fmaxf(x[d].x, x[d].y));
+                            for (int u = 0; u < 4; ++u)
+                                m4[u] = max3(max3(fmaxf(x[4 * u].x, x[4 * u].y), x[4 * u + 1].x, x[4 * u + 1].y), max3(x[4 * u + 2].x, x[4 * u + 2].y, x[4 * u + 3].x),
+                                             x[4 * u + 3].y);
+                            mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+                        }
                         if (__any_sync(0xffffffffu, mx > thr)) {
                             float f = 1.0f, up = 0.0f;
                             if (mx > thr) {
@@ -346,29 +414,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                             for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
 #pragma unroll
                             for (int d = 0; d < 16; ++d) x[d] = add2(x[d], u2);
-                            if (c) tc::tmem_st_wait();
+                            if (c) {
+                                tc::tmem_st_wait();
+                                tc::tmem_ld_wait();
+                            }
 #pragma unroll 1
-                            for (int e = 0; e < c; ++e) {  // this tile's P so far
-                                uint32_t pv[32];
-                                tc::tmem_ld32(sp + 32 * e, pv);
+                            for (int e = 0; e < 2 * c; ++e) {  // this tile's P so far, 16 keys at a time
+                                uint32_t ph[8], pl[8];
+                                const uint32_t at = sp + 32 * (e >> 1) + 8 * (e & 1);
+                                tc::tmem_ld8(at, ph);
+                                tc::tmem_ld8(at + 16, pl);
                                 tc::tmem_ld_wait();
 #pragma unroll
-                                for (int d = 0; d < 16; ++d) {
-                                    const float2 ph = __half22float2(*reinterpret_cast<const __half2*>(&pv[d]));
-                                    const float2 pl = __half22float2(*reinterpret_cast<const __half2*>(&pv[16 + d]));
-                                    split2((ph.x + pl.x) * f, (ph.y + pl.y) * f, pv[d], pv[16 + d]);
+                                for (int d = 0; d < 8; ++d) {
+                                    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&ph[d]));
+                                    const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&pl[d]));
+                                    split2((u.x + w.x) * f, (u.y + w.y) * f, ph[d], pl[d]);
                                 }
-                                tc::tmem_st32(sp + 32 * e, pv);
+                                tc::tmem_st8(at, ph);
+                                tc::tmem_st8(at + 16, pl);
                             }
                         }
-                        float2 ls = make_float2(0.f, 0.f);
+                        float2 l0 = make_float2(0.f, 0.f), l1 = l0;
 #pragma unroll
-                        for (int d = 0; d < 16; ++d) {
+                        for (int d = 0; d < 16; d += 2) {
                             x[d].x = fast_exp2(x[d].x);
                             x[d].y = fast_exp2(x[d].y);
-                            ls = add2(ls, x[d]);
+                            x[d + 1].x = fast_exp2(x[d + 1].x);
+                            x[d + 1].y = fast_exp2(x[d + 1].y);
+                            l0 = add2(l0, x[d]);
+                            l1 = add2(l1, x[d + 1]);
                         }
-                        l += ls.x + ls.y;
+                        l0 = add2(l0, l1);
+                        l += l0.x + l0.y;
                         if (draft) {
                             // keys whose V is not finite have zeros in the tile; rows that see one add it here
                             uint32_t bad = B->bad[(j - lo) % kTcExps][c];
@@ -391,15 +469,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                 }
                             }
                         }
+                        uint32_t pv[32];
 #pragma unroll
                         for (int d = 0; d < 16; ++d) {
                             const float2 t = make_float2(__uint_as_float(__float_as_uint(x[d].x) & 0xFFFFE000u),
                                                          __uint_as_float(__float_as_uint(x[d].y) & 0xFFFFE000u));
                             const float2 e = add2(x[d], make_float2(-t.x, -t.y));
-                            sv[d] = tc::pack_f16x2(t.x, t.y);
-                            sv[16 + d] = tc::pack_f16x2(e.x, e.y);
+                            pv[d] = tc::pack_f16x2(t.x, t.y);
+                            pv[16 + d] = tc::pack_f16x2(e.x, e.y);
                         }
-                        tc::tmem_st32(sp + 32 * c, sv);
+                        tc::tmem_st32(sp + 32 * c, pv);
+                        tc::tmem_ld_wait();
                     }
                     vs_last = ex.y;
                     pending = true;
@@ -410,95 +490,103 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
             // the last tile's output (o_full counts every tile of this group)
             if (ok && pending) {
-                ok = fp::wait_or_err(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
+                ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
                 ok = __all_sync(0xffffffffu, ok);
                 tc::fence_after();
                 if (ok) add_output();
             }
             tc::fence_before();
             if (!fp::prod_bar_and(2, 256, ok)) break;  // every MMA of the run is done; all threads leave together
-            // each group finishes 32 of the 64 dims: the other half goes to the other group
-            {
-                float4* mine = reinterpret_cast<float4*>(xch + (g * kTcRows + row) * 32);
+            const float m_mine = thr == -INFINITY && l == 0.0f ? -INFINITY : base;  // (NaN scores raise nothing)
+            if (g == 1) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float2 u = g ? O[2 * c] : O[16 + 2 * c], v = g ? O[2 * c + 1] : O[16 + 2 * c + 1];
-                    mine[c ^ (row & 7)] = make_float4(u.x, u.y, v.x, v.y);
-                }
-                mls[g * kTcRows + row] = make_float2(thr == -INFINITY && l == 0.0f ? -INFINITY : base, l);
+                for (int c = 0; c < 16; ++c) xch[c ^ (row & 7)] = make_float4(O[2 * c].x, O[2 * c].y, O[2 * c + 1].x, O[2 * c + 1].y);
+                *mls = make_float2(m_mine, l);
             }
             asm volatile("bar.sync 3, 256;" ::: "memory");
-            {
-                const float2 m0 = mls[g * kTcRows + row], m1 = mls[(g ^ 1) * kTcRows + row];
-                const float M = fmaxf(m0.x, m1.x);
-                const float f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - M), f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - M);
-                const float sum = (f0 == 0.0f ? 0.0f : f0 * m0.y) + (f1 == 0.0f ? 0.0f : f1 * m1.y);
-                const bool whole = r.t1 - r.t0 == r.T, seen = M != -INFINITY;
+            if (g == 0 && real) {
+                const float2 other = *mls;
+                const float M = fmaxf(m_mine, other.x);
+                const float f0 = m_mine == -INFINITY ? 0.0f : exp2f(m_mine - M), f1 = other.x == -INFINITY ? 0.0f : exp2f(other.x - M);
+                const float sum = (m_mine == -INFINITY ? 0.0f : f0 * l) + (other.x == -INFINITY ? 0.0f : f1 * other.y);
+                const bool whole = r.end - r.i == r.T, seen = M != -INFINITY;
                 const float inv = !whole ? 1.0f : seen ? 1.0f / sum : 0.0f;
-                const int slot = 2 * blockIdx.x + (first == lo ? 0 : 1);
-                float4* dst = whole ? reinterpret_cast<float4*>(a.out + (int64_t)r.s * a.out_nb_seq + (int64_t)node * a.out_nb_node + h * kD + 32 * g)
-                                    : reinterpret_cast<float4*>(ta.ws_o + ((int64_t)slot * kTcRows + row) * kD + 32 * g);
-                const float4* other = reinterpret_cast<const float4*>(xch + ((g ^ 1) * kTcRows + row) * 32);
-                if (real) {
+                const int64_t slot = (int64_t)(2 * blockIdx.x + (r.i == lo ? 0 : 1)) * kTcRows + row;
+                float4* dst = reinterpret_cast<float4*>(whole ? a.out + orow : ta.ws_o + slot * kD);
+                const float g0 = f0 * inv, g1 = f1 * inv;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const float2 u = g ? O[16 + 2 * c] : O[2 * c], v = g ? O[16 + 2 * c + 1] : O[2 * c + 1];
-                        const float4 w = other[c ^ (row & 7)];
-                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (f0 != 0.0f) o = make_float4(f0 * u.x, f0 * u.y, f0 * v.x, f0 * v.y);
-                        if (f1 != 0.0f) o = make_float4(fmaf(f1, w.x, o.x), fmaf(f1, w.y, o.y), fmaf(f1, w.z, o.z), fmaf(f1, w.w, o.w));
-                        dst[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-                    }
-                    if (g == 0) {
-                        if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + ((int64_t)slot * kTcRows + row) * 2) = make_float2(M, sum);
-                        else if (a.lse)
-                            a.lse[((int64_t)r.s * a.max_nodes + node) * a.Hq + h] = seen ? (M + log2f(sum)) * 0.69314718055994531f : -INFINITY;
-                    }
+                for (int c = 0; c < 16; ++c) {
+                    const float4 w = xch[c ^ (row & 7)];
+                    // (what has no weight is left out: it may not be finite)
+                    float4 o = g0 != 0.0f ? make_float4(g0 * O[2 * c].x, g0 * O[2 * c].y, g0 * O[2 * c + 1].x, g0 * O[2 * c + 1].y)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (g1 != 0.0f) o = make_float4(fmaf(g1, w.x, o.x), fmaf(g1, w.y, o.y), fmaf(g1, w.z, o.z), fmaf(g1, w.w, o.w));
+                    dst[c] = o;
                 }
+                if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + slot * 2) = make_float2(M, sum);
+                else if (a.lse)
+                    a.lse[((int64_t)r.s * a.max_nodes + node) * a.Hq + h] = seen ? (M + log2f(sum)) * 0.69314718055994531f : -INFINITY;
             }
-            i = last;
         }
     } else if (warp < 12) {
         // ------------------------------------------------------ producer: thread = key
         regs_down<kTcRegsProducer>();
         const int key = tid - 256;
-        auto tile_of = [&](const Run& r, int tile, bool& draft, int& p0, int& count) {
-            draft = tile >= r.x.cache_tiles;
-            p0 = (draft ? tile - r.x.cache_tiles : tile) * kTcTile;
-            count = min(kTcTile, (draft ? r.x.n : r.x.L) - p0);
-        };
         // keys [0, count) of a tile into shared memory, zeros up to 128
         auto copy = [&](auto type_tag, bool raw, uint8_t* dst, const uint8_t* src, int64_t nb1, int count) {
             constexpr int T = decltype(type_tag)::value;
             const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)nb1;
-            const int unit = T == kF16 && (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 2;
-            const int w = 2 * group_bytes(T) / unit, per = 128 / w;
-            const int k0 = key / w, col = (key - k0 * w) * unit;
+            if (T == kF16 && (al & 15) == 0) {
+                // 8 chunks of 16 bytes per key: this thread's chunk of every 16th key, whose swizzle is the same
+                const int k0 = key >> 3, col = (key & 7) << 4;
+                const uint8_t* from = src + (int64_t)k0 * nb1 + col;
+                uint8_t* to = dst + k0 * 128 + (col ^ ((k0 & 7) << 4));
+                const int64_t step = 16 * nb1;
+                if (count == kTcTile) {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) cp_async16(to + u * 2048, from + u * step, true);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < 8; ++u) cp_async16(to + u * 2048, k0 + 16 * u < count ? from + u * step : src, k0 + 16 * u < count);
+                }
+                return;
+            }
+            const int unit = (al & 3) == 0 ? 4 : 2;
+            const int w = 2 * group_bytes(T) / unit, per = unit == 4 ? 128 / (group_bytes(T) / 2) : 128 / group_bytes(T);
+            const int k0 = unit == 4 ? key / (group_bytes(T) / 2) : key / group_bytes(T), col = (key - k0 * w) * unit;
             if (k0 >= per) return;
-            for (int kk = k0; kk < kTcTile; kk += per) {
+            const uint8_t* from = src + (int64_t)k0 * nb1 + col;
+            const int64_t step = (int64_t)per * nb1;
+            if (raw && unit == 4) {
+                uint8_t* to = dst + k0 * raw_stride(T) + col;
+                const int tstep = per * raw_stride(T);
+                int kk = k0;
+#pragma unroll 4
+                for (; kk < count; kk += per, from += step, to += tstep) cp_async4(to, from, true);
+#pragma unroll 1
+                for (; kk < kTcTile; kk += per, to += tstep) *reinterpret_cast<uint32_t*>(to) = 0u;
+                return;
+            }
+#pragma unroll 1
+            for (int kk = k0; kk < kTcTile; kk += per, from += step) {
                 const bool there = kk < count;
-                const uint8_t* from = src + (int64_t)(there ? kk : 0) * nb1 + col;
                 uint8_t* to = raw ? dst + kk * raw_stride(T) + col : dst + kk * 128 + (col ^ ((kk & 7) << 4));
-                if (unit == 16) cp_async16(to, from, there);
-                else if (unit == 4) cp_async4(to, from, there);
+                if (unit == 4) cp_async4(to, there ? from : src, there);
                 else *reinterpret_cast<uint16_t*>(to) = there ? *reinterpret_cast<const uint16_t*>(from) : (uint16_t)0;
             }
         };
-        // cursors: the tile whose copies start (n_issue) and the tile that is finished (n)
-        Run ri{}, rc{};
-        int ii = lo, ic = lo;            // list entries
-        int fi = lo, fc = lo;            // first entries of the cursors' runs
-        if (lo < hi) ri = rc = run_at(a, pref, lo, hi);
+        // the runs of the tile whose copies start and of the tile that is finished
+        Run ri, rc;
+        ri.start(a, tab, lo, hi);
+        rc = ri;
+        int ii = lo;
         bool ok = true;
         auto issue = [&](int n) {        // copies of the CTA's tile n (list entry ii)
             if (ii < hi) {
-                if (ii - fi >= ri.t1 - ri.t0) {
-                    fi = ii;
-                    ri = run_at(a, pref, ii, hi);
-                }
+                if (ii == ri.end) ri.next(a, tab, hi);
                 bool draft;
                 int p0, count;
-                tile_of(ri, ri.t0 + (ii - fi), draft, p0, count);
+                ri.tile(ii, draft, p0, count);
                 const uint8_t* ks = (draft ? a.kd + (int64_t)ri.s * a.kd_nb2 : seq_base(a.k_seq_ptrs, a.k, a.k_nb2, ri.s)) + ri.kvh * sliceK;
                 const uint8_t* vs = (draft ? a.vd + (int64_t)ri.s * a.vd_nb2 : seq_base(a.v_seq_ptrs, a.v, a.v_nb2, ri.s)) + ri.kvh * sliceV;
                 const int64_t nk = draft ? a.kd_nb1 : a.k_nb1, nv = draft ? a.vd_nb1 : a.v_nb1;
@@ -507,31 +595,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 uint8_t* raw = smem + Sh::kRaw + (n & 1) * (Sh::rawK + Sh::rawV);
                 const uint32_t use = n / kSt;
                 if constexpr (NK == 1)
-                    if (use > 0) ok = ok && fp::wait_or_err(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 33);
+                    if (use > 0) ok = ok && tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 33);
+                if (ok) copy(std::integral_constant<int, KT>{}, NK == 2, NK == 2 ? raw : tiles, ks + (int64_t)p0 * nk, nk, count);
                 if constexpr (NV == 1)
-                    if (use > 0) ok = ok && fp::wait_or_err(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 34);
-                if (ok) {
-                    copy(std::integral_constant<int, KT>{}, NK == 2, NK == 2 ? raw : tiles, ks + (int64_t)p0 * nk, nk, count);
-                    copy(std::integral_constant<int, VT>{}, NV == 2, NV == 2 ? raw + Sh::rawK : tiles + NK * kTcTileBytes, vs + (int64_t)p0 * nv, nv, count);
-                }
+                    if (use > 0) ok = ok && tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 34);
+                if (ok) copy(std::integral_constant<int, VT>{}, NV == 2, NV == 2 ? raw + Sh::rawK : tiles + NK * kTcTileBytes, vs + (int64_t)p0 * nv, nv, count);
                 ++ii;
             }
             cp_async_commit();
         };
         constexpr int kAhead = NK + NV == 2 ? kSt - 2 : 1;  // tiles whose copies run ahead of the finished one
         for (int n = 0; n < kAhead; ++n) issue(n);
-        for (int n = 0; ic < hi; ++n, ++ic) {
+        for (int n = 0; lo + n < hi; ++n) {
             cp_async_wait<kAhead - 1>();
             // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
             if (!fp::prod_bar_and(4, 128, ok)) break;
             issue(n + kAhead);
-            if (ic - fc >= rc.t1 - rc.t0) {
-                fc = ic;
-                rc = run_at(a, pref, ic, hi);
-            }
+            if (lo + n == rc.end) rc.next(a, tab, hi);
             bool draft;
             int p0, count;
-            tile_of(rc, rc.t0 + (ic - fc), draft, p0, count);
+            rc.tile(lo + n, draft, p0, count);
             const int st = n % kSt;
             const uint32_t use = n / kSt;
             uint8_t* tiles = smem + Sh::kTiles + st * Sh::kStage;
@@ -579,7 +662,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 B->exps[n % kTcExps] = make_float2(1.0f, 1.0f);
             }
             if constexpr (NK == 2) {
-                if (use > 0) ok = ok && fp::wait_or_err(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 35);
+                if (use > 0) ok = ok && tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 35);
                 if (ok) {
 #pragma unroll 1
                     for (int b = 0; b < 2; ++b) {
@@ -601,7 +684,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                         for (int c = 0; c < 8; ++c) p[c] = make_uint4(0u, 0u, 0u, 0u);
                 }
             } else {
-                if (use > 0) ok = ok && fp::wait_or_err(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 36);
+                if (use > 0) ok = ok && tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 36);
                 if (ok) {
                     const bool drop = draft && bad;
 #pragma unroll 1
@@ -626,50 +709,57 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         cp_async_wait<0>();
     } else {
         regs_down<kTcRegsIssuer>();
-        if (warp < 14 && lane == 0) {
-        // ------------------------------------------------------ MMA issuer of group g
-        const int g = warp - 12;
-        const uint32_t idesc_s = tc::idesc_f16_f32(128, kTcTile, false), idesc_o = tc::idesc_f16_f32(128, 64, true);
-        const uint32_t sp = tmem + g * 128, ot = tmem + 256 + g * 64;
-        const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
-        const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
-        uint32_t k = 0, n_run = 0;
-        bool ok = true;
-        for (int i = lo; ok && i < hi; ++n_run) {
-            const Run r = run_at(a, pref, i, hi);
-            const int first = i, last = i + (r.t1 - r.t0);
-            ok = fp::wait_or_err(&B->q_full, n_run & 1, &B->err, a.status, 37);
-            for (int j = first + ((first ^ g ^ lo) & 1); ok && j < last; j += 2, ++k) {
-                const int n = j - lo, st = n % kSt;
-                const uint32_t tiles = smem_addr(smem + Sh::kTiles + st * Sh::kStage);
-                ok = fp::wait_or_err(&B->kv_full[st], (n / kSt) & 1, &B->err, a.status, 38);
-                if (!ok) break;
-                tc::fence_after();
-                const uint64_t dk = tc::sdesc_sw128(tiles, 16, 1024);
+        if (warp < 14) {
+            // -------------------------------------------------- MMA issuer of group g: the whole warp walks, one lane issues
+            const int g = __shfl_sync(0xffffffffu, warp, 0) - 12;
+            const uint32_t idesc_s = tc::idesc_f16_f32(128, kTcTile, false), idesc_o = tc::idesc_f16_f32(128, 64, true);
+            const uint32_t sp = tmem + g * 128, ot = tmem + 256 + g * 64;
+            const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
+            const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
+            const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
+            uint32_t k = 0, n_run = 0;
+            bool ok = true;
+            Run r;
+            for (r.start(a, tab, lo, hi); ok && r.i < hi; r.next(a, tab, hi), ++n_run) {
+                ok = tc_wait(&B->q_full, n_run & 1, &B->err, a.status, 37);
+                for (int j = r.i + ((r.i ^ g ^ lo) & 1); ok && j < r.end; j += 2, ++k) {
+                    const int n = j - lo, st = n % kSt;
+                    ok = tc_wait(&B->kv_full[st], (n / kSt) & 1, &B->err, a.status, 38);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint64_t dk = dt0 + (uint64_t)(st * (Sh::kStage >> 4));
+                    const uint64_t dv = dk + NK * (kTcTileBytes >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc_s, kk > 0 ? 1u : 0u);
-                    tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc_s, 1u);
-                    if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc_s, 1u);
-                }
-                tc::mma_commit(&B->s_full[g]);
-                tc::mma_commit(&B->k_empty[st]);
-                ok = fp::wait_or_err(&B->p_full[g], k & 1, &B->err, a.status, 39);
-                if (!ok) break;
-                tc::fence_after();
-                const uint64_t dv = tc::sdesc_sw128(tiles + NK * kTcTileBytes, 16, 1024);
+                        for (int kk = 0; kk < 4; ++kk) {
+                            tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc_s, kk > 0 ? 1u : 0u);
+                            tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc_s, 1u);
+                            if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc_s, 1u);
+                        }
+                        tc::mma_commit(&B->s_full[g]);
+                        tc::mma_commit(&B->k_empty[st]);
+                    }
+                    __syncwarp();
+                    ok = tc_wait(&B->p_full[g], k & 1, &B->err, a.status, 39);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc::fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk) {
-                    const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
-                    tc::mma_ts(ot, ph, dv + kk * 128, idesc_o, kk > 0 ? 1u : 0u);
-                    tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc_o, 1u);
-                    if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc_o, 1u);
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
+                            tc::mma_ts(ot, ph, dv + kk * 128, idesc_o, kk > 0 ? 1u : 0u);
+                            tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc_o, 1u);
+                            if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc_o, 1u);
+                        }
+                        tc::mma_commit(&B->o_full[g]);
+                        tc::mma_commit(&B->v_empty[st]);
+                    }
+                    __syncwarp();
                 }
-                tc::mma_commit(&B->o_full[g]);
-                tc::mma_commit(&B->v_empty[st]);
+                ok = __all_sync(0xffffffffu, ok);
             }
-            i = last;
-        }
         }
     }
 
