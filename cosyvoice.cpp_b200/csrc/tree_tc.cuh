@@ -7,10 +7,11 @@
 // written out directly, parts go to the workspace and tree_tc_combine_kernel joins
 // them.  (Ragged sequences and few long ones fill the SMs alike.)
 //   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the
-//                   CTA's tiles 2 k + g, so one computes while the other's MMAs run
+//                   CTA's tiles 2 k + g
 //   warps 8-11      producer: raw rows by cp.async, then f16 tiles (128B swizzle);
 //                   f16 caches are copied straight into the tiles
-//   warps 12, 13    MMA issuers of the two groups (14, 15 fill up their warpgroup)
+//   warp 12         issues S = Q K^T, up to two tiles ahead of the softmax
+//   warp 13         issues O = P V            (14, 15 fill up their warpgroup)
 // Precision: products of split numbers.  x = hi + lo in f16, S = Qh Kh + Ql Kh
 // (+ Qh Kl), O = Ph Vh + Pl Vh (+ Ph Vl); the dropped low x low term is 2^-22 of the
 // largest.  Q is scaled per row, K and V per tile, by powers of two so that hi and
@@ -19,8 +20,10 @@
 // is its own hi and has no lo.
 // The output of a tile is a fresh accumulator, added in f32 to the row's registers:
 // adds inside the tensor cores truncate, and over a long cache that would show.
-// TMEM per group: S of the tile (128 columns), overwritten 32 keys at a time by
-// that chunk's P (16 columns hi, 16 lo), and the tile's O (64 columns).
+// TMEM: three S buffers of 128 columns, tile n in n % 3, each overwritten 32 keys at
+// a time by that chunk's P (16 columns hi, 16 lo): a group never waits for the
+// S of its next tile.  Two outputs of 64 columns, one per group, read back while
+// the group's next tile is on its way.
 #pragma once
 
 #include "flash_pipe.cuh"
@@ -50,9 +53,10 @@ struct TcArgs {
 };
 
 struct TcBars {
-    uint64_t kv_full[4], k_empty[4], v_empty[4];
+    uint64_t k_full[4], v_full[4], k_empty[4], v_empty[4];  // by stage
     uint64_t q_full;
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[3], p_full[3], s_free[3];               // by S buffer
+    uint64_t o_full[2];                                     // by group
     uint32_t tmem_base;
     int err;
     uint32_t maxk[2], maxv[2];        // largest |scale| of a tile, by tile parity
@@ -84,6 +88,12 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r != 0;
+}
+// x - h, h an f16: what rounding x to h left over (exact)
+__device__ __forceinline__ float less_f16(float x, uint16_t h) {
+    float r;
+    asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(r) : "h"(h), "h"((uint16_t)0xBC00u), "f"(x));
+    return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -229,14 +239,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 
     if (tid == 0) {
         for (int i = 0; i < kSt; ++i) {
-            mbar_init(&B->kv_full[i], 128);
+            mbar_init(&B->k_full[i], 128);
+            mbar_init(&B->v_full[i], 128);
             mbar_init(&B->k_empty[i], 1);
             mbar_init(&B->v_empty[i], 1);
         }
         mbar_init(&B->q_full, 256);
+        for (int b = 0; b < 3; ++b) {
+            mbar_init(&B->s_full[b], 1);
+            mbar_init(&B->p_full[b], 128);
+            mbar_init(&B->s_free[b], 1);
+        }
         for (int g = 0; g < 2; ++g) {
-            mbar_init(&B->s_full[g], 1);
-            mbar_init(&B->p_full[g], 128);
             mbar_init(&B->o_full[g], 1);
             B->maxk[g] = B->maxv[g] = 0u;
         }
@@ -288,7 +302,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         regs_up<kTcRegsSoftmax>();
         const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-        const uint32_t sp = tmem + lane_base + g * 128, ot = tmem + lane_base + 256 + g * 64;
+        const uint32_t ot = tmem + lane_base + 384 + g * 64;
         uint8_t* qhi = smem + Sh::kQ;
         uint8_t* qlo = qhi + kTcTileBytes;
         float4* xch = reinterpret_cast<float4*>(smem + Sh::kQ) + row * 16;  // group 1's output row at a run's end
@@ -355,14 +369,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 bool draft;
                 int p0, count;
                 r.tile(j, draft, p0, count);
-                ok = tc_wait(&B->s_full[g], k & 1, &B->err, a.status, 31);
+                const int n = j - lo, buf = n % 3;
+                const uint32_t sp = tmem + lane_base + buf * 128;
+                ok = tc_wait(&B->s_full[buf], (n / 3) & 1, &B->err, a.status, 31);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                ++k;
                 tc::fence_after();
                 if (warp_real) {
                     uint32_t sv[32];
                     tc::tmem_ld32(sp, sv);
-                    if (pending) add_output();
                     const float2 ex = B->exps[(j - lo) % kTcExps];
                     const float rst = rs * ex.x;
                     const bool masked = draft || count < kTcTile;
@@ -408,6 +422,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                 base += up;
                                 thr = kLazy + kTcOffs;
                                 l *= f;
+                                vs_last *= f;
                             }
                             const float2 f2 = make_float2(f, f), u2 = make_float2(-up, -up);
 #pragma unroll
@@ -472,23 +487,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                         uint32_t pv[32];
 #pragma unroll
                         for (int d = 0; d < 16; ++d) {
-                            const float2 t = make_float2(__uint_as_float(__float_as_uint(x[d].x) & 0xFFFFE000u),
-                                                         __uint_as_float(__float_as_uint(x[d].y) & 0xFFFFE000u));
-                            const float2 e = add2(x[d], make_float2(-t.x, -t.y));
-                            pv[d] = tc::pack_f16x2(t.x, t.y);
-                            pv[16 + d] = tc::pack_f16x2(e.x, e.y);
+                            pv[d] = tc::pack_f16x2(x[d].x, x[d].y);
+                            pv[16 + d] = tc::pack_f16x2(less_f16(x[d].x, (uint16_t)pv[d]), less_f16(x[d].y, (uint16_t)(pv[d] >> 16)));
                         }
                         tc::tmem_st32(sp + 32 * c, pv);
                         tc::tmem_ld_wait();
+                    }
+                    if (pending) {  // the output of the group's tile before this one (o_full counts every tile of the group)
+                        ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
+                        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                        tc::fence_after();
+                        add_output();
                     }
                     vs_last = ex.y;
                     pending = true;
                     tc::tmem_st_wait();
                 }
+                ++k;
                 tc::fence_before();
-                mbar_arrive(&B->p_full[g]);
+                mbar_arrive(&B->p_full[buf]);
             }
-            // the last tile's output (o_full counts every tile of this group)
             if (ok && pending) {
                 ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
                 ok = __all_sync(0xffffffffu, ok);
@@ -610,7 +628,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             cp_async_wait<kAhead - 1>();
             // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
             if (!fp::prod_bar_and(4, 128, ok)) break;
-            issue(n + kAhead);
+            // raw copies of the next tile first; copies into a stage may have to wait for it, so they come last
+            if constexpr (NK + NV == 4) issue(n + kAhead);
             if (lo + n == rc.end) rc.next(a, tab, hi);
             bool draft;
             int p0, count;
@@ -661,6 +680,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             } else if (key == 0) {
                 B->exps[n % kTcExps] = make_float2(1.0f, 1.0f);
             }
+            if constexpr (NV == 1) {
+                if (draft) {  // this thread's key
+                    uint4* p = reinterpret_cast<uint4*>(tiles + NK * kTcTileBytes + key * 128);
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 w = p[c];
+                        bad |= f16x2_special(w.x) || f16x2_special(w.y) || f16x2_special(w.z) || f16x2_special(w.w);
+                    }
+                    if (bad)
+                        for (int c = 0; c < 8; ++c) p[c] = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            if (draft) {  // (the softmax reads it with S)
+                const uint32_t vote = __ballot_sync(0xffffffffu, bad);
+                if (lane == 0) B->bad[n % kTcExps][key >> 5] = vote;
+            }
             if constexpr (NK == 2) {
                 if (use > 0) ok = ok && tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 35);
                 if (ok) {
@@ -673,17 +707,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                     }
                 }
             }
-            if constexpr (NV == 1) {
-                if (draft) {  // this thread's key
-                    uint4* p = reinterpret_cast<uint4*>(tiles + NK * kTcTileBytes + key * 128);
-                    for (int c = 0; c < 8; ++c) {
-                        const uint4 w = p[c];
-                        bad |= f16x2_special(w.x) || f16x2_special(w.y) || f16x2_special(w.z) || f16x2_special(w.w);
-                    }
-                    if (bad)
-                        for (int c = 0; c < 8; ++c) p[c] = make_uint4(0u, 0u, 0u, 0u);
-                }
-            } else {
+            if (ok) {
+                fence_proxy_async_smem();
+                mbar_arrive(&B->k_full[st]);
+            }
+            if constexpr (NV == 2) {
                 if (use > 0) ok = ok && tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 36);
                 if (ok) {
                     const bool drop = draft && bad;
@@ -697,68 +725,80 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                     }
                 }
             }
-            if (draft) {
-                const uint32_t vote = __ballot_sync(0xffffffffu, bad);
-                if (lane == 0) B->bad[n % kTcExps][key >> 5] = vote;
-            }
             if (ok) {
                 fence_proxy_async_smem();
-                mbar_arrive(&B->kv_full[st]);
+                mbar_arrive(&B->v_full[st]);
             }
+            if constexpr (NK + NV < 4) issue(n + kAhead);
         }
         cp_async_wait<0>();
     } else {
         regs_down<kTcRegsIssuer>();
-        if (warp < 14) {
-            // -------------------------------------------------- MMA issuer of group g: the whole warp walks, one lane issues
-            const int g = __shfl_sync(0xffffffffu, warp, 0) - 12;
-            const uint32_t idesc_s = tc::idesc_f16_f32(128, kTcTile, false), idesc_o = tc::idesc_f16_f32(128, 64, true);
-            const uint32_t sp = tmem + g * 128, ot = tmem + 256 + g * 64;
+        // ------------------------------------------------------ MMA issuers: the whole warp walks, one lane issues
+        const int which = __shfl_sync(0xffffffffu, warp, 0);
+        const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
+        bool ok = true;
+        if (which == 12) {
+            const uint32_t idesc = tc::idesc_f16_f32(128, kTcTile, false);
             const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
             const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
-            const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
-            uint32_t k = 0, n_run = 0;
-            bool ok = true;
+            uint32_t n_run = 0;
+            int n = 0, st = 0, buf = 0;
+            uint32_t use = 0, turn = 0;  // n / kSt, n / 3
             Run r;
             for (r.start(a, tab, lo, hi); ok && r.i < hi; r.next(a, tab, hi), ++n_run) {
                 ok = tc_wait(&B->q_full, n_run & 1, &B->err, a.status, 37);
-                for (int j = r.i + ((r.i ^ g ^ lo) & 1); ok && j < r.end; j += 2, ++k) {
-                    const int n = j - lo, st = n % kSt;
-                    ok = tc_wait(&B->kv_full[st], (n / kSt) & 1, &B->err, a.status, 38);
+                for (int j = r.i; ok && j < r.end; ++j, ++n) {
+                    ok = tc_wait(&B->k_full[st], use & 1, &B->err, a.status, 38);
+                    if (ok && n >= 3) ok = tc_wait(&B->s_free[buf], (turn - 1) & 1, &B->err, a.status, 40);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc::fence_after();
                     const uint64_t dk = dt0 + (uint64_t)(st * (Sh::kStage >> 4));
-                    const uint64_t dv = dk + NK * (kTcTileBytes >> 4);
+                    const uint32_t sp = tmem + buf * 128;
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
-                            tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc_s, kk > 0 ? 1u : 0u);
-                            tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc_s, 1u);
-                            if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc_s, 1u);
+                            tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc, kk > 0 ? 1u : 0u);
+                            tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc, 1u);
+                            if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc, 1u);
                         }
-                        tc::mma_commit(&B->s_full[g]);
+                        tc::mma_commit(&B->s_full[buf]);
                         tc::mma_commit(&B->k_empty[st]);
                     }
                     __syncwarp();
-                    ok = tc_wait(&B->p_full[g], k & 1, &B->err, a.status, 39);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc::fence_after();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
-                            tc::mma_ts(ot, ph, dv + kk * 128, idesc_o, kk > 0 ? 1u : 0u);
-                            tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc_o, 1u);
-                            if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc_o, 1u);
-                        }
-                        tc::mma_commit(&B->o_full[g]);
-                        tc::mma_commit(&B->v_empty[st]);
-                    }
-                    __syncwarp();
+                    if (++st == kSt) { st = 0; ++use; }
+                    if (++buf == 3) { buf = 0; ++turn; }
                 }
                 ok = __all_sync(0xffffffffu, ok);
+            }
+        } else if (which == 13) {
+            const uint32_t idesc = tc::idesc_f16_f32(128, 64, true);
+            int st = 0, buf = 0;
+            uint32_t use = 0, turn = 0;
+            for (int n = 0; ok && lo + n < hi; ++n) {
+                ok = tc_wait(&B->v_full[st], use & 1, &B->err, a.status, 41);
+                if (ok) ok = tc_wait(&B->p_full[buf], turn & 1, &B->err, a.status, 39);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::fence_after();
+                const uint64_t dv = dt0 + (uint64_t)(st * (Sh::kStage >> 4) + NK * (kTcTileBytes >> 4));
+                const uint32_t sp = tmem + buf * 128, ot = tmem + 384 + (n & 1) * 64;
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
+                        tc::mma_ts(ot, ph, dv + kk * 128, idesc, kk > 0 ? 1u : 0u);
+                        tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc, 1u);
+                        if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc, 1u);
+                    }
+                    tc::mma_commit(&B->o_full[n & 1]);
+                    tc::mma_commit(&B->v_empty[st]);
+                    tc::mma_commit(&B->s_free[buf]);
+                }
+                __syncwarp();
+                if (++st == kSt) { st = 0; ++use; }
+                if (++buf == 3) { buf = 0; ++turn; }
             }
         }
     }
