@@ -62,6 +62,7 @@ struct TcBars {
     uint32_t maxk[2], maxv[2];        // largest |scale| of a tile, by tile parity
     float2 exps[kTcExps];             // 2^-e of K and V of tile i at i % kTcExps
     uint32_t bad[kTcExps][4];         // draft keys whose V is not finite
+    int32_t first_run[12];            // Run at the start of the CTA's part
 };
 
 template <int KT, int VT>
@@ -100,12 +101,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// Bounded wait; a short poll first, since most phases end within a few hundred cycles.
+// Bounded wait in little code (there are many): gives up after kWaitBudgetNs, or once another role has given up.
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* err, int* status, int site) {
+    uint64_t t0 = 0;
 #pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-        if (mbar_test(bar, parity)) return true;
-    return fp::wait_or_err(bar, parity, err, status, site);
+    for (uint32_t i = 0; !mbar_try_wait_hint(bar, parity, 20000u); ++i) {
+        if ((i & 63) != 63) continue;
+        const uint64_t now = global_timer_ns();
+        if (t0 == 0) t0 = now;
+        const bool late = now - t0 > kWaitBudgetNs;
+        if (late) {
+            record_status(status, kStatusTimeout | (site << 8));
+            *reinterpret_cast<volatile int*>(err) = 1;
+        }
+        if (late || *reinterpret_cast<volatile int*>(err)) return false;
+    }
+    return true;
 }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -288,6 +299,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             pref[a.n_seq] = carry;
             if (blockIdx.x == 0) ta.ws_pref[a.n_seq] = carry;
         }
+        __syncwarp();
+        Run r;
+        r.start(a, tab, tc_cut(blockIdx.x, carry, ta.grid), tc_cut(blockIdx.x + 1, carry, ta.grid));
+        static_assert(sizeof(Run) <= sizeof(B->first_run), "a run in shared memory");
+        if (lane == 0) *reinterpret_cast<Run*>(B->first_run) = r;
     }
     tc::fence_before();
     __syncthreads();
@@ -296,6 +312,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     const uint32_t tmem = B->tmem_base;
     const int total = pref[a.n_seq];
     const int lo = tc_cut(blockIdx.x, total, ta.grid), hi = tc_cut(blockIdx.x + 1, total, ta.grid);
+    Run r = *reinterpret_cast<const Run*>(B->first_run);
 
     if (warp < 8) {
         // ------------------------------------------------------ softmax group g
@@ -309,8 +326,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl) + row;
         uint32_t k = 0;  // tiles of this group so far
         bool ok = true;
-        Run r;
-        for (r.start(a, tab, lo, hi); r.i < hi; r.next(a, tab, hi)) {
+        for (; r.i < hi; r.next(a, tab, hi)) {
             const int rr = r.rt * kTcRows + row, rows = r.n * a.G;
             const bool real = rr < rows;
             const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
@@ -321,29 +337,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             {
                 const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)node * a.q_nb_node + h * kD);
                 float am = 0.0f;
-                float4 v[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float4 o = real ? q[8 * (g ^ 1) + c] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    v[c] = real ? q[8 * g + c] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    am = max3(am, fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
-                    am = max3(am, fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w)));
+                if (real) {
+#pragma unroll 4
+                    for (int c = 0; c < 16; ++c) {
+                        const float4 v = q[c];
+                        am = max3(am, fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+                    }
                 }
                 const int ex = dtc::norm_exp(am);
-                const float sc = pow2f(ex);
-                rs = pow2f(-ex) * a.scale_log2;
+                const float sc = a.scale_log2 < 0.0f ? -pow2f(ex) : pow2f(ex);
+                rs = pow2f(-ex) * fabsf(a.scale_log2);
                 // nothing reads the last run's Q, or its exchanged rows, any more
                 if (r.i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t wh[4], wl[4];
-                    split2(v[2 * c].x * sc, v[2 * c].y * sc, wh[0], wl[0]);
-                    split2(v[2 * c].z * sc, v[2 * c].w * sc, wh[1], wl[1]);
-                    split2(v[2 * c + 1].x * sc, v[2 * c + 1].y * sc, wh[2], wl[2]);
-                    split2(v[2 * c + 1].z * sc, v[2 * c + 1].w * sc, wh[3], wl[3]);
-                    const uint32_t at = tc::sw128_offset(row, 4 * g + c);
-                    *reinterpret_cast<uint4*>(qhi + at) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-                    *reinterpret_cast<uint4*>(qlo + at) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+#pragma unroll 1
+                for (int c = 4 * g; c < 4 * g + 4; ++c) {
+                    const float4 u = real ? q[2 * c] : make_float4(0.f, 0.f, 0.f, 0.f), v = real ? q[2 * c + 1] : u;
+                    uint4 wh, wl;
+                    split2(u.x * sc, u.y * sc, wh.x, wl.x);
+                    split2(u.z * sc, u.w * sc, wh.y, wl.y);
+                    split2(v.x * sc, v.y * sc, wh.z, wl.z);
+                    split2(v.z * sc, v.w * sc, wh.w, wl.w);
+                    const uint32_t at = tc::sw128_offset(row, c);
+                    *reinterpret_cast<uint4*>(qhi + at) = wh;
+                    *reinterpret_cast<uint4*>(qlo + at) = wl;
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(&B->q_full);
@@ -353,6 +369,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             for (int d = 0; d < 32; ++d) O[d] = make_float2(0.f, 0.f);
             float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 0.0f;
             bool pending = false;  // a tile's output still to be added, times vs_last
+            bool spoiled = false;  // the row sees a drafted value that is not finite
             auto add_output = [&]() {
                 uint32_t o0[32], o1[32];
                 tc::tmem_ld32(ot, o0);
@@ -378,19 +395,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                     uint32_t sv[32];
                     tc::tmem_ld32(sp, sv);
                     const float2 ex = B->exps[(j - lo) % kTcExps];
-                    const float rst = rs * ex.x;
+                    const float rst = fmaxf(rs * ex.x, 1e-37f);  // above 0, so that what is masked stays -infinity
                     const bool masked = draft || count < kTcTile;
                     tc::tmem_ld_wait();
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
-                        float2 x[16];
-                        {
-                            const float2 f = make_float2(rst, rst), b = make_float2(-base, -base);
-#pragma unroll
-                            for (int d = 0; d < 16; ++d)
-                                x[d] = ffma2(make_float2(__uint_as_float(sv[2 * d]), __uint_as_float(sv[2 * d + 1])), f, b);
-                        }
-                        tc::tmem_ld32(sp + 32 * min(c + 1, 3), sv);  // under way during this chunk's arithmetic
                         if (masked) {
                             const int left = count - 32 * c;
                             uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
@@ -400,39 +409,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                 else if (node < j0 + 31) bits &= node < j0 ? 0u : (2u << (node - j0)) - 1u;
                             }
 #pragma unroll
-                            for (int d = 0; d < 16; ++d) {
-                                if (!((bits >> (2 * d)) & 1u)) x[d].x = -INFINITY;
-                                if (!((bits >> (2 * d + 1)) & 1u)) x[d].y = -INFINITY;
-                            }
+                            for (int d = 0; d < 32; ++d)
+                                if (!((bits >> d) & 1u)) sv[d] = 0xff800000u;
                         }
+                        // the largest score of the row's 32 keys (rst > 0, so that of S)
                         float mx;
                         {
                             float m4[4];
 #pragma unroll
-                            for (int u = 0; u < 4; ++u)
-                                m4[u] = max3(max3(fmaxf(x[4 * u].x, x[4 * u].y), x[4 * u + 1].x, x[4 * u + 1].y), max3(x[4 * u + 2].x, x[4 * u + 2].y, x[4 * u + 3].x),
-                                             x[4 * u + 3].y);
-                            mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+                            for (int u = 0; u < 4; ++u) {
+                                const uint32_t* w = sv + 8 * u;
+                                m4[u] = max3(max3(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), __uint_as_float(w[2]), __uint_as_float(w[3])),
+                                             max3(__uint_as_float(w[4]), __uint_as_float(w[5]), __uint_as_float(w[6])), __uint_as_float(w[7]));
+                            }
+                            mx = fmaf(max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]), rst, -base);
                         }
                         if (__any_sync(0xffffffffu, mx > thr)) {
-                            float f = 1.0f, up = 0.0f;
+                            float f = 1.0f;
                             if (mx > thr) {
-                                up = mx - kTcOffs;
+                                const float up = mx - kTcOffs;
                                 f = thr == -INFINITY ? 0.0f : fast_exp2(-up);
                                 base += up;
                                 thr = kLazy + kTcOffs;
                                 l *= f;
                                 vs_last *= f;
                             }
-                            const float2 f2 = make_float2(f, f), u2 = make_float2(-up, -up);
+                            const float2 f2 = make_float2(f, f);
 #pragma unroll
                             for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
-#pragma unroll
-                            for (int d = 0; d < 16; ++d) x[d] = add2(x[d], u2);
-                            if (c) {
-                                tc::tmem_st_wait();
-                                tc::tmem_ld_wait();
-                            }
+                            if (c) tc::tmem_st_wait();
 #pragma unroll 1
                             for (int e = 0; e < 2 * c; ++e) {  // this tile's P so far, 16 keys at a time
                                 uint32_t ph[8], pl[8];
@@ -450,6 +455,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                 tc::tmem_st8(at + 16, pl);
                             }
                         }
+                        float2 x[16];
+                        {
+                            const float2 f = make_float2(rst, rst), b = make_float2(-base, -base);
+#pragma unroll
+                            for (int d = 0; d < 16; ++d)
+                                x[d] = ffma2(make_float2(__uint_as_float(sv[2 * d]), __uint_as_float(sv[2 * d + 1])), f, b);
+                        }
+                        tc::tmem_ld32(sp + 32 * min(c + 1, 3), sv);  // under way during this chunk's arithmetic
                         float2 l0 = make_float2(0.f, 0.f), l1 = l0;
 #pragma unroll
                         for (int d = 0; d < 16; d += 2) {
@@ -463,25 +476,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                         l0 = add2(l0, l1);
                         l += l0.x + l0.y;
                         if (draft) {
-                            // keys whose V is not finite have zeros in the tile; rows that see one add it here
-                            uint32_t bad = B->bad[(j - lo) % kTcExps][c];
-                            while (bad) {
-                                const int b = __ffs(bad) - 1;
-                                bad &= bad - 1;
-                                float pb = 0.0f;
+                            // keys whose V is not finite have zeros in the tile; a row that sees one is NaN in the end
+                            const uint32_t bad = B->bad[(j - lo) % kTcExps][c];
+                            if (bad) {
 #pragma unroll
-                                for (int d = 0; d < 16; ++d) {
-                                    if (2 * d == b) pb = x[d].x;
-                                    if (2 * d + 1 == b) pb = x[d].y;
-                                }
-                                if (pb == 0.0f) continue;
-                                const uint8_t* vr = a.vd + (int64_t)r.s * a.vd_nb2 + (int64_t)(p0 + 32 * c + b) * a.vd_nb1 + r.kvh * sliceV;
-#pragma unroll
-                                for (int d = 0; d < 32; ++d) {
-                                    const uint8_t* vg = vr + (d >> 4) * group_bytes(VT);
-                                    O[d].x = fmaf(pb, dequant_elem<VT>(vg, (2 * d) & 31), O[d].x);
-                                    O[d].y = fmaf(pb, dequant_elem<VT>(vg, (2 * d + 1) & 31), O[d].y);
-                                }
+                                for (int d = 0; d < 16; ++d)
+                                    spoiled |= ((bad >> (2 * d) & 1u) && x[d].x != 0.0f) || ((bad >> (2 * d + 1) & 1u) && x[d].y != 0.0f);
                             }
                         }
                         uint32_t pv[32];
@@ -519,7 +519,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             if (g == 1) {
 #pragma unroll
                 for (int c = 0; c < 16; ++c) xch[c ^ (row & 7)] = make_float4(O[2 * c].x, O[2 * c].y, O[2 * c + 1].x, O[2 * c + 1].y);
-                *mls = make_float2(m_mine, l);
+                mls[0] = make_float2(m_mine, l);
+                mls[kTcRows] = make_float2(spoiled ? 1.0f : 0.0f, 0.0f);
             }
             asm volatile("bar.sync 3, 256;" ::: "memory");
             if (g == 0 && real) {
@@ -528,18 +529,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 const float f0 = m_mine == -INFINITY ? 0.0f : exp2f(m_mine - M), f1 = other.x == -INFINITY ? 0.0f : exp2f(other.x - M);
                 const float sum = (m_mine == -INFINITY ? 0.0f : f0 * l) + (other.x == -INFINITY ? 0.0f : f1 * other.y);
                 const bool whole = r.end - r.i == r.T, seen = M != -INFINITY;
-                const float inv = !whole ? 1.0f : seen ? 1.0f / sum : 0.0f;
+                spoiled |= mls[kTcRows].x != 0.0f;
+                const float inv = spoiled ? __int_as_float(0x7fc00000) : !whole ? 1.0f : seen ? 1.0f / sum : 0.0f;
                 const int64_t slot = (int64_t)(2 * blockIdx.x + (r.i == lo ? 0 : 1)) * kTcRows + row;
                 float4* dst = reinterpret_cast<float4*>(whole ? a.out + orow : ta.ws_o + slot * kD);
-                const float g0 = f0 * inv, g1 = f1 * inv;
+                const float2 g0 = make_float2(f0 * inv, f0 * inv), g1 = make_float2(f1 * inv, f1 * inv);
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
                     const float4 w = xch[c ^ (row & 7)];
-                    // (what has no weight is left out: it may not be finite)
-                    float4 o = g0 != 0.0f ? make_float4(g0 * O[2 * c].x, g0 * O[2 * c].y, g0 * O[2 * c + 1].x, g0 * O[2 * c + 1].y)
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (g1 != 0.0f) o = make_float4(fmaf(g1, w.x, o.x), fmaf(g1, w.y, o.y), fmaf(g1, w.z, o.z), fmaf(g1, w.w, o.w));
-                    dst[c] = o;
+                    const float2 u = ffma2(g1, make_float2(w.x, w.y), mul2(g0, O[2 * c])), v = ffma2(g1, make_float2(w.z, w.w), mul2(g0, O[2 * c + 1]));
+                    dst[c] = make_float4(u.x, u.y, v.x, v.y);
                 }
                 if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + slot * 2) = make_float2(M, sum);
                 else if (a.lse)
@@ -594,9 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
         };
         // the runs of the tile whose copies start and of the tile that is finished
-        Run ri, rc;
-        ri.start(a, tab, lo, hi);
-        rc = ri;
+        Run ri = r, rc = r;
         int ii = lo;
         bool ok = true;
         auto issue = [&](int n) {        // copies of the CTA's tile n (list entry ii)
@@ -623,13 +620,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             cp_async_commit();
         };
         constexpr int kAhead = NK + NV == 2 ? kSt - 2 : 1;  // tiles whose copies run ahead of the finished one
-        for (int n = 0; n < kAhead; ++n) issue(n);
-        for (int n = 0; lo + n < hi; ++n) {
-            cp_async_wait<kAhead - 1>();
-            // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
-            if (!fp::prod_bar_and(4, 128, ok)) break;
+#pragma unroll 1
+        for (int n = -kAhead; lo + n < hi; ++n) {
+            if (n >= 0) {
+                cp_async_wait<kAhead - 1>();
+                // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
+                if (!fp::prod_bar_and(4, 128, ok)) break;
+            }
             // raw copies of the next tile first; copies into a stage may have to wait for it, so they come last
             if constexpr (NK + NV == 4) issue(n + kAhead);
+            if (n >= 0) {
             if (lo + n == rc.end) rc.next(a, tab, hi);
             bool draft;
             int p0, count;
@@ -729,6 +729,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 fence_proxy_async_smem();
                 mbar_arrive(&B->v_full[st]);
             }
+            }
             if constexpr (NK + NV < 4) issue(n + kAhead);
         }
         cp_async_wait<0>();
@@ -745,8 +746,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             uint32_t n_run = 0;
             int n = 0, st = 0, buf = 0;
             uint32_t use = 0, turn = 0;  // n / kSt, n / 3
-            Run r;
-            for (r.start(a, tab, lo, hi); ok && r.i < hi; r.next(a, tab, hi), ++n_run) {
+            for (; ok && r.i < hi; r.next(a, tab, hi), ++n_run) {
                 ok = tc_wait(&B->q_full, n_run & 1, &B->err, a.status, 37);
                 for (int j = r.i; ok && j < r.end; ++j, ++n) {
                     ok = tc_wait(&B->k_full[st], use & 1, &B->err, a.status, 38);
