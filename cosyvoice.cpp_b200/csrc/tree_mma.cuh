@@ -138,6 +138,12 @@ __device__ __forceinline__ void store_block(uint8_t* tile, int key, int blk, con
             make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
 }
 
+// Block BLK of a head's raw slice, which starts at a multiple of 4 bytes (so the quants' alignment is known).
+template <int T, int BLK>
+__device__ __forceinline__ void convert_block(const uint8_t* slice, uint32_t (&w)[16], float& d, float& m) {
+    dtc::convert_group<T>(static_cast<const uint8_t*>(__builtin_assume_aligned(slice, 4)) + BLK * group_bytes(T), w, d, m);
+}
+
 __device__ __forceinline__ bool f16x2_special(uint32_t w) {
     return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
 }

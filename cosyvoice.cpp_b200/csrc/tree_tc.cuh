@@ -35,8 +35,8 @@ namespace tree {
 constexpr int kTcTile = 128;
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 16 * 32;
-// Registers of a thread by role: launched with 128; 256 * 168 + 128 * 88 + 128 * 80 <= 512 * 128.
-constexpr int kTcRegsSoftmax = 168, kTcRegsProducer = 88, kTcRegsIssuer = 80;
+// Registers of a thread by role: launched with 128; 256 * 168 + 128 * 96 + 128 * 80 <= 512 * 128.
+constexpr int kTcRegsSoftmax = 168, kTcRegsProducer = 96, kTcRegsIssuer = 80;
 static_assert(256 * kTcRegsSoftmax + 128 * kTcRegsProducer + 128 * kTcRegsIssuer <= 65536, "the block's registers");
 constexpr int kTcMaxSeq = 1024;       // prefix table in shared memory
 constexpr int kTcExps = 8;            // tiles whose scales may be in flight
@@ -53,7 +53,7 @@ struct TcArgs {
 };
 
 struct TcBars {
-    uint64_t k_full[4], v_full[4], k_empty[4], v_empty[4];  // by stage
+    uint64_t k_full[5], v_full[5], k_empty[5], v_empty[5];  // by stage
     uint64_t q_full;
     uint64_t s_full[3], p_full[3], s_free[3];               // by S buffer
     uint64_t o_full[2];                                     // by group
@@ -68,7 +68,7 @@ struct TcBars {
 template <int KT, int VT>
 struct TcShape {
     static constexpr int NK = KT == kF16 ? 1 : 2, NV = VT == kF16 ? 1 : 2;  // pieces of an operand
-    static constexpr int kStages = NK + NV == 2 ? 4 : NK + NV == 3 ? 3 : 2;
+    static constexpr int kStages = NK + NV == 2 ? 5 : NK + NV == 3 ? 3 : 2;
     static constexpr int kStage = (NK + NV) * kTcTileBytes;
     static constexpr int rawK = NK == 1 ? 0 : kTcTile * raw_stride(KT), rawV = NV == 1 ? 0 : kTcTile * raw_stride(VT);
     static constexpr int kQ = 0;                       // Q hi, Q lo; then the groups' halves at a run's end
@@ -698,13 +698,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             if constexpr (NK == 2) {
                 if (use > 0) ok = ok && tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 35);
                 if (ok) {
-#pragma unroll 1
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t w[16];
-                        float d, m;
-                        dtc::convert_group<KT>(rawk + key * raw_stride(KT) + b * group_bytes(KT), w, d, m);
-                        split_block<KT>(tiles, tiles + kTcTileBytes, key, b, w, d * fk, m * fk);
-                    }
+                    uint32_t w0[16], w1[16];
+                    float d0, m0, d1, m1;
+                    convert_block<KT, 0>(rawk + key * raw_stride(KT), w0, d0, m0);
+                    convert_block<KT, 1>(rawk + key * raw_stride(KT), w1, d1, m1);
+                    split_block<KT>(tiles, tiles + kTcTileBytes, key, 0, w0, d0 * fk, m0 * fk);
+                    split_block<KT>(tiles, tiles + kTcTileBytes, key, 1, w1, d1 * fk, m1 * fk);
                 }
             }
             if (ok) {
@@ -715,14 +714,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 if (use > 0) ok = ok && tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 36);
                 if (ok) {
                     const bool drop = draft && bad;
-#pragma unroll 1
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t w[16];
-                        float d, m;
-                        dtc::convert_group<VT>(rawv + key * raw_stride(VT) + b * group_bytes(VT), w, d, m);
-                        split_block<VT>(tiles + NK * kTcTileBytes, tiles + (NK + 1) * kTcTileBytes, key, b, w, drop ? 0.0f : d * fv,
-                                        drop ? 0.0f : m * fv);
-                    }
+                    uint32_t w0[16], w1[16];
+                    float d0, m0, d1, m1;
+                    convert_block<VT, 0>(rawv + key * raw_stride(VT), w0, d0, m0);
+                    convert_block<VT, 1>(rawv + key * raw_stride(VT), w1, d1, m1);
+                    uint8_t* vt = tiles + NK * kTcTileBytes;
+                    split_block<VT>(vt, vt + kTcTileBytes, key, 0, w0, drop ? 0.0f : d0 * fv, drop ? 0.0f : m0 * fv);
+                    split_block<VT>(vt, vt + kTcTileBytes, key, 1, w1, drop ? 0.0f : d1 * fv, drop ? 0.0f : m1 * fv);
                 }
             }
             if (ok) {
