@@ -1,46 +1,22 @@
 // kv_scores.cu -- cvattn_kv_scores: the attention weight of each cached position.
-#include "internal.h"
-#include "common.cuh"
+#include "kv_scores.cuh"
 
 namespace cvattn {
 namespace kvscore {
 
-constexpr int kD = 64;
 constexpr int kTile = 64;   // keys per CTA
 constexpr int kRows = 32;   // (token, head) rows at a time
 constexpr int kPad = kD + 4;
 
-struct Args {
-    const float* q;
-    int64_t q_nb_node, q_nb_seq;
-    const float* lse;
-    const uint8_t* k;
-    int64_t k_nb1, k_nb2;
-    const uint64_t* k_seq_ptrs;
-    const int32_t *rows, *n_rows, *kv_len;
-    const float* scores;
-    float* out;
-    int64_t nb_head, nb_seq;
-    int k_type, n_seq, n_q_rows, max_rows, Hq, Hkv, G, max_kv_len;
-    float scale_log2, decay;
-    int* status;
-};
-
-// s_j = decay s_j + sum over rows of exp2(c q.k_j - lse log2 e): the row sums are
-// known, so a key's column needs no second pass and no exchange between CTAs.
+// f32 caches, on the CUDA cores: a thread owns 4 rows x 4 keys of a 32 x 64 tile.
 __global__ void __launch_bounds__(128) scores_f32_kernel(const __grid_constant__ Args a) {
     __shared__ float4 qs4[kRows][kPad / 4], ks4[kTile][kPad / 4];
     __shared__ float ls[kRows], red[8][kTile];
     __shared__ int far[kRows];  // keys that the row sees
     const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
     const int s = blockIdx.z, kvh = blockIdx.y, p0 = blockIdx.x * kTile;
-    const int L = a.kv_len[s], n = a.n_rows ? a.n_rows[s] : a.max_rows;
-    const bool odd = a.k_seq_ptrs && (a.k_seq_ptrs[s] & (a.k_type == kF32 ? 3 : 1));
-    if (L < 0 || L > a.max_kv_len || n < 0 || n > a.max_rows || n > L || odd) {
-        if (tid == 0) record_status(a.status, kStatusBadLength);
-        return;
-    }
-    if (p0 >= L) return;
+    int L, n;
+    if (!lens_of(a, s, L, n, tid == 0) || p0 >= L) return;
     const int count = min(kTile, L - p0);
     const uint8_t* kb = a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[s]) : a.k + (int64_t)s * a.k_nb2;
     float* ks = reinterpret_cast<float*>(ks4);
@@ -145,6 +121,15 @@ cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params&
     a.scale_log2 = p.scale * 1.4426950408889634f;
     a.decay = p.decay;
     a.status = status;
+    switch (a.k_type) {
+    case kF16: return launch_mma_for_k<kF16>(stream, a);
+    case kQ4_0: return launch_mma_for_k<kQ4_0>(stream, a);
+    case kQ4_1: return launch_mma_for_k<kQ4_1>(stream, a);
+    case kQ5_0: return launch_mma_for_k<kQ5_0>(stream, a);
+    case kQ5_1: return launch_mma_for_k<kQ5_1>(stream, a);
+    case kQ8_0: return launch_mma_for_k<kQ8_0>(stream, a);
+    default: break;
+    }
     const dim3 grid((unsigned)((a.max_kv_len + kTile - 1) / kTile), (unsigned)a.Hkv, (unsigned)a.n_seq);
     scores_f32_kernel<<<grid, 128, 0, stream>>>(a);
     return cudaGetLastError();

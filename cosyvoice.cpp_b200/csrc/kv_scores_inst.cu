@@ -1,0 +1,34 @@
+// kv_scores_inst.cu -- the attention score MMA kernels of one K type (CVATTN_KT).
+#include <atomic>
+
+#include "kv_scores.cuh"
+
+namespace cvattn {
+namespace kvscore {
+
+template <int KT, int NT>
+static cudaError_t run(cudaStream_t stream, const Args& a) {
+    const auto fn = scores_mma_kernel<KT, NT>;
+    constexpr int smem = Smem<KT, NT>::bytes, keys = Smem<KT, NT>::kKeys;
+    static std::atomic<bool> allowed[64];  // dynamic shared memory granted, per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !allowed[dev].load(std::memory_order_relaxed)) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) allowed[dev].store(true, std::memory_order_relaxed);
+    }
+    fn<<<dim3((unsigned)((a.max_kv_len + keys - 1) / keys), (unsigned)a.Hkv, (unsigned)a.n_seq), kThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+template <>
+cudaError_t launch_mma_for_k<CVATTN_KT>(cudaStream_t stream, const Args& a) {
+    // Many rows share more of each Q fragment with 32 keys a warp; few rows (and few keys) fill more SMs with 16.
+    const int64_t ctas = (int64_t)a.n_seq * a.Hkv * ((a.max_kv_len + 255) / 256);
+    return a.max_rows * a.G > 64 && ctas >= 296 ? run<CVATTN_KT, 4>(stream, a) : run<CVATTN_KT, 2>(stream, a);
+}
+
+}  // namespace kvscore
+}  // namespace cvattn
