@@ -8,6 +8,8 @@ namespace evict {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxKeySlots = 40 * 1024;  // 160 KB of keys
+constexpr int kFusedMoves = 256;         // up to so many rows a head the selecting CTA moves them itself: one launch
 constexpr int kLayersPerLaunch = 32;  // layer addresses that travel as kernel parameters
 
 struct Args {
@@ -24,6 +26,8 @@ struct Args {
     int layers, Hkv, max_kv_len, budget, n_sink, n_recent;
     int32_t* ws;     // per (layer, seq, head): move count (padded to 4), then `moves` destinations, then sources
     int moves;       // most moves of one head
+    int key_slots;   // slots whose keys fit shared memory
+    bool fused;      // the selecting CTA moves the rows too
     int* status;
 };
 
@@ -50,63 +54,113 @@ __device__ __forceinline__ uint32_t rank_key(float v, bool safe) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One CTA per (head, sequence, layer).  The budget-th largest key is found by a
-// radix select over 8 bits at a time; of the slots that equal it, the lowest stay.
-// Each warp owns a run of slots, so ranks in slot order are ballots plus one
-// prefix over the warps.
+// Bytes of one head of the listed rows, in units of 4 bytes where everything is aligned to them, else 2.
+template <typename T>
+__device__ __forceinline__ void move_rows(uint8_t* cache, int64_t nb1, int slice, const int32_t* dst, const int32_t* src,
+                                          int i0, int i1) {
+    const int units = slice / (int)sizeof(T);
+    for (int i = i0 * units + threadIdx.x; i < i1 * units; i += blockDim.x) {
+        const int m = i / units, u = i - m * units;
+        reinterpret_cast<T*>(cache + (int64_t)dst[m] * nb1)[u] = reinterpret_cast<const T*>(cache + (int64_t)src[m] * nb1)[u];
+    }
+}
+
+// K and V of one head: the rows dst[i] <- src[i], i0 <= i < i1.
+__device__ __forceinline__ void move_head(const Args& a, int layer, int s, int kvh, const int32_t* dst, const int32_t* src, int i0, int i1) {
+    uint8_t* k = a.k[layer] + (int64_t)s * a.k_nb2 + (int64_t)kvh * a.k_slice;
+    uint8_t* v = a.v[layer] + (int64_t)s * a.v_nb2 + (int64_t)kvh * a.v_slice;
+    if (((reinterpret_cast<uintptr_t>(k) | (uintptr_t)a.k_nb1) & 3) == 0) move_rows<uint32_t>(k, a.k_nb1, a.k_slice, dst, src, i0, i1);
+    else move_rows<uint16_t>(k, a.k_nb1, a.k_slice, dst, src, i0, i1);
+    if (((reinterpret_cast<uintptr_t>(v) | (uintptr_t)a.v_nb1) & 3) == 0) move_rows<uint32_t>(v, a.v_nb1, a.v_slice, dst, src, i0, i1);
+    else move_rows<uint16_t>(v, a.v_nb1, a.v_slice, dst, src, i0, i1);
+}
+
+// One CTA per (head, sequence, layer).  The keys are formed once, in shared memory
+// as far as they fit.  The budget-th largest is found by a radix select over 8 bits
+// at a time; of the slots that equal it, the lowest stay.  Each warp owns a run of
+// slots, so ranks in slot order are ballots plus one prefix over the warps.
 __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_constant__ Args a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t sh_prefix, sh_need;
-    __shared__ int wsum[3][kWarps];
+    extern __shared__ uint32_t keys[];
+    __shared__ uint32_t hist[2][256];
+    __shared__ uint32_t sh_prefix;
+    __shared__ int sh_need, wsum[3][kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int kvh = blockIdx.x, s = blockIdx.y, layer = blockIdx.z;
     const Seq x = seq_of(a, s);
     int32_t* ws = a.ws + (((int64_t)layer * gridDim.y + s) * gridDim.x + kvh) * (2 * (int64_t)a.moves + 4);
-    if (!x.ok) {
-        if (tid == 0) {
-            record_status(a.status, kStatusBadLength);
-            ws[0] = 0;
-            if (a.kv_len_out && kvh == 0 && layer == 0) a.kv_len_out[s] = x.L;
-        }
-        return;
+    if (tid == 0) {
+        if (!x.ok) record_status(a.status, kStatusBadLength);
+        if (a.kv_len_out && kvh == 0 && layer == 0) a.kv_len_out[s] = x.ok ? min(x.L, a.budget) : x.L;
+        if (!x.ok || x.L <= a.budget) ws[0] = 0;
     }
-    if (tid == 0 && a.kv_len_out && kvh == 0 && layer == 0) a.kv_len_out[s] = min(x.L, a.budget);
+    if (!x.ok) return;
     const int64_t base = (int64_t)layer * a.nb_layer + (int64_t)s * a.nb_seq + (int64_t)kvh * a.nb_head;
     const float* sc = a.scores + base;
     const int32_t* pos = a.pos ? a.pos + base : nullptr;
     auto token = [&](int j) { return j < x.kept ? pos[j] : x.total - x.L + j; };
-    auto key_at = [&](int j) {
-        const int t = token(j);
-        return rank_key(sc[j], t < a.n_sink || t >= x.total - a.n_recent);
-    };
     if (x.L <= a.budget) {
-        if (tid == 0) ws[0] = 0;
         for (int j = tid; j < x.L; j += kThreads) {
             a.pos_out[base + j] = token(j);
             a.scores_out[base + j] = sc[j];
         }
         return;
     }
+    auto form = [&](int j) {
+        const int t = token(j);
+        return rank_key(sc[j], t < a.n_sink || t >= x.total - a.n_recent);
+    };
+    auto key_at = [&](int j) { return j < a.key_slots ? keys[j] : form(j); };
+    hist[tid >> 8][tid & 255] = 0;
+    __syncthreads();
+    const int here = min(x.L, a.key_slots);
+#pragma unroll 4
+    for (int j = tid; j < here; j += kThreads) {
+        const uint32_t u = form(j);
+        keys[j] = u;
+        atomicAdd(&hist[0][u >> 24], 1u);
+    }
+    for (int j = here + tid; j < x.L; j += kThreads) atomicAdd(&hist[0][form(j) >> 24], 1u);
     uint32_t prefix = 0;
     int need = a.budget;  // how many of the keys that match the prefix stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+#pragma unroll 1
+    for (int shift = 24;; shift -= 8) {
+        uint32_t* now = hist[(shift >> 3) & 1 ? 0 : 1];   // 24, 8: hist[0]; 16, 0: hist[1]
+        uint32_t* next = hist[(shift >> 3) & 1 ? 1 : 0];
         __syncthreads();
-        const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-        for (int j = tid; j < x.L; j += kThreads) {
-            const uint32_t u = key_at(j);
-            if ((u & above) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int left = need, b = 255;
-            while (b > 0 && (int)hist[b] < left) left -= (int)hist[b--];
-            sh_prefix = prefix | ((uint32_t)b << shift);
-            sh_need = (uint32_t)left;
+        if (warp == 0) {
+            // lane i: bins 255 - 8 i downwards; the bin in which the need-th largest key lies
+            uint32_t c[8], own = 0;
+#pragma unroll
+            for (int b = 0; b < 8; ++b) own += c[b] = now[255 - 8 * lane - b];
+            uint32_t incl = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            uint32_t before = incl - own;
+            if (before < (uint32_t)need && incl >= (uint32_t)need) {
+                int b = 0;
+#pragma unroll
+                for (; b < 7; ++b) {
+                    if (before + c[b] >= (uint32_t)need) break;
+                    before += c[b];
+                }
+                sh_prefix = prefix | ((uint32_t)(255 - 8 * lane - b) << shift);
+                sh_need = need - (int)before;
+            }
+        } else {
+            for (int i = tid - 32; i < 256; i += kThreads - 32) next[i] = 0;
         }
         __syncthreads();
         prefix = sh_prefix;
-        need = (int)sh_need;
+        need = sh_need;
+        if (shift == 0) break;
+        const uint32_t above = 0xffffffffu << shift;
+        for (int j = tid; j < x.L; j += kThreads) {
+            const uint32_t u = key_at(j);
+            if ((u & above) == prefix) atomicAdd(&next[(u >> (shift - 8)) & 255], 1u);
+        }
     }
     // slots of this warp: [j0, j1)
     const int per = ((x.L + kWarps - 1) / kWarps + 31) & ~31;
@@ -165,7 +219,9 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
         m0 += __popc(mb);
     }
     __syncthreads();
+    griddep_launch_dependents();
     // the lists are complete: rows that stay, then rows that move, then the cleared tail
+#pragma unroll 4
     for (int j = tid; j < a.budget; j += kThreads) {
         a.pos_out[base + j] = token(j);
         if (a.scores_out != a.scores) a.scores_out[base + j] = sc[j];
@@ -175,19 +231,9 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
         a.pos_out[base + dst[i]] = token(src[i]);
         a.scores_out[base + dst[i]] = sc[src[i]];
     }
+    if (a.fused) move_head(a, layer, s, kvh, dst, src, 0, total);
     __syncthreads();
     for (int j = a.budget + tid; j < x.L; j += kThreads) a.scores_out[base + j] = 0.0f;
-}
-
-// Bytes of one head of the listed rows, in units of 4 bytes where everything is aligned to them, else 2.
-template <typename T>
-__device__ __forceinline__ void move_rows(uint8_t* cache, int64_t nb1, int slice, const int32_t* dst, const int32_t* src,
-                                          int i0, int i1) {
-    const int units = slice / (int)sizeof(T);
-    for (int i = i0 * units + threadIdx.x; i < i1 * units; i += blockDim.x) {
-        const int m = i / units, u = i - m * units;
-        reinterpret_cast<T*>(cache + (int64_t)dst[m] * nb1)[u] = reinterpret_cast<const T*>(cache + (int64_t)src[m] * nb1)[u];
-    }
 }
 
 constexpr int kMoveChunk = 64;  // rows of one head per CTA
@@ -195,15 +241,11 @@ constexpr int kMoveChunk = 64;  // rows of one head per CTA
 __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ Args a, int n_seq) {
     const int kvh = blockIdx.y % a.Hkv, s = blockIdx.y / a.Hkv, layer = blockIdx.z;
     const int32_t* ws = a.ws + (((int64_t)layer * n_seq + s) * a.Hkv + kvh) * (2 * (int64_t)a.moves + 4);
+    griddep_wait();
     const int n = ws[0], i0 = blockIdx.x * kMoveChunk, i1 = min(n, i0 + kMoveChunk);
     if (i0 >= i1) return;
     const int32_t *dst = ws + 4, *src = dst + a.moves;
-    uint8_t* k = a.k[layer] + (int64_t)s * a.k_nb2 + (int64_t)kvh * a.k_slice;
-    uint8_t* v = a.v[layer] + (int64_t)s * a.v_nb2 + (int64_t)kvh * a.v_slice;
-    if (((reinterpret_cast<uintptr_t>(k) | (uintptr_t)a.k_nb1) & 3) == 0) move_rows<uint32_t>(k, a.k_nb1, a.k_slice, dst, src, i0, i1);
-    else move_rows<uint16_t>(k, a.k_nb1, a.k_slice, dst, src, i0, i1);
-    if (((reinterpret_cast<uintptr_t>(v) | (uintptr_t)a.v_nb1) & 3) == 0) move_rows<uint32_t>(v, a.v_nb1, a.v_slice, dst, src, i0, i1);
-    else move_rows<uint16_t>(v, a.v_nb1, a.v_slice, dst, src, i0, i1);
+    move_head(a, layer, s, kvh, dst, src, i0, i1);
 }
 
 // kv_len_out that shares memory with a length read above: after every reader is done.
@@ -254,13 +296,26 @@ cudaError_t launch_kv_evict(cudaStream_t stream, const cvattn_kv_evict_params& p
         a.moves = moves;
         a.ws = static_cast<int32_t*>(p.workspace) + (int64_t)l0 * p.n_seq * Hkv * (2 * (int64_t)moves + 4);
         a.status = status;
-        evict_select_kernel<<<dim3((unsigned)Hkv, (unsigned)p.n_seq, (unsigned)n), kThreads, 0, stream>>>(a);
-        cudaError_t e = cudaGetLastError();
+        a.key_slots = p.max_kv_len < kMaxKeySlots ? p.max_kv_len : kMaxKeySlots;
+        a.fused = moves <= kFusedMoves;
+        const int smem = a.key_slots * 4;
+        cudaError_t e = cudaSuccess;
+        if (smem > 40 * 1024) e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeySlots * 4);
         if (e != cudaSuccess) return e;
-        if (moves) {
-            evict_move_kernel<<<dim3((unsigned)((moves + kMoveChunk - 1) / kMoveChunk), (unsigned)(Hkv * p.n_seq), (unsigned)n), 256, 0,
-                                stream>>>(a, p.n_seq);
-            e = cudaGetLastError();
+        evict_select_kernel<<<dim3((unsigned)Hkv, (unsigned)p.n_seq, (unsigned)n), kThreads, smem, stream>>>(a);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        if (!a.fused) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)((moves + kMoveChunk - 1) / kMoveChunk), (unsigned)(Hkv * p.n_seq), (unsigned)n);
+            cfg.blockDim = dim3(256);
+            cfg.stream = stream;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            e = cudaLaunchKernelEx(&cfg, evict_move_kernel, a, p.n_seq);
             if (e != cudaSuccess) return e;
         }
     }

@@ -112,6 +112,11 @@ __global__ void __launch_bounds__(kThreads, NT == 2 ? 3 : 2) scores_mma_kernel(c
 #pragma unroll
     for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = 0.0f;
     const int kw = warp * 8 * NT;      // this warp's first key
+    // the old scores of the two keys that this lane will write (row lane t for key tile t)
+    const int key_out = kw + 8 * gid + 2 * tig;
+    const int64_t at_out = (int64_t)s * a.nb_seq + (int64_t)kvh * a.nb_head + p0 + key_out;
+    const bool w0 = gid < NT && key_out < count, w1 = gid < NT && key_out + 1 < count;
+    const float old0 = w0 ? a.scores[at_out] : 0.0f, old1 = w1 ? a.scores[at_out + 1] : 0.0f;
 
     for (int base = 0; base < total; base += kRowTiles * 16) {
         if (base) __syncthreads();     // every warp is done with the last rows
@@ -246,6 +251,8 @@ __global__ void __launch_bounds__(kThreads, NT == 2 ? 3 : 2) scores_mma_kernel(c
             }
         }
     }
+    tree::cp_async_wait<0>();  // (no rows: nothing has waited for the copies)
+    float v0 = 0.0f, v1 = 0.0f;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -254,12 +261,10 @@ __global__ void __launch_bounds__(kThreads, NT == 2 ? 3 : 2) scores_mma_kernel(c
             v += __shfl_xor_sync(0xffffffffu, v, 4);
             v += __shfl_xor_sync(0xffffffffu, v, 8);
             v += __shfl_xor_sync(0xffffffffu, v, 16);
-            const int key = kw + 8 * t + 2 * tig + e;
-            if (gid == (t & 7) && key < count) {
-                const int64_t at = (int64_t)s * a.nb_seq + (int64_t)kvh * a.nb_head + p0 + key;
-                a.out[at] = fmaf(a.decay, a.scores[at], v);
-            }
+            if (gid == t) (e ? v1 : v0) = v;
         }
+    if (w0) a.out[at_out] = fmaf(a.decay, old0, v0);
+    if (w1) a.out[at_out + 1] = fmaf(a.decay, old1, v1);
 }
 
 // Launch for K type KT (kv_scores_inst.cu, one unit per K type).
