@@ -6,7 +6,7 @@
 namespace cvattn {
 namespace evict {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512;  // (1024 threads of 58 registers leave one CTA per SM: 31 us instead of 22 for 192 heads of 8192 slots)
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxKeySlots = 40 * 1024;  // 160 KB of keys
 constexpr int kFusedMoves = 256;         // up to so many rows a head the selecting CTA moves them itself: one launch
@@ -54,32 +54,39 @@ __device__ __forceinline__ uint32_t rank_key(float v, bool safe) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Bytes of one head of the listed rows, in units of 4 bytes where everything is aligned to them, else 2.
+// K and V of one head: the rows dst[i] <- src[i], i0 <= i < i1, in units of 4 bytes where everything is aligned to them,
+// else 2.  A warp takes a row, its lanes the units of the K and then of the V slice; four rows are on their way at once.
 template <typename T>
-__device__ __forceinline__ void move_rows(uint8_t* cache, int64_t nb1, int slice, const int32_t* dst, const int32_t* src,
-                                          int i0, int i1) {
-    const int units = slice / (int)sizeof(T);
-    for (int i = i0 * units + threadIdx.x; i < i1 * units; i += blockDim.x) {
-        const int m = i / units, u = i - m * units;
-        reinterpret_cast<T*>(cache + (int64_t)dst[m] * nb1)[u] = reinterpret_cast<const T*>(cache + (int64_t)src[m] * nb1)[u];
+__device__ __forceinline__ void move_rows(uint8_t* k, uint8_t* v, const Args& a, const int32_t* dst, const int32_t* src, int i0, int i1) {
+    const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    const int ku = a.k_slice / (int)sizeof(T), all = ku + a.v_slice / (int)sizeof(T);
+    for (int u = lane; u < all; u += 32) {
+        uint8_t* base = u < ku ? k + u * sizeof(T) : v + (u - ku) * sizeof(T);
+        const int64_t nb1 = u < ku ? a.k_nb1 : a.v_nb1;
+        for (int i = i0 + (threadIdx.x >> 5); i < i1; i += 4 * nw) {
+            T x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e * nw < i1) x[e] = *reinterpret_cast<const T*>(base + src[i + e * nw] * nb1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e * nw < i1) *reinterpret_cast<T*>(base + dst[i + e * nw] * nb1) = x[e];
+        }
     }
 }
-
-// K and V of one head: the rows dst[i] <- src[i], i0 <= i < i1.
 __device__ __forceinline__ void move_head(const Args& a, int layer, int s, int kvh, const int32_t* dst, const int32_t* src, int i0, int i1) {
     uint8_t* k = a.k[layer] + (int64_t)s * a.k_nb2 + (int64_t)kvh * a.k_slice;
     uint8_t* v = a.v[layer] + (int64_t)s * a.v_nb2 + (int64_t)kvh * a.v_slice;
-    if (((reinterpret_cast<uintptr_t>(k) | (uintptr_t)a.k_nb1) & 3) == 0) move_rows<uint32_t>(k, a.k_nb1, a.k_slice, dst, src, i0, i1);
-    else move_rows<uint16_t>(k, a.k_nb1, a.k_slice, dst, src, i0, i1);
-    if (((reinterpret_cast<uintptr_t>(v) | (uintptr_t)a.v_nb1) & 3) == 0) move_rows<uint32_t>(v, a.v_nb1, a.v_slice, dst, src, i0, i1);
-    else move_rows<uint16_t>(v, a.v_nb1, a.v_slice, dst, src, i0, i1);
+    const uint64_t all = reinterpret_cast<uint64_t>(k) | reinterpret_cast<uint64_t>(v) | (uint64_t)a.k_nb1 | (uint64_t)a.v_nb1;
+    if ((all & 3) == 0) move_rows<uint32_t>(k, v, a, dst, src, i0, i1);
+    else move_rows<uint16_t>(k, v, a, dst, src, i0, i1);
 }
 
 // One CTA per (head, sequence, layer).  The keys are formed once, in shared memory
 // as far as they fit.  The budget-th largest is found by a radix select over 8 bits
 // at a time; of the slots that equal it, the lowest stay.  Each warp owns a run of
 // slots, so ranks in slot order are ballots plus one prefix over the warps.
-__global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 2) evict_select_kernel(const __grid_constant__ Args a) {
     extern __shared__ uint32_t keys[];
     __shared__ uint32_t hist[2][256];
     __shared__ uint32_t sh_prefix;
