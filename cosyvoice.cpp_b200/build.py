@@ -42,8 +42,8 @@ def _units():
     for name, tid in K_TYPES.items():
         for stem in ("decode_inst", "flash_inst", "flash_pipe_inst", "decode_tc_inst", "decode_pipe_inst",
                      "decode_stream_inst", "decode_mma_inst", "tree_mma_inst",
-                     "tree_tc_inst", "kv_scores_inst"):
-            if stem in ("decode_tc_inst", "tree_mma_inst", "tree_tc_inst", "kv_scores_inst") and name == "f32":
+                     "tree_tc_inst", "kv_scores_inst", "kv_scores_tc_inst"):
+            if stem in ("decode_tc_inst", "tree_mma_inst", "tree_tc_inst", "kv_scores_inst", "kv_scores_tc_inst") and name == "f32":
                 continue  # the tensor-core decode, tree attention and scores cover block-quantized and f16 K only
             if stem in ("decode_pipe_inst", "decode_stream_inst", "decode_mma_inst") and name in ("f32", "f16"):
                 continue  # the persistent decodes cover block-quantized K only

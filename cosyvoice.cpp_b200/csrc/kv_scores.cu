@@ -1,5 +1,5 @@
 // kv_scores.cu -- cvattn_kv_scores: the attention weight of each cached position.
-#include "kv_scores.cuh"
+#include "kv_scores_tc.cuh"
 
 namespace cvattn {
 namespace kvscore {
@@ -121,6 +121,24 @@ cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params&
     a.scale_log2 = p.scale * 1.4426950408889634f;
     a.decay = p.decay;
     a.status = status;
+    // From two key tiles per SM on the persistent tcgen05 kernel; below, more and smaller CTAs answer sooner.
+    const int64_t entries = (int64_t)a.n_seq * a.Hkv * ((a.max_kv_len + kTcTile - 1) / kTcTile);
+    if (a.k_type != kF32 && entries >= 2 * 148 && entries < (int64_t)1 << 31 && a.n_seq <= kTcMaxSeq &&
+        (int64_t)a.max_rows * a.G <= kTcMaxRows) {
+        TcArgs ta{};
+        ta.a = a;
+        ta.inv_g = (uint32_t)((65536 + a.G - 1) / a.G);
+        ta.grid = 148;
+        switch (a.k_type) {
+        case kF16: return launch_tc_for_k<kF16>(stream, ta);
+        case kQ4_0: return launch_tc_for_k<kQ4_0>(stream, ta);
+        case kQ4_1: return launch_tc_for_k<kQ4_1>(stream, ta);
+        case kQ5_0: return launch_tc_for_k<kQ5_0>(stream, ta);
+        case kQ5_1: return launch_tc_for_k<kQ5_1>(stream, ta);
+        case kQ8_0: return launch_tc_for_k<kQ8_0>(stream, ta);
+        default: break;
+        }
+    }
     switch (a.k_type) {
     case kF16: return launch_mma_for_k<kF16>(stream, a);
     case kQ4_0: return launch_mma_for_k<kQ4_0>(stream, a);

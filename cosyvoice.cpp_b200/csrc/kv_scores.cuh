@@ -210,18 +210,25 @@ __global__ void __launch_bounds__(kThreads, NT == 2 ? 3 : 2) scores_mma_kernel(c
 #pragma unroll 1
         for (int rt = 0; rt < tiles; ++rt) {
             float acc[NT][K_Q ? 2 : 1][4];
+            // low parts of Q first, while the sums are small: adds inside the tensor cores truncate
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint4 h4 = qf[((rt * 4 + k) * 2 + 0) * 32 + lane], l4 = qf[((rt * 4 + k) * 2 + 1) * 32 + lane];
-                const uint32_t ah[4] = {h4.x, h4.y, h4.z, h4.w}, al[4] = {l4.x, l4.y, l4.z, l4.w};
+                const uint4 l4 = qf[((rt * 4 + k) * 2 + 1) * 32 + lane];
+                const uint32_t al[4] = {l4.x, l4.y, l4.z, l4.w};
                 const int b = K_Q ? k >> 1 : 0;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    if (k == 0 || (K_Q && k == 2)) mma16816_first(acc[t][b], ah, kf[t][k][0], kf[t][k][1]);
-                    else mma16816(acc[t][b], ah, kf[t][k][0], kf[t][k][1]);
+                    if (k == 0 || (K_Q && k == 2)) mma16816_first(acc[t][b], al, kf[t][k][0], kf[t][k][1]);
+                    else mma16816(acc[t][b], al, kf[t][k][0], kf[t][k][1]);
                 }
+            }
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma16816(acc[t][b], al, kf[t][k][0], kf[t][k][1]);
+            for (int k = 0; k < 4; ++k) {
+                const uint4 h4 = qf[((rt * 4 + k) * 2 + 0) * 32 + lane];
+                const uint32_t ah[4] = {h4.x, h4.y, h4.z, h4.w};
+                const int b = K_Q ? k >> 1 : 0;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma16816(acc[t][b], ah, kf[t][k][0], kf[t][k][1]);
             }
             const float4 i0 = info[rt * 16 + gid], i1 = info[rt * 16 + 8 + gid];
             const int f0 = masked ? far[rt * 16 + gid] - p0 : 0, f1 = masked ? far[rt * 16 + 8 + gid] - p0 : 0;

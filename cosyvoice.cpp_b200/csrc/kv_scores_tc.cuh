@@ -1,0 +1,464 @@
+// kv_scores_tc.cuh -- attention scores on the 5th-generation tensor cores (tcgen05),
+// for f16 and block-quantized caches, many keys and up to 512 rows.
+//
+// The product is taken transposed, S^T = K Q^T: a TMEM lane, and so a thread, is a
+// key, and the sum over the rows is a sum along the thread's columns, with no
+// exchange at all.  A key's block scales are then two scalars of its thread, so the
+// quants go into the product as the integers they are: S = d0 S0 + d1 S1 (+ mins),
+// with Q in f16 hi + lo scaled per row.
+//
+// The key tiles (128 keys) of all units (sequence, KV head) form one list, cut
+// evenly over the CTAs; a run is a CTA's part of one unit and shares its Q.
+//   warps 0-3, 4-7  groups: tile n of the CTA is summed up by group n & 1; all of them
+//                   prepare Q at the start of a run
+//   warps 8-15      producer: raw rows (one bulk copy per tile where they hold at most
+//                   two heads and lie packed, else the head's slices by cp.async), then
+//                   the f16 tile and the scales, a thread per block; an f16 cache is
+//                   copied straight into the tile
+//   warps 16, 17    MMA issuers of the groups
+#pragma once
+
+#include "kv_scores.cuh"
+#include "tree_tc.cuh"
+
+namespace cvattn {
+namespace kvscore {
+
+using tree::elect_one;
+using tree::kTcTile;
+using tree::kTcTileBytes;
+using tree::max3;
+using tree::tc_cut;
+using tree::tc_wait;
+
+constexpr int kTcThreads = 18 * 32;
+constexpr int kTcMaxSeq = 1024;
+constexpr int kTcMaxRows = 512;      // (token, head) rows of a KV head whose Q fits shared memory
+constexpr int kTcRowTiles = kTcMaxRows / 128;
+
+struct TcArgs {
+    Args a;
+    uint32_t inv_g;                  // ceil(2^16 / G)
+    int grid;
+};
+
+struct TcBars {
+    uint64_t k_full[4], k_empty[4];  // by stage
+    uint64_t raw_full[2];
+    uint64_t q_full;
+    uint64_t s_full[2], s_empty[2];  // by group
+    uint32_t tmem_base;
+    int err;
+    int any_out;                     // some row of the run is left out
+};
+
+template <int KT>
+struct TcShape {
+    static constexpr bool K_Q = KT != kF16;
+    static constexpr int kStages = K_Q ? 2 : 4;
+    static constexpr int kQ = 0;                                          // [row tile][hi, lo] tiles
+    static constexpr int kTiles = kTcRowTiles * 2 * kTcTileBytes;
+    static constexpr int kRaw = kTiles + kStages * kTcTileBytes;          // two buffers of up to two heads' rows
+    static constexpr int kRawOne = K_Q ? 2 * kTcTile * raw_stride(KT) : 0;
+    static constexpr int kInfo = kRaw + 2 * kRawOne;                      // float4 per row: factor, -log-sum, block sums of Q
+    static constexpr int kFar = kInfo + kTcMaxRows * 16;
+    static constexpr int kScale = kFar + kTcMaxRows * 4;                  // [tile n & 3][scales, mins][block][key]
+    static constexpr int kBars = kScale + (K_Q ? 4 * 4 * kTcTile * 4 : 0);
+    static constexpr int kPref = kBars + (int)((sizeof(TcBars) + 15) / 16 * 16);
+    static constexpr int kBytes = kPref + (kTcMaxSeq + 4) * 4;
+    static_assert(kBytes <= 227 * 1024, "one CTA per SM");
+};
+
+// A CTA's walk through its part of the list.  Lengths are read again where a run starts (they are few).
+struct Run {
+    int s, kvh, i, end, t0, T, L, n;
+    __device__ __forceinline__ void sequence(const Args& a, int seq) {
+        s = seq;
+        L = a.kv_len[seq];
+        n = a.n_rows ? a.n_rows[seq] : a.max_rows;
+        T = (L + kTcTile - 1) / kTcTile;
+    }
+    __device__ __forceinline__ void start(const Args& a, const int32_t* pref, int entry, int hi) {
+        i = end = entry;
+        if (entry >= hi) return;
+        int lo = 0, up = a.n_seq;  // last s with pref[s] <= entry: its list is not empty
+        while (up - lo > 1) {
+            const int mid = (lo + up) >> 1;
+            if (pref[mid] <= entry) lo = mid;
+            else up = mid;
+        }
+        sequence(a, lo);
+        kvh = (entry - pref[lo]) / T;
+        t0 = entry - pref[lo] - kvh * T;
+        end = min(hi, i + T - t0);
+    }
+    __device__ __forceinline__ void next(const Args& a, const int32_t* pref, int hi) {
+        i = end;
+        if (i >= hi) return;
+        t0 = 0;
+        if (++kvh == a.Hkv) {
+            kvh = 0;
+            int q = s + 1;
+            while (pref[q + 1] == i) ++q;  // sequences without entries
+            sequence(a, q);
+        }
+        end = min(hi, i + T);
+    }
+};
+
+template <int KT>
+__global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_constant__ TcArgs ta) {
+    using Sh = TcShape<KT>;
+    constexpr bool K_Q = Sh::K_Q, K_MIN = BlockTraits<KT>::HAS_MIN;
+    constexpr int kSt = Sh::kStages, slice = 2 * group_bytes(KT);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const Args& a = ta.a;
+    TcBars* B = reinterpret_cast<TcBars*>(smem + Sh::kBars);
+    int32_t* pref = reinterpret_cast<int32_t*>(smem + Sh::kPref);
+    if (smem_addr(smem) & 1023u) {
+        if (threadIdx.x == 0) record_status(a.status, kStatusTimeout);
+        return;
+    }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&B->k_full[i], 256);
+            mbar_init(&B->k_empty[i], 1);
+        }
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&B->raw_full[g], 1);
+            mbar_init(&B->s_full[g], 1);
+            mbar_init(&B->s_empty[g], 128);
+        }
+        mbar_init(&B->q_full, 256);
+        B->err = 0;
+        B->any_out = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tc::tmem_alloc(&B->tmem_base, 512);
+        tc::tmem_relinquish();
+    }
+    if (warp == 1) {  // list entries before each sequence
+        int carry = 0;
+        for (int base = 0; base < a.n_seq; base += 32) {
+            const int s = base + lane;
+            int x = 0, L, n;
+            if (s < a.n_seq && lens_of(a, s, L, n, blockIdx.x == 0)) x = (L + kTcTile - 1) / kTcTile * a.Hkv;
+            int incl = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (s < a.n_seq) pref[s] = carry + incl - x;
+            carry += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) pref[a.n_seq] = carry;
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = B->tmem_base;
+    const int total = pref[a.n_seq];
+    const int lo = tc_cut(blockIdx.x, total, ta.grid), hi = tc_cut(blockIdx.x + 1, total, ta.grid);
+    Run r;
+    r.start(a, pref, lo, hi);
+    float4* info = reinterpret_cast<float4*>(smem + Sh::kInfo);
+    int* far = reinterpret_cast<int*>(smem + Sh::kFar);
+    float* scale = reinterpret_cast<float*>(smem + Sh::kScale);
+
+    if (warp < 8) {
+        // ------------------------------------------------------ group g: thread = key of a tile
+        const int g = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
+        const uint32_t st = tmem + ((uint32_t)(quad * 32) << 16) + g * 256;
+        constexpr int kCols = K_Q ? 16 : 32;  // columns at a time
+        uint32_t k = 0;  // S tiles of this group so far
+        bool ok = true;
+        for (; r.i < hi; r.next(a, pref, hi)) {
+            const int R = r.n * a.G;
+            // every S of the last run has been read: its Q may go
+            if (!fp::prod_bar_and(1, 256, ok)) { ok = false; break; }
+            if (tid == 0) B->any_out = 0;
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+#pragma unroll 1
+            for (int q0 = tid; q0 < (R + 31) / 32 * 32; q0 += 256) {
+                const int t = (int)(((uint32_t)q0 * ta.inv_g) >> 16), h = r.kvh * a.G + q0 - t * a.G;
+                bool real = q0 < R;
+                int at = t;
+                float ls = -INFINITY;
+                if (real) {
+                    if (a.rows) at = a.rows[(int64_t)r.s * a.max_rows + t];
+                    if (at < 0 || at >= a.n_q_rows) {
+                        record_status(a.status, kStatusBadPosition);
+                        real = false;
+                    } else {
+                        ls = a.lse[((int64_t)r.s * a.n_q_rows + at) * a.Hq + h];
+                        real = ls != -INFINITY;
+                    }
+                    if (!real) B->any_out = 1;
+                }
+                const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)at * a.q_nb_node + h * kD);
+                float am = 0.0f, qs[2] = {0.0f, 0.0f};
+                if (real) {
+#pragma unroll 4
+                    for (int c = 0; c < 16; ++c) {
+                        const float4 v = q[c];
+                        am = max3(am, fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+                        if constexpr (K_MIN) qs[c >> 3] += (v.x + v.y) + (v.z + v.w);
+                    }
+                }
+                const int ex = dtc::norm_exp(am);
+                const float sc = pow2f(ex);
+                uint8_t* qh = smem + Sh::kQ + (q0 >> 7) * 2 * kTcTileBytes;
+#pragma unroll 2
+                for (int c = 0; c < 8; ++c) {
+                    const float4 u = real ? q[2 * c] : make_float4(0.f, 0.f, 0.f, 0.f), v = real ? q[2 * c + 1] : u;
+                    uint4 wh, wl;
+                    split2(u.x * sc, u.y * sc, wh.x, wl.x);
+                    split2(u.z * sc, u.w * sc, wh.y, wl.y);
+                    split2(v.x * sc, v.y * sc, wh.z, wl.z);
+                    split2(v.z * sc, v.w * sc, wh.w, wl.w);
+                    const uint32_t o = tc::sw128_offset(q0 & 127, c);
+                    *reinterpret_cast<uint4*>(qh + o) = wh;
+                    *reinterpret_cast<uint4*>(qh + kTcTileBytes + o) = wl;
+                }
+                info[q0] = make_float4(pow2f(-ex) * a.scale_log2, real ? -ls * 1.4426950408889634f : -INFINITY, qs[0] * a.scale_log2,
+                                       qs[1] * a.scale_log2);
+                far[q0] = real ? r.L - r.n + t + 1 : 0;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&B->q_full);
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            const bool any_out = B->any_out != 0;
+            for (int j = r.i + ((r.i ^ lo ^ g) & 1); ok && j < r.end; j += 2) {
+                const int n = j - lo, p0 = (r.t0 + j - r.i) * kTcTile, count = min(kTcTile, r.L - p0);
+                const int64_t at = (int64_t)r.s * a.nb_seq + (int64_t)r.kvh * a.nb_head + p0 + key;
+                const float old = key < count ? a.scores[at] : 0.0f;
+                const bool masked = any_out || p0 + kTcTile > r.L - r.n + 1;  // some (row, key) may be unseen
+                float d0 = 1.0f, d1 = 1.0f, m0 = 0.0f, m1 = 0.0f, s0 = 0.0f, s1 = 0.0f;
+                for (int rt = 0; rt * 128 < R; ++rt, ++k) {
+                    ok = tc_wait(&B->s_full[g], k & 1, &B->err, a.status, 51);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    tc::fence_after();
+                    if (K_Q && rt == 0) {
+                        const float* sp = scale + (n & 3) * 4 * kTcTile + key;
+                        d0 = sp[0];
+                        d1 = sp[kTcTile];
+                        if constexpr (K_MIN) {
+                            m0 = sp[2 * kTcTile];
+                            m1 = sp[3 * kTcTile];
+                        }
+                    }
+                    const int cols = min(128, R - rt * 128);
+#pragma unroll 1
+                    for (int c = 0; c < cols; c += kCols) {
+                        uint32_t u[kCols], w[kCols];
+                        if constexpr (K_Q) {
+                            tc::tmem_ld16(st + c, u);
+                            tc::tmem_ld16(st + 128 + c, w);
+                        } else {
+                            tc::tmem_ld32(st + c, u);
+                        }
+                        tc::tmem_ld_wait();
+                        const float4* ri = info + rt * 128 + c;
+                        float p[kCols];
+#pragma unroll
+                        for (int e = 0; e < kCols; ++e) {
+                            const float4 f = ri[e];
+                            float v = __uint_as_float(u[e]), off = f.y;
+                            if constexpr (K_Q) v = fmaf(v, d0, __uint_as_float(w[e]) * d1);
+                            if constexpr (K_MIN) off = fmaf(m0, f.z, fmaf(m1, f.w, off));
+                            p[e] = fast_exp2(fmaf(v, f.x, off));
+                        }
+                        if (masked) {
+                            const int* fr = far + rt * 128 + c;
+#pragma unroll
+                            for (int e = 0; e < kCols; ++e)
+                                if (p0 + key >= fr[e]) p[e] = 0.0f;
+                        }
+#pragma unroll
+                        for (int e = 0; e < kCols; e += 2) {
+                            s0 += p[e];
+                            s1 += p[e + 1];
+                        }
+                    }
+                    tc::fence_before();
+                    mbar_arrive(&B->s_empty[g]);
+                }
+                if (ok && key < count) a.out[at] = fmaf(a.decay, old, s0 + s1);
+            }
+            ok = __all_sync(0xffffffffu, ok);
+        }
+    } else if (warp < 16) {
+        // ------------------------------------------------------ producer
+        const int t = tid - 256, blk = warp & 1, key = ((warp - 8) >> 1) * 32 + lane;
+        auto base_of = [&](const Run& x) {
+            return a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[x.s]) : a.k + (int64_t)x.s * a.k_nb2;
+        };
+        Run rf = r;  // the run of the tile whose copies start
+        uint32_t waited[2] = {0u, 0u};
+        bool bulk_at[2] = {false, false};  // how the raw tile in each buffer came
+        int outstanding = 0;
+        bool ok = true;
+        constexpr int kAhead = K_Q ? 1 : kSt - 1;
+        auto start = [&](int m) {  // the copies of the CTA's tile m
+            const int e = lo + m;
+            if (e < hi) {
+                if (e == rf.end) rf.next(a, pref, hi);
+                const int p0 = (rf.t0 + e - rf.i) * kTcTile, count = min(kTcTile, rf.L - p0);
+                const uint8_t* src = base_of(rf) + (int64_t)p0 * a.k_nb1;
+                if constexpr (K_Q) {
+                    uint8_t* dst = smem + Sh::kRaw + (m & 1) * Sh::kRawOne;
+                    const bool bulk = a.Hkv <= 2 && a.k_nb1 == a.Hkv * slice && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+                    bulk_at[m & 1] = bulk;
+                    if (bulk) {
+                        ++outstanding;
+                        if (t == 0) {
+                            fence_proxy_async_smem();  // the reads of what was there come first
+                            const int bytes = count * a.Hkv * slice, main = bytes & ~15;
+                            for (int b = main; b < bytes; b += 2) *reinterpret_cast<uint16_t*>(dst + b) = *reinterpret_cast<const uint16_t*>(src + b);
+                            mbar_arrive_expect_tx(&B->raw_full[m & 1], (uint32_t)main);
+                            if (main) bulk_g2s(dst, src, (uint32_t)main, &B->raw_full[m & 1]);
+                        }
+                    } else {
+                        src += rf.kvh * slice;
+                        const int unit = ((reinterpret_cast<uint64_t>(src) | (uint64_t)a.k_nb1) & 3) == 0 ? 4 : 2;
+                        const int w = slice / unit, per = 256 / w, k0 = t / w, col = (t - k0 * w) * unit;
+#pragma unroll 1
+                        for (int kk = k0; k0 < per && kk < count; kk += per) {
+                            const uint8_t* from = src + (int64_t)kk * a.k_nb1 + col;
+                            uint8_t* to = dst + kk * raw_stride(KT) + col;
+                            if (unit == 4) tree::cp_async4(to, from, true);
+                            else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+                        }
+                    }
+                } else {
+                    const int sg = m % kSt;
+                    if (m >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (m / kSt - 1) & 1, &B->err, a.status, 53);
+                    src += rf.kvh * slice;
+                    uint8_t* dst = smem + Sh::kTiles + sg * kTcTileBytes;
+                    const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)a.k_nb1;
+                    const int unit = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 2, w = 128 / unit, per = 256 / w;
+                    const int k0 = t / w, col = (t - k0 * w) * unit;
+#pragma unroll 4
+                    for (int kk = k0; ok && kk < kTcTile; kk += per) {
+                        const bool there = kk < count;
+                        const uint8_t* from = there ? src + (int64_t)kk * a.k_nb1 + col : src;
+                        uint8_t* to = dst + kk * 128 + (col ^ ((kk & 7) << 4));
+                        if (unit == 16) tree::cp_async16(to, from, there);
+                        else if (unit == 4) tree::cp_async4(to, from, there);
+                        else *reinterpret_cast<uint16_t*>(to) = there ? *reinterpret_cast<const uint16_t*>(from) : (uint16_t)0;
+                    }
+                }
+            }
+        };
+#pragma unroll 1
+        for (int n = -kAhead; lo + n < hi; ++n) {
+            if (n >= 0) {
+                if constexpr (K_Q) {
+                    if (bulk_at[n & 1]) {
+                        ok = ok && tc_wait(&B->raw_full[n & 1], waited[n & 1]++ & 1, &B->err, a.status, 52);
+                        --outstanding;
+                    }
+                }
+                tree::cp_async_wait<kAhead - 1>();
+                // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
+                if (!fp::prod_bar_and(4, 256, ok)) break;
+            }
+            // raw copies of the next tile first; copies into a stage may have to wait for it, so they come last
+            if constexpr (K_Q) start(n + kAhead);
+            if (n >= 0) {
+            const int sg = n % kSt;
+            if constexpr (K_Q) {
+                if (lo + n == r.end) r.next(a, pref, hi);
+                const int p0 = (r.t0 + lo + n - r.i) * kTcTile, count = min(kTcTile, r.L - p0);
+                if (n >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (n / kSt - 1) & 1, &B->err, a.status, 54);
+                if (ok) {
+                    const uint8_t* raw = smem + Sh::kRaw + (n & 1) * Sh::kRawOne;
+                    const uint8_t* row = raw + (bulk_at[n & 1] ? key * a.Hkv * slice + r.kvh * slice : key * raw_stride(KT));
+                    uint8_t* tile = smem + Sh::kTiles + sg * kTcTileBytes;
+                    uint32_t w[16];
+                    float d, mn;
+                    if (blk) convert_block<KT, 1>(row, w, d, mn);
+                    else convert_block<KT, 0>(row, w, d, mn);
+                    store_block(tile, key, blk, w);
+                    float* sp = scale + ((n & 3) * 4 + blk) * kTcTile + key;
+                    sp[0] = key < count ? d : 0.0f;
+                    if constexpr (K_MIN) sp[2 * kTcTile] = key < count ? mn : 0.0f;
+                }
+            }
+            if (ok) {
+                fence_proxy_async_smem();
+                mbar_arrive(&B->k_full[sg]);
+            }
+            }
+            if constexpr (!K_Q) start(n + kAhead);
+            tree::cp_async_commit();
+        }
+        tree::cp_async_wait<0>();
+        // after an error a bulk copy may still be under way: none outlives the CTA
+        for (int i = 0; t == 0 && outstanding > 0 && i < 4096; ++i)
+            if (mbar_try_wait_hint(&B->raw_full[0], waited[0] & 1, 1000u) || mbar_try_wait_hint(&B->raw_full[1], waited[1] & 1, 1000u)) --outstanding;
+    } else {
+        // ------------------------------------------------------ MMA issuer of group g: the warp walks, one lane issues
+        const int g = __shfl_sync(0xffffffffu, warp, 0) - 16;
+        const uint64_t dq0 = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
+        const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
+        const uint32_t sp = tmem + g * 256;
+        uint32_t k = 0, n_run = 0;
+        bool ok = true;
+        for (; ok && r.i < hi; r.next(a, pref, hi), ++n_run) {
+            const int R = r.n * a.G;
+            ok = tc_wait(&B->q_full, n_run & 1, &B->err, a.status, 55);
+            for (int j = r.i + ((r.i ^ lo ^ g) & 1); ok && j < r.end; j += 2) {
+                const int n = j - lo, sg = n % kSt;
+                ok = tc_wait(&B->k_full[sg], (n / kSt) & 1, &B->err, a.status, 56);
+                ok = __all_sync(0xffffffffu, ok);
+                tc::fence_after();
+                const uint64_t dk = dt0 + (uint64_t)(sg * (kTcTileBytes >> 4));
+                for (int rt = 0; ok && rt * 128 < R; ++rt, ++k) {
+                    if (k) ok = tc_wait(&B->s_empty[g], (k - 1) & 1, &B->err, a.status, 57);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint32_t idesc = tc::idesc_f16_f32(128, (min(128, R - rt * 128) + 31) / 32 * 32, false);
+                    const uint64_t dh = dq0 + (uint64_t)(rt * 2 * (kTcTileBytes >> 4)), dl = dh + (kTcTileBytes >> 4);
+                    if (elect_one()) {
+                        if constexpr (K_Q) {
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {  // the low parts of Q first, while the sums are small
+                                tc::mma_ss(sp + 128 * b, dk + 4 * b, dl + 4 * b, idesc, 0u);
+                                tc::mma_ss(sp + 128 * b, dk + 4 * b + 2, dl + 4 * b + 2, idesc, 1u);
+                                tc::mma_ss(sp + 128 * b, dk + 4 * b, dh + 4 * b, idesc, 1u);
+                                tc::mma_ss(sp + 128 * b, dk + 4 * b + 2, dh + 4 * b + 2, idesc, 1u);
+                            }
+                        } else {
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dk + 2 * kk, dl + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dk + 2 * kk, dh + 2 * kk, idesc, 1u);
+                        }
+                        tc::mma_commit(&B->s_full[g]);
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one()) tc::mma_commit(&B->k_empty[sg]);
+                __syncwarp();
+            }
+            ok = __all_sync(0xffffffffu, ok);
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc::fence_after();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
+// Launch for K type KT (kv_scores_tc_inst.cu, one unit per K type).
+template <int KT> cudaError_t launch_tc_for_k(cudaStream_t stream, const TcArgs& a);
+
+}  // namespace kvscore
+}  // namespace cvattn

@@ -343,16 +343,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_mma_kernel(const __grid_c
                     constexpr int b1 = K_Q ? 1 : 0;
                     uint32_t r[4];
                     ldsm4(r, krow + ((lmat ^ lrow) << 4));
-                    mma16816_first(acc[0][tt], qa[0][0], r[0], r[1]);
-                    mma16816(acc[0][tt], qa[0][1], r[0], r[1]);
-                    mma16816(acc[0][tt], qa[1][0], r[2], r[3]);
+                    // small terms first, while the sums are small: adds inside the tensor cores truncate
+                    mma16816_first(acc[0][tt], qa[0][1], r[0], r[1]);
                     mma16816(acc[0][tt], qa[1][1], r[2], r[3]);
-                    ldsm4(r, krow + (((4 + lmat) ^ lrow) << 4));
-                    if constexpr (K_Q) mma16816_first(acc[b1][tt], qa[2][0], r[0], r[1]);
-                    else mma16816(acc[b1][tt], qa[2][0], r[0], r[1]);
-                    mma16816(acc[b1][tt], qa[2][1], r[0], r[1]);
-                    mma16816(acc[b1][tt], qa[3][0], r[2], r[3]);
-                    mma16816(acc[b1][tt], qa[3][1], r[2], r[3]);
+                    if constexpr (K_Q) {
+                        mma16816(acc[0][tt], qa[0][0], r[0], r[1]);
+                        mma16816(acc[0][tt], qa[1][0], r[2], r[3]);
+                        ldsm4(r, krow + (((4 + lmat) ^ lrow) << 4));
+                        mma16816_first(acc[b1][tt], qa[2][1], r[0], r[1]);
+                        mma16816(acc[b1][tt], qa[3][1], r[2], r[3]);
+                        mma16816(acc[b1][tt], qa[2][0], r[0], r[1]);
+                        mma16816(acc[b1][tt], qa[3][0], r[2], r[3]);
+                    } else {
+                        uint32_t u[4];
+                        ldsm4(u, krow + (((4 + lmat) ^ lrow) << 4));
+                        mma16816(acc[0][tt], qa[2][1], u[0], u[1]);
+                        mma16816(acc[0][tt], qa[3][1], u[2], u[3]);
+                        mma16816(acc[0][tt], qa[0][0], r[0], r[1]);
+                        mma16816(acc[0][tt], qa[1][0], r[2], r[3]);
+                        mma16816(acc[0][tt], qa[2][0], u[0], u[1]);
+                        mma16816(acc[0][tt], qa[3][0], u[2], u[3]);
+                    }
                 }
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
@@ -523,10 +534,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_mma_kernel(const __grid_c
                     uint32_t r[4];
                     ldsm4t(r, vrow + (((4 * b + 2 * u + (lmat >> 1)) ^ lrow) << 4));
                     const int j = 4 * b + 2 * u;
-                    mma16816(O[j], hi, r[0], r[1]);
-                    mma16816(O[j + 1], hi, r[2], r[3]);
                     mma16816(O[j], lo, r[0], r[1]);
                     mma16816(O[j + 1], lo, r[2], r[3]);
+                    mma16816(O[j], hi, r[0], r[1]);
+                    mma16816(O[j + 1], hi, r[2], r[3]);
                 }
             }
             if (++since == kFlush) flush();

@@ -756,11 +756,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                     const uint32_t sp = tmem + buf * 128;
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc, kk > 0 ? 1u : 0u);
-                            tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc, 1u);
+                        for (int kk = 0; kk < 4; ++kk) {  // small terms first, while the sums are small
+                            tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc, kk > 0 ? 1u : 0u);
                             if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc, 1u);
                         }
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc, 1u);
                         tc::mma_commit(&B->s_full[buf]);
                         tc::mma_commit(&B->k_empty[st]);
                     }
@@ -786,10 +787,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
                         const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
-                        tc::mma_ts(ot, ph, dv + kk * 128, idesc, kk > 0 ? 1u : 0u);
-                        tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc, 1u);
+                        tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc, kk > 0 ? 1u : 0u);
                         if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc, 1u);
                     }
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) tc::mma_ts(ot, sp + 32 * (kk >> 1) + 8 * (kk & 1), dv + kk * 128, idesc, 1u);
                     tc::mma_commit(&B->o_full[n & 1]);
                     tc::mma_commit(&B->v_empty[st]);
                     tc::mma_commit(&B->s_free[buf]);
