@@ -5,7 +5,9 @@
 // key, and the sum over the rows is a sum along the thread's columns, with no
 // exchange at all.  A key's block scales are then two scalars of its thread, so the
 // quants go into the product as the integers they are: S = d0 S0 + d1 S1 (+ mins),
-// with Q in f16 hi + lo scaled per row.
+// with Q in f16 hi + lo scaled per row.  A group has two S buffers in TMEM (128 rows
+// of an f16 cache, 64 of a quantized one, whose S0 and S1 lie side by side), so the
+// next rows' product runs while it sums one up.
 //
 // The key tiles (128 keys) of all units (sequence, KV head) form one list, cut
 // evenly over the CTAs; a run is a CTA's part of one unit and shares its Q.
@@ -46,7 +48,7 @@ struct TcBars {
     uint64_t k_full[4], k_empty[4];  // by stage
     uint64_t raw_full[2];
     uint64_t q_full;
-    uint64_t s_full[2], s_empty[2];  // by group
+    uint64_t s_full[2][2], s_empty[2][2];  // by group and S buffer
     uint32_t tmem_base;
     int err;
     int any_out;                     // some row of the run is left out
@@ -56,11 +58,12 @@ template <int KT>
 struct TcShape {
     static constexpr bool K_Q = KT != kF16;
     static constexpr int kStages = K_Q ? 2 : 4;
+    static constexpr int kSRows = K_Q ? 64 : 128;                         // rows of an S buffer
     static constexpr int kQ = 0;                                          // [row tile][hi, lo] tiles
     static constexpr int kTiles = kTcRowTiles * 2 * kTcTileBytes;
     static constexpr int kRaw = kTiles + kStages * kTcTileBytes;          // two buffers of up to two heads' rows
     static constexpr int kRawOne = K_Q ? 2 * kTcTile * raw_stride(KT) : 0;
-    static constexpr int kInfo = kRaw + 2 * kRawOne;                      // float4 per row: factor, -log-sum, block sums of Q
+    static constexpr int kInfo = kRaw + 2 * kRawOne;                      // float2 per row: factor, -log-sum; then the block sums of Q
     static constexpr int kFar = kInfo + kTcMaxRows * 16;
     static constexpr int kScale = kFar + kTcMaxRows * 4;                  // [tile n & 3][scales, mins][block][key]
     static constexpr int kBars = kScale + (K_Q ? 4 * 4 * kTcTile * 4 : 0);
@@ -127,8 +130,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(&B->raw_full[g], 1);
-            mbar_init(&B->s_full[g], 1);
-            mbar_init(&B->s_empty[g], 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&B->s_full[g][b], 1);
+                mbar_init(&B->s_empty[g][b], 128);
+            }
         }
         mbar_init(&B->q_full, 256);
         B->err = 0;
@@ -165,6 +170,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
     Run r;
     r.start(a, pref, lo, hi);
     float4* info = reinterpret_cast<float4*>(smem + Sh::kInfo);
+    float2* qsum = reinterpret_cast<float2*>(smem + Sh::kInfo + kTcMaxRows * 8);
     int* far = reinterpret_cast<int*>(smem + Sh::kFar);
     float* scale = reinterpret_cast<float*>(smem + Sh::kScale);
 
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         // ------------------------------------------------------ group g: thread = key of a tile
         const int g = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
         const uint32_t st = tmem + ((uint32_t)(quad * 32) << 16) + g * 256;
-        constexpr int kCols = K_Q ? 16 : 32;  // columns at a time
+        constexpr int kCols = 16;  // columns at a time
         uint32_t k = 0;  // S tiles of this group so far
         bool ok = true;
         for (; r.i < hi; r.next(a, pref, hi)) {
@@ -199,32 +205,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                     if (!real) B->any_out = 1;
                 }
                 const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)at * a.q_nb_node + h * kD);
+                float4 v[16];
                 float am = 0.0f, qs[2] = {0.0f, 0.0f};
-                if (real) {
-#pragma unroll 4
-                    for (int c = 0; c < 16; ++c) {
-                        const float4 v = q[c];
-                        am = max3(am, fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-                        if constexpr (K_MIN) qs[c >> 3] += (v.x + v.y) + (v.z + v.w);
-                    }
+#pragma unroll
+                for (int c = 0; c < 16; ++c) v[c] = real ? q[c] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    am = max3(am, fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w)));
+                    if constexpr (K_MIN) qs[c >> 3] += (v[c].x + v[c].y) + (v[c].z + v[c].w);
                 }
                 const int ex = dtc::norm_exp(am);
                 const float sc = pow2f(ex);
                 uint8_t* qh = smem + Sh::kQ + (q0 >> 7) * 2 * kTcTileBytes;
-#pragma unroll 2
+#pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    const float4 u = real ? q[2 * c] : make_float4(0.f, 0.f, 0.f, 0.f), v = real ? q[2 * c + 1] : u;
                     uint4 wh, wl;
-                    split2(u.x * sc, u.y * sc, wh.x, wl.x);
-                    split2(u.z * sc, u.w * sc, wh.y, wl.y);
-                    split2(v.x * sc, v.y * sc, wh.z, wl.z);
-                    split2(v.z * sc, v.w * sc, wh.w, wl.w);
+                    split2(v[2 * c].x * sc, v[2 * c].y * sc, wh.x, wl.x);
+                    split2(v[2 * c].z * sc, v[2 * c].w * sc, wh.y, wl.y);
+                    split2(v[2 * c + 1].x * sc, v[2 * c + 1].y * sc, wh.z, wl.z);
+                    split2(v[2 * c + 1].z * sc, v[2 * c + 1].w * sc, wh.w, wl.w);
                     const uint32_t o = tc::sw128_offset(q0 & 127, c);
                     *reinterpret_cast<uint4*>(qh + o) = wh;
                     *reinterpret_cast<uint4*>(qh + kTcTileBytes + o) = wl;
                 }
-                info[q0] = make_float4(pow2f(-ex) * a.scale_log2, real ? -ls * 1.4426950408889634f : -INFINITY, qs[0] * a.scale_log2,
-                                       qs[1] * a.scale_log2);
+                reinterpret_cast<float2*>(info)[q0] = make_float2(pow2f(-ex) * a.scale_log2, real ? -ls * 1.4426950408889634f : -INFINITY);
+                if constexpr (K_MIN) qsum[q0] = make_float2(qs[0] * a.scale_log2, qs[1] * a.scale_log2);
                 far[q0] = real ? r.L - r.n + t + 1 : 0;
             }
             fence_proxy_async_smem();
@@ -236,12 +241,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 const int64_t at = (int64_t)r.s * a.nb_seq + (int64_t)r.kvh * a.nb_head + p0 + key;
                 const float old = key < count ? a.scores[at] : 0.0f;
                 const bool masked = any_out || p0 + kTcTile > r.L - r.n + 1;  // some (row, key) may be unseen
-                float d0 = 1.0f, d1 = 1.0f, m0 = 0.0f, m1 = 0.0f, s0 = 0.0f, s1 = 0.0f;
-                for (int rt = 0; rt * 128 < R; ++rt, ++k) {
-                    ok = tc_wait(&B->s_full[g], k & 1, &B->err, a.status, 51);
+                float d0 = 1.0f, d1 = 1.0f, m0 = 0.0f, m1 = 0.0f, s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+                for (int r0 = 0; r0 < R; r0 += Sh::kSRows, ++k) {
+                    ok = tc_wait(&B->s_full[g][k & 1], (k >> 1) & 1, &B->err, a.status, 51);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     tc::fence_after();
-                    if (K_Q && rt == 0) {
+                    if (K_Q && r0 == 0) {
                         const float* sp = scale + (n & 3) * 4 * kTcTile + key;
                         d0 = sp[0];
                         d1 = sp[kTcTile];
@@ -250,43 +255,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                             m1 = sp[3 * kTcTile];
                         }
                     }
-                    const int cols = min(128, R - rt * 128);
+                    const uint32_t sb = st + (k & 1) * 128;
+                    const int cols = min(Sh::kSRows, R - r0);
+                    uint32_t u[kCols], w[kCols];
+                    auto load = [&](int c) {
+                        tc::tmem_ld16(sb + c, u);
+                        if constexpr (K_Q) tc::tmem_ld16(sb + 64 + c, w);
+                    };
+                    load(0);
+                    tc::tmem_ld_wait();
 #pragma unroll 1
                     for (int c = 0; c < cols; c += kCols) {
-                        uint32_t u[kCols], w[kCols];
-                        if constexpr (K_Q) {
-                            tc::tmem_ld16(st + c, u);
-                            tc::tmem_ld16(st + 128 + c, w);
-                        } else {
-                            tc::tmem_ld32(st + c, u);
-                        }
-                        tc::tmem_ld_wait();
-                        const float4* ri = info + rt * 128 + c;
+                        const float4* ri = info + (r0 + c) / 2;
                         float p[kCols];
 #pragma unroll
-                        for (int e = 0; e < kCols; ++e) {
-                            const float4 f = ri[e];
-                            float v = __uint_as_float(u[e]), off = f.y;
-                            if constexpr (K_Q) v = fmaf(v, d0, __uint_as_float(w[e]) * d1);
-                            if constexpr (K_MIN) off = fmaf(m0, f.z, fmaf(m1, f.w, off));
-                            p[e] = fast_exp2(fmaf(v, f.x, off));
+                        for (int e = 0; e < kCols; e += 2) {
+                            const float4 f = ri[e / 2];
+                            float o0 = f.y, o1 = f.w;
+                            if constexpr (K_MIN) {
+                                const float4 qq = reinterpret_cast<const float4*>(qsum + r0 + c)[e / 2];
+                                o0 = fmaf(m0, qq.x, fmaf(m1, qq.y, o0));
+                                o1 = fmaf(m0, qq.z, fmaf(m1, qq.w, o1));
+                            }
+                            float v0 = __uint_as_float(u[e]), v1 = __uint_as_float(u[e + 1]);
+                            if constexpr (K_Q) {
+                                v0 = fmaf(v0, d0, __uint_as_float(w[e]) * d1);
+                                v1 = fmaf(v1, d0, __uint_as_float(w[e + 1]) * d1);
+                            }
+                            p[e] = fmaf(v0, f.x, o0);
+                            p[e + 1] = fmaf(v1, f.z, o1);
                         }
+                        load(min(c + kCols, Sh::kSRows - kCols));  // under way during the exponentials
+#pragma unroll
+                        for (int e = 0; e < kCols; ++e) p[e] = fast_exp2(p[e]);
                         if (masked) {
-                            const int* fr = far + rt * 128 + c;
+                            const int* fr = far + r0 + c;
 #pragma unroll
                             for (int e = 0; e < kCols; ++e)
                                 if (p0 + key >= fr[e]) p[e] = 0.0f;
                         }
 #pragma unroll
-                        for (int e = 0; e < kCols; e += 2) {
+                        for (int e = 0; e < kCols; e += 4) {
                             s0 += p[e];
                             s1 += p[e + 1];
+                            s2 += p[e + 2];
+                            s3 += p[e + 3];
                         }
+                        tc::tmem_ld_wait();
                     }
                     tc::fence_before();
-                    mbar_arrive(&B->s_empty[g]);
+                    mbar_arrive(&B->s_empty[g][k & 1]);
                 }
-                if (ok && key < count) a.out[at] = fmaf(a.decay, old, s0 + s1);
+                if (ok && key < count) a.out[at] = fmaf(a.decay, old, (s0 + s1) + (s2 + s3));
             }
             ok = __all_sync(0xffffffffu, ok);
         }
@@ -405,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         const int g = __shfl_sync(0xffffffffu, warp, 0) - 16;
         const uint64_t dq0 = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
         const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
-        const uint32_t sp = tmem + g * 256;
+        const uint32_t sp0 = tmem + g * 256;
         uint32_t k = 0, n_run = 0;
         bool ok = true;
         for (; ok && r.i < hi; r.next(a, pref, hi), ++n_run) {
@@ -417,21 +437,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 ok = __all_sync(0xffffffffu, ok);
                 tc::fence_after();
                 const uint64_t dk = dt0 + (uint64_t)(sg * (kTcTileBytes >> 4));
-                for (int rt = 0; ok && rt * 128 < R; ++rt, ++k) {
-                    if (k) ok = tc_wait(&B->s_empty[g], (k - 1) & 1, &B->err, a.status, 57);
+                for (int r0 = 0; ok && r0 < R; r0 += Sh::kSRows, ++k) {
+                    if (k >= 2) ok = tc_wait(&B->s_empty[g][k & 1], ((k >> 1) - 1) & 1, &B->err, a.status, 57);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc::fence_after();
-                    const uint32_t idesc = tc::idesc_f16_f32(128, (min(128, R - rt * 128) + 31) / 32 * 32, false);
-                    const uint64_t dh = dq0 + (uint64_t)(rt * 2 * (kTcTileBytes >> 4)), dl = dh + (kTcTileBytes >> 4);
+                    const uint32_t idesc = tc::idesc_f16_f32(128, (min(Sh::kSRows, R - r0) + 15) / 16 * 16, false);
+                    const uint64_t dh = dq0 + (uint64_t)((r0 >> 7) * 2 * (kTcTileBytes >> 4) + (r0 & 127) * 8), dl = dh + (kTcTileBytes >> 4);
+                    const uint32_t sp = sp0 + (k & 1) * 128;
                     if (elect_one()) {
                         if constexpr (K_Q) {
 #pragma unroll
                             for (int b = 0; b < 2; ++b) {  // the low parts of Q first, while the sums are small
-                                tc::mma_ss(sp + 128 * b, dk + 4 * b, dl + 4 * b, idesc, 0u);
-                                tc::mma_ss(sp + 128 * b, dk + 4 * b + 2, dl + 4 * b + 2, idesc, 1u);
-                                tc::mma_ss(sp + 128 * b, dk + 4 * b, dh + 4 * b, idesc, 1u);
-                                tc::mma_ss(sp + 128 * b, dk + 4 * b + 2, dh + 4 * b + 2, idesc, 1u);
+                                tc::mma_ss(sp + 64 * b, dk + 4 * b, dl + 4 * b, idesc, 0u);
+                                tc::mma_ss(sp + 64 * b, dk + 4 * b + 2, dl + 4 * b + 2, idesc, 1u);
+                                tc::mma_ss(sp + 64 * b, dk + 4 * b, dh + 4 * b, idesc, 1u);
+                                tc::mma_ss(sp + 64 * b, dk + 4 * b + 2, dh + 4 * b + 2, idesc, 1u);
                             }
                         } else {
 #pragma unroll
@@ -439,7 +460,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dk + 2 * kk, dh + 2 * kk, idesc, 1u);
                         }
-                        tc::mma_commit(&B->s_full[g]);
+                        tc::mma_commit(&B->s_full[g][k & 1]);
                     }
                     __syncwarp();
                 }
