@@ -129,6 +129,9 @@ cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params&
         ta.a = a;
         ta.inv_g = (uint32_t)((65536 + a.G - 1) / a.G);
         ta.grid = 148;
+        const int spare = (kTcRowTiles - (a.max_rows * a.G + 127) / 128) * 2 * kTcTileBytes;  // of the Q tiles
+        const int raw = 2 * kTcTile * raw_stride(a.k_type);
+        ta.raw_buffers = 2 + spare / raw < kTcRawBuffers ? 2 + spare / raw : kTcRawBuffers;
         switch (a.k_type) {
         case kF16: return launch_tc_for_k<kF16>(stream, ta);
         case kQ4_0: return launch_tc_for_k<kQ4_0>(stream, ta);

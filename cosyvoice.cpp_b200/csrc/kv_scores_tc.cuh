@@ -37,16 +37,18 @@ constexpr int kTcThreads = 18 * 32;
 constexpr int kTcMaxSeq = 1024;
 constexpr int kTcMaxRows = 512;      // (token, head) rows of a KV head whose Q fits shared memory
 constexpr int kTcRowTiles = kTcMaxRows / 128;
+constexpr int kTcRawBuffers = 8;
 
 struct TcArgs {
     Args a;
     uint32_t inv_g;                  // ceil(2^16 / G)
     int grid;
+    int raw_buffers;                 // 2, and what fits the Q tiles that these rows do not need (up to kTcRawBuffers)
 };
 
 struct TcBars {
     uint64_t k_full[4], k_empty[4];  // by stage
-    uint64_t raw_full[2];
+    uint64_t raw_full[kTcRawBuffers];
     uint64_t q_full;
     uint64_t s_full[2][2], s_empty[2][2];  // by group and S buffer
     uint32_t tmem_base;
@@ -128,8 +130,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
             mbar_init(&B->k_full[i], 256);
             mbar_init(&B->k_empty[i], 1);
         }
+        for (int i = 0; i < kTcRawBuffers; ++i) mbar_init(&B->raw_full[i], 1);
         for (int g = 0; g < 2; ++g) {
-            mbar_init(&B->raw_full[g], 1);
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&B->s_full[g][b], 1);
                 mbar_init(&B->s_empty[g][b], 128);
@@ -317,11 +319,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
             return a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[x.s]) : a.k + (int64_t)x.s * a.k_nb2;
         };
         Run rf = r;  // the run of the tile whose copies start
-        uint32_t waited[2] = {0u, 0u};
-        bool bulk_at[2] = {false, false};  // how the raw tile in each buffer came
-        int outstanding = 0;
+        // raw buffers: the two behind the tiles, then the end of the Q tiles, whose last ones no row needs
+        const int nbuf = K_Q ? ta.raw_buffers : 1;
+        auto raw_at = [&](int b) { return b < 2 ? smem + Sh::kRaw + b * Sh::kRawOne : smem + Sh::kTiles - (b - 1) * Sh::kRawOne; };
+        uint32_t bulk_at = 0, phase = 0;   // by buffer: whether its tile came by bulk copy, the parity of its next one
+        int outstanding = 0, fb = 0, nb = 0;   // buffers of the tile whose copies start and of the tile that is finished
         bool ok = true;
-        constexpr int kAhead = K_Q ? 1 : kSt - 1;
+        const int kAhead = K_Q ? nbuf - 1 : kSt - 1;
         auto start = [&](int m) {  // the copies of the CTA's tile m
             const int e = lo + m;
             if (e < hi) {
@@ -329,17 +333,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 const int p0 = (rf.t0 + e - rf.i) * kTcTile, count = min(kTcTile, rf.L - p0);
                 const uint8_t* src = base_of(rf) + (int64_t)p0 * a.k_nb1;
                 if constexpr (K_Q) {
-                    uint8_t* dst = smem + Sh::kRaw + (m & 1) * Sh::kRawOne;
+                    uint8_t* dst = raw_at(fb);
                     const bool bulk = a.Hkv <= 2 && a.k_nb1 == a.Hkv * slice && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-                    bulk_at[m & 1] = bulk;
+                    bulk_at = (bulk_at & ~(1u << fb)) | (bulk ? 1u << fb : 0u);
                     if (bulk) {
                         ++outstanding;
                         if (t == 0) {
                             fence_proxy_async_smem();  // the reads of what was there come first
                             const int bytes = count * a.Hkv * slice, main = bytes & ~15;
                             for (int b = main; b < bytes; b += 2) *reinterpret_cast<uint16_t*>(dst + b) = *reinterpret_cast<const uint16_t*>(src + b);
-                            mbar_arrive_expect_tx(&B->raw_full[m & 1], (uint32_t)main);
-                            if (main) bulk_g2s(dst, src, (uint32_t)main, &B->raw_full[m & 1]);
+                            mbar_arrive_expect_tx(&B->raw_full[fb], (uint32_t)main);
+                            if (main) bulk_g2s(dst, src, (uint32_t)main, &B->raw_full[fb]);
                         }
                     } else {
                         src += rf.kvh * slice;
@@ -377,17 +381,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         for (int n = -kAhead; lo + n < hi; ++n) {
             if (n >= 0) {
                 if constexpr (K_Q) {
-                    if (bulk_at[n & 1]) {
-                        ok = ok && tc_wait(&B->raw_full[n & 1], waited[n & 1]++ & 1, &B->err, a.status, 52);
+                    if (bulk_at >> nb & 1u) {
+                        ok = ok && tc_wait(&B->raw_full[nb], phase >> nb & 1u, &B->err, a.status, 52);
+                        phase ^= 1u << nb;
                         --outstanding;
+                    } else {
+                        tree::cp_async_wait<0>();
                     }
+                } else {
+                    tree::cp_async_wait<kSt - 2>();
                 }
-                tree::cp_async_wait<kAhead - 1>();
                 // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
                 if (!fp::prod_bar_and(4, 256, ok)) break;
             }
-            // raw copies of the next tile first; copies into a stage may have to wait for it, so they come last
-            if constexpr (K_Q) start(n + kAhead);
+            // raw copies of a later tile first (into the buffer of the tile before this one); copies into a stage may have to
+            // wait for it, so they come last
+            if constexpr (K_Q) {
+                start(n + kAhead);
+                if (++fb == nbuf) fb = 0;
+            }
             if (n >= 0) {
             const int sg = n % kSt;
             if constexpr (K_Q) {
@@ -395,8 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 const int p0 = (r.t0 + lo + n - r.i) * kTcTile, count = min(kTcTile, r.L - p0);
                 if (n >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (n / kSt - 1) & 1, &B->err, a.status, 54);
                 if (ok) {
-                    const uint8_t* raw = smem + Sh::kRaw + (n & 1) * Sh::kRawOne;
-                    const uint8_t* row = raw + (bulk_at[n & 1] ? key * a.Hkv * slice + r.kvh * slice : key * raw_stride(KT));
+                    const uint8_t* row = raw_at(nb) + ((bulk_at >> nb & 1u) ? key * a.Hkv * slice + r.kvh * slice : key * raw_stride(KT));
                     uint8_t* tile = smem + Sh::kTiles + sg * kTcTileBytes;
                     uint32_t w[16];
                     float d, mn;
@@ -412,14 +423,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 fence_proxy_async_smem();
                 mbar_arrive(&B->k_full[sg]);
             }
+            if (++nb == nbuf) nb = 0;
             }
             if constexpr (!K_Q) start(n + kAhead);
             tree::cp_async_commit();
         }
         tree::cp_async_wait<0>();
         // after an error a bulk copy may still be under way: none outlives the CTA
-        for (int i = 0; t == 0 && outstanding > 0 && i < 4096; ++i)
-            if (mbar_try_wait_hint(&B->raw_full[0], waited[0] & 1, 1000u) || mbar_try_wait_hint(&B->raw_full[1], waited[1] & 1, 1000u)) --outstanding;
+        for (int i = 0; t == 0 && outstanding > 0 && i < 4096; ++i, nb = nb + 1 == nbuf ? 0 : nb + 1)
+            if ((bulk_at >> nb & 1u) && mbar_try_wait_hint(&B->raw_full[nb], phase >> nb & 1u, 1000u)) {
+                bulk_at &= ~(1u << nb);
+                --outstanding;
+            }
     } else {
         // ------------------------------------------------------ MMA issuer of group g: the warp walks, one lane issues
         const int g = __shfl_sync(0xffffffffu, warp, 0) - 16;
