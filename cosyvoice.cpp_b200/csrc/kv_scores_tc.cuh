@@ -13,11 +13,12 @@
 // evenly over the CTAs; a run is a CTA's part of one unit and shares its Q.
 //   warps 0-3, 4-7  groups: tile n of the CTA is summed up by group n & 1; all of them
 //                   prepare Q at the start of a run
-//   warps 8-15      producer: raw rows (one bulk copy per tile where they hold at most
-//                   two heads and lie packed, else the head's slices by cp.async), then
-//                   the f16 tile and the scales, a thread per block; an f16 cache is
-//                   copied straight into the tile
+//   warps 8-11, 12-15  producers of the groups' tiles, a thread per key: f16 tile and
+//                   scales from the raw rows; an f16 cache is copied straight into the
+//                   tile
 //   warps 16, 17    MMA issuers of the groups
+//   warp 18         loader: raw rows of the next tiles, one bulk copy each where they hold
+//                   at most two heads and lie packed (else the producers copy the slices)
 #pragma once
 
 #include "kv_scores.cuh"
@@ -33,7 +34,7 @@ using tree::max3;
 using tree::tc_cut;
 using tree::tc_wait;
 
-constexpr int kTcThreads = 18 * 32;
+constexpr int kTcThreads = 19 * 32;
 constexpr int kTcMaxSeq = 1024;
 constexpr int kTcMaxRows = 512;      // (token, head) rows of a KV head whose Q fits shared memory
 constexpr int kTcRowTiles = kTcMaxRows / 128;
@@ -48,7 +49,7 @@ struct TcArgs {
 
 struct TcBars {
     uint64_t k_full[4], k_empty[4];  // by stage
-    uint64_t raw_full[kTcRawBuffers];
+    uint64_t raw_full[kTcRawBuffers], raw_empty[kTcRawBuffers];
     uint64_t q_full;
     uint64_t s_full[2][2], s_empty[2][2];  // by group and S buffer
     uint32_t tmem_base;
@@ -111,6 +112,22 @@ struct Run {
     }
 };
 
+// Row 0 (every head) of the tile at list entry e of run r.
+__device__ __forceinline__ const uint8_t* tile_rows(const Args& a, const Run& r, int e) {
+    const uint8_t* b = a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[r.s]) : a.k + (int64_t)r.s * a.k_nb2;
+    return b + (int64_t)(r.t0 + e - r.i) * kTcTile * a.k_nb1;
+}
+// Whether a tile's rows come by one bulk copy: packed, 16-byte aligned, at most two heads.
+__device__ __forceinline__ bool whole_rows(const Args& a, const uint8_t* rows, int slice) {
+    return a.Hkv <= 2 && a.k_nb1 == a.Hkv * slice && (reinterpret_cast<uintptr_t>(rows) & 15) == 0;
+}
+// Raw buffers: two behind the tiles, then the end of the Q tiles, whose last ones no row needs.
+template <int KT>
+__device__ __forceinline__ uint8_t* raw_at(uint8_t* smem, int b) {
+    using Sh = TcShape<KT>;
+    return b < 2 ? smem + Sh::kRaw + b * Sh::kRawOne : smem + Sh::kTiles - (b - 1) * Sh::kRawOne;
+}
+
 template <int KT>
 __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_constant__ TcArgs ta) {
     using Sh = TcShape<KT>;
@@ -127,10 +144,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&B->k_full[i], 256);
+            mbar_init(&B->k_full[i], 128);
             mbar_init(&B->k_empty[i], 1);
         }
-        for (int i = 0; i < kTcRawBuffers; ++i) mbar_init(&B->raw_full[i], 1);
+        for (int i = 0; i < kTcRawBuffers; ++i) {
+            mbar_init(&B->raw_full[i], 1);
+            mbar_init(&B->raw_empty[i], 128);
+        }
         for (int g = 0; g < 2; ++g) {
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&B->s_full[g][b], 1);
@@ -189,50 +209,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
             if (!fp::prod_bar_and(1, 256, ok)) { ok = false; break; }
             if (tid == 0) B->any_out = 0;
             asm volatile("bar.sync 2, 256;" ::: "memory");
-#pragma unroll 1
-            for (int q0 = tid; q0 < (R + 31) / 32 * 32; q0 += 256) {
+            // 4 lanes a row, 16 dims each; rows from R to the next multiple of 32 are zeros
+            const int c = lane & 3;
+#pragma unroll 2
+            for (int q0 = warp * 8 + (lane >> 2); q0 < (R + 31) / 32 * 32; q0 += 64) {
                 const int t = (int)(((uint32_t)q0 * ta.inv_g) >> 16), h = r.kvh * a.G + q0 - t * a.G;
-                bool real = q0 < R;
-                int at = t;
+                float4 v[4];
                 float ls = -INFINITY;
-                if (real) {
-                    if (a.rows) at = a.rows[(int64_t)r.s * a.max_rows + t];
-                    if (at < 0 || at >= a.n_q_rows) {
-                        record_status(a.status, kStatusBadPosition);
-                        real = false;
-                    } else {
-                        ls = a.lse[((int64_t)r.s * a.n_q_rows + at) * a.Hq + h];
-                        real = ls != -INFINITY;
-                    }
-                    if (!real) B->any_out = 1;
-                }
-                const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)at * a.q_nb_node + h * kD);
-                float4 v[16];
-                float am = 0.0f, qs[2] = {0.0f, 0.0f};
+                int at = t;
+                if (q0 < R && a.rows) at = a.rows[(int64_t)r.s * a.max_rows + t];
+                const bool there = q0 < R && at >= 0 && at < a.n_q_rows;
+                if (there) ls = a.lse[((int64_t)r.s * a.n_q_rows + at) * a.Hq + h];
+                else if (q0 < R) record_status(a.status, kStatusBadPosition);
+                const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)at * a.q_nb_node + h * kD + 16 * c);
 #pragma unroll
-                for (int c = 0; c < 16; ++c) v[c] = real ? q[c] : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int u = 0; u < 4; ++u) v[u] = there ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
+                const bool real = ls != -INFINITY;
+                if (q0 < R && !real) B->any_out = 1;
+                float am = 0.0f, qs = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    am = max3(am, fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w)));
-                    if constexpr (K_MIN) qs[c >> 3] += (v[c].x + v[c].y) + (v[c].z + v[c].w);
+                for (int u = 0; u < 4; ++u) {
+                    if (!real) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    am = max3(am, fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w)));
+                    if constexpr (K_MIN) qs += (v[u].x + v[u].y) + (v[u].z + v[u].w);
                 }
+                am = quad_max(am);
+                if constexpr (K_MIN) qs += __shfl_xor_sync(0xffffffffu, qs, 1);  // over the two lanes of a block
                 const int ex = dtc::norm_exp(am);
                 const float sc = pow2f(ex);
                 uint8_t* qh = smem + Sh::kQ + (q0 >> 7) * 2 * kTcTileBytes;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int u = 0; u < 2; ++u) {
                     uint4 wh, wl;
-                    split2(v[2 * c].x * sc, v[2 * c].y * sc, wh.x, wl.x);
-                    split2(v[2 * c].z * sc, v[2 * c].w * sc, wh.y, wl.y);
-                    split2(v[2 * c + 1].x * sc, v[2 * c + 1].y * sc, wh.z, wl.z);
-                    split2(v[2 * c + 1].z * sc, v[2 * c + 1].w * sc, wh.w, wl.w);
-                    const uint32_t o = tc::sw128_offset(q0 & 127, c);
+                    split2(v[2 * u].x * sc, v[2 * u].y * sc, wh.x, wl.x);
+                    split2(v[2 * u].z * sc, v[2 * u].w * sc, wh.y, wl.y);
+                    split2(v[2 * u + 1].x * sc, v[2 * u + 1].y * sc, wh.z, wl.z);
+                    split2(v[2 * u + 1].z * sc, v[2 * u + 1].w * sc, wh.w, wl.w);
+                    const uint32_t o = tc::sw128_offset(q0 & 127, 2 * c + u);
                     *reinterpret_cast<uint4*>(qh + o) = wh;
                     *reinterpret_cast<uint4*>(qh + kTcTileBytes + o) = wl;
                 }
-                reinterpret_cast<float2*>(info)[q0] = make_float2(pow2f(-ex) * a.scale_log2, real ? -ls * 1.4426950408889634f : -INFINITY);
-                if constexpr (K_MIN) qsum[q0] = make_float2(qs[0] * a.scale_log2, qs[1] * a.scale_log2);
-                far[q0] = real ? r.L - r.n + t + 1 : 0;
+                if (c == 0) {
+                    reinterpret_cast<float2*>(info)[q0] = make_float2(pow2f(-ex) * a.scale_log2, real ? -ls * 1.4426950408889634f : -INFINITY);
+                    far[q0] = real ? r.L - r.n + t + 1 : 0;
+                }
+                if (K_MIN && (c & 1) == 0) reinterpret_cast<float*>(qsum + q0)[c >> 1] = qs * a.scale_log2;
             }
             fence_proxy_async_smem();
             mbar_arrive(&B->q_full);
@@ -313,58 +334,71 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
             ok = __all_sync(0xffffffffu, ok);
         }
     } else if (warp < 16) {
-        // ------------------------------------------------------ producer
-        const int t = tid - 256, blk = warp & 1, key = ((warp - 8) >> 1) * 32 + lane;
-        auto base_of = [&](const Run& x) {
-            return a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[x.s]) : a.k + (int64_t)x.s * a.k_nb2;
-        };
-        Run rf = r;  // the run of the tile whose copies start
-        // raw buffers: the two behind the tiles, then the end of the Q tiles, whose last ones no row needs
-        const int nbuf = K_Q ? ta.raw_buffers : 1;
-        auto raw_at = [&](int b) { return b < 2 ? smem + Sh::kRaw + b * Sh::kRawOne : smem + Sh::kTiles - (b - 1) * Sh::kRawOne; };
-        uint32_t bulk_at = 0, phase = 0;   // by buffer: whether its tile came by bulk copy, the parity of its next one
-        int outstanding = 0, fb = 0, nb = 0;   // buffers of the tile whose copies start and of the tile that is finished
+        // ------------------------------------------------------ producer of group g's tiles: thread = key
+        const int g = (warp - 8) >> 2, key = tid - 256 - g * 128;
+        const int nbuf = ta.raw_buffers;
         bool ok = true;
-        const int kAhead = K_Q ? nbuf - 1 : kSt - 1;
-        auto start = [&](int m) {  // the copies of the CTA's tile m
-            const int e = lo + m;
-            if (e < hi) {
-                if (e == rf.end) rf.next(a, pref, hi);
-                const int p0 = (rf.t0 + e - rf.i) * kTcTile, count = min(kTcTile, rf.L - p0);
-                const uint8_t* src = base_of(rf) + (int64_t)p0 * a.k_nb1;
-                if constexpr (K_Q) {
-                    uint8_t* dst = raw_at(fb);
-                    const bool bulk = a.Hkv <= 2 && a.k_nb1 == a.Hkv * slice && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-                    bulk_at = (bulk_at & ~(1u << fb)) | (bulk ? 1u << fb : 0u);
-                    if (bulk) {
-                        ++outstanding;
-                        if (t == 0) {
-                            fence_proxy_async_smem();  // the reads of what was there come first
-                            const int bytes = count * a.Hkv * slice, main = bytes & ~15;
-                            for (int b = main; b < bytes; b += 2) *reinterpret_cast<uint16_t*>(dst + b) = *reinterpret_cast<const uint16_t*>(src + b);
-                            mbar_arrive_expect_tx(&B->raw_full[fb], (uint32_t)main);
-                            if (main) bulk_g2s(dst, src, (uint32_t)main, &B->raw_full[fb]);
-                        }
-                    } else {
-                        src += rf.kvh * slice;
-                        const int unit = ((reinterpret_cast<uint64_t>(src) | (uint64_t)a.k_nb1) & 3) == 0 ? 4 : 2;
-                        const int w = slice / unit, per = 256 / w, k0 = t / w, col = (t - k0 * w) * unit;
-#pragma unroll 1
-                        for (int kk = k0; k0 < per && kk < count; kk += per) {
-                            const uint8_t* from = src + (int64_t)kk * a.k_nb1 + col;
-                            uint8_t* to = dst + kk * raw_stride(KT) + col;
-                            if (unit == 4) tree::cp_async4(to, from, true);
-                            else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
-                        }
+        if constexpr (K_Q) {
+            for (int n = g; lo + n < hi; n += 2) {
+                while (lo + n >= r.end) r.next(a, pref, hi);
+                const int count = min(kTcTile, r.L - (r.t0 + lo + n - r.i) * kTcTile), sg = n & 1, b = n % nbuf;
+                const uint8_t* src = tile_rows(a, r, lo + n);
+                ok = ok && tc_wait(&B->raw_full[b], (n / nbuf) & 1, &B->err, a.status, 52);
+                if (!fp::prod_bar_and(4 + g, 128, ok)) break;
+                uint8_t* raw = raw_at<KT>(smem, b);
+                const bool whole = whole_rows(a, src, slice);
+                if (!whole) {
+                    src += r.kvh * slice;
+                    const int unit = ((reinterpret_cast<uint64_t>(src) | (uint64_t)a.k_nb1) & 3) == 0 ? 4 : 2;
+                    const int w = slice / unit, per = 128 / w, k0 = key / w, col = (key - k0 * w) * unit;
+#pragma unroll 4
+                    for (int kk = k0; k0 < per && kk < count; kk += per) {
+                        const uint8_t* from = src + (int64_t)kk * a.k_nb1 + col;
+                        uint8_t* to = raw + kk * raw_stride(KT) + col;
+                        if (unit == 4) tree::cp_async4(to, from, true);
+                        else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
                     }
-                } else {
-                    const int sg = m % kSt;
-                    if (m >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (m / kSt - 1) & 1, &B->err, a.status, 53);
-                    src += rf.kvh * slice;
+                    tree::cp_async_commit();
+                    tree::cp_async_wait<0>();
+                    asm volatile("bar.sync %0, 128;" ::"r"(4 + g) : "memory");
+                }
+                if (n >= 2) ok = tc_wait(&B->k_empty[sg], (n / 2 - 1) & 1, &B->err, a.status, 54);
+                if (ok) {
+                    const uint8_t* row = raw + (whole ? key * a.Hkv * slice + r.kvh * slice : key * raw_stride(KT));
+                    uint8_t* tile = smem + Sh::kTiles + sg * kTcTileBytes;
+                    uint32_t w0[16], w1[16];
+                    float d0, m0, d1, m1;
+                    convert_block<KT, 0>(row, w0, d0, m0);
+                    convert_block<KT, 1>(row, w1, d1, m1);
+                    store_block(tile, key, 0, w0);
+                    store_block(tile, key, 1, w1);
+                    float* sp = scale + (n & 3) * 4 * kTcTile + key;
+                    const bool there = key < count;
+                    sp[0] = there ? d0 : 0.0f;
+                    sp[kTcTile] = there ? d1 : 0.0f;
+                    if constexpr (K_MIN) {
+                        sp[2 * kTcTile] = there ? m0 : 0.0f;
+                        sp[3 * kTcTile] = there ? m1 : 0.0f;
+                    }
+                    fence_proxy_async_smem();
+                    mbar_arrive(&B->k_full[sg]);
+                    mbar_arrive(&B->raw_empty[b]);
+                }
+            }
+        } else {
+            // the group's tiles n, n + 2, ..: the copies of the next one run while this one is used
+            Run rf = r;
+            auto start = [&](int n) {
+                const int e = lo + n, sg = n % kSt;
+                if (e < hi) {
+                    while (e >= rf.end) rf.next(a, pref, hi);
+                    const int count = min(kTcTile, rf.L - (rf.t0 + e - rf.i) * kTcTile);
+                    const uint8_t* src = tile_rows(a, rf, e) + rf.kvh * slice;
+                    if (n >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (n / kSt - 1) & 1, &B->err, a.status, 53);
                     uint8_t* dst = smem + Sh::kTiles + sg * kTcTileBytes;
                     const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)a.k_nb1;
-                    const int unit = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 2, w = 128 / unit, per = 256 / w;
-                    const int k0 = t / w, col = (t - k0 * w) * unit;
+                    const int unit = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 2, w = 128 / unit, per = 128 / w;
+                    const int k0 = key / w, col = (key - k0 * w) * unit;
 #pragma unroll 4
                     for (int kk = k0; ok && kk < kTcTile; kk += per) {
                         const bool there = kk < count;
@@ -375,66 +409,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                         else *reinterpret_cast<uint16_t*>(to) = there ? *reinterpret_cast<const uint16_t*>(from) : (uint16_t)0;
                     }
                 }
-            }
-        };
-#pragma unroll 1
-        for (int n = -kAhead; lo + n < hi; ++n) {
-            if (n >= 0) {
-                if constexpr (K_Q) {
-                    if (bulk_at >> nb & 1u) {
-                        ok = ok && tc_wait(&B->raw_full[nb], phase >> nb & 1u, &B->err, a.status, 52);
-                        phase ^= 1u << nb;
-                        --outstanding;
-                    } else {
-                        tree::cp_async_wait<0>();
-                    }
-                } else {
-                    tree::cp_async_wait<kSt - 2>();
-                }
-                // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
-                if (!fp::prod_bar_and(4, 256, ok)) break;
-            }
-            // raw copies of a later tile first (into the buffer of the tile before this one); copies into a stage may have to
-            // wait for it, so they come last
-            if constexpr (K_Q) {
-                start(n + kAhead);
-                if (++fb == nbuf) fb = 0;
-            }
-            if (n >= 0) {
-            const int sg = n % kSt;
-            if constexpr (K_Q) {
-                if (lo + n == r.end) r.next(a, pref, hi);
-                const int p0 = (r.t0 + lo + n - r.i) * kTcTile, count = min(kTcTile, r.L - p0);
-                if (n >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (n / kSt - 1) & 1, &B->err, a.status, 54);
+                tree::cp_async_commit();
+            };
+            start(g);
+            for (int n = g; lo + n < hi; n += 2) {
+                tree::cp_async_wait<0>();
                 if (ok) {
-                    const uint8_t* row = raw_at(nb) + ((bulk_at >> nb & 1u) ? key * a.Hkv * slice + r.kvh * slice : key * raw_stride(KT));
-                    uint8_t* tile = smem + Sh::kTiles + sg * kTcTileBytes;
-                    uint32_t w[16];
-                    float d, mn;
-                    if (blk) convert_block<KT, 1>(row, w, d, mn);
-                    else convert_block<KT, 0>(row, w, d, mn);
-                    store_block(tile, key, blk, w);
-                    float* sp = scale + ((n & 3) * 4 + blk) * kTcTile + key;
-                    sp[0] = key < count ? d : 0.0f;
-                    if constexpr (K_MIN) sp[2 * kTcTile] = key < count ? mn : 0.0f;
+                    fence_proxy_async_smem();
+                    mbar_arrive(&B->k_full[n % kSt]);
+                }
+                start(n + 2);  // (may have to wait for its stage)
+            }
+            tree::cp_async_wait<0>();
+        }
+    } else if (warp == 18) {
+        // ------------------------------------------------------ loader
+        if constexpr (K_Q) {
+            if (lane == 0) {
+                const int nbuf = ta.raw_buffers;
+                int b = 0, n = 0;
+                uint32_t turn = 0;
+                bool ok = true;
+                for (; ok && lo + n < hi; ++n) {
+                    if (lo + n == r.end) r.next(a, pref, hi);
+                    if (turn) ok = tc_wait(&B->raw_empty[b], (turn - 1) & 1, &B->err, a.status, 58);
+                    if (!ok) break;
+                    const uint8_t* src = tile_rows(a, r, lo + n);
+                    uint32_t main = 0;
+                    if (whole_rows(a, src, slice)) {
+                        uint8_t* dst = raw_at<KT>(smem, b);
+                        const int bytes = min(kTcTile, r.L - (r.t0 + lo + n - r.i) * kTcTile) * a.Hkv * slice;
+                        main = (uint32_t)bytes & ~15u;
+                        fence_proxy_async_smem();  // the reads of what was there come first
+                        for (int x = (int)main; x < bytes; x += 2) *reinterpret_cast<uint16_t*>(dst + x) = *reinterpret_cast<const uint16_t*>(src + x);
+                        mbar_arrive_expect_tx(&B->raw_full[b], main);
+                        if (main) bulk_g2s(dst, src, main, &B->raw_full[b]);
+                    } else {
+                        mbar_arrive(&B->raw_full[b]);
+                    }
+                    if (++b == nbuf) {
+                        b = 0;
+                        ++turn;
+                    }
+                }
+                // no copy outlives the CTA: every buffer's last one has landed (bounded, also after an error)
+                for (int k = 1; k <= nbuf && k <= n; ++k) {
+                    const int last = n - k;
+                    for (int x = 0; x < 4096 && !mbar_try_wait_hint(&B->raw_full[last % nbuf], (last / nbuf) & 1, 1000u); ++x) {}
                 }
             }
-            if (ok) {
-                fence_proxy_async_smem();
-                mbar_arrive(&B->k_full[sg]);
-            }
-            if (++nb == nbuf) nb = 0;
-            }
-            if constexpr (!K_Q) start(n + kAhead);
-            tree::cp_async_commit();
         }
-        tree::cp_async_wait<0>();
-        // after an error a bulk copy may still be under way: none outlives the CTA
-        for (int i = 0; t == 0 && outstanding > 0 && i < 4096; ++i, nb = nb + 1 == nbuf ? 0 : nb + 1)
-            if ((bulk_at >> nb & 1u) && mbar_try_wait_hint(&B->raw_full[nb], phase >> nb & 1u, 1000u)) {
-                bulk_at &= ~(1u << nb);
-                --outstanding;
-            }
     } else {
         // ------------------------------------------------------ MMA issuer of group g: the warp walks, one lane issues
         const int g = __shfl_sync(0xffffffffu, warp, 0) - 16;
