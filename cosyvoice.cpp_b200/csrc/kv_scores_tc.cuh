@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 const bool masked = any_out || p0 + kTcTile > r.L - r.n + 1;  // some (row, key) may be unseen
                 float d0 = 1.0f, d1 = 1.0f, m0 = 0.0f, m1 = 0.0f, s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
                 for (int r0 = 0; r0 < R; r0 += Sh::kSRows, ++k) {
-                    ok = tc_wait(&B->s_full[g][k & 1], (k >> 1) & 1, &B->err, a.status, 51);
+                    ok = tc_wait(&B->s_full[g][k & 1], (k >> 1) & 1, &B->err, 51);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     tc::fence_after();
                     if (K_Q && r0 == 0) {
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 while (lo + n >= r.end) r.next(a, pref, hi);
                 const int count = min(kTcTile, r.L - (r.t0 + lo + n - r.i) * kTcTile), sg = n & 1, b = n % nbuf;
                 const uint8_t* src = tile_rows(a, r, lo + n);
-                ok = ok && tc_wait(&B->raw_full[b], (n / nbuf) & 1, &B->err, a.status, 52);
+                ok = ok && tc_wait(&B->raw_full[b], (n / nbuf) & 1, &B->err, 52);
                 if (!fp::prod_bar_and(4 + g, 128, ok)) break;
                 uint8_t* raw = raw_at<KT>(smem, b);
                 const bool whole = whole_rows(a, src, slice);
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                     tree::cp_async_wait<0>();
                     asm volatile("bar.sync %0, 128;" ::"r"(4 + g) : "memory");
                 }
-                if (n >= 2) ok = tc_wait(&B->k_empty[sg], (n / 2 - 1) & 1, &B->err, a.status, 54);
+                if (n >= 2) ok = tc_wait(&B->k_empty[sg], (n / 2 - 1) & 1, &B->err, 54);
                 if (ok) {
                     const uint8_t* row = raw + (whole ? key * a.Hkv * slice + r.kvh * slice : key * raw_stride(KT));
                     uint8_t* tile = smem + Sh::kTiles + sg * kTcTileBytes;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                     while (e >= rf.end) rf.next(a, pref, hi);
                     const int count = min(kTcTile, rf.L - (rf.t0 + e - rf.i) * kTcTile);
                     const uint8_t* src = tile_rows(a, rf, e) + rf.kvh * slice;
-                    if (n >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (n / kSt - 1) & 1, &B->err, a.status, 53);
+                    if (n >= kSt) ok = ok && tc_wait(&B->k_empty[sg], (n / kSt - 1) & 1, &B->err, 53);
                     uint8_t* dst = smem + Sh::kTiles + sg * kTcTileBytes;
                     const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)a.k_nb1;
                     const int unit = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 2, w = 128 / unit, per = 128 / w;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 bool ok = true;
                 for (; ok && lo + n < hi; ++n) {
                     if (lo + n == r.end) r.next(a, pref, hi);
-                    if (turn) ok = tc_wait(&B->raw_empty[b], (turn - 1) & 1, &B->err, a.status, 58);
+                    if (turn) ok = tc_wait(&B->raw_empty[b], (turn - 1) & 1, &B->err, 58);
                     if (!ok) break;
                     const uint8_t* src = tile_rows(a, r, lo + n);
                     uint32_t main = 0;
@@ -469,15 +469,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         bool ok = true;
         for (; ok && r.i < hi; r.next(a, pref, hi), ++n_run) {
             const int R = r.n * a.G;
-            ok = tc_wait(&B->q_full, n_run & 1, &B->err, a.status, 55);
+            ok = tc_wait(&B->q_full, n_run & 1, &B->err, 55);
             for (int j = r.i + ((r.i ^ lo ^ g) & 1); ok && j < r.end; j += 2) {
                 const int n = j - lo, sg = n % kSt;
-                ok = tc_wait(&B->k_full[sg], (n / kSt) & 1, &B->err, a.status, 56);
+                ok = tc_wait(&B->k_full[sg], (n / kSt) & 1, &B->err, 56);
                 ok = __all_sync(0xffffffffu, ok);
                 tc::fence_after();
                 const uint64_t dk = dt0 + (uint64_t)(sg * (kTcTileBytes >> 4));
                 for (int r0 = 0; ok && r0 < R; r0 += Sh::kSRows, ++k) {
-                    if (k >= 2) ok = tc_wait(&B->s_empty[g][k & 1], ((k >> 1) - 1) & 1, &B->err, a.status, 57);
+                    if (k >= 2) ok = tc_wait(&B->s_empty[g][k & 1], ((k >> 1) - 1) & 1, &B->err, 57);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc::fence_after();
@@ -515,6 +515,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         tc::fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
+    if (tid == 0 && B->err) record_status(a.status, kStatusTimeout | (B->err << 8));
 }
 
 // Launch for K type KT (kv_scores_tc_inst.cu, one unit per K type).

@@ -8,10 +8,12 @@
 // them.  (Ragged sequences and few long ones fill the SMs alike.)
 //   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the
 //                   CTA's tiles 2 k + g
-//   warps 8-11      producer: raw rows by cp.async, then f16 tiles (128B swizzle);
-//                   f16 caches are copied straight into the tiles
-//   warp 12         issues S = Q K^T, up to two tiles ahead of the softmax
-//   warp 13         issues O = P V            (14, 15 fill up their warpgroup)
+//   warps 8-11      producer of the K tiles, 12-15 of the V tiles: cp.async of the raw rows
+//                   two tiles ahead, then thread = key: f16 tiles (128B swizzle) from
+//                   them; f16 caches are copied straight into the tiles
+//   warp 16         issues S = Q K^T, up to two tiles ahead of the softmax
+//   warp 17         issues O = P V
+//   (warps 18, 19 only complete the last warpgroup)
 // Precision: products of split numbers.  x = hi + lo in f16, S = Qh Kh + Ql Kh
 // (+ Qh Kl), O = Ph Vh + Pl Vh (+ Ph Vl); the dropped low x low term is 2^-22 of the
 // largest.  Q is scaled per row, K and V per tile, by powers of two so that hi and
@@ -34,10 +36,10 @@ namespace tree {
 
 constexpr int kTcTile = 128;
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 16 * 32;
-// Registers of a thread by role: launched with 128; 256 * 168 + 128 * 96 + 128 * 80 <= 512 * 128.
-constexpr int kTcRegsSoftmax = 168, kTcRegsProducer = 96, kTcRegsIssuer = 80;
-static_assert(256 * kTcRegsSoftmax + 128 * kTcRegsProducer + 128 * kTcRegsIssuer <= 65536, "the block's registers");
+constexpr int kTcThreads = 20 * 32;
+// Registers of a thread by role: launched with 96; 256 * 160 + 256 * 64 + 128 * 32 <= 640 * 96.
+constexpr int kTcRegsSoftmax = 160, kTcRegsProducer = 64, kTcRegsOther = 32;
+static_assert(256 * kTcRegsSoftmax + 256 * kTcRegsProducer + 128 * kTcRegsOther <= 640 * 96, "the block's registers");
 constexpr int kTcMaxSeq = 1024;       // prefix table in shared memory
 constexpr int kTcExps = 8;            // tiles whose scales may be in flight
 constexpr int kTcTileBytes = kTcTile * kD * 2;
@@ -54,13 +56,15 @@ struct TcArgs {
 
 struct TcBars {
     uint64_t k_full[5], v_full[5], k_empty[5], v_empty[5];  // by stage
+    uint64_t rawk_full[3], rawv_full[3];                    // by tile n % 3
     uint64_t q_full;
     uint64_t s_full[3], p_full[3], s_free[3];               // by S buffer
     uint64_t o_full[2];                                     // by group
     uint32_t tmem_base;
     int err;
-    uint32_t maxk[2], maxv[2];        // largest |scale| of a tile, by tile parity
-    float2 exps[kTcExps];             // 2^-e of K and V of tile i at i % kTcExps
+    uint32_t maxk[3], maxv[3];        // largest |scale| of tile n at n % 3
+    float expk[kTcExps], expv[kTcExps];  // 2^-e of K and V of tile n at n % kTcExps
+    uint32_t flags[kTcExps];          // 1: the tile starts a run, 2: drafted keys
     uint32_t bad[kTcExps][4];         // draft keys whose V is not finite
     int32_t first_run[12];            // Run at the start of the CTA's part
 };
@@ -74,8 +78,9 @@ struct TcShape {
     static constexpr int kQ = 0;                       // Q hi, Q lo; then the groups' halves at a run's end
     static constexpr int kTiles = 2 * kTcTileBytes;
     static constexpr int kRaw = kTiles + kStages * kStage;
-    static constexpr int kMl = kRaw + 2 * (rawK + rawV);
-    static constexpr int kBars = kMl + 2 * kTcRows * 8;
+    static constexpr int kMl = kRaw + 3 * (rawK + rawV);
+    static constexpr int kRs = kMl + 2 * kTcRows * 8;  // score factors of the rows
+    static constexpr int kBars = kRs + kTcRows * 4;
     static constexpr int kPref = kBars + (int)((sizeof(TcBars) + 15) / 16 * 16);
     static constexpr int kLen = kPref + (kTcMaxSeq + 4) * 4, kNodes = kLen + kTcMaxSeq * 4;
     static constexpr int kBytes = kNodes + kTcMaxSeq * 2;
@@ -101,20 +106,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// Bounded wait in little code (there are many): gives up after kWaitBudgetNs, or once another role has given up.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* err, int* status, int site) {
-    uint64_t t0 = 0;
+// Bounded wait in little code (it stands at every step of every role): gives up after kTcTries suspensions of up to 20 us, or
+// once another role has given up.  *err keeps the site; the kernel's end records it.
+constexpr uint32_t kTcTries = 100000;
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
 #pragma unroll 1
     for (uint32_t i = 0; !mbar_try_wait_hint(bar, parity, 20000u); ++i) {
-        if ((i & 63) != 63) continue;
-        const uint64_t now = global_timer_ns();
-        if (t0 == 0) t0 = now;
-        const bool late = now - t0 > kWaitBudgetNs;
-        if (late) {
-            record_status(status, kStatusTimeout | (site << 8));
-            *reinterpret_cast<volatile int*>(err) = 1;
-        }
-        if (late || *reinterpret_cast<volatile int*>(err)) return false;
+        if (i >= kTcTries) *reinterpret_cast<volatile int*>(err) = site;
+        if (*reinterpret_cast<volatile int*>(err)) return false;
     }
     return true;
 }
@@ -199,30 +198,63 @@ struct Run {
 __device__ __forceinline__ int tc_cut(int c, int n, int g) { return (int)((long long)c * n / g); }
 __device__ __forceinline__ int tc_owner(int i, int n, int g) { return (int)(((long long)(i + 1) * g - 1) / n); }
 
-// hi and lo of 32 values of one key into rows of two tiles; w holds exact integers (convert_group), d and m the block's
-// scale and min times the tile's power of two.
+// hi and lo of a key's 64 values into its rows of two tiles, times the tile's power of two f; `keep` false: zeros.  Eight
+// values at a time in a loop that is not unrolled: five roles run different code on an SM, and what they loop over has to
+// stay in its instruction cache together (64 sequences of up to 2048 positions, Q8_0 and Q4_0, 56 rows: 52.9 us unrolled, 43.3 so).
 template <int T>
-__device__ __forceinline__ void split_block(uint8_t* hi_tile, uint8_t* lo_tile, int key, int blk, const uint32_t (&w)[16], float d, float m) {
-    uint32_t h[16], l[16];
-    if constexpr (!BlockTraits<T>::HAS_MIN) {
+__device__ __forceinline__ void split_row(uint8_t* hi_tile, uint8_t* lo_tile, int key, const uint8_t* row, float f, bool keep) {
+    using BT = BlockTraits<T>;
+    constexpr bool kFive = BT::OFF_QH >= 0;
+    constexpr uint32_t bias = T == kQ8_0 ? dtc::kF16x2_1152 : kFive ? dtc::kF16x2_1040 : dtc::kF16x2_1032;
+    uint8_t* to = hi_tile + key * 128;
+    const int apart = (int)(lo_tile - hi_tile);
+    const uint32_t swz = (key & 7) << 4;
+#pragma unroll 1
+    for (int b = 0; b < 2; ++b) {
+        const uint8_t* g = row + b * group_bytes(T);
+        float d = h2f(*reinterpret_cast<const uint16_t*>(g)), m = 0.0f;
+        if constexpr (BT::HAS_MIN) m = fmaf(kFive ? 16.0f : 8.0f, d, h2f(*reinterpret_cast<const uint16_t*>(g + BT::OFF_M)));
+        d = keep ? d * f : 0.0f;
+        m = keep ? m * f : 0.0f;
         const __half2 d2 = __float2half2_rn(d);
+        uint32_t qh = 0;
+        if constexpr (kFive) qh = *reinterpret_cast<const uint16_t*>(g + BT::OFF_QH) | (uint32_t)*reinterpret_cast<const uint16_t*>(g + BT::OFF_QH + 2) << 16;
+        const uint32_t off = b * group_bytes(T) + BT::OFF_QS;  // rows start at multiples of 4
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(row + (off & ~3u));
+        const uint32_t turn = (off & 2) * 8;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            // bytes of the quants of values 8 c .. 8 c + 7
+            const uint32_t* w = words + 2 * (T == kQ8_0 ? c : c & 1);
+            const uint32_t mid = w[1];
+            uint32_t x[2] = {__funnelshift_r(w[0], mid, turn), __funnelshift_r(mid, w[2], turn)}, h[4], l[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const __half2 q = *reinterpret_cast<const __half2*>(&w[i]);
-            const __half2 p = __hmul2_rn(d2, q);
-            const __half2 e = __hfma2(d2, q, __hneg2(p));
-            h[i] = *reinterpret_cast<const uint32_t*>(&p);
-            l[i] = *reinterpret_cast<const uint32_t*>(&e);
-        }
-    } else {
+            for (int u = 0; u < 2; ++u) {
+                if constexpr (T == kQ8_0) {
+                    x[u] ^= 0x80808080u;
+                } else {
+                    x[u] = x[u] >> (4 * (c >> 1)) & 0x0f0f0f0fu;
+                    if constexpr (kFive) x[u] |= (((qh >> (8 * c + 4 * u) & 15u) * 0x00204081u) & 0x01010101u) << 4;
+                }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            split2(fmaf(q.x, d, m), fmaf(q.y, d, m), h[i], l[i]);
+                for (int v = 0; v < 2; ++v) {  // exact integers in f16
+                    const uint32_t n = dtc::hsub2_u32(__byte_perm(x[u], 0x64646464u, v ? 0x4342u : 0x4140u), bias);
+                    const __half2 q = *reinterpret_cast<const __half2*>(&n);
+                    if constexpr (BT::HAS_MIN) {
+                        const float2 y = __half22float2(q);
+                        split2(fmaf(y.x, d, m), fmaf(y.y, d, m), h[2 * u + v], l[2 * u + v]);
+                    } else {
+                        const __half2 p = __hmul2_rn(d2, q), e = __hfma2(d2, q, __hneg2(p));
+                        h[2 * u + v] = *reinterpret_cast<const uint32_t*>(&p);
+                        l[2 * u + v] = *reinterpret_cast<const uint32_t*>(&e);
+                    }
+                }
+            }
+            uint8_t* at = to + ((uint32_t)(64 * b + 16 * c) ^ swz);
+            *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(at + apart) = make_uint4(l[0], l[1], l[2], l[3]);
         }
     }
-    store_block(hi_tile, key, blk, h);
-    store_block(lo_tile, key, blk, l);
 }
 
 // Power of two that brings the largest scale (or min) of a tile to [2^6, 2^7): quants times it stay below 2^15.
@@ -232,11 +264,225 @@ __device__ __forceinline__ int tile_exp(float mx) {
     return e > 100 ? 100 : (e < -100 ? -100 : e);
 }
 
+// Rows of list entry e (every head), of K or V.
+struct TileRows {
+    const uint8_t* at;
+    int64_t nb1;
+    int count;
+    bool draft;
+};
+__device__ __forceinline__ TileRows tile_rows(const Args& a, const Run& r, int e, bool kV) {
+    TileRows x;
+    int p0;
+    r.tile(e, x.draft, p0, x.count);
+    x.nb1 = x.draft ? (kV ? a.vd_nb1 : a.kd_nb1) : (kV ? a.v_nb1 : a.k_nb1);
+    const uint8_t* b = x.draft ? (kV ? a.vd + (int64_t)r.s * a.vd_nb2 : a.kd + (int64_t)r.s * a.kd_nb2)
+                               : (kV ? seq_base(a.v_seq_ptrs, a.v, a.v_nb2, r.s) : seq_base(a.k_seq_ptrs, a.k, a.k_nb2, r.s));
+    x.at = b + (int64_t)p0 * x.nb1;
+    return x;
+}
+
+// A producer group's 128 threads: the slices of run r's head in the rows of entry e, to rows of raw_stride bytes; every
+// thread's copies arrive on `full`.
+template <int T>
+__device__ __forceinline__ void load_slices(const Args& a, const Run& r, int e, uint8_t* dst, uint64_t* full, int t, bool kV) {
+    constexpr int kWords = group_bytes(T) / 2, per = 128 / kWords;  // 4-byte words of a slice, keys per pass
+    const TileRows x = tile_rows(a, r, e, kV);
+    const uint8_t* src = x.at + r.kvh * 2 * group_bytes(T);
+    if (((reinterpret_cast<uint64_t>(src) | (uint64_t)x.nb1) & 3) == 0) {
+        const int k0 = t / kWords, col = (t - k0 * kWords) * 4;
+        if (k0 < per) {
+            const uint8_t* from = src + (int64_t)k0 * x.nb1 + col;
+            uint32_t to = smem_addr(dst + k0 * raw_stride(T) + col);
+            const int64_t step = (int64_t)per * x.nb1;
+#pragma unroll 4
+            for (int kk = k0; kk < x.count; kk += per, from += step, to += per * raw_stride(T))
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(full)) : "memory");
+    } else {
+        constexpr int kHalves = 2 * kWords;
+#pragma unroll 1
+        for (int i = t; i < x.count * kHalves; i += 128) {
+            const int kk = i / kHalves, h = i - kk * kHalves;
+            *reinterpret_cast<uint16_t*>(dst + kk * raw_stride(T) + 2 * h) = *reinterpret_cast<const uint16_t*>(src + (int64_t)kk * x.nb1 + 2 * h);
+        }
+        mbar_arrive(full);
+    }
+}
+
+// Largest |scale| of a row's two blocks (for types with a min a bound of |value| / 64), finite ones only.
+template <int T>
+__device__ __forceinline__ uint32_t row_max(const uint8_t* row, bool& special) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const uint8_t* gb = row + b * group_bytes(T);
+        float d = fabsf(h2f(*reinterpret_cast<const uint16_t*>(gb)));
+        if constexpr (BlockTraits<T>::HAS_MIN) {
+            const float mm = h2f(*reinterpret_cast<const uint16_t*>(gb + BlockTraits<T>::OFF_M));
+            special |= !isfinite(mm);
+            d = (32.0f * d + fabsf(mm)) * (1.0f / 64.0f);
+        }
+        special |= !isfinite(d);
+        if (isfinite(d)) m = max(m, __float_as_uint(d));
+    }
+    return m;
+}
+
+// A producer warpgroup: the K (or V) tiles of the CTA, thread = key.
+template <int KT, int VT, bool kV>
+__device__ __forceinline__ void produce(const TcArgs& ta, uint8_t* smem, TcBars* B, const SeqTab& tab, Run r, int lo, int hi) {
+    using Sh = TcShape<KT, VT>;
+    constexpr int T = kV ? VT : KT, kSt = Sh::kStages, kBar = kV ? 5 : 4, raw = kV ? Sh::rawV : Sh::rawK;
+    const Args& a = ta.a;
+    const int key = threadIdx.x - (kV ? 384 : 256), lane = threadIdx.x & 31;
+    uint8_t* tiles0 = smem + Sh::kTiles + (kV ? Sh::NK * kTcTileBytes : 0);
+    uint64_t* full = kV ? B->v_full : B->k_full;
+    uint64_t* empty = kV ? B->v_empty : B->k_empty;
+    bool ok = true;
+    if constexpr (T != kF16) {
+        uint64_t* raw_full = kV ? B->rawv_full : B->rawk_full;
+        uint32_t* slots = kV ? B->maxv : B->maxk;
+        uint8_t* raw0 = smem + Sh::kRaw + (kV ? 3 * Sh::rawK : 0);
+        Run rs = r;  // run of the tile that is fetched, two ahead of the one that is converted
+        int st = 0, slot = 0, ahead = 0, first = 1;  // slot, ahead: n % 3, (n + 2) % 3
+        uint32_t use = 0, turn = 0;                  // n / kSt, n / 3
+#pragma unroll 1
+        for (int n = -2; lo + n < hi; ++n) {
+            bool draft = false, bad = false, there = false;
+            const uint8_t* row = raw0 + slot * raw + key * raw_stride(T);
+            if (n >= 0) {
+                if (lo + n == r.end) {
+                    r.next(a, tab, hi);
+                    first = 1;
+                }
+                int p0, count;
+                r.tile(lo + n, draft, p0, count);
+                there = key < count;
+                ok = ok && tc_wait(&raw_full[slot], turn & 1, &B->err, kV ? 43 : 42);
+                const uint32_t m = __reduce_max_sync(0xffffffffu, ok && there ? row_max<T>(row, bad) : 0u);
+                if (lane == 0 && m) atomicMax(&slots[slot], m);
+                if (!fp::prod_bar_and(kBar, 128, ok)) break;  // (all leave together)
+            }
+            // every thread is past tile n - 1, whose buffer takes tile n + 2
+            if (lo + n + 2 < hi) {
+                if (lo + n + 2 == rs.end) rs.next(a, tab, hi);
+                load_slices<T>(a, rs, lo + n + 2, raw0 + ahead * raw, &raw_full[ahead], key, kV);
+            }
+            ahead = ahead == 2 ? 0 : ahead + 1;
+            if (n < 0) continue;
+            const int e = tile_exp(__uint_as_float(slots[slot]));
+            if (++slot == 3) {
+                slot = 0;
+                ++turn;
+            }
+            if (key == 0) {
+                slots[slot == 2 ? 0 : slot + 1] = 0u;  // of the tile after the next: read by all before this barrier
+                (kV ? B->expv : B->expk)[n % kTcExps] = pow2f(-e);
+                if (!kV) B->flags[n % kTcExps] = (uint32_t)first | (draft ? 2u : 0u);
+            }
+            first = 0;
+            if (kV && draft) {  // which keys hold values that are not finite (their tile rows are zeros)
+                const uint32_t vote = __ballot_sync(0xffffffffu, bad);
+                if (lane == 0) B->bad[n % kTcExps][key >> 5] = vote;
+            }
+            const bool keep = there && !(kV && draft && bad);
+            const float f = pow2f(e);
+            if (use) ok = ok && tc_wait(&empty[st], (use - 1) & 1, &B->err, kV ? 36 : 35);
+            if (ok) {
+                uint8_t* tile = tiles0 + st * Sh::kStage;
+                split_row<T>(tile, tile + kTcTileBytes, key, row, f, keep);
+                fence_proxy_async_smem();
+                mbar_arrive(&full[st]);
+            }
+            if (++st == kSt) {
+                st = 0;
+                ++use;
+            }
+        }
+        cp_async_wait<0>();
+    } else {
+        // f16 rows straight into the tiles, kPre of them ahead of the one that is handed on
+        constexpr int kPre = kSt - 2, slice = 2 * kD;
+        Run rs = r;
+        auto start = [&](int n) {
+            if (lo + n < hi) {
+                if (lo + n == rs.end) rs.next(a, tab, hi);
+                const TileRows x = tile_rows(a, rs, lo + n, kV);
+                const uint8_t* src = x.at + rs.kvh * slice;
+                if (n >= kSt) ok = ok && tc_wait(&empty[n % kSt], (n / kSt - 1) & 1, &B->err, kV ? 34 : 33);
+                uint8_t* dst = tiles0 + (n % kSt) * Sh::kStage;
+                const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)x.nb1;
+                if (ok && (al & 15) == 0) {
+                    // 8 chunks of 16 bytes per key: this thread's chunk of every 16th key, whose swizzle is the same
+                    const int k0 = key >> 3, col = (key & 7) << 4;
+                    const uint8_t* from = src + (int64_t)k0 * x.nb1 + col;
+                    uint8_t* to = dst + k0 * 128 + (col ^ ((k0 & 7) << 4));
+                    const int64_t step = 16 * x.nb1;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) cp_async16(to + u * 2048, k0 + 16 * u < x.count ? from + u * step : src, k0 + 16 * u < x.count);
+                } else if (ok) {
+                    const int unit = (al & 3) == 0 ? 4 : 2, w = slice / unit, per = unit;
+                    const int k0 = key / w, col = (key - k0 * w) * unit;
+#pragma unroll 1
+                    for (int kk = k0; kk < kTcTile; kk += per) {
+                        const bool there = kk < x.count;
+                        const uint8_t* from = there ? src + (int64_t)kk * x.nb1 + col : src;
+                        uint8_t* to = dst + kk * 128 + (col ^ ((kk & 7) << 4));
+                        if (unit == 4) cp_async4(to, from, there);
+                        else *reinterpret_cast<uint16_t*>(to) = there ? *reinterpret_cast<const uint16_t*>(from) : (uint16_t)0;
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+        int first = 1;
+#pragma unroll 1
+        for (int n = -kPre; lo + n < hi; ++n) {
+            if (n >= 0) {
+                if (lo + n == r.end) {
+                    r.next(a, tab, hi);
+                    first = 1;
+                }
+                bool draft;
+                int p0, count;
+                r.tile(lo + n, draft, p0, count);
+                cp_async_wait<kPre - 1>();
+                if (kV && draft) {
+                    if (!fp::prod_bar_and(kBar, 128, ok)) break;  // every thread's copies have landed (or all leave)
+                    bool bad = false;
+                    uint4* p = reinterpret_cast<uint4*>(tiles0 + (n % kSt) * Sh::kStage + key * 128);
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 w = p[c];
+                        bad |= f16x2_special(w.x) || f16x2_special(w.y) || f16x2_special(w.z) || f16x2_special(w.w);
+                    }
+#pragma unroll 1
+                    for (int c = 0; bad && c < 8; ++c) p[c] = make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t vote = __ballot_sync(0xffffffffu, bad);
+                    if (lane == 0) B->bad[n % kTcExps][key >> 5] = vote;
+                }
+                if (key == 0) {
+                    (kV ? B->expv : B->expk)[n % kTcExps] = 1.0f;
+                    if (!kV) B->flags[n % kTcExps] = (uint32_t)first | (draft ? 2u : 0u);
+                }
+                first = 0;
+                if (ok) {
+                    fence_proxy_async_smem();
+                    mbar_arrive(&full[n % kSt]);
+                }
+            }
+            start(n + kPre);  // (may have to wait for its stage, so it comes last)
+        }
+        cp_async_wait<0>();
+    }
+}
+
 template <int KT, int VT>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ TcArgs ta) {
     using Sh = TcShape<KT, VT>;
     constexpr int NK = Sh::NK, NV = Sh::NV, kSt = Sh::kStages;
-    constexpr int sliceK = 2 * group_bytes(KT), sliceV = 2 * group_bytes(VT);
     extern __shared__ __align__(1024) uint8_t smem[];
     const Args& a = ta.a;
     TcBars* B = reinterpret_cast<TcBars*>(smem + Sh::kBars);
@@ -263,7 +509,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(&B->o_full[g], 1);
-            B->maxk[g] = B->maxv[g] = 0u;
+        }
+        for (int b = 0; b < 3; ++b) {
+            mbar_init(&B->rawk_full[b], 128);
+            mbar_init(&B->rawv_full[b], 128);
+            B->maxk[b] = B->maxv[b] = 0u;
         }
         B->err = 0;
         fence_mbar_init();
@@ -324,6 +574,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         uint8_t* qlo = qhi + kTcTileBytes;
         float4* xch = reinterpret_cast<float4*>(smem + Sh::kQ) + row * 16;  // group 1's output row at a run's end
         float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl) + row;
+        float* rsb = reinterpret_cast<float*>(smem + Sh::kRs);
         uint32_t k = 0;  // tiles of this group so far
         bool ok = true;
         for (; r.i < hi; r.next(a, tab, hi)) {
@@ -332,50 +583,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
             const int node = (int)(((uint32_t)rr * ta.inv_g) >> 16), h = r.kvh * a.G + rr - node * a.G;
             const int64_t orow = (int64_t)r.s * a.out_nb_seq + (int64_t)node * a.out_nb_node + h * kD;
-            // Q: both groups look at the whole row, each writes its half of the dims
-            float rs;
-            {
-                const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)node * a.q_nb_node + h * kD);
-                float am = 0.0f;
-                if (real) {
-#pragma unroll 4
-                    for (int c = 0; c < 16; ++c) {
-                        const float4 v = q[c];
-                        am = max3(am, fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-                    }
-                }
-                const int ex = dtc::norm_exp(am);
-                const float sc = a.scale_log2 < 0.0f ? -pow2f(ex) : pow2f(ex);
-                rs = pow2f(-ex) * fabsf(a.scale_log2);
-                // nothing reads the last run's Q, or its exchanged rows, any more
-                if (r.i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
+            // Q: four lanes a row, 16 dims each
+            // (nothing reads the last run's Q, or its exchanged rows, any more)
+            if (r.i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll 1
-                for (int c = 4 * g; c < 4 * g + 4; ++c) {
-                    const float4 u = real ? q[2 * c] : make_float4(0.f, 0.f, 0.f, 0.f), v = real ? q[2 * c + 1] : u;
+            for (int q0 = tid >> 2; q0 < kTcRows; q0 += 64) {
+                const int qr = r.rt * kTcRows + q0, qn = (int)(((uint32_t)qr * ta.inv_g) >> 16), c = lane & 3;
+                const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)qn * a.q_nb_node +
+                                                                  (r.kvh * a.G + qr - qn * a.G) * kD + 16 * c);
+                float4 v[4];
+                float am = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = qr < rows ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) am = max3(am, fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w)));
+                const int ex = dtc::norm_exp(quad_max(am));
+                const float sc = a.scale_log2 < 0.0f ? -pow2f(ex) : pow2f(ex);
+                if (c == 0) rsb[q0] = pow2f(-ex) * fabsf(a.scale_log2);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
                     uint4 wh, wl;
-                    split2(u.x * sc, u.y * sc, wh.x, wl.x);
-                    split2(u.z * sc, u.w * sc, wh.y, wl.y);
-                    split2(v.x * sc, v.y * sc, wh.z, wl.z);
-                    split2(v.z * sc, v.w * sc, wh.w, wl.w);
-                    const uint32_t at = tc::sw128_offset(row, c);
+                    split2(v[2 * u].x * sc, v[2 * u].y * sc, wh.x, wl.x);
+                    split2(v[2 * u].z * sc, v[2 * u].w * sc, wh.y, wl.y);
+                    split2(v[2 * u + 1].x * sc, v[2 * u + 1].y * sc, wh.z, wl.z);
+                    split2(v[2 * u + 1].z * sc, v[2 * u + 1].w * sc, wh.w, wl.w);
+                    const uint32_t at = tc::sw128_offset(q0, 2 * c + u);
                     *reinterpret_cast<uint4*>(qhi + at) = wh;
                     *reinterpret_cast<uint4*>(qlo + at) = wl;
                 }
-                fence_proxy_async_smem();
-                mbar_arrive(&B->q_full);
             }
+            fence_proxy_async_smem();
+            mbar_arrive(&B->q_full);
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            const float rs = rsb[row];
             float2 O[32];
 #pragma unroll
             for (int d = 0; d < 32; ++d) O[d] = make_float2(0.f, 0.f);
-            float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 0.0f;
-            bool pending = false;  // a tile's output still to be added, times vs_last
+            float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 1.0f;
+            bool pending = false;  // a tile's output still to be added, times vs_last and its V's 2^-e
+            int n_last = 0;        // that tile
             bool spoiled = false;  // the row sees a drafted value that is not finite
             auto add_output = [&]() {
                 uint32_t o0[32], o1[32];
                 tc::tmem_ld32(ot, o0);
                 tc::tmem_ld32(ot + 32, o1);
                 tc::tmem_ld_wait();
-                const float2 f = make_float2(vs_last, vs_last);
+                const float vs = vs_last * B->expv[n_last % kTcExps];
+                const float2 f = make_float2(vs, vs);
 #pragma unroll
                 for (int d = 0; d < 16; ++d) {
                     O[d] = ffma2(make_float2(__uint_as_float(o0[2 * d]), __uint_as_float(o0[2 * d + 1])), f, O[d]);
@@ -388,14 +642,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 r.tile(j, draft, p0, count);
                 const int n = j - lo, buf = n % 3;
                 const uint32_t sp = tmem + lane_base + buf * 128;
-                ok = tc_wait(&B->s_full[buf], (n / 3) & 1, &B->err, a.status, 31);
+                ok = tc_wait(&B->s_full[buf], (n / 3) & 1, &B->err, 31);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc::fence_after();
                 if (warp_real) {
                     uint32_t sv[32];
                     tc::tmem_ld32(sp, sv);
-                    const float2 ex = B->exps[(j - lo) % kTcExps];
-                    const float rst = fmaxf(rs * ex.x, 1e-37f);  // above 0, so that what is masked stays -infinity
+                    const float rst = fmaxf(rs * B->expk[n % kTcExps], 1e-37f);  // above 0, so that what is masked stays -infinity
                     const bool masked = draft || count < kTcTile;
                     tc::tmem_ld_wait();
 #pragma unroll 1
@@ -494,12 +747,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                         tc::tmem_ld_wait();
                     }
                     if (pending) {  // the output of the group's tile before this one (o_full counts every tile of the group)
-                        ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
+                        ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, 32);
                         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                         tc::fence_after();
                         add_output();
                     }
-                    vs_last = ex.y;
+                    vs_last = 1.0f;
+                    n_last = n;
                     pending = true;
                     tc::tmem_st_wait();
                 }
@@ -508,7 +762,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 mbar_arrive(&B->p_full[buf]);
             }
             if (ok && pending) {
-                ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, a.status, 32);
+                ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, 32);
                 ok = __all_sync(0xffffffffu, ok);
                 tc::fence_after();
                 if (ok) add_output();
@@ -546,251 +800,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
         }
     } else if (warp < 12) {
-        // ------------------------------------------------------ producer: thread = key
         regs_down<kTcRegsProducer>();
-        const int key = tid - 256;
-        // keys [0, count) of a tile into shared memory, zeros up to 128
-        auto copy = [&](auto type_tag, bool raw, uint8_t* dst, const uint8_t* src, int64_t nb1, int count) {
-            constexpr int T = decltype(type_tag)::value;
-            const uint64_t al = reinterpret_cast<uint64_t>(src) | (uint64_t)nb1;
-            if (T == kF16 && (al & 15) == 0) {
-                // 8 chunks of 16 bytes per key: this thread's chunk of every 16th key, whose swizzle is the same
-                const int k0 = key >> 3, col = (key & 7) << 4;
-                const uint8_t* from = src + (int64_t)k0 * nb1 + col;
-                uint8_t* to = dst + k0 * 128 + (col ^ ((k0 & 7) << 4));
-                const int64_t step = 16 * nb1;
-                if (count == kTcTile) {
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) cp_async16(to + u * 2048, from + u * step, true);
-                } else {
-#pragma unroll 1
-                    for (int u = 0; u < 8; ++u) cp_async16(to + u * 2048, k0 + 16 * u < count ? from + u * step : src, k0 + 16 * u < count);
-                }
-                return;
-            }
-            const int unit = (al & 3) == 0 ? 4 : 2;
-            const int w = 2 * group_bytes(T) / unit, per = unit == 4 ? 128 / (group_bytes(T) / 2) : 128 / group_bytes(T);
-            const int k0 = unit == 4 ? key / (group_bytes(T) / 2) : key / group_bytes(T), col = (key - k0 * w) * unit;
-            if (k0 >= per) return;
-            const uint8_t* from = src + (int64_t)k0 * nb1 + col;
-            const int64_t step = (int64_t)per * nb1;
-            if (raw && unit == 4) {
-                uint8_t* to = dst + k0 * raw_stride(T) + col;
-                const int tstep = per * raw_stride(T);
-                int kk = k0;
-#pragma unroll 4
-                for (; kk < count; kk += per, from += step, to += tstep) cp_async4(to, from, true);
-#pragma unroll 1
-                for (; kk < kTcTile; kk += per, to += tstep) *reinterpret_cast<uint32_t*>(to) = 0u;
-                return;
-            }
-#pragma unroll 1
-            for (int kk = k0; kk < kTcTile; kk += per, from += step) {
-                const bool there = kk < count;
-                uint8_t* to = raw ? dst + kk * raw_stride(T) + col : dst + kk * 128 + (col ^ ((kk & 7) << 4));
-                if (unit == 4) cp_async4(to, there ? from : src, there);
-                else *reinterpret_cast<uint16_t*>(to) = there ? *reinterpret_cast<const uint16_t*>(from) : (uint16_t)0;
-            }
-        };
-        // the runs of the tile whose copies start and of the tile that is finished
-        Run ri = r, rc = r;
-        int ii = lo;
-        bool ok = true;
-        auto issue = [&](int n) {        // copies of the CTA's tile n (list entry ii)
-            if (ii < hi) {
-                if (ii == ri.end) ri.next(a, tab, hi);
-                bool draft;
-                int p0, count;
-                ri.tile(ii, draft, p0, count);
-                const uint8_t* ks = (draft ? a.kd + (int64_t)ri.s * a.kd_nb2 : seq_base(a.k_seq_ptrs, a.k, a.k_nb2, ri.s)) + ri.kvh * sliceK;
-                const uint8_t* vs = (draft ? a.vd + (int64_t)ri.s * a.vd_nb2 : seq_base(a.v_seq_ptrs, a.v, a.v_nb2, ri.s)) + ri.kvh * sliceV;
-                const int64_t nk = draft ? a.kd_nb1 : a.k_nb1, nv = draft ? a.vd_nb1 : a.v_nb1;
-                const int st = n % kSt;
-                uint8_t* tiles = smem + Sh::kTiles + st * Sh::kStage;
-                uint8_t* raw = smem + Sh::kRaw + (n & 1) * (Sh::rawK + Sh::rawV);
-                const uint32_t use = n / kSt;
-                if constexpr (NK == 1)
-                    if (use > 0) ok = ok && tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 33);
-                if (ok) copy(std::integral_constant<int, KT>{}, NK == 2, NK == 2 ? raw : tiles, ks + (int64_t)p0 * nk, nk, count);
-                if constexpr (NV == 1)
-                    if (use > 0) ok = ok && tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 34);
-                if (ok) copy(std::integral_constant<int, VT>{}, NV == 2, NV == 2 ? raw + Sh::rawK : tiles + NK * kTcTileBytes, vs + (int64_t)p0 * nv, nv, count);
-                ++ii;
-            }
-            cp_async_commit();
-        };
-        constexpr int kAhead = NK + NV == 2 ? kSt - 2 : 1;  // tiles whose copies run ahead of the finished one
-#pragma unroll 1
-        for (int n = -kAhead; lo + n < hi; ++n) {
-            if (n >= 0) {
-                cp_async_wait<kAhead - 1>();
-                // every thread's copies of the tile have landed, and every thread is done with the tile before (or all leave)
-                if (!fp::prod_bar_and(4, 128, ok)) break;
-            }
-            // raw copies of the next tile first; copies into a stage may have to wait for it, so they come last
-            if constexpr (NK + NV == 4) issue(n + kAhead);
-            if (n >= 0) {
-            if (lo + n == rc.end) rc.next(a, tab, hi);
-            bool draft;
-            int p0, count;
-            rc.tile(lo + n, draft, p0, count);
-            const int st = n % kSt;
-            const uint32_t use = n / kSt;
-            uint8_t* tiles = smem + Sh::kTiles + st * Sh::kStage;
-            const uint8_t* rawk = smem + Sh::kRaw + (n & 1) * (Sh::rawK + Sh::rawV);
-            const uint8_t* rawv = rawk + Sh::rawK;
-            bool bad = false;
-            float fk = 1.0f, fv = 1.0f;
-            if constexpr (NK + NV > 2) {
-                // the tile's largest scales
-                uint32_t mk = 0, mv = 0;
-                auto scale_max = [&](auto type_tag, const uint8_t* rowp, bool& special) {
-                    constexpr int T = decltype(type_tag)::value;
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint8_t* gb = rowp + b * group_bytes(T);
-                        float d = fabsf(h2f(*reinterpret_cast<const uint16_t*>(gb)));
-                        if constexpr (BlockTraits<T>::HAS_MIN) {
-                            // |d q + m| <= 16 d + |m + 16 d|: in units of 127 quants of a scale
-                            const float mm = h2f(*reinterpret_cast<const uint16_t*>(gb + BlockTraits<T>::OFF_M));
-                            special |= !isfinite(mm);
-                            d = (32.0f * d + fabsf(mm)) * (1.0f / 64.0f);
-                        }
-                        special |= !isfinite(d);
-                        if (isfinite(d)) m = max(m, __float_as_uint(d));
-                    }
-                    return __reduce_max_sync(0xffffffffu, m);
-                };
-                bool kbad = false;
-                if constexpr (NK == 2) mk = scale_max(std::integral_constant<int, KT>{}, rawk + key * raw_stride(KT), kbad);
-                if constexpr (NV == 2) mv = scale_max(std::integral_constant<int, VT>{}, rawv + key * raw_stride(VT), bad);
-                if (lane == 0) {
-                    if (mk) atomicMax(&B->maxk[n & 1], mk);
-                    if (mv) atomicMax(&B->maxv[n & 1], mv);
-                }
-                asm volatile("bar.sync 5, 128;" ::: "memory");
-                const int ek = tile_exp(__uint_as_float(B->maxk[n & 1])), ev = tile_exp(__uint_as_float(B->maxv[n & 1]));
-                fk = pow2f(ek);
-                fv = pow2f(ev);
-                if (key == 0) {
-                    B->exps[n % kTcExps] = make_float2(NK == 2 ? pow2f(-ek) : 1.0f, NV == 2 ? pow2f(-ev) : 1.0f);
-                    B->maxk[(n + 1) & 1] = B->maxv[(n + 1) & 1] = 0u;
-                }
-            } else if (key == 0) {
-                B->exps[n % kTcExps] = make_float2(1.0f, 1.0f);
-            }
-            if constexpr (NV == 1) {
-                if (draft) {  // this thread's key
-                    uint4* p = reinterpret_cast<uint4*>(tiles + NK * kTcTileBytes + key * 128);
-                    for (int c = 0; c < 8; ++c) {
-                        const uint4 w = p[c];
-                        bad |= f16x2_special(w.x) || f16x2_special(w.y) || f16x2_special(w.z) || f16x2_special(w.w);
-                    }
-                    if (bad)
-                        for (int c = 0; c < 8; ++c) p[c] = make_uint4(0u, 0u, 0u, 0u);
-                }
-            }
-            if (draft) {  // (the softmax reads it with S)
-                const uint32_t vote = __ballot_sync(0xffffffffu, bad);
-                if (lane == 0) B->bad[n % kTcExps][key >> 5] = vote;
-            }
-            if constexpr (NK == 2) {
-                if (use > 0) ok = ok && tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, a.status, 35);
-                if (ok) {
-                    uint32_t w0[16], w1[16];
-                    float d0, m0, d1, m1;
-                    convert_block<KT, 0>(rawk + key * raw_stride(KT), w0, d0, m0);
-                    convert_block<KT, 1>(rawk + key * raw_stride(KT), w1, d1, m1);
-                    split_block<KT>(tiles, tiles + kTcTileBytes, key, 0, w0, d0 * fk, m0 * fk);
-                    split_block<KT>(tiles, tiles + kTcTileBytes, key, 1, w1, d1 * fk, m1 * fk);
-                }
-            }
-            if (ok) {
-                fence_proxy_async_smem();
-                mbar_arrive(&B->k_full[st]);
-            }
-            if constexpr (NV == 2) {
-                if (use > 0) ok = ok && tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, a.status, 36);
-                if (ok) {
-                    const bool drop = draft && bad;
-                    uint32_t w0[16], w1[16];
-                    float d0, m0, d1, m1;
-                    convert_block<VT, 0>(rawv + key * raw_stride(VT), w0, d0, m0);
-                    convert_block<VT, 1>(rawv + key * raw_stride(VT), w1, d1, m1);
-                    uint8_t* vt = tiles + NK * kTcTileBytes;
-                    split_block<VT>(vt, vt + kTcTileBytes, key, 0, w0, drop ? 0.0f : d0 * fv, drop ? 0.0f : m0 * fv);
-                    split_block<VT>(vt, vt + kTcTileBytes, key, 1, w1, drop ? 0.0f : d1 * fv, drop ? 0.0f : m1 * fv);
-                }
-            }
-            if (ok) {
-                fence_proxy_async_smem();
-                mbar_arrive(&B->v_full[st]);
-            }
-            }
-            if constexpr (NK + NV < 4) issue(n + kAhead);
-        }
-        cp_async_wait<0>();
+        produce<KT, VT, false>(ta, smem, B, tab, r, lo, hi);
+    } else if (warp < 16) {
+        regs_down<kTcRegsProducer>();
+        produce<KT, VT, true>(ta, smem, B, tab, r, lo, hi);
     } else {
-        regs_down<kTcRegsIssuer>();
+        regs_down<kTcRegsOther>();
         // ------------------------------------------------------ MMA issuers: the whole warp walks, one lane issues
         const int which = __shfl_sync(0xffffffffu, warp, 0);
         const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
         bool ok = true;
-        if (which == 12) {
+        if (which == 16) {
             const uint32_t idesc = tc::idesc_f16_f32(128, kTcTile, false);
             const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
             const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
-            uint32_t n_run = 0;
-            int n = 0, st = 0, buf = 0;
-            uint32_t use = 0, turn = 0;  // n / kSt, n / 3
-            for (; ok && r.i < hi; r.next(a, tab, hi), ++n_run) {
-                ok = tc_wait(&B->q_full, n_run & 1, &B->err, a.status, 37);
-                for (int j = r.i; ok && j < r.end; ++j, ++n) {
-                    ok = tc_wait(&B->k_full[st], use & 1, &B->err, a.status, 38);
-                    if (ok && n >= 3) ok = tc_wait(&B->s_free[buf], (turn - 1) & 1, &B->err, a.status, 40);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc::fence_after();
-                    const uint64_t dk = dt0 + (uint64_t)(st * (Sh::kStage >> 4));
-                    const uint32_t sp = tmem + buf * 128;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {  // small terms first, while the sums are small
-                            tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc, kk > 0 ? 1u : 0u);
-                            if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc, 1u);
-                        }
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc, 1u);
-                        tc::mma_commit(&B->s_full[buf]);
-                        tc::mma_commit(&B->k_empty[st]);
-                    }
-                    __syncwarp();
-                    if (++st == kSt) { st = 0; ++use; }
-                    if (++buf == 3) { buf = 0; ++turn; }
-                }
+            int st = 0, buf = 0;
+            uint32_t use = 0, turn = 0, n_run = 0;  // n / kSt, n / 3
+            for (int n = 0; ok && lo + n < hi; ++n) {
+                ok = tc_wait(&B->k_full[st], use & 1, &B->err, 38);
+                const uint32_t flags = B->flags[n % kTcExps];
+                if (ok && (flags & 1)) ok = tc_wait(&B->q_full, n_run++ & 1, &B->err, 37);
+                if (ok && (flags & 2)) ok = tc_wait(&B->v_full[st], use & 1, &B->err, 44);  // (which values are bad)
+                if (ok && n >= 3) ok = tc_wait(&B->s_free[buf], (turn - 1) & 1, &B->err, 40);
                 ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::fence_after();
+                const uint64_t dk = dt0 + (uint64_t)(st * (Sh::kStage >> 4));
+                const uint32_t sp = tmem + buf * 128;
+                if (elect_one()) {
+#pragma unroll 1
+                    for (int kk = 0; kk < 4; ++kk) {  // small terms first, while the sums are small
+                        tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc, kk > 0 ? 1u : 0u);
+                        if constexpr (NK == 2) tc::mma_ss(sp, dqh + kk * 2, dk + (kTcTileBytes >> 4) + kk * 2, idesc, 1u);
+                    }
+#pragma unroll 1
+                    for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc, 1u);
+                    tc::mma_commit(&B->s_full[buf]);
+                    tc::mma_commit(&B->k_empty[st]);
+                }
+                __syncwarp();
+                if (++st == kSt) { st = 0; ++use; }
+                if (++buf == 3) { buf = 0; ++turn; }
             }
-        } else if (which == 13) {
+        } else if (which == 17) {
             const uint32_t idesc = tc::idesc_f16_f32(128, 64, true);
             int st = 0, buf = 0;
             uint32_t use = 0, turn = 0;
             for (int n = 0; ok && lo + n < hi; ++n) {
-                ok = tc_wait(&B->v_full[st], use & 1, &B->err, a.status, 41);
-                if (ok) ok = tc_wait(&B->p_full[buf], turn & 1, &B->err, a.status, 39);
+                ok = tc_wait(&B->v_full[st], use & 1, &B->err, 41);
+                if (ok) ok = tc_wait(&B->p_full[buf], turn & 1, &B->err, 39);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc::fence_after();
                 const uint64_t dv = dt0 + (uint64_t)(st * (Sh::kStage >> 4) + NK * (kTcTileBytes >> 4));
                 const uint32_t sp = tmem + buf * 128, ot = tmem + 384 + (n & 1) * 64;
                 if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
                     for (int kk = 0; kk < 8; ++kk) {
                         const uint32_t ph = sp + 32 * (kk >> 1) + 8 * (kk & 1);
                         tc::mma_ts(ot, ph + 16, dv + kk * 128, idesc, kk > 0 ? 1u : 0u);
                         if constexpr (NV == 2) tc::mma_ts(ot, ph, dv + (kTcTileBytes >> 4) + kk * 128, idesc, 1u);
                     }
-#pragma unroll
+#pragma unroll 1
                     for (int kk = 0; kk < 8; ++kk) tc::mma_ts(ot, sp + 32 * (kk >> 1) + 8 * (kk & 1), dv + kk * 128, idesc, 1u);
                     tc::mma_commit(&B->o_full[n & 1]);
                     tc::mma_commit(&B->v_empty[st]);
@@ -809,6 +881,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         tc::fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
+    if (tid == 0 && B->err) record_status(a.status, kStatusTimeout | (B->err << 8));
 }
 
 // Join of the parts of units that several CTAs shared, and the rows that no unit
