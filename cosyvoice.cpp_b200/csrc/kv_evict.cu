@@ -2,6 +2,7 @@
 // and cvattn_tree_commit (accepted drafts to the end of the cache).
 #include "common.cuh"
 #include "internal.h"
+#include "launch.cuh"
 
 namespace cvattn {
 namespace evict {
@@ -93,6 +94,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_select_kernel(const __grid_
     __shared__ int sh_need, wsum[3][kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int kvh = blockIdx.x, s = blockIdx.y, layer = blockIdx.z;
+    griddep_wait();
     const Seq x = seq_of(a, s);
     int32_t* ws = a.ws + (((int64_t)layer * gridDim.y + s) * gridDim.x + kvh) * (2 * (int64_t)a.moves + 4);
     if (tid == 0) {
@@ -258,6 +260,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
 // kv_len_out that shares memory with a length read above: after every reader is done.
 __global__ void evict_length_kernel(const int32_t* kv_len, const int32_t* kept, int32_t* out, int n, int most, int budget) {
     const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    griddep_wait();
     if (s >= n) return;
     const int L = kv_len[s], kp = kept ? kept[s] : 0;
     out[s] = L >= 0 && L <= most && kp >= 0 && kp <= L ? min(L, budget) : L;
@@ -309,27 +312,17 @@ cudaError_t launch_kv_evict(cudaStream_t stream, const cvattn_kv_evict_params& p
         cudaError_t e = cudaSuccess;
         if (smem > 40 * 1024) e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeySlots * 4);
         if (e != cudaSuccess) return e;
-        evict_select_kernel<<<dim3((unsigned)Hkv, (unsigned)p.n_seq, (unsigned)n), kThreads, smem, stream>>>(a);
-        e = cudaGetLastError();
+        e = launch_overlapped(evict_select_kernel, dim3((unsigned)Hkv, (unsigned)p.n_seq, (unsigned)n), kThreads, smem, stream, a);
         if (e != cudaSuccess) return e;
         if (!a.fused) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3((unsigned)((moves + kMoveChunk - 1) / kMoveChunk), (unsigned)(Hkv * p.n_seq), (unsigned)n);
-            cfg.blockDim = dim3(256);
-            cfg.stream = stream;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            attr[0].val.programmaticStreamSerializationAllowed = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            e = cudaLaunchKernelEx(&cfg, evict_move_kernel, a, p.n_seq);
+            const dim3 grid((unsigned)((moves + kMoveChunk - 1) / kMoveChunk), (unsigned)(Hkv * p.n_seq), (unsigned)n);
+            e = launch_overlapped(evict_move_kernel, grid, 256, 0, stream, a, p.n_seq);
             if (e != cudaSuccess) return e;
         }
     }
     if (shared_len) {
-        evict_length_kernel<<<(p.n_seq + 255) / 256, 256, 0, stream>>>(p.kv_len, p.kept_len, p.kv_len_out, p.n_seq, p.max_kv_len,
-                                                                    p.budget);
-        return cudaGetLastError();
+        return launch_overlapped(evict_length_kernel, dim3((unsigned)((p.n_seq + 255) / 256)), 256, 0, stream, p.kv_len, p.kept_len,
+                                 p.kv_len_out, p.n_seq, p.max_kv_len, p.budget);
     }
     return cudaSuccess;
 }
@@ -381,6 +374,7 @@ __device__ __forceinline__ bool fits(const Args& a, int s, int L, int n) {
 __global__ void __launch_bounds__(128) commit_kernel(const __grid_constant__ Args a) {
     const int s = blockIdx.x;
     const Tensor& t = a.t[blockIdx.y];
+    griddep_wait();
     const int L = a.kv_len[s], n = a.n_accepted[s];
     const bool ok = fits(a, s, L, n);
     if (threadIdx.x == 0 && blockIdx.y == 0) {
@@ -401,6 +395,7 @@ __global__ void __launch_bounds__(128) commit_kernel(const __grid_constant__ Arg
 
 __global__ void commit_length_kernel(const __grid_constant__ Args a, int32_t* out) {
     const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    griddep_wait();
     if (s >= a.n_seq) return;
     const int L = a.kv_len[s], n = a.n_accepted[s];
     out[s] = fits(a, s, L, n) ? L + n : L;
@@ -436,13 +431,11 @@ cudaError_t launch_tree_commit(cudaStream_t stream, const cvattn_tree_commit_par
                                  (uint64_t)t.dst_nb2 | (uint64_t)t.src_nb1 | (uint64_t)t.src_nb2 | (uint64_t)t.row;
             t.unit = (all & 15) == 0 ? 16 : (all & 7) == 0 ? 8 : (all & 3) == 0 ? 4 : 2;
         }
-        commit_kernel<<<dim3((unsigned)p.n_seq, (unsigned)n), 128, 0, stream>>>(a);
-        cudaError_t e = cudaGetLastError();
+        const cudaError_t e = launch_overlapped(commit_kernel, dim3((unsigned)p.n_seq, (unsigned)n), 128, 0, stream, a);
         if (e != cudaSuccess) return e;
     }
     if (shared_len) {
-        commit_length_kernel<<<(p.n_seq + 127) / 128, 128, 0, stream>>>(a, p.kv_len_out);
-        return cudaGetLastError();
+        return launch_overlapped(commit_length_kernel, dim3((unsigned)((p.n_seq + 127) / 128)), 128, 0, stream, a, p.kv_len_out);
     }
     return cudaSuccess;
 }

@@ -16,6 +16,7 @@ __global__ void __launch_bounds__(128) scores_f32_kernel(const __grid_constant__
     const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
     const int s = blockIdx.z, kvh = blockIdx.y, p0 = blockIdx.x * kTile;
     int L, n;
+    griddep_wait();
     if (!lens_of(a, s, L, n, tid == 0) || p0 >= L) return;
     const int count = min(kTile, L - p0);
     const uint8_t* kb = a.k_seq_ptrs ? reinterpret_cast<const uint8_t*>(a.k_seq_ptrs[s]) : a.k + (int64_t)s * a.k_nb2;
@@ -152,8 +153,7 @@ cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params&
     default: break;
     }
     const dim3 grid((unsigned)((a.max_kv_len + kTile - 1) / kTile), (unsigned)a.Hkv, (unsigned)a.n_seq);
-    scores_f32_kernel<<<grid, 128, 0, stream>>>(a);
-    return cudaGetLastError();
+    return launch_overlapped(scores_f32_kernel, grid, 128, 0, stream, a);
 }
 
 }  // namespace cvattn

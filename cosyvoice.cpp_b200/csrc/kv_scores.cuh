@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, NT == 2 ? 3 : 2) scores_mma_kernel(c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int s = blockIdx.z, kvh = blockIdx.y, p0 = blockIdx.x * kKeys;
     int L, n;
+    griddep_wait();
     if (!lens_of(a, s, L, n, tid == 0) || p0 >= L) return;
     const int count = min(kKeys, L - p0), total = n * a.G;
     {   // the keys' rows: f16 straight into the tile, quants raw

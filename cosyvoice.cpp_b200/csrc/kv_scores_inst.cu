@@ -19,8 +19,7 @@ static cudaError_t run(cudaStream_t stream, const Args& a) {
         if (e != cudaSuccess) return e;
         if (dev < 64) allowed[dev].store(true, std::memory_order_relaxed);
     }
-    fn<<<dim3((unsigned)((a.max_kv_len + keys - 1) / keys), (unsigned)a.Hkv, (unsigned)a.n_seq), kThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_overlapped(fn, dim3((unsigned)((a.max_kv_len + keys - 1) / keys), (unsigned)a.Hkv, (unsigned)a.n_seq), kThreads, smem, stream, a);
 }
 
 template <>

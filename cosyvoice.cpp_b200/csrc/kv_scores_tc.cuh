@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         tc::tmem_alloc(&B->tmem_base, 512);
         tc::tmem_relinquish();
     }
+    griddep_wait();
     if (warp == 1) {  // list entries before each sequence
         int carry = 0;
         for (int base = 0; base < a.n_seq; base += 32) {

@@ -38,6 +38,7 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const __grid_constant__ A
     float(*ps)[kPad] = vs + kTile;
     const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
     const int s = blockIdx.z, kvh = blockIdx.y % a.Hkv, r0 = (blockIdx.y / a.Hkv) * kRows, split = blockIdx.x;
+    griddep_wait();
     const Lens x = lens_of(a, s, tid == 0 && blockIdx.x == 0 && blockIdx.y == 0);
     const int rows = x.n * a.G, all_rows = a.max_nodes * a.G;
     const int tile0 = split * a.split_tiles, tile1 = min(x.tiles, tile0 + a.split_tiles);
@@ -281,31 +282,15 @@ static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_n
 template <int kLanes>
 static cudaError_t run_combine(cudaStream_t stream, const Args& a) {
     const int rows = a.max_nodes * a.G;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)a.Hkv, (unsigned)a.n_seq);
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tree_combine_kernel<kLanes>, a);
+    const dim3 grid((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)a.Hkv, (unsigned)a.n_seq);
+    return launch_overlapped(tree_combine_kernel<kLanes>, grid, 256, 0, stream, a);
 }
 
 template <int kLanes>
 static cudaError_t run_tc_combine(cudaStream_t stream, const TcArgs& ta) {
     const int rows = ta.a.max_nodes * ta.a.G;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)ta.a.Hkv, (unsigned)ta.a.n_seq);
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tree_tc_combine_kernel<kLanes>, ta);
+    const dim3 grid((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)ta.a.Hkv, (unsigned)ta.a.n_seq);
+    return launch_overlapped(tree_tc_combine_kernel<kLanes>, grid, 256, 0, stream, ta);
 }
 
 static cudaError_t launch_tc(cudaStream_t stream, const Args& a, const Plan& plan, void* workspace) {
@@ -416,8 +401,7 @@ cudaError_t launch_tree_decode(cudaStream_t stream, const cvattn_tree_params& p,
         e = cudaFuncSetAttribute(tree_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         const dim3 grid((unsigned)plan.n_splits, (unsigned)(a.Hkv * ((rows + kRows - 1) / kRows)), (unsigned)a.n_seq);
-        tree_f32_kernel<<<grid, 128, smem, stream>>>(a);
-        e = cudaGetLastError();
+        e = launch_overlapped(tree_f32_kernel, grid, 128, smem, stream, a);
     }
     if (e != cudaSuccess || plan.n_splits == 1) return e;
     return launch_combine(stream, a);

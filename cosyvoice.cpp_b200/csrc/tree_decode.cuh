@@ -11,6 +11,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "launch.cuh"
 #include "internal.h"
 
 namespace cvattn {

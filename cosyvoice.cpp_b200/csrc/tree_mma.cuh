@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_mma_kernel(const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int s = blockIdx.z, split = blockIdx.x;
     const int kvh = blockIdx.y % a.Hkv, r0 = blockIdx.y / a.Hkv * (16 * kWarps);
+    griddep_wait();
     const Lens x = lens_of(a, s, tid == 0 && blockIdx.x == 0 && blockIdx.y == 0);
     const int rows = x.n * a.G, all_rows = a.max_nodes * a.G;
     const int tile0 = split * a.split_tiles, tile1 = min(x.tiles, tile0 + a.split_tiles);

@@ -20,8 +20,7 @@ static cudaError_t run(cudaStream_t stream, const Args& a, const Shape& sh) {
         if (dev < 64) allowed[dev].store(smem, std::memory_order_relaxed);
     }
     const dim3 grid((unsigned)a.n_splits, (unsigned)(a.Hkv * sh.row_groups), (unsigned)a.n_seq);
-    fn<<<grid, kWarps * 32, smem, stream>>>(a, sh);
-    return cudaGetLastError();
+    return launch_overlapped(fn, grid, kWarps * 32, smem, stream, a, sh);
 }
 
 template <>

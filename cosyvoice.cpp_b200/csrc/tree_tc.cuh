@@ -523,6 +523,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         tc::tmem_relinquish();
     }
     if (warp == 1) {  // list entries before each sequence
+        griddep_wait();  // (every other thread touches global memory after the __syncthreads below)
         int carry = 0;
         for (int base = 0; base < a.n_seq; base += 32) {
             const int s = base + lane;

@@ -19,8 +19,7 @@ static cudaError_t run(cudaStream_t stream, const TcArgs& a) {
         if (e != cudaSuccess) return e;
         if (dev < 64) allowed[dev].store(true, std::memory_order_relaxed);
     }
-    fn<<<a.grid, kTcThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_overlapped(fn, dim3((unsigned)a.grid), kTcThreads, smem, stream, a);
 }
 
 template <>
