@@ -39,6 +39,9 @@ constexpr int kTcMaxSeq = 1024;
 constexpr int kTcMaxRows = 512;      // (token, head) rows of a KV head whose Q fits shared memory
 constexpr int kTcRowTiles = kTcMaxRows / 128;
 constexpr int kTcRawBuffers = 8;
+// Tiles whose scales are kept: tile n is written once S of tile n - 2 is done, which a group may still have to read together
+// with that of n - 4; S of n - 2 took the buffer of n - 6, whose scales have been read.
+constexpr int kTcScales = 6;
 
 struct TcArgs {
     Args a;
@@ -50,7 +53,7 @@ struct TcArgs {
 struct TcBars {
     uint64_t k_full[4], k_empty[4];  // by stage
     uint64_t raw_full[kTcRawBuffers], raw_empty[kTcRawBuffers];
-    uint64_t q_full;
+    uint64_t q_full, q_seen;         // by run: written; both issuers know (so they miss none)
     uint64_t s_full[2][2], s_empty[2][2];  // by group and S buffer
     uint32_t tmem_base;
     int err;
@@ -68,8 +71,8 @@ struct TcShape {
     static constexpr int kRawOne = K_Q ? 2 * kTcTile * raw_stride(KT) : 0;
     static constexpr int kInfo = kRaw + 2 * kRawOne;                      // float2 per row: factor, -log-sum; then the block sums of Q
     static constexpr int kFar = kInfo + kTcMaxRows * 16;
-    static constexpr int kScale = kFar + kTcMaxRows * 4;                  // [tile n & 3][scales, mins][block][key]
-    static constexpr int kBars = kScale + (K_Q ? 4 * 4 * kTcTile * 4 : 0);
+    static constexpr int kScale = kFar + kTcMaxRows * 4;                  // [tile n % 6][scales, mins][block][key]
+    static constexpr int kBars = kScale + (K_Q ? kTcScales * 4 * kTcTile * 4 : 0);
     static constexpr int kPref = kBars + (int)((sizeof(TcBars) + 15) / 16 * 16);
     static constexpr int kBytes = kPref + (kTcMaxSeq + 4) * 4;
     static_assert(kBytes <= 227 * 1024, "one CTA per SM");
@@ -158,6 +161,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
             }
         }
         mbar_init(&B->q_full, 256);
+        mbar_init(&B->q_seen, 2);
         B->err = 0;
         B->any_out = 0;
         fence_mbar_init();
@@ -202,10 +206,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         const int g = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
         const uint32_t st = tmem + ((uint32_t)(quad * 32) << 16) + g * 256;
         constexpr int kCols = 16;  // columns at a time
-        uint32_t k = 0;  // S tiles of this group so far
+        uint32_t k = 0, n_run = 0;  // S tiles of this group, runs so far
         bool ok = true;
-        for (; r.i < hi; r.next(a, pref, hi)) {
-            const int R = r.n * a.G;
+        for (; r.i < hi; r.next(a, pref, hi), ++n_run) {
+            const int rows = r.n * a.G, R = max(rows, 1);  // (without rows: one that is left out, so that every tile has its S)
+            if (n_run) ok = ok && tc_wait(&B->q_seen, (n_run - 1) & 1, &B->err, 59);
             // every S of the last run has been read: its Q may go
             if (!fp::prod_bar_and(1, 256, ok)) { ok = false; break; }
             if (tid == 0) B->any_out = 0;
@@ -218,10 +223,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                 float4 v[4];
                 float ls = -INFINITY;
                 int at = t;
-                if (q0 < R && a.rows) at = a.rows[(int64_t)r.s * a.max_rows + t];
-                const bool there = q0 < R && at >= 0 && at < a.n_q_rows;
+                if (q0 < rows && a.rows) at = a.rows[(int64_t)r.s * a.max_rows + t];
+                const bool there = q0 < rows && at >= 0 && at < a.n_q_rows;
                 if (there) ls = a.lse[((int64_t)r.s * a.n_q_rows + at) * a.Hq + h];
-                else if (q0 < R) record_status(a.status, kStatusBadPosition);
+                else if (q0 < rows) record_status(a.status, kStatusBadPosition);
                 const float4* q = reinterpret_cast<const float4*>(a.q + (int64_t)r.s * a.q_nb_seq + (int64_t)at * a.q_nb_node + h * kD + 16 * c);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) v[u] = there ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     tc::fence_after();
                     if (K_Q && r0 == 0) {
-                        const float* sp = scale + (n & 3) * 4 * kTcTile + key;
+                        const float* sp = scale + n % kTcScales * 4 * kTcTile + key;
                         d0 = sp[0];
                         d1 = sp[kTcTile];
                         if constexpr (K_MIN) {
@@ -373,7 +378,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
                     convert_block<KT, 1>(row, w1, d1, m1);
                     store_block(tile, key, 0, w0);
                     store_block(tile, key, 1, w1);
-                    float* sp = scale + (n & 3) * 4 * kTcTile + key;
+                    float* sp = scale + n % kTcScales * 4 * kTcTile + key;
                     const bool there = key < count;
                     sp[0] = there ? d0 : 0.0f;
                     sp[kTcTile] = there ? d1 : 0.0f;
@@ -469,8 +474,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) scores_tc_kernel(const __grid_c
         uint32_t k = 0, n_run = 0;
         bool ok = true;
         for (; ok && r.i < hi; r.next(a, pref, hi), ++n_run) {
-            const int R = r.n * a.G;
+            const int R = max(r.n * a.G, 1);
             ok = tc_wait(&B->q_full, n_run & 1, &B->err, 55);
+            ok = __all_sync(0xffffffffu, ok);
+            if (lane == 0) mbar_arrive(&B->q_seen);
             for (int j = r.i + ((r.i ^ lo ^ g) & 1); ok && j < r.end; j += 2) {
                 const int n = j - lo, sg = n % kSt;
                 ok = tc_wait(&B->k_full[sg], (n / kSt) & 1, &B->err, 56);
