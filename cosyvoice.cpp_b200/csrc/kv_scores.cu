@@ -132,7 +132,8 @@ cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params&
         ta.grid = 148;
         const int spare = (kTcRowTiles - (a.max_rows * a.G + 127) / 128) * 2 * kTcTileBytes;  // of the Q tiles
         const int raw = 2 * kTcTile * raw_stride(a.k_type);
-        ta.raw_buffers = 2 + spare / raw < kTcRawBuffers ? 2 + spare / raw : kTcRawBuffers;
+        // (an even number: each producer group sees every phase of its own buffers)
+        ta.raw_buffers = (2 + spare / raw < kTcRawBuffers ? 2 + spare / raw : kTcRawBuffers) & ~1;
         switch (a.k_type) {
         case kF16: return launch_tc_for_k<kF16>(stream, ta);
         case kQ4_0: return launch_tc_for_k<kQ4_0>(stream, ta);
