@@ -64,7 +64,7 @@ struct TcBars {
     int err;
     uint32_t maxk[3], maxv[3];        // largest |scale| of tile n at n % 3
     float expk[kTcExps], expv[kTcExps];  // 2^-e of K and V of tile n at n % kTcExps
-    uint32_t flags[kTcExps];          // 1: the tile starts a run, 2: drafted keys
+    uint32_t starts[kTcExps];         // whether the tile starts a run
     uint32_t bad[kTcExps][4];         // draft keys whose V is not finite
     int32_t first_run[12];            // Run at the start of the CTA's part
 };
@@ -380,7 +380,7 @@ __device__ __forceinline__ void produce(const TcArgs& ta, uint8_t* smem, TcBars*
             if (key == 0) {
                 slots[slot == 2 ? 0 : slot + 1] = 0u;  // of the tile after the next: read by all before this barrier
                 (kV ? B->expv : B->expk)[n % kTcExps] = pow2f(-e);
-                if (!kV) B->flags[n % kTcExps] = (uint32_t)first | (draft ? 2u : 0u);
+                if (!kV) B->starts[n % kTcExps] = (uint32_t)first;
             }
             first = 0;
             if (kV && draft) {  // which keys hold values that are not finite (their tile rows are zeros)
@@ -465,7 +465,7 @@ __device__ __forceinline__ void produce(const TcArgs& ta, uint8_t* smem, TcBars*
                 }
                 if (key == 0) {
                     (kV ? B->expv : B->expk)[n % kTcExps] = 1.0f;
-                    if (!kV) B->flags[n % kTcExps] = (uint32_t)first | (draft ? 2u : 0u);
+                    if (!kV) B->starts[n % kTcExps] = (uint32_t)first;
                 }
                 first = 0;
                 if (ok) {
@@ -624,11 +624,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             bool pending = false;  // a tile's output still to be added, times vs_last and its V's 2^-e
             int n_last = 0;        // that tile
             bool spoiled = false;  // the row sees a drafted value that is not finite
+            // drafts p0 + 32 c .. + 31 of a tile of `count` that the row sees
+            auto seen_drafts = [&](int p0, int count, int c) -> uint32_t {
+                const int left = count - 32 * c, j0 = p0 + 32 * c;
+                const uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                if (bits == 0) return 0u;
+                if (a.mask) return bits & a.mask[(int64_t)r.s * a.mask_nb_seq + (int64_t)node * a.mask_words + (j0 >> 5)];
+                return node >= j0 + 31 ? bits : node < j0 ? 0u : bits & ((2u << (node - j0)) - 1u);
+            };
             auto add_output = [&]() {
                 uint32_t o0[32], o1[32];
                 tc::tmem_ld32(ot, o0);
                 tc::tmem_ld32(ot + 32, o1);
                 tc::tmem_ld_wait();
+                {   // keys whose V is not finite have zeros in the tile; a row that sees one is NaN in the end
+                    bool draft;
+                    int p0, count;
+                    r.tile(lo + n_last, draft, p0, count);
+#pragma unroll 1
+                    for (int c = 0; draft && c < 4; ++c) {
+                        const uint32_t bad = B->bad[n_last % kTcExps][c];
+                        if (bad && real) spoiled |= (bad & seen_drafts(p0, count, c)) != 0;
+                    }
+                }
                 const float vs = vs_last * B->expv[n_last % kTcExps];
                 const float2 f = make_float2(vs, vs);
 #pragma unroll
@@ -656,12 +674,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                     for (int c = 0; c < 4; ++c) {
                         if (masked) {
                             const int left = count - 32 * c;
-                            uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-                            if (draft && bits && real) {
-                                const int j0 = p0 + 32 * c;
-                                if (a.mask) bits &= a.mask[(int64_t)r.s * a.mask_nb_seq + (int64_t)node * a.mask_words + (j0 >> 5)];
-                                else if (node < j0 + 31) bits &= node < j0 ? 0u : (2u << (node - j0)) - 1u;
-                            }
+                            const uint32_t bits = draft && real ? seen_drafts(p0, count, c)
+                                                  : left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
                             for (int d = 0; d < 32; ++d)
                                 if (!((bits >> d) & 1u)) sv[d] = 0xff800000u;
@@ -729,15 +743,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                         }
                         l0 = add2(l0, l1);
                         l += l0.x + l0.y;
-                        if (draft) {
-                            // keys whose V is not finite have zeros in the tile; a row that sees one is NaN in the end
-                            const uint32_t bad = B->bad[(j - lo) % kTcExps][c];
-                            if (bad) {
-#pragma unroll
-                                for (int d = 0; d < 16; ++d)
-                                    spoiled |= ((bad >> (2 * d) & 1u) && x[d].x != 0.0f) || ((bad >> (2 * d + 1) & 1u) && x[d].y != 0.0f);
-                            }
-                        }
                         uint32_t pv[32];
 #pragma unroll
                         for (int d = 0; d < 16; ++d) {
@@ -820,9 +825,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             uint32_t use = 0, turn = 0, n_run = 0;  // n / kSt, n / 3
             for (int n = 0; ok && lo + n < hi; ++n) {
                 ok = tc_wait(&B->k_full[st], use & 1, &B->err, 38);
-                const uint32_t flags = B->flags[n % kTcExps];
-                if (ok && (flags & 1)) ok = tc_wait(&B->q_full, n_run++ & 1, &B->err, 37);
-                if (ok && (flags & 2)) ok = tc_wait(&B->v_full[st], use & 1, &B->err, 44);  // (which values are bad)
+                if (ok && B->starts[n % kTcExps]) ok = tc_wait(&B->q_full, n_run++ & 1, &B->err, 37);
                 if (ok && n >= 3) ok = tc_wait(&B->s_free[buf], (turn - 1) & 1, &B->err, 40);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;

@@ -35,6 +35,14 @@ def test_tree_list_of_tiles_is_shared(ctx, cv, cuda, oracle, kname, shift):
     run_case(ctx, cv, cuda, oracle, kname, vname, 14, 2, lens, 9, counts=counts, sees=ancestors(random_parents(rng, 24, 9)), seed=shift)
 
 
+@pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("f16", "q8_0"), ("q5_1", "f16")])
+def test_tree_drafts_after_long_contexts(ctx, cv, cuda, oracle, kname, vname):
+    """K tiles run ahead of V tiles; whether a draft's values are finite must not be asked before its V tile is there."""
+    lens = np.random.default_rng(5).integers(128, 2049, 64).tolist()
+    for _ in range(2):
+        run_case(ctx, cv, cuda, oracle, kname, vname, 14, 2, lens, 8)
+
+
 @pytest.mark.parametrize("kname,vname", [("q8_0", "q8_0"), ("f16", "f16"), ("q4_1", "f16"), ("f16", "q5_1")])
 @pytest.mark.parametrize("pads,offsets", [((2, 6, 10, 14), (2, 2, 2, 2)), ((4, 8, 12, 4), (4, 12, 8, 4))])
 def test_tree_shared_list_strides_and_addresses(ctx, cv, cuda, oracle, kname, vname, pads, offsets):
