@@ -10,7 +10,10 @@ namespace tree {
 // A CTA of 128 threads takes 32 rows of one KV head and one split.  K and V tiles
 // are dequantized to f32 in shared memory; a thread owns 4 rows x 4 keys of S and
 // then 4 rows x 4 dims of the output.  Rows are padded to 68 floats, so the eight
-// float4s of a phase (keys apart by one row) touch different banks.
+// float4s of a phase (keys apart by one row) touch different banks.  Bound by its FMAs and
+// shared-memory reads: f32 rows have no exact f16 pieces, and the caches that matter are not
+// f32.  (This kernel with Q8_0 rows: 64 sequences of 128 to 2048, 8 nodes 315 us, where the
+// tcgen05 kernel takes 39.7.)
 constexpr int kTile = 64;  // keys per tile
 constexpr int kRows = 32;
 constexpr int kPad = kD + 4;
@@ -153,6 +156,7 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const __grid_constant__ A
 // out = sum_k 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k over the splits that the
 // sequence has.  16 threads (4 dims each) follow every kLanes-th split of a row;
 // the kLanes partial sums of a row are joined through shared memory in order.
+// Latency-bound: about 2 us, started early so that its launch is hidden.
 template <int kLanes>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Args a) {
     constexpr int kPer = 16 / kLanes;  // rows per CTA

@@ -18,6 +18,10 @@
 // P.V without leaving the registers.  Adds inside the tensor cores truncate, so
 // their chains are kept short: every 8 steps the output moves to f32 sums in
 // shared memory.  Warps that share rows merge at the end.
+// What bounds it: one sequence of 300 positions, 4 nodes, Q8_0: 10 us with the join, latency
+// (two launches, a tile's way through copy, conversion, products and merge).  3 sequences of
+// up to 777, 27 nodes, 16 / 16 heads, Q5_1 / Q4_1: 17.7 us for 3.5 MB, the instructions of
+// conversion and softmax (1.4 a cycle and SM; DRAM and tensor cores idle).
 #pragma once
 
 #include "decode_mma.cuh"

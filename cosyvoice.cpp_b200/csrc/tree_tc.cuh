@@ -26,6 +26,13 @@
 // a time by that chunk's P (16 columns hi, 16 lo): a group never waits for the
 // S of its next tile.  Two outputs of 64 columns, one per group, read back while
 // the group's next tile is on its way.
+// What bounds it: the softmax's instructions.  A tile of 128 rows x 128 keys costs the two
+// groups together some 2100 cycles (exponentials alone 1024, products 770).  16 sequences of
+// 4096 positions, 64 nodes, 14 / 2 heads, f16: 62 us, 246 TFLOP/s (twice that in the tensor
+// cores, for hi and lo).  Few tiles per CTA are bound by the start (10K cycles: launch, lists,
+// first rows, a cold instruction cache) and, for quants, by the producers (a tile's copies and
+// conversion 2700 cycles): 64 sequences of 128 to 2048, 8 nodes, Q8_0 / Q4_0: 39.7 us; one of
+// 65536, 16 nodes, Q8_0: 32.1 us, 558 GB/s.  Both times with the join's launch.
 #pragma once
 
 #include "flash_pipe.cuh"
@@ -890,7 +897,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 
 // Join of the parts of units that several CTAs shared, and the rows that no unit
 // holds (a sequence without keys, rows past the last node).  16 threads per row
-// (4 dims each) follow every kLanes-th part.
+// (4 dims each) follow every kLanes-th part.  Bound by its latency, most of which its
+// early launch hides: 2 to 3 us of the calls above.
 template <int kLanes>
 __global__ void __launch_bounds__(256) tree_tc_combine_kernel(const __grid_constant__ TcArgs ta) {
     constexpr int kPer = 16 / kLanes;

@@ -368,6 +368,10 @@ cvattn_status cvattn_flash(cvattn_context* ctx, void* stream, const cvattn_flash
  * in the cache and an accepted one attends exactly as it will once committed.
  * Products are exact in f32 for every cache type, as in cvattn_decode.
  *   - A row that sees nothing gives zeros and lse = -inf.
+ *   - Drafted rows that a row does not see may hold anything, NaN and infinities
+ *     included; one that it sees and that is not finite makes its output not
+ *     finite (every element, from a value row on some paths; its lse only from a
+ *     key row).  Committed rows are seen by all.
  *   - Rows from n_nodes[s] up to max_nodes are written as such rows too.
  *   - A kv_len[s] outside [0, max_kv_len] or n_nodes[s] outside [0, max_nodes]
  *     is recorded in the status word and the sequence gives such rows only.
