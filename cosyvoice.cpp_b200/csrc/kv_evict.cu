@@ -10,7 +10,9 @@ namespace evict {
 constexpr int kThreads = 512;  // (1024 threads of 58 registers leave one CTA per SM: 31 us instead of 22 for 192 heads of 8192 slots)
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxKeySlots = 40 * 1024;  // 160 KB of keys
-constexpr int kFusedMoves = 256;         // up to so many rows a head the selecting CTA moves them itself: one launch
+// Up to so many rows a head the selecting CTA moves them itself: one launch.  us of one | two launches, 4096 slots, Q8_0, 24 layers:
+// one sequence, 64 moves 12.6 | 17.5, 256 15.6 | 17.7, 512 20.0 | 18.5; 8 sequences, 256 33.6 | 37.8, 512 50.2 | 49.6.
+constexpr int kFusedMoves = 256;
 constexpr int kLayersPerLaunch = 32;  // layer addresses that travel as kernel parameters
 
 struct Args {

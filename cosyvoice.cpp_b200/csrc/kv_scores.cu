@@ -124,10 +124,16 @@ cudaError_t launch_kv_scores(cudaStream_t stream, const cvattn_kv_scores_params&
     a.scale_log2 = p.scale * 1.4426950408889634f;
     a.decay = p.decay;
     a.status = status;
-    // From two key tiles per SM on the persistent tcgen05 kernel; below, more and smaller CTAs answer sooner.
+    // From four 128-key tiles per SM on the persistent tcgen05 kernel, which starts later and goes through tiles faster (f16, whose
+    // tiles cost the other kernel no conversion, also needs rows enough).  us of scores_mma_kernel | tcgen05, 14 / 2 heads, Q8_0
+    // and f16: 16 sequences of 1000 (256 tiles), 28 rows 5.7 | 7.5 and 4.6 | 7.2; 16 of 2000 (512), 28 rows 7.7 | 8.7 and 5.7 |
+    // 8.5, 112 rows 12.6 | 14.9 and 10.3 | 13.0, 448 rows 36 | 36 and 33 | 32; 64 of 1000 (1024), 7 rows 11.4 | 10.5 and 7.7 |
+    // 10.4, 56 rows 17.1 | 13.7 and 13.6 | 12.4, 448 rows 69 | 47 and 63 | 41; 16 of 8192 (2048), 7 rows 20.0 | 14.6 and 13.7 |
+    // 14.9, 28 rows 24.1 | 16.2 and 17.9 | 15.5.
     const int64_t entries = (int64_t)a.n_seq * a.Hkv * ((a.max_kv_len + kTcTile - 1) / kTcTile);
-    if (a.k_type != kF32 && entries >= 2 * 148 && entries < (int64_t)1 << 31 && a.n_seq <= kTcMaxSeq &&
-        (int64_t)a.max_rows * a.G <= kTcMaxRows) {
+    const int64_t rows = (int64_t)a.max_rows * a.G;
+    if (a.k_type != kF32 && entries >= 4 * 148 && entries < (int64_t)1 << 31 && (a.k_type != kF16 || entries * rows >= 1 << 15) &&
+        a.n_seq <= kTcMaxSeq && rows <= kTcMaxRows) {
         TcArgs ta{};
         ta.a = a;
         ta.inv_g = (uint32_t)((65536 + a.G - 1) / a.G);

@@ -24,9 +24,10 @@ static cudaError_t run(cudaStream_t stream, const Args& a) {
 
 template <>
 cudaError_t launch_mma_for_k<CVATTN_KT>(cudaStream_t stream, const Args& a) {
-    // Many rows share more of each Q fragment with 32 keys a warp; few rows (and few keys) fill more SMs with 16.
-    const int64_t ctas = (int64_t)a.n_seq * a.Hkv * ((a.max_kv_len + 255) / 256);
-    return a.max_rows * a.G > 64 && ctas >= 296 ? run<CVATTN_KT, 4>(stream, a) : run<CVATTN_KT, 2>(stream, a);
+    // 32 keys a warp share more of each Q fragment, 16 keys fill more SMs.  us of 16 | 32 keys a warp, 14 / 2 heads, Q8_0 and f16: 64
+    // tiles of 128 keys, 28 rows 4.9 | 5.7 and 4.3 | 4.6; 256 tiles, 28 rows 6.4 | 5.7 and 5.0 | 4.6, 112 rows 9.8 | 8.7 and 7.9 | 7.4;
+    // 512 tiles, 28 rows 11.6 | 7.7 and 8.6 | 5.7.
+    return (int64_t)a.n_seq * a.Hkv * ((a.max_kv_len + 127) / 128) > 148 ? run<CVATTN_KT, 4>(stream, a) : run<CVATTN_KT, 2>(stream, a);
 }
 
 }  // namespace kvscore

@@ -1,5 +1,5 @@
 // kv_scores_tc.cuh -- attention scores on the 5th-generation tensor cores (tcgen05),
-// for f16 and block-quantized caches, many keys and up to 512 rows.
+// for f16 and block-quantized caches, many key tiles and up to 512 rows.
 //
 // The product is taken transposed, S^T = K Q^T: a TMEM lane, and so a thread, is a
 // key, and the sum over the rows is a sum along the thread's columns, with no
@@ -19,7 +19,7 @@
 //   warps 16, 17    MMA issuers of the groups
 //   warp 18         loader: raw rows of the next tiles, one bulk copy each where they hold
 //                   at most two heads and lie packed (else the producers copy the slices)
-// What bounds it: 8 sequences of 8192 positions, 64 rows of 14 heads, f16: 40 us, 188 TFLOP/s;
+// What bounds it: 8 sequences of 8192 positions, 64 rows of 14 heads, f16: 40.6 us, 185 TFLOP/s;
 // a group sums 128 x 128 in 2800 cycles, of which the exponentials are 2048 (a quarter of the
 // SM's unit per warp).  64 sequences of up to 4096, 4 rows, Q8_0: 20 us for 20 MB; start and
 // change of runs (10K and 2K cycles) are half of it, the rest the tiles' conversion.

@@ -13,7 +13,7 @@ namespace tree {
 // float4s of a phase (keys apart by one row) touch different banks.  Bound by its FMAs and
 // shared-memory reads: f32 rows have no exact f16 pieces, and the caches that matter are not
 // f32.  (This kernel with Q8_0 rows: 64 sequences of 128 to 2048, 8 nodes 315 us, where the
-// tcgen05 kernel takes 39.7.)
+// tcgen05 kernel takes 39.3.)
 constexpr int kTile = 64;  // keys per tile
 constexpr int kRows = 32;
 constexpr int kPad = kD + 4;
@@ -245,16 +245,22 @@ struct Plan {
 
 constexpr int kSms = 148;
 constexpr int kSlots = 2 * kSms;  // two CTAs of tree_mma_kernel per SM
-constexpr int kTcMinRows = 32;    // up to here tree_mma_kernel, whose row tiles are 16 rows
+// The tcgen05 kernel starts later (10 us before the first output) and goes through tiles faster, whatever rows they have up to
+// 128.  It takes over at this many 128-key tiles x rows of a KV head, and above 128 rows.  us of tree_mma_kernel | tcgen05, 14 / 2
+// heads, Q8_0 and f16: one sequence of 4096 (66 tiles), 112 rows 15.4 | 15.6 and 13.4 | 15.2, 252 rows 20.0 | 17.3 and 18.4 |
+// 16.3; 16 of 1000 (288), 56 rows 17.6 | 23.5 and 14.5 | 22.0, 112 rows 24.6 | 25.2 and 21.2 | 23.8; one of 65536 (1026), 28
+// rows 31.8 | 29.9 and 22.4 | 24.3, 56 rows 41.6 | 30.5 and 30.8 | 25.0; 64 of 4096 (4224), 7 rows 86 | 74 and 51 | 55, 28 rows
+// 108 | 75 and 69 | 55.
+constexpr int64_t kTcMinWork = 1 << 15;
 
 static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {
     Plan p{};
     const int64_t rows = (int64_t)max_nodes * (n_q_heads / n_kv_heads);
     p.mma = mma_type(k_type) && mma_type(v_type);
     int64_t units;
-    const int64_t entries = (int64_t)n_seq * n_kv_heads * ((rows + kTcRows - 1) / kTcRows) *
-                            ((max_kv_len + kTcTile - 1) / kTcTile + (max_nodes + kTcTile - 1) / kTcTile);
-    if (p.mma && rows > kTcMinRows && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
+    const int64_t key_tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile + (max_nodes + kTcTile - 1) / kTcTile);
+    const int64_t entries = key_tiles * ((rows + kTcRows - 1) / kTcRows);
+    if (p.mma && (rows > kTcRows || key_tiles * rows >= kTcMinWork) && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
         p.tile = kTcTile;
         p.tc_grid = (int)(entries < kSms ? entries : kSms);
         p.n_splits = p.tc_grid / (int64_t)(n_seq * n_kv_heads) > 0 ? p.tc_grid / (n_seq * n_kv_heads) : 1;  // (for the combine)
@@ -266,7 +272,9 @@ static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_n
         p.sh.stages = kMaxStages;
         while (p.sh.stages > 2 && Smem(k_type, v_type, p.sh.stages).total > kHalfSm) --p.sh.stages;
         units = (int64_t)n_seq * n_kv_heads * p.sh.row_groups;
-        if (units * ((max_kv_len + kKeys - 1) / kKeys) < kSlots / 2) p.tile = kKeys / 2;  // few tiles: smaller ones, on more SMs
+        // Few tiles: smaller ones, on more SMs.  us of 64 | 128 keys, Q8_0: one sequence of 300, 28 rows 9.9 | 10.5; 16 sequences of
+        // 1000 (256 tiles), 28 rows 18.6 | 14.7.
+        if (units * ((max_kv_len + kKeys - 1) / kKeys) < kSlots / 2) p.tile = kKeys / 2;
     } else {
         p.tile = kTile;
         units = (int64_t)n_seq * n_kv_heads * ((rows + kRows - 1) / kRows);

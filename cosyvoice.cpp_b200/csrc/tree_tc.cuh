@@ -1,5 +1,5 @@
 // tree_tc.cuh -- tree attention on the 5th-generation tensor cores (tcgen05), for
-// f16 and block-quantized caches and more than 32 rows per KV head.
+// f16 and block-quantized caches and much work (kTcMinWork, tree_decode.cu).
 //
 // Work is cut evenly: the key tiles (128 keys) of all units (sequence, KV head,
 // tile of 128 rows) form one list, and CTA c of G takes the entries [c N / G,
@@ -28,11 +28,11 @@
 // the group's next tile is on its way.
 // What bounds it: the softmax's instructions.  A tile of 128 rows x 128 keys costs the two
 // groups together some 2100 cycles (exponentials alone 1024, products 770).  16 sequences of
-// 4096 positions, 64 nodes, 14 / 2 heads, f16: 62 us, 246 TFLOP/s (twice that in the tensor
+// 4096 positions, 64 nodes, 14 / 2 heads, f16: 61 us, 249 TFLOP/s (twice that in the tensor
 // cores, for hi and lo).  Few tiles per CTA are bound by the start (10K cycles: launch, lists,
 // first rows, a cold instruction cache) and, for quants, by the producers (a tile's copies and
-// conversion 2700 cycles): 64 sequences of 128 to 2048, 8 nodes, Q8_0 / Q4_0: 39.7 us; one of
-// 65536, 16 nodes, Q8_0: 32.1 us, 558 GB/s.  Both times with the join's launch.
+// conversion 2700 cycles): 64 sequences of 128 to 2048, 8 nodes, Q8_0 / Q4_0: 39.3 us; one of
+// 65536, 16 nodes, Q8_0: 32.0 us, 560 GB/s.  All with the join's launch.
 #pragma once
 
 #include "flash_pipe.cuh"

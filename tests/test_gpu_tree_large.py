@@ -30,7 +30,7 @@ def ragged(seed, S, most):
 def test_tree_list_of_tiles_is_shared(ctx, cv, cuda, oracle, kname, shift):
     """More tiles than SMs, whole units next to parts; 63 rows: half a tile of rows is padding."""
     vname = TYPES[(TYPES.index(kname) + 2 * shift) % 6]
-    rng, lens = ragged(shift, 24, 900)
+    rng, lens = ragged(shift, 24, 1300)
     counts = rng.integers(0, 10, 24).tolist()
     run_case(ctx, cv, cuda, oracle, kname, vname, 14, 2, lens, 9, counts=counts, sees=ancestors(random_parents(rng, 24, 9)), seed=shift)
 
@@ -47,7 +47,7 @@ def test_tree_drafts_after_long_contexts(ctx, cv, cuda, oracle, kname, vname):
 @pytest.mark.parametrize("pads,offsets", [((2, 6, 10, 14), (2, 2, 2, 2)), ((4, 8, 12, 4), (4, 12, 8, 4))])
 def test_tree_shared_list_strides_and_addresses(ctx, cv, cuda, oracle, kname, vname, pads, offsets):
     _, lens = ragged(7, 20, 1100)
-    run_case(ctx, cv, cuda, oracle, kname, vname, 14, 2, lens, 5, pads=pads, offsets=offsets, seq_ptrs=True, q_extra=12)
+    run_case(ctx, cv, cuda, oracle, kname, vname, 14, 2, lens, 12, pads=pads, offsets=offsets, seq_ptrs=True, q_extra=12)
 
 
 @pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("f16", "f16")])
@@ -57,7 +57,7 @@ def test_tree_rows_around_the_tiles(ctx, cv, cuda, oracle, kname, vname, G, n):
 
 
 @pytest.mark.parametrize("kname", ["q8_0", "f16", "q5_1", "f32"])
-@pytest.mark.parametrize("n", [2, 9])
+@pytest.mark.parametrize("n", [2, 9, 20])
 def test_tree_negative_scale(ctx, cv, cuda, oracle, kname, n):
     run_case(ctx, cv, cuda, oracle, kname, kname, 14, 2, [400, 20], n, scale=-0.125)
 
@@ -70,9 +70,9 @@ def test_tree_more_sequences_than_the_table_holds(ctx, cv, cuda, oracle, kname, 
 
 
 @pytest.mark.parametrize("kname", TYPES)
-@pytest.mark.parametrize("Hq,Hkv,n", [(14, 2, 1), (16, 16, 5), (14, 2, 20)])
+@pytest.mark.parametrize("Hq,Hkv,n", [(14, 2, 1), (16, 16, 5), (16, 16, 20), (14, 2, 20)])
 def test_scores_list_of_tiles_is_shared(ctx, cv, cuda, oracle, kname, Hq, Hkv, n):
-    rng, lens = ragged(n, 20, 1000)
+    rng, lens = ragged(n, 20, 1000 if Hkv == 16 else 2000)
     counts = [int(rng.integers(0, min(L, n) + 1)) for L in lens]
     run_scores(ctx, cv, cuda, oracle, kname, Hq, Hkv, lens, n, counts=counts, picked=n == 5, in_place=n == 1)
 
@@ -81,20 +81,20 @@ def test_scores_list_of_tiles_is_shared(ctx, cv, cuda, oracle, kname, Hq, Hkv, n
 @pytest.mark.parametrize("n", [63, 64, 65])
 def test_scores_rows_around_the_limit(ctx, cv, cuda, oracle, kname, n):
     """8 rows a node: 512 rows fit the tensor cores' kernel, 520 take the other."""
-    run_scores(ctx, cv, cuda, oracle, kname, 16, 2, [1500, 1, 64, 1400] + [1300] * 14, n)
+    run_scores(ctx, cv, cuda, oracle, kname, 16, 2, [4000] * 8 + [1, 64, 3900], n)
 
 
 @pytest.mark.parametrize("kname", ["q8_0", "f16", "q5_0"])
 @pytest.mark.parametrize("pad,offset", [(2, 2), (12, 4)])
 def test_scores_shared_list_strides_and_addresses(ctx, cv, cuda, oracle, kname, pad, offset):
-    _, lens = ragged(5, 24, 900)
-    run_scores(ctx, cv, cuda, oracle, kname, 14, 2, lens, 4, pad=pad, offset=offset, seq_ptrs=True, extra=7)
+    _, lens = ragged(5, 24, 2000)
+    run_scores(ctx, cv, cuda, oracle, kname, 14, 2, lens, 8, pad=pad, offset=offset, seq_ptrs=True, extra=7)
 
 
 @pytest.mark.parametrize("kname", ["q8_0", "f16", "q4_1"])
 @pytest.mark.parametrize("size", [1e-3, 20.0])
 def test_scores_shared_list_small_and_large_rows(ctx, cv, cuda, oracle, kname, size):
-    run_scores(ctx, cv, cuda, oracle, kname, 14, 2, [900] * 24, 4, size=size)
+    run_scores(ctx, cv, cuda, oracle, kname, 14, 2, [1700] * 24, 8, size=size)
 
 
 @pytest.mark.parametrize("kname", ["q8_0", "f16"])
@@ -103,14 +103,14 @@ def test_scores_more_sequences_than_the_table_holds(ctx, cv, cuda, oracle, kname
     run_scores(ctx, cv, cuda, oracle, kname, 2, 1, lens, 2)
 
 
-@pytest.mark.parametrize("lens", [[300] * 2, [900] * 24], ids=["few", "many"])
+@pytest.mark.parametrize("lens", [[300] * 2, [2000] * 24], ids=["few", "many"])
 @pytest.mark.parametrize("kname", ["q8_0", "f16", "q5_1"])
 def test_scores_negative_scale_and_rows_without_keys(ctx, cv, cuda, oracle, lens, kname):
     torch = cuda
     from test_gpu_tree import Rows
 
     rng = np.random.default_rng(2)
-    S, n = len(lens), 3
+    S, n = len(lens), 7
     k = Rows(cv, torch, oracle, cv.TYPE_BY_NAME[kname], rng.standard_normal((S, max(lens), 128)).astype(np.float32), 2)
     q = rng.standard_normal((S, n, 14, D)).astype(np.float32)
     lse = true_lse(q, k.f, lens, [n] * S, scale=-0.125)
@@ -184,3 +184,37 @@ def test_rows_past_32_bit_offsets(ctx, cv, cuda, oracle, kname, n):
         assert np.array_equal(a[first:budget], b[first:budget])
         assert np.array_equal(a[:first], b[budget:L + n])
     assert kl.tolist() == [budget]
+
+
+@pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("f16", "f16"), ("q5_1", "q4_1"), ("f16", "q5_0")])
+def test_tree_shared_list_with_drafts_that_are_not_finite(ctx, cv, cuda, oracle, kname, vname):
+    """NaN in a drafted key and infinity in a drafted value, other ones in each sequence, reach only the rows that see them."""
+    torch = cuda
+    from test_gpu_tree import Rows, pack
+
+    rng = np.random.default_rng(2)
+    S, n, L = 40, 12, 600
+    kt, vt = cv.TYPE_BY_NAME[kname], cv.TYPE_BY_NAME[vname]
+    mk = lambda t, m: Rows(cv, torch, oracle, t, rng.standard_normal((S, m, 128)).astype(np.float32), 2)  # noqa: E731
+    k, v, kd, vd = mk(kt, L), mk(vt, L), mk(kt, n), mk(vt, n)
+    sees = ancestors(random_parents(rng, S, n))
+    q = rng.standard_normal((S, n, 14, D)).astype(np.float32)
+    lens = rng.integers(0, L + 1, S).tolist()
+    want, _ = reference(q, k.f, v.f, kd.f, vd.f, lens, [n] * S, sees, 0.125)
+    bad = {id(kd): rng.integers(0, n, S), id(vd): rng.integers(0, n, S)}
+    hit = np.zeros((S, n), dtype=bool)
+    for rows, half in ((kd, [0x00, 0x7E]), (vd, [0x00, 0x7C])):
+        raw = rows.raw().copy()
+        for s, at in enumerate(bad[id(rows)]):
+            if s % 4 == 0:
+                continue  # a sequence without any
+            step = 2 if rows.t == cv.F16 else rows.rb // 4
+            for b in range(0, rows.rb, step):
+                raw[s, at, b:b + 2] = half
+            hit[s] |= sees[s, :, at]
+        rows.buf.copy_(torch.tensor(raw.reshape(-1), device="cuda"))
+    out = cv.tree_decode(ctx, torch.tensor(q, device="cuda"), k.desc, v.desc, kd.desc, vd.desc,
+                         torch.tensor(lens, dtype=torch.int32, device="cuda"), L, mask=torch.tensor(pack(sees), device="cuda")).cpu().numpy()
+    assert np.isfinite(out[~hit]).all()
+    assert rel_l2(out[~hit], want[~hit]) <= REL_L2
+    assert not np.isfinite(out[hit]).all(axis=(1, 2)).any()
