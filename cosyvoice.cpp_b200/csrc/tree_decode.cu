@@ -326,11 +326,15 @@ static cudaError_t launch_tc(cudaStream_t stream, const Args& a, const Plan& pla
     default: break;
     }
     if (e != cudaSuccess) return e;
-    return plan.n_splits > 16 ? run_tc_combine<16>(stream, ta) : plan.n_splits > 4 ? run_tc_combine<4>(stream, ta)
+    // Lanes that share a row's parts.  us of a call with 1 | 4 | 16, 140 rows, Q8_0: 8 parts a unit (one sequence of 300) 15.1 | 13.5 |
+    // 13.9, 18 (4 of 4096) 31.0 | 25.8 | 27.9, 74 (one of 4096) 35.2 | 21.0 | 17.1, 4 (16 of 4096) 50 | 51 | 66.
+    return plan.n_splits > 24 ? run_tc_combine<16>(stream, ta) : plan.n_splits > 4 ? run_tc_combine<4>(stream, ta)
                                                                                    : run_tc_combine<1>(stream, ta);
 }
 
 static cudaError_t launch_combine(cudaStream_t stream, const Args& a) {
+    // The same, 14 rows, Q8_0: 7 parts (one sequence of 300) 9.1 | 8.9 | 9.2, 17 (one of 1000) 11.1 | 9.5 | 9.5, 66 (one of 4096) 18.7 |
+    // 12.3 | 10.8.
     return a.n_splits > 32 ? run_combine<16>(stream, a) : a.n_splits > 8 ? run_combine<4>(stream, a) : run_combine<1>(stream, a);
 }
 
