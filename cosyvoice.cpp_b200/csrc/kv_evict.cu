@@ -80,7 +80,9 @@ __device__ __forceinline__ void move_rows(uint8_t* k, uint8_t* v, const Args& a,
 __device__ __forceinline__ void move_head(const Args& a, int layer, int s, int kvh, const int32_t* dst, const int32_t* src, int i0, int i1) {
     uint8_t* k = a.k[layer] + (int64_t)s * a.k_nb2 + (int64_t)kvh * a.k_slice;
     uint8_t* v = a.v[layer] + (int64_t)s * a.v_nb2 + (int64_t)kvh * a.v_slice;
-    const uint64_t all = reinterpret_cast<uint64_t>(k) | reinterpret_cast<uint64_t>(v) | (uint64_t)a.k_nb1 | (uint64_t)a.v_nb1;
+    // (a slice of an odd number of 2-byte units, such as one Q8_0 block, starts aligned in every second head only)
+    const uint64_t all = reinterpret_cast<uint64_t>(k) | reinterpret_cast<uint64_t>(v) | (uint64_t)a.k_nb1 | (uint64_t)a.v_nb1 |
+                         (uint64_t)a.k_slice | (uint64_t)a.v_slice;
     if ((all & 3) == 0) move_rows<uint32_t>(k, v, a, dst, src, i0, i1);
     else move_rows<uint16_t>(k, v, a, dst, src, i0, i1);
 }
