@@ -9,6 +9,7 @@ CPU path: without the library, importing this package fails.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -107,6 +108,17 @@ def _stream(stream) -> int:
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+def _on(stream):
+    """Context in which what torch allocates belongs to the stream of a call.  A block that was allocated for another stream
+    could be handed out again there while the call still uses it, or be in use there when the call begins."""
+    if stream is None:
+        return contextlib.nullcontext()
+    torch = _torch()
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+    return torch.cuda.stream(stream)
 
 
 def _ptr(t) -> int | None:
@@ -412,9 +424,14 @@ def tree_decode(ctx: Context, q, k: Tensor, v: Tensor, k_draft: Tensor | None, v
                 out=None, lse=None, stream=None, **kw):
     """One verification of a tree of drafts; returns out f32 [n_seq, max_nodes, Hq, D]."""
     torch = _torch()
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    TreeDecoder(ctx, k, v, k_draft, v_draft, q, out, kv_len, max_kv_len, lse=lse, **kw)(stream)
+    with _on(stream):
+        mine = out is None
+        if mine:
+            out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        plan = TreeDecoder(ctx, k, v, k_draft, v_draft, q, out, kv_len, max_kv_len, lse=lse, **kw)
+    if mine and stream is not None:
+        out.record_stream(torch.cuda.current_stream())  # (the caller may drop it there)
+    plan(stream)
     return out
 
 
@@ -551,7 +568,9 @@ class KVEvictor:
 
 def kv_evict(ctx: Context, k, v, scores, pos, kv_len, kept_len, n_tokens, budget: int, stream=None, **kw) -> None:
     """Shrink the caches to the budget (in place unless *_out are given)."""
-    KVEvictor(ctx, k, v, scores, pos, kv_len, kept_len, n_tokens, budget, **kw)(stream)
+    with _on(stream):
+        plan = KVEvictor(ctx, k, v, scores, pos, kv_len, kept_len, n_tokens, budget, **kw)
+    plan(stream)
 
 
 class KVCache:
