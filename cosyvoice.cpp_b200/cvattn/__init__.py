@@ -360,6 +360,19 @@ def _dense(t, dtypes, what, shape=None):
     return t
 
 
+def _device_bytes(t, what):
+    """Scratch memory: contiguous and on the device; its size in bytes."""
+    if not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what}: want a contiguous CUDA tensor")
+    return t.numel() * t.element_size()
+
+
+def _row_ptrs(t, what, n_seq):
+    """Address of a table of row-0 addresses, one per sequence."""
+    torch = _torch()
+    return None if t is None else _dense(t, (torch.int64, torch.uint64), what, (n_seq,)).data_ptr()
+
+
 def _rows4(t, what):
     """A CUDA f32 tensor [n_seq, rows, heads, head_dim] whose rows are dense."""
     torch = _torch()
@@ -390,7 +403,8 @@ class TreeDecoder:
         if lse is not None:
             p.lse = _dense(lse, (torch.float32,), "TreeDecoder lse", (n_seq, n, Hq)).data_ptr()
         p.k, p.v = k, v
-        p.k_seq_ptrs, p.v_seq_ptrs = _ptr(k_seq_ptrs), _ptr(v_seq_ptrs)
+        p.k_seq_ptrs = _row_ptrs(k_seq_ptrs, "TreeDecoder k_seq_ptrs", n_seq)
+        p.v_seq_ptrs = _row_ptrs(v_seq_ptrs, "TreeDecoder v_seq_ptrs", n_seq)
         if k_draft is not None:
             p.k_draft = k_draft
         if v_draft is not None:
@@ -411,7 +425,7 @@ class TreeDecoder:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         self.workspace = workspace
         if workspace is not None:
-            p.workspace, p.workspace_size = workspace.data_ptr(), workspace.numel()
+            p.workspace, p.workspace_size = workspace.data_ptr(), _device_bytes(workspace, "TreeDecoder workspace")
         self.params = p
         self._ref = ctypes.byref(p)
         self._keep = (q, out, kv_len, lse, mask, n_nodes, k_seq_ptrs, v_seq_ptrs)
@@ -482,13 +496,14 @@ class KVScorer:
         n_seq, n, Hq, D = _rows4(q, "KVScorer q").shape
         _dense(lse, (torch.float32,), "KVScorer lse", (n_seq, n, Hq))
         _dense(kv_len, (torch.int32,), "KVScorer kv_len", (n_seq,))
-        if scores.dim() != 3 or scores.shape[:2] != (n_seq, k.n_heads) or scores.stride(2) != 1 or scores.dtype != torch.float32:
+        if scores.dim() != 3 or scores.shape[:2] != (n_seq, k.n_heads) or scores.stride(2) != 1:
             raise ValueError("KVScorer scores: want f32 [n_seq, Hkv, slots]")
-        if scores_out.shape != scores.shape or scores_out.stride() != scores.stride() or scores_out.dtype != torch.float32:
-            raise ValueError("KVScorer scores_out: want the layout of scores")
+        for t, what in ((scores, "scores"), (scores_out, "scores_out")):
+            if t.shape != scores.shape or t.stride() != scores.stride() or t.dtype != torch.float32 or not t.is_cuda:
+                raise ValueError(f"KVScorer {what}: want a CUDA f32 tensor in the layout of scores")
         p = KVScoresParams()
         p.q, p.q_nb_seq, p.q_nb_node = q.data_ptr(), q.stride(0), Hq * D if n == 1 else q.stride(1)
-        p.lse, p.k, p.k_seq_ptrs = lse.data_ptr(), k, _ptr(k_seq_ptrs)
+        p.lse, p.k, p.k_seq_ptrs = lse.data_ptr(), k, _row_ptrs(k_seq_ptrs, "KVScorer k_seq_ptrs", n_seq)
         p.n_q_rows = p.max_rows = n
         if rows is not None:
             _dense(rows, (torch.int32,), "KVScorer rows")
@@ -557,7 +572,7 @@ class KVEvictor:
             need = int(lib.cvattn_kv_evict_workspace_size(len(k), n_seq, k[0].n_heads, p.max_kv_len, budget))
             workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=scores.device)
         self.workspace = workspace
-        p.workspace, p.workspace_size = workspace.data_ptr(), workspace.numel()
+        p.workspace, p.workspace_size = workspace.data_ptr(), _device_bytes(workspace, "KVEvictor workspace")
         self.params = p
         self._ref = ctypes.byref(p)
         self._keep = (list(k), list(v), scores, scores_out, pos, pos_out, kv_len, kept_len, n_tokens, kv_len_out)

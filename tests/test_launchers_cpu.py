@@ -57,3 +57,68 @@ def test_one_shot_calls_allocate_on_the_stream_that_they_run_on(monkeypatch, str
     cv.tree_decode(None, q, None, None, None, None, None, 5)
     cv.kv_evict(None, None, None, None, None, None, None, None, 5)
     assert built[3:] == [[], []] and called[3:] == [None, None] and recorded == ["current"]
+
+
+def tree_arguments(S=2, n=4, L=640):
+    made = {name: cv.kv_tensor(torch.zeros(S * rows * 136, dtype=torch.uint8), cv.Q8_0, 2, D, rows, S)
+            for name, rows in (("k", L), ("v", L), ("k_draft", n), ("v_draft", n))}
+    q = on_device(torch.zeros(S, n, 14, D))
+    return {**made, "q": q, "out": on_device(torch.zeros(S, n, 14, D)), "kv_len": on_device(torch.zeros(S, dtype=torch.int32)), "max_kv_len": L,
+            "workspace": on_device(torch.zeros(cv.tree_decode_workspace_size(cv.Q8_0, cv.Q8_0, S, L, n, 14, 2), dtype=torch.uint8))}
+
+
+def scores_arguments(S=2, n=4, L=64):
+    return {"k": cv.kv_tensor(torch.zeros(S * L * 136, dtype=torch.uint8), cv.Q8_0, 2, D, L, S), "q": on_device(torch.zeros(S, n, 14, D)),
+            "lse": on_device(torch.zeros(S, n, 14)), "kv_len": on_device(torch.zeros(S, dtype=torch.int32)),
+            "scores": on_device(torch.zeros(S, 2, L)), "scores_out": on_device(torch.zeros(S, 2, L))}
+
+
+def evict_arguments(S=2, L=64, budget=32):
+    kv = [[cv.kv_tensor(torch.zeros(S * L * 136, dtype=torch.uint8), cv.Q8_0, 2, D, L, S)] for _ in "kv"]
+    f = lambda: on_device(torch.zeros(1, S, 2, L))  # noqa: E731
+    i = lambda: on_device(torch.zeros(1, S, 2, L, dtype=torch.int32))  # noqa: E731
+    n = lambda: on_device(torch.zeros(S, dtype=torch.int32))  # noqa: E731
+    need = int(cv.lib.cvattn_kv_evict_workspace_size(1, S, 2, L, budget))
+    return {"k": kv[0], "v": kv[1], "scores": f(), "pos": i(), "kv_len": n(), "kept_len": n(), "n_tokens": n(), "budget": budget,
+            "scores_out": f(), "pos_out": i(), "kv_len_out": n(), "workspace": on_device(torch.zeros(need, dtype=torch.uint8))}
+
+
+LAUNCHERS = [(cv.TreeDecoder, tree_arguments), (cv.KVScorer, scores_arguments), (cv.KVEvictor, evict_arguments)]
+
+
+def optional(cls, S=2):
+    table = {name: on_device(torch.zeros(S, dtype=torch.int64)) for name in ("k_seq_ptrs", "v_seq_ptrs")}
+    if cls is cv.TreeDecoder:
+        return {**table, "lse": on_device(torch.zeros(S, 4, 14)), "mask": on_device(torch.zeros(S, 4, 1, dtype=torch.int32)),
+                "n_nodes": on_device(torch.zeros(S, dtype=torch.int32))}
+    if cls is cv.KVScorer:
+        return {"k_seq_ptrs": table["k_seq_ptrs"], "rows": on_device(torch.zeros(S, 3, dtype=torch.int32)),
+                "n_rows": on_device(torch.zeros(S, dtype=torch.int32))}
+    return {}
+
+
+@pytest.mark.parametrize("cls,arguments", LAUNCHERS, ids=lambda x: getattr(x, "__name__", None))
+def test_host_tensors_are_refused(cls, arguments):
+    """Every tensor whose address a kernel gets."""
+    given = {**arguments(), **optional(cls)}
+    cls(None, **given)
+    tensors = [name for name, x in given.items() if isinstance(x, torch.Tensor)]
+    assert len(tensors) >= 7
+    for name in tensors:
+        with pytest.raises(ValueError):
+            cls(None, **{**given, name: given[name].as_subclass(torch.Tensor)})
+
+
+@pytest.mark.parametrize("cls,arguments,name", [(cv.TreeDecoder, tree_arguments, "k_seq_ptrs"), (cv.TreeDecoder, tree_arguments, "v_seq_ptrs"),
+                                                (cv.KVScorer, scores_arguments, "k_seq_ptrs")])
+def test_tables_of_addresses_have_an_address_for_each_sequence(cls, arguments, name):
+    for table in (torch.zeros(1, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)[::2]):
+        with pytest.raises(ValueError):
+            cls(None, **arguments(), **{name: on_device(table)})
+
+
+def test_a_workspace_counts_its_bytes():
+    for cls, arguments in (LAUNCHERS[0], LAUNCHERS[2]):
+        given = arguments()
+        words = on_device(torch.zeros((given["workspace"].numel() + 3) // 4, dtype=torch.float32))
+        assert cls(None, **{**given, "workspace": words}).params.workspace_size == 4 * words.numel()
