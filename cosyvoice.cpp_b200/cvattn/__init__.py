@@ -428,7 +428,7 @@ class TreeDecoder:
             p.workspace, p.workspace_size = workspace.data_ptr(), _device_bytes(workspace, "TreeDecoder workspace")
         self.params = p
         self._ref = ctypes.byref(p)
-        self._keep = (q, out, kv_len, lse, mask, n_nodes, k_seq_ptrs, v_seq_ptrs)
+        self._keep = (q, out, k, v, k_draft, v_draft, kv_len, lse, mask, n_nodes, k_seq_ptrs, v_seq_ptrs)
 
     def __call__(self, stream=None) -> None:
         check(lib.cvattn_tree_decode(self.ctx.handle, _stream(stream), self._ref), "tree_decode")
@@ -522,7 +522,7 @@ class KVScorer:
         p.scale, p.decay = 1.0 / math.sqrt(D) if scale is None else scale, decay
         self.params = p
         self._ref = ctypes.byref(p)
-        self._keep = (q, lse, kv_len, scores, scores_out, rows, n_rows, k_seq_ptrs)
+        self._keep = (q, lse, k, kv_len, scores, scores_out, rows, n_rows, k_seq_ptrs)
 
     def __call__(self, stream=None) -> None:
         check(lib.cvattn_kv_scores(self.ctx.handle, _stream(stream), self._ref), "kv_scores")

@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import contextlib
+import gc
+import weakref
 
 import pytest
 import torch
@@ -122,3 +124,30 @@ def test_a_workspace_counts_its_bytes():
         given = arguments()
         words = on_device(torch.zeros((given["workspace"].numel() + 3) // 4, dtype=torch.float32))
         assert cls(None, **{**given, "workspace": words}).params.workspace_size == 4 * words.numel()
+
+
+def commit_arguments(S=2, n=4, L=64):
+    of = lambda rows: [cv.kv_tensor(torch.zeros(S * rows * 136, dtype=torch.uint8), cv.Q8_0, 2, D, rows, S) for _ in "kv"]  # noqa: E731
+    ints = lambda *s: on_device(torch.zeros(s, dtype=torch.int32))  # noqa: E731
+    return {"caches": of(L), "drafts": of(n), "accepted": ints(S, n), "n_accepted": ints(S), "kv_len": ints(S), "kv_len_out": ints(S)}
+
+
+@pytest.mark.parametrize("cls,arguments", [*LAUNCHERS, (cv.TreeCommitter, commit_arguments)], ids=lambda x: getattr(x, "__name__", None))
+def test_a_launcher_keeps_its_buffers(cls, arguments):
+    """Tensors, and the buffers behind descriptors, live as long as the launcher that will use them again."""
+    given = {**arguments(), **(optional(cls) if cls is not cv.TreeCommitter else {})}
+    refs = []
+    for x in given.values():
+        for y in x if isinstance(x, list) else [x]:
+            if isinstance(y, torch.Tensor):
+                refs.append(weakref.ref(y))
+            elif isinstance(y, cv.Tensor):
+                refs.append(weakref.ref(y._buf))
+    plan = cls(None, **given)
+    assert len(refs) >= 8
+    del given, x, y
+    gc.collect()
+    assert all(r() is not None for r in refs)
+    del plan
+    gc.collect()
+    assert all(r() is None for r in refs)
