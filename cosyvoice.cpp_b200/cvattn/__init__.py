@@ -373,11 +373,12 @@ def _row_ptrs(t, what, n_seq):
     return None if t is None else _dense(t, (torch.int64, torch.uint64), what, (n_seq,)).data_ptr()
 
 
-def _rows4(t, what):
+def _rows4(t, what, head_dim):
     """A CUDA f32 tensor [n_seq, rows, heads, head_dim] whose rows are dense."""
     torch = _torch()
-    if t.dtype != torch.float32 or not t.is_cuda or t.dim() != 4 or t.stride(3) != 1 or t.stride(2) != t.shape[3]:
-        raise ValueError(f"{what}: want a CUDA f32 tensor [n_seq, rows, heads, head_dim] with dense rows")
+    if (t.dtype != torch.float32 or not t.is_cuda or t.dim() != 4 or t.shape[3] != head_dim or t.stride(3) != 1
+            or t.stride(2) != head_dim):
+        raise ValueError(f"{what}: want a CUDA f32 tensor [n_seq, rows, heads, {head_dim}] with dense rows")
     return t
 
 
@@ -391,8 +392,8 @@ class TreeDecoder:
                  scale: float | None = None, workspace=None):
         torch = _torch()
         self.ctx = ctx
-        n_seq, n, Hq, D = _rows4(q, "TreeDecoder q").shape
-        if _rows4(out, "TreeDecoder out").shape != q.shape:
+        n_seq, n, Hq, D = _rows4(q, "TreeDecoder q", k.head_dim).shape
+        if _rows4(out, "TreeDecoder out", k.head_dim).shape != q.shape:
             raise ValueError("TreeDecoder out: another shape than q")
         _dense(kv_len, (torch.int32,), "TreeDecoder kv_len", (n_seq,))
         p = TreeParams()
@@ -493,7 +494,7 @@ class KVScorer:
         torch = _torch()
         self.ctx = ctx
         scores_out = scores if scores_out is None else scores_out
-        n_seq, n, Hq, D = _rows4(q, "KVScorer q").shape
+        n_seq, n, Hq, D = _rows4(q, "KVScorer q", k.head_dim).shape
         _dense(lse, (torch.float32,), "KVScorer lse", (n_seq, n, Hq))
         _dense(kv_len, (torch.int32,), "KVScorer kv_len", (n_seq,))
         if scores.dim() != 3 or scores.shape[:2] != (n_seq, k.n_heads) or scores.stride(2) != 1:

@@ -151,3 +151,14 @@ def test_a_launcher_keeps_its_buffers(cls, arguments):
     del plan
     gc.collect()
     assert all(r() is None for r in refs)
+
+
+@pytest.mark.parametrize("cls,arguments", LAUNCHERS[:2], ids=lambda x: getattr(x, "__name__", None))
+@pytest.mark.parametrize("heads,head_dim", [(14, 128), (7, 128), (28, 32)])
+def test_queries_have_the_head_size_of_the_cache(cls, arguments, heads, head_dim):
+    """Wider heads would pass the checks of strides and be read as other heads."""
+    given = arguments()
+    q = on_device(torch.zeros(2, 4, heads, head_dim))
+    given |= {"q": q, "out": q.clone()} if cls is cv.TreeDecoder else {"q": q, "lse": on_device(torch.zeros(2, 4, heads))}
+    with pytest.raises(ValueError):
+        cls(None, **given)
