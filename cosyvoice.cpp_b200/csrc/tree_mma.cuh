@@ -45,6 +45,9 @@ constexpr int kOutPad = kD + 4;
 constexpr int kMaxStages = 4;
 constexpr int kHalfSm = 112 * 1024;  // shared memory of a CTA when two share an SM
 constexpr float kLazy = 8.0f;
+// The least scale d_V 2^ev of a drafted value that goes through f16: what hi + lo leave out of P' is then below 2^-19 of a
+// weight of 1.  (ev brings the largest scale of a first tile to [2^4, 2^5), so ordinary drafts lie well above.)
+constexpr float kLeastScale = 1.0f / 64.0f;
 
 struct Shape {
     int row_groups;    // CTAs along the rows, 128 rows each
@@ -468,7 +471,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_mma_kernel(const __grid_c
                     }
             }
             if (draft) {
-                // Drafts hold anything where no row may look: a step whose values are not all finite is added up key by
+                // Drafts hold anything where no row may look: a step whose values are not all finite, or lie so far below the
+                // largest of the tile (which a row may not see) that P' would leave f16's normal numbers, is added up key by
                 // key, and keys that a row does not see are left out instead of being multiplied by zero.
                 bool special = false;
                 if constexpr (V_Q) {
@@ -478,6 +482,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_mma_kernel(const __grid_c
                         for (int tt = 0; tt < 2; ++tt) {
                             special |= !isfinite(dv[b][tt].x) || !isfinite(dv[b][tt].y);
                             special |= !isfinite(vm[b][tt].x) || !isfinite(vm[b][tt].y);
+                            special |= dv[b][tt].x != 0.0f && fabsf(dv[b][tt].x) < kLeastScale;
+                            special |= dv[b][tt].y != 0.0f && fabsf(dv[b][tt].y) < kLeastScale;
                         }
                 } else {
 #pragma unroll 1
