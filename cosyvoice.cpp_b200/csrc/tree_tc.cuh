@@ -337,6 +337,11 @@ __device__ __forceinline__ uint32_t row_max(const uint8_t* row, bool& special) {
     return m;
 }
 
+// Least exponent e (tile_exp) of a tile of drafts that goes through f16.  With e >= 0 scales, f16 themselves, and hi and lo stay exact
+// however small they are; values with a min are rounded to multiples of 2^-25 / 2^e.  Below it the tile's largest row, which a row of
+// queries may not see, would cost the other rows bits.
+template <int T> constexpr int kLeastExp = BlockTraits<T>::HAS_MIN ? 2 : 0;
+
 // A producer warpgroup: the K (or V) tiles of the CTA, thread = key.
 template <int KT, int VT, bool kV>
 __device__ __forceinline__ void produce(const TcArgs& ta, uint8_t* smem, TcBars* B, const SeqTab& tab, Run r, int lo, int hi) {
@@ -386,7 +391,7 @@ __device__ __forceinline__ void produce(const TcArgs& ta, uint8_t* smem, TcBars*
             }
             if (key == 0) {
                 slots[slot == 2 ? 0 : slot + 1] = 0u;  // of the tile after the next: read by all before this barrier
-                (kV ? B->expv : B->expk)[n % kTcExps] = pow2f(-e);
+                (kV ? B->expv : B->expk)[n % kTcExps] = draft && e < kLeastExp<T> ? 0.0f : pow2f(-e);  // (0: kept out of the products)
                 if (!kV) B->starts[n % kTcExps] = (uint32_t)first;
             }
             first = 0;
@@ -662,6 +667,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                     O[16 + d] = ffma2(make_float2(__uint_as_float(o1[2 * d]), __uint_as_float(o1[2 * d + 1])), f, O[16 + d]);
                 }
             };
+            // The drafts of a tile that f16 does not hold beside one another (the group's last tile), in f32 and one after another: a
+            // lane has two dims of the key and the value, and every lane its row, which adds up only what it sees.  Its weights are
+            // in l already where only V kept the tile out (vs_last is not 0).
+            auto key_by_key = [&]() {
+                bool draft;
+                int p0, count;
+                r.tile(lo + n_last, draft, p0, count);
+                int s = r.s, t = threadIdx.x;
+                asm volatile("" : "+r"(s), "+r"(t));  // (addresses are formed here: ahead of the tiles' loop they would cost its registers)
+                const int rr = r.rt * kTcRows + (t & 127), node = (int)(((uint32_t)rr * ta.inv_g) >> 16);
+                const float2* q = reinterpret_cast<const float2*>(a.q + (int64_t)s * a.q_nb_seq +
+                                                                  (real ? (int64_t)node * a.q_nb_node + (r.kvh * a.G + rr - node * a.G) * kD : 0));
+                const int blk = r.kvh * 2 + ((t >> 4) & 1), e = 2 * t & 31;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t bits = real ? seen_drafts(p0, count, c) : 0u;
+#pragma unroll 1
+                    for (uint32_t any = __reduce_or_sync(0xffffffffu, bits); any; any &= any - 1) {
+                        const int b = __ffs(any) - 1;
+                        const int64_t at = p0 + 32 * c + b;
+                        const uint8_t* kr = a.kd + (int64_t)s * a.kd_nb2 + at * a.kd_nb1 + blk * group_bytes(KT);
+                        const uint8_t* vr = a.vd + (int64_t)s * a.vd_nb2 + at * a.vd_nb1 + blk * group_bytes(VT);
+                        const float k0 = dequant_elem<KT>(kr, e), k1 = dequant_elem<KT>(kr, e + 1);
+                        const float v0 = dequant_elem<VT>(vr, e), v1 = dequant_elem<VT>(vr, e + 1);
+                        float x = 0.0f;
+#pragma unroll 4
+                        for (int d = 0; d < 32; ++d) {
+                            const float2 y = q[d];
+                            x = fmaf(y.x, __shfl_sync(0xffffffffu, k0, d), x);
+                            x = fmaf(y.y, __shfl_sync(0xffffffffu, k1, d), x);
+                        }
+                        x = (bits >> b) & 1u ? fmaf(x, a.scale_log2, -base) : -INFINITY;
+                        if (__any_sync(0xffffffffu, x > thr)) {
+                            float f = 1.0f;
+                            if (x > thr) {
+                                const float up = x - kTcOffs;
+                                f = thr == -INFINITY ? 0.0f : fast_exp2(-up);
+                                base += up;
+                                thr = kLazy + kTcOffs;
+                                l *= f;
+                                x -= up;
+                            }
+                            const float2 f2 = make_float2(f, f);
+#pragma unroll
+                            for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
+                        }
+                        const float p = fast_exp2(x);
+                        if (vs_last == 0.0f) l += p;
+                        const float2 p2 = make_float2(p, p);
+#pragma unroll
+                        for (int d = 0; d < 32; ++d) {
+                            const float2 v = make_float2(__shfl_sync(0xffffffffu, v0, d), __shfl_sync(0xffffffffu, v1, d));
+                            if (p != 0.0f) O[d] = ffma2(p2, v, O[d]);
+                        }
+                    }
+                }
+            };
             for (int j = r.i + ((r.i ^ g ^ lo) & 1); j < r.end; j += 2) {  // the CTA's tiles j - lo of parity g
                 bool draft;
                 int p0, count;
@@ -671,6 +733,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 ok = tc_wait(&B->s_full[buf], (n / 3) & 1, &B->err, 31);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc::fence_after();
+                if constexpr (NK == 2) {
+                    if (B->expk[n % kTcExps] == 0.0f) count = 0;  // none of its keys is seen here
+                }
                 if (warp_real) {
                     uint32_t sv[32];
                     tc::tmem_ld32(sp, sv);
@@ -765,7 +830,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                         tc::fence_after();
                         add_output();
                     }
-                    vs_last = 1.0f;
+                    vs_last = NK == 2 && B->expk[n % kTcExps] == 0.0f ? 0.0f : 1.0f;
                     n_last = n;
                     pending = true;
                     tc::tmem_st_wait();
@@ -780,6 +845,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 tc::fence_after();
                 if (ok) add_output();
             }
+            if constexpr (NK == 2 || NV == 2)
+                if (ok && pending && vs_last * B->expv[n_last % kTcExps] == 0.0f) key_by_key();
             tc::fence_before();
             if (!fp::prod_bar_and(2, 256, ok)) break;  // every MMA of the run is done; all threads leave together
             const float m_mine = thr == -INFINITY && l == 0.0f ? -INFINITY : base;  // (NaN scores raise nothing)

@@ -26,7 +26,7 @@ def with_far_rows(rows, torch, at, half):
     rows.buf.copy_(torch.tensor(raw.reshape(-1), device="cuda"))
 
 
-def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0):
+def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0, broken=False):
     rng = np.random.default_rng(seed)
     S, cap = len(lens), max(max(lens), 1)
     kt, vt = cv.TYPE_BY_NAME[kname], cv.TYPE_BY_NAME[vname]
@@ -39,10 +39,16 @@ def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0):
     at = [rng.integers(1, n, S), rng.integers(1, n, S)]
     with_far_rows(kd, torch, at[0], half)
     with_far_rows(vd, torch, at[1], half)
-    hit = np.zeros((S, n), dtype=bool)
+    if broken:  # and others that are not finite
+        at += [rng.integers(1, n, S), rng.integers(1, n, S)]
+        with_far_rows(kd, torch, at[2], [0x00, 0x7E])
+        with_far_rows(vd, torch, at[3], [0x00, 0x7C])
+    hit, blown = np.zeros((S, n), dtype=bool), np.zeros((S, n), dtype=bool)
     for s in range(S):
-        for j in (at[0][s], at[1][s]):
-            hit[s] |= sees[s, :, j]
+        for j in at:
+            hit[s] |= sees[s, :, j[s]]
+        for j in at[2:]:
+            blown[s] |= sees[s, :, j[s]]
     lse = torch.empty((S, n, 14), device="cuda")
     out = cv.tree_decode(ctx, torch.tensor(q, device="cuda"), k.desc, v.desc, kd.desc, vd.desc,
                          torch.tensor(lens, dtype=torch.int32, device="cuda"), cap, mask=torch.tensor(pack(sees), device="cuda"), lse=lse,
@@ -51,6 +57,7 @@ def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0):
     worst = max(rel_l2(out[s, i], want[s, i]) for s in range(S) for i in range(n) if not hit[s, i])
     assert worst <= REL_L2, worst
     assert np.abs(lse.cpu().numpy()[~hit] - want_lse[~hit]).max() <= LSE_ABS
+    assert not np.isfinite(out[blown]).all(axis=(1, 2)).any()
 
 
 LARGE, SMALL = [0xFF, 0x7B], [0x01, 0x00]  # 65504 and the least f16 above 0
@@ -65,16 +72,30 @@ def test_far_drafts_little_work(ctx, cv, cuda, oracle, kname, vname, half):
 
 @pytest.mark.parametrize("size", [0.05, 30.0])
 @pytest.mark.parametrize("kname,vname", [("q8_0", "q8_0"), ("q4_1", "q5_0"), ("q5_1", "f16")])
-@pytest.mark.parametrize("lens,n", [([60, 0], 11), ([300, 7, 64], 8)])
+@pytest.mark.parametrize("lens,n", [([60, 0], 11), ([0, 130, 400], 60), ([200] * 40, 20), ([5], 200)])
 def test_far_drafts_of_other_sizes(ctx, cv, cuda, oracle, kname, vname, lens, n, size):
     run_far(ctx, cv, cuda, oracle, kname, vname, lens, n, size, LARGE)
 
 
+@pytest.mark.parametrize("kname", TYPES)
+@pytest.mark.parametrize("vname", TYPES)
+@pytest.mark.parametrize("half", [LARGE, SMALL], ids=["large", "small"])
+def test_far_drafts_on_the_persistent_kernel(ctx, cv, cuda, oracle, kname, vname, half):
+    """More than 128 rows of a KV head; the second sequence has drafts alone, in two tiles."""
+    run_far(ctx, cv, cuda, oracle, kname, vname, [60, 0], 140, 1.0, half)
+
+
+@pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("q5_1", "q5_0"), ("f16", "q8_0"), ("q4_1", "f16"), ("f16", "f16")])
+@pytest.mark.parametrize("lens,n", [([60, 0], 30), ([300] * 20, 12), ([0, 90], 200)])
+def test_far_drafts_beside_ones_that_are_not_finite(ctx, cv, cuda, oracle, kname, vname, lens, n):
+    run_far(ctx, cv, cuda, oracle, kname, vname, lens, n, 1.0, LARGE, seed=7, broken=True)
+
+
 @pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("q5_0", "q5_1"), ("f16", "q8_0"), ("q4_0", "f16")])
 def test_rows_that_see_a_far_draft(ctx, cv, cuda, oracle, kname, vname):
-    """A far value alone: rows that see it are right relative to their own size."""
+    """A far value alone: rows that see it are right relative to their own size, on either kernel."""
     torch = cuda
-    for lens, n in (([60, 3], 11), ([300, 7, 64], 8)):
+    for lens, n in (([60, 3], 11), ([200] * 40, 20), ([5, 90], 140)):
         rng = np.random.default_rng(n)
         S, cap = len(lens), max(lens)
         kt, vt = cv.TYPE_BY_NAME[kname], cv.TYPE_BY_NAME[vname]
