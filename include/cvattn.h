@@ -482,7 +482,7 @@ cvattn_status cvattn_kv_scores(cvattn_context* ctx, void* stream, const cvattn_k
  * pos[j] where j < kept_len (what the last eviction left), else the next tokens
  * in order, the last slot holding token n_tokens - 1.  Kept are the first n_sink
  * tokens, the last n_recent ones and, up to the budget, the highest scores (ties:
- * the lower slot; a NaN ranks below every number).  Kept rows at slots >= budget
+ * the lower slot; a NaN counts as -infinity).  Kept rows at slots >= budget
  * move into the freed slots below it, both in ascending order; other rows stay.
  * Attention does not depend on the order of the rows, and cached keys carry
  * their rotation, so the heads may keep different tokens.
