@@ -102,8 +102,9 @@ def _torch():
 def _stream(stream) -> int:
     if stream is None:
         torch = _torch()
-        if torch.cuda.is_initialized():  # the handle alone: building a Stream object costs 3.5 us a call
-            return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+        if raw and device and torch.cuda.is_initialized():  # the handle alone: building a Stream object costs 3.5 us a call
+            return raw(device())
         return torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream

@@ -22,6 +22,23 @@ def on_device(t):
     return t.as_subclass(Device)
 
 
+class Handle:
+    cuda_stream = 77
+
+
+@pytest.mark.parametrize("missing", [None, "_cuda_getCurrentRawStream", "_cuda_getDevice"])
+def test_the_current_stream_without_private_functions(monkeypatch, missing):
+    """The handle comes from functions of torch that are not public where there are such, else from the stream object."""
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: Handle)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 3, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 55 + device, raising=False)
+    if missing:
+        monkeypatch.delattr(torch._C, missing)
+    assert cv._stream(None) == (77 if missing else 58)
+    assert cv._stream(5) == 5 and cv._stream(Handle) == 77
+
+
 @pytest.fixture
 def streams(monkeypatch):
     """The streams that are current, innermost last."""
