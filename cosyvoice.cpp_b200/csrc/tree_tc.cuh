@@ -413,7 +413,8 @@ __device__ __forceinline__ void produce(const TcArgs& ta, uint8_t* smem, TcBars*
                 ++use;
             }
         }
-        cp_async_wait<0>();
+        // (after an error tiles are under way that nobody waited for; these copies are in no group)
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // f16 rows straight into the tiles, kPre of them ahead of the one that is handed on
         constexpr int kPre = kSt - 2, slice = 2 * kD;
