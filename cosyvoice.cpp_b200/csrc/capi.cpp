@@ -561,6 +561,9 @@ cvattn_status cvattn_tree_commit(cvattn_context* ctx, void* stream, const cvattn
         return CVATTN_ERR_INVALID_ARGUMENT;
     if (p->n_seq > 1 && p->accepted_stride < p->max_accepted) return CVATTN_ERR_INVALID_ARGUMENT;
     if (overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->n_accepted, 4 * (int64_t)p->n_seq)) return CVATTN_ERR_INVALID_ARGUMENT;
+    // (nodes are checked when they are read first, and read again for the copies)
+    if (overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->accepted, 4 * ((p->n_seq - 1) * p->accepted_stride + p->max_accepted)))
+        return CVATTN_ERR_INVALID_ARGUMENT;
     if (p->kv_len_out != p->kv_len && overlap(p->kv_len_out, 4 * (int64_t)p->n_seq, p->kv_len, 4 * (int64_t)p->n_seq))
         return CVATTN_ERR_INVALID_ARGUMENT;
     int64_t capacity = INT32_MAX, draft_rows = INT32_MAX;
