@@ -1,4 +1,4 @@
-"""GPU: which positions an eviction keeps where the scores leave it to the slots."""
+"""GPU: which positions an eviction keeps where the scores leave it to the slots, and in lists longer than a CTA keeps keys of."""
 from __future__ import annotations
 
 import numpy as np
@@ -28,3 +28,12 @@ def test_numbers_rank_above_both(ctx, cv, cuda, oracle, low):
         return x
 
     run_evict(ctx, cv, cuda, oracle, "q8_0", "q4_0", 2, [80], 40, make=make, kept=[0])
+
+
+@pytest.mark.parametrize("L,budget", [(40960, 40000), (40961, 40001), (43000, 300), (43000, 42990)])
+def test_evict_more_slots_than_a_cta_keeps_keys_of(ctx, cv, cuda, oracle, L, budget):
+    """Slots from 40960 on have their keys formed again at every step; ties fall on both sides of that line."""
+    def levels(rng, shape):
+        return rng.integers(0, 40, shape) * 0.125
+
+    run_evict(ctx, cv, cuda, oracle, "q8_0", "q4_0", 1, [L], budget, layers=1, sink=3, recent=17, make=levels)
