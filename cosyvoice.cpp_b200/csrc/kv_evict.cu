@@ -92,8 +92,10 @@ __device__ __forceinline__ void move_head(const Args& a, int layer, int s, int k
 // at a time; of the slots that equal it, the lowest stay.  Each warp owns a run of
 // slots, so ranks in slot order are ballots plus one prefix over the warps.
 // Latency-bound: four passes over keys in shared memory with a barrier each.  24 layers of one
-// sequence, 576 slots to 512: 7.8 us, moves included; 6 layers of 16 sequences of up to 8192
-// to 1024: 22 us of 32 (the moves are the rest), 1.3 TB/s of scores, tokens and rows in all.
+// sequence, 576 slots to 512: 7.7 us, moves included; 6 layers of 16 sequences of up to 8192
+// to 1024: 22 us of 31 (the moves are the rest), 1.3 TB/s of scores, tokens and rows in all.
+// (Calls in a graph that repeat on the same buffers: scores and tokens come from L2.  On buffers
+// that are not there the second takes 38 us.)
 __global__ void __launch_bounds__(kThreads, 2) evict_select_kernel(const __grid_constant__ Args a) {
     extern __shared__ uint32_t keys[];
     __shared__ uint32_t hist[2][256];
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_select_kernel(const __grid_
 constexpr int kMoveChunk = 64;  // rows of one head per CTA
 
 // The moves of long lists, spread over CTAs of their own.  Scattered slices of 36 to 128 bytes:
-// bound by the sectors that they touch; 16 sequences of 8192 to 1024, Q8_0 / Q4_0: 10 us.
+// bound by the sectors that they touch; 16 sequences of 8192 to 1024, Q8_0 / Q4_0: 9 us.
 __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ Args a, int n_seq) {
     const int kvh = blockIdx.y % a.Hkv, s = blockIdx.y / a.Hkv, layer = blockIdx.z;
     const int32_t* ws = a.ws + (((int64_t)layer * n_seq + s) * a.Hkv + kvh) * (2 * (int64_t)a.moves + 4);
@@ -381,8 +383,8 @@ __device__ __forceinline__ bool fits(const Args& a, int s, int L, int n) {
 }
 
 // A CTA per sequence and tensor.  Latency-bound (a launch, two dependent loads, the copy): 48
-// tensors of one sequence, 4 rows 2.3 us; of 64 sequences, up to 16 rows 5.7 us for 5.6 MB
-// read and written, 0.98 TB/s.
+// tensors of one sequence, 4 rows 2.2 us; of 64 sequences, up to 16 rows 5.5 us for 5.6 MB
+// read and written, 1.0 TB/s (in a graph; a call by itself, bound by the host, takes 5.0 and 5.4).
 __global__ void __launch_bounds__(128) commit_kernel(const __grid_constant__ Args a) {
     const int s = blockIdx.x;
     const Tensor& t = a.t[blockIdx.y];

@@ -9,8 +9,9 @@ constexpr int kRows = 32;   // (token, head) rows at a time
 constexpr int kPad = kD + 4;
 
 // f32 caches, on the CUDA cores: a thread owns 4 rows x 4 keys of a 32 x 64 tile.  Bound by
-// FMAs and shared-memory reads (8 sequences of 8192, 64 rows of 14 heads: 404 us; the tensor
-// cores' kernel 40 from f16).
+// FMAs, shared-memory reads and the loads of a tile, an element at a time (8 sequences of 8192,
+// 64 rows of 14 heads: 381 us, from f16 the tensor cores' kernel 40; 64 of up to 4096, 4 rows:
+// 146 us, from Q8_0 20).
 __global__ void __launch_bounds__(128) scores_f32_kernel(const __grid_constant__ Args a) {
     __shared__ float4 qs4[kRows][kPad / 4], ks4[kTile][kPad / 4];
     __shared__ float ls[kRows], red[8][kTile];

@@ -19,10 +19,12 @@
 //   warps 16, 17    MMA issuers of the groups
 //   warp 18         loader: raw rows of the next tiles, one bulk copy each where they hold
 //                   at most two heads and lie packed (else the producers copy the slices)
-// What bounds it: 8 sequences of 8192 positions, 64 rows of 14 heads, f16: 40.6 us, 185 TFLOP/s;
-// a group sums 128 x 128 in 2800 cycles, of which the exponentials are 2048 (a quarter of the
-// SM's unit per warp).  64 sequences of up to 4096, 4 rows, Q8_0: 20 us for 20 MB; start and
-// change of runs (10K and 2K cycles) are half of it, the rest the tiles' conversion.
+// What bounds it: 8 sequences of 8192 positions, 64 rows of 14 heads, f16: 40.2 us, 187 TFLOP/s.
+// A group sums 128 x 128 in 2800 cycles, in which the exponentials of both groups take 2048 of
+// the SM's unit; the sums are 34K of a CTA's 63K active cycles (over all of them the unit is 40 %
+// busy).  The rest is the start and Q: no product begins before all rows of a run are prepared.
+// 64 sequences of up to 4096, 4 rows, Q8_0: 19.9 us for 20 MB; start and change of runs (10K and
+// 2K cycles) are half of it, the rest the tiles' conversion.
 #pragma once
 
 #include "kv_scores.cuh"

@@ -10,10 +10,10 @@ namespace tree {
 // A CTA of 128 threads takes 32 rows of one KV head and one split.  K and V tiles
 // are dequantized to f32 in shared memory; a thread owns 4 rows x 4 keys of S and
 // then 4 rows x 4 dims of the output.  Rows are padded to 68 floats, so the eight
-// float4s of a phase (keys apart by one row) touch different banks.  Bound by its FMAs and
-// shared-memory reads: f32 rows have no exact f16 pieces, and the caches that matter are not
-// f32.  (This kernel with Q8_0 rows: 64 sequences of 128 to 2048, 8 nodes 315 us, where the
-// tcgen05 kernel takes 39.3.)
+// float4s of a phase (keys apart by one row) touch different banks.  For f32 rows on either
+// side, which have no two exact f16 pieces.  Bound by its FMAs, its shared-memory reads and the
+// loads of a tile, an element at a time: 64 sequences of 128 to 2048, 8 nodes, f32 388 us, f32 K
+// and Q8_0 V 325; 16 of 4096, 64 nodes, f32 2.2 ms.  (Q8_0 / Q4_0 on the tcgen05 kernel: 39.4.)
 constexpr int kTile = 64;  // keys per tile
 constexpr int kRows = 32;
 constexpr int kPad = kD + 4;
@@ -250,7 +250,7 @@ constexpr int kSlots = 2 * kSms;  // two CTAs of tree_mma_kernel per SM
 // heads, Q8_0 and f16: one sequence of 4096 (66 tiles), 112 rows 15.4 | 15.6 and 13.4 | 15.2, 252 rows 20.0 | 17.3 and 18.4 |
 // 16.3; 16 of 1000 (288), 56 rows 17.6 | 23.5 and 14.5 | 22.0, 112 rows 24.6 | 25.2 and 21.2 | 23.8; one of 65536 (1026), 28
 // rows 31.8 | 29.9 and 22.4 | 24.3, 56 rows 41.6 | 30.5 and 30.8 | 25.0; 64 of 4096 (4224), 7 rows 86 | 74 and 51 | 55, 28 rows
-// 108 | 75 and 69 | 55.
+// 108 | 75 and 69 | 55.  (One number for both kinds of cache: at 64 of 4096 with 7 rows, 29568, it keeps quants on the slower side.)
 constexpr int64_t kTcMinWork = 1 << 15;
 
 static Plan plan_of(int k_type, int v_type, int n_seq, int max_kv_len, int max_nodes, int n_q_heads, int n_kv_heads) {

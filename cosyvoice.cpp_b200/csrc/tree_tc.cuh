@@ -26,13 +26,18 @@
 // a time by that chunk's P (16 columns hi, 16 lo): a group never waits for the
 // S of its next tile.  Two outputs of 64 columns, one per group, read back while
 // the group's next tile is on its way.
+// Drafts that a row does not see may be of any size, and a tile has one power of two: a tile
+// of quantized drafts whose largest scales would cost the others bits (kLeastExp) is marked
+// by its producers, gets no weight in the products and is added row by row in f32.
 // What bounds it: the softmax's instructions.  A tile of 128 rows x 128 keys costs the two
 // groups together some 2100 cycles (exponentials alone 1024, products 770).  16 sequences of
-// 4096 positions, 64 nodes, 14 / 2 heads, f16: 61 us, 249 TFLOP/s (twice that in the tensor
-// cores, for hi and lo).  Few tiles per CTA are bound by the start (10K cycles: launch, lists,
-// first rows, a cold instruction cache) and, for quants, by the producers (a tile's copies and
-// conversion 2700 cycles): 64 sequences of 128 to 2048, 8 nodes, Q8_0 / Q4_0: 39.3 us; one of
-// 65536, 16 nodes, Q8_0: 32.0 us, 560 GB/s.  All with the join's launch.
+// 4096 positions, 64 nodes, 14 / 2 heads, f16: 60.5 us, 252 TFLOP/s (twice that in the tensor
+// cores, for hi and lo); 29 tiles a CTA and the start are four fifths of its active cycles.
+// Few tiles per CTA are bound by the start (10K cycles: launch, lists, first rows, a cold
+// instruction cache) and, for quants, by the producers (a tile's copies and conversion 2700
+// cycles): 64 sequences of 128 to 2048, 8 nodes, Q8_0 / Q4_0: 39.4 us (nine tiles and the
+// start are 34K of 53K active cycles; the rest is not accounted for); one of 65536, 16 nodes,
+// Q8_0: 31.7 us, 565 GB/s.  All with the join's launch, calls in a graph.
 #pragma once
 
 #include "flash_pipe.cuh"
@@ -54,7 +59,7 @@ constexpr float kTcOffs = 7.0f;
 
 struct TcArgs {
     Args a;
-    uint32_t inv_g;                   // ceil(2^16 / G): r * inv_g >> 16 = r / G for r < 2^13 / G
+    uint32_t inv_g;                   // ceil(2^16 / G): r * inv_g >> 16 = r / G while r (G inv_g - 2^16) < 2^16: G <= 8, so r < 13107
     int grid;                         // CTAs that share the list
     float* ws_o;                      // [2 * grid][128][64]
     float* ws_ml;                     // [2 * grid][128][2]
@@ -730,6 +735,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 int p0, count;
                 r.tile(j, draft, p0, count);
                 const int n = j - lo, buf = n % 3;
+                // (Of a buffer's phases a group sees every second one, always of the same parity.  It cannot pass on an older one:
+                // S of tile n - 3, the phase before, was committed ahead of S of n - 2, which this group has seen.)
                 const uint32_t sp = tmem + lane_base + buf * 128;
                 ok = tc_wait(&B->s_full[buf], (n / 3) & 1, &B->err, 31);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }

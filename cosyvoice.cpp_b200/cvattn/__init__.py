@@ -438,7 +438,8 @@ class TreeDecoder:
 
 def tree_decode(ctx: Context, q, k: Tensor, v: Tensor, k_draft: Tensor | None, v_draft: Tensor | None, kv_len, max_kv_len: int,
                 out=None, lse=None, stream=None, **kw):
-    """One verification of a tree of drafts; returns out f32 [n_seq, max_nodes, Hq, D]."""
+    """One verification of a tree of drafts; returns out f32 [n_seq, max_nodes, Hq, D].  (Builds a TreeDecoder each time: a
+    program that keeps its buffers keeps one.)"""
     torch = _torch()
     with _on(stream):
         mine = out is None
@@ -479,7 +480,8 @@ class TreeCommitter:
 
 
 def tree_commit(ctx: Context, caches, drafts, accepted, n_accepted, kv_len, kv_len_out=None, stream=None):
-    """Commit accepted drafts; returns kv_len_out (by default kv_len, in place)."""
+    """Commit accepted drafts; returns kv_len_out (by default kv_len, in place).  (Builds a TreeCommitter each time, which for
+    every layer's K and V of a model takes longer than the copies: a program that keeps its buffers keeps one.)"""
     kv_len_out = kv_len if kv_len_out is None else kv_len_out
     TreeCommitter(ctx, caches, drafts, accepted, n_accepted, kv_len, kv_len_out)(stream)
     return kv_len_out
@@ -584,7 +586,7 @@ class KVEvictor:
 
 
 def kv_evict(ctx: Context, k, v, scores, pos, kv_len, kept_len, n_tokens, budget: int, stream=None, **kw) -> None:
-    """Shrink the caches to the budget (in place unless *_out are given)."""
+    """Shrink the caches to the budget (in place unless *_out are given).  (Builds a KVEvictor each time.)"""
     with _on(stream):
         plan = KVEvictor(ctx, k, v, scores, pos, kv_len, kept_len, n_tokens, budget, **kw)
     plan(stream)

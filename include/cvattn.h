@@ -366,12 +366,14 @@ cvattn_status cvattn_flash(cvattn_context* ctx, void* stream, const cvattn_flash
  * (append them with cvattn_kv_append at positions 0 .. n - 1, their keys rotated
  * by their own positions with cvattn_rope), so a rejected draft leaves no trace
  * in the cache and an accepted one attends exactly as it will once committed.
- * Products are exact in f32 for every cache type, as in cvattn_decode.
+ * Products are exact in f32 for every cache type, as in cvattn_decode, relative
+ * to the largest of 128 neighbouring committed rows: a row whose scale lies 2^r
+ * below that one's keeps 22 - r bits of its own at least.
  *   - A row that sees nothing gives zeros and lse = -inf.
- *   - Drafted rows that a row does not see may hold anything, NaN and infinities
- *     included; one that it sees and that is not finite makes its output not
- *     finite (every element, from a value row on some paths; its lse only from a
- *     key row).  Committed rows are seen by all.
+ *   - Drafted rows that a row does not see may hold anything, NaN, infinities and
+ *     values of any size included; one that it sees and that is not finite makes
+ *     its output not finite (every element, from a value row on some paths; its
+ *     lse only from a key row).  Committed rows are seen by all.
  *   - Rows from n_nodes[s] up to max_nodes are written as such rows too.
  *   - A kv_len[s] outside [0, max_kv_len] or n_nodes[s] outside [0, max_nodes]
  *     is recorded in the status word and the sequence gives such rows only.
@@ -420,7 +422,8 @@ cvattn_status cvattn_tree_decode(cvattn_context* ctx, void* stream, const cvattn
  * kv_len[s] + i of cache tensor t, and kv_len_out[s] = kv_len[s] + n_accepted[s].
  * drafts[t] must have the type and heads of caches[t] and other memory.
  * A sequence whose rows do not fit its cache, or with a count or node out of
- * range, is left as it is and recorded in the status word. */
+ * range, is left as it is and recorded in the status word.  kv_len_out shares no
+ * memory with accepted or n_accepted. */
 typedef struct cvattn_tree_commit_params {
     const cvattn_tensor* caches;    /* host array [n_tensors] */
     const cvattn_tensor* drafts;    /* host array [n_tensors] */
