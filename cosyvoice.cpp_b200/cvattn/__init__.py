@@ -368,6 +368,14 @@ def _device_bytes(t, what):
     return t.numel() * t.element_size()
 
 
+def _cache(t: Tensor, what) -> Tensor:
+    """A descriptor whose memory, as far as it is known, kernels can reach."""
+    buf = getattr(t, "_buf", None)
+    if buf is not None and not buf.is_cuda and not buf.is_pinned():
+        raise ValueError(f"{what}: describes pageable memory of the host")
+    return t
+
+
 def _row_ptrs(t, what, n_seq):
     """Address of a table of row-0 addresses, one per sequence."""
     torch = _torch()
@@ -404,13 +412,13 @@ class TreeDecoder:
             p.q_nb_node = p.out_nb_node = Hq * D
         if lse is not None:
             p.lse = _dense(lse, (torch.float32,), "TreeDecoder lse", (n_seq, n, Hq)).data_ptr()
-        p.k, p.v = k, v
+        p.k, p.v = _cache(k, "TreeDecoder k"), _cache(v, "TreeDecoder v")
         p.k_seq_ptrs = _row_ptrs(k_seq_ptrs, "TreeDecoder k_seq_ptrs", n_seq)
         p.v_seq_ptrs = _row_ptrs(v_seq_ptrs, "TreeDecoder v_seq_ptrs", n_seq)
         if k_draft is not None:
-            p.k_draft = k_draft
+            p.k_draft = _cache(k_draft, "TreeDecoder k_draft")
         if v_draft is not None:
-            p.v_draft = v_draft
+            p.v_draft = _cache(v_draft, "TreeDecoder v_draft")
         p.kv_len = kv_len.data_ptr()
         if n_nodes is not None:
             p.n_nodes = _dense(n_nodes, (torch.int32,), "TreeDecoder n_nodes", (n_seq,)).data_ptr()
@@ -465,6 +473,8 @@ class TreeCommitter:
         n_seq, most = _dense(accepted, (torch.int32,), "TreeCommitter accepted").shape
         for t, what in ((n_accepted, "n_accepted"), (kv_len, "kv_len"), (kv_len_out, "kv_len_out")):
             _dense(t, (torch.int32,), f"TreeCommitter {what}", (n_seq,))
+        for t in (*caches, *drafts):
+            _cache(t, "TreeCommitter caches, drafts")
         self.ctx = ctx
         p = TreeCommitParams()
         self._caches, self._drafts = (Tensor * len(caches))(*caches), (Tensor * len(drafts))(*drafts)
@@ -507,7 +517,7 @@ class KVScorer:
                 raise ValueError(f"KVScorer {what}: want a CUDA f32 tensor in the layout of scores")
         p = KVScoresParams()
         p.q, p.q_nb_seq, p.q_nb_node = q.data_ptr(), q.stride(0), Hq * D if n == 1 else q.stride(1)
-        p.lse, p.k, p.k_seq_ptrs = lse.data_ptr(), k, _row_ptrs(k_seq_ptrs, "KVScorer k_seq_ptrs", n_seq)
+        p.lse, p.k, p.k_seq_ptrs = lse.data_ptr(), _cache(k, "KVScorer k"), _row_ptrs(k_seq_ptrs, "KVScorer k_seq_ptrs", n_seq)
         p.n_q_rows = p.max_rows = n
         if rows is not None:
             _dense(rows, (torch.int32,), "KVScorer rows")
@@ -552,6 +562,8 @@ class KVEvictor:
         kv_len_out = kv_len if kv_len_out is None else kv_len_out
         if len(k) != len(v) or not k:
             raise ValueError("KVEvictor: as many V as K tensors, one at least")
+        for t in (*k, *v):
+            _cache(t, "KVEvictor k, v")
         if scores.dim() != 4 or scores.shape[0] != len(k) or scores.shape[2] != k[0].n_heads or scores.stride(3) != 1:
             raise ValueError("KVEvictor scores: want [layers, n_seq, Hkv, slots]")
         for t, dtype, what in ((scores, torch.float32, "scores"), (scores_out, torch.float32, "scores_out"),

@@ -79,7 +79,7 @@ def test_one_shot_calls_allocate_on_the_stream_that_they_run_on(monkeypatch, str
 
 
 def tree_arguments(S=2, n=4, L=640):
-    made = {name: cv.kv_tensor(torch.zeros(S * rows * 136, dtype=torch.uint8), cv.Q8_0, 2, D, rows, S)
+    made = {name: cv.kv_tensor(on_device(torch.zeros(S * rows * 136, dtype=torch.uint8)), cv.Q8_0, 2, D, rows, S)
             for name, rows in (("k", L), ("v", L), ("k_draft", n), ("v_draft", n))}
     q = on_device(torch.zeros(S, n, 14, D))
     return {**made, "q": q, "out": on_device(torch.zeros(S, n, 14, D)), "kv_len": on_device(torch.zeros(S, dtype=torch.int32)), "max_kv_len": L,
@@ -87,13 +87,13 @@ def tree_arguments(S=2, n=4, L=640):
 
 
 def scores_arguments(S=2, n=4, L=64):
-    return {"k": cv.kv_tensor(torch.zeros(S * L * 136, dtype=torch.uint8), cv.Q8_0, 2, D, L, S), "q": on_device(torch.zeros(S, n, 14, D)),
+    return {"k": cv.kv_tensor(on_device(torch.zeros(S * L * 136, dtype=torch.uint8)), cv.Q8_0, 2, D, L, S), "q": on_device(torch.zeros(S, n, 14, D)),
             "lse": on_device(torch.zeros(S, n, 14)), "kv_len": on_device(torch.zeros(S, dtype=torch.int32)),
             "scores": on_device(torch.zeros(S, 2, L)), "scores_out": on_device(torch.zeros(S, 2, L))}
 
 
 def evict_arguments(S=2, L=64, budget=32):
-    kv = [[cv.kv_tensor(torch.zeros(S * L * 136, dtype=torch.uint8), cv.Q8_0, 2, D, L, S)] for _ in "kv"]
+    kv = [[cv.kv_tensor(on_device(torch.zeros(S * L * 136, dtype=torch.uint8)), cv.Q8_0, 2, D, L, S)] for _ in "kv"]
     f = lambda: on_device(torch.zeros(1, S, 2, L))  # noqa: E731
     i = lambda: on_device(torch.zeros(1, S, 2, L, dtype=torch.int32))  # noqa: E731
     n = lambda: on_device(torch.zeros(S, dtype=torch.int32))  # noqa: E731
@@ -144,7 +144,7 @@ def test_a_workspace_counts_its_bytes():
 
 
 def commit_arguments(S=2, n=4, L=64):
-    of = lambda rows: [cv.kv_tensor(torch.zeros(S * rows * 136, dtype=torch.uint8), cv.Q8_0, 2, D, rows, S) for _ in "kv"]  # noqa: E731
+    of = lambda rows: [cv.kv_tensor(on_device(torch.zeros(S * rows * 136, dtype=torch.uint8)), cv.Q8_0, 2, D, rows, S) for _ in "kv"]  # noqa: E731
     ints = lambda *s: on_device(torch.zeros(s, dtype=torch.int32))  # noqa: E731
     return {"caches": of(L), "drafts": of(n), "accepted": ints(S, n), "n_accepted": ints(S), "kv_len": ints(S), "kv_len_out": ints(S)}
 
@@ -179,3 +179,17 @@ def test_queries_have_the_head_size_of_the_cache(cls, arguments, heads, head_dim
     given |= {"q": q, "out": q.clone()} if cls is cv.TreeDecoder else {"q": q, "lse": on_device(torch.zeros(2, 4, heads))}
     with pytest.raises(ValueError):
         cls(None, **given)
+
+
+@pytest.mark.parametrize("cls,arguments", [*LAUNCHERS, (cv.TreeCommitter, commit_arguments)], ids=lambda x: getattr(x, "__name__", None))
+def test_descriptors_of_host_memory_are_refused(cls, arguments):
+    given = arguments()
+    cls(None, **given)
+    host = cv.kv_tensor(torch.zeros(2 * 640 * 136, dtype=torch.uint8), cv.Q8_0, 2, D, 64, 2)
+    seen = 0
+    for name, x in given.items():
+        if isinstance(x, cv.Tensor) or (isinstance(x, list) and isinstance(x[0], cv.Tensor)):
+            seen += 1
+            with pytest.raises(ValueError):
+                cls(None, **{**given, name: [host, *x[1:]] if isinstance(x, list) else host})
+    assert seen >= 1
