@@ -19,22 +19,22 @@ TYPES = ["q8_0", "q5_1", "q5_0", "q4_1", "q4_0", "f16"]
 def with_far_rows(rows, torch, at, half):
     """The same rows with the scale of every block (every value of f16) of node at[s] replaced by the f16 of these bits."""
     raw = rows.raw().copy()
-    step = 2 if rows.t == 1 else rows.rb // 4
+    step = 2 if rows.t == 1 else rows.rb // (2 * rows.heads)
     for s, j in enumerate(at):
         for b in range(0, rows.rb, step):
             raw[s, j, b:b + 2] = half
     rows.buf.copy_(torch.tensor(raw.reshape(-1), device="cuda"))
 
 
-def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0, broken=False):
+def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0, broken=False, Hq=14, Hkv=2, sign=1.0):
     rng = np.random.default_rng(seed)
     S, cap = len(lens), max(max(lens), 1)
     kt, vt = cv.TYPE_BY_NAME[kname], cv.TYPE_BY_NAME[vname]
-    mk = lambda t, m: Rows(cv, torch, oracle, t, (rng.standard_normal((S, m, 128)) * size).astype(np.float32), 2)  # noqa: E731
+    mk = lambda t, m: Rows(cv, torch, oracle, t, (rng.standard_normal((S, m, Hkv * D)) * size).astype(np.float32), Hkv)  # noqa: E731
     k, v, kd, vd = mk(kt, cap), mk(vt, cap), mk(kt, n), mk(vt, n)
     sees = ancestors(random_parents(rng, S, n))
-    q = rng.standard_normal((S, n, 14, D)).astype(np.float32)
-    scale = 0.125 / size
+    q = rng.standard_normal((S, n, Hq, D)).astype(np.float32)
+    scale = sign * 0.125 / size
     want, want_lse = reference(q, k.f, v.f, kd.f, vd.f, lens, [n] * S, sees, scale)
     at = [rng.integers(1, n, S), rng.integers(1, n, S)]
     with_far_rows(kd, torch, at[0], half)
@@ -49,7 +49,7 @@ def run_far(ctx, cv, torch, oracle, kname, vname, lens, n, size, half, seed=0, b
             hit[s] |= sees[s, :, j[s]]
         for j in at[2:]:
             blown[s] |= sees[s, :, j[s]]
-    lse = torch.empty((S, n, 14), device="cuda")
+    lse = torch.empty((S, n, Hq), device="cuda")
     out = cv.tree_decode(ctx, torch.tensor(q, device="cuda"), k.desc, v.desc, kd.desc, vd.desc,
                          torch.tensor(lens, dtype=torch.int32, device="cuda"), cap, mask=torch.tensor(pack(sees), device="cuda"), lse=lse,
                          scale=scale).cpu().numpy()
@@ -83,6 +83,19 @@ def test_far_drafts_of_other_sizes(ctx, cv, cuda, oracle, kname, vname, lens, n,
 def test_far_drafts_on_the_persistent_kernel(ctx, cv, cuda, oracle, kname, vname, half):
     """More than 128 rows of a KV head; the second sequence has drafts alone, in two tiles."""
     run_far(ctx, cv, cuda, oracle, kname, vname, [60, 0], 140, 1.0, half)
+
+
+@pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("q5_1", "q8_0"), ("f16", "q5_0")])
+@pytest.mark.parametrize("Hq,Hkv,n", [(16, 16, 140), (3, 1, 70), (16, 2, 30), (6, 2, 5)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_far_drafts_head_layouts(ctx, cv, cuda, oracle, kname, vname, Hq, Hkv, n, sign):
+    run_far(ctx, cv, cuda, oracle, kname, vname, [130, 0], n, 1.0, LARGE, seed=n, Hq=Hq, Hkv=Hkv, sign=sign)
+
+
+@pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("q4_1", "f16")])
+def test_far_drafts_after_long_contexts(ctx, cv, cuda, oracle, kname, vname):
+    """Parts of a sequence on many CTAs, the drafts on one of them."""
+    run_far(ctx, cv, cuda, oracle, kname, vname, [9001, 300, 128], 20, 1.0, LARGE)
 
 
 @pytest.mark.parametrize("kname,vname", [("q8_0", "q4_0"), ("q5_1", "q5_0"), ("f16", "q8_0"), ("q4_1", "f16"), ("f16", "f16")])
