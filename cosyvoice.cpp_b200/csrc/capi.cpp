@@ -3,7 +3,7 @@
 // Argument validation, the per-worker context (device status word), type
 // negotiation, host<->device KV copies, the cvattn_kv_cache host object and
 // the DiT step planner.  Kernels live in kv_append.cu, decode*.cu, flash_tc.cu,
-// tree_decode.cu, kv_scores.cu and kv_evict.cu; nothing here computes attention on the CPU.
+// tree_decode.cu, kv_scores.cu, kv_evict.cu, paged_*.cu, pages.cu and verify.cu; nothing here computes attention on the CPU.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -137,6 +137,13 @@ size_t cvattn_abi_sizeof(int32_t which) {
     case 7: return sizeof(cvattn_tree_commit_params);
     case 8: return sizeof(cvattn_kv_scores_params);
     case 9: return sizeof(cvattn_kv_evict_params);
+    case 10: return sizeof(cvattn_page_pool);
+    case 11: return sizeof(cvattn_paged_append_params);
+    case 12: return sizeof(cvattn_paged_read_params);
+    case 13: return sizeof(cvattn_paged_attention_params);
+    case 14: return sizeof(cvattn_pages_assign_params);
+    case 15: return sizeof(cvattn_pages_compact_params);
+    case 16: return sizeof(cvattn_verify_params);
     default: return 0;
     }
 }
@@ -640,6 +647,200 @@ cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv
     if (dg.error() != cudaSuccess) return from_cuda(dg.error());
     return from_cuda(launch_kv_evict(as_stream(stream), *p, type_row_bytes(k.type, k.head_dim), type_row_bytes(v.type, v.head_dim),
                                      ctx->status));
+}
+
+// ------------------------------------------------- paged cache, verification
+
+static bool mult4(int64_t a) { return (a & 3) == 0; }
+static bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Whether a pool's description is usable; one of another head size is not supported.
+static cvattn_status pool_ok(const cvattn_page_pool& q) {
+    if (!q.k || !q.v || !q.k_scale || !q.v_scale || q.reserved || q.n_heads <= 0 || q.n_pages <= 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (q.format != CVATTN_PAGE_I8 && q.format != CVATTN_PAGE_E4M3) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (q.page_size != 16 && q.page_size != 32 && q.page_size != 64 && q.page_size != 128) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (!aligned(q.k, 16) || !aligned(q.v, 16) || !aligned(q.k_scale, 4) || !aligned(q.v_scale, 4) || (q.nb_page & 15))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (q.head_dim != 64 || q.n_heads > 1024) return CVATTN_ERR_UNSUPPORTED;
+    const int64_t page = (int64_t)q.n_heads * q.page_size * q.head_dim, scales = (int64_t)q.n_heads * q.page_size / CVATTN_PAGE_BLOCK;
+    if (q.n_pages > 1 && (q.nb_page < page || q.nb_scale < scales)) return CVATTN_ERR_INVALID_ARGUMENT;
+    return CVATTN_OK;
+}
+
+static bool table_ok(const int32_t* table, int64_t nb_seq, int32_t width, int32_t n_seq, int32_t page_size) {
+    return table && aligned(table, 4) && width > 0 && (n_seq <= 1 || nb_seq >= width) && (int64_t)width * page_size <= INT32_MAX;
+}
+
+// Rows of a paged append or read: f32, dense heads.
+static bool rows_ok(const float* k, const float* v, int64_t nb_row, int64_t nb_seq, int32_t rows, int32_t n_seq, int32_t n_heads) {
+    return k && v && aligned(k, 16) && aligned(v, 16) && mult4(nb_row) && mult4(nb_seq) &&
+           (rows <= 1 || nb_row >= (int64_t)n_heads * 64) && (n_seq <= 1 || nb_seq >= 0);
+}
+
+cvattn_status cvattn_paged_append(cvattn_context* ctx, void* stream, const cvattn_paged_append_params* p) {
+    if (!ctx || !p || p->n_seq < 0 || p->max_new < 0 || p->reserved) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0 || p->max_new == 0) return CVATTN_OK;
+    const cvattn_status ok = pool_ok(p->pool);
+    if (ok != CVATTN_OK) return ok;
+    if (!p->kv_len || !table_ok(p->table, p->table_nb_seq, p->table_width, p->n_seq, p->pool.page_size) ||
+        !rows_ok(p->k, p->v, p->nb_row, p->nb_seq, p->max_new, p->n_seq, p->pool.n_heads))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq > kMaxGridSeq) return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_new > (int64_t)p->table_width * p->pool.page_size) return CVATTN_ERR_LENGTH;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_paged_append(as_stream(stream), *p, ctx->status));
+}
+
+cvattn_status cvattn_paged_read(cvattn_context* ctx, void* stream, const cvattn_paged_read_params* p) {
+    if (!ctx || !p || p->n_seq < 0 || p->max_rows < 0 || p->reserved) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0 || p->max_rows == 0) return CVATTN_OK;
+    const cvattn_status ok = pool_ok(p->pool);
+    if (ok != CVATTN_OK) return ok;
+    if (!table_ok(p->table, p->table_nb_seq, p->table_width, p->n_seq, p->pool.page_size) ||
+        !rows_ok(p->k, p->v, p->nb_row, p->nb_seq, p->max_rows, p->n_seq, p->pool.n_heads))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const int64_t row = (int64_t)p->pool.n_heads * 64;  // sequences may not share rows that are written
+    if (p->n_seq > 1 && p->nb_seq < (p->max_rows - 1) * p->nb_row + row) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq > kMaxGridSeq) return CVATTN_ERR_UNSUPPORTED;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_paged_read(as_stream(stream), *p, ctx->status));
+}
+
+size_t cvattn_paged_attention_workspace_size(int32_t n_seq, int32_t max_q, int32_t max_kv_len, int32_t n_q_heads, int32_t n_kv_heads) {
+    if (n_seq <= 0 || max_q <= 0 || max_kv_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads ||
+        n_q_heads / n_kv_heads > 8)
+        return 0;
+    return paged_attention_workspace_bytes(n_seq, max_q, max_kv_len, n_q_heads, n_kv_heads);
+}
+
+cvattn_status cvattn_paged_attention(cvattn_context* ctx, void* stream, const cvattn_paged_attention_params* p) {
+    if (!ctx || !p || p->n_seq < 0 || p->max_q < 0 || p->max_kv_len < 0 || p->n_q_heads <= 0 || p->flags || p->reserved)
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0 || p->max_q == 0) return CVATTN_OK;
+    const cvattn_status ok = pool_ok(p->pool);
+    if (ok != CVATTN_OK) return ok;
+    if (!p->q || !p->out || !p->kv_len || !table_ok(p->table, p->table_nb_seq, p->table_width, p->n_seq, p->pool.page_size))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_q_heads % p->pool.n_heads || p->n_q_heads / p->pool.n_heads > 8 || p->n_seq > kMaxGridSeq || p->max_q > (1 << 20))
+        return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_kv_len > (int64_t)p->table_width * p->pool.page_size) return CVATTN_ERR_LENGTH;
+    const int64_t row = (int64_t)p->n_q_heads * p->pool.head_dim;
+    if (!aligned(p->q, 16) || !aligned(p->out, 16) || !mult4(p->q_nb_tok) || !mult4(p->q_nb_seq) || !mult4(p->out_nb_tok) ||
+        !mult4(p->out_nb_seq) || (p->max_q > 1 && (p->q_nb_tok < row || p->out_nb_tok < row)))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    // sequences may share queries (stride 0) but not outputs
+    const int64_t all = (p->max_q - 1) * p->out_nb_tok + row;
+    if (p->n_seq > 1 && (p->q_nb_seq < 0 || p->out_nb_seq < row)) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq > 1 && p->out_nb_seq < all && p->out_nb_tok < (p->n_seq - 1) * p->out_nb_seq + row) return CVATTN_ERR_INVALID_ARGUMENT;
+    const size_t need = paged_attention_workspace_bytes(p->n_seq, p->max_q, p->max_kv_len, p->n_q_heads, p->pool.n_heads);
+    if (need && (!p->workspace || p->workspace_size < need || !aligned(p->workspace, 16))) return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_paged_attention(as_stream(stream), *p, ctx->status));
+}
+
+// Pools that one table indexes; the copied pages of two pools may not touch.
+static cvattn_status pools_ok(const cvattn_page_pool* pools, int32_t n) {
+    if (!pools || n <= 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    for (int32_t i = 0; i < n; ++i) {
+        const cvattn_status ok = pool_ok(pools[i]);
+        if (ok != CVATTN_OK) return ok;
+        if (pools[i].page_size != pools[0].page_size || pools[i].n_pages != pools[0].n_pages) return CVATTN_ERR_INVALID_ARGUMENT;
+    }
+    return CVATTN_OK;
+}
+
+// A table that is read and one that is written: the same, or apart.
+static bool tables_ok(const int32_t* in, const int32_t* out, int64_t nb_seq, int32_t width, int32_t n_seq, int32_t page_size) {
+    if (!table_ok(in, nb_seq, width, n_seq, page_size) || !table_ok(out, nb_seq, width, n_seq, page_size)) return false;
+    if ((int64_t)n_seq * width > INT32_MAX) return false;
+    const int64_t span = 4 * ((n_seq - 1) * nb_seq + width);
+    return in == out || !overlap(in, span, out, span);
+}
+
+size_t cvattn_pages_workspace_size(int32_t n_seq, int32_t table_width, int32_t n_pages) {
+    if (n_seq <= 0 || table_width <= 0 || n_pages <= 0) return 0;
+    return pages_workspace_bytes(n_seq, table_width, n_pages);
+}
+
+cvattn_status cvattn_pages_assign(cvattn_context* ctx, void* stream, const cvattn_pages_assign_params* p) {
+    if (!ctx || !p || p->n_seq < 0 || p->reserved) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0) return CVATTN_OK;
+    const cvattn_status ok = pools_ok(p->pools, p->n_pools);
+    if (ok != CVATTN_OK) return ok;
+    const cvattn_page_pool& q = p->pools[0];
+    if (!p->keep || !p->need || !p->room || !tables_ok(p->table, p->table_out, p->table_nb_seq, p->table_width, p->n_seq, q.page_size))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const int64_t per_seq = 4 * (int64_t)p->n_seq, span = 4 * ((p->n_seq - 1) * p->table_nb_seq + p->table_width);
+    const void* in[] = {p->src, p->keep, p->need};
+    const struct { const void* at; int64_t bytes; } out[] = {{p->room, per_seq}, {p->refs, 4 * (int64_t)q.n_pages}, {p->table_out, span}};
+    for (const auto& o : out) {
+        for (const void* i : in)
+            if (i && o.at && overlap(i, per_seq, o.at, o.bytes)) return CVATTN_ERR_INVALID_ARGUMENT;
+        if (o.at && o.at != p->table_out && overlap(p->table, span, o.at, o.bytes)) return CVATTN_ERR_INVALID_ARGUMENT;
+    }
+    const size_t need = pages_workspace_bytes(p->n_seq, p->table_width, q.n_pages);
+    if (!p->workspace || p->workspace_size < need || !aligned(p->workspace, 16)) return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_pages_assign(as_stream(stream), *p, q.page_size, q.n_pages, ctx->status));
+}
+
+cvattn_status cvattn_pages_compact(cvattn_context* ctx, void* stream, const cvattn_pages_compact_params* p) {
+    if (!ctx || !p || p->n_seq < 0 || p->reserved) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0) return CVATTN_OK;
+    const cvattn_status ok = pools_ok(p->pools, p->n_pools);
+    if (ok != CVATTN_OK) return ok;
+    const cvattn_page_pool& q = p->pools[0];
+    if (!p->n_live || !tables_ok(p->table, p->table_out, p->table_nb_seq, p->table_width, p->n_seq, q.page_size))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const int64_t span = 4 * ((p->n_seq - 1) * p->table_nb_seq + p->table_width);
+    if (overlap(p->n_live, 4, p->table, span) || overlap(p->n_live, 4, p->table_out, span)) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->refs && (overlap(p->refs, 4 * (int64_t)q.n_pages, p->table, span) || overlap(p->refs, 4 * (int64_t)q.n_pages, p->table_out, span) ||
+                    overlap(p->refs, 4 * (int64_t)q.n_pages, p->n_live, 4)))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const size_t need = pages_workspace_bytes(p->n_seq, p->table_width, q.n_pages);
+    if (!p->workspace || p->workspace_size < need || !aligned(p->workspace, 16)) return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_pages_compact(as_stream(stream), *p, q.n_pages, ctx->status));
+}
+
+size_t cvattn_verify_workspace_size(int32_t n_seq, int32_t max_nodes, int32_t vocab) {
+    if (n_seq <= 0 || max_nodes <= 0 || vocab <= 0) return 0;
+    return verify_workspace_bytes(n_seq, max_nodes, vocab);
+}
+
+cvattn_status cvattn_verify_drafts(cvattn_context* ctx, void* stream, const cvattn_verify_params* p) {
+    if (!ctx || !p || p->n_seq < 0 || p->max_nodes < 0 || p->vocab <= 0) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq == 0 || p->max_nodes == 0) return CVATTN_OK;
+    if (!p->logits || !p->tokens || !p->accept_u || !p->sample_u || !p->accepted || !p->n_accepted || !p->next_token)
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    const int t = p->logits_type;
+    if (t != CVATTN_TYPE_F32 && t != CVATTN_TYPE_F16 && t != CVATTN_TYPE_BF16) return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_nodes > CVATTN_TREE_MAX_NODES || p->n_seq > kMaxGridSeq) return CVATTN_ERR_UNSUPPORTED;
+    if (!aligned(p->logits, t == CVATTN_TYPE_F32 ? 4 : 2) || (p->max_nodes > 1 && p->logits_nb_node < p->vocab) ||
+        (p->n_seq > 1 && p->logits_nb_seq < 0))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->draft_probs && (!aligned(p->draft_probs, 4) || (p->max_nodes > 1 && p->probs_nb_node < p->vocab) ||
+                           (p->n_seq > 1 && p->probs_nb_seq < 0)))
+        return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->parents && p->parents_nb_seq && p->parents_nb_seq < p->max_nodes) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (p->n_seq > 1 && p->accepted_stride < p->max_nodes) return CVATTN_ERR_INVALID_ARGUMENT;
+    const int64_t n = p->n_seq, all = 4 * n * p->max_nodes, some = 4 * ((n - 1) * p->accepted_stride + p->max_nodes);
+    const struct { const void* at; int64_t bytes; } out[] = {{p->accepted, some}, {p->n_accepted, 4 * n}, {p->next_token, 4 * n}, {p->log_probs, all}},
+        in[] = {{p->tokens, all}, {p->parents, 4 * ((n - 1) * p->parents_nb_seq + p->max_nodes)}, {p->n_nodes, 4 * n},
+                {p->accept_u, all}, {p->sample_u, 4 * n}, {p->temperature, 4 * n}};
+    for (const auto& o : out)
+        for (const auto& i : in)
+            if (o.at && i.at && overlap(o.at, o.bytes, i.at, i.bytes)) return CVATTN_ERR_INVALID_ARGUMENT;
+    const size_t need = verify_workspace_bytes(p->n_seq, p->max_nodes, p->vocab);
+    if (need && (!p->workspace || p->workspace_size < need || !aligned(p->workspace, 16))) return CVATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard dg(ctx->device);
+    if (dg.error() != cudaSuccess) return from_cuda(dg.error());
+    return from_cuda(launch_verify(as_stream(stream), *p, ctx->status));
 }
 
 // ------------------------------------------------------------ copies

@@ -56,6 +56,9 @@ enum : int {
     kStatusBadPosition = 1,   // append position outside [0, capacity)
     kStatusBadLength = 2,     // kv_len outside [0, capacity] or above max_kv_len
     kStatusTimeout = 3,       // bounded mbarrier wait gave up
+    kStatusBadPage = 4,       // table entry outside the pool
+    kStatusSharedPage = 5,    // append into a page that other entries hold
+    kStatusBadDraft = 6,      // drafted node, token or temperature out of range
 };
 
 __device__ __forceinline__ void record_status(int* status, int code) {

@@ -67,4 +67,21 @@ cudaError_t launch_kv_evict(cudaStream_t stream, const cvattn_kv_evict_params& p
 cudaError_t launch_tree_commit(cudaStream_t stream, const cvattn_tree_commit_params& p, int64_t capacity,
                                int64_t draft_rows, int* status);
 
+// paged_append.cu
+cudaError_t launch_paged_append(cudaStream_t stream, const cvattn_paged_append_params& p, int* status);
+cudaError_t launch_paged_read(cudaStream_t stream, const cvattn_paged_read_params& p, int* status);
+
+// paged_attention.cu
+size_t paged_attention_workspace_bytes(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads);
+cudaError_t launch_paged_attention(cudaStream_t stream, const cvattn_paged_attention_params& p, int* status);
+
+// pages.cu
+size_t pages_workspace_bytes(int n_seq, int table_width, int n_pages);
+cudaError_t launch_pages_assign(cudaStream_t stream, const cvattn_pages_assign_params& p, int page_size, int n_pages, int* status);
+cudaError_t launch_pages_compact(cudaStream_t stream, const cvattn_pages_compact_params& p, int n_pages, int* status);
+
+// verify.cu
+size_t verify_workspace_bytes(int n_seq, int max_nodes, int vocab);
+cudaError_t launch_verify(cudaStream_t stream, const cvattn_verify_params& p, int* status);
+
 }  // namespace cvattn

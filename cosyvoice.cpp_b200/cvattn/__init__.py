@@ -694,3 +694,8 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+
+from .paged import (PAGE_BLOCK, PAGE_E4M3, PAGE_I8, PAGE_SIZES, DraftVerifier, PageAppender, PageAssigner,  # noqa: E402
+                    PageCompactor, PagedAttention, PagePool, PageReader, alloc_pages, paged_attention,
+                    paged_attention_workspace_size)

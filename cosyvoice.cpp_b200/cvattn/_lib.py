@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libcvattn.so")
 ABI_VERSION = 2
 MAX_CHUNK_BOUNDS = 64
 TREE_MAX_NODES = 256
+PAGE_BLOCK = 16
 
 c_void_p, c_int32, c_int64, c_uint32, c_float, c_size_t, c_uint8 = (
     ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_float, ctypes.c_size_t, ctypes.c_uint8)
@@ -113,8 +114,72 @@ class KVEvictParams(ctypes.Structure):
     ]
 
 
+class PagePoolDesc(ctypes.Structure):
+    """cvattn_page_pool: one layer's keys and values in pages of 8-bit codes."""
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("nb_page", c_int64),
+        ("nb_scale", c_int64), ("format", c_int32), ("n_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32),
+        ("n_pages", c_int32), ("reserved", c_int32),
+    ]
+
+
+class PagedAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("pool", PagePoolDesc), ("k", c_void_p), ("v", c_void_p), ("nb_row", c_int64), ("nb_seq", c_int64),
+        ("table", c_void_p), ("table_nb_seq", c_int64), ("table_width", c_int32), ("n_seq", c_int32), ("kv_len", c_void_p),
+        ("n_new", c_void_p), ("refs", c_void_p), ("max_new", c_int32), ("reserved", c_int32),
+    ]
+
+
+class PagedReadParams(ctypes.Structure):
+    _fields_ = [
+        ("pool", PagePoolDesc), ("k", c_void_p), ("v", c_void_p), ("nb_row", c_int64), ("nb_seq", c_int64),
+        ("table", c_void_p), ("table_nb_seq", c_int64), ("table_width", c_int32), ("n_seq", c_int32), ("first", c_void_p),
+        ("n_rows", c_void_p), ("max_rows", c_int32), ("reserved", c_int32),
+    ]
+
+
+class PagedAttentionParams(ctypes.Structure):
+    _fields_ = [
+        ("pool", PagePoolDesc), ("q", c_void_p), ("q_nb_tok", c_int64), ("q_nb_seq", c_int64), ("out", c_void_p),
+        ("out_nb_tok", c_int64), ("out_nb_seq", c_int64), ("lse", c_void_p), ("table", c_void_p), ("table_nb_seq", c_int64),
+        ("kv_len", c_void_p), ("n_q", c_void_p), ("n_seq", c_int32), ("max_q", c_int32), ("n_q_heads", c_int32),
+        ("max_kv_len", c_int32), ("table_width", c_int32), ("scale", c_float), ("flags", c_int32), ("reserved", c_int32),
+        ("workspace", c_void_p), ("workspace_size", c_size_t),
+    ]
+
+
+class PagesAssignParams(ctypes.Structure):
+    _fields_ = [
+        ("pools", ctypes.POINTER(PagePoolDesc)), ("n_pools", c_int32), ("n_seq", c_int32), ("table", c_void_p),
+        ("table_out", c_void_p), ("table_nb_seq", c_int64), ("table_width", c_int32), ("reserved", c_int32),
+        ("src", c_void_p), ("keep", c_void_p), ("need", c_void_p), ("room", c_void_p), ("refs", c_void_p),
+        ("workspace", c_void_p), ("workspace_size", c_size_t),
+    ]
+
+
+class PagesCompactParams(ctypes.Structure):
+    _fields_ = [
+        ("pools", ctypes.POINTER(PagePoolDesc)), ("n_pools", c_int32), ("n_seq", c_int32), ("table", c_void_p),
+        ("table_out", c_void_p), ("table_nb_seq", c_int64), ("table_width", c_int32), ("reserved", c_int32),
+        ("n_live", c_void_p), ("refs", c_void_p), ("workspace", c_void_p), ("workspace_size", c_size_t),
+    ]
+
+
+class VerifyParams(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("logits_nb_node", c_int64), ("logits_nb_seq", c_int64), ("draft_probs", c_void_p),
+        ("probs_nb_node", c_int64), ("probs_nb_seq", c_int64), ("tokens", c_void_p), ("parents", c_void_p),
+        ("parents_nb_seq", c_int64), ("n_nodes", c_void_p), ("accept_u", c_void_p), ("sample_u", c_void_p),
+        ("temperature", c_void_p), ("accepted", c_void_p), ("accepted_stride", c_int64), ("n_accepted", c_void_p),
+        ("next_token", c_void_p), ("log_probs", c_void_p), ("logits_type", c_int32), ("n_seq", c_int32),
+        ("max_nodes", c_int32), ("vocab", c_int32), ("workspace", c_void_p), ("workspace_size", c_size_t),
+    ]
+
+
 STRUCTS = {0: Tensor, 1: DecodeParams, 2: FlashParams, 3: KVCacheParams, 4: DitStep, 5: RopeParams, 6: TreeParams,
-           7: TreeCommitParams, 8: KVScoresParams, 9: KVEvictParams}
+           7: TreeCommitParams, 8: KVScoresParams, 9: KVEvictParams, 10: PagePoolDesc, 11: PagedAppendParams, 12: PagedReadParams,
+           13: PagedAttentionParams, 14: PagesAssignParams, 15: PagesCompactParams, 16: VerifyParams}
 
 # (name, restype, argtypes) for every symbol include/cvattn.h declares.
 P = ctypes.POINTER
@@ -152,6 +217,15 @@ SIGNATURES = [
     ("cvattn_kv_scores", c_int32, [c_void_p, c_void_p, P(KVScoresParams)]),
     ("cvattn_kv_evict_workspace_size", c_size_t, [c_int32] * 5),
     ("cvattn_kv_evict", c_int32, [c_void_p, c_void_p, P(KVEvictParams)]),
+    ("cvattn_paged_append", c_int32, [c_void_p, c_void_p, P(PagedAppendParams)]),
+    ("cvattn_paged_read", c_int32, [c_void_p, c_void_p, P(PagedReadParams)]),
+    ("cvattn_paged_attention_workspace_size", c_size_t, [c_int32] * 5),
+    ("cvattn_paged_attention", c_int32, [c_void_p, c_void_p, P(PagedAttentionParams)]),
+    ("cvattn_pages_workspace_size", c_size_t, [c_int32] * 3),
+    ("cvattn_pages_assign", c_int32, [c_void_p, c_void_p, P(PagesAssignParams)]),
+    ("cvattn_pages_compact", c_int32, [c_void_p, c_void_p, P(PagesCompactParams)]),
+    ("cvattn_verify_workspace_size", c_size_t, [c_int32] * 3),
+    ("cvattn_verify_drafts", c_int32, [c_void_p, c_void_p, P(VerifyParams)]),
     ("cvattn_kv_copy_to_host", c_int32, [c_void_p, P(Tensor), c_int32, c_void_p]),
     ("cvattn_kv_copy_from_host", c_int32, [c_void_p, P(Tensor), c_int32, c_void_p]),
     ("cvattn_kv_cache_create", c_int32, [c_void_p, P(KVCacheParams), P(c_void_p)]),

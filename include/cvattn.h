@@ -56,7 +56,11 @@ int32_t cvattn_status_to_ggml(cvattn_status s);
  * which: 0 cvattn_tensor, 1 cvattn_decode_params, 2 cvattn_flash_params,
  *        3 cvattn_kv_cache_params, 4 cvattn_dit_step, 5 cvattn_rope_params,
  *        6 cvattn_tree_params, 7 cvattn_tree_commit_params,
- *        8 cvattn_kv_scores_params, 9 cvattn_kv_evict_params. */
+ *        8 cvattn_kv_scores_params, 9 cvattn_kv_evict_params,
+ *        10 cvattn_page_pool, 11 cvattn_paged_append_params,
+ *        12 cvattn_paged_read_params, 13 cvattn_paged_attention_params,
+ *        14 cvattn_pages_assign_params, 15 cvattn_pages_compact_params,
+ *        16 cvattn_verify_params. */
 int32_t cvattn_abi_version(void);
 size_t cvattn_abi_sizeof(int32_t which);
 
@@ -64,7 +68,8 @@ size_t cvattn_abi_sizeof(int32_t which);
 
 enum {
     CVATTN_TYPE_F32 = 0, CVATTN_TYPE_F16 = 1, CVATTN_TYPE_Q4_0 = 2, CVATTN_TYPE_Q4_1 = 3,
-    CVATTN_TYPE_Q5_0 = 6, CVATTN_TYPE_Q5_1 = 7, CVATTN_TYPE_Q8_0 = 8
+    CVATTN_TYPE_Q5_0 = 6, CVATTN_TYPE_Q5_1 = 7, CVATTN_TYPE_Q8_0 = 8,
+    CVATTN_TYPE_BF16 = 30  /* logits only (cvattn_verify_drafts) */
 };
 
 /* A ggml KV tensor (or an uncached K/V activation in the same row layout). */
@@ -524,6 +529,255 @@ size_t cvattn_kv_evict_workspace_size(int32_t n_layers, int32_t n_seq, int32_t n
                                       int32_t budget);
 
 cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv_evict_params* p);
+
+/* ----------------------------------------------- a paged cache in 8 bits */
+
+/* A cache in pages (no counterpart in the reference, whose caches are one
+ * contiguous tensor per worker): utterances that share a voice prompt share its
+ * pages, candidates fork from one another, rejected drafts are given back.
+ * One layer's keys and values are two arrays of n_pages pages of page_size
+ * positions (16, 32, 64 or 128).  Page p, head h, block b of 16 positions x 64
+ * values is 1024 codes at  data + p*nb_page + (h*page_size/16 + b)*1024  with one
+ * scale at  scale + p*nb_scale + h*page_size/16 + b :  value = code value x scale.
+ *   CVATTN_PAGE_I8    code value = byte - 128, in -127 .. 127
+ *   CVATTN_PAGE_E4M3  the byte as an OCP e4m3 number
+ * The byte of position t, value d of a block is at
+ *   keys    t*64 + d
+ *   values  d/32*512 + (d%8*4 + t/4)*16 + d/8%4*4 + t%4
+ * (in the order in which the tensor cores take them).  A table lists, for each
+ * sequence, the page of its positions 0 .. page_size - 1, then the next, ..;
+ * every layer's pool is indexed by the same table.  Entries outside
+ * [0, n_pages) hold nothing. */
+enum { CVATTN_PAGE_I8 = 0, CVATTN_PAGE_E4M3 = 1 };
+#define CVATTN_PAGE_BLOCK 16
+
+typedef struct cvattn_page_pool {
+    void*   k;          /* device; 16-byte aligned */
+    void*   v;
+    float*  k_scale;    /* device */
+    float*  v_scale;
+    int64_t nb_page;    /* bytes between pages of k and v: a multiple of 16 */
+    int64_t nb_scale;   /* floats between pages of the scales */
+    int32_t format;     /* CVATTN_PAGE_* */
+    int32_t n_heads;
+    int32_t head_dim;   /* 64 */
+    int32_t page_size;
+    int32_t n_pages;
+    int32_t reserved;   /* 0 */
+} cvattn_page_pool;
+
+/* Append rows: row i < n_new[s] of sequence s to position kv_len[s] + i, rounded
+ * into its block.  A block's scale is the larger of what it has (0 if it held no
+ * position of this sequence, or if that is no positive number) and max |x| / 127 (/ 448 for e4m3) over the finite
+ * new values, as f32 (no scale that is not a normal number: the values count as 0);
+ * codes are the nearest values, ties to even, of x / scale; rows that the block
+ * held are rounded anew when the scale grows.  A NaN is stored as 0, an infinity
+ * as the block's largest.  Other rows of the block are left as they are.
+ * A sequence whose rows do not fit its table is recorded in the status word and
+ * skipped, and so is a block whose page is out of range or, with refs, held by
+ * more than one table entry.  k, v rotated beforehand (cvattn_rope). */
+typedef struct cvattn_paged_append_params {
+    cvattn_page_pool pool;
+    const float*    k;              /* device f32: row i of sequence s, n_heads*64 values, */
+    const float*    v;              /* at + s*nb_seq + i*nb_row (floats, multiples of 4)   */
+    int64_t         nb_row;
+    int64_t         nb_seq;
+    const int32_t*  table;          /* device: entry j of sequence s at s*table_nb_seq + j */
+    int64_t         table_nb_seq;
+    int32_t         table_width;    /* entries per sequence */
+    int32_t         n_seq;
+    const int32_t*  kv_len;         /* device [n_seq]: positions before the new ones */
+    const int32_t*  n_new;          /* optional device [n_seq]; NULL: max_new each */
+    const int32_t*  refs;           /* optional device [n_pages] (cvattn_pages_assign) */
+    int32_t         max_new;
+    int32_t         reserved;       /* 0 */
+} cvattn_paged_append_params;
+
+cvattn_status cvattn_paged_append(cvattn_context* ctx, void* stream, const cvattn_paged_append_params* p);
+
+/* Read rows back: position first[s] + i of sequence s to row i < n_rows[s] of k
+ * and v in f32; rows from there to max_rows, and positions without a page, are
+ * zeros (the latter, or a range outside the table, recorded). */
+typedef struct cvattn_paged_read_params {
+    cvattn_page_pool pool;
+    float*          k;              /* device f32, laid out as in cvattn_paged_append_params */
+    float*          v;
+    int64_t         nb_row;
+    int64_t         nb_seq;
+    const int32_t*  table;
+    int64_t         table_nb_seq;
+    int32_t         table_width;
+    int32_t         n_seq;
+    const int32_t*  first;          /* optional device [n_seq]; NULL: 0 */
+    const int32_t*  n_rows;         /* optional device [n_seq]; NULL: max_rows each */
+    int32_t         max_rows;
+    int32_t         reserved;       /* 0 */
+} cvattn_paged_read_params;
+
+cvattn_status cvattn_paged_read(cvattn_context* ctx, void* stream, const cvattn_paged_read_params* p);
+
+/* Attention of each sequence's last n_q[s] positions over its pages: one token,
+ * a chain of drafts or a piece of a prompt, appended beforehand.  Row i sees the
+ * positions j < kv_len[s] - n_q[s] + i + 1:
+ *   out[s][i][h] = sum_j p_j v_j,  p = softmax_j(scale q.k_j),
+ *   lse[s][i][h] = log(sum_j exp(scale q.k_j))                (natural log).
+ * Products are exact in f32, but for P times the values' scales, whose parts below
+ * 2^-22 of the largest of 128 neighbouring positions are left out.
+ *   - A row that sees nothing, and rows from n_q[s] to max_q: zeros, lse = -inf.
+ *   - What a page holds past kv_len is not looked at.
+ *   - A kv_len outside [0, max_kv_len] or n_q outside [0, max_q] is recorded and
+ *     the sequence gives such rows only; positions whose page is out of range are
+ *     recorded and left out. */
+typedef struct cvattn_paged_attention_params {
+    cvattn_page_pool pool;
+    const float*    q;            /* device f32; element (d, h, i, s) at        */
+    int64_t         q_nb_tok;     /* q + s*q_nb_seq + i*q_nb_tok + h*head_dim + d */
+    int64_t         q_nb_seq;     /* (strides in floats, multiples of 4)        */
+    float*          out;          /* device f32, laid out the same way          */
+    int64_t         out_nb_tok;
+    int64_t         out_nb_seq;
+    float*          lse;          /* optional device f32 [n_seq][max_q][n_q_heads] */
+    const int32_t*  table;
+    int64_t         table_nb_seq;
+    const int32_t*  kv_len;       /* device [n_seq]: positions, the rows' own included */
+    const int32_t*  n_q;          /* optional device [n_seq]; NULL: max_q each */
+    int32_t         n_seq;
+    int32_t         max_q;
+    int32_t         n_q_heads;    /* 1 to 8 per KV head */
+    int32_t         max_kv_len;   /* host bound on kv_len[], at most table_width*page_size */
+    int32_t         table_width;
+    float           scale;
+    int32_t         flags;        /* 0 */
+    int32_t         reserved;     /* 0 */
+    void*           workspace;    /* device scratch of cvattn_paged_attention_workspace_size bytes; */
+    size_t          workspace_size; /* needs no initialization                                      */
+} cvattn_paged_attention_params;
+
+size_t cvattn_paged_attention_workspace_size(int32_t n_seq, int32_t max_q, int32_t max_kv_len, int32_t n_q_heads,
+                                             int32_t n_kv_heads);
+
+cvattn_status cvattn_paged_attention(cvattn_context* ctx, void* stream, const cvattn_paged_attention_params* p);
+
+/* What the tables hold next, in one call: sequence s keeps the first keep[s]
+ * positions of src[s] (itself without src) and gets pages for need[s].  So
+ * keep = 0, need = 0 frees a sequence, keep < length rolls drafts back, several
+ * sequences with one src fork it, and src may permute them.
+ *   - A page is held by the entries that list it, and free when none does: there
+ *     is no other state.  refs (optional output) counts them.
+ *   - A sequence that will write (need > keep) into a partly filled page that
+ *     other entries hold gets a copy of it, in every pool; where only such
+ *     sequences hold the page, the first of them keeps it.
+ *   - Free pages are given in ascending order, sequence by sequence, as long as
+ *     the pages that the sequences up to it ask for are there; room[s] is then
+ *     max(keep, need), else keep.  (A sequence without room may hold a tail page
+ *     that others hold too.)
+ *   - Entries past a sequence's pages become -1, and so do kept ones out of range
+ *     (recorded).  A keep, need or src out of range is recorded and counts as
+ *     keep = need = 0.
+ * table_out may be table, other outputs share no memory with inputs. */
+typedef struct cvattn_pages_assign_params {
+    const cvattn_page_pool* pools;  /* host array [n_pools]: every layer, same page_size and n_pages */
+    int32_t         n_pools;
+    int32_t         n_seq;
+    const int32_t*  table;
+    int32_t*        table_out;
+    int64_t         table_nb_seq;   /* of both tables */
+    int32_t         table_width;
+    int32_t         reserved;       /* 0 */
+    const int32_t*  src;            /* optional device [n_seq] */
+    const int32_t*  keep;           /* device [n_seq] */
+    const int32_t*  need;           /* device [n_seq] */
+    int32_t*        room;           /* device [n_seq] */
+    int32_t*        refs;           /* optional device [n_pages] */
+    void*           workspace;      /* device scratch of cvattn_pages_workspace_size bytes; */
+    size_t          workspace_size; /* needs no initialization                              */
+} cvattn_pages_assign_params;
+
+size_t cvattn_pages_workspace_size(int32_t n_seq, int32_t table_width, int32_t n_pages);
+
+cvattn_status cvattn_pages_assign(cvattn_context* ctx, void* stream, const cvattn_pages_assign_params* p);
+
+/* Move the pages that the tables hold to the front of every pool: with n_live of
+ * them, the i-th held page at or above n_live goes to the i-th free one below it,
+ * both in ascending order, and the tables follow.  Pages from n_live on are then
+ * free.  Every table that lists pages of the pools has to be among the n_seq. */
+typedef struct cvattn_pages_compact_params {
+    const cvattn_page_pool* pools;
+    int32_t         n_pools;
+    int32_t         n_seq;
+    const int32_t*  table;
+    int32_t*        table_out;      /* may be table */
+    int64_t         table_nb_seq;
+    int32_t         table_width;
+    int32_t         reserved;       /* 0 */
+    int32_t*        n_live;         /* device [1] */
+    int32_t*        refs;           /* optional device [n_pages] */
+    void*           workspace;
+    size_t          workspace_size;
+} cvattn_pages_compact_params;
+
+cvattn_status cvattn_pages_compact(cvattn_context* ctx, void* stream, const cvattn_pages_compact_params* p);
+
+/* ------------------------------------------------ verification of drafts */
+
+/* Which drafted tokens stand, from the target's logits and given random numbers
+ * (speculative sampling; the reference samples one token a step).  Node 0 of a
+ * sequence is the token that was pending, always accepted; node i > 0 was drafted
+ * after node parents[i] < i.  At node x, with p = softmax(logits[x] / temperature),
+ * the nodes drafted after x are tried in their order:
+ *   with draft_probs  node c of token t stands if accept_u[c] * q(t) < p(t),
+ *                     q = draft_probs[x]; else p becomes max(p - q, 0), normalized;
+ *   without           it stands if accept_u[c] < p(t); else p(t) becomes 0 and p
+ *                     is normalized (drafts that were not drawn at random);
+ * where nothing would be left of p it stays as it was.  The first that stands is
+ * the next x.  Where none does, the token with the lowest number v for which
+ * p(0) + .. + p(v) > sample_u * sum(p) follows, and the sequence ends.
+ * The tokens are then distributed as the target's own.  temperature 0: a node
+ * stands if its token has the largest logit (ties: the lowest), and that follows.
+ *   accepted    the nodes in order, 0 first, then -1 up to accepted_stride's
+ *               max_nodes entries: what cvattn_tree_commit takes
+ *   n_accepted  how many
+ *   next_token  the token that follows (-1: none)
+ *   log_probs   optional: log p of each token that was gained, the accepted drafts'
+ *               and the following one's, before any draft was refused at its node;
+ *               0 from n_accepted on
+ * Logits may be infinite; a NaN counts as -infinity, a draft probability that is
+ * NaN or negative as 0.  At a node without any weight the sequence ends with
+ * next_token -1.  Sums over the vocabulary are in 64 bits, exponentials that
+ * decide the following token too.
+ * n_nodes 0: nothing is accepted, next_token -1; so also for n_nodes, temperatures
+ * (negative, NaN), tokens (outside [0, vocab)) or parents out of range, which are
+ * recorded. */
+typedef struct cvattn_verify_params {
+    const void*     logits;         /* device; element v of node i of sequence s at           */
+    int64_t         logits_nb_node; /* + s*logits_nb_seq + i*logits_nb_node + v (elements)    */
+    int64_t         logits_nb_seq;
+    const float*    draft_probs;    /* optional device f32, laid out likewise */
+    int64_t         probs_nb_node;
+    int64_t         probs_nb_seq;
+    const int32_t*  tokens;         /* device [n_seq][max_nodes] */
+    const int32_t*  parents;        /* optional device [n_seq][max_nodes]; NULL: chains */
+    int64_t         parents_nb_seq; /* max_nodes, or 0: one tree for all */
+    const int32_t*  n_nodes;        /* optional device [n_seq]; NULL: max_nodes each */
+    const float*    accept_u;       /* device [n_seq][max_nodes], in [0, 1) */
+    const float*    sample_u;       /* device [n_seq], in [0, 1) */
+    const float*    temperature;    /* optional device [n_seq]; NULL: 1 */
+    int32_t*        accepted;       /* device: entry i of sequence s at s*accepted_stride + i */
+    int64_t         accepted_stride;
+    int32_t*        n_accepted;     /* device [n_seq] */
+    int32_t*        next_token;     /* device [n_seq] */
+    float*          log_probs;      /* optional device [n_seq][max_nodes] */
+    int32_t         logits_type;    /* CVATTN_TYPE_F32, CVATTN_TYPE_F16 or CVATTN_TYPE_BF16 */
+    int32_t         n_seq;
+    int32_t         max_nodes;      /* at most CVATTN_TREE_MAX_NODES */
+    int32_t         vocab;
+    void*           workspace;      /* device scratch of cvattn_verify_workspace_size bytes; */
+    size_t          workspace_size; /* needs no initialization                               */
+} cvattn_verify_params;
+
+size_t cvattn_verify_workspace_size(int32_t n_seq, int32_t max_nodes, int32_t vocab);
+
+cvattn_status cvattn_verify_drafts(cvattn_context* ctx, void* stream, const cvattn_verify_params* p);
 
 /* ------------------------------------------------------- offload and load */
 
