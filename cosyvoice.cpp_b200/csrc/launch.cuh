@@ -26,4 +26,23 @@ inline cudaError_t launch_overlapped(void (*fn)(P...), dim3 grid, int block, siz
     return cudaLaunchKernelEx(&cfg, fn, std::forward<A>(args)...);
 }
 
+// The same with `cluster` CTAs of the grid's first dimension to a cluster.
+template <class... P, class... A>
+inline cudaError_t launch_overlapped_clusters(void (*fn)(P...), dim3 grid, int block, size_t smem, int cluster, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, fn, std::forward<A>(args)...);
+}
+
 }  // namespace cvattn

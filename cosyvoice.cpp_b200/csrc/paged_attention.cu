@@ -1,84 +1,131 @@
-// paged_attention.cu -- attention over a paged 8-bit cache.
+// paged_attention.cu -- the join of splits and the host side of attention over a paged 8-bit cache.
 #include "launch.cuh"
-#include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace cvattn {
 namespace paged {
 
-// A warp takes one row: a lane scores a position at a time, then carries two dims of the output.
-template <int F>
-__global__ void __launch_bounds__(128) paged_row_kernel(const __grid_constant__ cvattn_paged_attention_params p, int* status) {
+// --------------------------------------------------------------- combine --
+//
+// 16 threads (4 dims each) follow every kLanes-th split of a row; the partial sums are joined in order.
+template <int kLanes>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ AttArgs a) {
+    constexpr int kPer = 16 / kLanes;  // rows per CTA
+    __shared__ float4 so[16][16];
+    __shared__ float2 sml[16];
     griddep_wait();
-    __shared__ float qs[4][kD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = blockIdx.y;
-    const int item = blockIdx.x * 4 + warp, i = item / p.n_q_heads, h = item % p.n_q_heads;
-    if (i >= p.max_q) return;
-    const int kvh = h / (p.n_q_heads / p.pool.n_heads), blocks = p.pool.page_size / kBlock;
-    int L = p.kv_len[s], n = p.n_q ? p.n_q[s] : p.max_q;
-    if (L < 0 || L > p.max_kv_len || n < 0 || n > p.max_q) {
-        if (item == 0 && lane == 0) record_status(status, kStatusBadLength);
-        L = n = 0;
-    }
-    const int end = i < n ? min(L, L - n + i + 1) : 0;
-    const float* q = p.q + s * p.q_nb_seq + i * p.q_nb_tok + h * kD;
-    qs[warp][lane] = q[lane] * p.scale;
-    qs[warp][lane + 32] = q[lane + 32] * p.scale;
-    __syncwarp();
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int j0 = 0; j0 < end; j0 += 32) {
-        const int j = j0 + lane;
-        int page = -1;
-        float x = -INFINITY, vs = 0.0f;
-        const uint8_t* vc = nullptr;
-        if (j < end) {
-            page = page_of(p.table + s * p.table_nb_seq, j / p.pool.page_size, p.pool.n_pages);
-            if (page < 0) {
-                record_status(status, kStatusBadPage);
-            } else {
-                const int in = kvh * blocks + j % p.pool.page_size / kBlock, t = j % kBlock;
-                const uint8_t* kc = static_cast<const uint8_t*>(p.pool.k) + page * p.pool.nb_page + (int64_t)in * kBlockBytes + t * kD;
-                vc = static_cast<const uint8_t*>(p.pool.v) + page * p.pool.nb_page + (int64_t)in * kBlockBytes;
-                vs = p.pool.v_scale[page * p.pool.nb_scale + in];
-                float dot = 0.0f;
-                for (int d = 0; d < kD; ++d) dot = fmaf(code_value<F>(kc[d]), qs[warp][d], dot);
-                x = dot * p.pool.k_scale[page * p.pool.nb_scale + in];
+    const int unit = threadIdx.x >> 4, c = threadIdx.x & 15, lane = unit % kLanes;
+    const int all_rows = a.p.max_q * a.G;
+    const int r = blockIdx.x * kPer + unit / kLanes, kvh = blockIdx.y, s = blockIdx.z;
+    Join j;
+    if (r < all_rows) {
+        const int64_t slot = ((int64_t)s * a.p.pool.n_heads + kvh) * a.n_splits * all_rows + r;
+        for (int k0 = lane; k0 < a.n_splits; k0 += 4 * kLanes) {
+            float2 ml[4];
+            float4 v[4];
+            float top = j.M;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = k0 + u * kLanes;
+                ml[u] = make_float2(-INFINITY, 0.0f);
+                if (k < a.n_splits) {
+                    ml[u] = *reinterpret_cast<const float2*>(a.ws_ml + (slot + (int64_t)k * all_rows) * 2);
+                    v[u] = *reinterpret_cast<const float4*>(a.ws_o + (slot + (int64_t)k * all_rows) * kD + c * 4);
+                }
+                top = fmaxf(top, ml[u].x);
             }
-        }
-        float top = x;
-        for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        top = fmaxf(top, m);
-        if (top == -INFINITY) continue;
-        const float f = expf(m - top), e = expf(x - top);
-        float sum = e;
-        for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        l = fmaf(l, f, sum);
-        m = top;
-        o0 *= f;
-        o1 *= f;
-        for (int k = 0; k < min(32, end - j0); ++k) {
-            const float w = __shfl_sync(0xffffffffu, e * vs, k);
-            const uint8_t* c = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(vc), k));
-            if (c == nullptr) continue;
-            o0 = fmaf(w, code_value<F>(c[v_place((j0 + k) % kBlock, lane)]), o0);
-            o1 = fmaf(w, code_value<F>(c[v_place((j0 + k) % kBlock, lane + 32)]), o1);
+            if (top == -INFINITY) continue;
+            const float f = exp2f(j.M - top);
+            j.M = top;
+            j.l *= f;
+            j.o.x *= f; j.o.y *= f; j.o.z *= f; j.o.w *= f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) j.add(ml[u], v[u]);
         }
     }
-    float* out = p.out + s * p.out_nb_seq + i * p.out_nb_tok + h * kD;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    out[lane] = o0 * inv;
-    out[lane + 32] = o1 * inv;
-    if (p.lse && lane == 0) p.lse[((int64_t)s * p.max_q + i) * p.n_q_heads + h] = l > 0.0f ? m + logf(l) : -INFINITY;
+    if constexpr (kLanes > 1) {
+        so[unit][c] = j.o;
+        if (c == 0) sml[unit] = make_float2(j.M, j.l);
+        __syncthreads();
+        if (lane) return;
+        j = Join();
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) j.M = fmaxf(j.M, sml[unit + k].x);
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) j.add(sml[unit + k], so[unit + k][c]);
+    }
+    if (r < all_rows) j.write(a, s, kvh, r, c);
+}
+
+// ------------------------------------------------------------------ host --
+
+constexpr int kSms = 148;
+
+static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct Plan {
+    int R, row_tiles, cluster, n_splits;
+};
+
+static Plan plan_of(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
+    Plan p{};
+    const int64_t rows = (int64_t)max_q * (n_q_heads / n_kv_heads);
+    p.R = rows <= 8 ? 1 : 2;
+    p.row_tiles = (int)((rows + 8 * p.R * kMmaWarps - 1) / (8 * p.R * kMmaWarps));
+    const int64_t units = (int64_t)n_seq * n_kv_heads * p.row_tiles, blocks = (max_kv_len + kBlock - 1) / kBlock;
+    int64_t want = (kSms * (p.R == 1 ? 4 : 3)) / units, most = blocks / (2 * kMmaWarps);
+    if (want > most) want = most;
+    p.cluster = 1;
+    while (p.cluster < kMaxCluster && 2 * p.cluster <= want) p.cluster *= 2;
+    p.n_splits = want > p.cluster ? (int)(want / p.cluster) : 1;
+    return p;
+}
+
+template <int F, int R> static cudaError_t launch_mma(cudaStream_t stream, const AttArgs& a, const Plan& plan) {
+    constexpr int smem = MmaSmem<R>::kBytes;
+    auto* fn = paged_mma_kernel<F, R>;
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)(plan.cluster * plan.n_splits), (unsigned)(a.p.pool.n_heads * plan.row_tiles), (unsigned)a.p.n_seq);
+    return launch_overlapped_clusters(fn, grid, kMmaWarps * 32, smem, plan.cluster, stream, a);
+}
+
+template <int kLanes> static cudaError_t run_combine(cudaStream_t stream, const AttArgs& a) {
+    const int rows = a.p.max_q * a.G;
+    const dim3 grid((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)a.p.pool.n_heads, (unsigned)a.p.n_seq);
+    return launch_overlapped(paged_combine_kernel<kLanes>, grid, 256, 0, stream, a);
 }
 
 }  // namespace paged
 
-size_t paged_attention_workspace_bytes(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) { return 0; }
+size_t paged_attention_workspace_bytes(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
+    using namespace paged;
+    const Plan p = plan_of(n_seq, max_q, max_kv_len, n_q_heads, n_kv_heads);
+    if (p.n_splits == 1) return 0;
+    const size_t rows = (size_t)n_seq * p.n_splits * max_q * n_q_heads;
+    return align256(rows * 2 * 4) + rows * kD * 4;
+}
 
 cudaError_t launch_paged_attention(cudaStream_t stream, const cvattn_paged_attention_params& p, int* status) {
     using namespace paged;
-    const dim3 grid((unsigned)(((int64_t)p.max_q * p.n_q_heads + 3) / 4), (unsigned)p.n_seq);
-    auto* fn = p.pool.format == kI8 ? paged_row_kernel<kI8> : paged_row_kernel<kE4M3>;
-    return launch_overlapped(fn, grid, 128, 0, stream, p, status);
+    AttArgs a{};
+    a.p = p;
+    a.G = p.n_q_heads / p.pool.n_heads;
+    a.blocks = p.pool.page_size / kBlock;
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.status = status;
+    const Plan plan = plan_of(p.n_seq, p.max_q, p.max_kv_len, p.n_q_heads, p.pool.n_heads);
+    a.n_splits = plan.n_splits;
+    if (plan.n_splits > 1) {
+        const size_t rows = (size_t)p.n_seq * plan.n_splits * p.max_q * p.n_q_heads;
+        a.ws_ml = static_cast<float*>(p.workspace);
+        a.ws_o = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + align256(rows * 2 * 4));
+    }
+    cudaError_t e;
+    if (p.pool.format == kI8) e = plan.R == 1 ? launch_mma<kI8, 1>(stream, a, plan) : launch_mma<kI8, 2>(stream, a, plan);
+    else e = plan.R == 1 ? launch_mma<kE4M3, 1>(stream, a, plan) : launch_mma<kE4M3, 2>(stream, a, plan);
+    if (e != cudaSuccess || plan.n_splits == 1) return e;
+    return plan.n_splits > 32 ? run_combine<16>(stream, a) : plan.n_splits > 8 ? run_combine<4>(stream, a) : run_combine<1>(stream, a);
 }
 
 }  // namespace cvattn
