@@ -73,7 +73,7 @@ static Plan plan_of(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_k
     p.R = rows <= 8 ? 1 : 2;
     p.row_tiles = (int)((rows + 8 * p.R * kMmaWarps - 1) / (8 * p.R * kMmaWarps));
     const int64_t units = (int64_t)n_seq * n_kv_heads * p.row_tiles, blocks = (max_kv_len + kBlock - 1) / kBlock;
-    int64_t want = (kSms * (p.R == 1 ? 4 : 3)) / units, most = blocks / (2 * kMmaWarps);
+    int64_t want = (kSms * (p.R == 1 ? 4 : 3)) / units, most = blocks / kMmaWarps;
     if (want > most) want = most;
     p.cluster = 1;
     while (p.cluster < kMaxCluster && 2 * p.cluster <= want) p.cluster *= 2;

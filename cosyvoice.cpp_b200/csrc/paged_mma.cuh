@@ -1,13 +1,13 @@
 // paged_mma.cuh -- paged attention of few rows on warp-level tensor-core MMAs (mma.sync m16n8k16, f16 operands, f32
 // accumulators).
 //
-// Codes are exact in f16: int8 as integers, e4m3 by its bits in f16's places (2^-8 of the value).  A row of Q is scaled by a
+// Codes are exact in f16.  A row of Q is scaled by a
 // power of two and split into f16 hi + lo, which lie 8 rows apart in one A operand: a product over 16 rows serves 8 rows of
-// queries, and the sum of its two halves is the score.  P is split the same way.  A step is one block of 16 positions: its
-// scale of the keys multiplies the scores, its scale of the values the step's output, which is a fresh accumulator added to
-// f32 registers.  So every product is exact, and no sum stays in the tensor cores (whose adds truncate) for more than a step.
+// queries, and the sum of its two halves is the score.  P is split the same way.  A block of 16 positions has
+// its scale of the keys multiplied to the scores, its scale of the values to the block's output, which is a fresh accumulator
+// added to f32 registers.  So every product is exact, and no sum stays in the tensor cores (whose adds truncate) for longer.
 //
-// A warp takes 8 R rows and every WK-th block of its CTA's share; each lane copies (cp.async) the 64 bytes of a block that it
+// A warp takes 8 R rows and every WK-th pair of blocks of its CTA's share; each lane copies (cp.async) the 64 bytes of a block that it
 // reads itself, so that a ring of its own needs no barrier.  WR row groups x WK shares are the CTA's 4 warps.  The CTAs of a
 // cluster share the positions of a unit (sequence, KV head, row tile) and join through distributed shared memory; where one
 // cluster per unit would leave SMs idle, several do, and paged_combine_kernel joins their parts.
@@ -22,12 +22,12 @@ namespace paged {
 using dmma::mma16816;
 using dmma::quad_max;
 using dmma::quad_sum;
-using dmma::split2;
 using dtc::pow2f;
 
 constexpr int kMmaWarps = 4;
-constexpr int kStages = 4;               // blocks in flight per warp
-constexpr int kStageBytes = 2 * kBlockBytes;
+constexpr int kStages = 3;               // steps in flight per warp
+constexpr int kPair = 2;                 // blocks of a step
+constexpr int kStageBytes = kPair * 2 * kBlockBytes;
 constexpr int kMaxCluster = 8;
 constexpr float kLazy = 8.0f;            // a running maximum is raised when a score passes it by 2^8
 constexpr float kOffs = 7.0f;            // P is kept 2^7 larger, far from f16's subnormals
@@ -75,23 +75,29 @@ __device__ __forceinline__ float2 peer_ld2(uint32_t addr) {
     return v;
 }
 
-// Four codes as two pairs of f16 (int8: the value, e4m3: 2^-8 of it; every byte gives a finite number).
+// Four codes as two pairs of f16.
 template <int F> __device__ __forceinline__ void to_f16(uint32_t w, uint32_t& a, uint32_t& b) {
     if constexpr (F == kI8) {
         a = dtc::hsub2_u32(__byte_perm(w, 0x64646464u, 0x4140u), dtc::kF16x2_1152);
         b = dtc::hsub2_u32(__byte_perm(w, 0x64646464u, 0x4342u), dtc::kF16x2_1152);
     } else {
-        const uint32_t x = __byte_perm(w, 0u, 0x1404u), y = __byte_perm(w, 0u, 0x3424u);
-        a = (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
-        b = (y & 0x80008000u) | ((y >> 1) & 0x3f803f80u);
+        asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+            : "=r"(a), "=r"(b) : "r"(w));
     }
 }
-template <int F> constexpr float kUnit = F == kI8 ? 1.0f : 256.0f;  // a code's f16 times this is its value
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long ra = *reinterpret_cast<unsigned long long*>(&a), rb = *reinterpret_cast<unsigned long long*>(&b), rd;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
     return *reinterpret_cast<float2*>(&rd);
+}
+// x = hi + lo in f16 pairs, hi the nearest.
+__device__ __forceinline__ void split_near(float2 x, uint32_t& hi, uint32_t& lo) {
+    hi = tc::pack_f16x2(x.x, x.y);
+    float a, b;
+    asm("{\n\t.reg .b16 h, g;\n\tmov.b32 {h, g}, %2;\n\tfma.rn.f32.f16 %0, h, %3, %4;\n\tfma.rn.f32.f16 %1, g, %3, %5;\n\t}"
+        : "=f"(a), "=f"(b) : "r"(hi), "h"((uint16_t)0xBC00u), "f"(x.x), "f"(x.y));
+    lo = tc::pack_f16x2(a, b);
 }
 // A product into a fresh accumulator.
 __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -145,7 +151,7 @@ struct Join {
 template <int R> struct MmaSmem {
     static constexpr int kRows = 8 * R;                          // of a warp
     static constexpr int kRing = kMmaWarps * kStages * kStageBytes;
-    static constexpr int kScales = kMmaWarps * kStages * 8;
+    static constexpr int kScales = kMmaWarps * kStages * kPair * 8;
     static constexpr int kPad = kD + 4;
     // (at the end, in the ring's place) the warps' rows, then the CTA's
     static constexpr int kOut = kMmaWarps * kRows * kPad * 4, kMl = kMmaWarps * kRows * 8;
@@ -174,49 +180,54 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
     const int last_row = min(rows, r0 + S::kRows * kMmaWarps) - 1;
     const int end = last_row >= r0 ? max(0, before + last_row / a.G) : 0;
     const int n_blocks = (end + kBlock - 1) / kBlock, shares = C * a.n_splits, share = split * C + rank;
-    const int b0 = (int)((int64_t)n_blocks * share / shares), b1 = (int)((int64_t)n_blocks * (share + 1) / shares);
-    const int steps = rw < rows ? max(0, (b1 - b0 - wk + WK - 1) / WK) : 0;
+    const int n_steps = (n_blocks + kPair - 1) / kPair;
+    const int s0 = (int)((int64_t)n_steps * share / shares), s1 = (int)((int64_t)n_steps * (share + 1) / shares);
+    const int steps = rw < rows ? max(0, (s1 - s0 - wk + WK - 1) / WK) : 0;
 
     const int32_t* table = a.p.table + (int64_t)s * a.p.table_nb_seq;
-    // lane i knows of the warp's step 32 c + i: where its block lies, and its scales
+    // lane i knows of block i & 1 of the warp's step 16 c + i / 2: where it lies, and its scales
     int64_t off = 0, next_off = 0;
-    float2 sc = make_float2(0.f, 0.f), next_sc = sc;
+    float2 sc = make_float2(-1.0f, 0.0f), next_sc = sc;  // (-1: not seen)
     auto look = [&](int chunk, int64_t& o, float2& f) {
-        const int k = 32 * chunk + lane;
-        if (k >= steps) return;
-        const int b = b0 + wk + k * WK;
+        const int b = kPair * (s0 + wk + (16 * chunk + (lane >> 1)) * WK) + (lane & 1);
+        o = 0;
+        f = make_float2(-1.0f, 0.0f);
+        if (16 * chunk + (lane >> 1) >= steps || b >= n_blocks) return;
         const int page = page_of(table, b / a.blocks, a.p.pool.n_pages);
         if (page < 0) {
             record_status(a.status, kStatusBadPage);
-            o = 0;
-            f = make_float2(-1.0f, 0.0f);  // not seen
             return;
         }
         const int in = kvh * a.blocks + b % a.blocks;
         o = page * a.p.pool.nb_page + (int64_t)in * kBlockBytes;
-        f.x = a.p.pool.k_scale[page * a.p.pool.nb_scale + in] * kUnit<F>;
-        f.y = a.p.pool.v_scale[page * a.p.pool.nb_scale + in] * kUnit<F>;
+        f.x = a.p.pool.k_scale[page * a.p.pool.nb_scale + in];
+        f.y = a.p.pool.v_scale[page * a.p.pool.nb_scale + in];
     };
     const uint8_t* kp = static_cast<const uint8_t*>(a.p.pool.k) + (4 * (gid >> 1) + (gid & 1)) * kD + 16 * tig;
     const uint8_t* vp = static_cast<const uint8_t*>(a.p.pool.v) + lane * 16;
-    uint8_t* ring = smem + warp * kStages * kStageBytes;
-    float2* scales = reinterpret_cast<float2*>(smem + S::kBytes - S::kScales) + warp * kStages;
+    const uint8_t* ring = smem + warp * kStages * kStageBytes;
+    const uint32_t ring_at = smem_addr(ring) + lane * 16;
+    float2* scales = reinterpret_cast<float2*>(smem + S::kBytes - S::kScales) + warp * kStages * kPair;
+    int to = 0;  // the slot that is filled next
     auto issue = [&](int k) {
         if (k < steps) {
-            if (k && (k & 31) == 0) {
+            if (k && (k & 15) == 0) {
                 off = next_off;
                 sc = next_sc;
             }
-            if ((k & 31) == 8) look((k >> 5) + 1, next_off, next_sc);
-            const int64_t at = __shfl_sync(0xffffffffu, off, k & 31);
-            const int slot = k % kStages;
-            const uint32_t to = smem_addr(ring + slot * kStageBytes) + lane * 16;
-            copy16(to, kp + at);
-            copy16(to + 512, kp + at + 2 * kD);
-            copy16(to + 1024, vp + at);
-            copy16(to + 1536, vp + at + 512);
-            if (lane == (k & 31)) scales[slot] = sc;
+            if ((k & 15) == 4) look((k >> 4) + 1, next_off, next_sc);
+#pragma unroll
+            for (int e = 0; e < kPair; ++e) {
+                const int64_t at = __shfl_sync(0xffffffffu, off, 2 * (k & 15) + e);
+                const uint32_t dst = ring_at + to * kStageBytes + e * 2 * kBlockBytes;
+                copy16(dst, kp + at);
+                copy16(dst + 512, kp + at + 2 * kD);
+                copy16(dst + 1024, vp + at);
+                copy16(dst + 1536, vp + at + 512);
+            }
+            if ((lane >> 1) == (k & 15)) scales[to * kPair + (lane & 1)] = sc;
         }
+        to = to + 1 == kStages ? 0 : to + 1;
         copies_done();
     };
     look(0, off, sc);
@@ -243,66 +254,79 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
         lim[i] = r < rows ? before + r / a.G : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            split2(e[j].x * f, e[j].y * f, qa[i][j][0], qa[i][j][1]);
-            split2(e[j].z * f, e[j].w * f, qa[i][j][2], qa[i][j][3]);
+            split_near(make_float2(e[j].x * f, e[j].y * f), qa[i][j][0], qa[i][j][1]);
+            split_near(make_float2(e[j].z * f, e[j].w * f), qa[i][j][2], qa[i][j][3]);
         }
     }
     const int sure = before + rw / a.G;  // positions below it every row of the warp sees
-    float2 O[R][8];
-    float base[R], thr[R], l[R];
+    float2 O[R][8], l[R];
+    float base[R], thr[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         base[i] = 0.0f;
         thr[i] = -INFINITY;  // nothing seen: any score raises the reference
-        l[i] = 0.0f;
+        l[i] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) O[i][j] = make_float2(0.f, 0.f);
     }
 
+    int slot = 0;
 #pragma unroll 1
     for (int k = 0; k < steps; ++k) {
         copies_wait<kStages - 2>();
         __syncwarp();  // the scales of this step; and everybody has left the slot before
         issue(k + kStages - 1);
-        const int slot = k % kStages;
         const uint4* in = reinterpret_cast<const uint4*>(ring + slot * kStageBytes + lane * 16);
-        const float2 f = scales[slot];
-        float sco[R][2][2];
+        const float4 f4 = *reinterpret_cast<const float4*>(scales + slot * kPair);
+        const float ks[kPair] = {f4.x, f4.z}, vs[kPair] = {f4.y, f4.w};
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+        float2 sco[R][2 * kPair];  // scores by block and tile: positions 4 tig + 2 tile, + 1
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const uint4 w = in[32 * tt];
-            uint32_t b[8];
-            to_f16<F>(w.x, b[0], b[1]);
-            to_f16<F>(w.y, b[2], b[3]);
-            to_f16<F>(w.z, b[4], b[5]);
-            to_f16<F>(w.w, b[6], b[7]);
+        for (int e = 0; e < kPair; ++e)
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                float c[4];
-                mma_first(c, qa[i][0], b[0], b[1]);
-                mma16816(c, qa[i][1], b[2], b[3]);
-                mma16816(c, qa[i][2], b[4], b[5]);
-                mma16816(c, qa[i][3], b[6], b[7]);
-                sco[i][tt][0] = fmaf(c[0] + c[2], rs[i] * f.x, -base[i]);
-                sco[i][tt][1] = fmaf(c[1] + c[3], rs[i] * f.x, -base[i]);
+            for (int tt = 0; tt < 2; ++tt) {
+                const uint4 w = in[128 * e + 32 * tt];
+                uint32_t b[8];
+                to_f16<F>(w.x, b[0], b[1]);
+                to_f16<F>(w.y, b[2], b[3]);
+                to_f16<F>(w.z, b[4], b[5]);
+                to_f16<F>(w.w, b[6], b[7]);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    float c[4];
+                    mma_first(c, qa[i][0], b[0], b[1]);
+                    mma16816(c, qa[i][1], b[2], b[3]);
+                    mma16816(c, qa[i][2], b[4], b[5]);
+                    mma16816(c, qa[i][3], b[6], b[7]);
+                    const float g = rs[i] * ks[e];
+                    sco[i][2 * e + tt] = ffma2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), make_float2(g, g), make_float2(-base[i], -base[i]));
+                }
             }
-        }
-        const int j0 = (b0 + wk + k * WK) * kBlock;
-        if (j0 + kBlock > sure || f.x < 0.0f) {  // some row may not see some position of the block
+        const int j0 = kPair * (s0 + wk + k * WK) * kBlock;
+        const bool hidden = ks[0] < 0.0f || ks[1] < 0.0f;
+        uint32_t there[kPair] = {0xffffffffu, 0xffffffffu};  // the lane's four positions that exist, as bytes
+        if (j0 + kPair * kBlock > sure || hidden) {  // some row may not see some position of the step
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const int left = f.x < 0.0f ? 0 : lim[i] - j0 - 4 * tig;
-                if (left < 1) sco[i][0][0] = -INFINITY;
-                if (left < 2) sco[i][0][1] = -INFINITY;
-                if (left < 3) sco[i][1][0] = -INFINITY;
-                if (left < 4) sco[i][1][1] = -INFINITY;
+            for (int e = 0; e < kPair; ++e) {
+                const int first = j0 + e * kBlock + 4 * tig, exist = ks[e] < 0.0f ? 0 : end - first;
+                there[e] = exist >= 4 ? 0xffffffffu : exist <= 0 ? 0u : (1u << (8 * exist)) - 1u;
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int left = ks[e] < 0.0f ? 0 : lim[i] - first;
+                    if (left < 1) sco[i][2 * e].x = -INFINITY;
+                    if (left < 2) sco[i][2 * e].y = -INFINITY;
+                    if (left < 3) sco[i][2 * e + 1].x = -INFINITY;
+                    if (left < 4) sco[i][2 * e + 1].y = -INFINITY;
+                }
             }
         }
         float mx[R];
         bool up = false;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            mx[i] = fmaxf(fmaxf(sco[i][0][0], sco[i][0][1]), fmaxf(sco[i][1][0], sco[i][1][1]));
+            mx[i] = fmaxf(sco[i][0].x, sco[i][0].y);
+#pragma unroll
+            for (int t = 1; t < 2 * kPair; ++t) mx[i] = fmaxf(mx[i], fmaxf(sco[i][t].x, sco[i][t].y));
             up |= mx[i] > thr[i];
         }
         if (__any_sync(0xffffffffu, up)) {
@@ -313,49 +337,55 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
                     const float by = top - kOffs, g = thr[i] == -INFINITY ? 0.0f : fast_exp2(-by);
                     base[i] += by;
                     thr[i] = kLazy + kOffs;
-                    l[i] *= g;
+                    l[i].x *= g;
+                    l[i].y *= g;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         O[i][j].x *= g;
                         O[i][j].y *= g;
                     }
 #pragma unroll
-                    for (int tt = 0; tt < 2; ++tt) {
-                        sco[i][tt][0] -= by;
-                        sco[i][tt][1] -= by;
+                    for (int t = 0; t < 2 * kPair; ++t) {
+                        sco[i][t].x -= by;
+                        sco[i][t].y -= by;
                     }
                 }
             }
         }
-        uint32_t pa[R][4];
+        uint32_t pa[R][kPair][4];
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
-                sco[i][tt][0] = fast_exp2(sco[i][tt][0]);
-                sco[i][tt][1] = fast_exp2(sco[i][tt][1]);
-                split2(sco[i][tt][0], sco[i][tt][1], pa[i][2 * tt], pa[i][2 * tt + 1]);
+            for (int t = 0; t < 2 * kPair; ++t) {
+                sco[i][t] = make_float2(fast_exp2(sco[i][t].x), fast_exp2(sco[i][t].y));
+                split_near(sco[i][t], pa[i][t >> 1][2 * (t & 1)], pa[i][t >> 1][2 * (t & 1) + 1]);
+                l[i] = add2(l[i], sco[i][t]);
             }
-            l[i] += (sco[i][0][0] + sco[i][0][1]) + (sco[i][1][0] + sco[i][1][1]);
-        }
-        const float2 vs = make_float2(f.y, f.y);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint4 w = in[64 + 32 * h];
-            uint32_t b[8];
-            to_f16<F>(w.x, b[0], b[1]);
-            to_f16<F>(w.y, b[2], b[3]);
-            to_f16<F>(w.z, b[4], b[5]);
-            to_f16<F>(w.w, b[6], b[7]);
+        for (int e = 0; e < kPair; ++e)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    float c[4];
-                    mma_first(c, pa[i], b[2 * j], b[2 * j + 1]);
-                    O[i][4 * h + j] = ffma2(vs, add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), O[i][4 * h + j]);
+            for (int h = 0; h < 2; ++h) {
+                uint4 w = in[128 * e + 64 + 32 * h];
+                if (F == kE4M3 && there[e] != 0xffffffffu) {  // (what lies past the end may be NaN)
+                    w.x &= there[e];
+                    w.y &= there[e];
+                    w.z &= there[e];
+                    w.w &= there[e];
                 }
-        }
+                uint32_t b[8];
+                to_f16<F>(w.x, b[0], b[1]);
+                to_f16<F>(w.y, b[2], b[3]);
+                to_f16<F>(w.z, b[4], b[5]);
+                to_f16<F>(w.w, b[6], b[7]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        float c[4];
+                        mma_first(c, pa[i][e], b[2 * j], b[2 * j + 1]);
+                        O[i][4 * h + j] = ffma2(make_float2(vs[e], vs[e]), add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), O[i][4 * h + j]);
+                    }
+            }
     }
     griddep_launch_dependents();
 
@@ -369,7 +399,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int row = warp * S::kRows + 8 * i + gid;
-        const float ls = quad_sum(l[i]);
+        const float ls = quad_sum(l[i].x + l[i].y);
         // (a row whose scores are all NaN raises nothing, but was seen)
         if (tig == 0) wml[row] = make_float2(thr[i] == -INFINITY && ls == 0.0f ? -INFINITY : base[i], ls);
 #pragma unroll
