@@ -820,7 +820,7 @@ cvattn_status cvattn_verify_drafts(cvattn_context* ctx, void* stream, const cvat
         return CVATTN_ERR_INVALID_ARGUMENT;
     const int t = p->logits_type;
     if (t != CVATTN_TYPE_F32 && t != CVATTN_TYPE_F16 && t != CVATTN_TYPE_BF16) return CVATTN_ERR_UNSUPPORTED;
-    if (p->max_nodes > CVATTN_TREE_MAX_NODES || p->n_seq > kMaxGridSeq) return CVATTN_ERR_UNSUPPORTED;
+    if (p->max_nodes > CVATTN_TREE_MAX_NODES || p->n_seq > kMaxGridSeq || p->vocab > verify_most_vocab()) return CVATTN_ERR_UNSUPPORTED;
     if (!aligned(p->logits, t == CVATTN_TYPE_F32 ? 4 : 2) || (p->max_nodes > 1 && p->logits_nb_node < p->vocab) ||
         (p->n_seq > 1 && p->logits_nb_seq < 0))
         return CVATTN_ERR_INVALID_ARGUMENT;
@@ -836,8 +836,8 @@ cvattn_status cvattn_verify_drafts(cvattn_context* ctx, void* stream, const cvat
     for (const auto& o : out)
         for (const auto& i : in)
             if (o.at && i.at && overlap(o.at, o.bytes, i.at, i.bytes)) return CVATTN_ERR_INVALID_ARGUMENT;
-    const size_t need = verify_workspace_bytes(p->n_seq, p->max_nodes, p->vocab);
-    if (need && (!p->workspace || p->workspace_size < need || !aligned(p->workspace, 16))) return CVATTN_ERR_INVALID_ARGUMENT;
+    if (!p->workspace || p->workspace_size < verify_workspace_bytes(p->n_seq, p->max_nodes, p->vocab) || !aligned(p->workspace, 16))
+        return CVATTN_ERR_INVALID_ARGUMENT;
     DeviceGuard dg(ctx->device);
     if (dg.error() != cudaSuccess) return from_cuda(dg.error());
     return from_cuda(launch_verify(as_stream(stream), *p, ctx->status));

@@ -81,6 +81,7 @@ cudaError_t launch_pages_assign(cudaStream_t stream, const cvattn_pages_assign_p
 cudaError_t launch_pages_compact(cudaStream_t stream, const cvattn_pages_compact_params& p, int n_pages, int* status);
 
 // verify.cu
+int verify_most_vocab();
 size_t verify_workspace_bytes(int n_seq, int max_nodes, int vocab);
 cudaError_t launch_verify(cudaStream_t stream, const cvattn_verify_params& p, int* status);
 

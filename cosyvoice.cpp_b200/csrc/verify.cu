@@ -1,209 +1,692 @@
 // verify.cu -- drafted tokens against the target's logits, with given random numbers.
+//
+// verify_sums_kernel reads every row once: its largest logit m and the sum W of weights exp((l - m) / temperature), in parts
+// of 2048 vectors.  verify_walk_kernel joins a sequence's parts and walks down its drafts, u q(t) W < w(t) deciding about a
+// draft of token t, then finds the token that follows.
+// Weights of the first kernel are f32 exponentials added up in 64 bits: a decision that they could turn has a chance of 1e-7.
+// Where a draft has been refused or the path ends, there are as many borders as the vocabulary has tokens, so there the weights
+// are formed in 64 bits too: 2^(n/64) from a table, the rest by its Taylor polynomial (x^4/24 < 2^-34 at x = ln 2 / 128).  The
+// token that follows: sums of tiles of 32 vectors, then of the one tile that holds the border its elements in order.
 #include <cuda_bf16.h>
 
-#include "launch.cuh"
 #include "common.cuh"
 #include "internal.h"
+#include "launch.cuh"
 
 namespace cvattn {
 namespace verify {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512, kWarps = kThreads / 32;       // of the walk
+constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
 constexpr int kBF16 = CVATTN_TYPE_BF16;
+constexpr int kMaxNodes = CVATTN_TREE_MAX_NODES;
+constexpr int kMaxCluster = 8;
+constexpr int kHeld = 8;             // vectors of a row that a thread keeps between its passes
+constexpr int kSlice = kSumThreads * kHeld;
+constexpr int kMaxTiles = 2048;      // of 32 vectors, per CTA
 
-template <int T> __device__ __forceinline__ float logit(const void* row, int v) {
-    float x;
-    if constexpr (T == kF32) x = static_cast<const float*>(row)[v];
-    else if constexpr (T == kF16) x = __half2float(static_cast<const __half*>(row)[v]);
-    else x = __bfloat162float(static_cast<const __nv_bfloat16*>(row)[v]);
-    return isnan(x) ? -INFINITY : x;
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// The target at one node: weight(v) = exp((logit - m) / temperature), their sum W.
-struct Node {
-    const void* row;
-    const float* q;      // the drafts' probabilities there, or null
-    float m;
-    int hot;             // the lowest token with logit m
-    double inv, W;       // 1 / temperature (0: greedy)
+// A row of logits: `head` elements up to the first 16-byte boundary, `full` vectors of kPer elements, and the rest.
+template <int T> struct Row {
+    static constexpr int kSize = T == kF32 ? 4 : 2, kPer = 16 / kSize;
+    const uint8_t* at;     // element 0
+    int head, full, vocab;
+    __device__ __forceinline__ Row(const void* logits, int64_t elements, int v) {
+        at = static_cast<const uint8_t*>(logits) + elements * kSize;
+        head = min(v, (int)(-reinterpret_cast<uintptr_t>(at) & 15) / kSize);
+        full = (v - head) / kPer;
+        vocab = v;
+    }
+    __device__ __forceinline__ int first(int j) const { return head + j * kPer; }  // element of vector j's place 0
+    __device__ __forceinline__ uint4 load(int j) const { return __ldg(reinterpret_cast<const uint4*>(at + (int64_t)first(j) * kSize)); }
+    // Elements outside the vectors, one for each lane of a warp (-1: none): the head in lanes 0 .., the rest in lanes 16 ..
+    __device__ __forceinline__ int loose(int lane) const {
+        const int rest = head + full * kPer;
+        return lane < head ? lane : lane >= 16 && rest + lane - 16 < vocab ? rest + lane - 16 : -1;
+    }
+    __device__ __forceinline__ float one(int v) const {
+        if constexpr (T == kF32) return __ldg(reinterpret_cast<const float*>(at) + v);
+        const uint16_t h = __ldg(reinterpret_cast<const uint16_t*>(at) + v);
+        return T == kF16 ? h2f(h) : __uint_as_float((uint32_t)h << 16);
+    }
+    static __device__ __forceinline__ void values(uint4 v, float (&x)[kPer]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (T == kF32) {
+                x[i] = __uint_as_float(w[i]);
+            } else if constexpr (T == kF16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
 };
-template <int T> __device__ __forceinline__ double weight(const Node& x, bool greedy, int v) {
-    if (greedy) return v == x.hot ? 1.0 : 0.0;
-    const float l = logit<T>(x.row, v);
-    if (l == x.m) return 1.0;
-    if (l == -INFINITY || x.m == INFINITY) return 0.0;
-    return exp(((double)l - (double)x.m) * x.inv);
-}
-__device__ __forceinline__ float sane(float q) { return q > 0.0f ? q : 0.0f; }
 
-template <class X, class F> __device__ X block_reduce(X x, F join, X* tmp) {
-    for (int w = 16; w > 0; w >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, w));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5] = x;
-    __syncthreads();
-    X y = tmp[0];
-    for (int w = 1; w < kThreads / 32; ++w) y = join(y, tmp[w]);
-    return y;
+// The largest of a vector's elements (NaN left out), in the elements' own type.
+template <int T> __device__ __forceinline__ uint4 vector_max(uint4 a, uint4 b) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (T == kF32) r[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+        else if constexpr (T == kF16) asm("max.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(x[i]), "r"(y[i]));
+        else asm("max.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(x[i]), "r"(y[i]));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// The rule at one node.
+struct Node {
+    float m;             // the largest logit
+    float c;             // log2 e / temperature
+    float low;           // logits that are not above it have no weight
+    float reach;         // weights of logits this far below the largest: less than 2^-995
+    double inv;          // 1 / temperature
+    double u64;          // 64 / (temperature ln 2)
+    double W;            // sum of the weights (of f32 exponentials)
+    int hot;             // greedy: the lowest token with logit m
+    bool greedy;
+    __device__ __forceinline__ void most(float l) {
+        m = l;
+        low = l - reach;
+        if (!(low < l)) low = nextafterf(l, -INFINITY);
+    }
+};
+// exp((l - m) / temperature), l > -infinity finite or a NaN.
+__device__ __forceinline__ float weight32(const Node& x, float l) { return fast_exp2((fmaxf(l, x.low) - x.m) * x.c); }
+// The same in 64 bits, 0 where l is not above x.low or a NaN; m finite.  `table`: 2^(i / 64).
+__device__ __forceinline__ double weight64(const Node& x, float l, const double* table) {
+    constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: u + magic has u's nearest integer in its low bits
+    constexpr double step = 0.010830424696249145;  // ln 2 / 64
+    const double d = (double)fmaxf(l, x.low) - (double)x.m, t = fma(d, x.u64, magic), r = fma(d, x.u64, magic - t);
+    const int n = __double2loint(t);
+    double p = fma(r, step * step * step / 6, step * step / 2);
+    p = fma(p, r, step);
+    const double base = table[n & 63];
+    p = fma(p * r, base, base);
+    return l > x.low ? __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p)) : 0.0;
+}
+// Any l, m.
+__device__ __forceinline__ double weight_any(const Node& x, float l, int v, const double* table) {
+    if (x.greedy) return v == x.hot ? 1.0 : 0.0;
+    if (l == x.m) return 1.0;
+    return x.m == INFINITY ? 0.0 : weight64(x, l, table);
+}
+
+__device__ __forceinline__ double warp_add(double x) {
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+    return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+    return x;
+}
+__device__ __forceinline__ double positive(double x) {  // max(x, 0)
+    const int hi = __double2hiint(x), lo = __double2loint(x);
+    return __hiloint2double(hi < 0 ? 0 : hi, hi < 0 ? 0 : lo);
+}
+
+// Of a slice of a row: the largest logit, the sum of weights below it, and the lowest token with it (where it is asked for).
+struct __align__(16) Part {
+    double sum;
+    float most;
+    int hot;
+};
+
+__device__ __forceinline__ void set_heat(Node& x, float heat) {
+    x.greedy = heat == 0.0f;
+    x.inv = x.greedy ? 0.0 : 1.0 / (double)heat;
+    x.u64 = x.inv * 92.332482616893656;  // 64 / ln 2
+    x.c = (float)fmin(x.inv * 1.4426950408889634, 3.0e38);
+    x.reach = 690.0f * heat;
 }
 
 template <int T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ cvattn_verify_params p, int* status) {
+__global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const __grid_constant__ cvattn_verify_params p, Part* parts) {
+    using R = Row<T>;
+    constexpr int kPer = R::kPer;
+    __shared__ float most[kSumWarps];
+    __shared__ double sums[kSumWarps];
+    __shared__ int hots[kSumWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slice = blockIdx.x, node = blockIdx.y, s = blockIdx.z;
     griddep_wait();
-    __shared__ double tmp[kThreads / 32];
-    __shared__ float tmpf[kThreads / 32];
-    __shared__ int tmpi[kThreads / 32];
-    __shared__ double left_sum[CVATTN_TREE_MAX_NODES];  // of p after each refusal
-    __shared__ int gone[CVATTN_TREE_MAX_NODES];         // tokens refused
-    __shared__ int bad;
-    const int s = blockIdx.x, tid = threadIdx.x;
-    const int n = p.n_nodes ? p.n_nodes[s] : p.max_nodes;
+    griddep_launch_dependents();
+    if (p.n_nodes && node >= p.n_nodes[s]) return;
     const float heat = p.temperature ? p.temperature[s] : 1.0f;
-    const bool greedy = heat == 0.0f;
-    const int32_t* tokens = p.tokens + (int64_t)s * p.max_nodes;
-    const int32_t* parents = p.parents ? p.parents + s * p.parents_nb_seq : nullptr;
-    const float* u = p.accept_u + (int64_t)s * p.max_nodes;
-    int32_t* accepted = p.accepted + s * p.accepted_stride;
-    float* logs = p.log_probs ? p.log_probs + (int64_t)s * p.max_nodes : nullptr;
-    if (tid == 0) bad = n < 0 || n > p.max_nodes || !(heat >= 0.0f);
+    const R row(p.logits, s * p.logits_nb_seq + node * p.logits_nb_node, p.vocab);
+    const int j0 = slice * kSlice + tid, j1 = min(row.full, (slice + 1) * kSlice);
+    uint4 held[kHeld], top;
+    top.x = top.y = top.z = top.w = T == kF32 ? 0xff800000u : T == kF16 ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+        held[k] = top;
+        if (j0 + k * kSumThreads < j1) held[k] = row.load(j0 + k * kSumThreads);
+    }
+    float alone = -INFINITY;
+    int loose = -1;
+    if (warp == 0 && slice == 0) {
+        loose = row.loose(lane);
+        if (loose >= 0) alone = row.one(loose);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) top = vector_max<T>(top, held[k]);
+    float m = fmaxf(alone, -INFINITY);  // (a NaN counts as -infinity)
+    {
+        float l[kPer];
+        R::values(top, l);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) m = fmaxf(m, l[i]);
+    }
+    m = warp_max(m);
+    if (lane == 0) most[warp] = m;
     __syncthreads();
-    if (!bad)
-        for (int i = 1 + tid; i < n; i += kThreads) {
-            const int up = parents ? parents[i] : i - 1;
-            if (up < 0 || up >= i || (uint32_t)tokens[i] >= (uint32_t)p.vocab) bad = 1;
+    m = warp_max(most[lane % kSumWarps]);
+    double sum = 0.0;
+    int hot = INT32_MAX;
+    if (m == -INFINITY) {
+    } else if (heat == 0.0f || m == INFINITY) {
+        int same = 0;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            float l[kPer];
+            R::values(held[k], l);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (l[i] == m) {
+                    ++same;
+                    hot = min(hot, row.first(j0 + k * kSumThreads) + i);
+                }
         }
-    __syncthreads();
-    if (bad && tid == 0) record_status(status, kStatusBadDraft);
-    for (int i = tid; i < p.max_nodes; i += kThreads) {
-        accepted[i] = -1;
-        if (logs) logs[i] = 0.0f;
+        if (loose >= 0 && alone == m) {
+            ++same;
+            hot = min(hot, loose);
+        }
+        sum = same;
+        hot = __reduce_min_sync(0xffffffffu, hot);
+    } else {
+        Node x;
+        set_heat(x, heat);
+        x.most(m);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (j0 + k * kSumThreads < j1) {
+                float l[kPer], part = 0.0f;
+                R::values(held[k], l);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) part += weight32(x, l[i]);
+                sum += part;
+            }
+        if (loose >= 0) sum += weight32(x, alone);
+    }
+    sum = warp_add(sum);
+    if (lane == 0) {
+        sums[warp] = sum;
+        hots[warp] = hot;
     }
     __syncthreads();
-    if (bad || n == 0) {
-        if (tid == 0) {
+    if (tid == 0) {
+        Part out{0.0, m, INT32_MAX};
+#pragma unroll
+        for (int w = 0; w < kSumWarps; ++w) {
+            out.sum += sums[w];
+            out.hot = min(out.hot, hots[w]);
+        }
+        parts[((int64_t)s * p.max_nodes + node) * gridDim.x + slice] = out;
+    }
+}
+
+struct Shared {
+    double table[64];
+    double W[kMaxNodes];                     // of each node: sum of weights,
+    float m[kMaxNodes];                      // largest logit,
+    int hot[kMaxNodes];                      // lowest token with it
+    double num[kMaxNodes], den[kMaxNodes];   // log-probabilities: exponent, sum
+    double inv_left[kMaxNodes];              // 1 / the sum of p after each refusal
+    double post_sum[2][kMaxCluster];         // of the cluster's CTAs, in turn of two
+    int post_found[2][kMaxCluster], post_last[2][kMaxCluster];
+    int gone[kMaxNodes];                     // tokens refused
+    int parent[kMaxNodes], token[kMaxNodes], first_child[kMaxNodes];
+    float u[kMaxNodes];
+    float logit[kMaxNodes], prob[kMaxNodes]; // of the drafts' tokens at their parents
+    int bad;
+    // what warp 0 has decided
+    int what, at, refused;
+    double inv_W;
+};
+enum { kScan = 1, kFollow = 2, kStop = 3 };  // Shared::what
+
+template <int T>
+__global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_constant__ cvattn_verify_params p, const Part* parts,
+                                                                  int n_slices, int n_tiles, int* status) {
+    using R = Row<T>;
+    constexpr int kPer = R::kPer;
+    __shared__ Shared sh;
+    extern __shared__ double tile_sum[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t C, rank;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int s = blockIdx.x / C;
+    if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
+    if (tid == 0) sh.bad = 0;
+    __syncthreads();
+    griddep_wait();
+    const int n = p.n_nodes ? p.n_nodes[s] : p.max_nodes;
+    const float heat = p.temperature ? p.temperature[s] : 1.0f;
+    int32_t* accepted = p.accepted + s * p.accepted_stride;
+    float* logs = p.log_probs ? p.log_probs + (int64_t)s * p.max_nodes : nullptr;
+    const bool refused_all = n < 0 || n > p.max_nodes || !(heat >= 0.0f && heat < INFINITY);
+    const auto row_of = [&](int node) { return R(p.logits, s * p.logits_nb_seq + node * p.logits_nb_node, p.vocab); };
+    for (int i = tid; i < kMaxNodes; i += kThreads) {
+        sh.first_child[i] = kMaxNodes;
+        if (i < (refused_all ? 0 : n)) {
+            const int up = i == 0 ? -1 : p.parents ? p.parents[s * p.parents_nb_seq + i] : i - 1;
+            const int t = p.tokens[(int64_t)s * p.max_nodes + i];
+            sh.parent[i] = up;
+            sh.token[i] = t;
+            sh.u[i] = p.accept_u[(int64_t)s * p.max_nodes + i];
+            if (i > 0) {
+                if (up < 0 || up >= i || (uint32_t)t >= (uint32_t)p.vocab) {
+                    sh.bad = 1;
+                } else {
+                    sh.logit[i] = row_of(up).one(t);
+                    sh.prob[i] = p.draft_probs ? __ldg(p.draft_probs + s * p.probs_nb_seq + up * p.probs_nb_node + t) : 1.0f;
+                }
+            }
+        }
+    }
+    Node x;
+    set_heat(x, heat);
+    // a warp a node: its numbers from all slices
+    if (!refused_all)
+        for (int i = warp; i < n; i += kWarps) {
+            const Part* of = parts + ((int64_t)s * p.max_nodes + i) * n_slices;
+            Part q{0.0, -INFINITY, INT32_MAX};
+            for (int k = lane; k < n_slices; k += 32) {
+                const Part v = of[k];
+                if (v.most > q.most) {
+                    x.most(v.most);
+                    q.sum = v.sum + (q.sum > 0.0 && !x.greedy && v.most < INFINITY ? q.sum * weight64(x, q.most, sh.table) : 0.0);
+                    q.hot = v.hot;
+                    q.most = v.most;
+                } else if (v.most > -INFINITY) {
+                    x.most(q.most);
+                    q.sum += v.most == q.most ? v.sum : x.greedy || q.most == INFINITY ? 0.0 : v.sum * weight64(x, v.most, sh.table);
+                    if (v.most == q.most) q.hot = min(q.hot, v.hot);
+                }
+            }
+            const float top = warp_max(q.most);
+            x.most(top);
+            double w = q.most == top ? 1.0 : 0.0;
+            if (!x.greedy && top < INFINITY && q.most > -INFINITY && q.most < top) w = weight64(x, q.most, sh.table);
+            const double sum = warp_add(q.sum * w);
+            const int hot = __reduce_min_sync(0xffffffffu, q.most == top ? q.hot : INT32_MAX);
+            if (lane == 0) {
+                sh.m[i] = top;
+                sh.W[i] = x.greedy ? 1.0 : sum;
+                sh.hot[i] = hot;
+            }
+        }
+    if (rank == 0)
+        for (int i = tid; i < p.max_nodes; i += kThreads) {
+            accepted[i] = -1;
+            if (logs) logs[i] = 0.0f;
+        }
+    __syncthreads();
+    if (refused_all || sh.bad || n == 0) {
+        if (rank == 0 && tid == 0) {
+            if (refused_all || sh.bad) record_status(status, kStatusBadDraft);
             p.n_accepted[s] = 0;
             p.next_token[s] = -1;
         }
-        return;
+        return;  // (every CTA of the cluster alike)
     }
-    const auto add = [](double a, double b) { return a + b; };
-    const int chunk = (p.vocab + kThreads - 1) / kThreads;
-    const int v0 = min(p.vocab, tid * chunk), v1 = min(p.vocab, v0 + chunk);
-    int at = 0, count = 1, token = -1;
-    if (tid == 0) accepted[0] = 0;
+    for (int i = 1 + tid; i < n; i += kThreads) atomicMin(&sh.first_child[sh.parent[i]], i);
+    __syncthreads();
+
+    // Warp 0 posts this CTA's numbers to the slots of all CTAs, in turn of two: one is written while the other may still be
+    // read.  Then every thread arrives.
+    int turn = 0;
+    auto exchange = [&](double sum, int found, int last) {
+        if (tid < (int)C) {
+            uint32_t a, b, c;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(&sh.post_sum[turn][rank])), "r"(tid));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_addr(&sh.post_found[turn][rank])), "r"(tid));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(c) : "r"(smem_addr(&sh.post_last[turn][rank])), "r"(tid));
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(a), "d"(sum) : "memory");
+            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(b), "r"(found) : "memory");
+            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(c), "r"(last) : "memory");
+        }
+        __syncwarp();
+        if (warp == 0) cluster_arrive();
+        else cluster_arrive_relaxed();  // (they have posted nothing)
+        cluster_wait();
+    };
+
+    int at = 0, count = 1, token = -1, refused = 0;
+    double inv_W = 0.0;
+    R row = row_of(0);
+    const float* q = nullptr;
+    bool simple = false;
+    // this CTA's vectors, tiles of 32 each, in order
+    const int j0 = (int)rank * n_tiles * 32;
+    int j1 = 0, tiles = 0;
+    auto arrive_at = [&](int node) {
+        at = node;
+        row = row_of(node);
+        q = p.draft_probs ? p.draft_probs + s * p.probs_nb_seq + node * p.probs_nb_node : nullptr;
+        x.most(sh.m[node]);
+        x.hot = sh.hot[node];
+        simple = !x.greedy && x.m != INFINITY;
+        j1 = min(j0 + n_tiles * 32, row.full);
+        tiles = (j1 > j0 ? (j1 - j0 + 31) / 32 : 0) + 2;
+    };
+    // One token's part of p after the refusals so far, times its sum.  Weights stay as they are until the first subtraction, so
+    // that equal ones add up exactly.
+    auto less = [&](double w, float qv) {
+        const double g = (double)fmaxf(qv, 0.0f);  // (NaN: 0)
+        double r = positive(fma(w, inv_W, -g));
+        for (int k = 1; k < refused; ++k) r = positive(fma(r, sh.inv_left[k - 1], -g));
+        return r;
+    };
+    auto what = [&](float l, float qv, int v) {
+        double w = weight_any(x, l, v, sh.table);
+        if (!q)
+            for (int k = 0; k < refused; ++k) w = v == sh.gone[k] ? 0.0 : w;
+        else if (refused) w = less(w, qv);
+        return w;
+    };
+    // what() of a tile's elements e, e + 1, .. of this lane.  Tile 0 is the row's head (of the first CTA), the last one what its
+    // vectors leave over (of the last CTA).
+    auto tile = [&](int t, int& e, double (&w)[kPer]) {
+        if (t == 0 || t == tiles - 1) {
+            e = row.loose(lane);
+            const bool mine = e >= 0 && (t == 0 ? rank == 0 && lane < 16 : rank == C - 1 && lane >= 16);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) w[i] = 0.0;
+            if (mine) w[0] = what(row.one(e), q && refused ? __ldg(q + e) : 0.0f, e);
+            return;
+        }
+        const int j = j0 + 32 * (t - 1) + lane;
+        e = row.first(j);
+        if (j >= j1) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) w[i] = 0.0;
+            return;
+        }
+        const uint4 v = row.load(j);
+        float g[kPer], l[kPer];
+        if (q && refused) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) g[i] = __ldg(q + e + i);
+        }
+        R::values(v, l);
+        if (simple) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) w[i] = weight64(x, l[i], sh.table);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) w[i] = (x.greedy ? e + i == x.hot : l[i] == x.m) ? 1.0 : 0.0;
+        }
+        if (!q)
+            for (int k = 0; k < refused; ++k) {
+                const int off = sh.gone[k] - e;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) w[i] = off == i ? 0.0 : w[i];
+            }
+        if (q && refused) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) w[i] = less(w[i], g[i]);
+        }
+    };
+    double before = 0.0, all = 0.0;    // what() over the CTAs before this one, over the vocabulary (warp 0)
+    double total = 0.0, was = 0.0;     // warp 0: what()'s sum over the vocabulary, and before the last refusal
+    bool known = true, exact = false;  // warp 0: whether total is that sum; whether of 64-bit weights
+    bool scanned = false;
+    int c = 0, order = kStop;
+    auto enter = [&](int node) {       // warp 0
+        arrive_at(node);
+        refused = 0;
+        total = sh.W[node];
+        exact = !simple;
+        known = true;
+        c = sh.first_child[node];
+    };
+    if (warp == 0) enter(0);
     for (;;) {
-        Node x;
-        const int size = T == kF32 ? 4 : 2;
-        x.row = static_cast<const uint8_t*>(p.logits) + (s * p.logits_nb_seq + at * p.logits_nb_node) * size;
-        x.q = p.draft_probs ? p.draft_probs + s * p.probs_nb_seq + at * p.probs_nb_node : nullptr;
-        x.inv = greedy ? 0.0 : 1.0 / (double)heat;
-        float m = -INFINITY;
-        for (int v = tid; v < p.vocab; v += kThreads) m = fmaxf(m, logit<T>(x.row, v));
-        x.m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, tmpf);
-        if (x.m == -INFINITY) break;  // no weight anywhere
-        int hot = INT32_MAX;
-        for (int v = tid; v < p.vocab; v += kThreads)
-            if (logit<T>(x.row, v) == x.m) hot = min(hot, v);
-        x.hot = block_reduce(hot, [](int a, int b) { return min(a, b); }, tmpi);
-        double w = 0.0;
-        for (int v = tid; v < p.vocab; v += kThreads) w += weight<T>(x, greedy, v);
-        x.W = block_reduce(w, add, tmp);
-        int refused = 0;
-        double total = x.W;  // of left(v)
-        // p(v) after the refusals so far, times total: weights as they are until the first subtraction, so that equal ones add up exactly
-        auto left = [&](int v) {
-            double r = weight<T>(x, greedy, v);
-            if (!x.q) {
-                for (int k = 0; k < refused; ++k)
-                    if (v == gone[k]) r = 0.0;
-                return r;
-            }
-            if (refused) r /= x.W;
-            for (int k = 0; k < refused; ++k) r = fmax(r - (double)sane(x.q[v]), 0.0) / left_sum[k];
-            return r;
-        };
-        int down = -1;
-        for (int c = at + 1; c < n; ++c) {
-            if ((parents ? parents[c] : c - 1) != at) continue;
-            const int t = tokens[c];
-            const double pt = left(t), qt = x.q ? (double)sane(x.q[t]) : 1.0;
-            if ((double)u[c] * qt * total < pt) {
-                down = c;
-                break;
-            }
-            double sum = 0.0;
-            for (int v = tid; v < p.vocab; v += kThreads) {
-                const double r = left(v);
-                sum += x.q ? fmax(r / total - (double)sane(x.q[v]), 0.0) : v == t ? 0.0 : r;
-            }
-            sum = block_reduce(sum, add, tmp);
-            if (sum > 0.0) {
-                __syncthreads();
-                if (tid == 0) {
-                    left_sum[refused] = sum;
-                    gone[refused] = t;
+        if (warp == 0) {
+            if (scanned) {
+                known = exact = true;
+                if (refused && !(all > 0.0)) {  // the last refusal left nothing: as it was
+                    --refused;
+                    total = was;
+                    scanned = false;
+                } else {
+                    if (q && refused && lane == 0) sh.inv_left[refused - 1] = 1.0 / all;
+                    __syncwarp();
+                    total = all;
                 }
-                __syncthreads();
+            }
+            order = kScan;
+            if (scanned && c >= n) order = kFollow;
+            // drafts in turn, as long as the sum of what is left is known
+            while (order == kScan) {
+                if (x.m == -INFINITY) order = kStop;  // no weight anywhere
+                if (order == kStop || c >= n || !known) break;
+                if (sh.parent[c] != at) {
+                    ++c;
+                    continue;
+                }
+                const int t = sh.token[c];
+                const double pt = what(sh.logit[c], sh.prob[c], t);
+                if ((double)sh.u[c] * (double)fmaxf(sh.prob[c], 0.0f) * total < pt) {
+                    if (lane == 0) {
+                        if (rank == 0) accepted[count] = c;
+                        sh.num[count - 1] = x.greedy || sh.logit[c] == x.m ? 0.0 : ((double)sh.logit[c] - (double)x.m) * x.inv;
+                        sh.den[count - 1] = sh.W[at];
+                    }
+                    ++count;
+                    enter(c);
+                    continue;
+                }
+                if (q && !exact) {  // the subtraction takes a sum of exact weights
+                    known = false;
+                    break;
+                }
+                if (q && refused == 0) inv_W = 1.0 / total;
+                if (lane == 0) sh.gone[refused] = t;
+                __syncwarp();
                 ++refused;
-                total = x.q ? 1.0 : sum;
+                ++c;
+                was = total;
+                if (q) {
+                    known = false;
+                } else {  // (where too little is left for a difference of such sums, they are added up anew)
+                    total -= pt;
+                    known = total > was * (exact ? 0x1p-10 : 0.25);
+                }
             }
-        }
-        auto log_p = [&](int v) { return greedy ? 0.0f : (float)(log(weight<T>(x, greedy, v)) - log(x.W)); };
-        if (down >= 0) {
-            if (tid == 0) {
-                accepted[count] = down;
-                if (logs) logs[count - 1] = log_p(tokens[down]);
+            if (lane == 0) {
+                sh.what = order;
+                sh.at = at;
+                sh.refused = refused;
+                sh.inv_W = inv_W;
             }
-            at = down;
-            ++count;
-            continue;
-        }
-        // the token that follows
-        __shared__ double before[kThreads];
-        __shared__ int found;
-        double sum = 0.0;
-        for (int v = v0; v < v1; ++v) sum += left(v);
-        before[tid] = sum;
-        if (tid == 0) found = -1;
-        __syncthreads();
-        if (tid == 0) {
-            double all = 0.0;
-            for (int i = 0; i < kThreads; ++i) {
-                const double b = before[i];
-                before[i] = all;
-                all += b;
-            }
-            tmp[0] = all;
         }
         __syncthreads();
-        const double target = (double)p.sample_u[s] * tmp[0];
-        double c = before[tid];
-        int mine = -1, last = -1;
-        for (int v = v0; v < v1; ++v) {
-            const double r = left(v);
-            if (r > 0.0) last = v;
-            c += r;
-            if (mine < 0 && c > target) mine = v;
+        order = sh.what;
+        if (order != kScan) break;
+        if (warp) {
+            arrive_at(sh.at);
+            refused = sh.refused;
+            inv_W = sh.inv_W;
         }
-        const int lowest = block_reduce(mine < 0 ? INT32_MAX : mine, [](int a, int b) { return min(a, b); }, tmpi);
-        last = block_reduce(last, [](int a, int b) { return max(a, b); }, tmpi);
-        token = lowest == INT32_MAX ? last : lowest;
-        if (tid == 0 && logs && token >= 0) logs[count - 1] = log_p(token);
-        break;
+        // sums of tiles, of this CTA in the tiles' order, of the cluster
+#pragma unroll 1
+        for (int t = warp; t < tiles; t += kWarps) {
+            double w[kPer], sum = 0.0;
+            int e;
+            tile(t, e, w);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) sum += w[i];
+            sum = warp_add(sum);
+            if (lane == 0) tile_sum[t] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            all = 0.0;
+            for (int t = 0; t < tiles; t += 32) all += warp_add(t + lane < tiles ? tile_sum[t + lane] : 0.0);
+        }
+        if (C > 1) {
+            exchange(all, 0, 0);
+            if (warp == 0) {
+                const double v = lane < (int)C ? sh.post_sum[turn][lane] : 0.0;
+                before = warp_add(lane < (int)rank ? v : 0.0);
+                all = warp_add(v);
+            }
+            turn ^= 1;
+        }
+        scanned = true;
     }
-    if (tid == 0) {
-        p.n_accepted[s] = count;
-        p.next_token[s] = token;
+    if (order == kFollow) {
+        // The token that follows: the first tile whose end passes the target, and the last that has any weight (for a target
+        // that rounding keeps out of reach); then its elements in order.
+        int found = INT32_MAX, last = -1;
+        if (warp == 0) {
+            const double target = (double)p.sample_u[s] * all;
+            int first = INT32_MAX, some_tile = -1;
+            double run0 = before, start = 0.0;
+            for (int t = 0; t < tiles && first == INT32_MAX; t += 32) {
+                const double v = t + lane < tiles ? tile_sum[t + lane] : 0.0;
+                double y = v;
+#pragma unroll
+                for (int w = 1; w < 32; w <<= 1) {
+                    const double z = __shfl_up_sync(0xffffffffu, y, w);
+                    if (lane >= w) y += z;
+                }
+                const uint32_t over = __ballot_sync(0xffffffffu, t + lane < tiles && run0 + y > target && v > 0.0);
+                const uint32_t some = __ballot_sync(0xffffffffu, t + lane < tiles && v > 0.0);
+                if (some) some_tile = t + 31 - __clz(some);
+                if (over) {
+                    const int k = __ffs(over) - 1;
+                    first = t + k;
+                    start = run0 + __shfl_sync(0xffffffffu, y - v, k);
+                }
+                run0 += __shfl_sync(0xffffffffu, y, 31);
+            }
+            const bool out_of_reach = first == INT32_MAX;
+            const int t = out_of_reach ? some_tile : first;
+            if (t >= 0) {
+                double w[kPer], sum = 0.0;
+                int e;
+                tile(t, e, w);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) sum += w[i];
+                double y = sum;
+#pragma unroll
+                for (int k = 1; k < 32; k <<= 1) {
+                    const double z = __shfl_up_sync(0xffffffffu, y, k);
+                    if (lane >= k) y += z;
+                }
+                double run1 = start + (y - sum);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    run1 += w[i];
+                    if (w[i] > 0.0) {
+                        last = e + i;
+                        if (run1 > target && found == INT32_MAX) found = e + i;
+                    }
+                }
+                found = __reduce_min_sync(0xffffffffu, found);
+                last = __reduce_max_sync(0xffffffffu, last);
+                // (a tile whose sum passes the target while its elements, added in another order, do not: its last one)
+                if (!out_of_reach && found == INT32_MAX) found = last;
+                if (out_of_reach) found = INT32_MAX;
+            }
+        }
+        if (C > 1) {
+            exchange(0.0, found, last);
+            if (warp == 0) {
+                found = __reduce_min_sync(0xffffffffu, lane < (int)C ? sh.post_found[turn][lane] : INT32_MAX);
+                last = __reduce_max_sync(0xffffffffu, lane < (int)C ? sh.post_last[turn][lane] : -1);
+            }
+        }
+        if (warp == 0) {
+            token = found == INT32_MAX ? last : found;
+            if (lane == 0 && token >= 0) {
+                const float l = row.one(token);
+                sh.num[count - 1] = x.greedy || l == x.m ? 0.0 : ((double)l - (double)x.m) * x.inv;
+                sh.den[count - 1] = sh.W[at];
+            }
+        }
     }
+    griddep_launch_dependents();
+    if (rank == 0 && warp == 0) {
+        __syncwarp();
+        if (logs)
+            for (int i = lane; i < count - (token < 0); i += 32) logs[i] = (float)(sh.num[i] - log(sh.den[i]));
+        if (lane == 0) {
+            accepted[0] = 0;
+            p.n_accepted[s] = count;
+            p.next_token[s] = token;
+        }
+    }
+    if (C > 1) {  // nobody leaves while others may post to it
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+}
+
+// CTAs per sequence of the walk: two tiles a warp at least, and one wave of them in all.
+static int cluster_of(int n_seq, int vectors) {
+    int c = 1;
+    while (c < kMaxCluster && vectors > c * 2 * kThreads && n_seq * c * 2 <= 2 * 148) c *= 2;
+    while (c < kMaxCluster && vectors > c * kMaxTiles * 32) c *= 2;
+    return c;
+}
+
+static int slices_of(int vocab, int per) { return vocab / per / kSlice + 1; }
+
+template <int T> static cudaError_t launch_for(cudaStream_t stream, const cvattn_verify_params& p, int* status) {
+    constexpr int per = Row<T>::kPer;
+    Part* parts = static_cast<Part*>(p.workspace);
+    const int slices = slices_of(p.vocab, per);
+    const cudaError_t e = launch_overlapped(verify_sums_kernel<T>, dim3((unsigned)slices, (unsigned)p.max_nodes, (unsigned)p.n_seq), kSumThreads,
+                                            0, stream, p, parts);
+    if (e != cudaSuccess) return e;
+    const int vectors = p.vocab / per, c = cluster_of(p.n_seq, vectors), tiles = (vectors + 32 * c - 1) / (32 * c);
+    return launch_overlapped_clusters(verify_walk_kernel<T>, dim3((unsigned)(p.n_seq * c)), kThreads, (size_t)(tiles + 2) * 8, c, stream, p,
+                                      (const Part*)parts, slices, tiles, status);
 }
 
 }  // namespace verify
 
-size_t verify_workspace_bytes(int n_seq, int max_nodes, int vocab) { return 0; }
+// The longest vocabulary: a cluster's tiles of f32 vectors.
+int verify_most_vocab() { return verify::kMaxCluster * verify::kMaxTiles * 32 * 4; }
+
+size_t verify_workspace_bytes(int n_seq, int max_nodes, int vocab) {
+    return (size_t)n_seq * max_nodes * verify::slices_of(vocab, 4) * sizeof(verify::Part);
+}
 
 cudaError_t launch_verify(cudaStream_t stream, const cvattn_verify_params& p, int* status) {
     using namespace verify;
-    auto* fn = p.logits_type == kF32 ? verify_kernel<kF32> : p.logits_type == kF16 ? verify_kernel<kF16> : verify_kernel<kBF16>;
-    return launch_overlapped(fn, (unsigned)p.n_seq, kThreads, 0, stream, p, status);
+    switch (p.logits_type) {
+    case kF32: return launch_for<kF32>(stream, p, status);
+    case kF16: return launch_for<kF16>(stream, p, status);
+    default: return launch_for<kBF16>(stream, p, status);
+    }
 }
 
 }  // namespace cvattn

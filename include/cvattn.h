@@ -746,7 +746,7 @@ cvattn_status cvattn_pages_compact(cvattn_context* ctx, void* stream, const cvat
  * next_token -1.  Sums over the vocabulary are in 64 bits, exponentials that
  * decide the following token too.
  * n_nodes 0: nothing is accepted, next_token -1; so also for n_nodes, temperatures
- * (negative, NaN), tokens (outside [0, vocab)) or parents out of range, which are
+ * (negative, infinite, NaN), tokens (outside [0, vocab)) or parents out of range, which are
  * recorded. */
 typedef struct cvattn_verify_params {
     const void*     logits;         /* device; element v of node i of sequence s at           */
@@ -770,7 +770,7 @@ typedef struct cvattn_verify_params {
     int32_t         logits_type;    /* CVATTN_TYPE_F32, CVATTN_TYPE_F16 or CVATTN_TYPE_BF16 */
     int32_t         n_seq;
     int32_t         max_nodes;      /* at most CVATTN_TREE_MAX_NODES */
-    int32_t         vocab;
+    int32_t         vocab;          /* at most 2 million */
     void*           workspace;      /* device scratch of cvattn_verify_workspace_size bytes; */
     size_t          workspace_size; /* needs no initialization                               */
 } cvattn_verify_params;
