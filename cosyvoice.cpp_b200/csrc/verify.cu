@@ -83,12 +83,31 @@ template <int T> __device__ __forceinline__ uint4 vector_max(uint4 a, uint4 b) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+__constant__ double kPowers[64] = {  // 2^(i / 64)
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.1023825833078409, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.2021567314527031, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.2553807570246911, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.3396675240533029,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.5590044002378369, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.6457554781539649, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.7186192981224779, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509,
+};
+
 // The rule at one node.
 struct Node {
     float m;             // the largest logit
     float c;             // log2 e / temperature
     float low;           // logits that are not above it have no weight
-    float reach;         // weights of logits this far below the largest: less than 2^-995
+    float reach;         // weights of logits this far below the largest: less than kNothing
     double inv;          // 1 / temperature
     double u64;          // 64 / (temperature ln 2)
     double W;            // sum of the weights (of f32 exponentials)
@@ -100,9 +119,10 @@ struct Node {
         if (!(low < l)) low = nextafterf(l, -INFINITY);
     }
 };
-// exp((l - m) / temperature), l > -infinity finite or a NaN.
-__device__ __forceinline__ float weight32(const Node& x, float l) { return fast_exp2((fmaxf(l, x.low) - x.m) * x.c); }
-// The same in 64 bits, 0 where l is not above x.low or a NaN; m finite.  `table`: 2^(i / 64).
+// exp((l - m) / temperature) in f32, m finite; NaN for a NaN.
+__device__ __forceinline__ float weight32(const Node& x, float l) { return fast_exp2((l - x.m) * x.c); }
+// The same in 64 bits; below kNothing where l is not above x.low or a NaN.  `table`: kPowers.
+constexpr double kNothing = 1e-290;
 __device__ __forceinline__ double weight64(const Node& x, float l, const double* table) {
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: u + magic has u's nearest integer in its low bits
     constexpr double step = 0.010830424696249145;  // ln 2 / 64
@@ -112,13 +132,13 @@ __device__ __forceinline__ double weight64(const Node& x, float l, const double*
     p = fma(p, r, step);
     const double base = table[n & 63];
     p = fma(p * r, base, base);
-    return l > x.low ? __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p)) : 0.0;
+    return __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p));
 }
 // Any l, m.
 __device__ __forceinline__ double weight_any(const Node& x, float l, int v, const double* table) {
     if (x.greedy) return v == x.hot ? 1.0 : 0.0;
     if (l == x.m) return 1.0;
-    return x.m == INFINITY ? 0.0 : weight64(x, l, table);
+    return x.m == INFINITY || !(l > x.low) ? 0.0 : weight64(x, l, table);
 }
 
 __device__ __forceinline__ double warp_add(double x) {
@@ -148,7 +168,7 @@ __device__ __forceinline__ void set_heat(Node& x, float heat) {
     x.inv = x.greedy ? 0.0 : 1.0 / (double)heat;
     x.u64 = x.inv * 92.332482616893656;  // 64 / ln 2
     x.c = (float)fmin(x.inv * 1.4426950408889634, 3.0e38);
-    x.reach = 690.0f * heat;
+    x.reach = 680.0f * heat;
 }
 
 template <int T>
@@ -158,6 +178,7 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const __grid_c
     __shared__ float most[kSumWarps];
     __shared__ double sums[kSumWarps];
     __shared__ int hots[kSumWarps];
+    __shared__ float factor;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slice = blockIdx.x, node = blockIdx.y, s = blockIdx.z;
     griddep_wait();
@@ -190,6 +211,11 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const __grid_c
     }
     m = warp_max(m);
     if (lane == 0) most[warp] = m;
+    if (tid == 0) {
+        Node x;
+        set_heat(x, heat);
+        factor = x.c;
+    }
     __syncthreads();
     m = warp_max(most[lane % kSumWarps]);
     double sum = 0.0;
@@ -215,19 +241,29 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const __grid_c
         sum = same;
         hot = __reduce_min_sync(0xffffffffu, hot);
     } else {
-        Node x;
-        set_heat(x, heat);
-        x.most(m);
+        const float c = factor;
+        const float2 m2 = make_float2(-m, -m), c2 = make_float2(c, c), one = make_float2(1.0f, 1.0f);
+        auto add = [&](uint4 v) {
+            float l[kPer];
+            R::values(v, l);
+            float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < kPer; i += 2) {
+                const float2 d = ffma2(make_float2(l[i], l[i + 1]), one, m2), u = ffma2(d, c2, make_float2(0.f, 0.f));
+                part = ffma2(make_float2(fast_exp2(u.x), fast_exp2(u.y)), one, part);
+            }
+            float w = part.x + part.y;
+            if (w != w) {  // NaN among them: they have no weight
+                w = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) w += l[i] == l[i] ? fast_exp2((l[i] - m) * c) : 0.0f;
+            }
+            sum += w;
+        };
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
-            if (j0 + k * kSumThreads < j1) {
-                float l[kPer], part = 0.0f;
-                R::values(held[k], l);
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) part += weight32(x, l[i]);
-                sum += part;
-            }
-        if (loose >= 0) sum += weight32(x, alone);
+            if (j0 + k * kSumThreads < j1) add(held[k]);
+        if (loose >= 0 && alone == alone) sum += fast_exp2((alone - m) * c);
     }
     sum = warp_add(sum);
     if (lane == 0) {
@@ -259,6 +295,7 @@ struct Shared {
     int parent[kMaxNodes], token[kMaxNodes], first_child[kMaxNodes];
     float u[kMaxNodes];
     float logit[kMaxNodes], prob[kMaxNodes]; // of the drafts' tokens at their parents
+    double weight[kMaxNodes];                // what() of them there, before any refusal
     int bad;
     // what warp 0 has decided
     int what, at, refused;
@@ -267,7 +304,7 @@ struct Shared {
 enum { kScan = 1, kFollow = 2, kStop = 3 };  // Shared::what
 
 template <int T>
-__global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_constant__ cvattn_verify_params p, const Part* parts,
+__global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_constant__ cvattn_verify_params p, const Part* parts,
                                                                   int n_slices, int n_tiles, int* status) {
     using R = Row<T>;
     constexpr int kPer = R::kPer;
@@ -278,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int s = blockIdx.x / C;
-    if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
+    if (tid < 64) sh.table[tid] = kPowers[tid];
     if (tid == 0) sh.bad = 0;
     __syncthreads();
     griddep_wait();
@@ -352,7 +389,14 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
         }
         return;  // (every CTA of the cluster alike)
     }
-    for (int i = 1 + tid; i < n; i += kThreads) atomicMin(&sh.first_child[sh.parent[i]], i);
+    for (int i = 1 + tid; i < n; i += kThreads) {
+        const int up = sh.parent[i];
+        atomicMin(&sh.first_child[up], i);
+        x.most(sh.m[up]);
+        x.hot = sh.hot[up];
+        sh.weight[i] = weight_any(x, sh.logit[i], sh.token[i], sh.table);
+        sh.prob[i] = fmaxf(sh.prob[i], 0.0f);  // (NaN: 0)
+    }
     __syncthreads();
 
     // Warp 0 posts this CTA's numbers to the slots of all CTAs, in turn of two: one is written while the other may still be
@@ -400,54 +444,69 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
         for (int k = 1; k < refused; ++k) r = positive(fma(r, sh.inv_left[k - 1], -g));
         return r;
     };
-    auto what = [&](float l, float qv, int v) {
-        double w = weight_any(x, l, v, sh.table);
+    auto what = [&](double w, float qv, int v) {  // of a token of weight w
         if (!q)
             for (int k = 0; k < refused; ++k) w = v == sh.gone[k] ? 0.0 : w;
         else if (refused) w = less(w, qv);
         return w;
     };
-    // what() of a tile's elements e, e + 1, .. of this lane.  Tile 0 is the row's head (of the first CTA), the last one what its
-    // vectors leave over (of the last CTA).
-    auto tile = [&](int t, int& e, double (&w)[kPer]) {
+    // A tile is one vector a lane: elements e, e + 1, ..  Tile 0 is the row's head (of the first CTA), the last one what its
+    // vectors leave over (of the last CTA), an element a lane.
+    struct Fetched {
+        uint4 v;
+        float g[kPer];
+        int e;      // (-1: nothing)
+    };
+    auto fetch = [&](int t) {
+        Fetched f;
+        f.e = -1;
+        if (t >= tiles) return f;
         if (t == 0 || t == tiles - 1) {
-            e = row.loose(lane);
-            const bool mine = e >= 0 && (t == 0 ? rank == 0 && lane < 16 : rank == C - 1 && lane >= 16);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) w[i] = 0.0;
-            if (mine) w[0] = what(row.one(e), q && refused ? __ldg(q + e) : 0.0f, e);
-            return;
+            const int e = row.loose(lane);
+            if (e >= 0 && (t == 0 ? rank == 0 && lane < 16 : rank == C - 1 && lane >= 16)) {
+                f.e = e;
+                f.v.x = __float_as_uint(row.one(e));
+                f.g[0] = q && refused ? __ldg(q + e) : 0.0f;
+            }
+            return f;
         }
         const int j = j0 + 32 * (t - 1) + lane;
-        e = row.first(j);
-        if (j >= j1) {
+        if (j < j1) {
+            f.e = row.first(j);
+            f.v = row.load(j);
+            if (q && refused) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) w[i] = 0.0;
+                for (int i = 0; i < kPer; ++i) f.g[i] = __ldg(q + f.e + i);
+            }
+        }
+        return f;
+    };
+    auto weigh = [&](int t, const Fetched& f, double (&w)[kPer]) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) w[i] = 0.0;
+        if (f.e < 0) return;
+        if (t == 0 || t == tiles - 1) {
+            w[0] = what(weight_any(x, __uint_as_float(f.v.x), f.e, sh.table), f.g[0], f.e);
             return;
         }
-        const uint4 v = row.load(j);
-        float g[kPer], l[kPer];
-        if (q && refused) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) g[i] = __ldg(q + e + i);
-        }
-        R::values(v, l);
+        float l[kPer];
+        R::values(f.v, l);
         if (simple) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) w[i] = weight64(x, l[i], sh.table);
         } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) w[i] = (x.greedy ? e + i == x.hot : l[i] == x.m) ? 1.0 : 0.0;
+            for (int i = 0; i < kPer; ++i) w[i] = (x.greedy ? f.e + i == x.hot : l[i] == x.m) ? 1.0 : 0.0;
         }
         if (!q)
             for (int k = 0; k < refused; ++k) {
-                const int off = sh.gone[k] - e;
+                const int off = sh.gone[k] - f.e;
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) w[i] = off == i ? 0.0 : w[i];
             }
         if (q && refused) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) w[i] = less(w[i], g[i]);
+            for (int i = 0; i < kPer; ++i) w[i] = less(w[i], f.g[i]);
         }
     };
     double before = 0.0, all = 0.0;    // what() over the CTAs before this one, over the vocabulary (warp 0)
@@ -456,19 +515,20 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
     bool scanned = false;
     int c = 0, order = kStop;
     auto enter = [&](int node) {       // warp 0
-        arrive_at(node);
+        at = node;
         refused = 0;
         total = sh.W[node];
-        exact = !simple;
+        exact = x.greedy || sh.m[node] == INFINITY;
         known = true;
         c = sh.first_child[node];
     };
     if (warp == 0) enter(0);
+    q = p.draft_probs;  // (whether there are any)
     for (;;) {
         if (warp == 0) {
             if (scanned) {
                 known = exact = true;
-                if (refused && !(all > 0.0)) {  // the last refusal left nothing: as it was
+                if (refused && !(all > kNothing)) {  // the last refusal left nothing: as it was
                     --refused;
                     total = was;
                     scanned = false;
@@ -478,22 +538,18 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
                     total = all;
                 }
             }
-            order = kScan;
-            if (scanned && c >= n) order = kFollow;
+            order = scanned && c >= n ? kFollow : kScan;
             // drafts in turn, as long as the sum of what is left is known
             while (order == kScan) {
-                if (x.m == -INFINITY) order = kStop;  // no weight anywhere
+                if (sh.m[at] == -INFINITY) order = kStop;  // no weight anywhere
+                while (c < n && sh.parent[c] != at) ++c;
                 if (order == kStop || c >= n || !known) break;
-                if (sh.parent[c] != at) {
-                    ++c;
-                    continue;
-                }
                 const int t = sh.token[c];
-                const double pt = what(sh.logit[c], sh.prob[c], t);
-                if ((double)sh.u[c] * (double)fmaxf(sh.prob[c], 0.0f) * total < pt) {
+                const double pt = what(sh.weight[c], sh.prob[c], t);
+                if ((double)sh.u[c] * (double)sh.prob[c] * total < pt) {
                     if (lane == 0) {
                         if (rank == 0) accepted[count] = c;
-                        sh.num[count - 1] = x.greedy || sh.logit[c] == x.m ? 0.0 : ((double)sh.logit[c] - (double)x.m) * x.inv;
+                        sh.num[count - 1] = x.greedy || sh.logit[c] == sh.m[at] ? 0.0 : ((double)sh.logit[c] - (double)sh.m[at]) * x.inv;
                         sh.den[count - 1] = sh.W[at];
                     }
                     ++count;
@@ -508,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
                 if (lane == 0) sh.gone[refused] = t;
                 __syncwarp();
                 ++refused;
-                ++c;
+                for (++c; c < n && sh.parent[c] != at;) ++c;
                 was = total;
                 if (q) {
                     known = false;
@@ -527,17 +583,17 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
         __syncthreads();
         order = sh.what;
         if (order != kScan) break;
-        if (warp) {
-            arrive_at(sh.at);
-            refused = sh.refused;
-            inv_W = sh.inv_W;
-        }
+        arrive_at(sh.at);
+        refused = sh.refused;
+        inv_W = sh.inv_W;
         // sums of tiles, of this CTA in the tiles' order, of the cluster
+        Fetched f = fetch(warp);
 #pragma unroll 1
         for (int t = warp; t < tiles; t += kWarps) {
+            const Fetched next = fetch(t + kWarps);
             double w[kPer], sum = 0.0;
-            int e;
-            tile(t, e, w);
+            weigh(t, f, w);
+            f = next;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) sum += w[i];
             sum = warp_add(sum);
@@ -575,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
                     const double z = __shfl_up_sync(0xffffffffu, y, w);
                     if (lane >= w) y += z;
                 }
-                const uint32_t over = __ballot_sync(0xffffffffu, t + lane < tiles && run0 + y > target && v > 0.0);
-                const uint32_t some = __ballot_sync(0xffffffffu, t + lane < tiles && v > 0.0);
+                const uint32_t over = __ballot_sync(0xffffffffu, t + lane < tiles && run0 + y > target && v > kNothing);
+                const uint32_t some = __ballot_sync(0xffffffffu, t + lane < tiles && v > kNothing);
                 if (some) some_tile = t + 31 - __clz(some);
                 if (over) {
                     const int k = __ffs(over) - 1;
@@ -588,9 +644,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
             const bool out_of_reach = first == INT32_MAX;
             const int t = out_of_reach ? some_tile : first;
             if (t >= 0) {
+                const Fetched f = fetch(t);
                 double w[kPer], sum = 0.0;
-                int e;
-                tile(t, e, w);
+                weigh(t, f, w);
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) sum += w[i];
                 double y = sum;
@@ -603,9 +659,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     run1 += w[i];
-                    if (w[i] > 0.0) {
-                        last = e + i;
-                        if (run1 > target && found == INT32_MAX) found = e + i;
+                    if (w[i] > kNothing) {
+                        last = f.e + i;
+                        if (run1 > target && found == INT32_MAX) found = f.e + i;
                     }
                 }
                 found = __reduce_min_sync(0xffffffffu, found);
@@ -649,10 +705,10 @@ __global__ void __launch_bounds__(kThreads, 2) verify_walk_kernel(const __grid_c
     }
 }
 
-// CTAs per sequence of the walk: two tiles a warp at least, and one wave of them in all.
+// CTAs per sequence of the walk: two tiles a warp at least, and one a SM.
 static int cluster_of(int n_seq, int vectors) {
     int c = 1;
-    while (c < kMaxCluster && vectors > c * 2 * kThreads && n_seq * c * 2 <= 2 * 148) c *= 2;
+    while (c < kMaxCluster && vectors > c * 2 * kThreads && n_seq * c * 2 <= 148) c *= 2;
     while (c < kMaxCluster && vectors > c * kMaxTiles * 32) c *= 2;
     return c;
 }
