@@ -6,25 +6,72 @@ namespace cvattn {
 namespace paged {
 
 constexpr int kBookThreads = 1024;
-constexpr int kMaxPools = 48;  // pools of one copy launch (kernel arguments)
+constexpr int kMaxBookCtas = 8;  // of one cluster
+constexpr int kMaxPools = 48;    // pools of one copy launch (kernel arguments)
 
-// Workspace, int32: the next table [n_seq][width], per page its holders, writers and first writer, free pages in order,
-// copies (source, target), their count.
+// Workspace, int32: copies' count; the next table [n_seq][width]; per page its holders, writers and first writer, where it goes
+// or the free pages in order; per sequence what is asked for it; copies (source, target).
+// Where next, refs, writers, lowest and list fit into one CTA's shared memory, they lie there: then the books take one CTA, and
+// what takes a cluster barrier and a trip to L2 otherwise takes a block barrier.  MEASURED
 struct Books {
-    int32_t *next, *refs, *writers, *lowest, *list, *from, *to, *n_copies;
+    int32_t *n_copies, *next, *refs, *writers, *lowest, *list, *src, *keep, *need, *from, *to;
     size_t bytes;
     Books(void* base, int64_t n_seq, int64_t width, int64_t n_pages) {
-        int32_t* w = static_cast<int32_t*>(base);
         const int64_t most = n_pages > n_seq ? n_pages : n_seq;
-        n_copies = w; w += 4;
-        next = w; w += n_seq * width;
-        refs = w; w += n_pages;
-        writers = w; w += n_pages;
-        lowest = w; w += n_pages;
-        list = w; w += n_pages;
-        from = w; w += most;
-        to = w; w += most;
-        bytes = (size_t)(w - static_cast<int32_t*>(base)) * 4;
+        int64_t at = 0;
+        const auto take = [&](int64_t n) {
+            int32_t* p = base ? static_cast<int32_t*>(base) + at : nullptr;
+            at += n;
+            return p;
+        };
+        n_copies = take(4);
+        next = take(n_seq * width);
+        refs = take(n_pages);
+        writers = take(n_pages);
+        lowest = take(n_pages);
+        list = take(n_pages);
+        src = take(n_seq);
+        keep = take(n_seq);
+        need = take(n_seq);
+        from = take(most);
+        to = take(most);
+        bytes = (size_t)at * 4;
+    }
+    // Bytes of the arrays that may lie in shared memory, and their places there.
+    static __host__ __device__ int64_t local_bytes(int64_t entries, int64_t n_pages, int64_t n_seq) { return 4 * (entries + 4 * n_pages + 3 * n_seq); }
+    __device__ __forceinline__ void move_in(int32_t* to, int entries, int n_pages, int n_seq) {
+        next = to;
+        refs = next + entries;
+        writers = refs + n_pages;
+        lowest = writers + n_pages;
+        list = lowest + n_pages;
+        src = list + n_pages;
+        keep = src + n_seq;
+        need = keep + n_seq;
+    }
+};
+constexpr int kLocalBytes = 200 * 1024;
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The CTAs of one cluster keep the books together: what one writes to the workspace the others read after a cluster barrier.
+struct Crew {
+    int C, rank, at, of;  // CTAs, this one; this thread's place among all of theirs, how many
+    __device__ __forceinline__ Crew() {
+        uint32_t c, r;
+        asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(c));
+        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+        C = c;
+        rank = r;
+        at = rank * kBookThreads + threadIdx.x;
+        of = C * kBookThreads;
+    }
+    __device__ __forceinline__ void sync() const {
+        if (C == 1) __syncthreads();
+        else cluster_sync();
     }
 };
 
@@ -41,161 +88,185 @@ __device__ __forceinline__ int block_scan(int x, int& total) {
     __syncthreads();  // (sums may be in use from the call before)
     if (lane == 31) sums[warp] = y;
     __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
-        const int v = sums[w];
-        if (w < warp) before += v;
-        all += v;
+    int v = lane < kBookThreads / 32 ? sums[lane] : 0;
+#pragma unroll
+    for (int w = 1; w < kBookThreads / 32; w <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, v, w);
+        if (lane >= w) v += z;
     }
-    total = all;
-    return before + y - x;
+    total = __shfl_sync(0xffffffffu, v, kBookThreads / 32 - 1);
+    const int before = __shfl_sync(0xffffffffu, v, max(warp, 1) - 1);
+    return (warp ? before : 0) + y - x;
+}
+
+// Exclusive sums over the crew's items in order, `per` neighbouring ones a thread: value(i) of item i gives two numbers, take(i,
+// before) gets the sums before it.  All threads get the totals.
+template <class V, class F> __device__ __forceinline__ int2 crew_scan(const Crew& crew, int n, V value, F take) {
+    __shared__ int2 sums[kMaxBookCtas];
+    const int per = (n + crew.of - 1) / crew.of, i0 = min(n, crew.at * per), i1 = min(n, i0 + per);
+    int a = 0, b = 0, ta, tb;
+    for (int i = i0; i < i1; ++i) {
+        const int2 v = value(i);
+        a += v.x;
+        b += v.y;
+    }
+    a = block_scan(a, ta);
+    b = block_scan(b, tb);
+    if (crew.C > 1) {
+        crew.sync();  // (sums may be in use from the scan before)
+        if ((int)threadIdx.x < crew.C) {
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(&sums[crew.rank])), "r"((int)threadIdx.x));
+            asm volatile("st.shared::cluster.v2.s32 [%0], {%1, %2};" ::"r"(to), "r"(ta), "r"(tb) : "memory");
+        }
+        __syncwarp();
+        crew.sync();
+        ta = tb = 0;
+        for (int k = 0; k < crew.C; ++k) {
+            if (k < crew.rank) {
+                a += sums[k].x;
+                b += sums[k].y;
+            }
+            ta += sums[k].x;
+            tb += sums[k].y;
+        }
+    }
+    for (int i = i0; i < i1; ++i) {
+        const int2 v = value(i);
+        take(i, make_int2(a, b));
+        a += v.x;
+        b += v.y;
+    }
+    return make_int2(ta, tb);
 }
 
 __global__ void __launch_bounds__(kBookThreads) pages_assign_kernel(const __grid_constant__ cvattn_pages_assign_params p, Books w, int P,
-                                                                    int n_pages, int* status) {
+                                                                    int n_pages, int local, int* status) {
+    extern __shared__ int32_t local_books[];
+    const Crew crew;
     griddep_wait();
-    const int tid = threadIdx.x, width = p.table_width;
-    for (int i = tid; i < n_pages; i += kBookThreads) {
+    const int width = p.table_width;
+    if (local) w.move_in(local_books, p.n_seq * width, n_pages, p.n_seq);
+    for (int i = crew.at; i < n_pages; i += crew.of) {
         w.refs[i] = w.writers[i] = 0;
         w.lowest[i] = INT32_MAX;
     }
-    __syncthreads();
-    // kept entries
-    auto wish = [&](int s, int& src, int& keep, int& need) {
-        src = p.src ? p.src[s] : s;
-        keep = p.keep[s];
-        need = p.need[s];
-        const int64_t most = (int64_t)width * P;
+    if (crew.at == 0) *w.n_copies = 0;
+    const int64_t most = (int64_t)width * P;
+    for (int s = crew.at; s < p.n_seq; s += crew.of) {
+        int src = p.src ? p.src[s] : s, keep = p.keep[s], need = p.need[s];
         if (src < 0 || src >= p.n_seq || keep < 0 || keep > most || need < 0 || need > most) {
             record_status(status, kStatusBadLength);
             src = s;
             keep = need = 0;
         }
-    };
-    for (int64_t i = tid; i < (int64_t)p.n_seq * width; i += kBookThreads) {
-        const int s = (int)(i / width), j = (int)(i % width);
-        int src, keep, need, page = -1;
-        wish(s, src, keep, need);
+        w.src[s] = src;
+        w.keep[s] = keep;
+        w.need[s] = need;
+    }
+    crew.sync();
+    // kept entries, and who writes into a partly filled page
+#pragma unroll 4
+    for (int i = crew.at; i < p.n_seq * width; i += crew.of) {
+        const int s = i / width, j = i - s * width, keep = w.keep[s], need = w.need[s];
+        int page = -1;
         if (j < (keep + P - 1) / P) {
-            page = page_of(p.table + src * p.table_nb_seq, j, n_pages);
-            if (page < 0) record_status(status, kStatusBadPage);
-            else atomicAdd(&w.refs[page], 1);
+            page = page_of(p.table + w.src[s] * p.table_nb_seq, j, n_pages);
+            if (page < 0) {
+                record_status(status, kStatusBadPage);
+            } else {
+                atomicAdd(&w.refs[page], 1);
+                if (need > keep && keep % P && j == keep / P) {
+                    atomicAdd(&w.writers[page], 1);
+                    atomicMin(&w.lowest[page], s);
+                }
+            }
         }
         w.next[i] = page;
     }
-    __syncthreads();
-    // who writes into a shared tail
-    auto tail_of = [&](int s, int keep, int need) {
-        return need > keep && keep % P ? w.next[(int64_t)s * width + keep / P] : -1;
-    };
-    for (int s = tid; s < p.n_seq; s += kBookThreads) {
-        int src, keep, need;
-        wish(s, src, keep, need);
-        const int tail = tail_of(s, keep, need);
-        if (tail >= 0) {
-            atomicAdd(&w.writers[tail], 1);
-            atomicMin(&w.lowest[tail], s);
-        }
-    }
-    __syncthreads();
+    crew.sync();
     // free pages in order
-    int n_free = 0;
-    for (int i0 = 0; i0 < n_pages; i0 += kBookThreads) {
-        const int i = i0 + tid;
-        const int is = i < n_pages && w.refs[i] == 0;
-        int total;
-        const int at = n_free + block_scan(is, total);
-        if (is) w.list[at] = i;
-        n_free += total;
-    }
-    __syncthreads();
-    // sequence by sequence
-    int asked = 0, copied = 0;
-    for (int s0 = 0; s0 < p.n_seq; s0 += kBookThreads) {
-        const int s = s0 + tid;
-        int src, keep = 0, need = 0, tail = -1, copies = 0, fresh = 0;
-        if (s < p.n_seq) {
-            wish(s, src, keep, need);
-            tail = tail_of(s, keep, need);
-            copies = tail >= 0 && w.refs[tail] > 1 && !(w.writers[tail] == w.refs[tail] && w.lowest[tail] == s);
-            fresh = max(0, (need + P - 1) / P - (keep + P - 1) / P) + copies;
-        }
-        int total;
-        const int before = asked + block_scan(fresh, total);
-        asked += total;
-        const bool granted = before + fresh <= n_free;
-        const int which = copied + block_scan(granted ? copies : 0, total);
-        copied += total;
-        if (s < p.n_seq) {
-            p.room[s] = granted ? max(keep, need) : keep;
-            if (granted) {
-                if (copies) {
-                    w.from[which] = tail;
-                    w.to[which] = w.list[before];
-                }
-                for (int k = 0; k < fresh; ++k) w.next[(int64_t)s * width + (keep + P - 1) / P - copies + k] = w.list[before + k];
-            }
-        }
-    }
-    if (tid == 0) *w.n_copies = copied;
-    __syncthreads();
-    for (int64_t i = tid; i < (int64_t)p.n_seq * width; i += kBookThreads) p.table_out[i / width * p.table_nb_seq + i % width] = w.next[i];
+    const int n_free = crew_scan(crew, n_pages, [&](int i) { return make_int2(w.refs[i] == 0, 0); },
+                                 [&](int i, int2 before) {
+                                     if (w.refs[i] == 0) w.list[before.x] = i;
+                                 }).x;
+    crew.sync();
+    // sequence by sequence: the pages that it asks for, and whether it copies its tail
+    auto asks = [&](int s, int& keep, int& need, int& tail) {
+        keep = w.keep[s];
+        need = w.need[s];
+        tail = need > keep && keep % P ? w.next[(int64_t)s * width + keep / P] : -1;
+        const int copies = tail >= 0 && w.refs[tail] > 1 && !(w.writers[tail] == w.refs[tail] && w.lowest[tail] == s);
+        return make_int2(max(0, (need + P - 1) / P - (keep + P - 1) / P) + copies, copies);
+    };
+    int keep, need, tail;
+    // (those without room come after all with room that ask for anything, so the copies before one with room have room too)
+    crew_scan(crew, p.n_seq, [&](int s) { return asks(s, keep, need, tail); },
+              [&](int s, int2 before) {
+                  const int2 v = asks(s, keep, need, tail);
+                  const bool granted = before.x + v.x <= n_free;
+                  p.room[s] = granted ? max(keep, need) : keep;
+                  if (!granted) return;
+                  if (v.y) {
+                      w.from[before.y] = tail;
+                      w.to[before.y] = w.list[before.x];
+                      atomicMax(w.n_copies, before.y + 1);
+                  }
+                  const int first = (keep + P - 1) / P - v.y;
+                  for (int k = 0; k < v.x; ++k) w.next[(int64_t)s * width + first + k] = w.list[before.x + k];
+              });
+    crew.sync();
+    for (int i = crew.at; i < p.n_seq * width; i += crew.of) p.table_out[(int64_t)(i / width) * p.table_nb_seq + i % width] = w.next[i];
     if (p.refs) {
-        for (int i = tid; i < n_pages; i += kBookThreads) p.refs[i] = 0;
-        __syncthreads();
-        for (int64_t i = tid; i < (int64_t)p.n_seq * width; i += kBookThreads)
-            if (w.next[i] >= 0) atomicAdd(&p.refs[w.next[i]], 1);
+        int32_t* refs = local ? w.refs : p.refs;
+        for (int i = crew.at; i < n_pages; i += crew.of) refs[i] = 0;
+        crew.sync();
+        for (int i = crew.at; i < p.n_seq * width; i += crew.of)
+            if (w.next[i] >= 0) atomicAdd(&refs[w.next[i]], 1);
+        if (local) {
+            crew.sync();
+            for (int i = crew.at; i < n_pages; i += crew.of) p.refs[i] = refs[i];
+        }
     }
 }
 
 __global__ void __launch_bounds__(kBookThreads) pages_compact_kernel(const __grid_constant__ cvattn_pages_compact_params p, Books w,
-                                                                     int n_pages, int* status) {
+                                                                     int n_pages, int local, int* status) {
+    extern __shared__ int32_t local_books[];
+    const Crew crew;
     griddep_wait();
-    const int tid = threadIdx.x, width = p.table_width;
-    for (int i = tid; i < n_pages; i += kBookThreads) w.refs[i] = 0;
-    __syncthreads();
-    for (int64_t i = tid; i < (int64_t)p.n_seq * width; i += kBookThreads) {
-        const int page = page_of(p.table + i / width * p.table_nb_seq, (int)(i % width), n_pages);
+    const int width = p.table_width;
+    if (local) w.move_in(local_books, p.n_seq * width, n_pages, p.n_seq);
+    for (int i = crew.at; i < n_pages; i += crew.of) w.refs[i] = 0;
+    crew.sync();
+    for (int i = crew.at; i < p.n_seq * width; i += crew.of) {
+        const int page = page_of(p.table + (int64_t)(i / width) * p.table_nb_seq, i % width, n_pages);
+        w.next[i] = page;
         if (page >= 0) atomicAdd(&w.refs[page], 1);
     }
-    __syncthreads();
-    int live = 0;
-    for (int i0 = 0; i0 < n_pages; i0 += kBookThreads) {
-        const int i = i0 + tid;
-        int total;
-        block_scan(i < n_pages && w.refs[i] > 0, total);
-        live += total;
-    }
-    int moved = 0, free = 0;
-    for (int i0 = 0; i0 < n_pages; i0 += kBookThreads) {
-        const int i = i0 + tid;
-        const bool real = i < n_pages, held = real && w.refs[i] > 0;
-        int total;
-        int at = moved + block_scan(held && i >= live, total);
-        moved += total;
-        if (held && i >= live) w.from[at] = i;
-        at = free + block_scan(real && !held && i < live, total);
-        free += total;
-        if (real && !held && i < live) w.to[at] = i;
-        if (real) w.list[i] = i;  // where a page goes
-    }
-    __syncthreads();
-    for (int i = tid; i < moved; i += kBookThreads) w.list[w.from[i]] = w.to[i];
-    if (tid == 0) {
+    crew.sync();
+    const int live = crew_scan(crew, n_pages, [&](int i) { return make_int2(w.refs[i] > 0, 0); }, [](int, int2) {}).x;
+    // the k-th held page from `live` on goes to the k-th free one below it
+    const int moved = crew_scan(crew, n_pages, [&](int i) { return make_int2(w.refs[i] > 0 && i >= live, w.refs[i] == 0 && i < live); },
+                                [&](int i, int2 before) {
+                                    if (w.refs[i] > 0 && i >= live) w.from[before.x] = i;
+                                    if (w.refs[i] == 0 && i < live) w.to[before.y] = i;
+                                    w.list[i] = i;
+                                }).x;
+    crew.sync();
+    for (int i = crew.at; i < moved; i += crew.of) w.list[w.from[i]] = w.to[i];
+    if (crew.at == 0) {
         *w.n_copies = moved;
         *p.n_live = live;
     }
-    __syncthreads();
-    for (int64_t i = tid; i < (int64_t)p.n_seq * width; i += kBookThreads) {
-        const int page = page_of(p.table + i / width * p.table_nb_seq, (int)(i % width), n_pages);
-        p.table_out[i / width * p.table_nb_seq + i % width] = page < 0 ? -1 : w.list[page];
-    }
-    if (p.refs) {
-        for (int i = tid; i < n_pages; i += kBookThreads) p.refs[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < n_pages; i += kBookThreads)
+    if (p.refs)
+        for (int i = crew.at; i < n_pages; i += crew.of) p.refs[i] = 0;
+    crew.sync();
+    for (int i = crew.at; i < p.n_seq * width; i += crew.of)
+        p.table_out[(int64_t)(i / width) * p.table_nb_seq + i % width] = w.next[i] < 0 ? -1 : w.list[w.next[i]];
+    if (p.refs)
+        for (int i = crew.at; i < n_pages; i += crew.of)
             if (w.refs[i] > 0) p.refs[w.list[i]] = w.refs[i];
-    }
 }
 
 // Page from[c] of every pool to page to[c].
@@ -208,16 +279,28 @@ struct CopyArgs {
     int n;  // tensors: keys and values of each pool
 };
 
-__global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__ CopyArgs a) {
+// A warp takes 2 KB of a page of one tensor at a time, four 16-byte loads a lane before the first store.  Bound by memory:
+// MEASURED.
+constexpr int kCopyThreads = 256, kPiece = 2048;
+
+__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_constant__ CopyArgs a) {
     griddep_wait();
-    const int64_t n = (int64_t)*a.n_copies * a.n;
-    for (int64_t u = blockIdx.x; u < n; u += gridDim.x) {
-        const int c = (int)(u / a.n), t = (int)(u % a.n), pool = t >> 1;
+    const int t = blockIdx.y, pool = t >> 1, lane = threadIdx.x & 31;
+    const int pieces = (a.bytes[pool] + kPiece - 1) / kPiece, n = *a.n_copies * pieces;
+    for (int u = blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); u < n; u += gridDim.x * (kCopyThreads / 32)) {
+        const int c = u / pieces, at = (u - c * pieces) * kPiece + lane * 16;
         const int64_t from = a.from[c], to = a.to[c];
-        const uint4* src = reinterpret_cast<const uint4*>(a.data[t] + from * a.nb_page[pool]);
-        uint4* dst = reinterpret_cast<uint4*>(a.data[t] + to * a.nb_page[pool]);
-        for (int i = threadIdx.x; i < a.bytes[pool] / 16; i += 256) dst[i] = src[i];
-        for (int i = threadIdx.x; i < a.scales[pool]; i += 256) a.scale[t][to * a.nb_scale[pool] + i] = a.scale[t][from * a.nb_scale[pool] + i];
+        const uint8_t* src = a.data[t] + from * a.nb_page[pool] + at;
+        uint8_t* dst = a.data[t] + to * a.nb_page[pool] + at;
+        uint4 v[kPiece / 512];
+#pragma unroll
+        for (int i = 0; i < kPiece / 512; ++i)
+            if (at + i * 512 < a.bytes[pool]) v[i] = __ldcs(reinterpret_cast<const uint4*>(src + i * 512));
+#pragma unroll
+        for (int i = 0; i < kPiece / 512; ++i)
+            if (at + i * 512 < a.bytes[pool]) *reinterpret_cast<uint4*>(dst + i * 512) = v[i];
+        if (u == c * pieces)
+            for (int i = lane; i < a.scales[pool]; i += 32) a.scale[t][to * a.nb_scale[pool] + i] = a.scale[t][from * a.nb_scale[pool] + i];
     }
 }
 
@@ -240,7 +323,8 @@ static cudaError_t copy_pages(cudaStream_t stream, const cvattn_page_pool* pools
         a.to = w.to;
         a.n_copies = w.n_copies;
         a.n = 2 * n;
-        const cudaError_t e = launch_overlapped(pages_copy_kernel, 148 * 4, 256, 0, stream, a);
+        const int ctas = (148 * 8 + a.n - 1) / a.n;
+        const cudaError_t e = launch_overlapped(pages_copy_kernel, dim3((unsigned)ctas, (unsigned)a.n), kCopyThreads, 0, stream, a);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -250,15 +334,42 @@ static cudaError_t copy_pages(cudaStream_t stream, const cvattn_page_pool* pools
 
 size_t pages_workspace_bytes(int n_seq, int table_width, int n_pages) { return paged::Books(nullptr, n_seq, table_width, n_pages).bytes; }
 
+// Whether the books lie in shared memory, and else the CTAs that keep them: four entries or pages a thread at least.
+static int book_ctas(int64_t entries, int n_pages, int n_seq, int& local) {
+    local = paged::Books::local_bytes(entries, n_pages, n_seq) <= paged::kLocalBytes;
+    const int64_t items = entries > n_pages ? entries : n_pages;
+    int c = 1;
+    while (!local && c < paged::kMaxBookCtas && items > (int64_t)c * 4 * paged::kBookThreads) c *= 2;
+    return c;
+}
+
+template <class Fn> static cudaError_t allow_local(Fn* fn) {
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::kLocalBytes);
+}
+
 cudaError_t launch_pages_assign(cudaStream_t stream, const cvattn_pages_assign_params& p, int page_size, int n_pages, int* status) {
     const paged::Books w(p.workspace, p.n_seq, p.table_width, n_pages);
-    const cudaError_t e = launch_overlapped(paged::pages_assign_kernel, 1, paged::kBookThreads, 0, stream, p, w, page_size, n_pages, status);
+    const int64_t entries = (int64_t)p.n_seq * p.table_width;
+    int local;
+    const int c = book_ctas(entries, n_pages, p.n_seq, local);
+    const size_t smem = local ? (size_t)paged::Books::local_bytes(entries, n_pages, p.n_seq) : 0;
+    cudaError_t e = allow_local(paged::pages_assign_kernel);
+    if (e == cudaSuccess)
+        e = launch_overlapped_clusters(paged::pages_assign_kernel, dim3((unsigned)c), paged::kBookThreads, smem, c, stream, p, w, page_size, n_pages,
+                                       local, status);
     return e != cudaSuccess ? e : paged::copy_pages(stream, p.pools, p.n_pools, w);
 }
 
 cudaError_t launch_pages_compact(cudaStream_t stream, const cvattn_pages_compact_params& p, int n_pages, int* status) {
     const paged::Books w(p.workspace, p.n_seq, p.table_width, n_pages);
-    const cudaError_t e = launch_overlapped(paged::pages_compact_kernel, 1, paged::kBookThreads, 0, stream, p, w, n_pages, status);
+    const int64_t entries = (int64_t)p.n_seq * p.table_width;
+    int local;
+    const int c = book_ctas(entries, n_pages, p.n_seq, local);
+    const size_t smem = local ? (size_t)paged::Books::local_bytes(entries, n_pages, p.n_seq) : 0;
+    cudaError_t e = allow_local(paged::pages_compact_kernel);
+    if (e == cudaSuccess)
+        e = launch_overlapped_clusters(paged::pages_compact_kernel, dim3((unsigned)c), paged::kBookThreads, smem, c, stream, p, w, n_pages, local,
+                                       status);
     return e != cudaSuccess ? e : paged::copy_pages(stream, p.pools, p.n_pools, w);
 }
 
