@@ -5,7 +5,7 @@
 namespace cvattn {
 namespace paged {
 
-constexpr int kBookThreads = 1024;
+constexpr int kBookThreads = 1024;  // (block_scan: 32 warps)
 constexpr int kMaxBookCtas = 8;  // of one cluster
 constexpr int kMaxPools = 48;    // pools of one copy launch (kernel arguments)
 
@@ -58,61 +58,66 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // The CTAs of one cluster keep the books together: what one writes to the workspace the others read after a cluster barrier.
-struct Crew {
+// With the books in shared memory there is one CTA (kLocal, apart so that its code is short: run once, it is bound by fetching its
+// instructions).
+template <bool kLocal> struct Crew {
     int C, rank, at, of;  // CTAs, this one; this thread's place among all of theirs, how many
     __device__ __forceinline__ Crew() {
-        uint32_t c, r;
-        asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(c));
-        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+        uint32_t c = 1, r = 0;
+        if (!kLocal) {
+            asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(c));
+            asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+        }
         C = c;
         rank = r;
         at = rank * kBookThreads + threadIdx.x;
         of = C * kBookThreads;
     }
     __device__ __forceinline__ void sync() const {
-        if (C == 1) __syncthreads();
+        if (kLocal) __syncthreads();
         else cluster_sync();
     }
 };
 
-// Exclusive sum over the block of one number a thread; every thread gets the total too.
-__device__ __forceinline__ int block_scan(int x, int& total) {
-    __shared__ int sums[32];
+// Exclusive sums over the block of two numbers a thread, and their totals.  (Packed in 64 bits: one pass.)
+__device__ __forceinline__ void block_scan(int& a, int& b, int& total_a, int& total_b) {
+    __shared__ long long sums[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int y = x;
+    const long long x = (long long)a << 32 | b;
+    auto scan = [&](long long y) {
 #pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, y, w);
-        if (lane >= w) y += z;
-    }
+        for (int w = 1; w < 32; w <<= 1) {
+            const long long z = __shfl_up_sync(0xffffffffu, y, w);
+            if (lane >= w) y += z;
+        }
+        return y;
+    };
+    long long y = scan(x);
     __syncthreads();  // (sums may be in use from the call before)
     if (lane == 31) sums[warp] = y;
     __syncthreads();
-    int v = lane < kBookThreads / 32 ? sums[lane] : 0;
-#pragma unroll
-    for (int w = 1; w < kBookThreads / 32; w <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, v, w);
-        if (lane >= w) v += z;
-    }
-    total = __shfl_sync(0xffffffffu, v, kBookThreads / 32 - 1);
-    const int before = __shfl_sync(0xffffffffu, v, max(warp, 1) - 1);
-    return (warp ? before : 0) + y - x;
+    const long long v = scan(sums[lane]), all = __shfl_sync(0xffffffffu, v, 31), before = __shfl_sync(0xffffffffu, v, max(warp, 1) - 1);
+    y += (warp ? before : 0) - x;
+    a = (int)(y >> 32);
+    b = (int)y;
+    total_a = (int)(all >> 32);
+    total_b = (int)all;
 }
 
 // Exclusive sums over the crew's items in order, `per` neighbouring ones a thread: value(i) of item i gives two numbers, take(i,
 // before) gets the sums before it.  All threads get the totals.
-template <class V, class F> __device__ __forceinline__ int2 crew_scan(const Crew& crew, int n, V value, F take) {
+template <bool kLocal, class V, class F> __device__ __forceinline__ int2 crew_scan(const Crew<kLocal>& crew, int n, V value, F take) {
     __shared__ int2 sums[kMaxBookCtas];
     const int per = (n + crew.of - 1) / crew.of, i0 = min(n, crew.at * per), i1 = min(n, i0 + per);
     int a = 0, b = 0, ta, tb;
+#pragma unroll 1
     for (int i = i0; i < i1; ++i) {
         const int2 v = value(i);
         a += v.x;
         b += v.y;
     }
-    a = block_scan(a, ta);
-    b = block_scan(b, tb);
-    if (crew.C > 1) {
+    block_scan(a, b, ta, tb);
+    if (!kLocal) {
         crew.sync();  // (sums may be in use from the scan before)
         if ((int)threadIdx.x < crew.C) {
             uint32_t to;
@@ -131,6 +136,7 @@ template <class V, class F> __device__ __forceinline__ int2 crew_scan(const Crew
             tb += sums[k].y;
         }
     }
+#pragma unroll 1
     for (int i = i0; i < i1; ++i) {
         const int2 v = value(i);
         take(i, make_int2(a, b));
@@ -140,19 +146,22 @@ template <class V, class F> __device__ __forceinline__ int2 crew_scan(const Crew
     return make_int2(ta, tb);
 }
 
+template <bool kLocal>
 __global__ void __launch_bounds__(kBookThreads) pages_assign_kernel(const __grid_constant__ cvattn_pages_assign_params p, Books w, int P,
-                                                                    int n_pages, int local, int* status) {
+                                                                    int n_pages, int* status) {
     extern __shared__ int32_t local_books[];
-    const Crew crew;
+    const Crew<kLocal> crew;
     griddep_wait();
     const int width = p.table_width;
-    if (local) w.move_in(local_books, p.n_seq * width, n_pages, p.n_seq);
+    if (kLocal) w.move_in(local_books, p.n_seq * width, n_pages, p.n_seq);
+#pragma unroll 1
     for (int i = crew.at; i < n_pages; i += crew.of) {
         w.refs[i] = w.writers[i] = 0;
         w.lowest[i] = INT32_MAX;
     }
     if (crew.at == 0) *w.n_copies = 0;
     const int64_t most = (int64_t)width * P;
+#pragma unroll 1
     for (int s = crew.at; s < p.n_seq; s += crew.of) {
         int src = p.src ? p.src[s] : s, keep = p.keep[s], need = p.need[s];
         if (src < 0 || src >= p.n_seq || keep < 0 || keep > most || need < 0 || need > most) {
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_assign_kernel(const __grid
     }
     crew.sync();
     // kept entries, and who writes into a partly filled page
-#pragma unroll 4
+#pragma unroll 2
     for (int i = crew.at; i < p.n_seq * width; i += crew.of) {
         const int s = i / width, j = i - s * width, keep = w.keep[s], need = w.need[s];
         int page = -1;
@@ -213,30 +222,36 @@ __global__ void __launch_bounds__(kBookThreads) pages_assign_kernel(const __grid
                       atomicMax(w.n_copies, before.y + 1);
                   }
                   const int first = (keep + P - 1) / P - v.y;
+#pragma unroll 1
                   for (int k = 0; k < v.x; ++k) w.next[(int64_t)s * width + first + k] = w.list[before.x + k];
               });
     crew.sync();
+#pragma unroll 1
     for (int i = crew.at; i < p.n_seq * width; i += crew.of) p.table_out[(int64_t)(i / width) * p.table_nb_seq + i % width] = w.next[i];
     if (p.refs) {
-        int32_t* refs = local ? w.refs : p.refs;
+        int32_t* refs = kLocal ? w.refs : p.refs;
+#pragma unroll 1
         for (int i = crew.at; i < n_pages; i += crew.of) refs[i] = 0;
         crew.sync();
+#pragma unroll 1
         for (int i = crew.at; i < p.n_seq * width; i += crew.of)
             if (w.next[i] >= 0) atomicAdd(&refs[w.next[i]], 1);
-        if (local) {
+        if (kLocal) {
             crew.sync();
+#pragma unroll 1
             for (int i = crew.at; i < n_pages; i += crew.of) p.refs[i] = refs[i];
         }
     }
 }
 
+template <bool kLocal>
 __global__ void __launch_bounds__(kBookThreads) pages_compact_kernel(const __grid_constant__ cvattn_pages_compact_params p, Books w,
-                                                                     int n_pages, int local, int* status) {
+                                                                     int n_pages, int* status) {
     extern __shared__ int32_t local_books[];
-    const Crew crew;
+    const Crew<kLocal> crew;
     griddep_wait();
     const int width = p.table_width;
-    if (local) w.move_in(local_books, p.n_seq * width, n_pages, p.n_seq);
+    if (kLocal) w.move_in(local_books, p.n_seq * width, n_pages, p.n_seq);
     for (int i = crew.at; i < n_pages; i += crew.of) w.refs[i] = 0;
     crew.sync();
     for (int i = crew.at; i < p.n_seq * width; i += crew.of) {
@@ -334,42 +349,37 @@ static cudaError_t copy_pages(cudaStream_t stream, const cvattn_page_pool* pools
 
 size_t pages_workspace_bytes(int n_seq, int table_width, int n_pages) { return paged::Books(nullptr, n_seq, table_width, n_pages).bytes; }
 
-// Whether the books lie in shared memory, and else the CTAs that keep them: four entries or pages a thread at least.
-static int book_ctas(int64_t entries, int n_pages, int n_seq, int& local) {
-    local = paged::Books::local_bytes(entries, n_pages, n_seq) <= paged::kLocalBytes;
+// CTAs that keep books in the workspace: four entries or pages a thread at least.
+static int book_ctas(int64_t entries, int n_pages) {
     const int64_t items = entries > n_pages ? entries : n_pages;
     int c = 1;
-    while (!local && c < paged::kMaxBookCtas && items > (int64_t)c * 4 * paged::kBookThreads) c *= 2;
+    while (c < paged::kMaxBookCtas && items > (int64_t)c * 4 * paged::kBookThreads) c *= 2;
     return c;
 }
 
-template <class Fn> static cudaError_t allow_local(Fn* fn) {
-    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::kLocalBytes);
+// One of two kernels: with the books in shared memory where they fit, or by a cluster.
+template <class Local, class Crewed, class... A>
+static cudaError_t keep_books(Local* local, Crewed* crewed, cudaStream_t stream, int64_t entries, int n_pages, int n_seq, const A&... args) {
+    const int64_t bytes = paged::Books::local_bytes(entries, n_pages, n_seq);
+    if (bytes <= paged::kLocalBytes) {
+        const cudaError_t e = cudaFuncSetAttribute(local, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::kLocalBytes);
+        return e != cudaSuccess ? e : launch_overlapped(local, dim3(1), paged::kBookThreads, (size_t)bytes, stream, args...);
+    }
+    const int c = book_ctas(entries, n_pages);
+    return launch_overlapped_clusters(crewed, dim3((unsigned)c), paged::kBookThreads, 0, c, stream, args...);
 }
 
 cudaError_t launch_pages_assign(cudaStream_t stream, const cvattn_pages_assign_params& p, int page_size, int n_pages, int* status) {
     const paged::Books w(p.workspace, p.n_seq, p.table_width, n_pages);
-    const int64_t entries = (int64_t)p.n_seq * p.table_width;
-    int local;
-    const int c = book_ctas(entries, n_pages, p.n_seq, local);
-    const size_t smem = local ? (size_t)paged::Books::local_bytes(entries, n_pages, p.n_seq) : 0;
-    cudaError_t e = allow_local(paged::pages_assign_kernel);
-    if (e == cudaSuccess)
-        e = launch_overlapped_clusters(paged::pages_assign_kernel, dim3((unsigned)c), paged::kBookThreads, smem, c, stream, p, w, page_size, n_pages,
-                                       local, status);
+    const cudaError_t e = keep_books(paged::pages_assign_kernel<true>, paged::pages_assign_kernel<false>, stream, (int64_t)p.n_seq * p.table_width,
+                                     n_pages, p.n_seq, p, w, page_size, n_pages, status);
     return e != cudaSuccess ? e : paged::copy_pages(stream, p.pools, p.n_pools, w);
 }
 
 cudaError_t launch_pages_compact(cudaStream_t stream, const cvattn_pages_compact_params& p, int n_pages, int* status) {
     const paged::Books w(p.workspace, p.n_seq, p.table_width, n_pages);
-    const int64_t entries = (int64_t)p.n_seq * p.table_width;
-    int local;
-    const int c = book_ctas(entries, n_pages, p.n_seq, local);
-    const size_t smem = local ? (size_t)paged::Books::local_bytes(entries, n_pages, p.n_seq) : 0;
-    cudaError_t e = allow_local(paged::pages_compact_kernel);
-    if (e == cudaSuccess)
-        e = launch_overlapped_clusters(paged::pages_compact_kernel, dim3((unsigned)c), paged::kBookThreads, smem, c, stream, p, w, n_pages, local,
-                                       status);
+    const cudaError_t e = keep_books(paged::pages_compact_kernel<true>, paged::pages_compact_kernel<false>, stream, (int64_t)p.n_seq * p.table_width,
+                                     n_pages, p.n_seq, p, w, n_pages, status);
     return e != cudaSuccess ? e : paged::copy_pages(stream, p.pools, p.n_pools, w);
 }
 
