@@ -1,6 +1,9 @@
 // paged_attention.cu -- the join of splits and the host side of attention over a paged 8-bit cache.
 #include "launch.cuh"
-#include "paged_mma.cuh"
+#include "paged_tc.cuh"
+#ifndef KNOB
+#define KNOB(n, d) d
+#endif
 
 namespace cvattn {
 namespace paged {
@@ -64,12 +67,19 @@ constexpr int kSms = 148;
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Plan {
+    int tc_grid;   // > 0: the tcgen05 kernel on that many CTAs
     int R, row_tiles, cluster, n_splits;
 };
 
 static Plan plan_of(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
     Plan p{};
     const int64_t rows = (int64_t)max_q * (n_q_heads / n_kv_heads);
+    const int64_t tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile), entries = tiles * ((rows + kTcRows - 1) / kTcRows);
+    if (rows >= KNOB(XROWS, 40) && tiles * rows >= KNOB(XWORK, 1024) && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
+        p.tc_grid = (int)(entries < kSms ? entries : kSms);
+        p.n_splits = p.tc_grid / (int64_t)(n_seq * n_kv_heads) > 0 ? p.tc_grid / (n_seq * n_kv_heads) : 1;  // (for the combine)
+        return p;
+    }
     p.R = rows <= 8 ? 1 : 2;
     p.row_tiles = (int)((rows + 8 * p.R * kMmaWarps - 1) / (8 * p.R * kMmaWarps));
     const int64_t units = (int64_t)n_seq * n_kv_heads * p.row_tiles, blocks = (max_kv_len + kBlock - 1) / kBlock;
@@ -79,6 +89,18 @@ static Plan plan_of(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_k
     while (p.cluster < kMaxCluster && 2 * p.cluster <= want) p.cluster *= 2;
     p.n_splits = want > p.cluster ? (int)(want / p.cluster) : 1;
     return p;
+}
+
+template <int F> static cudaError_t launch_tc(cudaStream_t stream, const TcAttArgs& ta) {
+    auto* fn = paged_tc_kernel<F>;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem::kBytes);
+    return e != cudaSuccess ? e : launch_overlapped(fn, dim3((unsigned)ta.grid), kTcThreads, TcSmem::kBytes, stream, ta);
+}
+
+template <int kLanes> static cudaError_t run_tc_combine(cudaStream_t stream, const TcAttArgs& ta) {
+    const int rows = ta.a.p.max_q * ta.a.G;
+    const dim3 grid((unsigned)((rows + 16 / kLanes - 1) / (16 / kLanes)), (unsigned)ta.a.p.pool.n_heads, (unsigned)ta.a.p.n_seq);
+    return launch_overlapped(paged_tc_combine_kernel<kLanes>, grid, 256, 0, stream, ta);
 }
 
 template <int F, int R> static cudaError_t launch_mma(cudaStream_t stream, const AttArgs& a, const Plan& plan) {
@@ -101,6 +123,7 @@ template <int kLanes> static cudaError_t run_combine(cudaStream_t stream, const 
 size_t paged_attention_workspace_bytes(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
     using namespace paged;
     const Plan p = plan_of(n_seq, max_q, max_kv_len, n_q_heads, n_kv_heads);
+    if (p.tc_grid) return align256((size_t)(n_seq + 1) * 4) + (size_t)2 * p.tc_grid * kTcRows * (kD + 2) * 4;
     if (p.n_splits == 1) return 0;
     const size_t rows = (size_t)n_seq * p.n_splits * max_q * n_q_heads;
     return align256(rows * 2 * 4) + rows * kD * 4;
@@ -116,6 +139,18 @@ cudaError_t launch_paged_attention(cudaStream_t stream, const cvattn_paged_atten
     a.status = status;
     const Plan plan = plan_of(p.n_seq, p.max_q, p.max_kv_len, p.n_q_heads, p.pool.n_heads);
     a.n_splits = plan.n_splits;
+    if (plan.tc_grid) {
+        TcAttArgs ta{};
+        ta.a = a;
+        ta.grid = plan.tc_grid;
+        uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+        ta.ws_pref = reinterpret_cast<int32_t*>(ws);
+        ta.ws_o = reinterpret_cast<float*>(ws + align256((size_t)(p.n_seq + 1) * 4));
+        ta.ws_ml = ta.ws_o + (size_t)2 * ta.grid * kTcRows * kD;
+        const cudaError_t e = p.pool.format == kI8 ? launch_tc<kI8>(stream, ta) : launch_tc<kE4M3>(stream, ta);
+        if (e != cudaSuccess) return e;
+        return plan.n_splits > 24 ? run_tc_combine<16>(stream, ta) : plan.n_splits > 4 ? run_tc_combine<4>(stream, ta) : run_tc_combine<1>(stream, ta);
+    }
     if (plan.n_splits > 1) {
         const size_t rows = (size_t)p.n_seq * plan.n_splits * p.max_q * p.n_q_heads;
         a.ws_ml = static_cast<float*>(p.workspace);

@@ -1,0 +1,765 @@
+// paged_tc.cuh -- paged attention of many rows on the 5th-generation tensor cores (tcgen05).
+//
+// Work is cut evenly: the key tiles (128 positions) of all units (sequence, tile of 128 rows, KV head), each unit up to the
+// last position that one of its rows sees, form one list, and CTA c of G takes the entries [c N / G, (c + 1) N / G).  A run is
+// the part of one unit that a CTA has; a whole unit is written out directly, parts go to the workspace and
+// paged_tc_combine_kernel joins them.
+//   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the CTA's tiles 2 k + g
+//   warps 8-11      producer of the K tiles, 12-15 of the V tiles: codes from the pages to registers one tile ahead (table
+//                   entries two), f16 into shared memory (128B swizzle), V transposed as its blocks lie
+//   warp 16         issues S = Q K^T, up to two tiles ahead of the softmax;  warp 17 issues O = P V
+//   (warps 18, 19 only complete the last warpgroup)
+// Precision: codes are exact in f16, Q and P' = P w are split in f16 hi + lo, so S = Qh K + Ql K and O = Ph V + Pl V.  A block's
+// key scale multiplies its 16 columns of S; its value scale, over a power of two of the tile, is w, which leaves P' with what is
+// above 2^-22 of the largest of the tile.  The output of a tile is a fresh accumulator, added in f32 to the row's registers: adds
+// inside the tensor cores truncate.
+// TMEM: three S buffers of 128 columns, tile n in n % 3, each overwritten 32 positions at a time by that chunk's P' (16 columns
+// hi, 16 lo); two outputs of 64 columns, one per group, read back while the group's next tile is on its way.
+// MEASURED
+#pragma once
+
+#include "flash_pipe.cuh"
+#include "paged_mma.cuh"
+
+namespace cvattn {
+namespace paged {
+
+constexpr int kTcTile = 128;   // positions
+constexpr int kTcRows = 128;
+constexpr int kTcThreads = 20 * 32;
+// Registers of a thread by role: launched with 96.
+constexpr int kTcRegsSoftmax = 160, kTcRegsProducer = 64, kTcRegsOther = 32;
+static_assert(256 * kTcRegsSoftmax + 256 * kTcRegsProducer + 128 * kTcRegsOther <= 640 * 96, "the block's registers");
+constexpr int kTcMaxSeq = 1024;  // tables in shared memory
+constexpr int kTcSt = 5;         // K and V tiles under way
+constexpr int kTcInfos = 8;      // tiles whose scales may be in use
+constexpr int kTcTileBytes = kTcTile * kD * 2;
+constexpr int kTcBlocks = kTcTile / kBlock;
+
+struct TcAttArgs {
+    AttArgs a;
+    int grid;          // CTAs that share the list
+    float* ws_o;       // [2 * grid][128][64]
+    float* ws_ml;      // [2 * grid][128][2]
+    int32_t* ws_pref;  // [n_seq + 1], written by CTA 0 for the combine
+};
+
+struct TcInfo {                 // of a tile
+    float ks[kTcBlocks];        // key scales
+    float w[kTcBlocks];         // value scales times a power of two, below 1
+    float exp;                  // the inverse of that power
+    uint32_t valid;             // blocks that have a page
+    uint32_t starts;            // whether the tile starts a run
+    uint32_t pad;
+};
+
+struct TcAttBars {
+    uint64_t k_full[kTcSt], v_full[kTcSt], k_empty[kTcSt], v_empty[kTcSt];  // by stage
+    uint64_t q_full;
+    uint64_t s_full[3], p_full[3], s_free[3];                               // by S buffer
+    uint64_t o_full[2];                                                     // by group
+    uint32_t tmem_base;
+    int err;
+    TcInfo info[kTcInfos];      // tile n at n % kTcInfos
+    int32_t first_run[16];      // TcRun at the start of the CTA's part
+};
+
+struct TcSmem {
+    static constexpr int kQ = 0;                            // Q hi, Q lo; then the groups' halves at a run's end
+    static constexpr int kTiles = 2 * kTcTileBytes;         // [stage][K, V]
+    static constexpr int kMl = kTiles + kTcSt * 2 * kTcTileBytes;
+    static constexpr int kRs = kMl + kTcRows * 8;           // score factors of the rows
+    static constexpr int kBars = kRs + kTcRows * 4;
+    static constexpr int kPref = kBars + (int)((sizeof(TcAttBars) + 15) / 16 * 16);
+    static constexpr int kLen = kPref + (kTcMaxSeq + 4) * 4, kRowsOf = kLen + kTcMaxSeq * 4;
+    static constexpr int kBytes = kRowsOf + kTcMaxSeq * 4;
+};
+static_assert(TcSmem::kBytes <= 227 * 1024, "one CTA per SM");
+
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ float less_f16(float x, uint16_t h) {  // x - h, exact where h is x's nearest f16
+    float r;
+    asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(r) : "h"(h), "h"((uint16_t)0xBC00u), "f"(x));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long ra = *reinterpret_cast<unsigned long long*>(&a), rb = *reinterpret_cast<unsigned long long*>(&b), rd;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+    return *reinterpret_cast<float2*>(&rd);
+}
+// Bounded wait: gives up after kTcTries suspensions of up to 20 us, or once another role has given up.  *err keeps the site; the
+// kernel's end records it.
+constexpr uint32_t kTcTries = 100000;
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
+#pragma unroll 1
+    for (uint32_t i = 0; !mbar_try_wait_hint(bar, parity, 20000u); ++i) {
+        if (i >= kTcTries) *reinterpret_cast<volatile int*>(err) = site;
+        if (*reinterpret_cast<volatile int*>(err)) return false;
+    }
+    return true;
+}
+
+// Positions that the last row of row tile rt sees, of a sequence with L positions and n of them as rows.
+__device__ __forceinline__ int tc_end(int L, int n, int G, int rt) {
+    const int last = min(n * G, (rt + 1) * kTcRows) - 1;
+    return max(0, L - n + 1 + last / G);
+}
+__device__ __forceinline__ int tc_tiles(int L, int n, int G, int rt) { return (tc_end(L, n, G, rt) + kTcTile - 1) / kTcTile; }
+__device__ __forceinline__ int tc_cut(int c, int n, int g) { return (int)((long long)c * n / g); }
+__device__ __forceinline__ int tc_owner(int i, int n, int g) { return (int)(((long long)(i + 1) * g - 1) / n); }
+
+struct TcTab {  // in shared memory, by sequence: entries before it, positions, rows (tokens)
+    const int32_t *pref, *len, *n;
+};
+// A CTA's walk through its part of the list, run by run.
+struct TcRun {
+    int s, kvh, rt;   // unit
+    int i, end;       // list entries [i, end) of this run
+    int t0, T;        // its first tile, and the unit's tiles
+    int L, n, see;    // positions, tokens, positions that the unit's last row sees
+
+    __device__ __forceinline__ void unit(const AttArgs& a) {
+        see = tc_end(L, n, a.G, rt);
+        T = (see + kTcTile - 1) / kTcTile;
+    }
+    __device__ __forceinline__ void start(const AttArgs& a, const TcTab& tab, int entry, int hi) {
+        i = end = entry;
+        if (entry >= hi) return;
+        int lo = 0, up = a.p.n_seq;  // last s with pref[s] <= entry: its list is not empty
+        while (up - lo > 1) {
+            const int mid = (lo + up) >> 1;
+            if (tab.pref[mid] <= entry) lo = mid;
+            else up = mid;
+        }
+        s = lo;
+        L = tab.len[s];
+        n = tab.n[s];
+        int e = entry - tab.pref[s];
+        rt = 0;
+        for (unit(a); e >= T * a.p.pool.n_heads; unit(a)) {
+            e -= T * a.p.pool.n_heads;
+            ++rt;
+        }
+        kvh = e / T;
+        t0 = e - kvh * T;
+        end = min(hi, i + T - t0);
+    }
+    __device__ __forceinline__ void next(const AttArgs& a, const TcTab& tab, int hi) {
+        i = end;
+        if (i >= hi) return;
+        t0 = 0;
+        if (++kvh == a.p.pool.n_heads) {
+            kvh = 0;
+            ++rt;
+            if (i == tab.pref[s + 1]) {  // (row tiles without entries come first)
+                while (tab.pref[s + 1] == i) ++s;
+                L = tab.len[s];
+                n = tab.n[s];
+                rt = 0;
+            }
+            unit(a);
+            while (T == 0) {
+                ++rt;
+                unit(a);
+            }
+        }
+        end = min(hi, i + T);
+    }
+};
+
+// Four codes as f16 pairs, bytes where `there` is 0 as zeros.
+template <int F> __device__ __forceinline__ void to_f16_there(uint32_t w, uint32_t there, uint32_t& a, uint32_t& b) {
+    w &= there;
+    if constexpr (F == kI8) w |= 0x80808080u & ~there;
+    to_f16<F>(w, a, b);
+}
+
+// A producer group's 128 threads: the tiles of K or V.
+template <int F, bool kV>
+__device__ __forceinline__ void tc_produce(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int lo, int hi) {
+    const AttArgs& a = ta.a;
+    const int t = threadIdx.x & 127, w = t >> 5, lane = t & 31;
+    uint64_t *full = kV ? B->v_full : B->k_full, *empty = kV ? B->v_empty : B->k_empty;
+    uint8_t* tiles0 = smem + TcSmem::kTiles + (kV ? kTcTileBytes : 0);
+    const uint8_t* pool = static_cast<const uint8_t*>(kV ? a.p.pool.v : a.p.pool.k);
+    // Lane i of every warp looks after block i & 7 of a tile: its page (-1: bad, -2: past the end).
+    struct Ahead {
+        int page, in, count, first;
+    };
+    int n_next = 0, first_next = 1;  // the tile that r is at
+    auto look = [&]() {
+        Ahead x{-2, 0, 0, 0};
+        if (lo + n_next < hi) {
+            if (lo + n_next == r.end) {
+                r.next(a, tab, hi);
+                first_next = 1;
+            }
+            const int p0 = (r.t0 + lo + n_next - r.i) * kTcTile, b = p0 / kBlock + (lane & 7);
+            x.count = min(kTcTile, r.see - p0);
+            x.first = first_next;
+            if ((lane & 7) * kBlock < x.count) {
+                x.page = page_of(a.p.table + (int64_t)r.s * a.p.table_nb_seq, b / a.blocks, a.p.pool.n_pages);
+                x.in = r.kvh * a.blocks + b % a.blocks;
+                if (!kV && x.page < 0 && t < 8) record_status(a.status, kStatusBadPage);
+            }
+            first_next = 0;
+        }
+        ++n_next;
+        return x;
+    };
+    auto fetch = [&](const Ahead& x, uint4 (&d)[4], float2& sc) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int page = __shfl_sync(0xffffffffu, x.page, 2 * w + e), in = __shfl_sync(0xffffffffu, x.in, 2 * w + e);
+            const uint8_t* src = pool + page * a.p.pool.nb_page + (int64_t)in * kBlockBytes;
+            // K: 16 bytes of row lane / 4 (+ 8); V: (half, g, quarters 2 u and 2 u + 1)
+            const int at = kV ? (lane >> 4) * 512 + ((lane & 7) * 4 + (lane >> 3 & 1) * 2) * 16 : lane * 16;
+            const int step = kV ? 16 : 512;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                d[2 * e + i] = make_uint4(0u, 0u, 0u, 0u);
+                if (page >= 0) d[2 * e + i] = __ldg(reinterpret_cast<const uint4*>(src + at + i * step));
+            }
+        }
+        if (!kV && w == 0) {
+            sc = make_float2(0.f, 0.f);
+            if (x.page >= 0) {
+                const int64_t at = x.page * a.p.pool.nb_scale + x.in;
+                sc = make_float2(__ldg(a.p.pool.k_scale + at), __ldg(a.p.pool.v_scale + at));
+            }
+        }
+    };
+    Ahead now = look(), then = look();
+    uint4 d[4];
+    float2 sc = make_float2(0.f, 0.f);
+    fetch(now, d, sc);
+    bool ok = true;
+    int st = 0;
+    uint32_t use = 0;
+#pragma unroll 1
+    for (int n = 0; lo + n < hi; ++n) {
+        uint4 nd[4];
+        float2 nsc = make_float2(0.f, 0.f);
+        fetch(then, nd, nsc);
+        const Ahead later = look();
+        if (use) ok = ok && tc_wait(&empty[st], (use - 1) & 1, &B->err, kV ? 36 : 35);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* tile = tiles0 + st * 2 * kTcTileBytes;
+        if constexpr (!kV) {
+            if (w == 0) {
+                TcInfo& info = B->info[n % kTcInfos];
+                const uint32_t good = __ballot_sync(0xffffffffu, now.page >= 0) & 0xffu;
+                float mx = sc.y;
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
+                e = e > 100 ? 100 : e < -100 ? -100 : e;
+                if (lane < kTcBlocks) {
+                    info.ks[lane] = sc.x;
+                    info.w[lane] = sc.y * pow2f(e);
+                }
+                if (lane == 0) {
+                    info.exp = pow2f(-e);
+                    info.valid = good;
+                    info.starts = (uint32_t)now.first;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = w * 32 + i * 8 + (lane >> 2), c = 2 * (lane & 3);
+                uint4 u, v;
+                to_f16<F>(d[i].x, u.x, u.y);
+                to_f16<F>(d[i].y, u.z, u.w);
+                to_f16<F>(d[i].z, v.x, v.y);
+                to_f16<F>(d[i].w, v.z, v.w);
+                *reinterpret_cast<uint4*>(tile + tc::sw128_offset(row, c)) = u;
+                *reinterpret_cast<uint4*>(tile + tc::sw128_offset(row, c + 1)) = v;
+            }
+        } else {
+            const int g = lane & 7, u = lane >> 3 & 1, h = lane >> 4;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int b = 2 * w + e;
+                // positions 8 u .. + 7 of the block that exist, four bytes at a time
+                const int left = __shfl_sync(0xffffffffu, now.page, b) >= 0 ? now.count - b * kBlock - 8 * u : 0;
+                const uint32_t m0 = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+                const uint32_t m1 = left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u;
+                const uint32_t x[4] = {d[2 * e].x, d[2 * e].y, d[2 * e].z, d[2 * e].w};
+                const uint32_t y[4] = {d[2 * e + 1].x, d[2 * e + 1].y, d[2 * e + 1].z, d[2 * e + 1].w};
+                uint8_t* half = tile + (b >> 2) * (kTcTileBytes / 2);  // 64 positions: rows of dims, 128 bytes
+                const int c = (b & 3) * 2 + u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4 o;
+                    to_f16_there<F>(x[j], m0, o.x, o.y);
+                    to_f16_there<F>(y[j], m1, o.z, o.w);
+                    *reinterpret_cast<uint4*>(half + tc::sw128_offset(32 * h + 8 * j + g, c)) = o;
+                }
+            }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&full[st]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = nd[i];
+        sc = nsc;
+        now = then;
+        then = later;
+        if (++st == kTcSt) {
+            st = 0;
+            ++use;
+        }
+    }
+}
+
+template <int F>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ TcAttArgs ta) {
+    using Sh = TcSmem;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const AttArgs& a = ta.a;
+    TcAttBars* B = reinterpret_cast<TcAttBars*>(smem + Sh::kBars);
+    int32_t* pref = reinterpret_cast<int32_t*>(smem + Sh::kPref);
+    int32_t *len = reinterpret_cast<int32_t*>(smem + Sh::kLen), *toks = reinterpret_cast<int32_t*>(smem + Sh::kRowsOf);
+    const TcTab tab{pref, len, toks};
+    if (smem_addr(smem) & 1023u) {
+        if (threadIdx.x == 0) record_status(a.status, kStatusTimeout);
+        return;
+    }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kTcSt; ++i) {
+            mbar_init(&B->k_full[i], 128);
+            mbar_init(&B->v_full[i], 128);
+            mbar_init(&B->k_empty[i], 1);
+            mbar_init(&B->v_empty[i], 1);
+        }
+        mbar_init(&B->q_full, 256);
+        for (int b = 0; b < 3; ++b) {
+            mbar_init(&B->s_full[b], 1);
+            mbar_init(&B->p_full[b], 128);
+            mbar_init(&B->s_free[b], 1);
+        }
+        for (int g = 0; g < 2; ++g) mbar_init(&B->o_full[g], 1);
+        B->err = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tc::tmem_alloc(&B->tmem_base, 512);
+        tc::tmem_relinquish();
+    }
+    if (warp == 1) {  // list entries before each sequence
+        griddep_wait();  // (every other thread touches global memory after the __syncthreads below)
+        int carry = 0;
+        for (int base = 0; base < a.p.n_seq; base += 32) {
+            const int s = base + lane;
+            int n = 0;
+            if (s < a.p.n_seq) {
+                const AttLens x = att_lens(a, s, blockIdx.x == 0);
+                for (int rt = 0; rt * kTcRows < x.n * a.G; ++rt) n += tc_tiles(x.L, x.n, a.G, rt);
+                n *= a.p.pool.n_heads;
+                len[s] = x.L;
+                toks[s] = x.n;
+            }
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (s < a.p.n_seq) {
+                pref[s] = carry + incl - n;
+                if (blockIdx.x == 0) ta.ws_pref[s] = carry + incl - n;
+            }
+            carry += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) {
+            pref[a.p.n_seq] = carry;
+            if (blockIdx.x == 0) ta.ws_pref[a.p.n_seq] = carry;
+        }
+        __syncwarp();
+        TcRun r{};
+        r.start(a, tab, tc_cut(blockIdx.x, carry, ta.grid), tc_cut(blockIdx.x + 1, carry, ta.grid));
+        static_assert(sizeof(TcRun) <= sizeof(B->first_run), "a run in shared memory");
+        if (lane == 0) *reinterpret_cast<TcRun*>(B->first_run) = r;
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    griddep_launch_dependents();
+    const uint32_t tmem = B->tmem_base;
+    const int total = pref[a.p.n_seq];
+    const int lo = tc_cut(blockIdx.x, total, ta.grid), hi = tc_cut(blockIdx.x + 1, total, ta.grid);
+    TcRun r = *reinterpret_cast<const TcRun*>(B->first_run);
+
+    if (warp < 8) {
+        // ------------------------------------------------------ softmax group g
+        regs_up<kTcRegsSoftmax>();
+        const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        const uint32_t ot = tmem + lane_base + 384 + g * 64;
+        uint8_t* qhi = smem + Sh::kQ;
+        uint8_t* qlo = qhi + kTcTileBytes;
+        float4* xch = reinterpret_cast<float4*>(smem + Sh::kQ) + row * 16;  // group 1's output row at a run's end
+        float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl) + row;
+        float* rsb = reinterpret_cast<float*>(smem + Sh::kRs);
+        uint32_t k = 0;  // tiles of this group so far
+        bool ok = true;
+        for (; r.i < hi; r.next(a, tab, hi)) {
+            const int rr = r.rt * kTcRows + row, rows = r.n * a.G, before = r.L - r.n + 1;
+            const bool real = rr < rows;
+            const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
+            const int tok = rr / a.G, h = r.kvh * a.G + rr - tok * a.G;
+            const int lim = real ? before + tok : 0;                   // positions that the row sees
+            const int sure = before + r.rt * kTcRows / a.G;            // that all rows of the unit do
+            // Q: four lanes a row, 16 dims each
+            // (nothing reads the last run's Q, or its exchanged rows, any more)
+            if (r.i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 1
+            for (int q0 = tid >> 2; q0 < kTcRows; q0 += 64) {
+                const int qr = r.rt * kTcRows + q0, qt = qr / a.G, c = lane & 3;
+                const float4* q = reinterpret_cast<const float4*>(a.p.q + (int64_t)r.s * a.p.q_nb_seq + (int64_t)qt * a.p.q_nb_tok +
+                                                                  (r.kvh * a.G + qr - qt * a.G) * kD + 16 * c);
+                float4 v[4];
+                float am = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = qr < rows ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) am = fmaxf(am, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
+                const int ex = dtc::norm_exp(quad_max(am));
+                const float f = pow2f(ex);
+                if (c == 0) rsb[q0] = pow2f(-ex) * a.scale_log2;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint4 wh, wl;
+                    split_near(make_float2(v[2 * u].x * f, v[2 * u].y * f), wh.x, wl.x);
+                    split_near(make_float2(v[2 * u].z * f, v[2 * u].w * f), wh.y, wl.y);
+                    split_near(make_float2(v[2 * u + 1].x * f, v[2 * u + 1].y * f), wh.z, wl.z);
+                    split_near(make_float2(v[2 * u + 1].z * f, v[2 * u + 1].w * f), wh.w, wl.w);
+                    const uint32_t at = tc::sw128_offset(q0, 2 * c + u);
+                    *reinterpret_cast<uint4*>(qhi + at) = wh;
+                    *reinterpret_cast<uint4*>(qlo + at) = wl;
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&B->q_full);
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            const float rs = rsb[row];
+            float2 O[32];
+#pragma unroll
+            for (int d = 0; d < 32; ++d) O[d] = make_float2(0.f, 0.f);
+            float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 1.0f;
+            bool pending = false;  // a tile's output still to be added, times vs_last
+            auto add_output = [&]() {
+                uint32_t o0[32];
+                const float2 f = make_float2(vs_last, vs_last);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    tc::tmem_ld32(ot + 32 * e, o0);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int d = 0; d < 16; ++d)
+                        O[16 * e + d] = ffma2(make_float2(__uint_as_float(o0[2 * d]), __uint_as_float(o0[2 * d + 1])), f, O[16 * e + d]);
+                }
+            };
+            for (int j = r.i + ((r.i ^ g ^ lo) & 1); j < r.end; j += 2) {  // the CTA's tiles j - lo of parity g
+                const int p0 = (r.t0 + j - r.i) * kTcTile;
+                const int n = j - lo, buf = n % 3;
+                // (Of a buffer's phases a group sees every second one, always of the same parity.  It cannot pass on an older one:
+                // S of tile n - 3, the phase before, was committed ahead of S of n - 2, which this group has seen.)
+                const uint32_t sp = tmem + lane_base + buf * 128;
+                ok = tc_wait(&B->s_full[buf], (n / 3) & 1, &B->err, 31);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc::fence_after();
+                const TcInfo& info = B->info[n % kTcInfos];
+                float vs_now = 1.0f;
+                if (warp_real) {
+                    uint32_t sv[32];
+                    tc::tmem_ld32(sp, sv);
+                    const uint32_t valid = info.valid;
+                    const bool masked = p0 + kTcTile > sure || valid != 0xffu;
+                    vs_now = info.exp;
+                    tc::tmem_ld_wait();
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 ks = *reinterpret_cast<const float2*>(info.ks + 2 * c), w = *reinterpret_cast<const float2*>(info.w + 2 * c);
+                        float2 x[16];
+                        {
+                            const float f0 = rs * ks.x, f1 = rs * ks.y;
+                            const float2 b = make_float2(-base, -base);
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) {
+                                const float f = d < 8 ? f0 : f1;
+                                x[d] = ffma2(make_float2(__uint_as_float(sv[2 * d]), __uint_as_float(sv[2 * d + 1])), make_float2(f, f), b);
+                            }
+                        }
+                        tc::tmem_ld32(sp + 32 * min(c + 1, 3), sv);  // under way during this chunk's arithmetic
+                        if (masked) {
+                            const int left = lim - p0 - 32 * c;
+                            uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                            if (!(valid >> (2 * c) & 1u)) bits &= 0xffff0000u;
+                            if (!(valid >> (2 * c + 1) & 1u)) bits &= 0x0000ffffu;
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) {
+                                if (!(bits >> (2 * d) & 1u)) x[d].x = -INFINITY;
+                                if (!(bits >> (2 * d + 1) & 1u)) x[d].y = -INFINITY;
+                            }
+                        }
+                        float mx = fmaxf(x[0].x, x[0].y);
+#pragma unroll
+                        for (int d = 1; d < 16; ++d) mx = fmaxf(mx, fmaxf(x[d].x, x[d].y));
+                        if (__any_sync(0xffffffffu, mx > thr)) {
+                            float f = 1.0f, up = 0.0f;
+                            if (mx > thr) {
+                                up = mx - kOffs;
+                                f = thr == -INFINITY ? 0.0f : fast_exp2(-up);
+                                base += up;
+                                thr = kLazy + kOffs;
+                                l *= f;
+                                vs_last *= f;
+                            }
+                            const float2 f2 = make_float2(f, f);
+#pragma unroll
+                            for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) {
+                                x[d].x -= up;
+                                x[d].y -= up;
+                            }
+                            if (c) {  // this tile's P' so far, 16 positions at a time
+                                tc::tmem_ld_wait();
+                                tc::tmem_st_wait();
+#pragma unroll 1
+                                for (int e = 0; e < 2 * c; ++e) {
+                                    uint32_t ph[8], pl[8];
+                                    const uint32_t at = sp + 32 * (e >> 1) + 8 * (e & 1);
+                                    tc::tmem_ld8(at, ph);
+                                    tc::tmem_ld8(at + 16, pl);
+                                    tc::tmem_ld_wait();
+#pragma unroll
+                                    for (int d = 0; d < 8; ++d) {
+                                        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&ph[d]));
+                                        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&pl[d]));
+                                        split_near(make_float2((u.x + y.x) * f, (u.y + y.y) * f), ph[d], pl[d]);
+                                    }
+                                    tc::tmem_st8(at, ph);
+                                    tc::tmem_st8(at + 16, pl);
+                                }
+                            }
+                        }
+                        float2 l0 = make_float2(0.f, 0.f), l1 = l0;
+                        uint32_t pv[32];
+#pragma unroll
+                        for (int d = 0; d < 16; ++d) {
+                            x[d].x = fast_exp2(x[d].x);
+                            x[d].y = fast_exp2(x[d].y);
+                            if (d & 1) l1 = add2(l1, x[d]);
+                            else l0 = add2(l0, x[d]);
+                            const float wd = d < 8 ? w.x : w.y;
+                            const float2 y = mul2(x[d], make_float2(wd, wd));
+                            pv[d] = tc::pack_f16x2(y.x, y.y);
+                            pv[16 + d] = tc::pack_f16x2(less_f16(y.x, (uint16_t)pv[d]), less_f16(y.y, (uint16_t)(pv[d] >> 16)));
+                        }
+                        l0 = add2(l0, l1);
+                        l += l0.x + l0.y;
+                        tc::tmem_st32(sp + 32 * c, pv);
+                        tc::tmem_ld_wait();
+                    }
+                    if (pending) {  // the output of the group's tile before this one (o_full counts every tile of the group)
+                        ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, 32);
+                        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                        tc::fence_after();
+                        add_output();
+                    }
+                    vs_last = vs_now;
+                    pending = true;
+                    tc::tmem_st_wait();
+                }
+                ++k;
+                tc::fence_before();
+                mbar_arrive(&B->p_full[buf]);
+            }
+            if (ok && pending) {
+                ok = tc_wait(&B->o_full[g], (k - 1) & 1, &B->err, 32);
+                ok = __all_sync(0xffffffffu, ok);
+                tc::fence_after();
+                if (ok) add_output();
+            }
+            tc::fence_before();
+            if (!fp::prod_bar_and(2, 256, ok)) break;  // every MMA of the run is done; all threads leave together
+            const float m_mine = thr == -INFINITY && l == 0.0f ? -INFINITY : base;  // (NaN scores raise nothing)
+            if (g == 1) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) xch[c ^ (row & 7)] = make_float4(O[2 * c].x, O[2 * c].y, O[2 * c + 1].x, O[2 * c + 1].y);
+                *mls = make_float2(m_mine, l);
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (g == 0 && real) {
+                const float2 other = *mls;
+                const float M = fmaxf(m_mine, other.x);
+                const float f0 = m_mine == -INFINITY ? 0.0f : exp2f(m_mine - M), f1 = other.x == -INFINITY ? 0.0f : exp2f(other.x - M);
+                const float sum = (m_mine == -INFINITY ? 0.0f : f0 * l) + (other.x == -INFINITY ? 0.0f : f1 * other.y);
+                const bool whole = r.end - r.i == r.T, seen = M != -INFINITY;
+                const float inv = !whole ? 1.0f : seen ? 1.0f / sum : 0.0f;
+                const int64_t slot = (int64_t)(2 * blockIdx.x + (r.i == lo ? 0 : 1)) * kTcRows + row;
+                const int64_t orow = (int64_t)r.s * a.p.out_nb_seq + (int64_t)tok * a.p.out_nb_tok + h * kD;
+                float4* dst = reinterpret_cast<float4*>(whole ? a.p.out + orow : ta.ws_o + slot * kD);
+                const float2 g0 = make_float2(f0 * inv, f0 * inv), g1 = make_float2(f1 * inv, f1 * inv);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const float4 w = xch[c ^ (row & 7)];
+                    const float2 u = ffma2(g1, make_float2(w.x, w.y), mul2(g0, O[2 * c])), v = ffma2(g1, make_float2(w.z, w.w), mul2(g0, O[2 * c + 1]));
+                    dst[c] = make_float4(u.x, u.y, v.x, v.y);
+                }
+                if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + slot * 2) = make_float2(M, sum);
+                else if (a.p.lse)
+                    a.p.lse[((int64_t)r.s * a.p.max_q + tok) * a.p.n_q_heads + h] = seen ? (M + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+            }
+        }
+    } else if (warp < 12) {
+        regs_down<kTcRegsProducer>();
+        tc_produce<F, false>(ta, smem, B, tab, r, lo, hi);
+    } else if (warp < 16) {
+        regs_down<kTcRegsProducer>();
+        tc_produce<F, true>(ta, smem, B, tab, r, lo, hi);
+    } else {
+        regs_down<kTcRegsOther>();
+        // ------------------------------------------------------ MMA issuers: the whole warp walks, one lane issues
+        const int which = __shfl_sync(0xffffffffu, warp, 0);
+        const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
+        constexpr uint64_t kStep = 2 * kTcTileBytes >> 4;
+        bool ok = true;
+        int st = 0, buf = 0;
+        uint32_t use = 0, turn = 0, n_run = 0;  // n / kTcSt, n / 3
+        if (which == 16) {
+            const uint32_t idesc = tc::idesc_f16_f32(128, kTcTile, false);
+            const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
+            const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
+            for (int n = 0; ok && lo + n < hi; ++n) {
+                ok = tc_wait(&B->k_full[st], use & 1, &B->err, 38);
+                if (ok && B->info[n % kTcInfos].starts) ok = tc_wait(&B->q_full, n_run++ & 1, &B->err, 37);
+                if (ok && n >= 3) ok = tc_wait(&B->s_free[buf], (turn - 1) & 1, &B->err, 40);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::fence_after();
+                const uint64_t dk = dt0 + (uint64_t)st * kStep;
+                const uint32_t sp = tmem + buf * 128;
+                if (elect_one()) {
+#pragma unroll 1
+                    for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dql + kk * 2, dk + kk * 2, idesc, kk > 0 ? 1u : 0u);  // small terms first
+#pragma unroll 1
+                    for (int kk = 0; kk < 4; ++kk) tc::mma_ss(sp, dqh + kk * 2, dk + kk * 2, idesc, 1u);
+                    tc::mma_commit(&B->s_full[buf]);
+                    tc::mma_commit(&B->k_empty[st]);
+                }
+                __syncwarp();
+                if (++st == kTcSt) { st = 0; ++use; }
+                if (++buf == 3) { buf = 0; ++turn; }
+            }
+        } else if (which == 17) {
+            const uint32_t idesc = tc::idesc_f16_f32(128, 64, false);
+            for (int n = 0; ok && lo + n < hi; ++n) {
+                ok = tc_wait(&B->v_full[st], use & 1, &B->err, 41);
+                if (ok) ok = tc_wait(&B->p_full[buf], turn & 1, &B->err, 39);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::fence_after();
+                const uint64_t dv = dt0 + (uint64_t)st * kStep + (kTcTileBytes >> 4);
+                const uint32_t sp = tmem + buf * 128, ot = tmem + 384 + (n & 1) * 64;
+                if (elect_one()) {
+#pragma unroll 1
+                    for (int kk = 0; kk < 8; ++kk)
+                        tc::mma_ts(ot, sp + 32 * (kk >> 1) + 8 * (kk & 1) + 16, dv + (kk >> 2) * (kTcTileBytes >> 5) + (kk & 3) * 2, idesc, kk > 0 ? 1u : 0u);
+#pragma unroll 1
+                    for (int kk = 0; kk < 8; ++kk)
+                        tc::mma_ts(ot, sp + 32 * (kk >> 1) + 8 * (kk & 1), dv + (kk >> 2) * (kTcTileBytes >> 5) + (kk & 3) * 2, idesc, 1u);
+                    tc::mma_commit(&B->o_full[n & 1]);
+                    tc::mma_commit(&B->v_empty[st]);
+                    tc::mma_commit(&B->s_free[buf]);
+                }
+                __syncwarp();
+                if (++st == kTcSt) { st = 0; ++use; }
+                if (++buf == 3) { buf = 0; ++turn; }
+            }
+        }
+    }
+
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc::fence_after();
+        tc::tmem_dealloc(tmem, 512);
+    }
+    if (tid == 0 && B->err) record_status(a.status, kStatusTimeout | (B->err << 8));
+}
+
+// Join of the parts of units that several CTAs shared, and the rows that no unit holds (rows that see nothing, or past the last
+// token).  16 threads per row (4 dims each) follow every kLanes-th part.
+template <int kLanes>
+__global__ void __launch_bounds__(256) paged_tc_combine_kernel(const __grid_constant__ TcAttArgs ta) {
+    constexpr int kPer = 16 / kLanes;
+    __shared__ float4 so[16][16];
+    __shared__ float2 sml[16];
+    const AttArgs& a = ta.a;
+    griddep_wait();
+    const int unit = threadIdx.x >> 4, c = threadIdx.x & 15, lane = unit % kLanes;
+    const int all_rows = a.p.max_q * a.G;
+    const int r = blockIdx.x * kPer + unit / kLanes, kvh = blockIdx.y, s = blockIdx.z;
+    const AttLens x = att_lens(a, s, false);
+    const int rt = r / kTcRows, n = ta.ws_pref[a.p.n_seq];
+    int b0 = 0, c0 = 0, c1 = -1;
+    if (r < x.n * a.G) {
+        const int T = tc_tiles(x.L, x.n, a.G, rt);
+        if (T > 0) {
+            b0 = ta.ws_pref[s] + kvh * T;
+            for (int i = 0; i < rt; ++i) b0 += tc_tiles(x.L, x.n, a.G, i) * a.p.pool.n_heads;
+            c0 = tc_owner(b0, n, ta.grid);
+            c1 = tc_owner(b0 + T - 1, n, ta.grid);
+            if (kLanes == 1 && c0 == c1) return;  // written whole
+        }
+    }
+    const bool done = c0 == c1;
+    Join j;
+    for (int k0 = c0 + lane; k0 <= c1 && !done; k0 += 4 * kLanes) {
+        float2 ml[4];
+        float4 v[4];
+        float top = j.M;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int cta = k0 + u * kLanes;
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (cta <= c1 && tc_cut(cta + 1, n, ta.grid) > tc_cut(cta, n, ta.grid)) {
+                const int64_t at = (int64_t)(2 * cta + (tc_cut(cta, n, ta.grid) >= b0 ? 0 : 1)) * kTcRows + r % kTcRows;
+                ml[u] = *reinterpret_cast<const float2*>(ta.ws_ml + at * 2);
+                v[u] = *reinterpret_cast<const float4*>(ta.ws_o + at * kD + c * 4);
+            }
+            top = fmaxf(top, ml[u].x);
+        }
+        if (top == -INFINITY) continue;
+        const float f0 = exp2f(j.M - top);
+        j.M = top;
+        j.l *= f0;
+        j.o.x *= f0; j.o.y *= f0; j.o.z *= f0; j.o.w *= f0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) j.add(ml[u], v[u]);
+    }
+    if constexpr (kLanes > 1) {
+        so[unit][c] = j.o;
+        if (c == 0) sml[unit] = make_float2(j.M, j.l);
+        __syncthreads();
+        if (lane || done) return;
+        j = Join();
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) j.M = fmaxf(j.M, sml[unit + k].x);
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) j.add(sml[unit + k], so[unit + k][c]);
+    }
+    if (r < all_rows) j.write(a, s, kvh, r, c);
+}
+
+}  // namespace paged
+}  // namespace cvattn
