@@ -162,7 +162,7 @@ template <int R> struct MmaSmem {
 template <int F, int R>
 __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kernel(const __grid_constant__ AttArgs a) {
     using S = MmaSmem<R>;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int s = blockIdx.z;
     const int kvh = blockIdx.y % a.p.pool.n_heads, r0 = blockIdx.y / a.p.pool.n_heads * (S::kRows * kMmaWarps);

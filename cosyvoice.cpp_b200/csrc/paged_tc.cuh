@@ -5,10 +5,10 @@
 // the part of one unit that a CTA has; a whole unit is written out directly, parts go to the workspace and
 // paged_tc_combine_kernel joins them.
 //   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the CTA's tiles 2 k + g
-//   warps 8-11      producer of the K tiles, 12-15 of the V tiles: codes from the pages to registers one tile ahead (table
-//                   entries two), f16 into shared memory (128B swizzle), V transposed as its blocks lie
-//   warp 16         issues S = Q K^T, up to two tiles ahead of the softmax;  warp 17 issues O = P V
-//   (warps 18, 19 only complete the last warpgroup)
+//   warps 8-11      producers: codes from the pages (cp.async, two tiles ahead; table entries three), each warp two blocks, which
+//                   it turns into f16 itself (128B swizzle, V transposed as its blocks lie)
+//   warp 12         issues S = Q K^T, up to two tiles ahead of the softmax;  warp 13 issues O = P V
+//   (warps 14, 15 only complete the last warpgroup)
 // Precision: codes are exact in f16, Q and P' = P w are split in f16 hi + lo, so S = Qh K + Ql K and O = Ph V + Pl V.  A block's
 // key scale multiplies its 16 columns of S; its value scale, over a power of two of the tile, is w, which leaves P' with what is
 // above 2^-22 of the largest of the tile.  The output of a tile is a fresh accumulator, added in f32 to the row's registers: adds
@@ -26,12 +26,13 @@ namespace paged {
 
 constexpr int kTcTile = 128;   // positions
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 20 * 32;
-// Registers of a thread by role: launched with 96.
-constexpr int kTcRegsSoftmax = 160, kTcRegsProducer = 64, kTcRegsOther = 32;
-static_assert(256 * kTcRegsSoftmax + 256 * kTcRegsProducer + 128 * kTcRegsOther <= 640 * 96, "the block's registers");
+constexpr int kTcThreads = 16 * 32;
+// Registers of a thread by role: launched with 128.
+constexpr int kTcRegsSoftmax = 200, kTcRegsProducer = 72, kTcRegsOther = 32;
+static_assert(256 * kTcRegsSoftmax + 128 * kTcRegsProducer + 128 * kTcRegsOther <= 512 * 128, "the block's registers");
 constexpr int kTcMaxSeq = 1024;  // tables in shared memory
-constexpr int kTcSt = 5;         // K and V tiles under way
+constexpr int kTcSt = 4;         // K and V tiles under way
+constexpr int kTcRaw = 3;        // tiles of codes under way
 constexpr int kTcInfos = 8;      // tiles whose scales may be in use
 constexpr int kTcTileBytes = kTcTile * kD * 2;
 constexpr int kTcBlocks = kTcTile / kBlock;
@@ -67,7 +68,9 @@ struct TcAttBars {
 struct TcSmem {
     static constexpr int kQ = 0;                            // Q hi, Q lo; then the groups' halves at a run's end
     static constexpr int kTiles = 2 * kTcTileBytes;         // [stage][K, V]
-    static constexpr int kMl = kTiles + kTcSt * 2 * kTcTileBytes;
+    static constexpr int kRaw = kTiles + kTcSt * 2 * kTcTileBytes;  // [slot][16-byte piece of a thread][thread]
+    static constexpr int kRawBytes = 8 * 128 * 16, kRawScales = kRaw + kTcRaw * kRawBytes;
+    static constexpr int kMl = kRawScales + kTcRaw * 2 * kTcBlocks * 4;
     static constexpr int kRs = kMl + kTcRows * 8;           // score factors of the rows
     static constexpr int kBars = kRs + kTcRows * 4;
     static constexpr int kPref = kBars + (int)((sizeof(TcAttBars) + 15) / 16 * 16);
@@ -86,6 +89,11 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ float less_f16(float x, uint16_t h) {  // x - h, exact where h is x's nearest f16
     float r;
     asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(r) : "h"(h), "h"((uint16_t)0xBC00u), "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -173,148 +181,165 @@ struct TcRun {
     }
 };
 
-// Four codes as f16 pairs, bytes where `there` is 0 as zeros.
-template <int F> __device__ __forceinline__ void to_f16_there(uint32_t w, uint32_t there, uint32_t& a, uint32_t& b) {
-    w &= there;
-    if constexpr (F == kI8) w |= 0x80808080u & ~there;
-    to_f16<F>(w, a, b);
+// Codes of 0 where `keep` is 0.
+template <int F> __device__ __forceinline__ void keep_bytes(uint4& v, uint32_t keep) {
+    const uint32_t zero = F == kI8 ? 0x80808080u & ~keep : 0u;
+    v = make_uint4((v.x & keep) | zero, (v.y & keep) | zero, (v.z & keep) | zero, (v.w & keep) | zero);
 }
 
-// A producer group's 128 threads: the tiles of K or V.
-template <int F, bool kV>
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// The producers' 128 threads.  Pieces of 16 bytes: of K four (rows 8 apart), of V four.
+template <int F>
 __device__ __forceinline__ void tc_produce(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int lo, int hi) {
     const AttArgs& a = ta.a;
     const int t = threadIdx.x & 127, w = t >> 5, lane = t & 31;
-    uint64_t *full = kV ? B->v_full : B->k_full, *empty = kV ? B->v_empty : B->k_empty;
-    uint8_t* tiles0 = smem + TcSmem::kTiles + (kV ? kTcTileBytes : 0);
-    const uint8_t* pool = static_cast<const uint8_t*>(kV ? a.p.pool.v : a.p.pool.k);
-    // Lane i of every warp looks after block i & 7 of a tile: its page (-1: bad, -2: past the end).
-    struct Ahead {
-        int page, in, count, first;
-    };
-    int n_next = 0, first_next = 1;  // the tile that r is at
+    const uint8_t* kpool = static_cast<const uint8_t*>(a.p.pool.k) + lane * 16;
+    // V: a lane turns the pieces (half, g, quarters 2 u and 2 u + 1) that its warp has copied
+    const int u = lane & 1, g = lane >> 1 & 7, h = lane >> 4, vrow = (32 * h + g) * 128;
+    const uint8_t* vpool = static_cast<const uint8_t*>(a.p.pool.v) + lane * 16;
+    const int krow = (w * 32 + (lane >> 2)) * 128, k0 = ((2 * (lane & 3)) ^ (lane >> 2)) * 16, k1 = k0 ^ 16;  // (rows 8 apart swizzle alike)
+    const int shift = __ffs(a.blocks) - 1;
+    // The tile that is looked up next, and of the one looked up last: its blocks' pages (lane i: block i & 7; -1: none or past the
+    // end) and places, positions and whether it starts a run.
+    int n_next = 0, starts = 1;
+    int page = -1, in = 0, count = 0, first = 0;
+    bool bad = false;
     auto look = [&]() {
-        Ahead x{-2, 0, 0, 0};
+        page = -1;
+        count = 0;
+        bad = false;
         if (lo + n_next < hi) {
             if (lo + n_next == r.end) {
                 r.next(a, tab, hi);
-                first_next = 1;
+                starts = 1;
             }
-            const int p0 = (r.t0 + lo + n_next - r.i) * kTcTile, b = p0 / kBlock + (lane & 7);
-            x.count = min(kTcTile, r.see - p0);
-            x.first = first_next;
-            if ((lane & 7) * kBlock < x.count) {
-                x.page = page_of(a.p.table + (int64_t)r.s * a.p.table_nb_seq, b / a.blocks, a.p.pool.n_pages);
-                x.in = r.kvh * a.blocks + b % a.blocks;
-                if (!kV && x.page < 0 && t < 8) record_status(a.status, kStatusBadPage);
+            const int p0 = (r.t0 + lo + n_next - r.i) * kTcTile, b = p0 / kBlock + (lane & 7), entry = b >> shift;
+            count = min(kTcTile, r.see - p0);
+            first = starts;
+            starts = 0;
+            if ((lane & 7) * kBlock < count) {
+                page = __ldg(a.p.table + (int64_t)r.s * a.p.table_nb_seq + entry);
+                in = ((r.kvh - entry) << shift) + b;
+                bad = true;  // (if the page is out of range)
             }
-            first_next = 0;
         }
         ++n_next;
-        return x;
     };
-    auto fetch = [&](const Ahead& x, uint4 (&d)[4], float2& sc) {
+    // What is said of a tile (packed: positions, whether it starts a run, the blocks that have a page), and its copies.
+    auto fetch = [&](int slot) -> uint32_t {
+        const bool good = (uint32_t)page < (uint32_t)a.p.pool.n_pages;
+        if (!good && bad && t < 8) record_status(a.status, kStatusBadPage);
+        const uint32_t valid = __ballot_sync(0xffffffffu, good) & 0xffu;
+        // (where there is nothing, the pool's first block is read and left out later)
+        const int64_t at = good ? page * a.p.pool.nb_page + (int64_t)in * kBlockBytes : 0;
+        const uint32_t raw = smem_addr(smem + TcSmem::kRaw) + slot * TcSmem::kRawBytes + t * 16;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int page = __shfl_sync(0xffffffffu, x.page, 2 * w + e), in = __shfl_sync(0xffffffffu, x.in, 2 * w + e);
-            const uint8_t* src = pool + page * a.p.pool.nb_page + (int64_t)in * kBlockBytes;
-            // K: 16 bytes of row lane / 4 (+ 8); V: (half, g, quarters 2 u and 2 u + 1)
-            const int at = kV ? (lane >> 4) * 512 + ((lane & 7) * 4 + (lane >> 3 & 1) * 2) * 16 : lane * 16;
-            const int step = kV ? 16 : 512;
+            const int64_t off = __shfl_sync(0xffffffffu, at, 2 * w + e);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                d[2 * e + i] = make_uint4(0u, 0u, 0u, 0u);
-                if (page >= 0) d[2 * e + i] = __ldg(reinterpret_cast<const uint4*>(src + at + i * step));
+                copy16(raw + (2 * e + i) * 2048, kpool + off + i * 512);
+                copy16(raw + (4 + 2 * e + i) * 2048, vpool + off + i * 512);
             }
         }
-        if (!kV && w == 0) {
-            sc = make_float2(0.f, 0.f);
-            if (x.page >= 0) {
-                const int64_t at = x.page * a.p.pool.nb_scale + x.in;
-                sc = make_float2(__ldg(a.p.pool.k_scale + at), __ldg(a.p.pool.v_scale + at));
-            }
+        if (t < kTcBlocks) {
+            const int64_t sat = good ? page * a.p.pool.nb_scale + in : 0;
+            const uint32_t to = smem_addr(smem + TcSmem::kRawScales) + (slot * 2 * kTcBlocks + t) * 4;
+            copy4(to, a.p.pool.k_scale + sat);
+            copy4(to + kTcBlocks * 4, a.p.pool.v_scale + sat);
         }
+        copies_done();
+        return valid | (uint32_t)first << 8 | (uint32_t)count << 16;
     };
-    Ahead now = look(), then = look();
-    uint4 d[4];
-    float2 sc = make_float2(0.f, 0.f);
-    fetch(now, d, sc);
+    look();
+    uint32_t said = fetch(0);
+    look();
+    uint32_t said_next = fetch(1);
+    look();
     bool ok = true;
-    int st = 0;
+    int st = 0, slot = 0;
     uint32_t use = 0;
 #pragma unroll 1
     for (int n = 0; lo + n < hi; ++n) {
-        uint4 nd[4];
-        float2 nsc = make_float2(0.f, 0.f);
-        fetch(then, nd, nsc);
-        const Ahead later = look();
-        if (use) ok = ok && tc_wait(&empty[st], (use - 1) & 1, &B->err, kV ? 36 : 35);
+        const uint32_t said_then = fetch(slot == 0 ? 2 : slot - 1);
+        look();
+        copies_wait<2>();
+        __syncwarp();
+        const uint4* raw = reinterpret_cast<const uint4*>(smem + TcSmem::kRaw + slot * TcSmem::kRawBytes) + t;
+        const uint32_t valid = said & 0xffu;
+        const int here = (int)(said >> 16);
+        if (use) ok = tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, 35);
         if (!__all_sync(0xffffffffu, ok)) break;
-        uint8_t* tile = tiles0 + st * 2 * kTcTileBytes;
-        if constexpr (!kV) {
-            if (w == 0) {
-                TcInfo& info = B->info[n % kTcInfos];
-                const uint32_t good = __ballot_sync(0xffffffffu, now.page >= 0) & 0xffu;
-                float mx = sc.y;
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
-                e = e > 100 ? 100 : e < -100 ? -100 : e;
-                if (lane < kTcBlocks) {
-                    info.ks[lane] = sc.x;
-                    info.w[lane] = sc.y * pow2f(e);
-                }
-                if (lane == 0) {
-                    info.exp = pow2f(-e);
-                    info.valid = good;
-                    info.starts = (uint32_t)now.first;
-                }
+        uint8_t* tile = smem + TcSmem::kTiles + st * 2 * kTcTileBytes;
+        if (w == 0) {
+            TcInfo& info = B->info[n % kTcInfos];
+            const float* sc = reinterpret_cast<const float*>(smem + TcSmem::kRawScales) + slot * 2 * kTcBlocks;
+            const bool good = lane < kTcBlocks && (valid >> lane & 1u);
+            const float ks = good ? sc[lane] : 0.0f, vs = good ? sc[kTcBlocks + lane] : 0.0f;
+            const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
+            int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
+            e = e > 100 ? 100 : e < -100 ? -100 : e;
+            if (lane < kTcBlocks) {
+                info.ks[lane] = ks;
+                info.w[lane] = vs * pow2f(e);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = w * 32 + i * 8 + (lane >> 2), c = 2 * (lane & 3);
-                uint4 u, v;
-                to_f16<F>(d[i].x, u.x, u.y);
-                to_f16<F>(d[i].y, u.z, u.w);
-                to_f16<F>(d[i].z, v.x, v.y);
-                to_f16<F>(d[i].w, v.z, v.w);
-                *reinterpret_cast<uint4*>(tile + tc::sw128_offset(row, c)) = u;
-                *reinterpret_cast<uint4*>(tile + tc::sw128_offset(row, c + 1)) = v;
+            if (lane == 0) {
+                info.exp = pow2f(-e);
+                info.valid = valid;
+                info.starts = said >> 8 & 1u;
             }
-        } else {
-            const int g = lane & 7, u = lane >> 3 & 1, h = lane >> 4;
+        }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int b = 2 * w + e;
-                // positions 8 u .. + 7 of the block that exist, four bytes at a time
-                const int left = __shfl_sync(0xffffffffu, now.page, b) >= 0 ? now.count - b * kBlock - 8 * u : 0;
-                const uint32_t m0 = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-                const uint32_t m1 = left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u;
-                const uint32_t x[4] = {d[2 * e].x, d[2 * e].y, d[2 * e].z, d[2 * e].w};
-                const uint32_t y[4] = {d[2 * e + 1].x, d[2 * e + 1].y, d[2 * e + 1].z, d[2 * e + 1].w};
-                uint8_t* half = tile + (b >> 2) * (kTcTileBytes / 2);  // 64 positions: rows of dims, 128 bytes
-                const int c = (b & 3) * 2 + u;
+        for (int i = 0; i < 4; ++i) {
+            const uint4 d = raw[i * 128];
+            uint4 x, y;
+            to_f16<F>(d.x, x.x, x.y);
+            to_f16<F>(d.y, x.z, x.w);
+            to_f16<F>(d.z, y.x, y.y);
+            to_f16<F>(d.w, y.z, y.w);
+            *reinterpret_cast<uint4*>(tile + krow + i * 8 * 128 + k0) = x;
+            *reinterpret_cast<uint4*>(tile + krow + i * 8 * 128 + k1) = y;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&B->k_full[st]);
+        if (use) ok = tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, 36);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tile += kTcTileBytes;
+        const bool part = here < kTcTile || valid != 0xffu;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint4 o;
-                    to_f16_there<F>(x[j], m0, o.x, o.y);
-                    to_f16_there<F>(y[j], m1, o.z, o.w);
-                    *reinterpret_cast<uint4*>(half + tc::sw128_offset(32 * h + 8 * j + g, c)) = o;
-                }
+        for (int e = 0; e < 2; ++e) {
+            const uint4* of = raw - lane + (4 + 2 * e + h) * 128 + 4 * g + 2 * u;
+            uint4 x4 = of[0], y4 = of[1];
+            if (part) {  // (what lies past the end may be NaN): positions 8 u .. + 7 of the block that exist, four bytes at a time
+                const int left = valid >> (2 * w + e) & 1u ? here - (2 * w + e) * kBlock - 8 * u : 0;
+                keep_bytes<F>(x4, left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u);
+                keep_bytes<F>(y4, left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u);
+            }
+            const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+            uint8_t* to = tile + (w >> 1) * (kTcTileBytes / 2) + vrow + ((((2 * w + e) & 3) * 2 + u) ^ g) * 16;  // 64 positions: rows of dims
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint4 o;
+                to_f16<F>(x[j], o.x, o.y);
+                to_f16<F>(y[j], o.z, o.w);
+                *reinterpret_cast<uint4*>(to + j * 8 * 128) = o;
             }
         }
         fence_proxy_async_smem();
-        mbar_arrive(&full[st]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = nd[i];
-        sc = nsc;
-        now = then;
-        then = later;
+        mbar_arrive(&B->v_full[st]);
+        __syncwarp();  // (the slot is filled again next)
+        said = said_next;
+        said_next = said_then;
+        slot = slot == 2 ? 0 : slot + 1;
         if (++st == kTcSt) {
             st = 0;
             ++use;
         }
     }
+    copies_wait<0>();
 }
 
 template <int F>
@@ -509,9 +534,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                                 if (!(bits >> (2 * d + 1) & 1u)) x[d].y = -INFINITY;
                             }
                         }
-                        float mx = fmaxf(x[0].x, x[0].y);
+                        float m4[4];
 #pragma unroll
-                        for (int d = 1; d < 16; ++d) mx = fmaxf(mx, fmaxf(x[d].x, x[d].y));
+                        for (int u = 0; u < 4; ++u)
+                            m4[u] = max3(max3(max3(x[4 * u].x, x[4 * u].y, x[4 * u + 1].x), x[4 * u + 1].y, x[4 * u + 2].x),
+                                         fmaxf(x[4 * u + 2].y, x[4 * u + 3].x), x[4 * u + 3].y);
+                        const float mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
                         if (__any_sync(0xffffffffu, mx > thr)) {
                             float f = 1.0f, up = 0.0f;
                             if (mx > thr) {
@@ -622,10 +650,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         }
     } else if (warp < 12) {
         regs_down<kTcRegsProducer>();
-        tc_produce<F, false>(ta, smem, B, tab, r, lo, hi);
-    } else if (warp < 16) {
-        regs_down<kTcRegsProducer>();
-        tc_produce<F, true>(ta, smem, B, tab, r, lo, hi);
+        tc_produce<F>(ta, smem, B, tab, r, lo, hi);
     } else {
         regs_down<kTcRegsOther>();
         // ------------------------------------------------------ MMA issuers: the whole warp walks, one lane issues
@@ -635,7 +660,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         bool ok = true;
         int st = 0, buf = 0;
         uint32_t use = 0, turn = 0, n_run = 0;  // n / kTcSt, n / 3
-        if (which == 16) {
+        if (which == 12) {
             const uint32_t idesc = tc::idesc_f16_f32(128, kTcTile, false);
             const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
             const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
@@ -660,7 +685,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 if (++st == kTcSt) { st = 0; ++use; }
                 if (++buf == 3) { buf = 0; ++turn; }
             }
-        } else if (which == 17) {
+        } else if (which == 13) {
             const uint32_t idesc = tc::idesc_f16_f32(128, 64, false);
             for (int n = 0; ok && lo + n < hi; ++n) {
                 ok = tc_wait(&B->v_full[st], use & 1, &B->err, 41);
