@@ -5,10 +5,10 @@
 // the part of one unit that a CTA has; a whole unit is written out directly, parts go to the workspace and
 // paged_tc_combine_kernel joins them.
 //   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the CTA's tiles 2 k + g
-//   warps 8-11      producers: codes from the pages (cp.async, two tiles ahead; table entries three), each warp two blocks, which
-//                   it turns into f16 itself (128B swizzle, V transposed as its blocks lie)
+//   warps 8-11      producers: codes to f16 tiles (128B swizzle), V transposed as its blocks lie
 //   warp 12         issues S = Q K^T, up to two tiles ahead of the softmax;  warp 13 issues O = P V
-//   (warps 14, 15 only complete the last warpgroup)
+//   warp 14         looks the tiles' pages up, copies their blocks (1 KB each, cp.async.bulk) and scales, up to three tiles ahead
+//   (warp 15 only completes the last warpgroup)
 // Precision: codes are exact in f16, Q and P' = P w are split in f16 hi + lo, so S = Qh K + Ql K and O = Ph V + Pl V.  A block's
 // key scale multiplies its 16 columns of S; its value scale, over a power of two of the tile, is w, which leaves P' with what is
 // above 2^-22 of the largest of the tile.  The output of a tile is a fresh accumulator, added in f32 to the row's registers: adds
@@ -51,11 +51,12 @@ struct TcInfo {                 // of a tile
     float exp;                  // the inverse of that power
     uint32_t valid;             // blocks that have a page
     uint32_t starts;            // whether the tile starts a run
-    uint32_t pad;
+    int32_t count;              // positions that exist
 };
 
 struct TcAttBars {
     uint64_t k_full[kTcSt], v_full[kTcSt], k_empty[kTcSt], v_empty[kTcSt];  // by stage
+    uint64_t raw_full[kTcRaw], raw_empty[kTcRaw];                           // by slot of codes
     uint64_t q_full;
     uint64_t s_full[3], p_full[3], s_free[3];                               // by S buffer
     uint64_t o_full[2];                                                     // by group
@@ -68,9 +69,9 @@ struct TcAttBars {
 struct TcSmem {
     static constexpr int kQ = 0;                            // Q hi, Q lo; then the groups' halves at a run's end
     static constexpr int kTiles = 2 * kTcTileBytes;         // [stage][K, V]
-    static constexpr int kRaw = kTiles + kTcSt * 2 * kTcTileBytes;  // [slot][16-byte piece of a thread][thread]
-    static constexpr int kRawBytes = 8 * 128 * 16, kRawScales = kRaw + kTcRaw * kRawBytes;
-    static constexpr int kMl = kRawScales + kTcRaw * 2 * kTcBlocks * 4;
+    static constexpr int kRaw = kTiles + kTcSt * 2 * kTcTileBytes;  // [slot][K, V][block]
+    static constexpr int kRawBytes = 2 * kTcBlocks * kBlockBytes;
+    static constexpr int kMl = kRaw + kTcRaw * kRawBytes;
     static constexpr int kRs = kMl + kTcRows * 8;           // score factors of the rows
     static constexpr int kBars = kRs + kTcRows * 4;
     static constexpr int kPref = kBars + (int)((sizeof(TcAttBars) + 15) / 16 * 16);
@@ -187,114 +188,103 @@ template <int F> __device__ __forceinline__ void keep_bytes(uint4& v, uint32_t k
     v = make_uint4((v.x & keep) | zero, (v.y & keep) | zero, (v.z & keep) | zero, (v.w & keep) | zero);
 }
 
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// The producers' 128 threads.  Pieces of 16 bytes: of K four (rows 8 apart), of V four.
-template <int F>
-__device__ __forceinline__ void tc_produce(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int lo, int hi) {
+// Warp 14: lane i < 8 looks after block i of each tile.
+__device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int lo, int hi) {
     const AttArgs& a = ta.a;
-    const int t = threadIdx.x & 127, w = t >> 5, lane = t & 31;
-    const uint8_t* kpool = static_cast<const uint8_t*>(a.p.pool.k) + lane * 16;
-    // V: a lane turns the pieces (half, g, quarters 2 u and 2 u + 1) that its warp has copied
-    const int u = lane & 1, g = lane >> 1 & 7, h = lane >> 4, vrow = (32 * h + g) * 128;
-    const uint8_t* vpool = static_cast<const uint8_t*>(a.p.pool.v) + lane * 16;
-    const int krow = (w * 32 + (lane >> 2)) * 128, k0 = ((2 * (lane & 3)) ^ (lane >> 2)) * 16, k1 = k0 ^ 16;  // (rows 8 apart swizzle alike)
-    const int shift = __ffs(a.blocks) - 1;
-    // The tile that is looked up next, and of the one looked up last: its blocks' pages (lane i: block i & 7; -1: none or past the
-    // end) and places, positions and whether it starts a run.
-    int n_next = 0, starts = 1;
+    const int lane = threadIdx.x & 31, shift = __ffs(a.blocks) - 1;
+    int starts = 1;
+    // of the tile that is looked up: this lane's page and place, its positions
     int page = -1, in = 0, count = 0, first = 0;
-    bool bad = false;
-    auto look = [&]() {
+    auto look = [&](int entry) {
         page = -1;
         count = 0;
-        bad = false;
-        if (lo + n_next < hi) {
-            if (lo + n_next == r.end) {
-                r.next(a, tab, hi);
-                starts = 1;
-            }
-            const int p0 = (r.t0 + lo + n_next - r.i) * kTcTile, b = p0 / kBlock + (lane & 7), entry = b >> shift;
-            count = min(kTcTile, r.see - p0);
-            first = starts;
-            starts = 0;
-            if ((lane & 7) * kBlock < count) {
-                page = __ldg(a.p.table + (int64_t)r.s * a.p.table_nb_seq + entry);
-                in = ((r.kvh - entry) << shift) + b;
-                bad = true;  // (if the page is out of range)
+        if (entry >= hi) return;
+        if (entry == r.end) {
+            r.next(a, tab, hi);
+            starts = 1;
+        }
+        const int p0 = (r.t0 + entry - r.i) * kTcTile, b = p0 / kBlock + lane, at = b >> shift;
+        count = min(kTcTile, r.see - p0);
+        first = starts;
+        starts = 0;
+        if (lane < kTcBlocks && lane * kBlock < count) {
+            page = __ldg(a.p.table + (int64_t)r.s * a.p.table_nb_seq + at);
+            in = ((r.kvh - at) << shift) + b;
+            if ((uint32_t)page >= (uint32_t)a.p.pool.n_pages) {
+                record_status(a.status, kStatusBadPage);
+                page = -1;
             }
         }
-        ++n_next;
     };
-    // What is said of a tile (packed: positions, whether it starts a run, the blocks that have a page), and its copies.
-    auto fetch = [&](int slot) -> uint32_t {
-        const bool good = (uint32_t)page < (uint32_t)a.p.pool.n_pages;
-        if (!good && bad && t < 8) record_status(a.status, kStatusBadPage);
-        const uint32_t valid = __ballot_sync(0xffffffffu, good) & 0xffu;
-        // (where there is nothing, the pool's first block is read and left out later)
-        const int64_t at = good ? page * a.p.pool.nb_page + (int64_t)in * kBlockBytes : 0;
-        const uint32_t raw = smem_addr(smem + TcSmem::kRaw) + slot * TcSmem::kRawBytes + t * 16;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int64_t off = __shfl_sync(0xffffffffu, at, 2 * w + e);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                copy16(raw + (2 * e + i) * 2048, kpool + off + i * 512);
-                copy16(raw + (4 + 2 * e + i) * 2048, vpool + off + i * 512);
-            }
+    bool ok = true;
+    int slot = 0, n = 0;
+    uint32_t use = 0;
+    look(lo);
+#pragma unroll 1
+    for (; lo + n < hi; ++n) {
+        if (use) ok = tc_wait(&B->raw_empty[slot], (use - 1) & 1, &B->err, 34);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const bool good = page >= 0;
+        const uint32_t valid = __ballot_sync(0xffffffffu, good);
+        const int64_t at = good ? page * a.p.pool.nb_page + (int64_t)in * kBlockBytes : 0, sat = good ? page * a.p.pool.nb_scale + in : 0;
+        if (lane == 0) mbar_arrive_expect_tx(&B->raw_full[slot], __popc(valid) * 2 * kBlockBytes);
+        __syncwarp();
+        uint8_t* raw = smem + TcSmem::kRaw + slot * TcSmem::kRawBytes;
+        if (good) {
+            bulk_g2s(raw + lane * kBlockBytes, static_cast<const uint8_t*>(a.p.pool.k) + at, kBlockBytes, &B->raw_full[slot]);
+            bulk_g2s(raw + (kTcBlocks + lane) * kBlockBytes, static_cast<const uint8_t*>(a.p.pool.v) + at, kBlockBytes, &B->raw_full[slot]);
         }
-        if (t < kTcBlocks) {
-            const int64_t sat = good ? page * a.p.pool.nb_scale + in : 0;
-            const uint32_t to = smem_addr(smem + TcSmem::kRawScales) + (slot * 2 * kTcBlocks + t) * 4;
-            copy4(to, a.p.pool.k_scale + sat);
-            copy4(to + kTcBlocks * 4, a.p.pool.v_scale + sat);
+        const float ks = good ? a.p.pool.k_scale[sat] : 0.0f, vs = good ? a.p.pool.v_scale[sat] : 0.0f;
+        const int here = count, starts_here = first;
+        look(lo + n + 1);
+        const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
+        int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
+        e = e > 100 ? 100 : e < -100 ? -100 : e;
+        TcInfo& info = B->info[n % kTcInfos];
+        if (lane < kTcBlocks) {
+            info.ks[lane] = ks;
+            info.w[lane] = vs * pow2f(e);
         }
-        copies_done();
-        return valid | (uint32_t)first << 8 | (uint32_t)count << 16;
-    };
-    look();
-    uint32_t said = fetch(0);
-    look();
-    uint32_t said_next = fetch(1);
-    look();
+        if (lane == 0) {
+            info.exp = pow2f(-e);
+            info.valid = valid;
+            info.starts = (uint32_t)starts_here;
+            info.count = here;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->raw_full[slot]);  // (the second of its two arrivals: what is said of the tile)
+        if (++slot == kTcRaw) {
+            slot = 0;
+            ++use;
+        }
+    }
+    // after an error copies are under way that nobody waited for
+    if (!ok)
+        for (int k = n > kTcRaw ? n - kTcRaw : 0; k < n; ++k)
+            for (uint32_t i = 0; i < kTcTries && !mbar_try_wait_hint(&B->raw_full[k % kTcRaw], (k / kTcRaw) & 1, 20000u); ++i) {}
+}
+
+// The producers' 128 threads: warp w blocks 2 w and 2 w + 1 of a tile.
+template <int F> __device__ __forceinline__ void tc_produce(uint8_t* smem, TcAttBars* B, int lo, int hi) {
+    const int t = threadIdx.x & 127, w = t >> 5, lane = t & 31;
+    // K: rows 8 apart, which swizzle alike; V: pieces (half, g, quarters 2 u and 2 u + 1)
+    const int krow = (w * 32 + (lane >> 2)) * 128, k0 = ((2 * (lane & 3)) ^ (lane >> 2)) * 16, k1 = k0 ^ 16;
+    const int u = lane & 1, g = lane >> 1 & 7, h = lane >> 4, vrow = (w >> 1) * (kTcTileBytes / 2) + (32 * h + g) * 128;
     bool ok = true;
     int st = 0, slot = 0;
-    uint32_t use = 0;
+    uint32_t use = 0, turn = 0;
 #pragma unroll 1
     for (int n = 0; lo + n < hi; ++n) {
-        const uint32_t said_then = fetch(slot == 0 ? 2 : slot - 1);
-        look();
-        copies_wait<2>();
-        __syncwarp();
-        const uint4* raw = reinterpret_cast<const uint4*>(smem + TcSmem::kRaw + slot * TcSmem::kRawBytes) + t;
-        const uint32_t valid = said & 0xffu;
-        const int here = (int)(said >> 16);
-        if (use) ok = tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, 35);
+        ok = tc_wait(&B->raw_full[slot], turn & 1, &B->err, 33);
+        if (ok && use) ok = tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, 35);
         if (!__all_sync(0xffffffffu, ok)) break;
+        const uint32_t valid = B->info[n % kTcInfos].valid;
+        const int count = B->info[n % kTcInfos].count;
         uint8_t* tile = smem + TcSmem::kTiles + st * 2 * kTcTileBytes;
-        if (w == 0) {
-            TcInfo& info = B->info[n % kTcInfos];
-            const float* sc = reinterpret_cast<const float*>(smem + TcSmem::kRawScales) + slot * 2 * kTcBlocks;
-            const bool good = lane < kTcBlocks && (valid >> lane & 1u);
-            const float ks = good ? sc[lane] : 0.0f, vs = good ? sc[kTcBlocks + lane] : 0.0f;
-            const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
-            int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
-            e = e > 100 ? 100 : e < -100 ? -100 : e;
-            if (lane < kTcBlocks) {
-                info.ks[lane] = ks;
-                info.w[lane] = vs * pow2f(e);
-            }
-            if (lane == 0) {
-                info.exp = pow2f(-e);
-                info.valid = valid;
-                info.starts = said >> 8 & 1u;
-            }
-        }
+        const uint4* raw = reinterpret_cast<const uint4*>(smem + TcSmem::kRaw + slot * TcSmem::kRawBytes + 2 * w * kBlockBytes);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 d = raw[i * 128];
+            const uint4 d = raw[i * 32 + lane];
             uint4 x, y;
             to_f16<F>(d.x, x.x, x.y);
             to_f16<F>(d.y, x.z, x.w);
@@ -305,21 +295,29 @@ __device__ __forceinline__ void tc_produce(const TcAttArgs& ta, uint8_t* smem, T
         }
         fence_proxy_async_smem();
         mbar_arrive(&B->k_full[st]);
+        uint4 v[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            v[2 * e] = raw[(kTcBlocks + e) * 64 + h * 32 + 4 * g + 2 * u];
+            v[2 * e + 1] = raw[(kTcBlocks + e) * 64 + h * 32 + 4 * g + 2 * u + 1];
+        }
+        mbar_arrive(&B->raw_empty[slot]);
+        if (count < kTcTile || valid != 0xffu) {  // (what lies past the end may be NaN)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                // positions 8 u .. + 7 of the block that exist, four bytes at a time
+                const int left = valid >> (2 * w + e) & 1u ? count - (2 * w + e) * kBlock - 8 * u : 0;
+                keep_bytes<F>(v[2 * e], left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u);
+                keep_bytes<F>(v[2 * e + 1], left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u);
+            }
+        }
         if (use) ok = tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, 36);
         if (!__all_sync(0xffffffffu, ok)) break;
         tile += kTcTileBytes;
-        const bool part = here < kTcTile || valid != 0xffu;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const uint4* of = raw - lane + (4 + 2 * e + h) * 128 + 4 * g + 2 * u;
-            uint4 x4 = of[0], y4 = of[1];
-            if (part) {  // (what lies past the end may be NaN): positions 8 u .. + 7 of the block that exist, four bytes at a time
-                const int left = valid >> (2 * w + e) & 1u ? here - (2 * w + e) * kBlock - 8 * u : 0;
-                keep_bytes<F>(x4, left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u);
-                keep_bytes<F>(y4, left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u);
-            }
-            const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
-            uint8_t* to = tile + (w >> 1) * (kTcTileBytes / 2) + vrow + ((((2 * w + e) & 3) * 2 + u) ^ g) * 16;  // 64 positions: rows of dims
+            const uint32_t x[4] = {v[2 * e].x, v[2 * e].y, v[2 * e].z, v[2 * e].w}, y[4] = {v[2 * e + 1].x, v[2 * e + 1].y, v[2 * e + 1].z, v[2 * e + 1].w};
+            uint8_t* to = tile + vrow + ((((2 * w + e) & 3) * 2 + u) ^ g) * 16;  // 64 positions: rows of dims
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint4 o;
@@ -330,16 +328,15 @@ __device__ __forceinline__ void tc_produce(const TcAttArgs& ta, uint8_t* smem, T
         }
         fence_proxy_async_smem();
         mbar_arrive(&B->v_full[st]);
-        __syncwarp();  // (the slot is filled again next)
-        said = said_next;
-        said_next = said_then;
-        slot = slot == 2 ? 0 : slot + 1;
         if (++st == kTcSt) {
             st = 0;
             ++use;
         }
+        if (++slot == kTcRaw) {
+            slot = 0;
+            ++turn;
+        }
     }
-    copies_wait<0>();
 }
 
 template <int F>
@@ -362,6 +359,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             mbar_init(&B->v_full[i], 128);
             mbar_init(&B->k_empty[i], 1);
             mbar_init(&B->v_empty[i], 1);
+        }
+        for (int i = 0; i < kTcRaw; ++i) {
+            mbar_init(&B->raw_full[i], 2);
+            mbar_init(&B->raw_empty[i], 128);
         }
         mbar_init(&B->q_full, 256);
         for (int b = 0; b < 3; ++b) {
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         }
     } else if (warp < 12) {
         regs_down<kTcRegsProducer>();
-        tc_produce<F>(ta, smem, B, tab, r, lo, hi);
+        tc_produce<F>(smem, B, lo, hi);
     } else {
         regs_down<kTcRegsOther>();
         // ------------------------------------------------------ MMA issuers: the whole warp walks, one lane issues
@@ -710,6 +711,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 if (++st == kTcSt) { st = 0; ++use; }
                 if (++buf == 3) { buf = 0; ++turn; }
             }
+        } else if (which == 14) {
+            tc_load(ta, smem, B, tab, r, lo, hi);
         }
     }
 
