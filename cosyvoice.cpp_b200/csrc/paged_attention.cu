@@ -1,9 +1,6 @@
 // paged_attention.cu -- the join of splits and the host side of attention over a paged 8-bit cache.
 #include "launch.cuh"
 #include "paged_tc.cuh"
-#ifndef KNOB
-#define KNOB(n, d) d
-#endif
 
 namespace cvattn {
 namespace paged {
@@ -66,6 +63,13 @@ constexpr int kSms = 148;
 
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// The tcgen05 kernel starts later (about 9 us) and takes 1.5 us for a tile of 128 positions on an SM, whatever rows it has up to
+// 128; the other takes 0.44 ns for a row of such a tile (all SMs together).  us of mma.sync | tcgen05, 14 / 2 heads: 1
+// sequence of 4096, 56 rows of a KV head 14.9 | 14.8; 1 of 65536, 14 rows 22.7 | 24.7, 56 48 | 27; 4 of 2500, 112 23.1 | 20.4, 224
+// 27.8 | 25.7; 16 of 1000, 112 23.6 | 26.2, 224 33.5 | 28.4; 16 of 8192, 28 33.4 | 39.2, 56 59 | 41; 64 of 1000, 28 20.4 | 27.8, 56
+// 34.4 | 29.5; 64 of 4096, 28 53 | 55, 56 95 | 59.
+constexpr int64_t kTcWork = 1 << 14, kTcPerTile = 24;
+
 struct Plan {
     int tc_grid;   // > 0: the tcgen05 kernel on that many CTAs
     int R, row_tiles, cluster, n_splits;
@@ -75,7 +79,7 @@ static Plan plan_of(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_k
     Plan p{};
     const int64_t rows = (int64_t)max_q * (n_q_heads / n_kv_heads);
     const int64_t tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile), entries = tiles * ((rows + kTcRows - 1) / kTcRows);
-    if (rows >= KNOB(XROWS, 40) && tiles * rows >= KNOB(XWORK, 1024) && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
+    if (tiles * rows >= kTcWork + kTcPerTile * entries && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
         p.tc_grid = (int)(entries < kSms ? entries : kSms);
         p.n_splits = p.tc_grid / (int64_t)(n_seq * n_kv_heads) > 0 ? p.tc_grid / (n_seq * n_kv_heads) : 1;  // (for the combine)
         return p;
