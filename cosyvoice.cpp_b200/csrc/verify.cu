@@ -121,7 +121,8 @@ struct Node {
 };
 // exp((l - m) / temperature) in f32, m finite; NaN for a NaN.
 __device__ __forceinline__ float weight32(const Node& x, float l) { return fast_exp2((l - x.m) * x.c); }
-// The same in 64 bits; below kNothing where l is not above x.low or a NaN.  `table`: kPowers.
+// The same in 64 bits; below kNothing where l is not above x.low or a NaN.  `table`: kPowers, one entry of 16 apart (each lane of
+// half a warp has a copy in banks of its own: entries are read at random, and without copies that took as long as the rest).
 constexpr double kNothing = 1e-290;
 __device__ __forceinline__ double weight64(const Node& x, float l, const double* table) {
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: u + magic has u's nearest integer in its low bits
@@ -130,7 +131,7 @@ __device__ __forceinline__ double weight64(const Node& x, float l, const double*
     const int n = __double2loint(t);
     double p = fma(r, step * step * step / 6, step * step / 2);
     p = fma(p, r, step);
-    const double base = table[n & 63];
+    const double base = table[(n & 63) * 16];
     p = fma(p * r, base, base);
     return __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p));
 }
@@ -283,13 +284,15 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const __grid_c
 }
 
 struct Shared {
-    double table[64];
+    double table[64 * 16];
     double W[kMaxNodes];                     // of each node: sum of weights,
     float m[kMaxNodes];                      // largest logit,
     int hot[kMaxNodes];                      // lowest token with it
-    double num[kMaxNodes], den[kMaxNodes];   // log-probabilities: exponent, sum
+    int path[kMaxNodes];                     // accepted nodes, from 1 on
+    float last_logit;                        // of the token that follows
+    bool stands[kMaxNodes];                  // whether a draft stands where none was refused before it
     double inv_left[kMaxNodes];              // 1 / the sum of p after each refusal
-    double post_sum[2][kMaxCluster];         // of the cluster's CTAs, in turn of two
+    double post_sum[2][kMaxCluster], post_b[2][kMaxCluster], post_w[2][kMaxCluster];  // of the cluster's CTAs, in turn of two
     int post_found[2][kMaxCluster], post_last[2][kMaxCluster];
     int gone[kMaxNodes];                     // tokens refused
     int parent[kMaxNodes], token[kMaxNodes], first_child[kMaxNodes];
@@ -297,8 +300,9 @@ struct Shared {
     float logit[kMaxNodes], prob[kMaxNodes]; // of the drafts' tokens at their parents
     double weight[kMaxNodes];                // what() of them there, before any refusal
     int bad;
+    double warp_w[kWarps];
     // what warp 0 has decided
-    int what, at, refused;
+    int what, at, refused, first;
     double inv_W;
 };
 enum { kScan = 1, kFollow = 2, kStop = 3 };  // Shared::what
@@ -310,12 +314,14 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
     constexpr int kPer = R::kPer;
     __shared__ Shared sh;
     extern __shared__ double tile_sum[];
+    double* tile_b = tile_sum + n_tiles + 2;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t C, rank;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int s = blockIdx.x / C;
-    if (tid < 64) sh.table[tid] = kPowers[tid];
+    for (int i = tid; i < 64 * 16; i += kThreads) sh.table[i] = kPowers[i >> 4];
+    const double* table = sh.table + (tid & 15);
     if (tid == 0) sh.bad = 0;
     __syncthreads();
     griddep_wait();
@@ -325,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
     float* logs = p.log_probs ? p.log_probs + (int64_t)s * p.max_nodes : nullptr;
     const bool refused_all = n < 0 || n > p.max_nodes || !(heat >= 0.0f && heat < INFINITY);
     const auto row_of = [&](int node) { return R(p.logits, s * p.logits_nb_seq + node * p.logits_nb_node, p.vocab); };
-    for (int i = tid; i < kMaxNodes; i += kThreads) {
+    static_assert(kThreads == 2 * kMaxNodes, "a thread a node, and as many for their sums");
+    if (const int i = tid; i < kMaxNodes) {
         sh.first_child[i] = kMaxNodes;
         if (i < (refused_all ? 0 : n)) {
             const int up = i == 0 ? -1 : p.parents ? p.parents[s * p.parents_nb_seq + i] : i - 1;
@@ -345,28 +352,28 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
     }
     Node x;
     set_heat(x, heat);
-    // a warp a node: its numbers from all slices
-    if (!refused_all)
-        for (int i = warp; i < n; i += kWarps) {
+    // the other warps, one a node: its numbers from all slices
+    if (!refused_all && tid >= kMaxNodes)
+        for (int i = warp - kWarps / 2; i < n; i += kWarps / 2) {
             const Part* of = parts + ((int64_t)s * p.max_nodes + i) * n_slices;
             Part q{0.0, -INFINITY, INT32_MAX};
             for (int k = lane; k < n_slices; k += 32) {
                 const Part v = of[k];
                 if (v.most > q.most) {
                     x.most(v.most);
-                    q.sum = v.sum + (q.sum > 0.0 && !x.greedy && v.most < INFINITY ? q.sum * weight64(x, q.most, sh.table) : 0.0);
+                    q.sum = v.sum + (q.sum > 0.0 && !x.greedy && v.most < INFINITY ? q.sum * weight64(x, q.most, table) : 0.0);
                     q.hot = v.hot;
                     q.most = v.most;
                 } else if (v.most > -INFINITY) {
                     x.most(q.most);
-                    q.sum += v.most == q.most ? v.sum : x.greedy || q.most == INFINITY ? 0.0 : v.sum * weight64(x, v.most, sh.table);
+                    q.sum += v.most == q.most ? v.sum : x.greedy || q.most == INFINITY ? 0.0 : v.sum * weight64(x, v.most, table);
                     if (v.most == q.most) q.hot = min(q.hot, v.hot);
                 }
             }
             const float top = warp_max(q.most);
             x.most(top);
             double w = q.most == top ? 1.0 : 0.0;
-            if (!x.greedy && top < INFINITY && q.most > -INFINITY && q.most < top) w = weight64(x, q.most, sh.table);
+            if (!x.greedy && top < INFINITY && q.most > -INFINITY && q.most < top) w = weight64(x, q.most, table);
             const double sum = warp_add(q.sum * w);
             const int hot = __reduce_min_sync(0xffffffffu, q.most == top ? q.hot : INT32_MAX);
             if (lane == 0) {
@@ -394,21 +401,26 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
         atomicMin(&sh.first_child[up], i);
         x.most(sh.m[up]);
         x.hot = sh.hot[up];
-        sh.weight[i] = weight_any(x, sh.logit[i], sh.token[i], sh.table);
+        sh.weight[i] = weight_any(x, sh.logit[i], sh.token[i], table);
         sh.prob[i] = fmaxf(sh.prob[i], 0.0f);  // (NaN: 0)
+        sh.stands[i] = (double)sh.u[i] * (double)sh.prob[i] * sh.W[up] < sh.weight[i];
     }
     __syncthreads();
 
     // Warp 0 posts this CTA's numbers to the slots of all CTAs, in turn of two: one is written while the other may still be
     // read.  Then every thread arrives.
     int turn = 0;
-    auto exchange = [&](double sum, int found, int last) {
+    auto exchange = [&](double sum, double sum_b, double sum_w, int found, int last) {
         if (tid < (int)C) {
-            uint32_t a, b, c;
+            uint32_t a, b, c, d, e;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(&sh.post_sum[turn][rank])), "r"(tid));
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_addr(&sh.post_found[turn][rank])), "r"(tid));
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(c) : "r"(smem_addr(&sh.post_last[turn][rank])), "r"(tid));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(&sh.post_b[turn][rank])), "r"(tid));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(e) : "r"(smem_addr(&sh.post_w[turn][rank])), "r"(tid));
             asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(a), "d"(sum) : "memory");
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(d), "d"(sum_b) : "memory");
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(e), "d"(sum_w) : "memory");
             asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(b), "r"(found) : "memory");
             asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(c), "r"(last) : "memory");
         }
@@ -441,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
     auto less = [&](double w, float qv) {
         const double g = (double)fmaxf(qv, 0.0f);  // (NaN: 0)
         double r = positive(fma(w, inv_W, -g));
-        for (int k = 1; k < refused; ++k) r = positive(fma(r, sh.inv_left[k - 1], -g));
+        if (refused > 1)
+            for (int k = 1; k < refused; ++k) r = positive(fma(r, sh.inv_left[k - 1], -g));
         return r;
     };
     auto what = [&](double w, float qv, int v) {  // of a token of weight w
@@ -486,14 +499,14 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
         for (int i = 0; i < kPer; ++i) w[i] = 0.0;
         if (f.e < 0) return;
         if (t == 0 || t == tiles - 1) {
-            w[0] = what(weight_any(x, __uint_as_float(f.v.x), f.e, sh.table), f.g[0], f.e);
+            w[0] = what(weight_any(x, __uint_as_float(f.v.x), f.e, table), f.g[0], f.e);
             return;
         }
         float l[kPer];
         R::values(f.v, l);
         if (simple) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) w[i] = weight64(x, l[i], sh.table);
+            for (int i = 0; i < kPer; ++i) w[i] = weight64(x, l[i], table);
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) w[i] = (x.greedy ? f.e + i == x.hot : l[i] == x.m) ? 1.0 : 0.0;
@@ -506,13 +519,43 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
             }
         if (q && refused) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) w[i] = less(w[i], f.g[i]);
+            for (int i = 0; i < kPer; ++i) w[i] = positive(fma(w[i], inv_W, -(double)fmaxf(f.g[i], 0.0f)));
+#pragma unroll 1
+            for (int k = 1; k < refused; ++k) {
+                const double by = sh.inv_left[k - 1];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) w[i] = positive(fma(w[i], by, -(double)fmaxf(f.g[i], 0.0f)));
+            }
+        }
+    };
+    // The first refusal against draft probabilities, in one scan: W, which the subtraction takes, is known to 1e-7 only (W~).  With S
+    // the tokens of which W~ leaves something,  sum_S (w / W - q) = R + (R + B) (W~ / W - 1),  R = sum_S (w / W~ - q),  B = sum_S q.
+    // (A token that the exact W would put on the other side of S has a part below 1e-7 of its own weight.)
+    auto weigh_first = [&](int t, const Fetched& f, double& R1, float& B1, double& W1) {
+        if (f.e < 0) return;
+        if (t == 0 || t == tiles - 1) {
+            const double w = weight_any(x, __uint_as_float(f.v.x), f.e, table), r = fma(w, inv_W, -(double)fmaxf(f.g[0], 0.0f));
+            W1 += w;
+            R1 += positive(r);
+            if (r > 0.0) B1 += fmaxf(f.g[0], 0.0f);
+            return;
+        }
+        float l[kPer];
+        R::values(f.v, l);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const double w = weight64(x, l[i], table);
+            const float g = fmaxf(f.g[i], 0.0f);
+            const double r = fma(w, inv_W, -(double)g);
+            W1 += w;
+            R1 += positive(r);
+            B1 += __double2hiint(r) < 0 ? 0.0f : g;
         }
     };
     double before = 0.0, all = 0.0;    // what() over the CTAs before this one, over the vocabulary (warp 0)
     double total = 0.0, was = 0.0;     // warp 0: what()'s sum over the vocabulary, and before the last refusal
     bool known = true, exact = false;  // warp 0: whether total is that sum; whether of 64-bit weights
-    bool scanned = false;
+    bool scanned = false, first = false;
     int c = 0, order = kStop;
     auto enter = [&](int node) {       // warp 0
         at = node;
@@ -539,6 +582,21 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
                 }
             }
             order = scanned && c >= n ? kFollow : kScan;
+            // first drafts that stand, one below the other
+            if (!scanned) {
+                bool moved = false;
+                while (c < n && sh.stands[c] && sh.m[at] != -INFINITY && refused == 0) {
+                    if (lane == 0) {
+                        if (rank == 0) accepted[count] = c;
+                        sh.path[count] = c;
+                    }
+                    ++count;
+                    at = c;
+                    c = sh.first_child[c];
+                    moved = true;
+                }
+                if (moved) enter(at);
+            }
             // drafts in turn, as long as the sum of what is left is known
             while (order == kScan) {
                 if (sh.m[at] == -INFINITY) order = kStop;  // no weight anywhere
@@ -549,18 +607,16 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
                 if ((double)sh.u[c] * (double)sh.prob[c] * total < pt) {
                     if (lane == 0) {
                         if (rank == 0) accepted[count] = c;
-                        sh.num[count - 1] = x.greedy || sh.logit[c] == sh.m[at] ? 0.0 : ((double)sh.logit[c] - (double)sh.m[at]) * x.inv;
-                        sh.den[count - 1] = sh.W[at];
+                        sh.path[count] = c;
                     }
                     ++count;
                     enter(c);
                     continue;
                 }
-                if (q && !exact) {  // the subtraction takes a sum of exact weights
-                    known = false;
-                    break;
+                if (q && refused == 0) {
+                    inv_W = 1.0 / total;
+                    first = !exact;  // (the subtraction takes a sum of exact weights)
                 }
-                if (q && refused == 0) inv_W = 1.0 / total;
                 if (lane == 0) sh.gone[refused] = t;
                 __syncwarp();
                 ++refused;
@@ -577,6 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
                 sh.what = order;
                 sh.at = at;
                 sh.refused = refused;
+                sh.first = first;
                 sh.inv_W = inv_W;
             }
         }
@@ -585,34 +642,74 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
         if (order != kScan) break;
         arrive_at(sh.at);
         refused = sh.refused;
+        first = sh.first;
         inv_W = sh.inv_W;
         // sums of tiles, of this CTA in the tiles' order, of the cluster
+        double my_w = 0.0;
         Fetched f = fetch(warp);
 #pragma unroll 1
         for (int t = warp; t < tiles; t += kWarps) {
             const Fetched next = fetch(t + kWarps);
-            double w[kPer], sum = 0.0;
-            weigh(t, f, w);
-            f = next;
+            double sum = 0.0;
+            if (first) {
+                float b = 0.0f;
+                weigh_first(t, f, sum, b, my_w);
+                const double all_b = warp_add((double)b);
+                if (lane == 0) tile_b[t] = all_b;
+            } else {
+                double w[kPer];
+                weigh(t, f, w);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) sum += w[i];
+                for (int i = 0; i < kPer; ++i) sum += w[i];
+            }
+            f = next;
             sum = warp_add(sum);
             if (lane == 0) tile_sum[t] = sum;
         }
+        if (first) {
+            my_w = warp_add(my_w);
+            if (lane == 0) sh.warp_w[warp] = my_w;
+        }
         __syncthreads();
         if (warp == 0) {
-            all = 0.0;
-            for (int t = 0; t < tiles; t += 32) all += warp_add(t + lane < tiles ? tile_sum[t + lane] : 0.0);
-        }
-        if (C > 1) {
-            exchange(all, 0, 0);
-            if (warp == 0) {
-                const double v = lane < (int)C ? sh.post_sum[turn][lane] : 0.0;
-                before = warp_add(lane < (int)rank ? v : 0.0);
-                all = warp_add(v);
+            double sum = 0.0, sum_b = 0.0, sum_w = 0.0;
+            for (int t = lane; t < tiles; t += 32) {
+                sum += tile_sum[t];
+                if (first) sum_b += tile_b[t];
             }
-            turn ^= 1;
+            all = warp_add(sum);
+            if (first) {
+                sum_b = warp_add(sum_b);
+                sum_w = warp_add(lane < kWarps ? sh.warp_w[lane] : 0.0);
+            }
+            before = 0.0;
+            double lead = 0.0;  // W~ / W - 1
+            if (C == 1 && first) lead = 1.0 / (inv_W * sum_w) - 1.0;
+            if (C > 1) exchange(all, sum_b, sum_w, 0, 0);
+            if (C > 1) {
+                const bool has = lane < (int)C;
+                const double v = has ? sh.post_sum[turn][lane] : 0.0, v_b = has ? sh.post_b[turn][lane] : 0.0;
+                if (first) {
+                    sum_w = warp_add(has ? sh.post_w[turn][lane] : 0.0);
+                    lead = 1.0 / (inv_W * sum_w) - 1.0;
+                }
+                const double u = first ? fma(v + v_b, lead, v) : v;
+                before = warp_add(lane < (int)rank ? u : 0.0);
+                all = warp_add(u);
+            } else if (first) {
+                all = fma(all + sum_b, lead, all);
+            }
+            if (first) {
+                inv_W = 1.0 / sum_w;
+                was = sum_w;
+                for (int t = lane; t < tiles; t += 32) tile_sum[t] = fma(tile_sum[t] + tile_b[t], lead, tile_sum[t]);
+                __syncwarp();
+                first = false;
+            }
+        } else if (C > 1) {
+            exchange(0.0, 0.0, 0.0, 0, 0);
         }
+        turn ^= C > 1;
         scanned = true;
     }
     if (order == kFollow) {
@@ -672,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
             }
         }
         if (C > 1) {
-            exchange(0.0, found, last);
+            exchange(0.0, 0.0, 0.0, found, last);
             if (warp == 0) {
                 found = __reduce_min_sync(0xffffffffu, lane < (int)C ? sh.post_found[turn][lane] : INT32_MAX);
                 last = __reduce_max_sync(0xffffffffu, lane < (int)C ? sh.post_last[turn][lane] : -1);
@@ -680,18 +777,18 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
         }
         if (warp == 0) {
             token = found == INT32_MAX ? last : found;
-            if (lane == 0 && token >= 0) {
-                const float l = row.one(token);
-                sh.num[count - 1] = x.greedy || l == x.m ? 0.0 : ((double)l - (double)x.m) * x.inv;
-                sh.den[count - 1] = sh.W[at];
-            }
+            if (lane == 0 && token >= 0) sh.last_logit = row.one(token);
         }
     }
     griddep_launch_dependents();
     if (rank == 0 && warp == 0) {
         __syncwarp();
         if (logs)
-            for (int i = lane; i < count - (token < 0); i += 32) logs[i] = (float)(sh.num[i] - log(sh.den[i]));
+            for (int i = lane; i < count - (token < 0); i += 32) {  // of path[i + 1] at path[i], of the following token at the last
+                const int from = i == 0 ? 0 : sh.path[i];
+                const float l = i + 1 < count ? sh.logit[sh.path[i + 1]] : sh.last_logit, m = sh.m[from];
+                logs[i] = (float)((x.greedy || l == m ? 0.0 : ((double)l - (double)m) * x.inv) - log(sh.W[from]));
+            }
         if (lane == 0) {
             accepted[0] = 0;
             p.n_accepted[s] = count;
@@ -719,11 +816,13 @@ template <int T> static cudaError_t launch_for(cudaStream_t stream, const cvattn
     constexpr int per = Row<T>::kPer;
     Part* parts = static_cast<Part*>(p.workspace);
     const int slices = slices_of(p.vocab, per);
-    const cudaError_t e = launch_overlapped(verify_sums_kernel<T>, dim3((unsigned)slices, (unsigned)p.max_nodes, (unsigned)p.n_seq), kSumThreads,
+    cudaError_t e = cudaFuncSetAttribute(verify_walk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxTiles + 2) * 16);
+    if (e != cudaSuccess) return e;
+    e = launch_overlapped(verify_sums_kernel<T>, dim3((unsigned)slices, (unsigned)p.max_nodes, (unsigned)p.n_seq), kSumThreads,
                                             0, stream, p, parts);
     if (e != cudaSuccess) return e;
     const int vectors = p.vocab / per, c = cluster_of(p.n_seq, vectors), tiles = (vectors + 32 * c - 1) / (32 * c);
-    return launch_overlapped_clusters(verify_walk_kernel<T>, dim3((unsigned)(p.n_seq * c)), kThreads, (size_t)(tiles + 2) * 8, c, stream, p,
+    return launch_overlapped_clusters(verify_walk_kernel<T>, dim3((unsigned)(p.n_seq * c)), kThreads, (size_t)(tiles + 2) * 16, c, stream, p,
                                       (const Part*)parts, slices, tiles, status);
 }
 

@@ -202,3 +202,19 @@ def test_verify_replays(ctx, cv, cuda):
         got = [x.clone() for x in (accepted, count, token)]
         plan()
         assert all(torch.equal(a, b) for a, b in zip(got, (accepted, count, token)))
+
+
+def test_verify_of_the_largest_vocabulary(ctx, cv, cuda):
+    """As many tokens as a call takes: drafts with probabilities, one refused."""
+    torch, rng = cuda, np.random.default_rng(16)
+    V = 2 ** 21
+    logits = torch.randn(1, 2, V, device="cuda") * 2
+    probs = torch.softmax(logits + 0.5 * torch.randn(1, 2, V, device="cuda"), -1)
+    host, q = logits.cpu().numpy(), probs.cpu().numpy()
+    worse = int(np.argmax(q[0, 0] - softmax(host[0, 0].astype(np.float64))))
+    for u, last in ((0.0, 0.3), (0.999, 0.7)):
+        check(cv, ctx, torch, logits, np.array([[0, worse]]), np.array([[-1, 0]]), np.array([[0.0, u]]), [last], None, q, chain=True)
+    with pytest.raises(cv.CvattnError, match="UNSUPPORTED"):
+        big = torch.zeros(1, 1, V + 1, device="cuda")
+        one = [torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((1, 1), (1, 1), (1,), (1,))]
+        cv.DraftVerifier(ctx, big, one[0], torch.zeros(1, 1, device="cuda"), torch.zeros(1, device="cuda"), *one[1:])()
