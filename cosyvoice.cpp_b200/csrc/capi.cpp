@@ -661,7 +661,7 @@ static cvattn_status pool_ok(const cvattn_page_pool& q) {
     if (q.page_size != 16 && q.page_size != 32 && q.page_size != 64 && q.page_size != 128) return CVATTN_ERR_INVALID_ARGUMENT;
     if (!aligned(q.k, 16) || !aligned(q.v, 16) || !aligned(q.k_scale, 4) || !aligned(q.v_scale, 4) || (q.nb_page & 15))
         return CVATTN_ERR_INVALID_ARGUMENT;
-    if (q.head_dim != 64 || q.n_heads > 1024) return CVATTN_ERR_UNSUPPORTED;
+    if (q.head_dim != 64 || q.n_heads > 1024 || q.n_pages > (1 << 30)) return CVATTN_ERR_UNSUPPORTED;
     const int64_t page = (int64_t)q.n_heads * q.page_size * q.head_dim, scales = (int64_t)q.n_heads * q.page_size / CVATTN_PAGE_BLOCK;
     if (q.n_pages > 1 && (q.nb_page < page || q.nb_scale < scales)) return CVATTN_ERR_INVALID_ARGUMENT;
     return CVATTN_OK;
@@ -726,6 +726,7 @@ cvattn_status cvattn_paged_attention(cvattn_context* ctx, void* stream, const cv
     if (p->n_q_heads % p->pool.n_heads || p->n_q_heads / p->pool.n_heads > 8 || p->n_seq > kMaxGridSeq || p->max_q > (1 << 20))
         return CVATTN_ERR_UNSUPPORTED;
     if (p->max_kv_len > (int64_t)p->table_width * p->pool.page_size) return CVATTN_ERR_LENGTH;
+    if (!paged_attention_fits(p->n_seq, p->max_q, p->max_kv_len, p->n_q_heads, p->pool.n_heads)) return CVATTN_ERR_UNSUPPORTED;
     const int64_t row = (int64_t)p->n_q_heads * p->pool.head_dim;
     if (!aligned(p->q, 16) || !aligned(p->out, 16) || !mult4(p->q_nb_tok) || !mult4(p->q_nb_seq) || !mult4(p->out_nb_tok) ||
         !mult4(p->out_nb_seq) || (p->max_q > 1 && (p->q_nb_tok < row || p->out_nb_tok < row)))
@@ -755,7 +756,7 @@ static cvattn_status pools_ok(const cvattn_page_pool* pools, int32_t n) {
 // A table that is read and one that is written: the same, or apart.
 static bool tables_ok(const int32_t* in, const int32_t* out, int64_t nb_seq, int32_t width, int32_t n_seq, int32_t page_size) {
     if (!table_ok(in, nb_seq, width, n_seq, page_size) || !table_ok(out, nb_seq, width, n_seq, page_size)) return false;
-    if ((int64_t)n_seq * width > INT32_MAX) return false;
+    if ((int64_t)n_seq * width > (1 << 30)) return false;
     const int64_t span = 4 * ((n_seq - 1) * nb_seq + width);
     return in == out || !overlap(in, span, out, span);
 }

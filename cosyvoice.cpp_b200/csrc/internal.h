@@ -72,6 +72,7 @@ cudaError_t launch_paged_append(cudaStream_t stream, const cvattn_paged_append_p
 cudaError_t launch_paged_read(cudaStream_t stream, const cvattn_paged_read_params& p, int* status);
 
 // paged_attention.cu
+bool paged_attention_fits(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads);
 size_t paged_attention_workspace_bytes(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads);
 cudaError_t launch_paged_attention(cudaStream_t stream, const cvattn_paged_attention_params& p, int* status);
 

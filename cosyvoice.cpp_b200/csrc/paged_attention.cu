@@ -75,7 +75,7 @@ struct Plan {
     int R, row_tiles, cluster, n_splits;
 };
 
-static Plan plan_of(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
+static Plan plan_of(int n_seq, int max_q, int64_t max_kv_len, int n_q_heads, int n_kv_heads) {
     Plan p{};
     const int64_t rows = (int64_t)max_q * (n_q_heads / n_kv_heads);
     const int64_t tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile), entries = tiles * ((rows + kTcRows - 1) / kTcRows);
@@ -123,6 +123,12 @@ template <int kLanes> static cudaError_t run_combine(cudaStream_t stream, const 
 }
 
 }  // namespace paged
+
+// Whether numbers of positions, and the grid, stay in range.
+bool paged_attention_fits(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
+    const paged::Plan p = paged::plan_of(n_seq, max_q, max_kv_len, n_q_heads, n_kv_heads);
+    return max_kv_len <= 1 << 30 && (p.tc_grid || (int64_t)n_kv_heads * p.row_tiles <= 65535);
+}
 
 size_t paged_attention_workspace_bytes(int n_seq, int max_q, int max_kv_len, int n_q_heads, int n_kv_heads) {
     using namespace paged;

@@ -744,7 +744,11 @@ __global__ void __launch_bounds__(256) paged_tc_combine_kernel(const __grid_cons
         const int T = tc_tiles(x.L, x.n, a.G, rt);
         if (T > 0) {
             b0 = ta.ws_pref[s] + kvh * T;
-            for (int i = 0; i < rt; ++i) b0 += tc_tiles(x.L, x.n, a.G, i) * a.p.pool.n_heads;
+            int above = 0;  // the unit's 16 threads share the row tiles before it
+            for (int i = c; i < rt; i += 16) above += tc_tiles(x.L, x.n, a.G, i);
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) above += __shfl_xor_sync(0xffffu << (threadIdx.x & 16), above, w);
+            b0 += above * a.p.pool.n_heads;
             c0 = tc_owner(b0, n, ta.grid);
             c1 = tc_owner(b0 + T - 1, n, ta.grid);
             if (kLanes == 1 && c0 == c1) return;  // written whole

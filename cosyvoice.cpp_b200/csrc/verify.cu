@@ -106,8 +106,9 @@ __constant__ double kPowers[64] = {  // 2^(i / 64)
 struct Node {
     float m;             // the largest logit
     float c;             // log2 e / temperature
-    float low;           // logits that are not above it have no weight
     float reach;         // weights of logits this far below the largest: less than kNothing
+    float low;           // the next number below m - reach: logits that are not above it have no weight
+    double floor;        // -reach, which they count as
     double inv;          // 1 / temperature
     double u64;          // 64 / (temperature ln 2)
     double W;            // sum of the weights (of f32 exponentials)
@@ -115,8 +116,7 @@ struct Node {
     bool greedy;
     __device__ __forceinline__ void most(float l) {
         m = l;
-        low = l - reach;
-        if (!(low < l)) low = nextafterf(l, -INFINITY);
+        low = __fsub_rd(l, reach);  // (so what is above it lies within reach, however far apart numbers of that size are)
     }
 };
 // exp((l - m) / temperature) in f32, m finite; NaN for a NaN.
@@ -127,7 +127,7 @@ constexpr double kNothing = 1e-290;
 __device__ __forceinline__ double weight64(const Node& x, float l, const double* table) {
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: u + magic has u's nearest integer in its low bits
     constexpr double step = 0.010830424696249145;  // ln 2 / 64
-    const double d = (double)fmaxf(l, x.low) - (double)x.m, t = fma(d, x.u64, magic), r = fma(d, x.u64, magic - t);
+    const double d = l > x.low ? (double)l - (double)x.m : x.floor, t = fma(d, x.u64, magic), r = fma(d, x.u64, magic - t);
     const int n = __double2loint(t);
     double p = fma(r, step * step * step / 6, step * step / 2);
     p = fma(p, r, step);
@@ -170,6 +170,7 @@ __device__ __forceinline__ void set_heat(Node& x, float heat) {
     x.u64 = x.inv * 92.332482616893656;  // 64 / ln 2
     x.c = (float)fmin(x.inv * 1.4426950408889634, 3.0e38);
     x.reach = 680.0f * heat;
+    x.floor = -680.0 * (double)heat;
 }
 
 template <int T>

@@ -544,7 +544,7 @@ cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv
  * The byte of position t, value d of a block is at
  *   keys    t*64 + d
  *   values  d/32*512 + (d%8*4 + t/4)*16 + d/8%4*4 + t%4
- * (in the order in which the tensor cores take them).  A table lists, for each
+ * (in the order in which the tensor cores take them).  Scales are not negative.  A table lists, for each
  * sequence, the page of its positions 0 .. page_size - 1, then the next, ..;
  * every layer's pool is indexed by the same table.  Entries outside
  * [0, n_pages) hold nothing. */
@@ -575,7 +575,8 @@ typedef struct cvattn_page_pool {
  * as the block's largest.  Other rows of the block are left as they are.
  * A sequence whose rows do not fit its table is recorded in the status word and
  * skipped, and so is a block whose page is out of range or, with refs, held by
- * more than one table entry.  k, v rotated beforehand (cvattn_rope). */
+ * more than one table entry.  (Without refs two sequences that append to one page
+ * spoil each other's blocks.)  k, v rotated beforehand (cvattn_rope). */
 typedef struct cvattn_paged_append_params {
     cvattn_page_pool pool;
     const float*    k;              /* device f32: row i of sequence s, n_heads*64 values, */
@@ -621,8 +622,9 @@ cvattn_status cvattn_paged_read(cvattn_context* ctx, void* stream, const cvattn_
  * positions j < kv_len[s] - n_q[s] + i + 1:
  *   out[s][i][h] = sum_j p_j v_j,  p = softmax_j(scale q.k_j),
  *   lse[s][i][h] = log(sum_j exp(scale q.k_j))                (natural log).
- * Products are exact in f32, but for P times the values' scales, whose parts below
- * 2^-22 of the largest of 128 neighbouring positions are left out.
+ * Queries are taken to 2^-22 of a row's largest value and codes exactly; sums are
+ * in f32.  With many rows P times the values' scales is taken to 2^-22 of the
+ * largest of 128 neighbouring positions.
  *   - A row that sees nothing, and rows from n_q[s] to max_q: zeros, lse = -inf.
  *   - What a page holds past kv_len is not looked at.
  *   - A kv_len outside [0, max_kv_len] or n_q outside [0, max_q] is recorded and
@@ -644,7 +646,7 @@ typedef struct cvattn_paged_attention_params {
     int32_t         n_seq;
     int32_t         max_q;
     int32_t         n_q_heads;    /* 1 to 8 per KV head */
-    int32_t         max_kv_len;   /* host bound on kv_len[], at most table_width*page_size */
+    int32_t         max_kv_len;   /* host bound on kv_len[], at most table_width*page_size and 2^30 */
     int32_t         table_width;
     float           scale;
     int32_t         flags;        /* 0 */
@@ -670,10 +672,12 @@ cvattn_status cvattn_paged_attention(cvattn_context* ctx, void* stream, const cv
  *   - Free pages are given in ascending order, sequence by sequence, as long as
  *     the pages that the sequences up to it ask for are there; room[s] is then
  *     max(keep, need), else keep.  (A sequence without room may hold a tail page
- *     that others hold too.)
+ *     that others hold too, one with room among them; cvattn_paged_append with
+ *     refs refuses to write there until all but one have let go.)
  *   - Entries past a sequence's pages become -1, and so do kept ones out of range
  *     (recorded).  A keep, need or src out of range is recorded and counts as
  *     keep = need = 0.
+ *   - n_seq * table_width and n_pages are at most 2^30.
  * table_out may be table, other outputs share no memory with inputs. */
 typedef struct cvattn_pages_assign_params {
     const cvattn_page_pool* pools;  /* host array [n_pools]: every layer, same page_size and n_pages */

@@ -225,6 +225,31 @@ def test_attention_of_long_contexts(ctx, cv, cuda, fmt, size, max_q):
     check_attention(cv, ctx, cuda, rng, host, table, lens, [max_q] * 2, 14, max_q)
 
 
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_attention_of_a_long_prompt(ctx, cv, cuda, fmt):
+    """Many tiles of rows per sequence, behind positions of their own and without."""
+    rng = np.random.default_rng(fmt)
+    lens = [700, 131, 900]
+    host, table = filled(rng, fmt, lens, 64, 2)
+    check_attention(cv, ctx, cuda, rng, host, table, lens, [700, 131, 650], 14, 700)
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_attention_of_more_sequences_than_one_list_holds(ctx, cv, cuda, fmt):
+    rng = np.random.default_rng(fmt)
+    lens = rng.integers(0, 90, 1030)
+    host, table = filled(rng, fmt, lens.tolist(), 16, 1)
+    check_attention(cv, ctx, cuda, rng, host, table, lens, np.minimum(lens, rng.integers(0, 13, 1030)), 8, 12)
+
+
+@pytest.mark.parametrize("max_q", [1, 40])
+def test_attention_over_nothing(ctx, cv, cuda, max_q):
+    """A bound of no positions at all."""
+    rng = np.random.default_rng(0)
+    host, table = filled(rng, 0, [0, 0], 16, 2)
+    check_attention(cv, ctx, cuda, rng, host, table, [0, 0], [max_q, 0], 14, max_q, max_kv_len=0)
+
+
 @pytest.mark.parametrize("max_q", [1, 12, 40])
 def test_attention_over_strided_memory(ctx, cv, cuda, max_q):
     """Pages and query rows that lie apart, a table wider than it has to be, a scale of one's own, a bound above the lengths."""

@@ -120,6 +120,26 @@ def test_infinities_and_nan(ctx, cv, cuda, dtype):
             check(cv, ctx, torch, logits, tokens, parents, u, last, np.full(S, heat), q, chain=True)
 
 
+def test_temperatures_that_leave_a_single_token(ctx, cv, cuda):
+    """Temperatures so low, and logits so large, that neighbouring numbers are far more than all weights apart."""
+    torch, rng = cuda, np.random.default_rng(7)
+    S, N, V = 12, 3, 300
+    logits, tokens, parents, u, last, probs = case(rng, torch, S, N, V, "float32", True, True)
+    logits[:, :, 7] = 9.0
+    logits[:, :, 250] = float(np.nextafter(np.float32(9), np.float32(8)))
+    logits[4] *= 1e10
+    logits[5] *= 1e30
+    logits[6] = torch.finfo(torch.float32).min
+    logits[6:8, :, ::3] = -np.inf
+    logits[8, :, 20:] = torch.finfo(torch.float32).min
+    heat = np.array([1e-9, 3e-9, 1e-8, 1e-6, 1.0, 0.5, 2.0, 1e-7, 1e-30, 1e-42, 3e38, 1e-9], np.float32)
+    tokens[::2, 1] = 7
+    for q in (probs, None):
+        for numbers in (u, np.zeros((S, N)), np.full((S, N), 0.9999)):
+            check(cv, ctx, torch, logits, tokens, parents, numbers, last, heat, q, chain=True)
+            check(cv, ctx, torch, logits, tokens, parents, numbers, np.full(S, 1 - 2.0 ** -24), heat, q, chain=True)
+
+
 def test_nothing_left_stays_as_it_was(ctx, cv, cuda):
     """Draft and target alike: a refusal cannot happen by the rule, but with numbers at 1 it is asked for."""
     torch, rng = cuda, np.random.default_rng(8)

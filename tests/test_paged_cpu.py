@@ -206,6 +206,26 @@ def test_no_sequences_are_no_work(make):
     assert getattr(cv.lib, name)(ctypes.byref(Fake(0, None)), None, ctypes.byref(p)) == 0
 
 
+def test_sizes_past_the_grids_and_32_bits_are_refused():
+    ctx, most = Fake(0, None), 1 << 20
+    rows = {"max_q": most, "out_nb_seq": most * 896, "workspace_size": 1 << 62}
+    bad = [(c_attention, {"pool": c_pool(n_heads=1000, nb_page=1000 * 32 * D, nb_scale=2000), "n_q_heads": 1000, "n_seq": 1025, "max_q": 4161,
+                          "q_nb_tok": 64000, "out_nb_tok": 64000, "out_nb_seq": 4161 * 64000, "workspace_size": 1 << 62}),
+           (c_attention, {**rows, "max_kv_len": 0, "n_seq": 1}),
+           (c_attention, {**rows, "max_q": most + 1}),
+           (c_attention, {"max_kv_len": (1 << 30) + 1, "table_width": (1 << 31) // 32 - 1, "table_nb_seq": 1 << 26, "workspace_size": 1 << 62}),
+           *[(c, {"pool": c_pool(n_pages=(1 << 30) + 1)}) for c in (c_append, c_read, c_attention)]]
+    for make, values in bad:
+        name, p, _ = make()
+        for k, v in values.items():
+            setattr(p, k, v)
+        assert getattr(cv.lib, name)(ctypes.byref(ctx), None, ctypes.byref(p)) == UNSUPPORTED, values
+    for make in (c_assign, c_compact):
+        name, p, _ = make()
+        p.n_seq, p.table_width, p.table_nb_seq = 1 << 20, 1025, 1025
+        assert getattr(cv.lib, name)(ctypes.byref(ctx), None, ctypes.byref(p)) == INVALID
+
+
 def test_pools_of_one_table_agree():
     for bad in (c_pool(page_size=16), c_pool(n_pages=7)):
         name, p, _ = c_assign()
