@@ -7,7 +7,8 @@ namespace paged {
 
 // --------------------------------------------------------------- combine --
 //
-// 16 threads (4 dims each) follow every kLanes-th split of a row; the partial sums are joined in order.
+// 16 threads (4 dims each) follow every kLanes-th split of a row; the partial sums are joined in order.  Bound by latency: about
+// 2 us behind the kernel before it, whose parts are in L2.
 template <int kLanes>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ AttArgs a) {
     constexpr int kPer = 16 / kLanes;  // rows per CTA
