@@ -79,9 +79,10 @@ struct Plan {
 static Plan plan_of(int n_seq, int max_q, int64_t max_kv_len, int n_q_heads, int n_kv_heads) {
     Plan p{};
     const int64_t rows = (int64_t)max_q * (n_q_heads / n_kv_heads);
-    const int64_t tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile), entries = tiles * ((rows + kTcRows - 1) / kTcRows);
-    if (tiles * rows >= kTcWork + kTcPerTile * entries && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 31) {
-        p.tc_grid = (int)(entries < kSms ? entries : kSms);
+    const int64_t tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile), row_tiles = (rows + kTcRows - 1) / kTcRows, entries = tiles * row_tiles;
+    if (tiles * rows >= kTcWork + kTcPerTile * entries && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 28) {
+        const int64_t list = entries + kTcGap * (int64_t)n_seq * n_kv_heads * row_tiles;
+        p.tc_grid = (int)(list < kSms ? list : kSms);
         p.n_splits = p.tc_grid / (int64_t)(n_seq * n_kv_heads) > 0 ? p.tc_grid / (n_seq * n_kv_heads) : 1;  // (for the combine)
         return p;
     }

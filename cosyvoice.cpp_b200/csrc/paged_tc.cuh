@@ -35,8 +35,9 @@ constexpr int kTcThreads = 16 * 32;
 constexpr int kTcRegsSoftmax = 200, kTcRegsProducer = 72, kTcRegsOther = 32;
 static_assert(256 * kTcRegsSoftmax + 128 * kTcRegsProducer + 128 * kTcRegsOther <= 512 * 128, "the block's registers");
 constexpr int kTcMaxSeq = 1024;  // tables in shared memory
-constexpr int kTcSt = 4;         // K and V tiles under way
+constexpr int kTcSt = 3;         // K and V tiles under way
 constexpr int kTcRaw = 3;        // tiles of codes under way
+constexpr int kTcGap = 4;        // what a change of runs costs, in tiles
 constexpr int kTcInfos = 8;      // tiles whose scales may be in use
 constexpr int kTcTileBytes = kTcTile * kD * 2;
 constexpr int kTcBlocks = kTcTile / kBlock;
@@ -49,19 +50,19 @@ struct TcAttArgs {
     int32_t* ws_pref;  // [n_seq + 1], written by CTA 0 for the combine
 };
 
-struct TcInfo {                 // of a tile
+struct __align__(16) TcInfo {   // of a tile
     float ks[kTcBlocks];        // key scales
     float w[kTcBlocks];         // value scales times a power of two, below 1
     float exp;                  // the inverse of that power
     uint32_t valid;             // blocks that have a page
-    uint32_t starts;            // whether the tile starts a run
+    uint32_t starts, last;      // whether the tile starts a run; is the CTA's last
     int32_t count;              // positions that exist
 };
 
 struct TcAttBars {
     uint64_t k_full[kTcSt], v_full[kTcSt], k_empty[kTcSt], v_empty[kTcSt];  // by stage
     uint64_t raw_full[kTcRaw], raw_empty[kTcRaw];                           // by slot of codes
-    uint64_t q_full;
+    uint64_t q_full[2], q_free[2];                                          // by Q buffer: run n in n % 2
     uint64_t s_full[3], p_full[3], s_free[3];                               // by S buffer
     uint64_t o_full[2];                                                     // by group
     uint32_t tmem_base;
@@ -71,18 +72,19 @@ struct TcAttBars {
 };
 
 struct TcSmem {
-    static constexpr int kQ = 0;                            // Q hi, Q lo; then the groups' halves at a run's end
-    static constexpr int kTiles = 2 * kTcTileBytes;         // [stage][K, V]
+    static constexpr int kQ = 0;                            // [run % 2][Q hi, Q lo]; at the run's end its output
+    static constexpr int kTiles = 4 * kTcTileBytes;         // [stage][K, V]
     static constexpr int kRaw = kTiles + kTcSt * 2 * kTcTileBytes;  // [slot][K, V][block]
     static constexpr int kRawBytes = 2 * kTcBlocks * kBlockBytes;
     static constexpr int kMl = kRaw + kTcRaw * kRawBytes;
-    static constexpr int kRs = kMl + kTcRows * 8;           // score factors of the rows
-    static constexpr int kBars = kRs + kTcRows * 4;
+    static constexpr int kRs = kMl + kTcRows * 8;           // [run % 2] score factors of the rows
+    static constexpr int kBars = kRs + 2 * kTcRows * 4;
     static constexpr int kPref = kBars + (int)((sizeof(TcAttBars) + 15) / 16 * 16);
     static constexpr int kLen = kPref + (kTcMaxSeq + 4) * 4, kRowsOf = kLen + kTcMaxSeq * 4;
     static constexpr int kBytes = kRowsOf + kTcMaxSeq * 4;
 };
 static_assert(TcSmem::kBytes <= 227 * 1024, "one CTA per SM");
+static_assert(TcSmem::kBars % 16 == 0 && sizeof(TcInfo) % 16 == 0, "pairs of scales are read at once");
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -124,65 +126,73 @@ __device__ __forceinline__ int tc_end(int L, int n, int G, int rt) {
     return max(0, L - n + 1 + last / G);
 }
 __device__ __forceinline__ int tc_tiles(int L, int n, int G, int rt) { return (tc_end(L, n, G, rt) + kTcTile - 1) / kTcTile; }
+// List entries of a unit.
+__device__ __forceinline__ int tc_entries(int L, int n, int G, int rt) {
+    const int T = tc_tiles(L, n, G, rt);
+    return T ? T + kTcGap : 0;
+}
 __device__ __forceinline__ int tc_cut(int c, int n, int g) { return (int)((long long)c * n / g); }
 __device__ __forceinline__ int tc_owner(int i, int n, int g) { return (int)(((long long)(i + 1) * g - 1) / n); }
 
-struct TcTab {  // in shared memory, by sequence: entries before it, positions, rows (tokens)
+struct TcTab {  // in shared memory, by sequence: list entries before it, positions, rows (tokens)
     const int32_t *pref, *len, *n;
 };
-// A CTA's walk through its part of the list, run by run.
+// A CTA's walk through its part [lo, hi) of the list, run by run.
 struct TcRun {
     int s, kvh, rt;   // unit
-    int i, end;       // list entries [i, end) of this run
-    int t0, T;        // its first tile, and the unit's tiles
+    int v;            // its first entry
+    int t0, t1, T;    // the CTA's tiles of it (none: the part has ended), the unit's
+    int at;           // tiles of the CTA before this run
     int L, n, see;    // positions, tokens, positions that the unit's last row sees
 
     __device__ __forceinline__ void unit(const AttArgs& a) {
         see = tc_end(L, n, a.G, rt);
         T = (see + kTcTile - 1) / kTcTile;
     }
-    __device__ __forceinline__ void start(const AttArgs& a, const TcTab& tab, int entry, int hi) {
-        i = end = entry;
-        if (entry >= hi) return;
-        int lo = 0, up = a.p.n_seq;  // last s with pref[s] <= entry: its list is not empty
-        while (up - lo > 1) {
-            const int mid = (lo + up) >> 1;
-            if (tab.pref[mid] <= entry) lo = mid;
+    __device__ __forceinline__ void start(const AttArgs& a, const TcTab& tab, int lo, int hi) {
+        at = t0 = t1 = 0;
+        if (lo >= hi) return;
+        int below = 0, up = a.p.n_seq;  // last s with pref[s] <= lo: its list is not empty
+        while (up - below > 1) {
+            const int mid = (below + up) >> 1;
+            if (tab.pref[mid] <= lo) below = mid;
             else up = mid;
         }
-        s = lo;
+        s = below;
         L = tab.len[s];
         n = tab.n[s];
-        int e = entry - tab.pref[s];
+        int e = lo - tab.pref[s];
         rt = 0;
-        for (unit(a); e >= T * a.p.pool.n_heads; unit(a)) {
-            e -= T * a.p.pool.n_heads;
+        for (unit(a); T == 0 || e >= (T + kTcGap) * a.p.pool.n_heads; unit(a)) {
+            if (T) e -= (T + kTcGap) * a.p.pool.n_heads;
             ++rt;
         }
-        kvh = e / T;
-        t0 = e - kvh * T;
-        end = min(hi, i + T - t0);
+        kvh = e / (T + kTcGap);
+        t0 = e - kvh * (T + kTcGap);
+        v = lo - t0;
+        t1 = min(T, hi - v);
+        if (t0 >= T) {
+            t0 = t1;
+            next(a, tab, hi);
+        }
     }
     __device__ __forceinline__ void next(const AttArgs& a, const TcTab& tab, int hi) {
-        i = end;
-        if (i >= hi) return;
-        t0 = 0;
+        at += t1 - t0;
+        v += T + kTcGap;
+        t0 = t1 = 0;
+        if (v >= hi) return;
         if (++kvh == a.p.pool.n_heads) {
             kvh = 0;
-            ++rt;
-            if (i == tab.pref[s + 1]) {  // (row tiles without entries come first)
-                while (tab.pref[s + 1] == i) ++s;
+            if (++rt * kTcRows >= n * a.G) {
+                do ++s;
+                while (tab.pref[s + 1] == tab.pref[s]);
                 L = tab.len[s];
                 n = tab.n[s];
                 rt = 0;
             }
-            unit(a);
-            while (T == 0) {
-                ++rt;
-                unit(a);
-            }
+            for (unit(a); T == 0; unit(a)) ++rt;  // (row tiles without entries come first)
         }
-        end = min(hi, i + T);
+        t1 = min(T, hi - v);
     }
 };
 
@@ -193,42 +203,42 @@ template <int F> __device__ __forceinline__ void keep_bytes(uint4& v, uint32_t k
 }
 
 // Warp 14: lane i < 8 looks after block i of each tile.
-__device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int lo, int hi) {
+__device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int hi) {
     const AttArgs& a = ta.a;
     const int lane = threadIdx.x & 31, shift = __ffs(a.blocks) - 1;
-    int starts = 1;
-    // of the tile that is looked up: this lane's page and place, its positions
-    int page = -1, in = 0, count = 0, first = 0;
-    auto look = [&](int entry) {
-        page = -1;
+    // of the tile that is looked up: whether this lane has a block, its page and place; the tile's positions
+    bool has = false;
+    int page = -1, in = 0, count = 0, first = 1, t = r.t0;
+    auto look = [&]() {
+        has = false;
         count = 0;
-        if (entry >= hi) return;
-        if (entry == r.end) {
+        if (r.t0 == r.t1) return;
+        first = t == r.t0;
+        if (t == r.t1) {
             r.next(a, tab, hi);
-            starts = 1;
+            if (r.t0 == r.t1) return;
+            t = r.t0;
+            first = 1;
         }
-        const int p0 = (r.t0 + entry - r.i) * kTcTile, b = p0 / kBlock + lane, at = b >> shift;
+        const int p0 = t * kTcTile, b = p0 / kBlock + lane, at = b >> shift;
+        ++t;
         count = min(kTcTile, r.see - p0);
-        first = starts;
-        starts = 0;
-        if (lane < kTcBlocks && lane * kBlock < count) {
-            page = __ldg(a.p.table + (int64_t)r.s * a.p.table_nb_seq + at);
+        has = lane < kTcBlocks && lane * kBlock < count;
+        if (has) {
+            page = __ldg(a.p.table + (int64_t)r.s * a.p.table_nb_seq + at);  // (looked at when the tile's turn has come)
             in = ((r.kvh - at) << shift) + b;
-            if ((uint32_t)page >= (uint32_t)a.p.pool.n_pages) {
-                record_status(a.status, kStatusBadPage);
-                page = -1;
-            }
         }
     };
     bool ok = true;
     int slot = 0, n = 0;
     uint32_t use = 0;
-    look(lo);
+    look();
 #pragma unroll 1
-    for (; lo + n < hi; ++n) {
+    for (; count > 0; ++n) {
         if (use) ok = tc_wait(&B->raw_empty[slot], (use - 1) & 1, &B->err, 34);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const bool good = page >= 0;
+        const bool good = has && (uint32_t)page < (uint32_t)a.p.pool.n_pages;
+        if (has && !good) record_status(a.status, kStatusBadPage);
         const uint32_t valid = __ballot_sync(0xffffffffu, good);
         const int64_t at = good ? page * a.p.pool.nb_page + (int64_t)in * kBlockBytes : 0, sat = good ? page * a.p.pool.nb_scale + in : 0;
         if (lane == 0) mbar_arrive_expect_tx(&B->raw_full[slot], __popc(valid) * 2 * kBlockBytes);
@@ -240,7 +250,7 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
         }
         const float ks = good ? a.p.pool.k_scale[sat] : 0.0f, vs = good ? a.p.pool.v_scale[sat] : 0.0f;
         const int here = count, starts_here = first;
-        look(lo + n + 1);
+        look();
         const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
         int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
         e = e > 100 ? 100 : e < -100 ? -100 : e;
@@ -253,6 +263,7 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
             info.exp = pow2f(-e);
             info.valid = valid;
             info.starts = (uint32_t)starts_here;
+            info.last = count == 0;
             info.count = here;
         }
         __syncwarp();
@@ -268,70 +279,127 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
             for (uint32_t i = 0; i < kTcTries && !mbar_try_wait_hint(&B->raw_full[k % kTcRaw], (k / kTcRaw) & 1, 20000u); ++i) {}
 }
 
-// The producers' 128 threads: warp w blocks 2 w and 2 w + 1 of a tile.
-template <int F> __device__ __forceinline__ void tc_produce(uint8_t* smem, TcAttBars* B, int lo, int hi) {
-    const int t = threadIdx.x & 127, w = t >> 5, lane = t & 31;
-    // K: rows 8 apart, which swizzle alike; V: pieces (half, g, quarters 2 u and 2 u + 1)
-    const int krow = (w * 32 + (lane >> 2)) * 128, k0 = ((2 * (lane & 3)) ^ (lane >> 2)) * 16, k1 = k0 ^ 16;
-    const int u = lane & 1, g = lane >> 1 & 7, h = lane >> 4, vrow = (w >> 1) * (kTcTileBytes / 2) + (32 * h + g) * 128;
+// Q of a run, by kThreads threads: four lanes a row, 16 dims each.
+template <int kThreads> __device__ __forceinline__ void tc_queries(const AttArgs& a, uint8_t* smem, const TcRun& r, int buf) {
+    const int t = threadIdx.x & (kThreads - 1), c = t & 3, rows = r.n * a.G;
+    uint8_t* hi = smem + TcSmem::kQ + buf * 2 * kTcTileBytes;
+    float* rsb = reinterpret_cast<float*>(smem + TcSmem::kRs) + buf * kTcRows;
+#pragma unroll 2
+    for (int q0 = t >> 2; q0 < kTcRows; q0 += kThreads / 4) {
+        const int qr = r.rt * kTcRows + q0, qt = qr / a.G;
+        const float4* q = reinterpret_cast<const float4*>(a.p.q + (int64_t)r.s * a.p.q_nb_seq + (int64_t)qt * a.p.q_nb_tok +
+                                                          (r.kvh * a.G + qr - qt * a.G) * kD + 16 * c);
+        float4 v[4];
+        float am = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = qr < rows ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) am = fmaxf(am, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
+        const int ex = dtc::norm_exp(quad_max(am));
+        const float f = pow2f(ex);
+        if (c == 0) rsb[q0] = pow2f(-ex) * a.scale_log2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            uint4 wh, wl;
+            split_near(make_float2(v[2 * u].x * f, v[2 * u].y * f), wh.x, wl.x);
+            split_near(make_float2(v[2 * u].z * f, v[2 * u].w * f), wh.y, wl.y);
+            split_near(make_float2(v[2 * u + 1].x * f, v[2 * u + 1].y * f), wh.z, wl.z);
+            split_near(make_float2(v[2 * u + 1].z * f, v[2 * u + 1].w * f), wh.w, wl.w);
+            const uint32_t at = tc::sw128_offset(q0, 2 * c + u);
+            *reinterpret_cast<uint4*>(hi + at) = wh;
+            *reinterpret_cast<uint4*>(hi + kTcTileBytes + at) = wl;
+        }
+    }
+    fence_proxy_async_smem();
+}
+
+// The producers: Q of each run but the first, then warps 0 and 1 turn a tile's keys into f16 rows, 2 and 3 its values, four blocks each.
+template <int F> __device__ __forceinline__ void tc_produce(const TcAttArgs& ta, uint8_t* smem, TcAttBars* B, const TcTab& tab, TcRun r, int hi) {
+    const int w = threadIdx.x >> 5 & 1, lane = threadIdx.x & 31;
+    const bool keys = !(threadIdx.x & 64);
+    // keys: rows 8 apart, which swizzle alike; values: pieces (half of the dims, g, quarters 2 u and 2 u + 1) to rows of dims, 64
+    // positions each
+    const int k0 = ((2 * (lane & 3)) ^ (lane >> 2)) * 16, k1 = k0 ^ 16;
+    const int u = lane & 1, g = lane >> 1 & 7, h = lane >> 4;
+    const int to0 = keys ? (w * 64 + (lane >> 2)) * 128 : kTcTileBytes + w * (kTcTileBytes / 2) + (32 * h + g) * 128;
+    const int from0 = keys ? 4 * w * 64 + lane : (kTcBlocks + 4 * w) * 64 + h * 32 + 4 * g + 2 * u;
+    uint64_t *empty = keys ? B->k_empty : B->v_empty, *full = keys ? B->k_full : B->v_full;
     bool ok = true;
     int st = 0, slot = 0;
-    uint32_t use = 0, turn = 0;
+    uint32_t use = 0, turn = 0, run = 0;
+    bool last = r.t0 == r.t1;
 #pragma unroll 1
-    for (int n = 0; lo + n < hi; ++n) {
+    for (int n = 0; !last; ++n) {
         ok = tc_wait(&B->raw_full[slot], turn & 1, &B->err, 33);
-        if (ok && use) ok = tc_wait(&B->k_empty[st], (use - 1) & 1, &B->err, 35);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const uint32_t valid = B->info[n % kTcInfos].valid;
-        const int count = B->info[n % kTcInfos].count;
-        uint8_t* tile = smem + TcSmem::kTiles + st * 2 * kTcTileBytes;
-        const uint4* raw = reinterpret_cast<const uint4*>(smem + TcSmem::kRaw + slot * TcSmem::kRawBytes + 2 * w * kBlockBytes);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 d = raw[i * 32 + lane];
-            uint4 x, y;
-            to_f16<F>(d.x, x.x, x.y);
-            to_f16<F>(d.y, x.z, x.w);
-            to_f16<F>(d.z, y.x, y.y);
-            to_f16<F>(d.w, y.z, y.w);
-            *reinterpret_cast<uint4*>(tile + krow + i * 8 * 128 + k0) = x;
-            *reinterpret_cast<uint4*>(tile + krow + i * 8 * 128 + k1) = y;
+        last = B->info[n % kTcInfos].last;
+        if (n && B->info[n % kTcInfos].starts) {
+            r.next(ta.a, tab, hi);
+            if (++run > 1) ok = tc_wait(&B->q_free[run & 1], ((run >> 1) - 1) & 1, &B->err, 42);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_queries<128>(ta.a, smem, r, run & 1);
+            mbar_arrive(&B->q_full[run & 1]);
         }
-        fence_proxy_async_smem();
-        mbar_arrive(&B->k_full[st]);
-        uint4 v[4];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            v[2 * e] = raw[(kTcBlocks + e) * 64 + h * 32 + 4 * g + 2 * u];
-            v[2 * e + 1] = raw[(kTcBlocks + e) * 64 + h * 32 + 4 * g + 2 * u + 1];
-        }
-        mbar_arrive(&B->raw_empty[slot]);
-        if (count < kTcTile || valid != 0xffu) {  // (what lies past the end may be NaN)
+        if (ok && use) ok = tc_wait(&empty[st], (use - 1) & 1, &B->err, 35);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* tile = smem + TcSmem::kTiles + st * 2 * kTcTileBytes + to0;
+        const uint4* raw = reinterpret_cast<const uint4*>(smem + TcSmem::kRaw + slot * TcSmem::kRawBytes) + from0;
+        if (keys) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                // positions 8 u .. + 7 of the block that exist, four bytes at a time
-                const int left = valid >> (2 * w + e) & 1u ? count - (2 * w + e) * kBlock - 8 * u : 0;
-                keep_bytes<F>(v[2 * e], left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u);
-                keep_bytes<F>(v[2 * e + 1], left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u);
+                uint4 d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = raw[(4 * e + i) * 32];
+                if (e) mbar_arrive(&B->raw_empty[slot]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint4 x, y;
+                    to_f16<F>(d[i].x, x.x, x.y);
+                    to_f16<F>(d[i].y, x.z, x.w);
+                    to_f16<F>(d[i].z, y.x, y.y);
+                    to_f16<F>(d[i].w, y.z, y.w);
+                    *reinterpret_cast<uint4*>(tile + (4 * e + i) * 8 * 128 + k0) = x;
+                    *reinterpret_cast<uint4*>(tile + (4 * e + i) * 8 * 128 + k1) = y;
+                }
             }
-        }
-        if (use) ok = tc_wait(&B->v_empty[st], (use - 1) & 1, &B->err, 36);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        tile += kTcTileBytes;
+        } else {
+            const uint32_t valid = B->info[n % kTcInfos].valid;
+            const int count = B->info[n % kTcInfos].count;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint32_t x[4] = {v[2 * e].x, v[2 * e].y, v[2 * e].z, v[2 * e].w}, y[4] = {v[2 * e + 1].x, v[2 * e + 1].y, v[2 * e + 1].z, v[2 * e + 1].w};
-            uint8_t* to = tile + vrow + ((((2 * w + e) & 3) * 2 + u) ^ g) * 16;  // 64 positions: rows of dims
+            for (int e0 = 0; e0 < 4; e0 += 2) {
+                uint4 v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint4 o;
-                to_f16<F>(x[j], o.x, o.y);
-                to_f16<F>(y[j], o.z, o.w);
-                *reinterpret_cast<uint4*>(to + j * 8 * 128) = o;
+                for (int e = 0; e < 2; ++e) {
+                    v[2 * e] = raw[(e0 + e) * 64];
+                    v[2 * e + 1] = raw[(e0 + e) * 64 + 1];
+                }
+                if (e0) mbar_arrive(&B->raw_empty[slot]);
+                if (count < kTcTile || valid != 0xffu) {  // (what lies past the end may be NaN)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        // positions 8 u .. + 7 of the block that exist, four bytes at a time
+                        const int b = 4 * w + e0 + e, left = valid >> b & 1u ? count - b * kBlock - 8 * u : 0;
+                        keep_bytes<F>(v[2 * e], left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u);
+                        keep_bytes<F>(v[2 * e + 1], left >= 8 ? 0xffffffffu : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1u);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t x[4] = {v[2 * e].x, v[2 * e].y, v[2 * e].z, v[2 * e].w};
+                    const uint32_t y[4] = {v[2 * e + 1].x, v[2 * e + 1].y, v[2 * e + 1].z, v[2 * e + 1].w};
+                    uint8_t* to = tile + (((e0 + e) * 2 + u) ^ g) * 16;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 o;
+                        to_f16<F>(x[j], o.x, o.y);
+                        to_f16<F>(y[j], o.z, o.w);
+                        *reinterpret_cast<uint4*>(to + j * 8 * 128) = o;
+                    }
+                }
             }
         }
         fence_proxy_async_smem();
-        mbar_arrive(&B->v_full[st]);
+        mbar_arrive(&full[st]);
         if (++st == kTcSt) {
             st = 0;
             ++use;
@@ -359,8 +427,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < kTcSt; ++i) {
-            mbar_init(&B->k_full[i], 128);
-            mbar_init(&B->v_full[i], 128);
+            mbar_init(&B->k_full[i], 64);
+            mbar_init(&B->v_full[i], 64);
             mbar_init(&B->k_empty[i], 1);
             mbar_init(&B->v_empty[i], 1);
         }
@@ -368,7 +436,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             mbar_init(&B->raw_full[i], 2);
             mbar_init(&B->raw_empty[i], 128);
         }
-        mbar_init(&B->q_full, 256);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&B->q_full[b], 128);
+            mbar_init(&B->q_free[b], 256);
+        }
         for (int b = 0; b < 3; ++b) {
             mbar_init(&B->s_full[b], 1);
             mbar_init(&B->p_full[b], 128);
@@ -390,7 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             int n = 0;
             if (s < a.p.n_seq) {
                 const AttLens x = att_lens(a, s, blockIdx.x == 0);
-                for (int rt = 0; rt * kTcRows < x.n * a.G; ++rt) n += tc_tiles(x.L, x.n, a.G, rt);
+                for (int rt = 0; rt * kTcRows < x.n * a.G; ++rt) n += tc_entries(x.L, x.n, a.G, rt);
                 n *= a.p.pool.n_heads;
                 len[s] = x.L;
                 toks[s] = x.n;
@@ -432,53 +503,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         const uint32_t ot = tmem + lane_base + 384 + g * 64;
-        uint8_t* qhi = smem + Sh::kQ;
-        uint8_t* qlo = qhi + kTcTileBytes;
-        float4* xch = reinterpret_cast<float4*>(smem + Sh::kQ) + row * 16;  // group 1's output row at a run's end
         float2* mls = reinterpret_cast<float2*>(smem + Sh::kMl) + row;
-        float* rsb = reinterpret_cast<float*>(smem + Sh::kRs);
-        uint32_t k = 0;  // tiles of this group so far
+        const float* rsb = reinterpret_cast<const float*>(smem + Sh::kRs);
+        uint32_t k = 0, run = 0;  // tiles of this group, runs so far
         bool ok = true;
-        for (; r.i < hi; r.next(a, tab, hi)) {
+        if (r.t0 < r.t1) {
+            tc_queries<256>(a, smem, r, 0);
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (g == 0) mbar_arrive(&B->q_full[0]);
+        }
+        for (; r.t0 < r.t1; r.next(a, tab, hi), ++run) {
             const int rr = r.rt * kTcRows + row, rows = r.n * a.G, before = r.L - r.n + 1;
             const bool real = rr < rows;
             const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
             const int tok = rr / a.G, h = r.kvh * a.G + rr - tok * a.G;
             const int lim = real ? before + tok : 0;                   // positions that the row sees
             const int sure = before + r.rt * kTcRows / a.G;            // that all rows of the unit do
-            // Q: four lanes a row, 16 dims each
-            // (nothing reads the last run's Q, or its exchanged rows, any more)
-            if (r.i != lo) asm volatile("bar.sync 1, 256;" ::: "memory");
-#pragma unroll 1
-            for (int q0 = tid >> 2; q0 < kTcRows; q0 += 64) {
-                const int qr = r.rt * kTcRows + q0, qt = qr / a.G, c = lane & 3;
-                const float4* q = reinterpret_cast<const float4*>(a.p.q + (int64_t)r.s * a.p.q_nb_seq + (int64_t)qt * a.p.q_nb_tok +
-                                                                  (r.kvh * a.G + qr - qt * a.G) * kD + 16 * c);
-                float4 v[4];
-                float am = 0.0f;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = qr < rows ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) am = fmaxf(am, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
-                const int ex = dtc::norm_exp(quad_max(am));
-                const float f = pow2f(ex);
-                if (c == 0) rsb[q0] = pow2f(-ex) * a.scale_log2;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    uint4 wh, wl;
-                    split_near(make_float2(v[2 * u].x * f, v[2 * u].y * f), wh.x, wl.x);
-                    split_near(make_float2(v[2 * u].z * f, v[2 * u].w * f), wh.y, wl.y);
-                    split_near(make_float2(v[2 * u + 1].x * f, v[2 * u + 1].y * f), wh.z, wl.z);
-                    split_near(make_float2(v[2 * u + 1].z * f, v[2 * u + 1].w * f), wh.w, wl.w);
-                    const uint32_t at = tc::sw128_offset(q0, 2 * c + u);
-                    *reinterpret_cast<uint4*>(qhi + at) = wh;
-                    *reinterpret_cast<uint4*>(qlo + at) = wl;
-                }
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&B->q_full);
-            asm volatile("bar.sync 3, 256;" ::: "memory");
-            const float rs = rsb[row];
+            ok = tc_wait(&B->q_full[run & 1], run >> 1 & 1, &B->err, 37);
+            ok = __all_sync(0xffffffffu, ok);
+            const float rs = rsb[(run & 1) * kTcRows + row];
             float2 O[32];
 #pragma unroll
             for (int d = 0; d < 32; ++d) O[d] = make_float2(0.f, 0.f);
@@ -496,9 +539,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         O[16 * e + d] = ffma2(make_float2(__uint_as_float(o0[2 * d]), __uint_as_float(o0[2 * d + 1])), f, O[16 * e + d]);
                 }
             };
-            for (int j = r.i + ((r.i ^ g ^ lo) & 1); j < r.end; j += 2) {  // the CTA's tiles j - lo of parity g
-                const int p0 = (r.t0 + j - r.i) * kTcTile;
-                const int n = j - lo, buf = n % 3;
+            for (int n = r.at + ((r.at ^ g) & 1); ok && n < r.at + r.t1 - r.t0; n += 2) {  // the CTA's tiles of parity g
+                const int p0 = (r.t0 + n - r.at) * kTcTile, buf = n % 3;
                 // (Of a buffer's phases a group sees every second one, always of the same parity.  It cannot pass on an older one:
                 // S of tile n - 3, the phase before, was committed ahead of S of n - 2, which this group has seen.)
                 const uint32_t sp = tmem + lane_base + buf * 128;
@@ -625,58 +667,77 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             tc::fence_before();
             if (!fp::prod_bar_and(2, 256, ok)) break;  // every MMA of the run is done; all threads leave together
             const float m_mine = thr == -INFINITY && l == 0.0f ? -INFINITY : base;  // (NaN scores raise nothing)
+            // group 1's rows to where Q was, joined there by group 0, written by both
+            float4* rows_at = reinterpret_cast<float4*>(smem + Sh::kQ + (run & 1) * 2 * kTcTileBytes);
+            float4* mine = rows_at + row * 16;
             if (g == 1) {
 #pragma unroll
-                for (int c = 0; c < 16; ++c) xch[c ^ (row & 7)] = make_float4(O[2 * c].x, O[2 * c].y, O[2 * c + 1].x, O[2 * c + 1].y);
+                for (int c = 0; c < 16; ++c) mine[c ^ (row & 7)] = make_float4(O[2 * c].x, O[2 * c].y, O[2 * c + 1].x, O[2 * c + 1].y);
                 *mls = make_float2(m_mine, l);
             }
             asm volatile("bar.sync 3, 256;" ::: "memory");
-            if (g == 0 && real) {
+            const bool whole = r.t1 - r.t0 == r.T;
+            const int64_t slot = (int64_t)(2 * blockIdx.x + (r.at == 0 ? 0 : 1)) * kTcRows;
+            if (g == 0) {
                 const float2 other = *mls;
                 const float M = fmaxf(m_mine, other.x);
                 const float f0 = m_mine == -INFINITY ? 0.0f : exp2f(m_mine - M), f1 = other.x == -INFINITY ? 0.0f : exp2f(other.x - M);
                 const float sum = (m_mine == -INFINITY ? 0.0f : f0 * l) + (other.x == -INFINITY ? 0.0f : f1 * other.y);
-                const bool whole = r.end - r.i == r.T, seen = M != -INFINITY;
+                const bool seen = M != -INFINITY;
                 const float inv = !whole ? 1.0f : seen ? 1.0f / sum : 0.0f;
-                const int64_t slot = (int64_t)(2 * blockIdx.x + (r.i == lo ? 0 : 1)) * kTcRows + row;
-                const int64_t orow = (int64_t)r.s * a.p.out_nb_seq + (int64_t)tok * a.p.out_nb_tok + h * kD;
-                float4* dst = reinterpret_cast<float4*>(whole ? a.p.out + orow : ta.ws_o + slot * kD);
                 const float2 g0 = make_float2(f0 * inv, f0 * inv), g1 = make_float2(f1 * inv, f1 * inv);
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
-                    const float4 w = xch[c ^ (row & 7)];
+                    const float4 w = mine[c ^ (row & 7)];
                     const float2 u = ffma2(g1, make_float2(w.x, w.y), mul2(g0, O[2 * c])), v = ffma2(g1, make_float2(w.z, w.w), mul2(g0, O[2 * c + 1]));
-                    dst[c] = make_float4(u.x, u.y, v.x, v.y);
+                    mine[c ^ (row & 7)] = make_float4(u.x, u.y, v.x, v.y);
                 }
-                if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + slot * 2) = make_float2(M, sum);
-                else if (a.p.lse)
-                    a.p.lse[((int64_t)r.s * a.p.max_q + tok) * a.p.n_q_heads + h] = seen ? (M + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+                if (real) {
+                    if (!whole) *reinterpret_cast<float2*>(ta.ws_ml + (slot + row) * 2) = make_float2(M, sum);
+                    else if (a.p.lse)
+                        a.p.lse[((int64_t)r.s * a.p.max_q + tok) * a.p.n_q_heads + h] = seen ? (M + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+                }
             }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+#pragma unroll 4
+            for (int rl = tid >> 4; rl < kTcRows; rl += 16) {  // 16 lanes a row
+                const int c = tid & 15, qr = r.rt * kTcRows + rl, qt = qr / a.G;
+                if (qr >= rows) break;
+                const float4 v = rows_at[rl * 16 + (c ^ (rl & 7))];
+                float* dst = whole ? a.p.out + (int64_t)r.s * a.p.out_nb_seq + (int64_t)qt * a.p.out_nb_tok + (r.kvh * a.G + qr - qt * a.G) * kD
+                                   : ta.ws_o + (slot + rl) * kD;
+                reinterpret_cast<float4*>(dst)[c] = v;
+            }
+            mbar_arrive(&B->q_free[run & 1]);
         }
     } else if (warp < 12) {
         regs_down<kTcRegsProducer>();
-        tc_produce<F>(smem, B, lo, hi);
+        tc_produce<F>(ta, smem, B, tab, r, hi);
     } else {
         regs_down<kTcRegsOther>();
         // ------------------------------------------------------ MMA issuers: the whole warp walks, one lane issues
         const int which = __shfl_sync(0xffffffffu, warp, 0);
         const uint64_t dt0 = tc::sdesc_sw128(smem_addr(smem + Sh::kTiles), 16, 1024);
         constexpr uint64_t kStep = 2 * kTcTileBytes >> 4;
-        bool ok = true;
+        bool ok = true, last = r.t0 == r.t1;
         int st = 0, buf = 0;
         uint32_t use = 0, turn = 0, n_run = 0;  // n / kTcSt, n / 3
         if (which == 12) {
             const uint32_t idesc = tc::idesc_f16_f32(128, kTcTile, false);
-            const uint64_t dqh = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
-            const uint64_t dql = tc::sdesc_sw128(smem_addr(smem + Sh::kQ) + kTcTileBytes, 16, 1024);
-            for (int n = 0; ok && lo + n < hi; ++n) {
+            const uint64_t dq0 = tc::sdesc_sw128(smem_addr(smem + Sh::kQ), 16, 1024);
+            uint64_t dqh = dq0;
+            for (int n = 0; !last; ++n) {
                 ok = tc_wait(&B->k_full[st], use & 1, &B->err, 38);
-                if (ok && B->info[n % kTcInfos].starts) ok = tc_wait(&B->q_full, n_run++ & 1, &B->err, 37);
+                last = B->info[n % kTcInfos].last;
+                if (ok && B->info[n % kTcInfos].starts) {
+                    ok = tc_wait(&B->q_full[n_run & 1], n_run >> 1 & 1, &B->err, 43);
+                    dqh = dq0 + (n_run++ & 1) * (2 * kTcTileBytes >> 4);
+                }
                 if (ok && n >= 3) ok = tc_wait(&B->s_free[buf], (turn - 1) & 1, &B->err, 40);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc::fence_after();
-                const uint64_t dk = dt0 + (uint64_t)st * kStep;
+                const uint64_t dk = dt0 + (uint64_t)st * kStep, dql = dqh + (kTcTileBytes >> 4);
                 const uint32_t sp = tmem + buf * 128;
                 if (elect_one()) {
 #pragma unroll 1
@@ -692,8 +753,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             }
         } else if (which == 13) {
             const uint32_t idesc = tc::idesc_f16_f32(128, 64, false);
-            for (int n = 0; ok && lo + n < hi; ++n) {
+            for (int n = 0; !last; ++n) {
                 ok = tc_wait(&B->v_full[st], use & 1, &B->err, 41);
+                last = B->info[n % kTcInfos].last;
                 if (ok) ok = tc_wait(&B->p_full[buf], turn & 1, &B->err, 39);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -716,7 +778,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 if (++buf == 3) { buf = 0; ++turn; }
             }
         } else if (which == 14) {
-            tc_load(ta, smem, B, tab, r, lo, hi);
+            tc_load(ta, smem, B, tab, r, hi);
         }
     }
 
@@ -747,9 +809,9 @@ __global__ void __launch_bounds__(256) paged_tc_combine_kernel(const __grid_cons
     if (r < x.n * a.G) {
         const int T = tc_tiles(x.L, x.n, a.G, rt);
         if (T > 0) {
-            b0 = ta.ws_pref[s] + kvh * T;
+            b0 = ta.ws_pref[s] + kvh * (T + kTcGap);
             int above = 0;  // the unit's 16 threads share the row tiles before it
-            for (int i = c; i < rt; i += 16) above += tc_tiles(x.L, x.n, a.G, i);
+            for (int i = c; i < rt; i += 16) above += tc_entries(x.L, x.n, a.G, i);
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) above += __shfl_xor_sync(0xffffu << (threadIdx.x & 16), above, w);
             b0 += above * a.p.pool.n_heads;
@@ -769,7 +831,7 @@ __global__ void __launch_bounds__(256) paged_tc_combine_kernel(const __grid_cons
             const int cta = k0 + u * kLanes;
             ml[u] = make_float2(-INFINITY, 0.0f);
             if (cta <= c1 && tc_cut(cta + 1, n, ta.grid) > tc_cut(cta, n, ta.grid)) {
-                const int64_t at = (int64_t)(2 * cta + (tc_cut(cta, n, ta.grid) >= b0 ? 0 : 1)) * kTcRows + r % kTcRows;
+                const int64_t at = (int64_t)(2 * cta + (tc_cut(cta, n, ta.grid) >= b0 - kTcGap ? 0 : 1)) * kTcRows + r % kTcRows;
                 ml[u] = *reinterpret_cast<const float2*>(ta.ws_ml + at * 2);
                 v[u] = *reinterpret_cast<const float4*>(ta.ws_o + at * kD + c * 4);
             }
