@@ -151,6 +151,8 @@ cudaError_t launch_paged_attention(cudaStream_t stream, const cvattn_paged_atten
     a.status = status;
     const Plan plan = plan_of(p.n_seq, p.max_q, p.max_kv_len, p.n_q_heads, p.pool.n_heads);
     a.n_splits = plan.n_splits;
+    a.by_G = inverse_of(a.G);
+    a.by_parts = inverse_of(plan.tc_grid ? plan.tc_grid : plan.cluster * plan.n_splits);
     if (plan.tc_grid) {
         TcAttArgs ta{};
         ta.a = a;

@@ -42,10 +42,21 @@ struct AttArgs {
     cvattn_paged_attention_params p;
     int G, blocks;                       // query heads per KV head; blocks of a page
     int n_splits;                        // clusters per unit
+    uint32_t by_G, by_parts;             // inverse_of(G); of the CTAs that share a unit (tcgen05: the list)
     float scale_log2;
     float *ws_ml, *ws_o;                 // [seq][KV head][split][max_q * G][2], [..][64]
     int* status;
 };
+
+// x / n for x below 2^31 / n, without a division (which takes some 25 instructions, on the way to a CTA's first load): with
+// inverse = (2^31 + e) / n, e < n, the product is off by x e / (n 2^31) < 1 / n.
+__host__ __device__ constexpr uint32_t inverse_of(uint32_t n) { return ((1u << 31) + n - 1) / n; }
+__device__ __forceinline__ int divided(int x, uint32_t inverse) { return (int)__umulhi((uint32_t)x << 1, inverse); }
+// c / parts of n, c <= parts <= 2^10.
+__device__ __forceinline__ int cut_at(int c, int n, int parts, uint32_t by_parts) {
+    const uint32_t q = (uint32_t)n / (uint32_t)parts, rest = (uint32_t)n - q * parts;
+    return c * (int)q + divided(c * (int)rest, by_parts);
+}
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -141,7 +152,7 @@ struct Join {
     __device__ __forceinline__ void write(const AttArgs& a, int s, int kvh, int r, int c) const {
         const bool seen = M != -INFINITY;
         const float inv = seen ? 1.0f / l : 0.0f;
-        const int tok = r / a.G, h = kvh * a.G + r % a.G;
+        const int tok = divided(r, a.by_G), h = kvh * a.G + r - tok * a.G;
         *reinterpret_cast<float4*>(a.p.out + (int64_t)s * a.p.out_nb_seq + (int64_t)tok * a.p.out_nb_tok + h * kD + c * 4) =
             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         if (a.p.lse && c == 0)
@@ -184,13 +195,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
     // row r of token i sees the positions below L - n + i + 1
     const int before = x.L - x.n + 1;
     const int last_row = min(rows, r0 + S::kRows * kMmaWarps) - 1;
-    const int end = last_row >= r0 ? max(0, before + last_row / a.G) : 0;
+    const int end = last_row >= r0 ? max(0, before + divided(last_row, a.by_G)) : 0;
     const int n_blocks = (end + kBlock - 1) / kBlock, shares = C * a.n_splits, share = split * C + rank;
     const int n_steps = (n_blocks + kPair - 1) / kPair;
-    const int s0 = (int)((int64_t)n_steps * share / shares), s1 = (int)((int64_t)n_steps * (share + 1) / shares);
+    const int s0 = cut_at(share, n_steps, shares, a.by_parts), s1 = cut_at(share + 1, n_steps, shares, a.by_parts);
     const int steps = rw < rows ? max(0, (s1 - s0 - wk + WK - 1) / WK) : 0;
 
     const int32_t* table = a.p.table + (int64_t)s * a.p.table_nb_seq;
+    const int shift = __ffs(a.blocks) - 1;
     // lane i knows of block i & 1 of the warp's step 16 c + i / 2: where it lies, and its scales
     int64_t off = 0, next_off = 0;
     float2 sc = make_float2(-1.0f, 0.0f), next_sc = sc;  // (-1: not seen)
@@ -199,12 +211,12 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
         o = 0;
         f = make_float2(-1.0f, 0.0f);
         if (16 * chunk + (lane >> 1) >= steps || b >= n_blocks) return;
-        const int page = page_of(table, b / a.blocks, a.p.pool.n_pages);
+        const int entry = b >> shift, page = page_of(table, entry, a.p.pool.n_pages);
         if (page < 0) {
             record_status(a.status, kStatusBadPage);
             return;
         }
-        const int in = kvh * a.blocks + b % a.blocks;
+        const int in = ((kvh - entry) << shift) + b;
         o = page * a.p.pool.nb_page + (int64_t)in * kBlockBytes;
         f.x = a.p.pool.k_scale[page * a.p.pool.nb_scale + in];
         f.y = a.p.pool.v_scale[page * a.p.pool.nb_scale + in];
@@ -245,8 +257,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
     int lim[R];             // positions that the row sees
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int r = rw + 8 * i + gid;
-        const float* q = a.p.q + (int64_t)s * a.p.q_nb_seq + (int64_t)(r / a.G) * a.p.q_nb_tok + (kvh * a.G + r % a.G) * kD + 16 * tig;
+        const int r = rw + 8 * i + gid, tok = divided(r, a.by_G);
+        const float* q = a.p.q + (int64_t)s * a.p.q_nb_seq + (int64_t)tok * a.p.q_nb_tok + (kvh * a.G + r - tok * a.G) * kD + 16 * tig;
         float4 e[4];
         float am = 0.0f;
 #pragma unroll
@@ -257,14 +269,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
         const int ex = dtc::norm_exp(quad_max(am));
         const float f = pow2f(ex);
         rs[i] = pow2f(-ex) * a.scale_log2;
-        lim[i] = r < rows ? before + r / a.G : 0;
+        lim[i] = r < rows ? before + tok : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             split_near(make_float2(e[j].x * f, e[j].y * f), qa[i][j][0], qa[i][j][1]);
             split_near(make_float2(e[j].z * f, e[j].w * f), qa[i][j][2], qa[i][j][3]);
         }
     }
-    const int sure = before + rw / a.G;  // positions below it every row of the warp sees
+    const int sure = before + divided(rw, a.by_G);  // positions below it every row of the warp sees
     float2 O[R][8], l[R];
     float base[R], thr[R];
 #pragma unroll

@@ -69,6 +69,7 @@ struct TcAttBars {
     int err;
     TcInfo info[kTcInfos];      // tile n at n % kTcInfos
     int32_t first_run[16];      // TcRun at the start of the CTA's part
+    int32_t hi;                 // the part's end
 };
 
 struct TcSmem {
@@ -121,18 +122,24 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* err
 }
 
 // Positions that the last row of row tile rt sees, of a sequence with L positions and n of them as rows.
-__device__ __forceinline__ int tc_end(int L, int n, int G, int rt) {
-    const int last = min(n * G, (rt + 1) * kTcRows) - 1;
-    return max(0, L - n + 1 + last / G);
+__device__ __forceinline__ int tc_end(const AttArgs& a, int L, int n, int rt) {  // n > 0
+    const int last = min(n * a.G, (rt + 1) * kTcRows) - 1;
+    return max(0, L - n + 1 + divided(last, a.by_G));
 }
-__device__ __forceinline__ int tc_tiles(int L, int n, int G, int rt) { return (tc_end(L, n, G, rt) + kTcTile - 1) / kTcTile; }
+__device__ __forceinline__ int tc_tiles(const AttArgs& a, int L, int n, int rt) { return (tc_end(a, L, n, rt) + kTcTile - 1) / kTcTile; }
 // List entries of a unit.
-__device__ __forceinline__ int tc_entries(int L, int n, int G, int rt) {
-    const int T = tc_tiles(L, n, G, rt);
+__device__ __forceinline__ int tc_entries(const AttArgs& a, int L, int n, int rt) {
+    const int T = tc_tiles(a, L, n, rt);
     return T ? T + kTcGap : 0;
 }
-__device__ __forceinline__ int tc_cut(int c, int n, int g) { return (int)((long long)c * n / g); }
-__device__ __forceinline__ int tc_owner(int i, int n, int g) { return (int)(((long long)(i + 1) * g - 1) / n); }
+// Where CTA c's part of n entries begins; whose part entry i lies in.
+__device__ __forceinline__ int tc_cut(const TcAttArgs& ta, int c, int n) { return cut_at(c, n, ta.grid, ta.a.by_parts); }
+__device__ __forceinline__ int tc_owner(const TcAttArgs& ta, int i, int n) {
+    int c = min((int)((float)i * (float)ta.grid / (float)n), ta.grid - 1);  // off by one at most
+    while (tc_cut(ta, c, n) > i) --c;
+    while (tc_cut(ta, c + 1, n) <= i) ++c;
+    return c;
+}
 
 struct TcTab {  // in shared memory, by sequence: list entries before it, positions, rows (tokens)
     const int32_t *pref, *len, *n;
@@ -146,7 +153,7 @@ struct TcRun {
     int L, n, see;    // positions, tokens, positions that the unit's last row sees
 
     __device__ __forceinline__ void unit(const AttArgs& a) {
-        see = tc_end(L, n, a.G, rt);
+        see = tc_end(a, L, n, rt);
         T = (see + kTcTile - 1) / kTcTile;
     }
     __device__ __forceinline__ void start(const AttArgs& a, const TcTab& tab, int lo, int hi) {
@@ -241,6 +248,7 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
         if (has && !good) record_status(a.status, kStatusBadPage);
         const uint32_t valid = __ballot_sync(0xffffffffu, good);
         const int64_t at = good ? page * a.p.pool.nb_page + (int64_t)in * kBlockBytes : 0, sat = good ? page * a.p.pool.nb_scale + in : 0;
+        const float ks = good ? a.p.pool.k_scale[sat] : 0.0f, vs = good ? a.p.pool.v_scale[sat] : 0.0f;
         if (lane == 0) mbar_arrive_expect_tx(&B->raw_full[slot], __popc(valid) * 2 * kBlockBytes);
         __syncwarp();
         uint8_t* raw = smem + TcSmem::kRaw + slot * TcSmem::kRawBytes;
@@ -248,9 +256,7 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
             bulk_g2s(raw + lane * kBlockBytes, static_cast<const uint8_t*>(a.p.pool.k) + at, kBlockBytes, &B->raw_full[slot]);
             bulk_g2s(raw + (kTcBlocks + lane) * kBlockBytes, static_cast<const uint8_t*>(a.p.pool.v) + at, kBlockBytes, &B->raw_full[slot]);
         }
-        const float ks = good ? a.p.pool.k_scale[sat] : 0.0f, vs = good ? a.p.pool.v_scale[sat] : 0.0f;
-        const int here = count, starts_here = first;
-        look();
+        const uint32_t last = t == r.t1 && r.v + r.T + kTcGap >= hi;
         const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
         int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
         e = e > 100 ? 100 : e < -100 ? -100 : e;
@@ -262,12 +268,13 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
         if (lane == 0) {
             info.exp = pow2f(-e);
             info.valid = valid;
-            info.starts = (uint32_t)starts_here;
-            info.last = count == 0;
-            info.count = here;
+            info.starts = (uint32_t)first;
+            info.last = last;
+            info.count = count;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&B->raw_full[slot]);  // (the second of its two arrivals: what is said of the tile)
+        look();
         if (++slot == kTcRaw) {
             slot = 0;
             ++use;
@@ -286,7 +293,7 @@ template <int kThreads> __device__ __forceinline__ void tc_queries(const AttArgs
     float* rsb = reinterpret_cast<float*>(smem + TcSmem::kRs) + buf * kTcRows;
 #pragma unroll 2
     for (int q0 = t >> 2; q0 < kTcRows; q0 += kThreads / 4) {
-        const int qr = r.rt * kTcRows + q0, qt = qr / a.G;
+        const int qr = r.rt * kTcRows + q0, qt = divided(qr, a.by_G);
         const float4* q = reinterpret_cast<const float4*>(a.p.q + (int64_t)r.s * a.p.q_nb_seq + (int64_t)qt * a.p.q_nb_tok +
                                                           (r.kvh * a.G + qr - qt * a.G) * kD + 16 * c);
         float4 v[4];
@@ -461,7 +468,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             int n = 0;
             if (s < a.p.n_seq) {
                 const AttLens x = att_lens(a, s, blockIdx.x == 0);
-                for (int rt = 0; rt * kTcRows < x.n * a.G; ++rt) n += tc_entries(x.L, x.n, a.G, rt);
+                for (int rt = 0; rt * kTcRows < x.n * a.G; ++rt) n += tc_entries(a, x.L, x.n, rt);
                 n *= a.p.pool.n_heads;
                 len[s] = x.L;
                 toks[s] = x.n;
@@ -484,7 +491,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         }
         __syncwarp();
         TcRun r{};
-        r.start(a, tab, tc_cut(blockIdx.x, carry, ta.grid), tc_cut(blockIdx.x + 1, carry, ta.grid));
+        const int lo = tc_cut(ta, blockIdx.x, carry), hi = tc_cut(ta, blockIdx.x + 1, carry);
+        r.start(a, tab, lo, hi);
+        if (lane == 0) B->hi = hi;
         static_assert(sizeof(TcRun) <= sizeof(B->first_run), "a run in shared memory");
         if (lane == 0) *reinterpret_cast<TcRun*>(B->first_run) = r;
     }
@@ -493,8 +502,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     tc::fence_after();
     griddep_launch_dependents();
     const uint32_t tmem = B->tmem_base;
-    const int total = pref[a.p.n_seq];
-    const int lo = tc_cut(blockIdx.x, total, ta.grid), hi = tc_cut(blockIdx.x + 1, total, ta.grid);
+    const int hi = B->hi;
     TcRun r = *reinterpret_cast<const TcRun*>(B->first_run);
 
     if (warp < 8) {
@@ -516,9 +524,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             const int rr = r.rt * kTcRows + row, rows = r.n * a.G, before = r.L - r.n + 1;
             const bool real = rr < rows;
             const bool warp_real = r.rt * kTcRows + quad * 32 < rows;  // some row of this warp is
-            const int tok = rr / a.G, h = r.kvh * a.G + rr - tok * a.G;
+            const int tok = divided(rr, a.by_G), h = r.kvh * a.G + rr - tok * a.G;
             const int lim = real ? before + tok : 0;                   // positions that the row sees
-            const int sure = before + r.rt * kTcRows / a.G;            // that all rows of the unit do
+            const int sure = before + divided(r.rt * kTcRows, a.by_G);          // that all rows of the unit do
             ok = tc_wait(&B->q_full[run & 1], run >> 1 & 1, &B->err, 37);
             ok = __all_sync(0xffffffffu, ok);
             const float rs = rsb[(run & 1) * kTcRows + row];
@@ -701,7 +709,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             asm volatile("bar.sync 3, 256;" ::: "memory");
 #pragma unroll 4
             for (int rl = tid >> 4; rl < kTcRows; rl += 16) {  // 16 lanes a row
-                const int c = tid & 15, qr = r.rt * kTcRows + rl, qt = qr / a.G;
+                const int c = tid & 15, qr = r.rt * kTcRows + rl, qt = divided(qr, a.by_G);
                 if (qr >= rows) break;
                 const float4 v = rows_at[rl * 16 + (c ^ (rl & 7))];
                 float* dst = whole ? a.p.out + (int64_t)r.s * a.p.out_nb_seq + (int64_t)qt * a.p.out_nb_tok + (r.kvh * a.G + qr - qt * a.G) * kD
@@ -807,16 +815,16 @@ __global__ void __launch_bounds__(256) paged_tc_combine_kernel(const __grid_cons
     const int rt = r / kTcRows, n = ta.ws_pref[a.p.n_seq];
     int b0 = 0, c0 = 0, c1 = -1;
     if (r < x.n * a.G) {
-        const int T = tc_tiles(x.L, x.n, a.G, rt);
+        const int T = tc_tiles(a, x.L, x.n, rt);
         if (T > 0) {
             b0 = ta.ws_pref[s] + kvh * (T + kTcGap);
             int above = 0;  // the unit's 16 threads share the row tiles before it
-            for (int i = c; i < rt; i += 16) above += tc_entries(x.L, x.n, a.G, i);
+            for (int i = c; i < rt; i += 16) above += tc_entries(a, x.L, x.n, i);
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) above += __shfl_xor_sync(0xffffu << (threadIdx.x & 16), above, w);
             b0 += above * a.p.pool.n_heads;
-            c0 = tc_owner(b0, n, ta.grid);
-            c1 = tc_owner(b0 + T - 1, n, ta.grid);
+            c0 = tc_owner(ta, b0, n);
+            c1 = tc_owner(ta, b0 + T - 1, n);
             if (kLanes == 1 && c0 == c1) return;  // written whole
         }
     }
@@ -830,8 +838,9 @@ __global__ void __launch_bounds__(256) paged_tc_combine_kernel(const __grid_cons
         for (int u = 0; u < 4; ++u) {
             const int cta = k0 + u * kLanes;
             ml[u] = make_float2(-INFINITY, 0.0f);
-            if (cta <= c1 && tc_cut(cta + 1, n, ta.grid) > tc_cut(cta, n, ta.grid)) {
-                const int64_t at = (int64_t)(2 * cta + (tc_cut(cta, n, ta.grid) >= b0 - kTcGap ? 0 : 1)) * kTcRows + r % kTcRows;
+            const int from = tc_cut(ta, cta, n);
+            if (cta <= c1 && tc_cut(ta, cta + 1, n) > from) {
+                const int64_t at = (int64_t)(2 * cta + (from >= b0 - kTcGap ? 0 : 1)) * kTcRows + r % kTcRows;
                 ml[u] = *reinterpret_cast<const float2*>(ta.ws_ml + at * 2);
                 v[u] = *reinterpret_cast<const float4*>(ta.ws_o + at * kD + c * 4);
             }
