@@ -64,12 +64,14 @@ constexpr int kSms = 148;
 
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// The tcgen05 kernel starts later (about 9 us) and takes 1.5 us for a tile of 128 positions on an SM, whatever rows it has up to
-// 128; the other takes 0.44 ns for a row of such a tile (all SMs together).  us of mma.sync | tcgen05, 14 / 2 heads: 1
-// sequence of 4096, 56 rows of a KV head 14.9 | 14.8; 1 of 65536, 14 rows 22.7 | 24.7, 56 48 | 27; 4 of 2500, 112 23.1 | 20.4, 224
-// 27.8 | 25.7; 16 of 1000, 112 23.6 | 26.2, 224 33.5 | 28.4; 16 of 8192, 28 33.4 | 39.2, 56 59 | 41; 64 of 1000, 28 20.4 | 27.8, 56
-// 34.4 | 29.5; 64 of 4096, 28 53 | 55, 56 95 | 59.
-constexpr int64_t kTcWork = 1 << 14, kTcPerTile = 24;
+// The tcgen05 kernel starts later (13 us in all for a single tile) and takes 1.5 us for an entry of its list on an SM, whatever rows
+// a unit has up to 128: tiles, and four entries more for each unit (a sequence's tile of 128 rows for a KV head).  The other starts
+// with 4 us and takes 0.4 ns for a row of a tile of 128 positions (all SMs together).  us of mma.sync | tcgen05, 14 / 2 heads: 1
+// sequence of 4096, 112 rows of a KV head 16.8 | 16.1, 224 22.5 | 16.8; 1 of 65536, 14 rows 21.4 | 24.4, 28 29.9 | 25.6, 56
+// 45.9 | 26.4; 4 of 2500, 56 16.8 | 17.4, 112 22.9 | 18.2; 16 of 1000, 56 19.7 | 19.3, 112 23.0 | 20.1; 16 of 8192, 28 32.5 |
+// 36.1, 56 58 | 37; 64 of 1000, 28 19.7 | 27.1, 56 33.4 | 28.9; 64 of 4096, 28 49 | 56, 56 93 | 59; 256 of 500, 56 47 | 60, 112
+// 78 | 65.
+constexpr int64_t kTcWork = 8000, kTcPerTile = 36, kTcPerUnit = 68;
 
 struct Plan {
     int tc_grid;   // > 0: the tcgen05 kernel on that many CTAs
@@ -79,17 +81,18 @@ struct Plan {
 static Plan plan_of(int n_seq, int max_q, int64_t max_kv_len, int n_q_heads, int n_kv_heads) {
     Plan p{};
     const int64_t rows = (int64_t)max_q * (n_q_heads / n_kv_heads);
-    const int64_t tiles = (int64_t)n_seq * n_kv_heads * ((max_kv_len + kTcTile - 1) / kTcTile), row_tiles = (rows + kTcRows - 1) / kTcRows, entries = tiles * row_tiles;
-    if (tiles * rows >= kTcWork + kTcPerTile * entries && n_seq <= kTcMaxSeq && entries < (int64_t)1 << 28) {
-        const int64_t list = entries + kTcGap * (int64_t)n_seq * n_kv_heads * row_tiles;
+    const int64_t row_tiles = (rows + kTcRows - 1) / kTcRows, units = (int64_t)n_seq * n_kv_heads * row_tiles;
+    const int64_t of_unit = (max_kv_len + kTcTile - 1) / kTcTile, tiles = units * of_unit, list = tiles + kTcGap * units;
+    const int64_t work = (int64_t)n_seq * n_kv_heads * of_unit * rows;
+    if (tiles && work >= kTcWork + kTcPerTile * tiles + kTcPerUnit * units && n_seq <= kTcMaxSeq && list < (int64_t)1 << 30) {
         p.tc_grid = (int)(list < kSms ? list : kSms);
         p.n_splits = p.tc_grid / (int64_t)(n_seq * n_kv_heads) > 0 ? p.tc_grid / (n_seq * n_kv_heads) : 1;  // (for the combine)
         return p;
     }
     p.R = rows <= 8 ? 1 : 2;
     p.row_tiles = (int)((rows + 8 * p.R * kMmaWarps - 1) / (8 * p.R * kMmaWarps));
-    const int64_t units = (int64_t)n_seq * n_kv_heads * p.row_tiles, blocks = (max_kv_len + kBlock - 1) / kBlock;
-    int64_t want = (kSms * (p.R == 1 ? 4 : 3)) / units, most = blocks / kMmaWarps;
+    const int64_t blocks = (max_kv_len + kBlock - 1) / kBlock, ctas = (int64_t)n_seq * n_kv_heads * p.row_tiles;
+    int64_t want = (kSms * (p.R == 1 ? 4 : 3)) / ctas, most = blocks / kMmaWarps;
     if (want > most) want = most;
     p.cluster = 1;
     while (p.cluster < kMaxCluster && 2 * p.cluster <= want) p.cluster *= 2;

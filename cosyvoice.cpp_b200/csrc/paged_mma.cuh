@@ -12,7 +12,7 @@
 // cluster share the positions of a unit (sequence, KV head, row tile) and join through distributed shared memory; where one
 // cluster per unit would leave SMs idle, several do, and paged_combine_kernel joins their parts.
 //
-// What bounds it: 64 sequences of one token over up to 4096, 14 / 2 heads, e4m3: 13.6 us for 33 MB.  Of 19 thousand cycles the loop is
+// What bounds it: 64 sequences of one token over up to 4096, 14 / 2 heads, e4m3: 13.3 us for 33 MB.  Of 19 thousand cycles the loop is
 // 9 to 10 (6 to 7 TB/s while it runs), 5 pass before its first block is there (length, page, scale, block: four dependent loads),
 // 4 in the joins.  Steps of one block: 20.7 us, as a warp's waits come twice as often; e4m3 turned into f16 by shifts and a product
 // in place of its conversion instruction 19.2 where that has 15.0.  CTAs: one wave at 4 (3 with 16 rows a warp) on an SM; two waves

@@ -1,11 +1,12 @@
 // paged_tc.cuh -- paged attention of many rows on the 5th-generation tensor cores (tcgen05).
 //
 // Work is cut evenly: the key tiles (128 positions) of all units (sequence, tile of 128 rows, KV head), each unit up to the
-// last position that one of its rows sees, form one list, and CTA c of G takes the entries [c N / G, (c + 1) N / G).  A run is
-// the part of one unit that a CTA has; a whole unit is written out directly, parts go to the workspace and
-// paged_tc_combine_kernel joins them.
+// last position that one of its rows sees, form one list, in which kTcGap empty entries follow each unit's (a change of units
+// takes a CTA as long), and CTA c of G takes the entries [c N / G, (c + 1) N / G).  A run is the part of one unit that a CTA has; a
+// whole unit is written out directly, parts go to the workspace and paged_tc_combine_kernel joins them.
 //   warps 0-3, 4-7  softmax groups: thread = row = TMEM lane; group g takes the CTA's tiles 2 k + g
-//   warps 8-11      producers: codes to f16 tiles (128B swizzle), V transposed as its blocks lie
+//   warps 8-11      producers: codes to f16 tiles (128B swizzle), two warps K, two V, which is transposed as its blocks lie; Q of the
+//                   next run while the softmax is still at this one
 //   warp 12         issues S = Q K^T, up to two tiles ahead of the softmax;  warp 13 issues O = P V
 //   warp 14         looks the tiles' pages up, copies their blocks (1 KB each, cp.async.bulk) and scales, up to three tiles ahead
 //   (warp 15 only completes the last warpgroup)
@@ -15,11 +16,11 @@
 // inside the tensor cores truncate.
 // TMEM: three S buffers of 128 columns, tile n in n % 3, each overwritten 32 positions at a time by that chunk's P' (16 columns
 // hi, 16 lo); two outputs of 64 columns, one per group, read back while the group's next tile is on its way.
-// What bounds it: a tile takes a CTA about 2700 cycles, the producers 2600 of them, a softmax group 5500 for every second tile; before
-// the first and after the last lie 8 to 10 thousand.  16 sequences of 16 rows over up to 8192, i8: 43.8 us (the bytes alone take 5.4;
-// tensor pipe 24 % of active cycles, exponentials' unit 25 %, issue 39 %); 4 of 512 rows over 2501, e4m3: 65.7.  Codes copied by the
-// producers' own loads instead of warp 14: 44.6 and 66; these loads through registers, and fewer registers for the
-// softmax, 64 and 93.
+// What bounds it: a tile takes a CTA about 2800 cycles, as its softmax groups take 5600 for every second one (850 for 32 positions:
+// maxima, exponentials, the split into hi and lo; neither fewer instructions for that split nor faster producers changed the sum).  The
+// first S is there after 11 thousand cycles (lengths, list, page, block, f16 tile, all run once, with cold instructions),
+// the last tile's end takes 6.  16 sequences of 16 rows over 8192, i8: 39.0 us (the bytes alone take 5.4; tensor pipe 24 % of active
+// cycles, exponentials' unit 25 %, issue 39 %); 4 of 512 rows over up to 2501, e4m3: 44.6.
 #pragma once
 
 #include "flash_pipe.cuh"
@@ -37,7 +38,8 @@ static_assert(256 * kTcRegsSoftmax + 128 * kTcRegsProducer + 128 * kTcRegsOther 
 constexpr int kTcMaxSeq = 1024;  // tables in shared memory
 constexpr int kTcSt = 3;         // K and V tiles under way
 constexpr int kTcRaw = 3;        // tiles of codes under way
-constexpr int kTcGap = 4;        // what a change of runs costs, in tiles
+constexpr int kTcGap = 4;        // what a change of runs costs, in tiles (us of 16 x 16 over 8192 | 4 x 512 of 2501: 2 43.7 | 52.1,
+                                 // 4 41.7 | 47.6, 6 42.5 | 48.5, 8 42.7 | 49.0; none 43.4 | 64)
 constexpr int kTcInfos = 8;      // tiles whose scales may be in use
 constexpr int kTcTileBytes = kTcTile * kD * 2;
 constexpr int kTcBlocks = kTcTile / kBlock;
