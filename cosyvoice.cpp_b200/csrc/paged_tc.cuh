@@ -19,8 +19,8 @@
 // What bounds it: a tile takes a CTA about 2800 cycles, as its softmax groups take 5600 for every second one (850 for 32 positions:
 // maxima, exponentials, the split into hi and lo; neither fewer instructions for that split nor faster producers changed the sum).  The
 // first S is there after 11 thousand cycles (lengths, list, page, block, f16 tile, all run once, with cold instructions),
-// the last tile's end takes 6.  16 sequences of 16 rows over 8192, i8: 39.0 us (the bytes alone take 5.4; tensor pipe 24 % of active
-// cycles, exponentials' unit 25 %, issue 39 %); 4 of 512 rows over up to 2501, e4m3: 44.6.
+// the last tile's end takes 6.  16 sequences of 16 rows over 8192, i8: 38.9 us (the bytes alone take 5.4; tensor pipe 24 % of active
+// cycles, exponentials' unit 24 %, issue 38 %); 4 of 512 rows over up to 2501, e4m3: 44.6.
 #pragma once
 
 #include "flash_pipe.cuh"
