@@ -94,13 +94,13 @@ def test_pools_are_checked():
     u8 = lambda *s: dev(*s, dtype=torch.uint8)  # noqa: E731
     args = lambda **kw: {**{"k": u8(4, 2, 1024), "v": u8(4, 2, 1024), "k_scale": dev(4, 2, 1), "v_scale": dev(4, 2, 1), "format": 0}, **kw}  # noqa: E731
     cv.PagePool(**args())
-    for bad in ({"k": u8(4, 2, 1000)}, {"k": u8(4, 2, 48 * D)}, {"k": u8(4, 2048)}, {"v": u8(4, 2, 2048)}, {"v": u8(4, 3, 1024)}, {"k_scale": dev(4, 2, 2)},
+    for bad in ({"k": u8(4, 2, 1000)}, {"k": u8(4, 2, 40 * D)}, {"k": u8(4, 2048)}, {"v": u8(4, 2, 2048)}, {"v": u8(4, 3, 1024)}, {"k_scale": dev(4, 2, 2)},
                 {"v_scale": dev(4, 2, 1, dtype=torch.float16)}, {"v": torch.zeros(4, 2, 1024, dtype=torch.uint8)}, {"k": u8(4, 2, 2048)[:, :, ::2]},
                 {"v": u8(4, 3, 1024)[:, :2]}):
         with pytest.raises(ValueError):
             cv.PagePool(**args(**bad))
-    wide = cv.PagePool(u8(4, 3, 1024)[:, :2], u8(4, 3, 1024)[:, :2], dev(4, 2, 1), dev(4, 2, 1), 1)
-    assert wide.desc.nb_page == 3072 and good.desc.nb_page == 2 * 32 * D
+    wide = cv.PagePool(u8(4, 5, 1024)[:, :2], u8(4, 5, 1024)[:, :2], dev(4, 2, 1), dev(4, 2, 1), 1)
+    assert wide.desc.nb_page == 5 * 1024 and good.desc.nb_page == 2 * 32 * D
     with pytest.raises(ValueError):
         cv.PageAssigner(None, [], i32(2, 4), i32(2), i32(2))
 
