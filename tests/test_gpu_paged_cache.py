@@ -235,6 +235,16 @@ def test_attention_of_a_long_prompt(ctx, cv, cuda, fmt):
 
 
 @pytest.mark.parametrize("fmt", [0, 1])
+def test_attention_of_many_short_sequences(ctx, cv, cuda, fmt):
+    """A dozen sequences' heads, one or two tiles each, follow one another on an SM; empty ones among them."""
+    rng = np.random.default_rng(fmt)
+    lens = rng.integers(0, 300, 100)
+    lens[::9] = 0
+    host, table = filled(rng, fmt, lens.tolist(), 32, 16)
+    check_attention(cv, ctx, cuda, rng, host, table, lens, np.minimum(lens, rng.integers(0, 101, 100)), 16, 100)
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
 def test_attention_of_more_sequences_than_one_list_holds(ctx, cv, cuda, fmt):
     rng = np.random.default_rng(fmt)
     lens = rng.integers(0, 90, 1030)
