@@ -329,6 +329,8 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int s = blockIdx.x / C;
+    // (shared memory of another CTA may be written once it is known to have started: all wait for this before the first exchange)
+    if (C > 1) cluster_arrive_relaxed();
     for (int i = tid; i < 64 * 16; i += kThreads) sh.table[i] = kPowers[i >> 4];
     const double* table = sh.table + (tid & 15);
     if (tid == 0) sh.bad = 0;
@@ -397,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) verify_walk_kernel(const __grid_c
             if (logs) logs[i] = 0.0f;
         }
     __syncthreads();
+    if (C > 1) cluster_wait();
     if (refused_all || sh.bad || n == 0) {
         if (rank == 0 && tid == 0) {
             if (refused_all || sh.bad) record_status(status, kStatusBadDraft);
