@@ -3,7 +3,9 @@
 //
 // Codes are exact in f16.  A row of Q is scaled by a
 // power of two and split into f16 hi + lo, which lie 8 rows apart in one A operand: a product over 16 rows serves 8 rows of
-// queries, and the sum of its two halves is the score.  P is split the same way.  A block of 16 positions has
+// queries, and the sum of its two halves is the score.  P is split without a power of its own, so what is
+// left out of a weight is 2^-22 of it or 2^-32 of the row's largest.  (With the power that the tcgen05 kernel has, which follows weight
+// times value scale, 64 sequences of one token over up to 4096 took 13.6 us in place of 13.2.)  A block of 16 positions has
 // its scale of the keys multiplied to the scores, its scale of the values to the block's output, which is a fresh accumulator
 // added to f32 registers.  So every product is exact, and no sum stays in the tensor cores (whose adds truncate) for longer.
 //

@@ -11,17 +11,21 @@
 //   warp 14         looks the tiles' pages up, copies their blocks (1 KB each, cp.async.bulk) and scales, up to three tiles ahead
 //   (warp 15 only completes the last warpgroup)
 // Precision: codes are exact in f16, Q and P' = P w are split in f16 hi + lo, so S = Qh K + Ql K and O = Ph V + Pl V.  A block's
-// key scale multiplies its 16 columns of S; its value scale, over a power of two of the tile, is w, which leaves P' with what is
-// above 2^-22 of the largest of the tile.  The output of a tile is a fresh accumulator, added in f32 to the row's registers: adds
-// inside the tensor cores truncate.
+// key scale multiplies its 16 columns of S; its value scale times a power of two of the row is w.  That power follows the largest
+// P times value scale that the row has seen, apart from the reference that follows its largest score, so P' keeps 2^-22 of itself
+// or 2^-27 of the row's largest such product, and what a row does not see costs it nothing.  Both references move by whole powers of
+// two, exactly.  The output of a tile is a fresh accumulator, added in f32 to the row's registers: adds inside the tensor cores
+// truncate.
 // TMEM: three S buffers of 128 columns, tile n in n % 3, each overwritten 32 positions at a time by that chunk's P' (16 columns
 // hi, 16 lo); two outputs of 64 columns, one per group, read back while the group's next tile is on its way.
 // What bounds it: a tile takes a CTA about 2800 cycles, as its softmax groups take 5600 for every second one (850 for 32 positions:
 // maxima, exponentials, the split into hi and lo; neither fewer instructions for that split nor faster producers changed the sum).  The
 // first S is there after 11 thousand cycles (lengths, list, page, block, f16 tile, all run once, with cold instructions),
-// the last tile's end takes 6.  16 sequences of 16 rows over 8192, i8: 38.9 us (the bytes alone take 5.4; tensor pipe 24 % of active
-// cycles, exponentials' unit 24 %, issue 38 %); 4 of 512 rows over up to 2501, e4m3: 44.6.
+// the last tile's end takes 6.  16 sequences of 16 rows over 8192, i8: 38.4 us (the bytes alone take 5.4; tensor pipe 24 % of active
+// cycles, exponentials' unit 24 %, issue 38 %); 4 of 512 rows over up to 2501, e4m3: 44.2.
 #pragma once
+
+#include <cfloat>
 
 #include "flash_pipe.cuh"
 #include "paged_mma.cuh"
@@ -53,9 +57,8 @@ struct TcAttArgs {
 };
 
 struct __align__(16) TcInfo {   // of a tile
-    float ks[kTcBlocks];        // key scales
-    float w[kTcBlocks];         // value scales times a power of two, below 1
-    float exp;                  // the inverse of that power
+    float4 scales[kTcBlocks / 2];  // by 32 positions: two blocks' of the keys, of the values
+    float lg;                      // log2 of the largest of the latter (of 0: -infinity), about
     uint32_t valid;             // blocks that have a page
     uint32_t starts, last;      // whether the tile starts a run; is the CTA's last
     int32_t count;              // positions that exist
@@ -111,6 +114,51 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
     return *reinterpret_cast<float2*>(&rd);
 }
+__device__ __forceinline__ float log2_of(float scale) { return scale > 0.0f ? __log2f(scale) : -INFINITY; }
+// 2^e for whole e <= 0 (0 below f32's normal numbers).
+__device__ __forceinline__ float shrink_by(float e) { return e < -126.0f ? 0.0f : pow2f((int)e); }
+
+// What a row's weights and outputs are kept relative to.  P is 2^(score - base); a score above thr raises base.  P' is P times value
+// scale times wk = 2^ko, and a score plus log2 of its value scale above thr_o lowers ko: to a largest P' of 2^kOutOffs, with room up to
+// 2^15, which leaves lo's last bit (2^-24) 2^-27 of it.  (From 2^7 on, as P, P' outgrew its room and was rounded anew in TMEM more often
+// than P: 16 sequences of 16 rows over 8192 40.6 us, 38.4 so.)  Both move by whole powers of two, exactly.  (thr, thr_o -infinity: no
+// score, no scale above 0 yet)
+constexpr float kOutOffs = 3.0f;
+struct RowRef {
+    float base = 0.0f, thr = -INFINITY, ko = 0.0f, wk = 1.0f, thr_o = -INFINITY;
+    // Below it no score passes thr, nor with a value scale of up to 2^lg thr_o.
+    __device__ __forceinline__ float quiet(float lg) const { return fminf(thr, thr_o - lg); }
+    // (past FLT_MAX only where P is below 2^-113)
+    __device__ __forceinline__ float weight(float scale) const { return fminf(scale * wk, FLT_MAX); }
+    // Of outputs, to units of P times value.
+    __device__ __forceinline__ float unit() const { return pow2f(-(int)ko); }
+    // For largest scores m0, m1 of blocks with value scales s0, s1: returns what is to be taken from scores, the outputs' factor in f;
+    // l, the sum of P, is brought along.
+    __device__ __forceinline__ float raise(float m0, float s0, float m1, float s1, float& l, float& f) {
+        float top = fmaxf(m0 + log2_of(s0), m1 + log2_of(s1)), up = 0.0f;
+        const float mx = fmaxf(m0, m1);
+        if (mx > thr) {
+            up = rintf(mx) - kOffs;
+            l *= thr == -INFINITY ? 0.0f : shrink_by(-up);
+            base += up;
+            thr = kLazy + kOffs;
+            top -= up;
+        }
+        const bool had = thr_o != -INFINITY;
+        const float k = had ? ko + up : 0.0f;  // what leaves the outputs as they are
+        ko = k;
+        if (top > thr_o - up) {
+            ko = kOutOffs - rintf(top);
+            thr_o = 0.0f;
+        }
+        ko = fminf(fmaxf(ko, -126.0f), 126.0f);
+        wk = pow2f((int)ko);
+        f = had ? shrink_by(ko - k) : 1.0f;
+        if (thr_o != -INFINITY) thr_o = kLazy + kOffs - ko;
+        return up;
+    }
+};
+
 // Bounded wait: gives up after kTcTries suspensions of up to 20 us, or once another role has given up.  *err keeps the site; the
 // kernel's end records it.
 constexpr uint32_t kTcTries = 100000;
@@ -259,16 +307,12 @@ __device__ __forceinline__ void tc_load(const TcAttArgs& ta, uint8_t* smem, TcAt
             bulk_g2s(raw + (kTcBlocks + lane) * kBlockBytes, static_cast<const uint8_t*>(a.p.pool.v) + at, kBlockBytes, &B->raw_full[slot]);
         }
         const uint32_t last = t == r.t1 && r.v + r.T + kTcGap >= hi;
-        const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
-        int e = mx > 0.0f ? -1 - dstream::ilog2f(mx) : 0;
-        e = e > 100 ? 100 : e < -100 ? -100 : e;
         TcInfo& info = B->info[n % kTcInfos];
-        if (lane < kTcBlocks) {
-            info.ks[lane] = ks;
-            info.w[lane] = vs * pow2f(e);
-        }
+        const float ks1 = __shfl_down_sync(0xffffffffu, ks, 1), vs1 = __shfl_down_sync(0xffffffffu, vs, 1);
+        const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.0f))));
+        if (lane < kTcBlocks && !(lane & 1)) info.scales[lane >> 1] = make_float4(ks, ks1, vs, vs1);
         if (lane == 0) {
-            info.exp = pow2f(-e);
+            info.lg = log2_of(most);
             info.valid = valid;
             info.starts = (uint32_t)first;
             info.last = last;
@@ -535,11 +579,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             float2 O[32];
 #pragma unroll
             for (int d = 0; d < 32; ++d) O[d] = make_float2(0.f, 0.f);
-            float base = 0.0f, thr = -INFINITY, l = 0.0f, vs_last = 1.0f;
-            bool pending = false;  // a tile's output still to be added, times vs_last
+            RowRef ref;
+            float l = 0.0f, late = 1.0f;
+            bool pending = false;  // a tile's output still to be added, times late
             auto add_output = [&]() {
                 uint32_t o0[32];
-                const float2 f = make_float2(vs_last, vs_last);
+                const float2 f = make_float2(late, late);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     tc::tmem_ld32(ot + 32 * e, o0);
@@ -558,21 +603,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc::fence_after();
                 const TcInfo& info = B->info[n % kTcInfos];
-                float vs_now = 1.0f;
                 if (warp_real) {
                     uint32_t sv[32];
                     tc::tmem_ld32(sp, sv);
                     const uint32_t valid = info.valid;
                     const bool masked = p0 + kTcTile > sure || valid != 0xffu;
-                    vs_now = info.exp;
+                    float quiet = ref.quiet(info.lg);
                     tc::tmem_ld_wait();
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
-                        const float2 ks = *reinterpret_cast<const float2*>(info.ks + 2 * c), w = *reinterpret_cast<const float2*>(info.w + 2 * c);
+                        const float4 sc = info.scales[c];
+                        const float2 ks = make_float2(sc.x, sc.y);
+                        float2 w = make_float2(ref.weight(sc.z), ref.weight(sc.w));
                         float2 x[16];
                         {
                             const float f0 = rs * ks.x, f1 = rs * ks.y;
-                            const float2 b = make_float2(-base, -base);
+                            const float2 b = make_float2(-ref.base, -ref.base);
 #pragma unroll
                             for (int d = 0; d < 16; ++d) {
                                 const float f = d < 8 ? f0 : f1;
@@ -596,26 +642,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         for (int u = 0; u < 4; ++u)
                             m4[u] = max3(max3(max3(x[4 * u].x, x[4 * u].y, x[4 * u + 1].x), x[4 * u + 1].y, x[4 * u + 2].x),
                                          fmaxf(x[4 * u + 2].y, x[4 * u + 3].x), x[4 * u + 3].y);
-                        const float mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
-                        if (__any_sync(0xffffffffu, mx > thr)) {
-                            float f = 1.0f, up = 0.0f;
-                            if (mx > thr) {
-                                up = mx - kOffs;
-                                f = thr == -INFINITY ? 0.0f : fast_exp2(-up);
-                                base += up;
-                                thr = kLazy + kOffs;
-                                l *= f;
-                                vs_last *= f;
-                            }
-                            const float2 f2 = make_float2(f, f);
-#pragma unroll
-                            for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
+                        const float m0 = fmaxf(m4[0], m4[1]), m1 = fmaxf(m4[2], m4[3]), mx = fmaxf(m0, m1);
+                        if (__any_sync(0xffffffffu, mx > quiet)) {
+                            float f;
+                            const float up = ref.raise(m0, sc.z, m1, sc.w, l, f);
+                            late *= f;
+                            quiet = ref.quiet(info.lg);
+                            w = make_float2(ref.weight(sc.z), ref.weight(sc.w));
 #pragma unroll
                             for (int d = 0; d < 16; ++d) {
                                 x[d].x -= up;
                                 x[d].y -= up;
                             }
-                            if (c) {  // this tile's P' so far, 16 positions at a time
+                            const bool shrinks = __any_sync(0xffffffffu, f != 1.0f);
+                            if (shrinks) {
+                                const float2 f2 = make_float2(f, f);
+#pragma unroll
+                                for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], f2);
+                            }
+                            if (shrinks && c) {  // this tile's P' so far, 16 positions at a time
                                 tc::tmem_ld_wait();
                                 tc::tmem_st_wait();
 #pragma unroll 1
@@ -660,7 +705,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         tc::fence_after();
                         add_output();
                     }
-                    vs_last = vs_now;
+                    late = 1.0f;
                     pending = true;
                     tc::tmem_st_wait();
                 }
@@ -676,7 +721,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             }
             tc::fence_before();
             if (!fp::prod_bar_and(2, 256, ok)) break;  // every MMA of the run is done; all threads leave together
-            const float m_mine = thr == -INFINITY && l == 0.0f ? -INFINITY : base;  // (NaN scores raise nothing)
+            const float m_mine = ref.thr == -INFINITY && l == 0.0f ? -INFINITY : ref.base;  // (NaN scores raise nothing)
+            const float unit = ref.unit();
+#pragma unroll
+            for (int d = 0; d < 32; ++d) O[d] = mul2(O[d], make_float2(unit, unit));
             // group 1's rows to where Q was, joined there by group 0, written by both
             float4* rows_at = reinterpret_cast<float4*>(smem + Sh::kQ + (run & 1) * 2 * kTcTileBytes);
             float4* mine = rows_at + row * 16;

@@ -623,8 +623,11 @@ cvattn_status cvattn_paged_read(cvattn_context* ctx, void* stream, const cvattn_
  *   out[s][i][h] = sum_j p_j v_j,  p = softmax_j(scale q.k_j),
  *   lse[s][i][h] = log(sum_j exp(scale q.k_j))                (natural log).
  * Queries are taken to 2^-22 of a row's largest value and codes exactly; sums are
- * in f32.  With many rows P times the values' scales is taken to 2^-22 of the
- * largest of 128 neighbouring positions.
+ * in f32.  A weight p_j is taken to 2^-22 of itself or 2^-31 of the row's largest
+ * weight; with many rows, p_j times its block's value scale to 2^-22 of itself or
+ * 2^-27 of the row's largest such product.  Positions that a row does not see cost
+ * it nothing.  Sums hold the largest weight as up to 2^15: outputs are finite for
+ * values of up to 2^80.
  *   - A row that sees nothing, and rows from n_q[s] to max_q: zeros, lse = -inf.
  *   - What a page holds past kv_len is not looked at.
  *   - A kv_len outside [0, max_kv_len] or n_q outside [0, max_q] is recorded and
