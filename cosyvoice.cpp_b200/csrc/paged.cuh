@@ -22,9 +22,11 @@ __host__ __device__ constexpr int v_place(int t, int d) { return d / 32 * 512 + 
 
 template <int F> constexpr float kMostCode = F == kI8 ? 127.0f : 448.0f;
 
-// e4m3 to f32, exactly: its exponent and mantissa in f16's place are 2^-8 of the value (subnormals too).
+// e4m3 to f32, exactly (0x7f, 0xff: NaN).
 __device__ __forceinline__ float e4m3_value(uint32_t b) {
-    return h2f((uint16_t)((b & 0x80u) << 8 | (b & 0x7fu) << 7)) * 256.0f;
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)b));
+    return h2f((uint16_t)r);
 }
 template <int F> __device__ __forceinline__ float code_value(uint32_t b) {
     if constexpr (F == kI8) return (float)((int)b - 128);

@@ -540,7 +540,9 @@ cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv
  * values is 1024 codes at  data + p*nb_page + (h*page_size/16 + b)*1024  with one
  * scale at  scale + p*nb_scale + h*page_size/16 + b :  value = code value x scale.
  *   CVATTN_PAGE_I8    code value = byte - 128, in -127 .. 127
- *   CVATTN_PAGE_E4M3  the byte as an OCP e4m3 number
+ *   CVATTN_PAGE_E4M3  the byte as an OCP e4m3 number (0x7f, 0xff are NaN: no call
+ *                     writes them, one of a value makes that dim NaN in all rows
+ *                     of cvattn_paged_attention whose sequence holds its position)
  * The byte of position t, value d of a block is at
  *   keys    t*64 + d
  *   values  d/32*512 + (d%8*4 + t/4)*16 + d/8%4*4 + t%4
