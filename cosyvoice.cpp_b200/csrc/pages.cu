@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_assign_kernel(const __grid
         return make_int2(max(0, (need + P - 1) / P - (keep + P - 1) / P) + copies, copies);
     };
     int keep, need, tail;
-    // (those without room come after all with room that ask for anything, so the copies before one with room have room too)
+    // (the sums only grow, so all behind the first without room are without it, and the copies before one with room have room too)
     crew_scan(crew, p.n_seq, [&](int s) { return asks(s, keep, need, tail); },
               [&](int s, int2 before) {
                   const int2 v = asks(s, keep, need, tail);

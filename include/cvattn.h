@@ -676,9 +676,13 @@ cvattn_status cvattn_paged_attention(cvattn_context* ctx, void* stream, const cv
  *     sequences hold the page, the first of them keeps it.
  *   - Free pages are given in ascending order, sequence by sequence, as long as
  *     the pages that the sequences up to it ask for are there; room[s] is then
- *     max(keep, need), else keep.  (A sequence without room may hold a tail page
- *     that others hold too, one with room among them; cvattn_paged_append with
- *     refs refuses to write there until all but one have let go.)
+ *     max(keep, need), else keep.  The first one that cannot be served ends it for
+ *     all behind it, those that ask for no page among them, and may go on holding
+ *     a tail page with one that has room (cvattn_paged_append with refs refuses to
+ *     write there until all but one have let go).  So where some room[s] is below
+ *     need[s], decide who waits (need = keep) or gives up (keep = need = 0) and call
+ *     again, on the new table and with every sequence its own src: the others then
+ *     get their pages, and copies of tails that they share with those who wait.
  *   - Entries past a sequence's pages become -1, and so do kept ones out of range
  *     (recorded).  A keep, need or src out of range is recorded and counts as
  *     keep = need = 0.
