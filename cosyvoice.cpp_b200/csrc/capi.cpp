@@ -742,7 +742,7 @@ cvattn_status cvattn_paged_attention(cvattn_context* ctx, void* stream, const cv
     return from_cuda(launch_paged_attention(as_stream(stream), *p, ctx->status));
 }
 
-// Pools that one table indexes; the copied pages of two pools may not touch.
+// Pools that one table indexes.  (That none lies in another's pages is up to the caller: pages of several may alternate.)
 static cvattn_status pools_ok(const cvattn_page_pool* pools, int32_t n) {
     if (!pools || n <= 0) return CVATTN_ERR_INVALID_ARGUMENT;
     for (int32_t i = 0; i < n; ++i) {

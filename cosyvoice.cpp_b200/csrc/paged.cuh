@@ -18,8 +18,6 @@ constexpr int kBlock = CVATTN_PAGE_BLOCK;       // positions
 constexpr int kBlockBytes = kBlock * kD;
 constexpr int kI8 = CVATTN_PAGE_I8, kE4M3 = CVATTN_PAGE_E4M3;
 
-__host__ __device__ constexpr int v_place(int t, int d) { return d / 32 * 512 + (d % 8 * 4 + t / 4) * 16 + d / 8 % 4 * 4 + t % 4; }
-
 template <int F> constexpr float kMostCode = F == kI8 ? 127.0f : 448.0f;
 
 // e4m3 to f32, exactly (0x7f, 0xff: NaN).

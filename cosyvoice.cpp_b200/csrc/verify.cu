@@ -117,7 +117,6 @@ struct Node {
     double floor;        // -reach, which they count as
     double inv;          // 1 / temperature
     double u64;          // 64 / (temperature ln 2)
-    double W;            // sum of the weights (of f32 exponentials)
     int hot;             // greedy: the lowest token with logit m
     bool greedy;
     __device__ __forceinline__ void most(float l) {
@@ -125,10 +124,9 @@ struct Node {
         low = __fsub_rd(l, reach);  // (so what is above it lies within reach, however far apart numbers of that size are)
     }
 };
-// exp((l - m) / temperature) in f32, m finite; NaN for a NaN.
-__device__ __forceinline__ float weight32(const Node& x, float l) { return fast_exp2((l - x.m) * x.c); }
-// The same in 64 bits; below kNothing where l is not above x.low or a NaN.  `table`: kPowers, one entry of 16 apart (each lane of
-// half a warp has a copy in banks of its own: entries are read at random, and without copies that took as long as the rest).
+// exp((l - m) / temperature) in 64 bits, m finite; below kNothing where l is not above x.low or a NaN.  `table`: kPowers, one entry of
+// 16 apart (each lane of half a warp has a copy in banks of its own: entries are read at random, and without copies that took as long
+// as the rest).
 constexpr double kNothing = 1e-290;
 __device__ __forceinline__ double weight64(const Node& x, float l, const double* table) {
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: u + magic has u's nearest integer in its low bits
