@@ -68,7 +68,7 @@ static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // same whatever rows a unit (a sequence's tile of 128 rows for a KV head) has up to 128, a unit some more; the other's cost goes with
 // rows times tiles of positions.  So: work, rows times tiles, against a constant and a share for each tile and unit.  The three numbers
 // are fitted to these times, us of mma.sync | tcgen05, 14 / 2 heads, and pick the slower side of three: 1 of 65536 with 28 rows, and
-// within 0.7 us 1 of 4096 with 112 and 16 of 1000 with 56 (a single sequence's tiles keep few SMs of the other busy).  1
+// within 0.7 us 1 of 4096 with 112 and 16 of 1000 with 56.  1
 // sequence of 4096, 112 rows of a KV head 16.8 | 16.1, 224 22.5 | 16.8; 1 of 65536, 14 rows 21.4 | 24.4, 28 29.9 | 25.6, 56
 // 45.9 | 26.4; 4 of 2500, 56 16.8 | 17.4, 112 22.9 | 18.2; 16 of 1000, 56 19.7 | 19.3, 112 23.0 | 20.1; 16 of 8192, 28 32.5 |
 // 36.1, 56 58 | 37; 64 of 1000, 28 19.7 | 27.1, 56 33.4 | 28.9; 64 of 4096, 28 49 | 56, 56 93 | 59; 256 of 500, 56 47 | 60, 112

@@ -14,7 +14,10 @@ constexpr int kMaxPools = 48;    // pools of one copy launch (kernel arguments)
 // Where next, refs, writers, lowest and list fit into one CTA's shared memory, they lie there: then the books take one CTA, and
 // what takes a cluster barrier and a trip to L2 otherwise takes a block barrier.  An assignment to
 // 64 sequences: 16.0 us by a cluster, 13.2 in shared memory, 10.0 since this form's code is a kernel of its own and the wishes are read
-// once.  All of it is latency (barriers, each behind a dependent load, and instructions fetched once).
+// once.  All of it is latency (barriers, each behind a dependent load, and instructions fetched once).  Where the books do not fit, us
+// of assignment | compaction with the copies (16 positions, one pool of one head): 500 x 40 entries of 20000 pages 19.5 | 19.0, 60 x 30
+// of 60000 22.3 | 22.0, 8192 x 1 of 8000 34.9 | 19.4, 1024 x 256 of 100000 58.5 | 73.8; just below, 256 x 40 of 8000 in shared memory
+// 18.0 | 16.0.
 struct Books {
     int32_t *n_copies, *next, *refs, *writers, *lowest, *list, *src, *keep, *need, *from, *to;
     size_t bytes;

@@ -1,7 +1,8 @@
 """Launchers of the paged 8-bit cache and of the verification of drafts (include/cvattn.h).
 
 As in the rest of the package a launcher checks its tensors and builds its parameters once; calling it launches on the given
-or the current stream and reads the tensors' contents at that time."""
+or the current stream and reads the tensors' contents at that time.  Its scratch memory is its own (or the given workspace): what may
+be under way at the same time, on two streams or in two graphs, wants launchers of its own."""
 from __future__ import annotations
 
 import ctypes

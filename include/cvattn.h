@@ -549,7 +549,12 @@ cvattn_status cvattn_kv_evict(cvattn_context* ctx, void* stream, const cvattn_kv
  * (in the order in which the tensor cores take them).  Scales are not negative.  A table lists, for each
  * sequence, the page of its positions 0 .. page_size - 1, then the next, ..;
  * every layer's pool is indexed by the same table.  Entries outside
- * [0, n_pages) hold nothing. */
+ * [0, n_pages) hold nothing.
+ * Unlike the ggml caches: heads of 64 only, chains of tokens only (a row sees all
+ * positions up to its own; trees of drafts want cvattn_tree_decode), and keys are
+ * rotated by a call of their own (cvattn_rope).
+ * Calls that may be under way at the same time, on two streams or in two graphs,
+ * want workspaces of their own. */
 enum { CVATTN_PAGE_I8 = 0, CVATTN_PAGE_E4M3 = 1 };
 #define CVATTN_PAGE_BLOCK 16
 
@@ -574,7 +579,9 @@ typedef struct cvattn_page_pool {
  * new values, as f32 (no scale that is not a normal number: the values count as 0);
  * codes are the nearest values, ties to even, of x / scale; rows that the block
  * held are rounded anew when the scale grows.  A NaN is stored as 0, an infinity
- * as the block's largest.  Other rows of the block are left as they are.
+ * as the block's largest.  Other rows of the block are left as they are.  Taking
+ * rows back (a shorter length) takes neither the scale that they left nor that
+ * rounding back.
  * A sequence whose rows do not fit its table is recorded in the status word and
  * skipped, and so is a block whose page is out of range or, with refs, held by
  * more than one table entry.  (Without refs two sequences that append to one page
