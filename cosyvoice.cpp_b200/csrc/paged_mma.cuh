@@ -118,6 +118,8 @@ __device__ __forceinline__ void split_near(float2 x, uint32_t& hi, uint32_t& lo)
         : "=f"(a), "=f"(b) : "r"(hi), "h"((uint16_t)0xBC00u), "f"(x.x), "f"(x.y));
     lo = tc::pack_f16x2(a, b);
 }
+// Power of two that brings a row's largest query value into [128, 256) (from 2^-119 on; smaller ones it makes normal).
+__device__ __forceinline__ int query_exp(float amax) { return min(7 - (max((__float_as_int(amax) >> 23) & 0xff, 1) - 127), 126); }
 // A product into a fresh accumulator.
 __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, R == 1 ? 4 : 3) paged_mma_kern
             e[j] = r < rows ? *reinterpret_cast<const float4*>(q + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
             am = fmaxf(am, fmaxf(fmaxf(fabsf(e[j].x), fabsf(e[j].y)), fmaxf(fabsf(e[j].z), fabsf(e[j].w))));
         }
-        const int ex = dtc::norm_exp(quad_max(am));
+        const int ex = query_exp(quad_max(am));
         const float f = pow2f(ex);
         rs[i] = pow2f(-ex) * a.scale_log2;
         lim[i] = r < rows ? before + tok : 0;

@@ -348,7 +348,7 @@ template <int kThreads> __device__ __forceinline__ void tc_queries(const AttArgs
         for (int u = 0; u < 4; ++u) v[u] = qr < rows ? q[u] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < 4; ++u) am = fmaxf(am, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
-        const int ex = dtc::norm_exp(quad_max(am));
+        const int ex = query_exp(quad_max(am));
         const float f = pow2f(ex);
         if (c == 0) rsb[q0] = pow2f(-ex) * a.scale_log2;
 #pragma unroll

@@ -150,3 +150,19 @@ def test_values_near_the_ends_of_f32(ctx, cv, cuda, fmt, S, n, Hq, heads, tcgen0
     # weights up to 2^15 times values below 2^(r + 1) M, and 47 more of 2^7.5: below 2^(r + 1) M 2^15.3
     assert (2.0 ** (r + 1)) * MOST[fmt] * 2.0 ** 15.3 < 2.0 ** 128
     hold(cv, ctx, cuda, host, table, lens, q, 1.0, tcgen05)
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("S,n,Hq,heads,tcgen05", SHAPES)
+@pytest.mark.parametrize("r", [117, 112, -112])
+def test_queries_near_the_ends_of_f32(ctx, cv, cuda, fmt, S, n, Hq, heads, tcgen05, r):
+    """Queries 2^r larger over keys 2^r smaller give what they give at ordinary sizes."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(n, 250, S)]
+    lens[0] = max(lens[0], 129)
+    host, table = filled(rng, fmt, lens, 32, heads)
+    host.scales["k"] *= np.float32(2.0 ** -r)
+    assert np.nanmin(np.where(host.scales["k"] > 0, host.scales["k"], np.nan)) >= 2.0 ** -126
+    q = rng.standard_normal((S, n, Hq, D)).astype(np.float32)
+    q[:, :, 0] *= np.float32(2.0 ** -6)  # (a row whose largest value is smaller)
+    hold(cv, ctx, cuda, host, table, lens, q * np.float32(2.0 ** r), 0.125, tcgen05)
